@@ -1,0 +1,801 @@
+// The residual sum between two sub-layers' norms on the flat node layout:
+//   rows'  = rows + s * act(z) * (g_p * norm(u) + b_p)
+//   normed = g_n * norm(rows') + b_n
+// with norm the merged equivariant normalisation (frequency 0 centred, one
+// denominator sqrt(sum_k w_k c_k^2 + eps) pooled over the frequencies'
+// mean squares: w = 1 / (a0 present) on frequency 0 and 1 / (2 m present) on a
+// frequency of m copies), act(z) = factor sigmoid(z) one gate a copy, s one
+// scale a coordinate.  Without g_p the branch is not normalised, without g_n
+// nothing is normalised behind the sum, without z or s the factor is one.
+// The next norm reads the sum before it is rounded to the rows' type.
+//
+// Backward, from dy (of rows') and dh (of normed):
+//   G  = dy + norm'(rows')^T (g_n dh)          (the gradient of rows)
+//   dz = act'(z) sum over the copy of G s (g_p uhat + b_p)
+//   du = norm'(u)^T (G act(z) s g_p)
+// and the per-coordinate sums over the rows A = sum G act uhat, B = sum G act,
+// C = sum dh xhat, E = sum dh, of which the parameters' gradients are made:
+// dg_p = s A, ds = g_p A + b_p B, db_p = s B, dg_n = C, db_n = E.  rows' is
+// formed again from rows, u and z, which the pass reads anyway: what rounding
+// the stored rows' to bfloat16 loses would otherwise enter C and the rows'
+// gradient.
+//
+// One pass over the data each way, so the bytes bound it.  A row's units (16
+// bytes of the rows' type, or one copy where a multiplicity, a pointer or the
+// gates' rows are not whole units) are shared by 2^k lanes with at most
+// kMaxUnits<...> units a lane, all in registers; the norms' sums are shuffles
+// within those lanes; a wave holds 64 / 2^k rows.  Coefficients sit in LDS (the
+// unit form), since each lane would otherwise hold four registers of them for
+// every number of a row.  The waves are persistent; the backward's sums stay in
+// registers over a wave's rows, are added over the workgroup in a fixed order,
+// and a second kernel adds the workgroups' rows in a fixed order (no atomics).
+#include <algorithm>
+#include <type_traits>
+
+#include "common.hpp"
+
+namespace gm {
+namespace {
+
+constexpr int kRnMaxFreq = 8;
+constexpr int kRnThreads = 256;
+constexpr int kRnWaves = kRnThreads / kWave;
+constexpr int kRnMaxWidth = 1024;
+
+struct rbf16 {
+  uint16_t bits;
+};
+
+template <typename T>
+struct RnAcc {
+  using type = float;
+};
+template <>
+struct RnAcc<double> {
+  using type = double;
+};
+
+__device__ __forceinline__ float widen(float x) { return x; }
+__device__ __forceinline__ double widen(double x) { return x; }
+__device__ __forceinline__ float widen(rbf16 x) { return __uint_as_float((uint32_t)x.bits << 16); }
+
+// The row type's numbers, bfloat16 rounded to nearest even.
+__device__ __forceinline__ void narrow(float v, float& o) { o = v; }
+__device__ __forceinline__ void narrow(double v, double& o) { o = v; }
+__device__ __forceinline__ void narrow(float v, rbf16& o) {
+  const __bf16 b = static_cast<__bf16>(v);
+  __builtin_memcpy(&o.bits, &b, 2);
+}
+
+// V consecutive numbers of type T at p as one load or store of up to 16 bytes each.
+template <typename T, int V>
+struct alignas(sizeof(T) * V >= 16 ? 16 : sizeof(T) * V) Pack {
+  T v[V];
+};
+
+template <int V, typename T, typename A>
+__device__ __forceinline__ void load_n(const T* p, A (&out)[V]) {
+  const Pack<T, V> x = *reinterpret_cast<const Pack<T, V>*>(p);
+#pragma unroll
+  for (int i = 0; i < V; ++i) out[i] = widen(x.v[i]);
+}
+template <int V, typename T, typename A>
+__device__ __forceinline__ void store_n(T* p, const A (&in)[V]) {
+  Pack<T, V> x;
+#pragma unroll
+  for (int i = 0; i < V; ++i) narrow(in[i], x.v[i]);
+  *reinterpret_cast<Pack<T, V>*>(p) = x;
+}
+
+template <typename X, typename U>
+struct RnArgs {
+  using A = typename RnAcc<X>::type;
+  int64_t n_rows;
+  int D, a0, copies, present, nf;
+  int off[kRnMaxFreq], mult[kRnMaxFreq];
+  int units, scalar_units;  // a row's units, the first of them frequency 0's
+  int lanes, shift;         // lanes a row (a power of two), its logarithm
+  const X* x;
+  const U* u;
+  const X* z;           // (n_rows, copies) or null
+  const A* gain;        // (D) or null: the branch is not normalised
+  const A* offset;      // (a0) or null
+  const A* scale;       // (D) or null
+  const A* next_gain;   // (D) or null: nothing normalised behind the sum
+  const A* next_offset; // (a0) or null
+  A factor, eps, next_eps;
+  X* y;
+  X* normed;
+  A* stats;  // (n_rows, 4): the branch's mean and 1 / d, the sum's
+  // backward
+  const X* dy;  // or null
+  const X* dn;  // or null
+  X* dx;
+  U* du;
+  X* dz;
+  A* partial;  // (workgroups, 4, units V)
+  A* dparams;  // dgain (D), doffset (a0), dscale (D), dnext_gain (D), dnext_offset (a0)
+};
+
+// Coordinate k's share of the pooled mean square.
+template <typename Args>
+__device__ __forceinline__ typename Args::A share_of(const Args& a, int k) {
+  using A = typename Args::A;
+  if (k < a.a0) return A(1) / (A(a.a0) * A(a.present));
+  int m = 1;
+  for (int f = 0; f < a.nf; ++f)
+    if (k >= a.off[f]) m = a.mult[f];
+  return A(1) / (A(2) * A(m) * A(a.present));
+}
+
+// What a row's unit is.  Units: V numbers of one kind (scalars, or whole pairs), their gates V or V / 2 numbers.
+// Copies (kCopies): one copy, of one or two numbers, V = 2.
+template <typename X, typename U, bool kCopies>
+struct RnUnit {
+  using A = typename RnAcc<X>::type;
+  using Args = RnArgs<X, U>;
+  static constexpr int V = kCopies ? 2 : 16 / (int)sizeof(X);
+  static __device__ __forceinline__ int first(const Args& a, int unit) {
+    if constexpr (kCopies)
+      return unit < a.a0 ? unit : 2 * unit - a.a0;
+    else
+      return unit * V;
+  }
+  template <typename T>
+  static __device__ __forceinline__ void load(const Args& a, const T* row, int unit, A (&v)[V]) {
+    const int k = first(a, unit);
+    if constexpr (kCopies) {
+      v[0] = widen(row[k]);
+      v[1] = unit < a.a0 ? A(0) : widen(row[k + 1]);
+    } else {
+      load_n<V>(row + k, v);
+    }
+  }
+  template <typename T>
+  static __device__ __forceinline__ void store(const Args& a, T* row, int unit, const A (&v)[V]) {
+    const int k = first(a, unit);
+    if constexpr (kCopies) {
+      T t;
+      narrow(v[0], t);
+      row[k] = t;
+      if (unit >= a.a0) {
+        narrow(v[1], t);
+        row[k + 1] = t;
+      }
+    } else {
+      store_n<V>(row + k, v);
+    }
+  }
+  // the gates of a unit's numbers, a pair's given twice
+  static __device__ __forceinline__ void load_gates(const Args& a, const X* row, int unit, A (&g)[V]) {
+    if constexpr (kCopies) {
+      g[0] = g[1] = widen(row[unit]);
+    } else if (unit < a.scalar_units) {
+      A lo[V / 2], hi[V / 2];
+      load_n<V / 2>(row + unit * V, lo);
+      load_n<V / 2>(row + unit * V + V / 2, hi);
+#pragma unroll
+      for (int i = 0; i < V / 2; ++i) {
+        g[i] = lo[i];
+        g[V / 2 + i] = hi[i];
+      }
+    } else {
+      A z[V / 2];
+      load_n<V / 2>(row + a.a0 + (unit * V - a.a0) / 2, z);
+#pragma unroll
+      for (int i = 0; i < V; ++i) g[i] = z[i / 2];
+    }
+  }
+  static __device__ __forceinline__ void store_gates(const Args& a, X* row, int unit, const A (&d)[V]) {
+    if constexpr (kCopies) {
+      X t;
+      narrow(unit < a.a0 ? d[0] : d[0] + d[1], t);
+      row[unit] = t;
+    } else if (unit < a.scalar_units) {
+      A lo[V / 2], hi[V / 2];
+#pragma unroll
+      for (int i = 0; i < V / 2; ++i) {
+        lo[i] = d[i];
+        hi[i] = d[V / 2 + i];
+      }
+      store_n<V / 2>(row + unit * V, lo);
+      store_n<V / 2>(row + unit * V + V / 2, hi);
+    } else {
+      A z[V / 2];
+#pragma unroll
+      for (int i = 0; i < V / 2; ++i) z[i] = d[2 * i] + d[2 * i + 1];
+      store_n<V / 2>(row + a.a0 + (unit * V - a.a0) / 2, z);
+    }
+  }
+};
+
+enum Table { kGain = 0, kOffset = 1, kNextGain = 2, kNextOffset = 3, kShare = 4, kTables = 5 };
+
+// Coordinate k's number of table t: s g_p, s b_p, g_n, b_n, its share.
+template <typename Args>
+__device__ __forceinline__ typename Args::A coefficient(const Args& a, int t, int k) {
+  using A = typename Args::A;
+  const A s = a.scale ? a.scale[k] : A(1);
+  switch (t) {
+    case kGain: return a.gain ? s * a.gain[k] : s;
+    case kOffset: return a.offset && k < a.a0 ? s * a.offset[k] : A(0);
+    case kNextGain: return a.next_gain ? a.next_gain[k] : A(0);
+    case kNextOffset: return a.next_offset && k < a.a0 ? a.next_offset[k] : A(0);
+    default: return share_of(a, k);
+  }
+}
+
+// The coefficients of a unit's numbers: from LDS (units), or from memory (copies: zero past a scalar).
+template <typename X, typename U, bool kCopies>
+struct RnTables {
+  using A = typename RnAcc<X>::type;
+  using Args = RnArgs<X, U>;
+  using Unit = RnUnit<X, U, kCopies>;
+  static constexpr int V = Unit::V;
+  A* lds;
+  __device__ __forceinline__ void fill(const Args& a, A* shared, int first, int last) {
+    lds = shared;
+    if constexpr (!kCopies) {
+      for (int t = first; t < last; ++t)
+        for (int k = threadIdx.x; k < a.D; k += kRnThreads) lds[t * a.D + k] = coefficient(a, t, k);
+      __syncthreads();
+    }
+  }
+  __device__ __forceinline__ void get(const Args& a, int t, int unit, A (&c)[V]) const {
+    const int k = Unit::first(a, unit);
+    if constexpr (kCopies) {
+      c[0] = coefficient(a, t, k);
+      c[1] = unit < a.a0 ? A(0) : coefficient(a, t, k + 1);
+    } else {
+      load_n<V>(lds + t * a.D + k, c);
+    }
+  }
+};
+
+// Sum over a row's lanes; every lane gets it.
+template <typename A>
+__device__ __forceinline__ A row_sum(A v, int lanes) {
+  for (int o = 1; o < lanes; o <<= 1) v += __shfl_xor(v, o, kWave);
+  return v;
+}
+
+// Mean of the scalars and 1 / d of the numbers a row's lanes hold.
+template <typename X, typename U, bool kCopies, int NS>
+__device__ __forceinline__ void row_stats(const RnArgs<X, U>& a, const RnTables<X, U, kCopies>& tables, int lane,
+                                          const typename RnAcc<X>::type (&v)[NS][RnUnit<X, U, kCopies>::V],
+                                          typename RnAcc<X>::type eps, typename RnAcc<X>::type& mean,
+                                          typename RnAcc<X>::type& inv_d) {
+  using A = typename RnAcc<X>::type;
+  constexpr int V = RnUnit<X, U, kCopies>::V;
+  A s = A(0);
+#pragma unroll
+  for (int j = 0; j < NS; ++j) {
+    if (lane + j * a.lanes < a.scalar_units) {
+#pragma unroll
+      for (int i = 0; i < V; ++i) s += v[j][i];  // a scalar copy's second number is zero
+    }
+  }
+  mean = a.a0 > 0 ? row_sum(s, a.lanes) / A(a.a0) : A(0);
+  A q = A(0);
+#pragma unroll
+  for (int j = 0; j < NS; ++j) {
+    const int unit = lane + j * a.lanes;
+    if (unit < a.units) {
+      A w[V];
+      tables.get(a, kShare, unit, w);
+      const A m = unit < a.scalar_units ? mean : A(0);
+#pragma unroll
+      for (int i = 0; i < V; ++i) {
+        const A c = v[j][i] - m;
+        q += w[i] * c * c;
+      }
+    }
+  }
+  inv_d = A(1) / sqrt(row_sum(q, a.lanes) + eps);
+}
+
+template <typename A>
+__device__ __forceinline__ A rn_sigmoid(A z) {
+  return A(1) / (A(1) + gm_exp(-z));
+}
+
+template <typename X, typename U, bool kCopies, int NS>
+__global__ __launch_bounds__(kRnThreads) void residual_norm_forward_kernel(RnArgs<X, U> a) {
+  using A = typename RnAcc<X>::type;
+  using Unit = RnUnit<X, U, kCopies>;
+  constexpr int V = Unit::V;
+  extern __shared__ __align__(16) unsigned char rn_lds[];
+  RnTables<X, U, kCopies> tables;
+  tables.fill(a, reinterpret_cast<A*>(rn_lds), 0, kTables);
+  const int in_wave = threadIdx.x % kWave, lane = in_wave & (a.lanes - 1);
+  const int per_wave = kWave >> a.shift;
+  const int64_t step = (int64_t)gridDim.x * kRnWaves * per_wave;
+  int64_t row = ((int64_t)blockIdx.x * kRnWaves + threadIdx.x / kWave) * per_wave + (in_wave >> a.shift);
+  // whole waves take every step: the rows past the last one shadow it and store nothing
+  for (int64_t at = row - (in_wave >> a.shift); at < a.n_rows; at += step, row += step) {
+    const bool live = row < a.n_rows;
+    const int64_t r = live ? row : a.n_rows - 1;
+    A x[NS][V], u[NS][V], g[NS][V];
+#pragma unroll
+    for (int j = 0; j < NS; ++j) {
+      const int unit = lane + j * a.lanes;
+#pragma unroll
+      for (int i = 0; i < V; ++i) x[j][i] = u[j][i] = g[j][i] = A(0);
+      if (unit < a.units) {
+        Unit::load(a, a.u + r * a.D, unit, u[j]);
+        Unit::load(a, a.x + r * a.D, unit, x[j]);
+        if (a.z) Unit::load_gates(a, a.z + r * a.copies, unit, g[j]);
+      }
+    }
+    A mean = A(0), inv = A(1);
+    if (a.gain) row_stats<X, U, kCopies, NS>(a, tables, lane, u, a.eps, mean, inv);
+#pragma unroll
+    for (int j = 0; j < NS; ++j) {
+      const int unit = lane + j * a.lanes;
+      if (unit < a.units) {
+        A gain[V], offset[V];
+        tables.get(a, kGain, unit, gain);
+        tables.get(a, kOffset, unit, offset);
+        const A m = unit < a.scalar_units ? mean : A(0);
+#pragma unroll
+        for (int i = 0; i < V; ++i) {
+          const A b = gain[i] * ((u[j][i] - m) * inv) + offset[i];
+          x[j][i] += a.z ? a.factor * rn_sigmoid(g[j][i]) * b : b;
+        }
+        if (kCopies && unit < a.a0) x[j][1] = A(0);
+        if (live) Unit::store(a, a.y + r * a.D, unit, x[j]);
+      }
+    }
+    A mean2 = A(0), inv2 = A(1);
+    if (a.next_gain) {
+      row_stats<X, U, kCopies, NS>(a, tables, lane, x, a.next_eps, mean2, inv2);
+#pragma unroll
+      for (int j = 0; j < NS; ++j) {
+        const int unit = lane + j * a.lanes;
+        if (unit < a.units) {
+          A gain[V], offset[V], out[V];
+          tables.get(a, kNextGain, unit, gain);
+          tables.get(a, kNextOffset, unit, offset);
+          const A m = unit < a.scalar_units ? mean2 : A(0);
+#pragma unroll
+          for (int i = 0; i < V; ++i) out[i] = gain[i] * ((x[j][i] - m) * inv2) + offset[i];
+          if (live) Unit::store(a, a.normed + r * a.D, unit, out);
+        }
+      }
+    }
+    if (a.stats && live && lane == 0) {
+      A* st = a.stats + 4 * r;
+      st[0] = mean;
+      st[1] = inv;
+      st[2] = mean2;
+      st[3] = inv2;
+    }
+  }
+}
+
+template <typename X, typename U, bool kCopies, int NS>
+__global__ __launch_bounds__(kRnThreads) void residual_norm_backward_kernel(RnArgs<X, U> a) {
+  using A = typename RnAcc<X>::type;
+  using Unit = RnUnit<X, U, kCopies>;
+  constexpr int V = Unit::V;
+  extern __shared__ __align__(16) unsigned char rn_lds[];
+  RnTables<X, U, kCopies> tables;
+  tables.fill(a, reinterpret_cast<A*>(rn_lds), 0, kTables);
+  const int in_wave = threadIdx.x % kWave, lane = in_wave & (a.lanes - 1);
+  const int per_wave = kWave >> a.shift;
+  const int64_t step = (int64_t)gridDim.x * kRnWaves * per_wave;
+  const A by_scalars = a.a0 > 0 ? A(1) / A(a.a0) : A(0);
+  // the sums over this lane's rows: G act uhat, G act, dn xhat, dn
+  A sums[4][NS][V];
+#pragma unroll
+  for (int t = 0; t < 4; ++t)
+#pragma unroll
+    for (int j = 0; j < NS; ++j)
+#pragma unroll
+      for (int i = 0; i < V; ++i) sums[t][j][i] = A(0);
+  int64_t row = ((int64_t)blockIdx.x * kRnWaves + threadIdx.x / kWave) * per_wave + (in_wave >> a.shift);
+  for (int64_t at = row - (in_wave >> a.shift); at < a.n_rows; at += step, row += step) {
+    const bool live = row < a.n_rows;
+    const int64_t r = live ? row : a.n_rows - 1;
+    const A* st = a.stats + 4 * r;
+    const A mean = st[0], inv = st[1], mean2 = st[2], inv2 = st[3];
+    A uh[NS][V], G[NS][V], act[NS][V], xh[NS][V], dn[NS][V];
+#pragma unroll
+    for (int j = 0; j < NS; ++j) {
+      const int unit = lane + j * a.lanes;
+#pragma unroll
+      for (int i = 0; i < V; ++i) uh[j][i] = G[j][i] = xh[j][i] = dn[j][i] = act[j][i] = A(0);
+      if (unit < a.units) {
+        Unit::load(a, a.u + r * a.D, unit, uh[j]);
+        if (a.z) Unit::load_gates(a, a.z + r * a.copies, unit, act[j]);
+        if (a.dy) Unit::load(a, a.dy + r * a.D, unit, G[j]);
+        if (a.dn) {
+          Unit::load(a, a.x + r * a.D, unit, xh[j]);
+          Unit::load(a, a.dn + r * a.D, unit, dn[j]);
+        }
+      }
+    }
+    // uhat, and xhat from the sum formed again; p and m, the next norm's two sums
+    A p = A(0), m = A(0);
+#pragma unroll
+    for (int j = 0; j < NS; ++j) {
+      const int unit = lane + j * a.lanes;
+      if (unit < a.units) {
+        const bool scalar = unit < a.scalar_units;
+#pragma unroll
+        for (int i = 0; i < V; ++i) {
+          uh[j][i] = (uh[j][i] - (scalar ? mean : A(0))) * inv;
+          act[j][i] = a.z ? rn_sigmoid(act[j][i]) : A(1);
+        }
+        if (a.dn) {
+          A gain[V], offset[V], next[V];
+          tables.get(a, kGain, unit, gain);
+          tables.get(a, kOffset, unit, offset);
+          tables.get(a, kNextGain, unit, next);
+#pragma unroll
+          for (int i = 0; i < V; ++i) {
+            const A b = gain[i] * uh[j][i] + offset[i];
+            const A y = xh[j][i] + (a.z ? a.factor * act[j][i] * b : b);
+            xh[j][i] = (y - (scalar ? mean2 : A(0))) * inv2;
+            const A gh = next[i] * dn[j][i];
+            p += gh * xh[j][i];
+            if (scalar) m += gh;
+          }
+        }
+      }
+    }
+    if (a.dn) {
+      p = row_sum(p, a.lanes);
+      m = row_sum(m, a.lanes) * by_scalars;
+    }
+    A p1 = A(0), m1 = A(0);
+#pragma unroll
+    for (int j = 0; j < NS; ++j) {
+      const int unit = lane + j * a.lanes;
+      if (unit < a.units) {
+        const bool scalar = unit < a.scalar_units;
+        A gain[V], offset[V], d[V];
+        if (a.dn) {
+          A next[V], w[V];
+          tables.get(a, kNextGain, unit, next);
+          tables.get(a, kShare, unit, w);
+#pragma unroll
+          for (int i = 0; i < V; ++i)
+            G[j][i] += inv2 * (next[i] * dn[j][i] - (scalar ? m : A(0)) - p * xh[j][i] * w[i]);
+        }
+        if (kCopies && scalar) G[j][1] = A(0);
+        if (live) Unit::store(a, a.dx + r * a.D, unit, G[j]);
+        tables.get(a, kGain, unit, gain);
+        tables.get(a, kOffset, unit, offset);
+#pragma unroll
+        for (int i = 0; i < V; ++i) {
+          const A s = act[j][i], f = a.z ? a.factor * s : A(1);
+          d[i] = G[j][i] * (gain[i] * uh[j][i] + offset[i]) * f * (A(1) - s);  // of the gate's argument
+          G[j][i] *= f;
+          if (live) {
+            sums[0][j][i] += G[j][i] * uh[j][i];
+            if (scalar) sums[1][j][i] += G[j][i];
+            if (a.dn) {
+              sums[2][j][i] += dn[j][i] * xh[j][i];
+              if (scalar) sums[3][j][i] += dn[j][i];
+            }
+          }
+          G[j][i] *= gain[i];
+          p1 += G[j][i] * uh[j][i];
+          if (scalar) m1 += G[j][i];
+        }
+        if (a.z && live) Unit::store_gates(a, a.dz + r * a.copies, unit, d);
+      }
+    }
+    if (a.gain) {
+      p1 = row_sum(p1, a.lanes);
+      m1 = row_sum(m1, a.lanes) * by_scalars;
+    }
+#pragma unroll
+    for (int j = 0; j < NS; ++j) {
+      const int unit = lane + j * a.lanes;
+      if (unit < a.units) {
+        if (a.gain) {
+          A w[V];
+          tables.get(a, kShare, unit, w);
+#pragma unroll
+          for (int i = 0; i < V; ++i)
+            G[j][i] = inv * (G[j][i] - (unit < a.scalar_units ? m1 : A(0)) - p1 * uh[j][i] * w[i]);
+        }
+        if (live) Unit::store(a, a.du + r * a.D, unit, G[j]);
+      }
+    }
+  }
+  // over the wave's rows, then over the workgroup's waves in order
+  A* shared = reinterpret_cast<A*>(rn_lds);
+  const int width = a.units * V;
+  const int wave = threadIdx.x / kWave;
+#pragma unroll
+  for (int t = 0; t < 4; ++t) {
+#pragma unroll
+    for (int j = 0; j < NS; ++j)
+#pragma unroll
+      for (int i = 0; i < V; ++i)
+        for (int o = a.lanes; o < kWave; o <<= 1) sums[t][j][i] += __shfl_xor(sums[t][j][i], o, kWave);
+    __syncthreads();  // the coefficients, and the last table's sums, have been read
+    for (int w = 0; w < kRnWaves; ++w) {
+      if (wave == w && in_wave < a.lanes) {
+#pragma unroll
+        for (int j = 0; j < NS; ++j) {
+          const int unit = lane + j * a.lanes;
+          if (unit < a.units) {
+#pragma unroll
+            for (int i = 0; i < V; ++i) {
+              A* to = shared + unit * V + i;
+              *to = w == 0 ? sums[t][j][i] : *to + sums[t][j][i];
+            }
+          }
+        }
+      }
+      __syncthreads();
+    }
+    for (int k = threadIdx.x; k < width; k += kRnThreads)
+      a.partial[((int64_t)blockIdx.x * 4 + t) * width + k] = shared[k];
+  }
+}
+
+// The parameters' gradients from the workgroups' sums: kCols coordinates a workgroup, kRnThreads / kCols threads a
+// coordinate, each over every kRnThreads / kCols-th row in order, then in order over the threads.
+constexpr int kRnCols = 8;
+template <typename X, typename U, bool kCopies>
+__global__ __launch_bounds__(kRnThreads) void residual_norm_reduce_kernel(RnArgs<X, U> a, int64_t blocks) {
+  using A = typename RnAcc<X>::type;
+  using Unit = RnUnit<X, U, kCopies>;
+  constexpr int V = Unit::V, kParts = kRnThreads / kRnCols;
+  __shared__ A part[4][kParts][kRnCols];
+  const int c = threadIdx.x % kRnCols, from = threadIdx.x / kRnCols;
+  const int k = blockIdx.x * kRnCols + c, width = a.units * V;
+  const bool live = k < a.D;
+  int at = k;  // where the sums hold coordinate k
+  if constexpr (kCopies) at = k < a.a0 ? 2 * k : k + a.a0;
+  A s[4] = {A(0), A(0), A(0), A(0)};
+  if (live) {
+    for (int64_t b = from; b < blocks; b += kParts)
+#pragma unroll
+      for (int t = 0; t < 4; ++t) s[t] += a.partial[(b * 4 + t) * width + at];
+  }
+#pragma unroll
+  for (int t = 0; t < 4; ++t) part[t][from][c] = s[t];
+  __syncthreads();
+  if (from != 0 || !live) return;
+#pragma unroll
+  for (int t = 0; t < 4; ++t) {
+    s[t] = A(0);
+    for (int w = 0; w < kParts; ++w) s[t] += part[t][w][c];
+  }
+  const bool scalar = k < a.a0;
+  const A scale = a.scale ? a.scale[k] : A(1), gain = a.gain ? a.gain[k] : A(1);
+  const A offset = a.offset && scalar ? a.offset[k] : A(0);
+  A* out = a.dparams;
+  out[k] = scale * s[0];
+  if (scalar) out[a.D + k] = scale * s[1];
+  out[a.D + a.a0 + k] = gain * s[0] + offset * s[1];
+  out[2 * a.D + a.a0 + k] = s[2];
+  if (scalar) out[3 * a.D + a.a0 + k] = s[3];
+}
+
+// ------------------------------------------------------------------ launch
+
+// Units a lane holds at most: the rows' numbers and the backward's sums are registers (20 numbers of float rows, 24 of
+// bfloat16 ones, 16 of double ones; a wide row's copies, 32).
+template <typename X, bool kCopies>
+constexpr int kMaxUnits = kCopies ? 16 : (sizeof(X) == 4 ? 5 : (sizeof(X) == 2 ? 3 : 8));
+
+template <typename X, typename U, bool kCopies, int NS>
+int launch_rn(bool backward, const RnArgs<X, U>& a, hipStream_t stream, int64_t& blocks) {
+  using A = typename RnAcc<X>::type;
+  const int64_t rows_per_block = (int64_t)kRnWaves * (kWave >> a.shift);
+  const int width = a.units * RnUnit<X, U, kCopies>::V;
+  const size_t lds = sizeof(A) * std::max<size_t>(kCopies ? 0 : (size_t)kTables * a.D, backward ? width : 0);
+  const void* kernel = backward ? reinterpret_cast<const void*>(&residual_norm_backward_kernel<X, U, kCopies, NS>)
+                                : reinterpret_cast<const void*>(&residual_norm_forward_kernel<X, U, kCopies, NS>);
+  const int64_t want = (a.n_rows + rows_per_block - 1) / rows_per_block;
+  const int64_t slots = resident_blocks(kernel, kRnThreads, lds);
+  // the backward's rows of sums are one a workgroup: its persistent workgroups are what the caller's array was sized for
+  if (backward)
+    blocks = std::min<int64_t>(want, blocks);
+  else
+    blocks = std::min<int64_t>(want, slots > 0 ? slots : 1024);
+  if (backward)
+    hipLaunchKernelGGL((residual_norm_backward_kernel<X, U, kCopies, NS>), dim3((unsigned)blocks), dim3(kRnThreads),
+                       lds, stream, a);
+  else
+    hipLaunchKernelGGL((residual_norm_forward_kernel<X, U, kCopies, NS>), dim3((unsigned)blocks), dim3(kRnThreads),
+                       lds, stream, a);
+  return check_launch(backward ? "residual_norm_backward" : "residual_norm_forward");
+}
+
+template <typename X, typename U, bool kCopies>
+int dispatch_rn(bool backward, RnArgs<X, U>& a, hipStream_t stream, int64_t& blocks) {
+  a.units = kCopies ? a.copies : a.D / RnUnit<X, U, kCopies>::V;
+  a.scalar_units = kCopies ? a.a0 : a.a0 / RnUnit<X, U, kCopies>::V;
+  a.lanes = 1;
+  a.shift = 0;
+  // as few lanes a row as hold it within kMaxUnits a lane, or four copies (whose loads are a number each); the
+  // backward within three units, since its sums take as many registers again as its rows (float rows of five units a
+  // lane: 266 registers and one wave a SIMD, of three 180 and two); the widest rows take the whole wave
+  const int most = kCopies ? 4 : std::min(backward ? 3 : 5, kMaxUnits<X, kCopies>);
+  while (a.lanes < kWave && (a.units + a.lanes - 1) / a.lanes > most) {
+    a.lanes *= 2;
+    ++a.shift;
+  }
+  const int ns = (a.units + a.lanes - 1) / a.lanes;
+#define GM_RN_CASE(n)                                           \
+  if constexpr (n <= kMaxUnits<X, kCopies>) {                   \
+    if (ns <= n) return launch_rn<X, U, kCopies, n>(backward, a, stream, blocks); \
+  }
+  GM_RN_CASE(1)
+  GM_RN_CASE(2)
+  GM_RN_CASE(3)
+  if constexpr (!kCopies && sizeof(X) == 4) {
+    GM_RN_CASE(4)
+    GM_RN_CASE(5)
+  } else {
+    GM_RN_CASE(4)
+    GM_RN_CASE(8)
+    GM_RN_CASE(16)
+  }
+#undef GM_RN_CASE
+  return fail(GM_ERR_UNSUPPORTED, "residual_norm: the row is wider than 1024");
+}
+
+template <typename X, typename U>
+int fill_rn(RnArgs<X, U>& a, int64_t n_rows, int64_t D, int64_t a0, int64_t nf, const int64_t* offsets,
+            const int64_t* mults, double factor, double eps, double next_eps) {
+  using A = typename RnAcc<X>::type;
+  GM_REQUIRE(n_rows >= 0, "the number of rows must be non-negative");
+  GM_REQUIRE(D >= 1 && D <= kRnMaxWidth, "the flat width must lie in 1..1024");
+  GM_REQUIRE(nf >= 0 && nf <= kRnMaxFreq, "at most 8 nonzero frequencies");
+  GM_REQUIRE(a0 >= 0 && a0 <= D, "a0 must lie in 0..D");
+  GM_REQUIRE(nf == 0 || (offsets && mults), "offsets and multiplicities (host arrays) are required");
+  GM_REQUIRE(eps > 0 && next_eps > 0, "eps must be positive");
+  int64_t next = a0, copies = a0;
+  for (int64_t f = 0; f < nf; ++f) {
+    GM_REQUIRE(mults[f] >= 1 && offsets[f] == next, "frequency blocks must follow frequency 0 contiguously");
+    a.off[f] = (int)offsets[f];
+    a.mult[f] = (int)mults[f];
+    next += 2 * mults[f];
+    copies += mults[f];
+  }
+  GM_REQUIRE(next == D, "the frequency blocks must fill the flat width");
+  a.n_rows = n_rows;
+  a.D = (int)D;
+  a.a0 = (int)a0;
+  a.nf = (int)nf;
+  a.copies = (int)copies;
+  a.present = (int)nf + (a0 > 0 ? 1 : 0);
+  a.factor = (A)factor;
+  a.eps = (A)eps;
+  a.next_eps = (A)next_eps;
+  return GM_OK;
+}
+
+// Whole units: every frequency's numbers fill 16-byte pieces of the rows' type, the gates' rows half of them, and the
+// pointers are aligned to them (a wider branch's to 16 bytes as well).
+template <typename X, typename U>
+bool whole_units(const RnArgs<X, U>& a) {
+  constexpr int V = 16 / (int)sizeof(X);
+  if (a.D % V != 0 || a.a0 % V != 0) return false;
+  if (a.z && (a.copies % std::max(V / 2, 1) != 0 || !aligned(a.z, 16) || !aligned(a.dz, 16))) return false;
+  return aligned(a.x, 16) && aligned(a.u, 16) && aligned(a.y, 16) && aligned(a.normed, 16) && aligned(a.dy, 16) &&
+         aligned(a.dn, 16) && aligned(a.dx, 16) && aligned(a.du, 16);
+}
+
+constexpr int64_t kRnMaxBlocks = 512;  // two workgroups a CU: what the backward's registers leave room for
+
+int64_t rn_blocks(int64_t n_rows) {
+  // at least 32 rows a workgroup, so that few rows do not leave many rows of sums to add
+  return std::max<int64_t>(1, std::min<int64_t>((n_rows + 31) / 32, kRnMaxBlocks));
+}
+
+template <typename X, typename U>
+int residual_forward(const X* x, const U* u, const X* z, const typename RnAcc<X>::type* gain,
+                     const typename RnAcc<X>::type* offset, const typename RnAcc<X>::type* scale,
+                     const typename RnAcc<X>::type* next_gain, const typename RnAcc<X>::type* next_offset,
+                     int64_t n_rows, int64_t D, int64_t a0, int64_t nf, const int64_t* offsets, const int64_t* mults,
+                     double factor, double eps, double next_eps, X* y, X* normed, typename RnAcc<X>::type* stats,
+                     void* stream) {
+  RnArgs<X, U> a{};
+  const int rc = fill_rn(a, n_rows, D, a0, nf, offsets, mults, factor, eps, next_eps);
+  if (rc != GM_OK) return rc;
+  if (n_rows == 0) return GM_OK;
+  GM_REQUIRE(x && u && y, "x, u and y must be device pointers");
+  GM_REQUIRE(!next_gain || normed, "normed must be a device pointer where there is a next norm");
+  a.x = x;
+  a.u = u;
+  a.z = z;
+  a.gain = gain;
+  a.offset = gain ? offset : nullptr;
+  a.scale = scale;
+  a.next_gain = next_gain;
+  a.next_offset = next_gain ? next_offset : nullptr;
+  a.y = y;
+  a.normed = normed;
+  a.stats = stats;
+  int64_t blocks = 0;
+  return whole_units(a) ? dispatch_rn<X, U, false>(false, a, (hipStream_t)stream, blocks)
+                        : dispatch_rn<X, U, true>(false, a, (hipStream_t)stream, blocks);
+}
+
+template <typename X, typename U>
+int residual_backward(const X* dy, const X* dn, const X* x, const U* u, const X* z,
+                      const typename RnAcc<X>::type* gain, const typename RnAcc<X>::type* offset,
+                      const typename RnAcc<X>::type* scale, const typename RnAcc<X>::type* next_gain,
+                      const typename RnAcc<X>::type* stats, int64_t n_rows, int64_t D, int64_t a0, int64_t nf,
+                      const int64_t* offsets, const int64_t* mults, double factor, X* dx, U* du, X* dz,
+                      typename RnAcc<X>::type* partial, typename RnAcc<X>::type* dparams, void* stream) {
+  RnArgs<X, U> a{};
+  const int rc = fill_rn(a, n_rows, D, a0, nf, offsets, mults, factor, 1.0, 1.0);
+  if (rc != GM_OK) return rc;
+  GM_REQUIRE(partial && dparams, "partial and dparams must be device pointers");
+  if (n_rows > 0) {
+    GM_REQUIRE(x && u && stats && dx && du, "x, u, stats, dx and du must be device pointers");
+    GM_REQUIRE(!z || dz, "dz must be a device pointer where there are gates");
+    GM_REQUIRE(!dn || next_gain, "a gradient of the next norm needs its gains");
+  }
+  a.dy = dy;
+  a.dn = dn;
+  a.x = x;
+  a.u = u;
+  a.z = z;
+  a.gain = gain;
+  a.offset = gain ? offset : nullptr;
+  a.scale = scale;
+  a.next_gain = next_gain;
+  a.stats = const_cast<typename RnAcc<X>::type*>(stats);  // read only here
+  a.dx = dx;
+  a.du = du;
+  a.dz = dz;
+  a.partial = partial;
+  a.dparams = dparams;
+  int64_t blocks = n_rows > 0 ? rn_blocks(n_rows) : 0;
+  const bool units = whole_units(a);
+  const hipStream_t s = (hipStream_t)stream;
+  if (n_rows > 0) {
+    const int status = units ? dispatch_rn<X, U, false>(true, a, s, blocks) : dispatch_rn<X, U, true>(true, a, s, blocks);
+    if (status != GM_OK) return status;
+  }
+  const dim3 grid((unsigned)((D + kRnCols - 1) / kRnCols));
+  if (units)
+    hipLaunchKernelGGL((residual_norm_reduce_kernel<X, U, false>), grid, dim3(kRnThreads), 0, s, a, blocks);
+  else
+    hipLaunchKernelGGL((residual_norm_reduce_kernel<X, U, true>), grid, dim3(kRnThreads), 0, s, a, blocks);
+  return check_launch("residual_norm_backward (reduce)");
+}
+
+}  // namespace
+}  // namespace gm
+
+extern "C" int64_t gm_residual_norm_partial_rows(int64_t n_rows) { return n_rows > 0 ? 4 * gm::rn_blocks(n_rows) : 4; }
+
+// X, U: the rows' and the branch's element types in the C signature, TX, TU the kernels'; A the parameters'.
+#define GM_RESIDUAL_ENTRY(SFX, X, U, TX, TU, A)                                                                        \
+  extern "C" int gm_residual_norm_forward_##SFX(                                                                       \
+      const X* x, const U* u, const X* z, const A* gain, const A* offset, const A* scale, const A* next_gain,          \
+      const A* next_offset, int64_t n_rows, int64_t D, int64_t a0, int64_t nf, const int64_t* offsets,                 \
+      const int64_t* mults, double factor, double eps, double next_eps, X* y, X* normed, A* stats, void* stream) {     \
+    return gm::residual_forward<TX, TU>(reinterpret_cast<const TX*>(x), reinterpret_cast<const TU*>(u),                \
+                                        reinterpret_cast<const TX*>(z), gain, offset, scale, next_gain, next_offset,   \
+                                        n_rows, D, a0, nf, offsets, mults, factor, eps, next_eps,                      \
+                                        reinterpret_cast<TX*>(y), reinterpret_cast<TX*>(normed), stats, stream);       \
+  }                                                                                                                    \
+  extern "C" int gm_residual_norm_backward_##SFX(                                                                      \
+      const X* dy, const X* dn, const X* x, const U* u, const X* z, const A* gain, const A* offset, const A* scale,    \
+      const A* next_gain, const A* stats, int64_t n_rows, int64_t D, int64_t a0, int64_t nf, const int64_t* offsets,   \
+      const int64_t* mults, double factor, X* dx, U* du, X* dz, A* partial, A* dparams, void* stream) {                \
+    return gm::residual_backward<TX, TU>(                                                                              \
+        reinterpret_cast<const TX*>(dy), reinterpret_cast<const TX*>(dn), reinterpret_cast<const TX*>(x),              \
+        reinterpret_cast<const TU*>(u), reinterpret_cast<const TX*>(z), gain, offset, scale, next_gain, stats, n_rows, \
+        D, a0, nf, offsets, mults, factor, reinterpret_cast<TX*>(dx), reinterpret_cast<TU*>(du),                       \
+        reinterpret_cast<TX*>(dz), partial, dparams, stream);                                                          \
+  }
+
+GM_RESIDUAL_ENTRY(f32, float, float, float, float, float)
+GM_RESIDUAL_ENTRY(f64, double, double, double, double, double)
+GM_RESIDUAL_ENTRY(bf16, uint16_t, uint16_t, gm::rbf16, gm::rbf16, float)
+GM_RESIDUAL_ENTRY(bf16_f32, uint16_t, float, gm::rbf16, float, float)

@@ -111,6 +111,11 @@ SIGNATURES_F32 = {
        for sfx in ("f32", "f64", "bf16")},
     **{f"gm_gate_backward_{sfx}": (ctypes.c_int, [_P] * 3 + [_I] * 4 + [_P, _P, _I] + [_P] * 3)
        for sfx in ("f32", "f64", "bf16")},
+    "gm_residual_norm_partial_rows": (ctypes.c_int64, [_I]),
+    **{f"gm_residual_norm_forward_{sfx}": (ctypes.c_int, [_P] * 8 + [_I] * 4 + [_P, _P, _D, _D, _D] + [_P] * 4)
+       for sfx in ("f32", "f64", "bf16", "bf16_f32")},
+    **{f"gm_residual_norm_backward_{sfx}": (ctypes.c_int, [_P] * 10 + [_I] * 4 + [_P, _P, _D] + [_P] * 6)
+       for sfx in ("f32", "f64", "bf16", "bf16_f32")},
 }
 
 
@@ -1546,3 +1551,64 @@ def gate_backward(gy: Tensor, h: Tensor, pre: Tensor, layout: PointwiseLayout,
     _call(f"gm_gate_backward_{sfx}", _ptr(gy), _ptr(h), _ptr(pre), h.shape[0], *layout.args(), int(double_sigmoid),
           _ptr(dh), _ptr(dpre), _stream(h.device))
     return dh, dpre
+
+
+def _residual_check(x: Tensor, u: Tensor, z: Tensor | None, layout: PointwiseLayout,
+                    vectors: tuple[tuple[str, Tensor | None, int], ...]) -> str:
+    """The residual sum's suffix, its rows and per-coordinate vectors checked."""
+    sfx = _pw_check(x, layout)
+    _require_device(x, u, *(t for t in (z, *(v for _, v, _ in vectors)) if t is not None))
+    wide = x.dtype == torch.bfloat16 and u.dtype == torch.float32
+    _check(u.dtype == x.dtype or wide, f"u must be {x.dtype} (or float32 for bfloat16 rows), got {u.dtype}")
+    _check(u.shape == x.shape, "u must be shaped as x")
+    copies = layout.a0 + layout.G
+    _check(z is None or (z.dtype == x.dtype and tuple(z.shape) == (x.shape[0], copies)),
+           f"z must be (n_nodes, {copies}) in x's dtype")
+    pd = param_dtype(x.dtype)
+    for name, t, n in vectors:
+        _check(t is None or (t.dtype == pd and tuple(t.shape) == (n,)), f"{name} must be ({n},) {pd}")
+    return sfx + ("_f32" if wide else "")
+
+
+def residual_norm_forward(x: Tensor, u: Tensor, z: Tensor | None, gain: Tensor | None, offset: Tensor | None,
+                          scale: Tensor | None, next_gain: Tensor | None, next_offset: Tensor | None,
+                          layout: PointwiseLayout, factor: float, eps: float, next_eps: float,
+                          train: bool) -> tuple[Tensor, Tensor | None, Tensor | None]:
+    """``(y, normed, stats)``: the residual sum and the norm behind it (None without ``next_gain``);
+    ``stats (n_nodes, 4)``, what the backward reads of both norms, under ``train``."""
+    D, a0 = layout.D, layout.a0
+    sfx = _residual_check(x, u, z, layout, (("gain", gain, D), ("offset", offset, a0), ("scale", scale, D),
+                                            ("next_gain", next_gain, D), ("next_offset", next_offset, a0)))
+    y = torch.empty_like(x)
+    normed = None if next_gain is None else torch.empty_like(x)
+    stats = torch.empty(x.shape[0], 4, dtype=param_dtype(x.dtype), device=x.device) if train else None
+    with torch.cuda.device(x.device):
+        _call(f"gm_residual_norm_forward_{sfx}", _ptr(x), _ptr(u), _ptr(z), _ptr(gain), _ptr(offset), _ptr(scale),
+              _ptr(next_gain), _ptr(next_offset), x.shape[0], *layout.args(), float(factor), float(eps),
+              float(next_eps), _ptr(y), _ptr(normed), _ptr(stats), _stream(x.device))
+    return y, normed, stats
+
+
+def residual_norm_backward(dy: Tensor | None, dn: Tensor | None, x: Tensor, u: Tensor, z: Tensor | None,
+                           gain: Tensor | None, offset: Tensor | None, scale: Tensor | None,
+                           next_gain: Tensor | None, stats: Tensor, layout: PointwiseLayout,
+                           factor: float) -> tuple[Tensor, Tensor, Tensor | None, Tensor]:
+    """``(dx, du, dz, dparams)`` with ``dparams = (dgain (D), doffset (a0), dscale (D),
+    dnext_gain (D), dnext_offset (a0))`` summed over the nodes in a fixed order."""
+    D, a0, n = layout.D, layout.a0, x.shape[0]
+    sfx = _residual_check(x, u, z, layout, (("gain", gain, D), ("offset", offset, a0), ("scale", scale, D),
+                                            ("next_gain", next_gain, D)))
+    pd = param_dtype(x.dtype)
+    for name, t in (("dy", dy), ("dn", dn)):
+        _check(t is None or (t.dtype == x.dtype and t.shape == x.shape and t.is_contiguous()
+                             and t.device == x.device), f"{name} must match x (contiguous)")
+    _check(stats.dtype == pd and tuple(stats.shape) == (n, 4) and stats.is_contiguous(), f"stats must be ({n}, 4) {pd}")
+    dx, du = torch.empty_like(x), torch.empty_like(u)
+    dz = None if z is None else torch.empty_like(z)
+    partial = torch.empty(int(library().gm_residual_norm_partial_rows(n)), D + a0, dtype=pd, device=x.device)
+    dparams = torch.empty(3 * D + 2 * a0, dtype=pd, device=x.device)
+    with torch.cuda.device(x.device):
+        _call(f"gm_residual_norm_backward_{sfx}", _ptr(dy), _ptr(dn), _ptr(x), _ptr(u), _ptr(z), _ptr(gain),
+              _ptr(offset), _ptr(scale), _ptr(next_gain), _ptr(stats), n, *layout.args(), float(factor), _ptr(dx),
+              _ptr(du), _ptr(dz), _ptr(partial), _ptr(dparams), _stream(x.device))
+    return dx, du, dz, dparams
