@@ -21,12 +21,13 @@
 // gradient.
 //
 // One pass over the data each way, so the bytes bound it.  A row's units (16
-// bytes of the rows' type, or one copy where a multiplicity, a pointer or the
-// gates' rows are not whole units) are shared by 2^k lanes with at most
+// bytes of float or double, 8 of bfloat16, or one copy where a multiplicity, a
+// pointer or the gates' rows are not whole units) are shared by 2^k lanes with at most
 // kMaxUnits<...> units a lane, all in registers; the norms' sums are shuffles
-// within those lanes; a wave holds 64 / 2^k rows.  Coefficients sit in LDS (the
-// unit form), since each lane would otherwise hold four registers of them for
-// every number of a row.  The waves are persistent; the backward's sums stay in
+// within those lanes; a wave holds 64 / 2^k rows.  Coefficients sit in LDS, since
+// each lane would otherwise hold five registers of them for every number of a row;
+// a workgroup makes them from the parameters as the modules hold them, so a call
+// is one launch forward and two backward.  The waves are persistent; the backward's sums stay in
 // registers over a wave's rows, are added over the workgroup in a fixed order,
 // and a second kernel adds the workgroups' rows in a fixed order (no atomics).
 #include <algorithm>
@@ -37,7 +38,8 @@
 namespace gm {
 namespace {
 
-constexpr int kRnMaxFreq = 8;
+constexpr int kRnMaxFreq = 8;           // nonzero frequencies
+constexpr int kRnSlots = kRnMaxFreq + 1;  // frequency 0, then the nonzero ones
 constexpr int kRnThreads = 256;
 constexpr int kRnWaves = kRnThreads / kWave;
 constexpr int kRnMaxWidth = 1024;
@@ -67,12 +69,44 @@ __device__ __forceinline__ void narrow(float v, rbf16& o) {
   __builtin_memcpy(&o.bits, &b, 2);
 }
 
-// V consecutive numbers of type T at p as one load or store of up to 16 bytes each.
+// V consecutive numbers of type T at p as one load or store of up to 16 bytes each; bfloat16 ones as 32-bit words.
 template <typename T, int V>
 struct alignas(sizeof(T) * V >= 16 ? 16 : sizeof(T) * V) Pack {
   T v[V];
 };
 
+typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
+template <int V>
+__device__ __forceinline__ void load_n(const rbf16* p, float (&out)[V]) {
+  static_assert(V == 2 || V == 4, "whole words");
+  uint32_t w[V / 2];
+  if constexpr (V == 4) {
+    const uint2 x = *reinterpret_cast<const uint2*>(p);
+    w[0] = x.x;
+    w[1] = x.y;
+  } else {
+    w[0] = *reinterpret_cast<const uint32_t*>(p);
+  }
+#pragma unroll
+  for (int i = 0; i < V / 2; ++i) {
+    out[2 * i] = __uint_as_float(w[i] << 16);
+    out[2 * i + 1] = __uint_as_float(w[i] & 0xFFFF0000u);
+  }
+}
+template <int V>
+__device__ __forceinline__ void store_n(rbf16* p, const float (&in)[V]) {
+  static_assert(V == 2 || V == 4, "whole words");
+  uint32_t w[V / 2];
+#pragma unroll
+  for (int i = 0; i < V / 2; ++i) {
+    const bf16x2 b = {static_cast<__bf16>(in[2 * i]), static_cast<__bf16>(in[2 * i + 1])};
+    w[i] = __builtin_bit_cast(uint32_t, b);
+  }
+  if constexpr (V == 4)
+    *reinterpret_cast<uint2*>(p) = make_uint2(w[0], w[1]);
+  else
+    *reinterpret_cast<uint32_t*>(p) = w[0];
+}
 template <int V, typename T, typename A>
 __device__ __forceinline__ void load_n(const T* p, A (&out)[V]) {
   const Pack<T, V> x = *reinterpret_cast<const Pack<T, V>*>(p);
@@ -98,11 +132,13 @@ struct RnArgs {
   const X* x;
   const U* u;
   const X* z;           // (n_rows, copies) or null
-  const A* gain;        // (D) or null: the branch is not normalised
-  const A* offset;      // (a0) or null
-  const A* scale;       // (D) or null
-  const A* next_gain;   // (D) or null: nothing normalised behind the sum
-  const A* next_offset; // (a0) or null
+  // the parameters as the modules hold them: a vector a frequency, one number a copy
+  const A* gain[kRnSlots];       // where normalise
+  const A* scale[kRnSlots];      // where scaled
+  const A* next_gain[kRnSlots];  // where next
+  const A* offset;               // (a0) or null
+  const A* next_offset;          // (a0) or null
+  bool normalise, scaled, next;  // the branch is normalised, its copies scaled, the sum normalised
   A factor, eps, next_eps;
   X* y;
   X* normed;
@@ -114,27 +150,30 @@ struct RnArgs {
   U* du;
   X* dz;
   A* partial;  // (workgroups, 4, units V)
-  A* dparams;  // dgain (D), doffset (a0), dscale (D), dnext_gain (D), dnext_offset (a0)
+  A* dparams;  // dgain (copies), doffset (a0), dscale (copies), dnext_gain (copies), dnext_offset (a0)
 };
 
-// Coordinate k's share of the pooled mean square.
+// Where coordinate k sits: its frequency's slot, its copy among that frequency's, that frequency's copies.
+struct RnPlace {
+  int slot, copy, mult;
+};
 template <typename Args>
-__device__ __forceinline__ typename Args::A share_of(const Args& a, int k) {
-  using A = typename Args::A;
-  if (k < a.a0) return A(1) / (A(a.a0) * A(a.present));
-  int m = 1;
-  for (int f = 0; f < a.nf; ++f)
-    if (k >= a.off[f]) m = a.mult[f];
-  return A(1) / (A(2) * A(m) * A(a.present));
+__device__ __forceinline__ RnPlace place_of(const Args& a, int k) {
+  if (k < a.a0) return {0, k, a.a0};
+  int f = 0;
+  for (int g = 1; g < a.nf; ++g)
+    if (k >= a.off[g]) f = g;
+  return {1 + f, (k - a.off[f]) / 2, a.mult[f]};
 }
 
-// What a row's unit is.  Units: V numbers of one kind (scalars, or whole pairs), their gates V or V / 2 numbers.
-// Copies (kCopies): one copy, of one or two numbers, V = 2.
+// What a row's unit is.  Units: V numbers of one kind (scalars, or whole pairs), their gates V or V / 2 numbers; four
+// of bfloat16 too (eight a unit leave a lane 24 numbers of each row and the backward one wave a SIMD).  Copies
+// (kCopies): one copy, of one or two numbers, V = 2.
 template <typename X, typename U, bool kCopies>
 struct RnUnit {
   using A = typename RnAcc<X>::type;
   using Args = RnArgs<X, U>;
-  static constexpr int V = kCopies ? 2 : 16 / (int)sizeof(X);
+  static constexpr int V = kCopies || sizeof(X) == 8 ? 2 : 4;
   static __device__ __forceinline__ int first(const Args& a, int unit) {
     if constexpr (kCopies)
       return unit < a.a0 ? unit : 2 * unit - a.a0;
@@ -170,20 +209,16 @@ struct RnUnit {
   static __device__ __forceinline__ void load_gates(const Args& a, const X* row, int unit, A (&g)[V]) {
     if constexpr (kCopies) {
       g[0] = g[1] = widen(row[unit]);
-    } else if (unit < a.scalar_units) {
-      A lo[V / 2], hi[V / 2];
-      load_n<V / 2>(row + unit * V, lo);
-      load_n<V / 2>(row + unit * V + V / 2, hi);
-#pragma unroll
-      for (int i = 0; i < V / 2; ++i) {
-        g[i] = lo[i];
-        g[V / 2 + i] = hi[i];
-      }
     } else {
-      A z[V / 2];
-      load_n<V / 2>(row + a.a0 + (unit * V - a.a0) / 2, z);
+      // selects, not a branch's stores: those went through scratch for bfloat16 (510 us against 345 for the backward of
+      // 262,144 rows of 160 with a float branch, 189 against 108 for the forward)
+      const bool scalar = unit < a.scalar_units;
+      A lo[V / 2], hi[V / 2];
+      const X* p = row + (scalar ? unit * V : (unit * V + a.a0) / 2);
+      load_n<V / 2>(p, lo);
+      load_n<V / 2>(scalar ? p + V / 2 : p, hi);
 #pragma unroll
-      for (int i = 0; i < V; ++i) g[i] = z[i / 2];
+      for (int i = 0; i < V; ++i) g[i] = scalar ? (i < V / 2 ? lo[i] : hi[i - V / 2]) : lo[i / 2];
     }
   }
   static __device__ __forceinline__ void store_gates(const Args& a, X* row, int unit, const A (&d)[V]) {
@@ -191,41 +226,24 @@ struct RnUnit {
       X t;
       narrow(unit < a.a0 ? d[0] : d[0] + d[1], t);
       row[unit] = t;
-    } else if (unit < a.scalar_units) {
+    } else {
+      const bool scalar = unit < a.scalar_units;
       A lo[V / 2], hi[V / 2];
+      X* p = row + (scalar ? unit * V : (unit * V + a.a0) / 2);
 #pragma unroll
       for (int i = 0; i < V / 2; ++i) {
-        lo[i] = d[i];
+        lo[i] = scalar ? d[i] : d[2 * i] + d[2 * i + 1];
         hi[i] = d[V / 2 + i];
       }
-      store_n<V / 2>(row + unit * V, lo);
-      store_n<V / 2>(row + unit * V + V / 2, hi);
-    } else {
-      A z[V / 2];
-#pragma unroll
-      for (int i = 0; i < V / 2; ++i) z[i] = d[2 * i] + d[2 * i + 1];
-      store_n<V / 2>(row + a.a0 + (unit * V - a.a0) / 2, z);
+      store_n<V / 2>(p, lo);
+      if (scalar) store_n<V / 2>(p + V / 2, hi);
     }
   }
 };
 
 enum Table { kGain = 0, kOffset = 1, kNextGain = 2, kNextOffset = 3, kShare = 4, kTables = 5 };
 
-// Coordinate k's number of table t: s g_p, s b_p, g_n, b_n, its share.
-template <typename Args>
-__device__ __forceinline__ typename Args::A coefficient(const Args& a, int t, int k) {
-  using A = typename Args::A;
-  const A s = a.scale ? a.scale[k] : A(1);
-  switch (t) {
-    case kGain: return a.gain ? s * a.gain[k] : s;
-    case kOffset: return a.offset && k < a.a0 ? s * a.offset[k] : A(0);
-    case kNextGain: return a.next_gain ? a.next_gain[k] : A(0);
-    case kNextOffset: return a.next_offset && k < a.a0 ? a.next_offset[k] : A(0);
-    default: return share_of(a, k);
-  }
-}
-
-// The coefficients of a unit's numbers: from LDS (units), or from memory (copies: zero past a scalar).
+// The coefficients of every coordinate in LDS: s g_p, s b_p, g_n, b_n, its share of the pooled mean square.
 template <typename X, typename U, bool kCopies>
 struct RnTables {
   using A = typename RnAcc<X>::type;
@@ -233,19 +251,25 @@ struct RnTables {
   using Unit = RnUnit<X, U, kCopies>;
   static constexpr int V = Unit::V;
   A* lds;
-  __device__ __forceinline__ void fill(const Args& a, A* shared, int first, int last) {
+  __device__ __forceinline__ void fill(const Args& a, A* shared) {
     lds = shared;
-    if constexpr (!kCopies) {
-      for (int t = first; t < last; ++t)
-        for (int k = threadIdx.x; k < a.D; k += kRnThreads) lds[t * a.D + k] = coefficient(a, t, k);
-      __syncthreads();
+    for (int k = threadIdx.x; k < a.D; k += kRnThreads) {
+      const RnPlace at = place_of(a, k);
+      const A s = a.scaled ? a.scale[at.slot][at.copy] : A(1);
+      lds[kGain * a.D + k] = a.normalise ? s * a.gain[at.slot][at.copy] : s;
+      lds[kOffset * a.D + k] = a.offset && at.slot == 0 ? s * a.offset[k] : A(0);
+      lds[kNextGain * a.D + k] = a.next ? a.next_gain[at.slot][at.copy] : A(0);
+      lds[kNextOffset * a.D + k] = a.next_offset && at.slot == 0 ? a.next_offset[k] : A(0);
+      lds[kShare * a.D + k] = A(1) / (A(at.slot == 0 ? 1 : 2) * A(at.mult) * A(a.present));
     }
+    __syncthreads();
   }
+  // a unit's numbers (zero past a scalar copy)
   __device__ __forceinline__ void get(const Args& a, int t, int unit, A (&c)[V]) const {
     const int k = Unit::first(a, unit);
     if constexpr (kCopies) {
-      c[0] = coefficient(a, t, k);
-      c[1] = unit < a.a0 ? A(0) : coefficient(a, t, k + 1);
+      c[0] = lds[t * a.D + k];
+      c[1] = unit < a.a0 ? A(0) : lds[t * a.D + k + 1];
     } else {
       load_n<V>(lds + t * a.D + k, c);
     }
@@ -306,7 +330,7 @@ __global__ __launch_bounds__(kRnThreads) void residual_norm_forward_kernel(RnArg
   constexpr int V = Unit::V;
   extern __shared__ __align__(16) unsigned char rn_lds[];
   RnTables<X, U, kCopies> tables;
-  tables.fill(a, reinterpret_cast<A*>(rn_lds), 0, kTables);
+  tables.fill(a, reinterpret_cast<A*>(rn_lds));
   const int in_wave = threadIdx.x % kWave, lane = in_wave & (a.lanes - 1);
   const int per_wave = kWave >> a.shift;
   const int64_t step = (int64_t)gridDim.x * kRnWaves * per_wave;
@@ -328,7 +352,7 @@ __global__ __launch_bounds__(kRnThreads) void residual_norm_forward_kernel(RnArg
       }
     }
     A mean = A(0), inv = A(1);
-    if (a.gain) row_stats<X, U, kCopies, NS>(a, tables, lane, u, a.eps, mean, inv);
+    if (a.normalise) row_stats<X, U, kCopies, NS>(a, tables, lane, u, a.eps, mean, inv);
 #pragma unroll
     for (int j = 0; j < NS; ++j) {
       const int unit = lane + j * a.lanes;
@@ -347,7 +371,7 @@ __global__ __launch_bounds__(kRnThreads) void residual_norm_forward_kernel(RnArg
       }
     }
     A mean2 = A(0), inv2 = A(1);
-    if (a.next_gain) {
+    if (a.next) {
       row_stats<X, U, kCopies, NS>(a, tables, lane, x, a.next_eps, mean2, inv2);
 #pragma unroll
       for (int j = 0; j < NS; ++j) {
@@ -380,7 +404,7 @@ __global__ __launch_bounds__(kRnThreads) void residual_norm_backward_kernel(RnAr
   constexpr int V = Unit::V;
   extern __shared__ __align__(16) unsigned char rn_lds[];
   RnTables<X, U, kCopies> tables;
-  tables.fill(a, reinterpret_cast<A*>(rn_lds), 0, kTables);
+  tables.fill(a, reinterpret_cast<A*>(rn_lds));
   const int in_wave = threadIdx.x % kWave, lane = in_wave & (a.lanes - 1);
   const int per_wave = kWave >> a.shift;
   const int64_t step = (int64_t)gridDim.x * kRnWaves * per_wave;
@@ -487,7 +511,7 @@ __global__ __launch_bounds__(kRnThreads) void residual_norm_backward_kernel(RnAr
         if (a.z && live) Unit::store_gates(a, a.dz + r * a.copies, unit, d);
       }
     }
-    if (a.gain) {
+    if (a.normalise) {
       p1 = row_sum(p1, a.lanes);
       m1 = row_sum(m1, a.lanes) * by_scalars;
     }
@@ -495,7 +519,7 @@ __global__ __launch_bounds__(kRnThreads) void residual_norm_backward_kernel(RnAr
     for (int j = 0; j < NS; ++j) {
       const int unit = lane + j * a.lanes;
       if (unit < a.units) {
-        if (a.gain) {
+        if (a.normalise) {
           A w[V];
           tables.get(a, kShare, unit, w);
 #pragma unroll
@@ -539,64 +563,69 @@ __global__ __launch_bounds__(kRnThreads) void residual_norm_backward_kernel(RnAr
   }
 }
 
-// The parameters' gradients from the workgroups' sums: kCols coordinates a workgroup, kRnThreads / kCols threads a
-// coordinate, each over every kRnThreads / kCols-th row in order, then in order over the threads.
-constexpr int kRnCols = 8;
+// The parameters' gradients from the workgroups' sums: kRnCols copies a workgroup, kParts threads a copy, each over
+// every kParts-th row in order, then in order over the threads.
+constexpr int kRnCols = 4;
 template <typename X, typename U, bool kCopies>
 __global__ __launch_bounds__(kRnThreads) void residual_norm_reduce_kernel(RnArgs<X, U> a, int64_t blocks) {
   using A = typename RnAcc<X>::type;
-  using Unit = RnUnit<X, U, kCopies>;
-  constexpr int V = Unit::V, kParts = kRnThreads / kRnCols;
+  constexpr int V = RnUnit<X, U, kCopies>::V, kParts = kRnThreads / kRnCols;
   __shared__ A part[4][kParts][kRnCols];
-  const int c = threadIdx.x % kRnCols, from = threadIdx.x / kRnCols;
-  const int k = blockIdx.x * kRnCols + c, width = a.units * V;
-  const bool live = k < a.D;
-  int at = k;  // where the sums hold coordinate k
-  if constexpr (kCopies) at = k < a.a0 ? 2 * k : k + a.a0;
+  const int col = threadIdx.x % kRnCols, from = threadIdx.x / kRnCols;
+  const int c = blockIdx.x * kRnCols + col, width = a.units * V;
+  const bool live = c < a.copies, scalar = c < a.a0;
+  // where the sums hold the copy's first number
+  const int at = kCopies ? 2 * c : (scalar ? c : 2 * c - a.a0);
   A s[4] = {A(0), A(0), A(0), A(0)};
   if (live) {
+#pragma unroll 4
     for (int64_t b = from; b < blocks; b += kParts)
 #pragma unroll
-      for (int t = 0; t < 4; ++t) s[t] += a.partial[(b * 4 + t) * width + at];
+      for (int t = 0; t < 4; ++t) {
+        const A* row = a.partial + (b * 4 + t) * width + at;
+        s[t] += scalar ? row[0] : row[0] + row[1];
+      }
   }
 #pragma unroll
-  for (int t = 0; t < 4; ++t) part[t][from][c] = s[t];
+  for (int t = 0; t < 4; ++t) part[t][from][col] = s[t];
   __syncthreads();
   if (from != 0 || !live) return;
 #pragma unroll
   for (int t = 0; t < 4; ++t) {
     s[t] = A(0);
-    for (int w = 0; w < kParts; ++w) s[t] += part[t][w][c];
+#pragma unroll 8
+    for (int w = 0; w < kParts; ++w) s[t] += part[t][w][col];
   }
-  const bool scalar = k < a.a0;
-  const A scale = a.scale ? a.scale[k] : A(1), gain = a.gain ? a.gain[k] : A(1);
-  const A offset = a.offset && scalar ? a.offset[k] : A(0);
+  const RnPlace p = place_of(a, scalar ? c : 2 * c - a.a0);
+  const A scale = a.scaled ? a.scale[p.slot][p.copy] : A(1), gain = a.normalise ? a.gain[p.slot][p.copy] : A(1);
+  const A offset = a.offset && scalar ? a.offset[c] : A(0);
+  const int C = a.copies;
   A* out = a.dparams;
-  out[k] = scale * s[0];
-  if (scalar) out[a.D + k] = scale * s[1];
-  out[a.D + a.a0 + k] = gain * s[0] + offset * s[1];
-  out[2 * a.D + a.a0 + k] = s[2];
-  if (scalar) out[3 * a.D + a.a0 + k] = s[3];
+  out[c] = scale * s[0];
+  if (scalar) out[C + c] = scale * s[1];
+  out[C + a.a0 + c] = gain * s[0] + offset * s[1];
+  out[2 * C + a.a0 + c] = s[2];
+  if (scalar) out[3 * C + a.a0 + c] = s[3];
 }
 
 // ------------------------------------------------------------------ launch
 
-// Units a lane holds at most: the rows' numbers and the backward's sums are registers (20 numbers of float rows, 24 of
-// bfloat16 ones, 16 of double ones; a wide row's copies, 32).
+// Units a lane holds at most: the rows' numbers and the backward's sums are registers (20 numbers of float and
+// bfloat16 rows, 16 of double ones; a wide row's copies, 32).
 template <typename X, bool kCopies>
-constexpr int kMaxUnits = kCopies ? 16 : (sizeof(X) == 4 ? 5 : (sizeof(X) == 2 ? 3 : 8));
+constexpr int kMaxUnits = kCopies ? 16 : (sizeof(X) == 8 ? 8 : 5);
 
 template <typename X, typename U, bool kCopies, int NS>
 int launch_rn(bool backward, const RnArgs<X, U>& a, hipStream_t stream, int64_t& blocks) {
   using A = typename RnAcc<X>::type;
   const int64_t rows_per_block = (int64_t)kRnWaves * (kWave >> a.shift);
   const int width = a.units * RnUnit<X, U, kCopies>::V;
-  const size_t lds = sizeof(A) * std::max<size_t>(kCopies ? 0 : (size_t)kTables * a.D, backward ? width : 0);
+  const size_t lds = sizeof(A) * std::max<size_t>((size_t)kTables * a.D, backward ? width : 0);
   const void* kernel = backward ? reinterpret_cast<const void*>(&residual_norm_backward_kernel<X, U, kCopies, NS>)
                                 : reinterpret_cast<const void*>(&residual_norm_forward_kernel<X, U, kCopies, NS>);
   const int64_t want = (a.n_rows + rows_per_block - 1) / rows_per_block;
   const int64_t slots = resident_blocks(kernel, kRnThreads, lds);
-  // the backward's rows of sums are one a workgroup: its persistent workgroups are what the caller's array was sized for
+  // the backward writes a row of sums a workgroup: as many as the caller's array was sized for
   if (backward)
     blocks = std::min<int64_t>(want, blocks);
   else
@@ -632,7 +661,7 @@ int dispatch_rn(bool backward, RnArgs<X, U>& a, hipStream_t stream, int64_t& blo
   GM_RN_CASE(1)
   GM_RN_CASE(2)
   GM_RN_CASE(3)
-  if constexpr (!kCopies && sizeof(X) == 4) {
+  if constexpr (!kCopies && sizeof(X) != 8) {
     GM_RN_CASE(4)
     GM_RN_CASE(5)
   } else {
@@ -675,15 +704,41 @@ int fill_rn(RnArgs<X, U>& a, int64_t n_rows, int64_t D, int64_t a0, int64_t nf, 
   return GM_OK;
 }
 
-// Whole units: every frequency's numbers fill 16-byte pieces of the rows' type, the gates' rows half of them, and the
-// pointers are aligned to them (a wider branch's to 16 bytes as well).
+// Whole units: frequency 0's and the row's numbers are units, the gates' rows halves of them, and the pointers are
+// aligned to them.
 template <typename X, typename U>
 bool whole_units(const RnArgs<X, U>& a) {
-  constexpr int V = 16 / (int)sizeof(X);
+  constexpr int V = RnUnit<X, U, false>::V;
+  constexpr size_t ax = V * sizeof(X), au = std::min<size_t>(16, V * sizeof(U));
   if (a.D % V != 0 || a.a0 % V != 0) return false;
-  if (a.z && (a.copies % std::max(V / 2, 1) != 0 || !aligned(a.z, 16) || !aligned(a.dz, 16))) return false;
-  return aligned(a.x, 16) && aligned(a.u, 16) && aligned(a.y, 16) && aligned(a.normed, 16) && aligned(a.dy, 16) &&
-         aligned(a.dn, 16) && aligned(a.dx, 16) && aligned(a.du, 16);
+  if (a.z && (a.copies % (V / 2) != 0 || !aligned(a.z, ax) || !aligned(a.dz, ax))) return false;
+  return aligned(a.x, ax) && aligned(a.u, au) && aligned(a.y, ax) && aligned(a.normed, ax) && aligned(a.dy, ax) &&
+         aligned(a.dn, ax) && aligned(a.dx, ax) && aligned(a.du, au);
+}
+
+// The parameters' pointers (HOST array, 3 (nf + 1) + 2): the gains by frequency (slot 0 frequency 0), the scales, the
+// next gains, then the offsets.  A whole group is given or missing; a slot without copies is not read.
+template <typename X, typename U>
+int take_parameters(RnArgs<X, U>& a, const void* const* params) {
+  using A = typename RnAcc<X>::type;
+  GM_REQUIRE(params, "the parameters' pointers (a host array) are required");
+  const int slots = a.nf + 1;
+  for (int g = 0; g < 3; ++g) {
+    const A** to = g == 0 ? a.gain : (g == 1 ? a.scale : a.next_gain);
+    int given = 0, wanted = 0;
+    for (int f = 0; f < slots; ++f) {
+      to[f] = static_cast<const A*>(params[g * slots + f]);
+      if (f > 0 || a.a0 > 0) {
+        ++wanted;
+        given += to[f] != nullptr;
+      }
+    }
+    GM_REQUIRE(given == 0 || given == wanted, "a group of parameters needs a vector of every frequency");
+    (g == 0 ? a.normalise : (g == 1 ? a.scaled : a.next)) = given > 0;
+  }
+  a.offset = a.normalise ? static_cast<const A*>(params[3 * slots]) : nullptr;
+  a.next_offset = a.next ? static_cast<const A*>(params[3 * slots + 1]) : nullptr;
+  return GM_OK;
 }
 
 constexpr int64_t kRnMaxBlocks = 512;  // two workgroups a CU: what the backward's registers leave room for
@@ -694,26 +749,19 @@ int64_t rn_blocks(int64_t n_rows) {
 }
 
 template <typename X, typename U>
-int residual_forward(const X* x, const U* u, const X* z, const typename RnAcc<X>::type* gain,
-                     const typename RnAcc<X>::type* offset, const typename RnAcc<X>::type* scale,
-                     const typename RnAcc<X>::type* next_gain, const typename RnAcc<X>::type* next_offset,
-                     int64_t n_rows, int64_t D, int64_t a0, int64_t nf, const int64_t* offsets, const int64_t* mults,
-                     double factor, double eps, double next_eps, X* y, X* normed, typename RnAcc<X>::type* stats,
-                     void* stream) {
+int residual_forward(const X* x, const U* u, const X* z, const void* const* params, int64_t n_rows, int64_t D,
+                     int64_t a0, int64_t nf, const int64_t* offsets, const int64_t* mults, double factor, double eps,
+                     double next_eps, X* y, X* normed, typename RnAcc<X>::type* stats, void* stream) {
   RnArgs<X, U> a{};
-  const int rc = fill_rn(a, n_rows, D, a0, nf, offsets, mults, factor, eps, next_eps);
+  int rc = fill_rn(a, n_rows, D, a0, nf, offsets, mults, factor, eps, next_eps);
+  if (rc == GM_OK) rc = take_parameters(a, params);
   if (rc != GM_OK) return rc;
   if (n_rows == 0) return GM_OK;
   GM_REQUIRE(x && u && y, "x, u and y must be device pointers");
-  GM_REQUIRE(!next_gain || normed, "normed must be a device pointer where there is a next norm");
+  GM_REQUIRE(!a.next || normed, "normed must be a device pointer where there is a next norm");
   a.x = x;
   a.u = u;
   a.z = z;
-  a.gain = gain;
-  a.offset = gain ? offset : nullptr;
-  a.scale = scale;
-  a.next_gain = next_gain;
-  a.next_offset = next_gain ? next_offset : nullptr;
   a.y = y;
   a.normed = normed;
   a.stats = stats;
@@ -723,30 +771,25 @@ int residual_forward(const X* x, const U* u, const X* z, const typename RnAcc<X>
 }
 
 template <typename X, typename U>
-int residual_backward(const X* dy, const X* dn, const X* x, const U* u, const X* z,
-                      const typename RnAcc<X>::type* gain, const typename RnAcc<X>::type* offset,
-                      const typename RnAcc<X>::type* scale, const typename RnAcc<X>::type* next_gain,
+int residual_backward(const X* dy, const X* dn, const X* x, const U* u, const X* z, const void* const* params,
                       const typename RnAcc<X>::type* stats, int64_t n_rows, int64_t D, int64_t a0, int64_t nf,
                       const int64_t* offsets, const int64_t* mults, double factor, X* dx, U* du, X* dz,
                       typename RnAcc<X>::type* partial, typename RnAcc<X>::type* dparams, void* stream) {
   RnArgs<X, U> a{};
-  const int rc = fill_rn(a, n_rows, D, a0, nf, offsets, mults, factor, 1.0, 1.0);
+  int rc = fill_rn(a, n_rows, D, a0, nf, offsets, mults, factor, 1.0, 1.0);
+  if (rc == GM_OK) rc = take_parameters(a, params);
   if (rc != GM_OK) return rc;
   GM_REQUIRE(partial && dparams, "partial and dparams must be device pointers");
   if (n_rows > 0) {
     GM_REQUIRE(x && u && stats && dx && du, "x, u, stats, dx and du must be device pointers");
     GM_REQUIRE(!z || dz, "dz must be a device pointer where there are gates");
-    GM_REQUIRE(!dn || next_gain, "a gradient of the next norm needs its gains");
+    GM_REQUIRE(!dn || a.next, "a gradient of the next norm needs its gains");
   }
   a.dy = dy;
   a.dn = dn;
   a.x = x;
   a.u = u;
   a.z = z;
-  a.gain = gain;
-  a.offset = gain ? offset : nullptr;
-  a.scale = scale;
-  a.next_gain = next_gain;
   a.stats = const_cast<typename RnAcc<X>::type*>(stats);  // read only here
   a.dx = dx;
   a.du = du;
@@ -757,10 +800,11 @@ int residual_backward(const X* dy, const X* dn, const X* x, const U* u, const X*
   const bool units = whole_units(a);
   const hipStream_t s = (hipStream_t)stream;
   if (n_rows > 0) {
-    const int status = units ? dispatch_rn<X, U, false>(true, a, s, blocks) : dispatch_rn<X, U, true>(true, a, s, blocks);
+    const int status =
+        units ? dispatch_rn<X, U, false>(true, a, s, blocks) : dispatch_rn<X, U, true>(true, a, s, blocks);
     if (status != GM_OK) return status;
   }
-  const dim3 grid((unsigned)((D + kRnCols - 1) / kRnCols));
+  const dim3 grid((unsigned)((a.copies + kRnCols - 1) / kRnCols));
   if (units)
     hipLaunchKernelGGL((residual_norm_reduce_kernel<X, U, false>), grid, dim3(kRnThreads), 0, s, a, blocks);
   else
@@ -774,25 +818,26 @@ int residual_backward(const X* dy, const X* dn, const X* x, const U* u, const X*
 extern "C" int64_t gm_residual_norm_partial_rows(int64_t n_rows) { return n_rows > 0 ? 4 * gm::rn_blocks(n_rows) : 4; }
 
 // X, U: the rows' and the branch's element types in the C signature, TX, TU the kernels'; A the parameters'.
-#define GM_RESIDUAL_ENTRY(SFX, X, U, TX, TU, A)                                                                        \
-  extern "C" int gm_residual_norm_forward_##SFX(                                                                       \
-      const X* x, const U* u, const X* z, const A* gain, const A* offset, const A* scale, const A* next_gain,          \
-      const A* next_offset, int64_t n_rows, int64_t D, int64_t a0, int64_t nf, const int64_t* offsets,                 \
-      const int64_t* mults, double factor, double eps, double next_eps, X* y, X* normed, A* stats, void* stream) {     \
-    return gm::residual_forward<TX, TU>(reinterpret_cast<const TX*>(x), reinterpret_cast<const TU*>(u),                \
-                                        reinterpret_cast<const TX*>(z), gain, offset, scale, next_gain, next_offset,   \
-                                        n_rows, D, a0, nf, offsets, mults, factor, eps, next_eps,                      \
-                                        reinterpret_cast<TX*>(y), reinterpret_cast<TX*>(normed), stats, stream);       \
-  }                                                                                                                    \
-  extern "C" int gm_residual_norm_backward_##SFX(                                                                      \
-      const X* dy, const X* dn, const X* x, const U* u, const X* z, const A* gain, const A* offset, const A* scale,    \
-      const A* next_gain, const A* stats, int64_t n_rows, int64_t D, int64_t a0, int64_t nf, const int64_t* offsets,   \
-      const int64_t* mults, double factor, X* dx, U* du, X* dz, A* partial, A* dparams, void* stream) {                \
-    return gm::residual_backward<TX, TU>(                                                                              \
-        reinterpret_cast<const TX*>(dy), reinterpret_cast<const TX*>(dn), reinterpret_cast<const TX*>(x),              \
-        reinterpret_cast<const TU*>(u), reinterpret_cast<const TX*>(z), gain, offset, scale, next_gain, stats, n_rows, \
-        D, a0, nf, offsets, mults, factor, reinterpret_cast<TX*>(dx), reinterpret_cast<TU*>(du),                       \
-        reinterpret_cast<TX*>(dz), partial, dparams, stream);                                                          \
+#define GM_RESIDUAL_ENTRY(SFX, X, U, TX, TU, A)                                                                       \
+  extern "C" int gm_residual_norm_forward_##SFX(const X* x, const U* u, const X* z, const void* const* params,        \
+                                                int64_t n_rows, int64_t D, int64_t a0, int64_t nf,                    \
+                                                const int64_t* offsets, const int64_t* mults, double factor,          \
+                                                double eps, double next_eps, X* y, X* normed, A* stats,               \
+                                                void* stream) {                                                       \
+    return gm::residual_forward<TX, TU>(reinterpret_cast<const TX*>(x), reinterpret_cast<const TU*>(u),               \
+                                        reinterpret_cast<const TX*>(z), params, n_rows, D, a0, nf, offsets, mults,    \
+                                        factor, eps, next_eps, reinterpret_cast<TX*>(y),                              \
+                                        reinterpret_cast<TX*>(normed), stats, stream);                                \
+  }                                                                                                                   \
+  extern "C" int gm_residual_norm_backward_##SFX(                                                                     \
+      const X* dy, const X* dn, const X* x, const U* u, const X* z, const void* const* params, const A* stats,        \
+      int64_t n_rows, int64_t D, int64_t a0, int64_t nf, const int64_t* offsets, const int64_t* mults, double factor, \
+      X* dx, U* du, X* dz, A* partial, A* dparams, void* stream) {                                                    \
+    return gm::residual_backward<TX, TU>(reinterpret_cast<const TX*>(dy), reinterpret_cast<const TX*>(dn),            \
+                                         reinterpret_cast<const TX*>(x), reinterpret_cast<const TU*>(u),              \
+                                         reinterpret_cast<const TX*>(z), params, stats, n_rows, D, a0, nf, offsets,   \
+                                         mults, factor, reinterpret_cast<TX*>(dx), reinterpret_cast<TU*>(du),         \
+                                         reinterpret_cast<TX*>(dz), partial, dparams, stream);                        \
   }
 
 GM_RESIDUAL_ENTRY(f32, float, float, float, float, float)

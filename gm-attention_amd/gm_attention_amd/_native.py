@@ -112,9 +112,9 @@ SIGNATURES_F32 = {
     **{f"gm_gate_backward_{sfx}": (ctypes.c_int, [_P] * 3 + [_I] * 4 + [_P, _P, _I] + [_P] * 3)
        for sfx in ("f32", "f64", "bf16")},
     "gm_residual_norm_partial_rows": (ctypes.c_int64, [_I]),
-    **{f"gm_residual_norm_forward_{sfx}": (ctypes.c_int, [_P] * 8 + [_I] * 4 + [_P, _P, _D, _D, _D] + [_P] * 4)
+    **{f"gm_residual_norm_forward_{sfx}": (ctypes.c_int, [_P] * 4 + [_I] * 4 + [_P, _P, _D, _D, _D] + [_P] * 4)
        for sfx in ("f32", "f64", "bf16", "bf16_f32")},
-    **{f"gm_residual_norm_backward_{sfx}": (ctypes.c_int, [_P] * 10 + [_I] * 4 + [_P, _P, _D] + [_P] * 6)
+    **{f"gm_residual_norm_backward_{sfx}": (ctypes.c_int, [_P] * 7 + [_I] * 4 + [_P, _P, _D] + [_P] * 6)
        for sfx in ("f32", "f64", "bf16", "bf16_f32")},
 }
 
@@ -1553,51 +1553,71 @@ def gate_backward(gy: Tensor, h: Tensor, pre: Tensor, layout: PointwiseLayout,
     return dh, dpre
 
 
-def _residual_check(x: Tensor, u: Tensor, z: Tensor | None, layout: PointwiseLayout,
-                    vectors: tuple[tuple[str, Tensor | None, int], ...]) -> str:
-    """The residual sum's suffix, its rows and per-coordinate vectors checked."""
+class ResidualParameters:
+    """The residual sum's parameter vectors by frequency, ``gains``, ``scales`` and
+    ``next_gains`` (None where left out), and the two offsets: checked, with the
+    host array of their pointers that the entry points take."""
+
+    def __init__(self, layout: PointwiseLayout, x: Tensor, gains: list[Tensor] | None, offset: Tensor | None,
+                 scales: list[Tensor] | None, next_gains: list[Tensor] | None, next_offset: Tensor | None):
+        self.next = next_gains is not None
+        pd, device = param_dtype(x.dtype), x.device
+        mults = ([layout.a0] if layout.a0 else []) + list(layout.mults[: layout.nf])
+        pointers: list[int | None] = []
+        for name, group in (("gains", gains), ("scales", scales), ("next_gains", next_gains)):
+            if group is None:
+                pointers += [None] * (layout.nf + 1)
+                continue
+            _check(len(group) == len(mults), f"{name} must hold a vector of every frequency")
+            for t, m in zip(group, mults):
+                _check(t.dtype == pd and t.device == device and t.ndim == 1 and t.shape[0] == m and t.is_contiguous(),
+                       f"{name} must be contiguous {pd} vectors of {mults} on the rows' device")
+            pointers += ([] if layout.a0 else [None]) + [t.data_ptr() for t in group]
+        for name, t in (("offset", offset), ("next_offset", next_offset)):
+            _check(t is None or (t.dtype == pd and t.device == device and tuple(t.shape) == (layout.a0,)
+                                 and t.is_contiguous()), f"{name} must be a contiguous ({layout.a0},) {pd} vector")
+            pointers.append(_ptr(t))
+        self.array = (ctypes.c_void_p * len(pointers))(*pointers)
+
+    def arg(self) -> Any:
+        return ctypes.cast(self.array, _P)
+
+
+def _residual_check(x: Tensor, u: Tensor, z: Tensor | None, layout: PointwiseLayout) -> str:
+    """The residual sum's suffix, its rows checked."""
     sfx = _pw_check(x, layout)
-    _require_device(x, u, *(t for t in (z, *(v for _, v, _ in vectors)) if t is not None))
+    _require_device(x, u, *(() if z is None else (z,)))
     wide = x.dtype == torch.bfloat16 and u.dtype == torch.float32
     _check(u.dtype == x.dtype or wide, f"u must be {x.dtype} (or float32 for bfloat16 rows), got {u.dtype}")
     _check(u.shape == x.shape, "u must be shaped as x")
     copies = layout.a0 + layout.G
     _check(z is None or (z.dtype == x.dtype and tuple(z.shape) == (x.shape[0], copies)),
            f"z must be (n_nodes, {copies}) in x's dtype")
-    pd = param_dtype(x.dtype)
-    for name, t, n in vectors:
-        _check(t is None or (t.dtype == pd and tuple(t.shape) == (n,)), f"{name} must be ({n},) {pd}")
     return sfx + ("_f32" if wide else "")
 
 
-def residual_norm_forward(x: Tensor, u: Tensor, z: Tensor | None, gain: Tensor | None, offset: Tensor | None,
-                          scale: Tensor | None, next_gain: Tensor | None, next_offset: Tensor | None,
+def residual_norm_forward(x: Tensor, u: Tensor, z: Tensor | None, params: ResidualParameters,
                           layout: PointwiseLayout, factor: float, eps: float, next_eps: float,
                           train: bool) -> tuple[Tensor, Tensor | None, Tensor | None]:
-    """``(y, normed, stats)``: the residual sum and the norm behind it (None without ``next_gain``);
+    """``(y, normed, stats)``: the residual sum and the norm behind it (None without next gains);
     ``stats (n_nodes, 4)``, what the backward reads of both norms, under ``train``."""
-    D, a0 = layout.D, layout.a0
-    sfx = _residual_check(x, u, z, layout, (("gain", gain, D), ("offset", offset, a0), ("scale", scale, D),
-                                            ("next_gain", next_gain, D), ("next_offset", next_offset, a0)))
+    sfx = _residual_check(x, u, z, layout)
     y = torch.empty_like(x)
-    normed = None if next_gain is None else torch.empty_like(x)
+    normed = torch.empty_like(x) if params.next else None
     stats = torch.empty(x.shape[0], 4, dtype=param_dtype(x.dtype), device=x.device) if train else None
     with torch.cuda.device(x.device):
-        _call(f"gm_residual_norm_forward_{sfx}", _ptr(x), _ptr(u), _ptr(z), _ptr(gain), _ptr(offset), _ptr(scale),
-              _ptr(next_gain), _ptr(next_offset), x.shape[0], *layout.args(), float(factor), float(eps),
-              float(next_eps), _ptr(y), _ptr(normed), _ptr(stats), _stream(x.device))
+        _call(f"gm_residual_norm_forward_{sfx}", _ptr(x), _ptr(u), _ptr(z), params.arg(), x.shape[0], *layout.args(),
+              float(factor), float(eps), float(next_eps), _ptr(y), _ptr(normed), _ptr(stats), _stream(x.device))
     return y, normed, stats
 
 
 def residual_norm_backward(dy: Tensor | None, dn: Tensor | None, x: Tensor, u: Tensor, z: Tensor | None,
-                           gain: Tensor | None, offset: Tensor | None, scale: Tensor | None,
-                           next_gain: Tensor | None, stats: Tensor, layout: PointwiseLayout,
+                           params: ResidualParameters, stats: Tensor, layout: PointwiseLayout,
                            factor: float) -> tuple[Tensor, Tensor, Tensor | None, Tensor]:
-    """``(dx, du, dz, dparams)`` with ``dparams = (dgain (D), doffset (a0), dscale (D),
-    dnext_gain (D), dnext_offset (a0))`` summed over the nodes in a fixed order."""
-    D, a0, n = layout.D, layout.a0, x.shape[0]
-    sfx = _residual_check(x, u, z, layout, (("gain", gain, D), ("offset", offset, a0), ("scale", scale, D),
-                                            ("next_gain", next_gain, D)))
+    """``(dx, du, dz, dparams)`` with ``dparams = (dgain (copies), doffset (a0), dscale (copies),
+    dnext_gain (copies), dnext_offset (a0))`` summed over the nodes in a fixed order."""
+    n, copies = x.shape[0], layout.a0 + layout.G
+    sfx = _residual_check(x, u, z, layout)
     pd = param_dtype(x.dtype)
     for name, t in (("dy", dy), ("dn", dn)):
         _check(t is None or (t.dtype == x.dtype and t.shape == x.shape and t.is_contiguous()
@@ -1605,10 +1625,11 @@ def residual_norm_backward(dy: Tensor | None, dn: Tensor | None, x: Tensor, u: T
     _check(stats.dtype == pd and tuple(stats.shape) == (n, 4) and stats.is_contiguous(), f"stats must be ({n}, 4) {pd}")
     dx, du = torch.empty_like(x), torch.empty_like(u)
     dz = None if z is None else torch.empty_like(z)
-    partial = torch.empty(int(library().gm_residual_norm_partial_rows(n)), D + a0, dtype=pd, device=x.device)
-    dparams = torch.empty(3 * D + 2 * a0, dtype=pd, device=x.device)
+    partial = torch.empty(int(library().gm_residual_norm_partial_rows(n)), layout.D + layout.a0, dtype=pd,
+                          device=x.device)
+    dparams = torch.empty(3 * copies + 2 * layout.a0, dtype=pd, device=x.device)
     with torch.cuda.device(x.device):
-        _call(f"gm_residual_norm_backward_{sfx}", _ptr(dy), _ptr(dn), _ptr(x), _ptr(u), _ptr(z), _ptr(gain),
-              _ptr(offset), _ptr(scale), _ptr(next_gain), _ptr(stats), n, *layout.args(), float(factor), _ptr(dx),
-              _ptr(du), _ptr(dz), _ptr(partial), _ptr(dparams), _stream(x.device))
+        _call(f"gm_residual_norm_backward_{sfx}", _ptr(dy), _ptr(dn), _ptr(x), _ptr(u), _ptr(z), params.arg(),
+              _ptr(stats), n, *layout.args(), float(factor), _ptr(dx), _ptr(du), _ptr(dz), _ptr(partial),
+              _ptr(dparams), _stream(x.device))
     return dx, du, dz, dparams

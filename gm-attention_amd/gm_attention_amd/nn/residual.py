@@ -29,7 +29,6 @@ import torch
 from torch import Tensor, nn
 
 from gm_attention_amd import _native
-from gm_attention_amd.nn.assembly import assembled
 from gm_attention_amd.nn.linear import FlatLinear
 from gm_attention_amd.nn.normalization import MAX_WIDTH, SO2LayerNorm
 from gm_attention_amd.representations.field_type import SO2FeatureField, SO2FieldType
@@ -38,39 +37,54 @@ GateKind = Literal["sigmoid", "double_sigmoid"]
 _GATES = {"sigmoid": 1.0, "double_sigmoid": 2.0}
 
 
+#: Groups of parameters by their place in the op's arguments: the branch's gains
+#: and offset, the scales, the next norm's gains and offset.
+_OFFSETS = (1, 4)
+
+
 class ResidualNormOp(torch.autograd.Function):
-    """``(x', h)`` (``x'`` alone without a next norm) from the rows, the branch,
-    the gates' pre-activations and the parameters per flat coordinate."""
+    """``(x', h)`` (``x'`` alone without a next norm) from the rows, the branch, the
+    gates' pre-activations and the parameters, a vector a frequency; ``counts``
+    how many of ``params`` each group has, zero for a group left out."""
 
     @staticmethod
-    def forward(ctx, x: Tensor, u: Tensor, z: Tensor | None, gain: Tensor | None, offset: Tensor | None,
-                scale: Tensor | None, next_gain: Tensor | None, next_offset: Tensor | None, layout, factor: float,
-                eps: float, next_eps: float):
+    def forward(ctx, x: Tensor, u: Tensor, z: Tensor | None, layout, factor: float, eps: float, next_eps: float,
+                counts: tuple[int, ...], *params: Tensor):
         ctx.set_materialize_grads(False)
         train = any(ctx.needs_input_grad)
         with torch.profiler.record_function("gm::pointwise/residual_norm"):
-            y, normed, stats = _native.residual_norm_forward(x, u, z, gain, offset, scale, next_gain, next_offset,
-                                                             layout, factor, eps, next_eps, train)
+            y, normed, stats = _native.residual_norm_forward(x, u, z, _grouped(layout, x, counts, params), layout,
+                                                             factor, eps, next_eps, train)
         if train:
-            ctx.save_for_backward(x, u, z, gain, offset, scale, next_gain, stats)
-            ctx.layout, ctx.factor, ctx.next_offset = layout, factor, next_offset is not None
+            ctx.save_for_backward(x, u, z, stats, *params)
+            ctx.layout, ctx.factor, ctx.counts = layout, factor, counts
         return y if normed is None else (y, normed)
 
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, dy: Tensor | None, dn: Tensor | None = None):
-        x, u, z, gain, offset, scale, next_gain, stats = ctx.saved_tensors
+        x, u, z, stats, *params = ctx.saved_tensors
         if dy is None and dn is None:
-            return (None,) * 12
+            return (None,) * len(ctx.needs_input_grad)
+        layout, counts = ctx.layout, ctx.counts
         with torch.profiler.record_function("gm::pointwise/residual_norm_backward"):
             dx, du, dz, dparams = _native.residual_norm_backward(
-                None if dy is None else dy.contiguous(), None if dn is None else dn.contiguous(), x, u, z, gain,
-                offset, scale, next_gain, stats, ctx.layout, ctx.factor)
-        D, a0 = ctx.layout.D, ctx.layout.a0
-        dgain, doffset, dscale, dnext, dnext_offset = dparams.split([D, a0, D, D, a0])
-        return (dx, du, dz, None if gain is None else dgain, None if offset is None else doffset,
-                None if scale is None else dscale, None if next_gain is None else dnext,
-                dnext_offset if ctx.next_offset else None, None, None, None, None)
+                None if dy is None else dy.contiguous(), None if dn is None else dn.contiguous(), x, u, z,
+                _grouped(layout, x, counts, params), stats, layout, ctx.factor)
+        copies, sizes, held = layout.a0 + layout.G, [], []
+        mults = ([layout.a0] if layout.a0 else []) + list(layout.mults[: layout.nf])
+        for i, count in enumerate(counts):
+            split = [layout.a0] if i in _OFFSETS else (mults if count else [copies])
+            sizes += split
+            held += [count > 0] * len(split)
+        return (dx, du, dz, None, None, None, None, None,
+                *(g for g, h in zip(dparams.split(sizes), held, strict=True) if h))
+
+
+def _grouped(layout, x: Tensor, counts: tuple[int, ...], params) -> _native.ResidualParameters:
+    it = iter(params)
+    groups = [[next(it) for _ in range(count)] if count else None for count in counts]
+    return _native.ResidualParameters(layout, x, *(g[0] if i in _OFFSETS and g else g for i, g in enumerate(groups)))
 
 
 class SO2ResidualNorm(nn.Module):
@@ -139,28 +153,6 @@ class SO2ResidualNorm(nn.Module):
         scales = None if self.scale is None else [self.scale[str(f)] for f in frequencies]
         return [gains(self.post), offset(self.post), scales, gains(self.norm), offset(self.norm)]
 
-    def _forms(self, dtype: torch.dtype) -> list[Tensor | None]:
-        """The groups per flat coordinate (a copy's number for both of its
-        coordinates), the offsets per scalar."""
-        groups = self._groups()
-        params = [p for group in groups if group is not None for p in group]
-        if not params:
-            return [None] * len(groups)
-        frequencies = self.field_type.frequencies
-
-        def build(ps: list[Tensor]) -> list[Tensor]:
-            it, forms = iter(ps), []
-            for i, group in enumerate(groups):
-                if group is not None:
-                    mine = [next(it) for _ in group]
-                    forms.append(mine[0].clone() if i in (1, 4) else torch.cat(
-                        [p if f == 0 else p.repeat_interleave(2) for f, p in zip(frequencies, mine, strict=True)]))
-            return forms
-
-        name = "residual " + "".join("-" if group is None else "+" for group in groups)
-        forms = iter(assembled(self, name, params, build))
-        return [None if group is None else next(forms).to(dtype) for group in groups]
-
     def uses_hip(self, flat: Tensor) -> bool:
         return flat.device.type == "cuda" and flat.dtype in (torch.float32, torch.float64, torch.bfloat16) \
             and self.field_type.dimension <= MAX_WIDTH
@@ -184,12 +176,13 @@ class SO2ResidualNorm(nn.Module):
             return self._eager(rows, branch, pre)
         if branch.dtype != rows.dtype and not (rows.dtype == torch.bfloat16 and branch.dtype == torch.float32):
             branch = branch.to(rows.dtype)
-        gain, offset, scale, next_gain, next_offset = self._forms(_native.param_dtype(rows.dtype))
+        pd, groups = _native.param_dtype(rows.dtype), self._groups()
         out = ResidualNormOp.apply(rows.contiguous(), branch.contiguous(),
-                                   None if pre is None else pre.to(rows.dtype).contiguous(), gain, offset, scale,
-                                   next_gain, next_offset, self._layout(), _GATES.get(self.gate, 1.0),
-                                   self.post.eps if self.post is not None else 1.0,
-                                   self.norm.eps if self.norm is not None else 1.0)
+                                   None if pre is None else pre.to(rows.dtype).contiguous(), self._layout(),
+                                   _GATES.get(self.gate, 1.0), self.post.eps if self.post is not None else 1.0,
+                                   self.norm.eps if self.norm is not None else 1.0,
+                                   tuple(0 if group is None else len(group) for group in groups),
+                                   *(p.to(pd).contiguous() for group in groups if group is not None for p in group))
         return out if self.norm is not None else (out, None)
 
     def forward(self, x: SO2FeatureField, branch: SO2FeatureField,

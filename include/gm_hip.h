@@ -336,61 +336,58 @@ int gm_gate_backward_bf16(const uint16_t* gy, const uint16_t* h, const uint16_t*
  *   normed = next_gain * norm(y) + next_offset [frequency 0]
  * with norm the normalization above without gains (its eps: eps, next_eps),
  * act(z) = factor sigmoid(z) with one gate a copy (z (n_rows, copies): the
- * scalars, then every frequency's copies), and gain, scale, next_gain (D) per
- * coordinate, offset, next_offset (a0).  NULL gain: the branch is not
- * normalised (offset is then not read); NULL z: no gates; NULL scale: one;
- * NULL next_gain: nothing is normalised behind the sum, which is normalised
- * before it is rounded to the rows' type.  stats (n_rows, 4), or NULL where no
- * backward follows: the branch's mean and 1 / d, the sum's.  Suffix _bf16_f32:
- * bfloat16 rows, the branch (and its gradient) in float.
+ * scalars, then every frequency's copies), gain, scale and next_gain one number
+ * a copy, offset and next_offset (a0).  `params` is a HOST array of
+ * 3 (nf + 1) + 2 device pointers to the parameters' vectors by frequency (slot 0
+ * frequency 0, not read where a0 = 0): the gains, the scales, the next gains,
+ * then offset and next_offset.  A group of NULLs is left out: without gains the
+ * branch is not normalised, without next gains nothing is normalised behind the
+ * sum, without scales they are one; NULL z: no gates; NULL offsets: zero.  The
+ * sum is normalised before it is rounded to the rows' type.  stats (n_rows, 4),
+ * or NULL where no backward follows: the branch's mean and 1 / d, the sum's.
+ * Suffix _bf16_f32: bfloat16 rows, the branch (and its gradient) in float.
  *
  * Backward from dy (of y) and dn (of normed), either NULL for zero: dx, du, dz
- * (where z is given) and dparams (3 D + 2 a0) = (dgain (D), doffset (a0),
- * dscale (D), dnext_gain (D), dnext_offset (a0)), summed over the rows in a
- * fixed order through `partial` (gm_residual_norm_partial_rows(n_rows) rows of
- * D + a0).  No reference counterpart. */
+ * (where z is given) and dparams (3 copies + 2 a0) = (dgain (copies),
+ * doffset (a0), dscale (copies), dnext_gain (copies), dnext_offset (a0)), summed
+ * over the rows in a fixed order through `partial`
+ * (gm_residual_norm_partial_rows(n_rows) rows of D + a0).  No reference
+ * counterpart. */
 int64_t gm_residual_norm_partial_rows(int64_t n_rows);
-int gm_residual_norm_forward_f32(const float* x, const float* u, const float* z, const float* gain, const float*
-                                 offset, const float* scale, const float* next_gain, const float* next_offset, int64_t
+int gm_residual_norm_forward_f32(const float* x, const float* u, const float* z, const void* const* params, int64_t
                                  n_rows, int64_t D, int64_t a0, int64_t nf, const int64_t* offsets, const int64_t*
                                  mults, double factor, double eps, double next_eps, float* y, float* normed, float*
                                  stats, void* stream);
-int gm_residual_norm_forward_f64(const double* x, const double* u, const double* z, const double* gain, const double*
-                                 offset, const double* scale, const double* next_gain, const double* next_offset,
-                                 int64_t n_rows, int64_t D, int64_t a0, int64_t nf, const int64_t* offsets, const
-                                 int64_t* mults, double factor, double eps, double next_eps, double* y, double*
-                                 normed, double* stats, void* stream);
-int gm_residual_norm_forward_bf16(const uint16_t* x, const uint16_t* u, const uint16_t* z, const float* gain, const
-                                  float* offset, const float* scale, const float* next_gain, const float* next_offset,
+int gm_residual_norm_forward_f64(const double* x, const double* u, const double* z, const void* const* params, int64_t
+                                 n_rows, int64_t D, int64_t a0, int64_t nf, const int64_t* offsets, const int64_t*
+                                 mults, double factor, double eps, double next_eps, double* y, double* normed, double*
+                                 stats, void* stream);
+int gm_residual_norm_forward_bf16(const uint16_t* x, const uint16_t* u, const uint16_t* z, const void* const* params,
                                   int64_t n_rows, int64_t D, int64_t a0, int64_t nf, const int64_t* offsets, const
                                   int64_t* mults, double factor, double eps, double next_eps, uint16_t* y, uint16_t*
                                   normed, float* stats, void* stream);
-int gm_residual_norm_forward_bf16_f32(const uint16_t* x, const float* u, const uint16_t* z, const float* gain, const
-                                      float* offset, const float* scale, const float* next_gain, const float*
-                                      next_offset, int64_t n_rows, int64_t D, int64_t a0, int64_t nf, const int64_t*
-                                      offsets, const int64_t* mults, double factor, double eps, double next_eps,
-                                      uint16_t* y, uint16_t* normed, float* stats, void* stream);
+int gm_residual_norm_forward_bf16_f32(const uint16_t* x, const float* u, const uint16_t* z, const void* const* params,
+                                      int64_t n_rows, int64_t D, int64_t a0, int64_t nf, const int64_t* offsets, const
+                                      int64_t* mults, double factor, double eps, double next_eps, uint16_t* y,
+                                      uint16_t* normed, float* stats, void* stream);
 int gm_residual_norm_backward_f32(const float* dy, const float* dn, const float* x, const float* u, const float* z,
-                                  const float* gain, const float* offset, const float* scale, const float* next_gain,
-                                  const float* stats, int64_t n_rows, int64_t D, int64_t a0, int64_t nf, const
-                                  int64_t* offsets, const int64_t* mults, double factor, float* dx, float* du, float*
-                                  dz, float* partial, float* dparams, void* stream);
+                                  const void* const* params, const float* stats, int64_t n_rows, int64_t D, int64_t
+                                  a0, int64_t nf, const int64_t* offsets, const int64_t* mults, double factor, float*
+                                  dx, float* du, float* dz, float* partial, float* dparams, void* stream);
 int gm_residual_norm_backward_f64(const double* dy, const double* dn, const double* x, const double* u, const double*
-                                  z, const double* gain, const double* offset, const double* scale, const double*
-                                  next_gain, const double* stats, int64_t n_rows, int64_t D, int64_t a0, int64_t nf,
-                                  const int64_t* offsets, const int64_t* mults, double factor, double* dx, double* du,
-                                  double* dz, double* partial, double* dparams, void* stream);
+                                  z, const void* const* params, const double* stats, int64_t n_rows, int64_t D,
+                                  int64_t a0, int64_t nf, const int64_t* offsets, const int64_t* mults, double factor,
+                                  double* dx, double* du, double* dz, double* partial, double* dparams, void* stream);
 int gm_residual_norm_backward_bf16(const uint16_t* dy, const uint16_t* dn, const uint16_t* x, const uint16_t* u, const
-                                   uint16_t* z, const float* gain, const float* offset, const float* scale, const
-                                   float* next_gain, const float* stats, int64_t n_rows, int64_t D, int64_t a0,
-                                   int64_t nf, const int64_t* offsets, const int64_t* mults, double factor, uint16_t*
-                                   dx, uint16_t* du, uint16_t* dz, float* partial, float* dparams, void* stream);
+                                   uint16_t* z, const void* const* params, const float* stats, int64_t n_rows, int64_t
+                                   D, int64_t a0, int64_t nf, const int64_t* offsets, const int64_t* mults, double
+                                   factor, uint16_t* dx, uint16_t* du, uint16_t* dz, float* partial, float* dparams,
+                                   void* stream);
 int gm_residual_norm_backward_bf16_f32(const uint16_t* dy, const uint16_t* dn, const uint16_t* x, const float* u,
-                                       const uint16_t* z, const float* gain, const float* offset, const float* scale,
-                                       const float* next_gain, const float* stats, int64_t n_rows, int64_t D, int64_t
-                                       a0, int64_t nf, const int64_t* offsets, const int64_t* mults, double factor,
-                                       uint16_t* dx, float* du, uint16_t* dz, float* partial, float* dparams, void*
-                                       stream);
+                                       const uint16_t* z, const void* const* params, const float* stats, int64_t
+                                       n_rows, int64_t D, int64_t a0, int64_t nf, const int64_t* offsets, const
+                                       int64_t* mults, double factor, uint16_t* dx, float* du, uint16_t* dz, float*
+                                       partial, float* dparams, void* stream);
 
 /* Fused feed-forward of the transformer block; replaces the norm2 -> linear1 ->
  * activation -> linear2 -> residual sequence of SO2TransformerBlock.forward

@@ -55,7 +55,8 @@ def oracle(copies, v, post, gate, scale, norm, eps=1e-5):
         uh, muh = c * inv, (u.abs() + mean0(u.abs())) * inv
         gain, off = v["post.gamma"][index], offset(v["post.beta"])
     else:
-        uh, muh, gain, off, inv = u, u.abs(), torch.ones(D, dtype=torch.float64), torch.zeros(D, dtype=torch.float64), 1.0
+        uh, muh, inv = u, u.abs(), 1.0
+        gain, off = torch.ones(D, dtype=torch.float64), torch.zeros(D, dtype=torch.float64)
     factor = {"": 1.0, "sigmoid": 1.0, "double_sigmoid": 2.0}[gate]
     sig = torch.sigmoid(v["z"]) if gate else None
     act = factor * sig[:, index] if gate else torch.ones_like(x)
@@ -102,8 +103,8 @@ def values(copies, nodes, post, gate, scale, norm, dtype, branch, seed=0):
     def normal(i, *shape, to=dtype):
         return problems.normal(shape, 10 * seed + i).to(to).double()
 
-    v = {"x": (1.5 * normal(0, nodes, D) + 0.3).to(dtype).double(), "u": (0.5 * normal(1, nodes, D)).to(branch).double(),
-         "dy": normal(2, nodes, D)}
+    v = {"x": (1.5 * normal(0, nodes, D) + 0.3).to(dtype).double(),
+         "u": (0.5 * normal(1, nodes, D)).to(branch).double(), "dy": normal(2, nodes, D)}
     if gate:
         v["z"] = normal(3, nodes, C)
     if norm:
@@ -118,8 +119,8 @@ def values(copies, nodes, post, gate, scale, norm, dtype, branch, seed=0):
 
 def module_of(copies, v, post, gate, scale, norm, dtype, device):
     pd = torch.float64 if dtype == torch.float64 else torch.float32
-    m = SO2ResidualNorm(SO2FieldType(copies), post_norm=post, gate=gate or None, scale=0.5 if scale else None, norm=norm,
-                        dtype=pd, device=device)
+    m = SO2ResidualNorm(SO2FieldType(copies), post_norm=post, gate=gate or None, scale=0.5 if scale else None,
+                        norm=norm, dtype=pd, device=device)
     named = {}
     for kind in ("post", "norm"):
         if getattr(m, kind) is not None:
@@ -402,11 +403,13 @@ def test_the_library_refuses_bad_arguments():
 
     lib = _native.library()
     offsets, mults = (ctypes.c_int64 * 1)(4), (ctypes.c_int64 * 1)(4)
+    params = (ctypes.c_void_p * 8)()
 
     def forward(n=1, D=12, a0=4, nf=1, eps=1e-5):
-        return lib.gm_residual_norm_forward_f32(None, None, None, None, None, None, None, None, n, D, a0, nf,
-                                                ctypes.cast(offsets, ctypes.c_void_p), ctypes.cast(mults, ctypes.c_void_p),
-                                                1.0, eps, eps, None, None, None, None)
+        return lib.gm_residual_norm_forward_f32(None, None, None, ctypes.cast(params, ctypes.c_void_p), n, D, a0, nf,
+                                                ctypes.cast(offsets, ctypes.c_void_p),
+                                                ctypes.cast(mults, ctypes.c_void_p), 1.0, eps, eps, None, None, None,
+                                                None)
 
     for kw, message in ((dict(n=-1), b"non-negative"), (dict(D=1025), b"1..1024"), (dict(a0=13), b"a0 must lie"),
                         (dict(D=14), b"fill the flat width"), (dict(nf=9), b"at most 8"), (dict(eps=0.0), b"eps"),
@@ -414,3 +417,5 @@ def test_the_library_refuses_bad_arguments():
         assert forward(**kw) == 1
         assert message in lib.gm_last_error(), kw
     assert forward(n=0) == 0
+    params[1] = 64  # the gains of one frequency alone (an address nothing reads)
+    assert forward(n=0) == 1 and b"every frequency" in lib.gm_last_error()
