@@ -1,0 +1,234 @@
+"""The differential neighbourhood softmax: per head the difference of two maps.
+
+Head h scores every edge ``e = (i <- j)`` twice, with the maps ``p = 2h, 2h + 1``
+of ``map_type`` each,
+
+    s_p   = scale <q_i,p , rho(g_ij) k_j,p> + bias(e),
+    a_p   = softmax of s_p over i's edges inside the window,
+    alpha = a_2h - lambda_h a_2h+1,
+
+``lambda`` one learned number a head.  What both maps give to every neighbour
+cancels, so the weights keep what tells neighbours apart.  A map's copies sit
+side by side in the rows (map-major within each frequency), so rows of H heads
+with an even number of copies hold H heads of two maps of half the copies each:
+the layers' query and key rows serve as they are.
+
+Edges outside the window count for nothing, whatever their rows hold; a target
+with no edge inside has only zero weights (and zero gradients).
+
+The op reads an edge set through :class:`EdgeTables`, which its owner builds once
+and keeps.  On the GPU (``gm_differential_*``) neither the maps nor their
+gradients are written: the forward keeps one number a target and map for the
+backward.  bfloat16 rows take float32 tables, arithmetic and weights, and get
+bfloat16 gradients, rounded once.  CPU tensors take the formulas in torch.
+"""
+
+from __future__ import annotations
+
+import functools
+import math
+from typing import Any
+
+import torch
+from torch import Tensor
+
+from gm_attention_amd import _native
+from gm_attention_amd.nn import fused_attention
+from gm_attention_amd.representations.field_type import SO2FieldType
+
+MAX_H, MAX_F, MAX_D = fused_attention.MAX_H, fused_attention.MAX_F, fused_attention.MAX_D
+
+
+class EdgeTables:
+    """What the op reads of one edge set: the CSR over targets (``row_ptr``,
+    ``source``), the transport phases ``(E, orders, 2)``, the softmax bias and the
+    window's support (:class:`fused_attention.Geometry`'s tables).
+
+    ``n_sources`` is the number of key rows (the targets' by default).  The
+    indices are checked here, once; the GPU's copies of the tables are packed here,
+    so a table written to afterwards is not seen.  A step under graph capture needs
+    its tables (for training :meth:`group_sources` too) from before the capture."""
+
+    def __init__(self, row_ptr: Tensor, source: Tensor, transport: Tensor, bias: Tensor, inside: Tensor, *,
+                 n_sources: int | None = None) -> None:
+        _outside_capture(row_ptr, "EdgeTables")
+        n_edges = source.shape[0]
+        if row_ptr.dtype != torch.int64 or row_ptr.ndim != 1 or row_ptr.shape[0] < 1:
+            raise ValueError("row_ptr must be int64 (n_targets + 1,).")
+        if source.dtype != torch.int64 or source.ndim != 1:
+            raise ValueError("source must be int64 (n_edges,).")
+        if transport.ndim != 3 or transport.shape[0] != n_edges or transport.shape[1] < 1 or transport.shape[2] != 2:
+            raise ValueError(f"transport must be ({n_edges}, orders, 2), got {tuple(transport.shape)}.")
+        if transport.dtype not in (torch.float32, torch.float64):
+            raise ValueError(f"the tables must be float32 or float64, got {transport.dtype}.")
+        if bias.dtype != transport.dtype or tuple(bias.shape) != (n_edges,):
+            raise ValueError(f"bias must be ({n_edges},) in transport's dtype.")
+        if inside.dtype not in (torch.uint8, torch.bool) or tuple(inside.shape) != (n_edges,):
+            raise ValueError(f"inside must be uint8 or bool ({n_edges},).")
+        if any(t.device != row_ptr.device for t in (source, transport, bias, inside)):
+            raise ValueError("every table must live on the same device.")
+        self.n_targets = row_ptr.shape[0] - 1
+        self.n_sources = self.n_targets if n_sources is None else int(n_sources)
+        self.n_edges = n_edges
+        if max(self.n_targets, self.n_sources, n_edges) >= 2**31:
+            raise ValueError("nodes and edges are indexed in 32 bits.")
+        bad = (row_ptr[0] != 0) | (row_ptr[-1] != n_edges) | (row_ptr[1:] < row_ptr[:-1]).any()
+        if n_edges:
+            bad = bad | (source.amin() < 0) | (source.amax() >= self.n_sources)
+        if bool(bad):
+            raise ValueError("row_ptr must rise from 0 to n_edges and every source lie in 0 .. n_sources - 1.")
+        self.device, self.dtype, self.orders = transport.device, transport.dtype, transport.shape[1]
+        self.row_ptr = row_ptr.detach().clone()
+        self._sources = None
+        masked = bias.detach().masked_fill(inside == 0, -math.inf)
+        phases = transport.detach()[:, 1:].reshape(n_edges, 2 * (self.orders - 1))
+        if self.device.type != "cuda":
+            self._source, self._phases, self._bias = source.detach(), phases, masked
+            return
+        records = torch.empty(n_edges, 2 * self.orders, dtype=self.dtype, device=self.device)
+        words = records.view(_WORD[self.dtype])
+        words[:, 0] = source
+        records[:, 1] = masked
+        records[:, 2:] = phases
+        self.records = records
+        self._kept = [_native.Made(self.row_ptr, records)]
+
+    def group_sources(self) -> tuple[Tensor, Tensor]:
+        """``(src_ptr, records_s)``: the edges sorted by source, each with its target,
+        its place and its tables, for the backward; found once."""
+        if self._sources is None:
+            with _native.LOCK:
+                if self._sources is None:
+                    self._sources = self._group()
+        return self._sources
+
+    def _group(self) -> tuple[Tensor, Tensor]:
+        _outside_capture(self.row_ptr, "EdgeTables.group_sources")
+        self.found()
+        sorted_source, order = torch.sort(self.records.view(_WORD[self.dtype])[:, 0].to(torch.int32), stable=True)
+        bounds = torch.arange(self.n_sources + 1, dtype=torch.int32, device=self.device)
+        src_ptr = torch.searchsorted(sorted_source, bounds)
+        target = torch.repeat_interleave(torch.arange(self.n_targets, device=self.device),
+                                         self.row_ptr[1:] - self.row_ptr[:-1], output_size=self.n_edges)
+        records_s = torch.empty(self.n_edges, 2 + 2 * self.orders, dtype=self.dtype, device=self.device)
+        words = records_s.view(_WORD[self.dtype])
+        words[:, 0] = target.index_select(0, order)
+        words[:, 1] = order
+        words[:, 3] = 0
+        mine = self.records.index_select(0, order)
+        records_s[:, 2] = mine[:, 1]
+        records_s[:, 4:] = mine[:, 2:]
+        self._kept.append(_native.Made(src_ptr, records_s))
+        return src_ptr, records_s
+
+    def found(self) -> None:
+        """The current stream reads what is kept from here on."""
+        for made in self._kept:
+            made.found()
+
+
+_WORD = {torch.float32: torch.int32, torch.float64: torch.int64}
+
+
+def _outside_capture(t: Tensor, what: str) -> None:
+    if t.is_cuda and torch.cuda.is_current_stream_capturing():
+        raise RuntimeError(f"{what} waits for the device: build it before the capture.")
+
+
+@functools.lru_cache(maxsize=256)
+def maps_plan(map_type: SO2FieldType, heads: int) -> fused_attention.Plan:
+    """The descriptor rows of the rows' ``2 heads`` maps of ``map_type``."""
+    if not isinstance(map_type, SO2FieldType):
+        raise TypeError(f"map_type must be an SO2FieldType, got {type(map_type).__name__}.")
+    if not 1 <= heads <= MAX_H:
+        raise ValueError(f"heads must lie in 1..{MAX_H}, got {heads}.")
+    full = map_type.scaled(2 * heads)
+    if len(map_type) > MAX_F or full.dimension > MAX_D:
+        raise ValueError(f"the maps must hold at most {MAX_F} frequencies and {MAX_D} numbers a row, "
+                         f"got {full!r} ({full.dimension}).")
+    return fused_attention.plan_of(map_type, full, 2 * heads)
+
+
+@functools.lru_cache(maxsize=256)
+def _host_rows(map_type: SO2FieldType, heads: int) -> Tensor:
+    return torch.tensor([list(row) for row in maps_plan(map_type, heads).rows], dtype=torch.int64)
+
+
+class DifferentialSoftmax(torch.autograd.Function):
+    """``alpha (n_edges, H)`` from the maps' rows and ``lam (H,)``; ``dq``, ``dk``
+    in the rows' dtype and ``dlam`` back."""
+
+    @staticmethod
+    def forward(ctx: Any, q: Tensor, k: Tensor, lam: Tensor, tables: EdgeTables, desc: Tensor, heads: int,
+                scale: float) -> Tensor:
+        train = any(ctx.needs_input_grad)
+        if train:
+            tables.group_sources()  # here: the backward may be captured, or run on a thread and stream of its own
+        with torch.profiler.record_function("gm::attention/differential_softmax"):
+            alpha, lse = _native.differential_forward(q, k, lam, tables, desc, heads, scale, train)
+        if train:
+            ctx.save_for_backward(q, k, lam, lse)
+            ctx.rest = (tables, desc, heads, scale)
+        return alpha
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx: Any, grad_alpha: Tensor) -> tuple:
+        q, k, lam, lse = ctx.saved_tensors
+        with torch.profiler.record_function("gm::attention/differential_softmax_backward"):
+            dq, dk, dlam = _native.differential_backward(grad_alpha.contiguous(), q, k, lam, lse, *ctx.rest)
+        return dq, dk, dlam, None, None, None, None
+
+
+def differential_softmax(q: Tensor, k: Tensor, lam: Tensor, tables: EdgeTables, map_type: SO2FieldType, heads: int,
+                         scale: float | None = None) -> Tensor:
+    """The heads' attention weights ``(n_edges, heads)`` of ``q (n_targets, D)`` and
+    ``k (n_sources, D)``, rows of ``2 heads`` maps of ``map_type``, under ``lam
+    (heads,)``; ``scale`` is ``1 / sqrt(dim map_type)`` by default."""
+    plan = maps_plan(map_type, heads)
+    table = torch.float32 if q.dtype == torch.bfloat16 else q.dtype
+    if table != tables.dtype or k.dtype != q.dtype:
+        raise ValueError(f"q and k must share a dtype, {tables.dtype} (or bfloat16 with float32 tables), "
+                         f"got {q.dtype} and {k.dtype}.")
+    if tuple(q.shape) != (tables.n_targets, plan.width) or tuple(k.shape) != (tables.n_sources, plan.width):
+        raise ValueError(f"q and k must be ({tables.n_targets}, {plan.width}) and ({tables.n_sources}, {plan.width}), "
+                         f"got {tuple(q.shape)} and {tuple(k.shape)}.")
+    if tuple(lam.shape) != (heads,):
+        raise ValueError(f"lam must be ({heads},), got {tuple(lam.shape)}.")
+    if any(t.device != tables.device for t in (q, k, lam)):
+        raise ValueError("q, k and lam must live on the tables' device.")
+    top = max((n for n, *_ in plan.rows), default=0)
+    if top >= tables.orders:
+        raise ValueError(f"the tables hold orders below {tables.orders}, the maps need {top}.")
+    scale = 1.0 / math.sqrt(map_type.dimension) if scale is None else float(scale)
+    if q.device.type != "cuda":
+        return _eager(q, k, lam, tables, plan, scale)
+    return DifferentialSoftmax.apply(q.contiguous(), k.contiguous(), lam.to(table).contiguous(), tables,
+                                     _host_rows(map_type, heads), heads, scale)
+
+
+def _eager(q: Tensor, k: Tensor, lam: Tensor, tables: EdgeTables, plan: fused_attention.Plan, scale: float) -> Tensor:
+    """The formulas in torch, in the tables' arithmetic."""
+    n, maps = tables.n_targets, plan.heads
+    target = torch.repeat_interleave(torch.arange(n, device=q.device), tables.row_ptr[1:] - tables.row_ptr[:-1])
+    # an edge outside the window reads nothing: its row may hold anything
+    inside = (tables._bias != -math.inf).unsqueeze(-1)
+    qe = q.to(tables.dtype).index_select(0, target).masked_fill(~inside, 0.0)
+    ke = k.to(tables.dtype).index_select(0, tables._source).masked_fill(~inside, 0.0)
+    score = 0.0
+    for f, a, off, _, dim in plan.rows:
+        block = slice(off, off + maps * a * dim)
+        if f == 0:
+            score = score + (qe[:, block] * ke[:, block]).reshape(-1, maps, a).sum(-1)
+        else:
+            qr, qi = qe[:, block].reshape(-1, maps, a, 2).unbind(-1)
+            kr, ki = ke[:, block].reshape(-1, maps, a, 2).unbind(-1)
+            cos, sin = tables._phases[:, 2 * f - 2, None], tables._phases[:, 2 * f - 1, None]
+            score = score + cos * (qr * kr + qi * ki).sum(-1) + sin * (qi * kr - qr * ki).sum(-1)
+    score = scale * score + tables._bias.unsqueeze(-1)
+    index = target.unsqueeze(-1).expand(-1, maps)
+    top = score.new_full((n, maps), -math.inf).scatter_reduce(0, index, score.detach(), "amax")
+    weight = torch.exp(score - top.masked_fill(top == -math.inf, 0.0).index_select(0, target))
+    total = score.new_zeros(n, maps).index_add(0, target, weight)
+    weight = weight / total.masked_fill(total == 0, 1.0).index_select(0, target)
+    return weight[:, 0::2] - lam.to(tables.dtype) * weight[:, 1::2]

@@ -264,6 +264,59 @@ int gm_edge_tables_f64(const double* targets, const double* target_frames, const
                        double* log_coordinates, double* distances, double* polar_angles, double* transport_angles,
                        double* tangent_quadrature, double* angular_phases, double* transport_phases, void* stream);
 
+/* ---------------- the differential neighbourhood softmax ----------------
+ *
+ * Head h has two score maps p = 2 h, 2 h + 1; desc has one row a frequency
+ * (n, copies a MAP, flat offset, unused, dim), the 2 H maps filling the flat
+ * width D map-major within each frequency, frequencies rising.
+ *   s_p = scale sum_n Re< q_i,n,p , tau_n(e) k_j,n,p > + bias(e)
+ *   a_p = softmax of s_p over target i's edges inside the window
+ *   alpha[e, h] = a_2h - lambda[h] a_2h+1
+ * A target with no edge inside has zero weights and gradients; what the rows of
+ * an edge outside hold is not read into anything.
+ * records (n_edges, 2 orders) in the order of the CSR row_ptr over targets, in
+ * words of the tables' type: the source node (as an integer of that size), the
+ * bias (-inf outside the window), then (cos, sin) of orders 1 .. orders - 1.
+ * records_s (n_edges, 2 + 2 orders) in the order of the edges sorted by source,
+ * src_ptr its CSR: target, edge (integers), bias, 0, (cos, sin).  Nodes must lie
+ * inside their tables (the kernels follow them).
+ * lse (n_targets, 2 H), or NULL where no backward follows: the log sum of
+ * exponentials.  Backward from g = d alpha: dq, dk in the rows' type,
+ * dlambda (H); pairs (n_targets, 2 H, 2), ds (n_edges, 2 H) and partial
+ * (gm_differential_partials(H) doubles) are workspaces.  Sums in a fixed order.
+ * Suffix _bf16: bfloat16 rows, float tables and arithmetic.  No reference
+ * counterpart (the single map's: gm_softmax_*). */
+int64_t gm_differential_partials(int64_t heads);
+int gm_differential_forward_f32(const float* q, const float* k, const float* lambda, const float* records, const
+                                int64_t* desc, const int64_t* row_ptr, int64_t n_targets, int64_t n_sources, int64_t
+                                n_edges, int64_t D, int64_t orders, int64_t F, int64_t H, double scale, float* alpha,
+                                float* lse, void* stream);
+int gm_differential_forward_f64(const double* q, const double* k, const double* lambda, const double* records, const
+                                int64_t* desc, const int64_t* row_ptr, int64_t n_targets, int64_t n_sources, int64_t
+                                n_edges, int64_t D, int64_t orders, int64_t F, int64_t H, double scale, double* alpha,
+                                double* lse, void* stream);
+int gm_differential_forward_bf16(const uint16_t* q, const uint16_t* k, const float* lambda, const float* records,
+                                 const int64_t* desc, const int64_t* row_ptr, int64_t n_targets, int64_t n_sources,
+                                 int64_t n_edges, int64_t D, int64_t orders, int64_t F, int64_t H, double scale,
+                                 float* alpha, float* lse, void* stream);
+int gm_differential_backward_f32(const float* g, const float* q, const float* k, const float* lambda, const float*
+                                 records, const float* records_s, const int64_t* desc, const int64_t* row_ptr, const
+                                 int64_t* src_ptr, int64_t n_targets, int64_t n_sources, int64_t n_edges, int64_t D,
+                                 int64_t orders, int64_t F, int64_t H, double scale, const float* lse, float* pairs,
+                                 float* ds, double* partial, float* dq, float* dk, float* dlambda, void* stream);
+int gm_differential_backward_f64(const double* g, const double* q, const double* k, const double* lambda, const
+                                 double* records, const double* records_s, const int64_t* desc, const int64_t*
+                                 row_ptr, const int64_t* src_ptr, int64_t n_targets, int64_t n_sources, int64_t
+                                 n_edges, int64_t D, int64_t orders, int64_t F, int64_t H, double scale, const double*
+                                 lse, double* pairs, double* ds, double* partial, double* dq, double* dk, double*
+                                 dlambda, void* stream);
+int gm_differential_backward_bf16(const float* g, const uint16_t* q, const uint16_t* k, const float* lambda, const
+                                  float* records, const float* records_s, const int64_t* desc, const int64_t* row_ptr,
+                                  const int64_t* src_ptr, int64_t n_targets, int64_t n_sources, int64_t n_edges,
+                                  int64_t D, int64_t orders, int64_t F, int64_t H, double scale, const float* lse,
+                                  float* pairs, float* ds, double* partial, uint16_t* dq, uint16_t* dk, float*
+                                  dlambda, void* stream);
+
 /* ---------------- transformer block pointwise operators ----------------
  *
  * Flat node rows of width D: frequency 0 in [0, a0), then the nf nonzero
