@@ -22,24 +22,10 @@
 // other node, the bias (-inf outside the window) and the transport's (cos, sin) of
 // orders 1 .., packed once for an edge set; the source side's, in the order of the
 // edges sorted by source, name the edge too, whose g they read.
-#include <hip/hip_runtime.h>
-
-#include <algorithm>
-#include <type_traits>
-
-#include "common.hpp"
+#include "differential.hpp"
 
 namespace gm {
 namespace {
-
-constexpr int kDfMaxFreq = GM_ATTN_MAX_F;
-constexpr int kDfMaxMaps = 2 * GM_ATTN_MAX_H;
-
-// The 2 H maps in the rows: frequency f's order n, copies a a map, flat offset.
-struct DfLayout {
-  int F, H, P, D, orders;
-  int n[kDfMaxFreq], a[kDfMaxFreq], off[kDfMaxFreq];
-};
 
 template <typename T>
 struct DfWord {
@@ -49,39 +35,6 @@ template <>
 struct DfWord<double> {
   using type = int64_t;
 };
-
-// T: the arithmetic's type; rows of T, or of bfloat16 (uint16_t) with T = float.
-template <typename T, typename R>
-struct DfArgs {
-  DfLayout L;
-  const R* q;
-  const R* k;
-  const T* lambda;       // (H)
-  const T* records;      // (n_edges, 2 orders): other node, bias, (cos, sin) of orders 1 ..
-  const T* records_s;    // (n_edges, 2 + 2 orders): target, edge, bias, 0, (cos, sin) of orders 1 ..
-  const int64_t* row_ptr;  // over targets
-  const int64_t* src_ptr;  // over sources
-  const T* g;            // (n_edges, H)
-  T* alpha;              // (n_edges, H)
-  T* lse;                // (n_targets, 2 H): log sum exp (-inf where no edge is inside)
-  T* pairs;              // (n_targets, 2 H, 2): that beside T, the backward's workspace
-  T* ds;                 // (n_edges, 2 H): the generic backward's workspace
-  R* dq;
-  R* dk;
-  int64_t n_targets, n_sources;
-  T scale;
-};
-
-__device__ __forceinline__ float df_log(float x) { return logf(x); }
-__device__ __forceinline__ double df_log(double x) { return log(x); }
-__device__ __forceinline__ float df_widen(float x) { return x; }
-__device__ __forceinline__ double df_widen(double x) { return x; }
-__device__ __forceinline__ float df_widen(uint16_t x) { return __uint_as_float((uint32_t)x << 16); }
-__device__ __forceinline__ void df_narrow(float v, float& o) { o = v; }
-__device__ __forceinline__ void df_narrow(double v, double& o) { o = v; }
-__device__ __forceinline__ void df_narrow(float v, uint16_t& o) {  // to nearest even
-  o = __builtin_bit_cast(uint16_t, static_cast<__bf16>(v));
-}
 
 template <typename T>
 __device__ __forceinline__ int64_t node_of(const T* word) {
@@ -338,9 +291,29 @@ int df_prepare(DfArgs<T, R>& a, const R* q, const R* k, const T* lambda, const T
   return GM_OK;
 }
 
+// The rows' classes (order null: the simple kernels), which the lane kernels must serve.
+template <typename T, typename R>
+int df_rows(const DfArgs<T, R>& a, const int32_t* order, const int64_t* counts, int64_t n, DfRows& rows) {
+  rows = DfRows{order, {0, 0, 0}};
+  if (!order) return GM_OK;
+  GM_REQUIRE((std::is_same<T, float>::value) && df_slots(a.L) > 0, "the lane kernels do not serve this layout");
+  GM_REQUIRE(counts, "the classes' counts (a host array of three) are required");
+  int64_t sum = 0;
+  for (int c = 0; c < 3; ++c) {
+    GM_REQUIRE(counts[c] >= 0, "a class has a negative count");
+    rows.count[c] = counts[c];
+    sum += counts[c];
+  }
+  GM_REQUIRE(sum == n, "the classes must hold every row once");
+  GM_REQUIRE(aligned(a.q, 16) && aligned(a.k, 16) && aligned(a.dq, 16) && aligned(a.dk, 16) && aligned(a.records, 8) &&
+                 aligned(a.records_s, 8) && aligned(a.pairs, 8),
+             "the lane kernels take rows at multiples of 16 bytes");
+  return GM_OK;
+}
+
 template <typename T, typename R>
 int differential_forward(const R* q, const R* k, const T* lambda, const T* records, const int64_t* desc,
-                         const int64_t* row_ptr, int64_t n_targets, int64_t n_sources, int64_t n_edges, int64_t D,
+                         const int64_t* row_ptr, const int32_t* order, const int64_t* counts, int64_t n_targets, int64_t n_sources, int64_t n_edges, int64_t D,
                          int64_t orders, int64_t F, int64_t H, double scale, T* alpha, T* lse, void* stream) {
   DfArgs<T, R> a{};
   const int rc = df_prepare(a, q, k, lambda, records, desc, row_ptr, n_targets, n_sources, n_edges, D, orders, F, H,
@@ -350,6 +323,12 @@ int differential_forward(const R* q, const R* k, const T* lambda, const T* recor
   if (n_edges > 0) GM_REQUIRE(alpha, "alpha must be a device pointer");
   a.alpha = alpha;
   a.lse = lse;
+  DfRows rows;
+  const int status = df_rows(a, order, counts, n_targets, rows);
+  if (status != GM_OK) return status;
+  if constexpr (std::is_same<T, float>::value) {
+    if (order) return df_launch_units(DfPass::Forward, a, rows, (hipStream_t)stream);
+  }
   hipLaunchKernelGGL((differential_forward_generic<T, R>), dim3((unsigned)blocks_for(n_targets)), dim3(256), 0,
                      (hipStream_t)stream, a);
   return check_launch("differential_forward");
@@ -357,7 +336,8 @@ int differential_forward(const R* q, const R* k, const T* lambda, const T* recor
 
 template <typename T, typename R>
 int differential_backward(const T* g, const R* q, const R* k, const T* lambda, const T* records, const T* records_s,
-                          const int64_t* desc, const int64_t* row_ptr, const int64_t* src_ptr, int64_t n_targets,
+                          const int64_t* desc, const int64_t* row_ptr, const int64_t* src_ptr, const int32_t* order,
+                          const int64_t* counts, const int32_t* order_s, const int64_t* counts_s, int64_t n_targets,
                           int64_t n_sources, int64_t n_edges, int64_t D, int64_t orders, int64_t F, int64_t H,
                           double scale, const T* lse, T* pairs, T* ds, double* partial, R* dq, R* dk, T* dlambda, void* stream) {
   DfArgs<T, R> a{};
@@ -367,7 +347,10 @@ int differential_backward(const T* g, const R* q, const R* k, const T* lambda, c
   GM_REQUIRE(partial && dlambda, "partial and dlambda must be device pointers");
   if (n_targets > 0) GM_REQUIRE(lse && pairs && dq, "lse, pairs and dq must be device pointers");
   if (n_sources > 0) GM_REQUIRE(src_ptr && dk, "src_ptr and dk must be device pointers");
-  if (n_edges > 0) GM_REQUIRE(g && records_s && ds, "g, the sources' records and ds must be device pointers");
+  if (n_edges > 0) GM_REQUIRE(g && records_s, "g and the sources' records must be device pointers");
+  GM_REQUIRE(!order == !order_s || n_targets == 0 || n_sources == 0, "both sides' rows are in classes, or neither's");
+  const bool lanes = order || order_s;
+  if (n_edges > 0 && !lanes) GM_REQUIRE(ds, "ds must be a device pointer without the rows' classes");
   a.g = g;
   a.records_s = records_s;
   a.src_ptr = src_ptr;
@@ -377,12 +360,23 @@ int differential_backward(const T* g, const R* q, const R* k, const T* lambda, c
   a.dq = dq;
   a.dk = dk;
   const hipStream_t s = (hipStream_t)stream;
-  if (n_targets > 0) {
+  DfRows targets, sources;
+  int status = df_rows(a, order, counts, n_targets, targets);
+  if (status == GM_OK) status = df_rows(a, order_s, counts_s, n_sources, sources);
+  if (status != GM_OK) return status;
+  if constexpr (std::is_same<T, float>::value) {
+    if (lanes) {
+      status = df_launch_units(DfPass::BackwardTarget, a, targets, s);
+      if (status == GM_OK) status = df_launch_units(DfPass::BackwardSource, a, sources, s);
+      if (status != GM_OK) return status;
+    }
+  }
+  if (n_targets > 0 && !lanes) {
     const dim3 grid((unsigned)blocks_for(n_targets));
     hipLaunchKernelGGL((differential_backward_scores_generic<T, R>), grid, dim3(256), 0, s, a);
     hipLaunchKernelGGL((differential_backward_target_generic<T, R>), grid, dim3(256), 0, s, a);
   }
-  if (n_sources > 0)
+  if (n_sources > 0 && !lanes)
     hipLaunchKernelGGL((differential_backward_source_generic<T, R>), dim3((unsigned)blocks_for(n_sources)), dim3(256),
                        0, s, a);
   hipLaunchKernelGGL(differential_lambda_partial<T>, dim3(kLambdaBlocks), dim3(256), 0, s, (const T*)pairs, n_targets,
@@ -397,23 +391,34 @@ int differential_backward(const T* g, const R* q, const R* k, const T* lambda, c
 
 extern "C" int64_t gm_differential_partials(int64_t heads) { return gm::kLambdaBlocks * heads; }
 
+extern "C" int gm_differential_slots(const int64_t* desc, int64_t F, int64_t H, int64_t D, int64_t orders,
+                                     int64_t* slots) {
+  GM_REQUIRE(slots, "slots must be a host pointer");
+  gm::DfLayout L{};
+  const int rc = gm::parse_maps(desc, F, H, D, orders, L);
+  if (rc != GM_OK) return rc;
+  *slots = gm::df_slots(L);
+  return GM_OK;
+}
+
 // T: the arithmetic's type, R the rows'.
 #define GM_DIFFERENTIAL_ENTRY(SFX, T, R)                                                                              \
   extern "C" int gm_differential_forward_##SFX(                                                                       \
       const R* q, const R* k, const T* lambda, const T* records, const int64_t* desc, const int64_t* row_ptr,         \
-      int64_t n_targets, int64_t n_sources, int64_t n_edges, int64_t D, int64_t orders, int64_t F, int64_t H,         \
-      double scale, T* alpha, T* lse, void* stream) {                                                                 \
-    return gm::differential_forward<T, R>(q, k, lambda, records, desc, row_ptr, n_targets, n_sources, n_edges, D,     \
-                                          orders, F, H, scale, alpha, lse, stream);                                   \
+      const int32_t* order, const int64_t* counts, int64_t n_targets, int64_t n_sources, int64_t n_edges, int64_t D,  \
+      int64_t orders, int64_t F, int64_t H, double scale, T* alpha, T* lse, void* stream) {                           \
+    return gm::differential_forward<T, R>(q, k, lambda, records, desc, row_ptr, order, counts, n_targets, n_sources,  \
+                                          n_edges, D, orders, F, H, scale, alpha, lse, stream);                       \
   }                                                                                                                   \
   extern "C" int gm_differential_backward_##SFX(                                                                      \
       const T* g, const R* q, const R* k, const T* lambda, const T* records, const T* records_s, const int64_t* desc, \
-      const int64_t* row_ptr, const int64_t* src_ptr, int64_t n_targets, int64_t n_sources, int64_t n_edges,          \
+      const int64_t* row_ptr, const int64_t* src_ptr, const int32_t* order, const int64_t* counts,                    \
+      const int32_t* order_s, const int64_t* counts_s, int64_t n_targets, int64_t n_sources, int64_t n_edges,         \
       int64_t D, int64_t orders, int64_t F, int64_t H, double scale, const T* lse, T* pairs, T* ds, double* partial,  \
       R* dq, R* dk, T* dlambda, void* stream) {                                                                       \
-    return gm::differential_backward<T, R>(g, q, k, lambda, records, records_s, desc, row_ptr, src_ptr, n_targets,    \
-                                           n_sources, n_edges, D, orders, F, H, scale, lse, pairs, ds, partial, dq,   \
-                                           dk, dlambda, stream);                                                      \
+    return gm::differential_backward<T, R>(g, q, k, lambda, records, records_s, desc, row_ptr, src_ptr, order,        \
+                                           counts, order_s, counts_s, n_targets, n_sources, n_edges, D, orders, F, H, \
+                                           scale, lse, pairs, ds, partial, dq, dk, dlambda, stream);                  \
   }
 
 GM_DIFFERENTIAL_ENTRY(f32, float, float)

@@ -1,0 +1,628 @@
+// The differential softmax's lane kernels: a map's copies are `per_map` units of
+// (A0, A1, A2) copies of frequencies 0, 1, 2, and a lane holds one unit of the query
+// (the key, in the pass over sources) and reads the same unit of every row it meets,
+// so that the lanes of an edge read its row as whole cache lines.  A wave's 64 lanes
+// are (edge slot, unit), units rounded up to a power of two.
+//
+// What bounds them is the L1's line accesses: an edge's row is D words whatever is
+// done with it.  (The single softmax's lanes hold a head's 16-byte pieces, which at
+// frequencies above 0 lie 32 bytes apart, so each load touches twice the lines it
+// uses: nine line accesses an edge at 160 numbers a row against the five here.)
+//
+// Each edge's record is copied once per 64 edges into the wave's LDS (the next 64
+// requested before the present ones are used) and read from there by the lanes of
+// its edge.  A row of more edges than a wave's LDS holds scores of goes to four or
+// sixteen waves, which combine their maxima and sums (their gradients) through LDS.
+#include <algorithm>
+
+#include "differential.hpp"
+
+namespace gm {
+namespace {
+
+constexpr int kDfSteps = 32;     // steps of a wave whose scores LDS holds: 32 S edges
+constexpr int kDfInFlight = 4;   // the forward's steps whose rows are requested together
+constexpr int kDfInFlightB = 2;  // the backward's
+
+struct DfUnits {
+  int units, per_map;    // lanes of an edge that hold something; units a map
+  int lanes, shift;      // units rounded up to a power of two; log2
+  int slots;             // 64 / lanes
+  int base0, base1, base2;
+  const int32_t* order;
+  int64_t first, count;  // rows order[first .. first + count)
+  int per_row;           // waves a row: 1 (four rows a workgroup) or the workgroup's
+};
+
+// W numbers of a row at p.
+template <int W>
+__device__ __forceinline__ void load_w(const float* p, float* v) {
+  if constexpr (W == 4) {
+    const float4 x = *reinterpret_cast<const float4*>(p);
+    v[0] = x.x;
+    v[1] = x.y;
+    v[2] = x.z;
+    v[3] = x.w;
+  } else if constexpr (W == 2) {
+    const float2 x = *reinterpret_cast<const float2*>(p);
+    v[0] = x.x;
+    v[1] = x.y;
+  } else {
+#pragma unroll
+    for (int i = 0; i < W; ++i) v[i] = p[i];
+  }
+}
+template <int W>
+__device__ __forceinline__ void load_w(const uint16_t* p, float* v) {
+  if constexpr (W == 4) {
+    const uint2 x = *reinterpret_cast<const uint2*>(p);
+    v[0] = __uint_as_float(x.x << 16);
+    v[1] = __uint_as_float(x.x & 0xFFFF0000u);
+    v[2] = __uint_as_float(x.y << 16);
+    v[3] = __uint_as_float(x.y & 0xFFFF0000u);
+  } else if constexpr (W == 2) {
+    const uint32_t x = *reinterpret_cast<const uint32_t*>(p);
+    v[0] = __uint_as_float(x << 16);
+    v[1] = __uint_as_float(x & 0xFFFF0000u);
+  } else {
+#pragma unroll
+    for (int i = 0; i < W; ++i) v[i] = df_widen(p[i]);
+  }
+}
+typedef __bf16 df_bf16x2 __attribute__((ext_vector_type(2)));
+__device__ __forceinline__ uint32_t df_pack(float lo, float hi) {
+  const df_bf16x2 b = {static_cast<__bf16>(lo), static_cast<__bf16>(hi)};
+  return __builtin_bit_cast(uint32_t, b);
+}
+template <int W>
+__device__ __forceinline__ void store_w(float* p, const float* v) {
+  if constexpr (W == 4)
+    *reinterpret_cast<float4*>(p) = make_float4(v[0], v[1], v[2], v[3]);
+  else if constexpr (W == 2)
+    *reinterpret_cast<float2*>(p) = make_float2(v[0], v[1]);
+  else
+#pragma unroll
+    for (int i = 0; i < W; ++i) p[i] = v[i];
+}
+template <int W>
+__device__ __forceinline__ void store_w(uint16_t* p, const float* v) {
+  if constexpr (W == 4)
+    *reinterpret_cast<uint2*>(p) = make_uint2(df_pack(v[0], v[1]), df_pack(v[2], v[3]));
+  else if constexpr (W == 2)
+    *reinterpret_cast<uint32_t*>(p) = df_pack(v[0], v[1]);
+  else
+#pragma unroll
+    for (int i = 0; i < W; ++i) df_narrow(v[i], p[i]);
+}
+
+template <int A0, int A1, int A2>
+struct Unit {
+  static constexpr int W0 = A0, W1 = 2 * A1, W2 = 2 * A2, N = W0 + W1 + W2;
+  static constexpr int NO = A2 > 0 ? 2 : 1;  // orders above 0
+  static constexpr int RW = 2 + 2 * NO;      // a record's words; the sources' two more
+
+  template <typename R>
+  static __device__ __forceinline__ void load(const R* row, const DfUnits& w, int unit, float (&v)[N]) {
+    load_w<W0>(row + w.base0 + unit * W0, v);
+    load_w<W1>(row + w.base1 + unit * W1, v + W0);
+    if constexpr (W2 > 0) load_w<W2>(row + w.base2 + unit * W2, v + W0 + W1);
+  }
+  template <typename R>
+  static __device__ __forceinline__ void store(R* row, const DfUnits& w, int unit, const float (&v)[N]) {
+    store_w<W0>(row + w.base0 + unit * W0, v);
+    store_w<W1>(row + w.base1 + unit * W1, v + W0);
+    if constexpr (W2 > 0) store_w<W2>(row + w.base2 + unit * W2, v + W0 + W1);
+  }
+  // Re< q, tau k >: per order cos sum (q0 k0 + q1 k1) + sin sum (q1 k0 - q0 k1)
+  static __device__ __forceinline__ float dot(const float (&q)[N], const float (&k)[N], const float (&cs)[NO],
+                                              const float (&sn)[NO]) {
+    float acc = 0.f;
+#pragma unroll
+    for (int i = 0; i < W0; ++i) acc = fmaf(q[i], k[i], acc);
+#pragma unroll
+    for (int o = 0; o < NO; ++o) {
+      const int at = o == 0 ? W0 : W0 + W1, width = o == 0 ? W1 : W2;
+      float re = 0.f, im = 0.f;
+#pragma unroll
+      for (int i = 0; i < width; i += 2) {
+        re = fmaf(q[at + i], k[at + i], fmaf(q[at + i + 1], k[at + i + 1], re));
+        im = fmaf(q[at + i + 1], k[at + i], fmaf(-q[at + i], k[at + i + 1], im));
+      }
+      acc = fmaf(cs[o], re, fmaf(sn[o], im, acc));
+    }
+    return acc;
+  }
+  // tau k, or with `back` conj(tau) k, in place
+  static __device__ __forceinline__ void turn(float (&k)[N], const float (&cs)[NO], const float (&sn)[NO], bool back) {
+#pragma unroll
+    for (int o = 0; o < NO; ++o) {
+      const int at = o == 0 ? W0 : W0 + W1, width = o == 0 ? W1 : W2;
+      const float s = back ? -sn[o] : sn[o];
+#pragma unroll
+      for (int i = 0; i < width; i += 2) {
+        const float k0 = k[at + i], k1 = k[at + i + 1];
+        k[at + i] = cs[o] * k0 - s * k1;
+        k[at + i + 1] = cs[o] * k1 + s * k0;
+      }
+    }
+  }
+};
+
+// One wave's records of 64 edges: `words` a record, in flight a batch ahead.
+template <int WORDS>
+struct Records {
+  static constexpr int kLoads = WORDS / 2;
+  float2 next[kLoads];
+  // request the records of edges [base, min(base + 64, end)); what lies past them is an edge outside the window of node 0
+  __device__ __forceinline__ void request(const float* records, int64_t base, int64_t end, int lane) {
+    const int64_t left = end - base;
+    const int pieces = (int)(left < kWave ? left : kWave) * kLoads;
+    const float2* from = reinterpret_cast<const float2*>(records + base * WORDS);
+#pragma unroll
+    for (int i = 0; i < kLoads; ++i) {
+      const int at = i * kWave + lane;
+      next[i] = at < pieces ? from[at] : make_float2(0.f, neg_inf<float>());
+    }
+  }
+  __device__ __forceinline__ void put(float* lds, int lane) const {
+    float2* to = reinterpret_cast<float2*>(lds);
+#pragma unroll
+    for (int i = 0; i < kLoads; ++i) to[i * kWave + lane] = next[i];
+  }
+};
+
+// The wave's LDS writes are seen by its other lanes' reads, and the reads before them are done.
+__device__ __forceinline__ void wave_lds() {
+  __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+  __builtin_amdgcn_wave_barrier();
+}
+
+__device__ __forceinline__ float sum_units(float v, int per_map) {
+  for (int o = 1; o < per_map; o <<= 1) v += __shfl_xor(v, o, kWave);
+  return v;
+}
+
+// Which row a wave works on, and which of its edges.
+struct Share {
+  int64_t row, e0, e1;  // the row; this wave's edges
+  int part;
+  bool live;
+};
+__device__ __forceinline__ Share share_of(const DfUnits& w, const int64_t* ptr) {
+  const int wave = threadIdx.x >> 6, waves = blockDim.x >> 6;
+  const int64_t at = xcd_spread_block(blockIdx.x, gridDim.x) * (waves / w.per_row) + wave / w.per_row;
+  Share s;
+  s.part = wave % w.per_row;
+  s.live = at < w.count;
+  s.row = s.live ? w.order[w.first + at] : 0;
+  const int64_t e0 = s.live ? ptr[s.row] : 0, e1 = s.live ? ptr[s.row + 1] : 0;
+  const int64_t steps = (e1 - e0 + w.slots - 1) / w.slots;
+  const int64_t per = (steps + w.per_row - 1) / w.per_row * w.slots;
+  s.e0 = e0 + s.part * per < e1 ? e0 + s.part * per : e1;
+  s.e1 = s.e0 + per < e1 ? s.e0 + per : e1;
+  return s;
+}
+
+// ---------------------------------------------------------------- forward
+
+template <typename R, int A0, int A1, int A2>
+__global__ __launch_bounds__(1024) void differential_forward_units(DfArgs<float, R> a, DfUnits w) {
+  using U = Unit<A0, A1, A2>;
+  constexpr int kWords = kWave * U::RW, UN = kDfInFlight;
+  extern __shared__ __align__(16) float df_lds[];
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, waves = blockDim.x >> 6;
+  const Share sh = share_of(w, a.row_ptr);
+  if (!sh.live) return;  // one wave a row, or the whole workgroup
+  float* rec = df_lds + wave * (kWords + kDfSteps * kWave);
+  float* sc = rec + kWords + lane;
+  float* shared = df_lds + waves * (kWords + kDfSteps * kWave);  // (waves, 64): the waves' maxima, then sums
+  const int u = lane & (w.lanes - 1), s = lane >> w.shift, unit = u < w.units ? u : w.units - 1;
+  const int p = unit / w.per_map;
+  float q[U::N];
+  U::load(a.q + sh.row * a.L.D, w, unit, q);
+  const float lambda = a.lambda[p >> 1];
+  const bool second = p & 1, writes = u < w.units && unit % w.per_map == 0;
+  const int steps = (int)((sh.e1 - sh.e0 + w.slots - 1) / w.slots);
+  const int held = steps < kDfSteps ? steps : kDfSteps;
+  float m = neg_inf<float>(), l = 0.f, inv = 0.f;
+
+  auto over_waves = [&](float v, bool maximum) {
+    for (int o = w.lanes; o < kWave; o <<= 1) {
+      const float x = __shfl_xor(v, o, kWave);
+      v = maximum ? (x > v || x != x ? x : v) : v + x;
+    }
+    if (w.per_row > 1) {
+      __syncthreads();
+      shared[wave * kWave + lane] = v;
+      __syncthreads();
+      v = shared[lane];
+      for (int o = 1; o < waves; ++o) {
+        const float x = shared[o * kWave + lane];
+        v = maximum ? (x > v || x != x ? x : v) : v + x;
+      }
+    }
+    return v;
+  };
+  // two steps' weights: the pair of maps' lanes exchange one each and write one edge each
+  auto write = [&](int t, float w0, float w1) {
+    const float other = __shfl_xor(second ? w0 : w1, w.per_map, kWave);
+    const int64_t e = sh.e0 + (int64_t)(t + (second ? 1 : 0)) * w.slots + s;
+    const float v = second ? other - lambda * w1 : w0 - lambda * other;
+    if (writes && e < sh.e1) a.alpha[e * a.L.H + (p >> 1)] = v;
+  };
+
+  // phase 0: every score, its maximum; the first kDfSteps steps' stay in LDS.  The steps past them are scored again
+  // for the sum (1) and the weights (2): rows beyond 16 waves' LDS only.
+  for (int phase = 0; phase < 3; ++phase) {
+    if (phase == 1) {
+      m = over_waves(m, true);
+      const float top = m == neg_inf<float>() ? 0.f : m;  // no edge inside: exp(-inf) = 0 everywhere
+      for (int t = 0; t < held; ++t) {
+        const float x = gm_exp(sc[t * kWave] - top);
+        sc[t * kWave] = x;
+        l += x;
+      }
+    }
+    if (phase == 2) {
+      l = over_waves(l, false);
+      inv = l == 0.f ? 0.f : 1.f / l;
+      if (a.lse && sh.part == 0 && s == 0 && writes)
+        a.lse[sh.row * a.L.P + p] = l == 0.f ? neg_inf<float>() : m + df_log(l);
+      for (int t = 0; t < held; t += 2) {
+        const float w0 = sc[t * kWave] * inv, w1 = t + 1 < held ? sc[(t + 1) * kWave] * inv : 0.f;
+        write(t, w0, w1);
+      }
+    }
+    const int first = phase == 0 ? 0 : kDfSteps / w.lanes * w.lanes;  // a batch's first step
+    const int skip = phase == 0 ? 0 : kDfSteps;
+    if (skip >= steps) continue;
+    Records<U::RW> records;
+    records.request(a.records, sh.e0 + (int64_t)first * w.slots, sh.e1, lane);
+    for (int b = first; b < steps; b += w.lanes) {
+      wave_lds();
+      records.put(rec, lane);
+      wave_lds();
+      if (b + w.lanes < steps) records.request(a.records, sh.e0 + (int64_t)(b + w.lanes) * w.slots, sh.e1, lane);
+      const int ends = steps - b < w.lanes ? steps - b : w.lanes;
+      for (int t = skip > b ? skip - b : 0; t < ends; t += UN) {
+        float k[UN][U::N], bias[UN], cs[UN][U::NO], sn[UN][U::NO], v[UN];
+#pragma unroll
+        for (int n = 0; n < UN; ++n) {
+          // a step past the batch takes its last record once more
+          const int at = t + n < w.lanes ? t + n : w.lanes - 1;
+          const float* r = rec + (at * w.slots + s) * U::RW;
+          const float2 head = *reinterpret_cast<const float2*>(r);
+          bias[n] = t + n < w.lanes ? head.y : neg_inf<float>();
+#pragma unroll
+          for (int o = 0; o < U::NO; ++o) {
+            const float2 x = *reinterpret_cast<const float2*>(r + 2 + 2 * o);
+            cs[n][o] = x.x;
+            sn[n][o] = x.y;
+          }
+          U::load(a.k + (int64_t)__float_as_int(head.x) * a.L.D, w, unit, k[n]);
+        }
+#pragma unroll
+        for (int n = 0; n < UN; ++n) {
+          const float d = sum_units(U::dot(q, k[n], cs[n], sn[n]), w.per_map);
+          v[n] = bias[n] == neg_inf<float>() ? neg_inf<float>() : fmaf(a.scale, d, bias[n]);
+        }
+        if (phase == 0) {
+#pragma unroll
+          for (int n = 0; n < UN; ++n) {
+            if (b + t + n < kDfSteps && t + n < w.lanes) sc[(b + t + n) * kWave] = v[n];
+            m = v[n] > m || v[n] != v[n] ? v[n] : m;
+          }
+        } else {
+          const float top = m == neg_inf<float>() ? 0.f : m;
+#pragma unroll
+          for (int n = 0; n < UN; ++n) {
+            v[n] = gm_exp(v[n] - top);
+            if (phase == 1) l += v[n];
+          }
+          if (phase == 2) {
+#pragma unroll
+            for (int n = 0; n < UN; n += 2)
+              if (t + n < w.lanes) write(b + t + n, v[n] * inv, v[n + 1] * inv);
+          }
+        }
+      }
+    }
+  }
+}
+
+// ---------------------------------------------------------------- backward
+
+// Sums over the wave's slots, then over a row's waves; the first wave's lanes of slot 0 hold them.
+template <int M>
+__device__ __forceinline__ void row_sums(const DfUnits& w, float (&v)[M], float* shared) {
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, waves = blockDim.x >> 6;
+#pragma unroll
+  for (int i = 0; i < M; ++i)
+    for (int o = w.lanes; o < kWave; o <<= 1) v[i] += __shfl_xor(v[i], o, kWave);
+  if (w.per_row == 1) return;
+  __syncthreads();  // the records have been read
+  if (lane < w.lanes) {
+#pragma unroll
+    for (int i = 0; i < M; ++i) shared[(wave * M + i) * w.lanes + lane] = v[i];
+  }
+  __syncthreads();
+  if (wave == 0 && lane < w.lanes) {
+    for (int o = 1; o < waves; ++o)
+#pragma unroll
+      for (int i = 0; i < M; ++i) v[i] += shared[(o * M + i) * w.lanes + lane];
+  }
+}
+
+// Per target, in one walk: T = sum a g, sum a g tau k and sum a tau k, of which dq = scale c (the second - T the third).
+template <typename R, int A0, int A1, int A2>
+__global__ __launch_bounds__(1024) void differential_backward_target_units(DfArgs<float, R> a, DfUnits w) {
+  using U = Unit<A0, A1, A2>;
+  constexpr int kWords = kWave * U::RW, UN = kDfInFlightB, M = 2 * U::N + 1;
+  extern __shared__ __align__(16) float df_lds[];
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const Share sh = share_of(w, a.row_ptr);
+  if (!sh.live) return;
+  float* rec = df_lds + wave * kWords;
+  const int u = lane & (w.lanes - 1), s = lane >> w.shift, unit = u < w.units ? u : w.units - 1;
+  const int p = unit / w.per_map;
+  float q[U::N];
+  U::load(a.q + sh.row * a.L.D, w, unit, q);
+  const float lse = a.lse[sh.row * a.L.P + p];
+  const int steps = (int)((sh.e1 - sh.e0 + w.slots - 1) / w.slots);
+  float sums[M];
+#pragma unroll
+  for (int i = 0; i < M; ++i) sums[i] = 0.f;
+  Records<U::RW> records;
+  if (steps > 0) records.request(a.records, sh.e0, sh.e1, lane);
+  for (int b = 0; b < steps; b += w.lanes) {
+    wave_lds();
+    records.put(rec, lane);
+    wave_lds();
+    if (b + w.lanes < steps) records.request(a.records, sh.e0 + (int64_t)(b + w.lanes) * w.slots, sh.e1, lane);
+    const int ends = steps - b < w.lanes ? steps - b : w.lanes;
+    for (int t = 0; t < ends; t += UN) {
+      float k[UN][U::N], bias[UN], cs[UN][U::NO], sn[UN][U::NO], g[UN];
+#pragma unroll
+      for (int n = 0; n < UN; ++n) {
+        const int at = t + n < w.lanes ? t + n : w.lanes - 1;
+        const float* r = rec + (at * w.slots + s) * U::RW;
+        const float2 head = *reinterpret_cast<const float2*>(r);
+        bias[n] = t + n < w.lanes ? head.y : neg_inf<float>();
+#pragma unroll
+        for (int o = 0; o < U::NO; ++o) {
+          const float2 x = *reinterpret_cast<const float2*>(r + 2 + 2 * o);
+          cs[n][o] = x.x;
+          sn[n][o] = x.y;
+        }
+        U::load(a.k + (int64_t)__float_as_int(head.x) * a.L.D, w, unit, k[n]);
+        const int64_t e = sh.e0 + (int64_t)(b + at) * w.slots + s;
+        g[n] = a.g[(e < sh.e1 ? e : sh.e0) * a.L.H + (p >> 1)];
+      }
+#pragma unroll
+      for (int n = 0; n < UN; ++n) {
+        const float d = sum_units(U::dot(q, k[n], cs[n], sn[n]), w.per_map);
+        if (bias[n] != neg_inf<float>()) {
+          const float al = gm_exp(fmaf(a.scale, d, bias[n]) - lse), ag = al * g[n];
+          U::turn(k[n], cs[n], sn[n], false);
+          sums[2 * U::N] += ag;
+#pragma unroll
+          for (int i = 0; i < U::N; ++i) {
+            sums[i] = fmaf(ag, k[n][i], sums[i]);
+            sums[U::N + i] = fmaf(al, k[n][i], sums[U::N + i]);
+          }
+        }
+      }
+    }
+  }
+  row_sums<M>(w, sums, df_lds);
+  if (sh.part == 0 && s == 0 && u < w.units) {
+    const float total = sums[2 * U::N];
+    const float factor = a.scale * ((p & 1) ? -a.lambda[p >> 1] : 1.f);
+    float dq[U::N];
+#pragma unroll
+    for (int i = 0; i < U::N; ++i) dq[i] = factor * (sums[i] - total * sums[U::N + i]);
+    U::store(a.dq + sh.row * a.L.D, w, unit, dq);
+    if (unit % w.per_map == 0)
+      *reinterpret_cast<float2*>(a.pairs + (sh.row * a.L.P + p) * 2) = make_float2(lse, total);
+  }
+}
+
+// Per source, over the edges sorted by source: dk = scale c sum a (g - T) conj(tau) q.
+template <typename R, int A0, int A1, int A2>
+__global__ __launch_bounds__(1024) void differential_backward_source_units(DfArgs<float, R> a, DfUnits w) {
+  using U = Unit<A0, A1, A2>;
+  constexpr int kWords = kWave * (U::RW + 2), UN = kDfInFlightB;
+  extern __shared__ __align__(16) float df_lds[];
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const Share sh = share_of(w, a.src_ptr);
+  if (!sh.live) return;
+  float* rec = df_lds + wave * kWords;
+  const int u = lane & (w.lanes - 1), s = lane >> w.shift, unit = u < w.units ? u : w.units - 1;
+  const int p = unit / w.per_map;
+  float k[U::N];
+  U::load(a.k + sh.row * a.L.D, w, unit, k);
+  const int steps = (int)((sh.e1 - sh.e0 + w.slots - 1) / w.slots);
+  float sums[U::N];
+#pragma unroll
+  for (int i = 0; i < U::N; ++i) sums[i] = 0.f;
+  Records<U::RW + 2> records;
+  if (steps > 0) records.request(a.records_s, sh.e0, sh.e1, lane);
+  for (int b = 0; b < steps; b += w.lanes) {
+    wave_lds();
+    records.put(rec, lane);
+    wave_lds();
+    if (b + w.lanes < steps) records.request(a.records_s, sh.e0 + (int64_t)(b + w.lanes) * w.slots, sh.e1, lane);
+    const int ends = steps - b < w.lanes ? steps - b : w.lanes;
+    for (int t = 0; t < ends; t += UN) {
+      float q[UN][U::N], bias[UN], cs[UN][U::NO], sn[UN][U::NO], g[UN];
+      float2 pair[UN];
+#pragma unroll
+      for (int n = 0; n < UN; ++n) {
+        const int at = t + n < w.lanes ? t + n : w.lanes - 1;
+        const float* r = rec + (at * w.slots + s) * (U::RW + 2);
+        const float2 head = *reinterpret_cast<const float2*>(r);
+        // past the row's end: node 0, edge -inf's bits -- the row's first edge instead
+        const bool in = sh.e0 + (int64_t)(b + t + n) * w.slots + s < sh.e1 && t + n < w.lanes;
+        bias[n] = in ? r[2] : neg_inf<float>();
+#pragma unroll
+        for (int o = 0; o < U::NO; ++o) {
+          const float2 x = *reinterpret_cast<const float2*>(r + 4 + 2 * o);
+          cs[n][o] = x.x;
+          sn[n][o] = x.y;
+        }
+        const int64_t i = __float_as_int(head.x), e = in ? __float_as_int(head.y) : 0;
+        U::load(a.q + i * a.L.D, w, unit, q[n]);
+        pair[n] = *reinterpret_cast<const float2*>(a.pairs + (i * a.L.P + p) * 2);
+        g[n] = a.g[e * a.L.H + (p >> 1)];
+      }
+#pragma unroll
+      for (int n = 0; n < UN; ++n) {
+        const float d = sum_units(U::dot(q[n], k, cs[n], sn[n]), w.per_map);
+        if (bias[n] != neg_inf<float>()) {
+          const float ds = gm_exp(fmaf(a.scale, d, bias[n]) - pair[n].x) * (g[n] - pair[n].y);
+          U::turn(q[n], cs[n], sn[n], true);
+#pragma unroll
+          for (int i = 0; i < U::N; ++i) sums[i] = fmaf(ds, q[n][i], sums[i]);
+        }
+      }
+    }
+  }
+  row_sums<U::N>(w, sums, df_lds);
+  if (sh.part == 0 && s == 0 && u < w.units) {
+    const float factor = a.scale * ((p & 1) ? -a.lambda[p >> 1] : 1.f);
+#pragma unroll
+    for (int i = 0; i < U::N; ++i) sums[i] *= factor;
+    U::store(a.dk + sh.row * a.L.D, w, unit, sums);
+  }
+}
+
+// ------------------------------------------------------------------ launch
+
+// The unit a map's copies (a0, a1, a2) are `per_map` of, a power of two of them; the widest that serves.
+struct UnitShape {
+  int a0, a1, a2;
+};
+constexpr UnitShape kShapes[] = {{4, 2, 1}, {2, 2, 2}, {2, 2, 0}, {2, 1, 1}, {1, 1, 1}, {1, 1, 0}};
+constexpr int kShapeCount = sizeof(kShapes) / sizeof(kShapes[0]);
+
+// The shape's index and the units a map, or -1.
+int find_shape(const DfLayout& L, int& per_map) {
+  if (L.F < 2 || L.F > 3 || L.orders != L.F) return -1;
+  for (int f = 0; f < L.F; ++f)
+    if (L.n[f] != f) return -1;
+  const int c[3] = {L.a[0], L.a[1], L.F == 3 ? L.a[2] : 0};
+  for (int i = 0; i < kShapeCount; ++i) {
+    const UnitShape& u = kShapes[i];
+    if ((u.a2 == 0) != (c[2] == 0)) continue;
+    for (per_map = 1; per_map * L.P <= kWave; per_map *= 2)
+      if (c[0] == per_map * u.a0 && c[1] == per_map * u.a1 && c[2] == per_map * u.a2) return i;
+  }
+  return -1;
+}
+
+int lanes_for(int units) {
+  int lanes = 1;
+  while (lanes < units) lanes *= 2;
+  return lanes;
+}
+
+// LDS words of a pass: the records a wave (and the forward's scores), or the waves' sums.
+template <typename U>
+size_t lds_bytes(DfPass pass, int waves, int lanes) {
+  size_t words = 0;
+  switch (pass) {
+    case DfPass::Forward: words = (size_t)waves * (kWave * U::RW + kDfSteps * kWave + (waves > 1 ? kWave : 0)); break;
+    case DfPass::BackwardTarget:
+      words = (size_t)waves * std::max(kWave * U::RW, (2 * U::N + 1) * lanes);
+      break;
+    case DfPass::BackwardSource: words = (size_t)waves * std::max(kWave * (U::RW + 2), U::N * lanes); break;
+  }
+  return words * sizeof(float);
+}
+
+template <typename R, int A0, int A1, int A2>
+int launch_shape(DfPass pass, const DfArgs<float, R>& a, DfUnits w, const DfRows& rows, hipStream_t stream) {
+  using U = Unit<A0, A1, A2>;
+  constexpr int kWaves[3] = {16, 4, 1};
+  const void* kernels[3] = {reinterpret_cast<const void*>(&differential_forward_units<R, A0, A1, A2>),
+                            reinterpret_cast<const void*>(&differential_backward_target_units<R, A0, A1, A2>),
+                            reinterpret_cast<const void*>(&differential_backward_source_units<R, A0, A1, A2>)};
+  w.first = 0;
+  for (int c = 0; c < 3; ++c) {
+    w.count = rows.count[c];
+    w.per_row = kWaves[c];
+    const int waves = c == 2 ? kWavesPerBlock : kWaves[c];
+    if (w.count > 0) {
+      const int64_t blocks = c == 2 ? blocks_for(w.count) : w.count;
+      const size_t lds = lds_bytes<U>(pass, waves, w.lanes);
+      if (lds > 64 * 1024 &&
+          hipFuncSetAttribute(kernels[(int)pass], hipFuncAttributeMaxDynamicSharedMemorySize, 160 * 1024) != hipSuccess)
+        return check_launch("differential (LDS)");
+      switch (pass) {
+        case DfPass::Forward:
+          hipLaunchKernelGGL((differential_forward_units<R, A0, A1, A2>), dim3((unsigned)blocks), dim3(waves * kWave),
+                             lds, stream, a, w);
+          break;
+        case DfPass::BackwardTarget:
+          hipLaunchKernelGGL((differential_backward_target_units<R, A0, A1, A2>), dim3((unsigned)blocks),
+                             dim3(waves * kWave), lds, stream, a, w);
+          break;
+        case DfPass::BackwardSource:
+          hipLaunchKernelGGL((differential_backward_source_units<R, A0, A1, A2>), dim3((unsigned)blocks),
+                             dim3(waves * kWave), lds, stream, a, w);
+          break;
+      }
+      const int rc = check_launch("differential");
+      if (rc != GM_OK) return rc;
+    }
+    w.first += w.count;
+  }
+  return GM_OK;
+}
+
+template <typename R>
+int launch_units(DfPass pass, const DfArgs<float, R>& a, const DfRows& rows, hipStream_t stream) {
+  DfUnits w{};
+  const int shape = find_shape(a.L, w.per_map);
+  if (shape < 0) return fail(GM_ERR_UNSUPPORTED, "differential: the lane kernels do not serve this layout");
+  w.units = a.L.P * w.per_map;
+  w.lanes = lanes_for(w.units);
+  while ((1 << w.shift) < w.lanes) ++w.shift;
+  w.slots = kWave / w.lanes;
+  w.base0 = a.L.off[0];
+  w.base1 = a.L.off[1];
+  w.base2 = a.L.F == 3 ? a.L.off[2] : 0;
+  w.order = rows.order;
+  switch (shape) {
+    case 0: return launch_shape<R, 4, 2, 1>(pass, a, w, rows, stream);
+    case 1: return launch_shape<R, 2, 2, 2>(pass, a, w, rows, stream);
+    case 2: return launch_shape<R, 2, 2, 0>(pass, a, w, rows, stream);
+    case 3: return launch_shape<R, 2, 1, 1>(pass, a, w, rows, stream);
+    case 4: return launch_shape<R, 1, 1, 1>(pass, a, w, rows, stream);
+    default: return launch_shape<R, 1, 1, 0>(pass, a, w, rows, stream);
+  }
+}
+
+}  // namespace
+
+// Every frequency's unit is loaded as one piece of 1, 2 or 4 numbers: the row's width and the frequency's offset are
+// multiples of it (and the table's address one of 16 bytes, which the entry points check).
+int df_slots(const DfLayout& L) {
+  int per_map = 0;
+  const int shape = find_shape(L, per_map);
+  if (shape < 0) return 0;
+  const UnitShape& u = kShapes[shape];
+  const int width[3] = {u.a0, 2 * u.a1, 2 * u.a2};
+  for (int f = 0; f < L.F; ++f)
+    if (L.off[f] % width[f] != 0 || L.D % width[f] != 0) return 0;
+  return kWave / lanes_for(L.P * per_map);
+}
+
+int df_launch_units(DfPass pass, const DfArgs<float, float>& a, const DfRows& rows, hipStream_t stream) {
+  return launch_units<float>(pass, a, rows, stream);
+}
+int df_launch_units(DfPass pass, const DfArgs<float, uint16_t>& a, const DfRows& rows, hipStream_t stream) {
+  return launch_units<uint16_t>(pass, a, rows, stream);
+}
+
+}  // namespace gm

@@ -112,9 +112,10 @@ SIGNATURES_F32 = {
     **{f"gm_gate_backward_{sfx}": (ctypes.c_int, [_P] * 3 + [_I] * 4 + [_P, _P, _I] + [_P] * 3)
        for sfx in ("f32", "f64", "bf16")},
     "gm_differential_partials": (ctypes.c_int64, [_I]),
-    **{f"gm_differential_forward_{sfx}": (ctypes.c_int, [_P] * 6 + [_I] * 7 + [_D] + [_P] * 3)
+    "gm_differential_slots": (ctypes.c_int, [_P] + [_I] * 4 + [_P]),
+    **{f"gm_differential_forward_{sfx}": (ctypes.c_int, [_P] * 8 + [_I] * 7 + [_D] + [_P] * 3)
        for sfx in ("f32", "f64", "bf16")},
-    **{f"gm_differential_backward_{sfx}": (ctypes.c_int, [_P] * 9 + [_I] * 7 + [_D] + [_P] * 8)
+    **{f"gm_differential_backward_{sfx}": (ctypes.c_int, [_P] * 13 + [_I] * 7 + [_D] + [_P] * 8)
        for sfx in ("f32", "f64", "bf16")},
     "gm_residual_norm_partial_rows": (ctypes.c_int64, [_I]),
     **{f"gm_residual_norm_forward_{sfx}": (ctypes.c_int, [_P] * 4 + [_I] * 4 + [_P, _P, _D, _D, _D] + [_P] * 4)
@@ -1643,7 +1644,7 @@ def residual_norm_backward(dy: Tensor | None, dn: Tensor | None, x: Tensor, u: T
 # ---------------------------------------------------------------- differential softmax
 
 
-def _differential_check(q: Tensor, k: Tensor, lam: Tensor, tables: Any, desc: Tensor, H: int) -> str:
+def _differential_check(q: Tensor, k: Tensor, lam: Tensor, tables: Any, maps: Any) -> str:
     """The differential softmax's suffix, its rows checked against the tables."""
     _require_device(q, k, lam, tables.records, tables.row_ptr)
     _check(q.dtype in _PW_SUFFIX and k.dtype == q.dtype, "q and k must share float32, float64 or bfloat16")
@@ -1651,45 +1652,56 @@ def _differential_check(q: Tensor, k: Tensor, lam: Tensor, tables: Any, desc: Te
     _check(tables.dtype == table and lam.dtype == table,
            "the tables and lam must be q's dtype (float32 for bfloat16 rows)")
     _check(q.dim() == 2 and k.dim() == 2 and q.shape[0] == tables.n_targets and k.shape[0] == tables.n_sources
-           and q.shape[1] == k.shape[1], "q must be (n_targets, D) and k (n_sources, D)")
-    _check(1 <= H <= 16 and tuple(lam.shape) == (H,), "lam must be (H,) with at most 16 heads")
-    _check(desc.device.type == "cpu" and desc.dtype == torch.int64 and desc.dim() == 2 and desc.shape[1] == 5
-           and desc.is_contiguous(), "desc must be a contiguous int64 (F, 5) host table")
+           and q.shape[1] == k.shape[1] == maps.plan.width, "q must be (n_targets, D) and k (n_sources, D)")
+    _check(tuple(lam.shape) == (maps.heads,), "lam must be (H,)")
+    _check(maps.top < tables.orders, "the maps need higher orders than the tables hold")
     return _PW_SUFFIX[q.dtype]
 
 
-def differential_forward(q: Tensor, k: Tensor, lam: Tensor, tables: Any, desc: Tensor, H: int, scale: float,
+def differential_slots(desc: Tensor, D: int, orders: int, H: int) -> int:
+    """The edge slots of a wave of the lane kernels, 0 where they do not serve the layout."""
+    slots = ctypes.c_int64(0)
+    _call("gm_differential_slots", desc.data_ptr(), desc.shape[0], H, D, orders, ctypes.addressof(slots))
+    return int(slots.value)
+
+
+def differential_forward(q: Tensor, k: Tensor, lam: Tensor, tables: Any, maps: Any, scale: float,
                          train: bool) -> tuple[Tensor, Tensor | None]:
     """``(alpha (n_edges, H), lse)``: the differential softmax's weights and, under ``train``,
     the log sums of exponentials ``(n_targets, 2 H)`` its backward reads."""
-    sfx = _differential_check(q, k, lam, tables, desc, H)
+    sfx = _differential_check(q, k, lam, tables, maps)
+    H, desc = maps.heads, maps.desc
+    order, counts = tables.target_rows(maps.slots(tables))
     tables.found()
     alpha = torch.empty(tables.n_edges, H, dtype=tables.dtype, device=q.device)
     lse = torch.empty(tables.n_targets, 2 * H, dtype=tables.dtype, device=q.device) if train else None
     with torch.cuda.device(q.device):
         _call(f"gm_differential_forward_{sfx}", _ptr(q), _ptr(k), _ptr(lam), _ptr(tables.records), desc.data_ptr(),
-              _ptr(tables.row_ptr), tables.n_targets, tables.n_sources, tables.n_edges, q.shape[1], tables.orders,
-              desc.shape[0], H, float(scale), _ptr(alpha), _ptr(lse), _stream(q.device))
+              _ptr(tables.row_ptr), _ptr(order), counts, tables.n_targets, tables.n_sources, tables.n_edges,
+              q.shape[1], tables.orders, desc.shape[0], H, float(scale), _ptr(alpha), _ptr(lse), _stream(q.device))
     return alpha, lse
 
 
-def differential_backward(g: Tensor, q: Tensor, k: Tensor, lam: Tensor, lse: Tensor, tables: Any, desc: Tensor,
-                          H: int, scale: float) -> tuple[Tensor, Tensor, Tensor]:
+def differential_backward(g: Tensor, q: Tensor, k: Tensor, lam: Tensor, lse: Tensor, tables: Any, maps: Any,
+                          scale: float) -> tuple[Tensor, Tensor, Tensor]:
     """``(dq, dk, dlam)``: the rows' gradients in their dtype, the factors' in the tables'; no atomics."""
-    sfx = _differential_check(q, k, lam, tables, desc, H)
+    sfx = _differential_check(q, k, lam, tables, maps)
+    H, desc, slots = maps.heads, maps.desc, maps.slots(tables)
     _check(g.dtype == tables.dtype and tuple(g.shape) == (tables.n_edges, H) and g.is_contiguous()
            and g.device == q.device, "g must be contiguous (n_edges, H) in the tables' dtype")
     _check(lse.dtype == tables.dtype and tuple(lse.shape) == (tables.n_targets, 2 * H) and lse.is_contiguous(),
            "lse must be the forward's")
     src_ptr, records_s = tables.group_sources()
+    (order, counts), (order_s, counts_s) = tables.target_rows(slots), tables.source_rows(slots)
     tables.found()
     pairs = torch.empty(tables.n_targets, 2 * H, 2, dtype=tables.dtype, device=q.device)
-    ds = torch.empty(tables.n_edges, 2 * H, dtype=tables.dtype, device=q.device)
+    # the simple kernels' workspace
+    ds = None if slots else torch.empty(tables.n_edges, 2 * H, dtype=tables.dtype, device=q.device)
     partial = torch.empty(int(library().gm_differential_partials(H)), dtype=torch.float64, device=q.device)
     dq, dk, dlam = torch.empty_like(q), torch.empty_like(k), torch.empty_like(lam)
     with torch.cuda.device(q.device):
         _call(f"gm_differential_backward_{sfx}", _ptr(g), _ptr(q), _ptr(k), _ptr(lam), _ptr(tables.records),
-              _ptr(records_s), desc.data_ptr(), _ptr(tables.row_ptr), _ptr(src_ptr), tables.n_targets,
-              tables.n_sources, tables.n_edges, q.shape[1], tables.orders, desc.shape[0], H, float(scale),
+              _ptr(records_s), desc.data_ptr(), _ptr(tables.row_ptr), _ptr(src_ptr), _ptr(order), counts,
+              _ptr(order_s), counts_s, tables.n_targets, tables.n_sources, tables.n_edges, q.shape[1], tables.orders, desc.shape[0], H, float(scale),
               _ptr(lse), _ptr(pairs), _ptr(ds), _ptr(partial), _ptr(dq), _ptr(dk), _ptr(dlam), _stream(q.device))
     return dq, dk, dlam

@@ -25,6 +25,7 @@ bfloat16 gradients, rounded once.  CPU tensors take the formulas in torch.
 
 from __future__ import annotations
 
+import ctypes
 import functools
 import math
 from typing import Any
@@ -79,7 +80,7 @@ class EdgeTables:
             raise ValueError("row_ptr must rise from 0 to n_edges and every source lie in 0 .. n_sources - 1.")
         self.device, self.dtype, self.orders = transport.device, transport.dtype, transport.shape[1]
         self.row_ptr = row_ptr.detach().clone()
-        self._sources = None
+        self._sources, self._classes = None, {}
         masked = bias.detach().masked_fill(inside == 0, -math.inf)
         phases = transport.detach()[:, 1:].reshape(n_edges, 2 * (self.orders - 1))
         if self.device.type != "cuda":
@@ -121,6 +122,37 @@ class EdgeTables:
         self._kept.append(_native.Made(src_ptr, records_s))
         return src_ptr, records_s
 
+    def target_rows(self, slots: int) -> tuple[Tensor | None, Any]:
+        """The targets in the classes of degree that the lane kernels with ``slots``
+        edge slots a wave take, and the classes' counts as the entry points read
+        them; ``(None, None)`` for ``slots`` 0, the simple kernels."""
+        return self._rows(("targets", slots), lambda: self.row_ptr)
+
+    def source_rows(self, slots: int) -> tuple[Tensor | None, Any]:
+        """The same of the sources and their edges."""
+        return self._rows(("sources", slots), lambda: self.group_sources()[0])
+
+    def _rows(self, key: tuple[str, int], ptr: Any) -> tuple[Tensor | None, Any]:
+        if key[1] == 0:
+            return None, None
+        held = self._classes.get(key)
+        if held is None:
+            with _native.LOCK:
+                held = self._classes.get(key)
+                if held is None:
+                    held = self._classes[key] = self._in_classes(ptr(), key[1])
+        return held
+
+    def _in_classes(self, ptr: Tensor, slots: int) -> tuple[Tensor, Any]:
+        _outside_capture(ptr, "EdgeTables' rows in classes (a first call with these tables and heads)")
+        self.found()
+        degree = ptr[1:] - ptr[:-1]
+        rank = (degree <= 128 * slots).to(torch.uint8) + (degree <= 32 * slots).to(torch.uint8)
+        order = torch.sort(rank, stable=True).indices.to(torch.int32)
+        counts = torch.stack([(rank == c).sum() for c in range(3)]).tolist()
+        self._kept.append(_native.Made(order))
+        return order, (ctypes.c_int64 * 3)(*counts)
+
     def found(self) -> None:
         """The current stream reads what is kept from here on."""
         for made in self._kept:
@@ -135,23 +167,36 @@ def _outside_capture(t: Tensor, what: str) -> None:
         raise RuntimeError(f"{what} waits for the device: build it before the capture.")
 
 
-@functools.lru_cache(maxsize=256)
-def maps_plan(map_type: SO2FieldType, heads: int) -> fused_attention.Plan:
-    """The descriptor rows of the rows' ``2 heads`` maps of ``map_type``."""
-    if not isinstance(map_type, SO2FieldType):
-        raise TypeError(f"map_type must be an SO2FieldType, got {type(map_type).__name__}.")
-    if not 1 <= heads <= MAX_H:
-        raise ValueError(f"heads must lie in 1..{MAX_H}, got {heads}.")
-    full = map_type.scaled(2 * heads)
-    if len(map_type) > MAX_F or full.dimension > MAX_D:
-        raise ValueError(f"the maps must hold at most {MAX_F} frequencies and {MAX_D} numbers a row, "
-                         f"got {full!r} ({full.dimension}).")
-    return fused_attention.plan_of(map_type, full, 2 * heads)
+class Maps:
+    """The rows' ``2 heads`` maps of ``map_type`` as the entry points take them."""
+
+    def __init__(self, map_type: SO2FieldType, heads: int) -> None:
+        if not isinstance(map_type, SO2FieldType):
+            raise TypeError(f"map_type must be an SO2FieldType, got {type(map_type).__name__}.")
+        if not 1 <= heads <= MAX_H:
+            raise ValueError(f"heads must lie in 1..{MAX_H}, got {heads}.")
+        full = map_type.scaled(2 * heads)
+        if len(map_type) > MAX_F or full.dimension > MAX_D:
+            raise ValueError(f"the maps must hold at most {MAX_F} frequencies and {MAX_D} numbers a row, "
+                             f"got {full!r} ({full.dimension}).")
+        self.heads, self.scale = heads, 1.0 / math.sqrt(map_type.dimension)
+        self.plan = fused_attention.plan_of(map_type, full, 2 * heads)
+        self.top = max(n for n, *_ in self.plan.rows)
+        self.desc = torch.tensor([list(row) for row in self.plan.rows], dtype=torch.int64)
+        self._slots: dict[int, int] = {}
+
+    def slots(self, tables: EdgeTables) -> int:
+        """Edge slots of a wave of the lane kernels (0: the simple kernels serve)."""
+        if tables.dtype == torch.float64:
+            return 0
+        held = self._slots.get(tables.orders)
+        if held is None:
+            held = self._slots[tables.orders] = _native.differential_slots(self.desc, self.plan.width, tables.orders,
+                                                                           self.heads)
+        return held
 
 
-@functools.lru_cache(maxsize=256)
-def _host_rows(map_type: SO2FieldType, heads: int) -> Tensor:
-    return torch.tensor([list(row) for row in maps_plan(map_type, heads).rows], dtype=torch.int64)
+maps_of = functools.lru_cache(maxsize=256)(Maps)
 
 
 class DifferentialSoftmax(torch.autograd.Function):
@@ -159,16 +204,16 @@ class DifferentialSoftmax(torch.autograd.Function):
     in the rows' dtype and ``dlam`` back."""
 
     @staticmethod
-    def forward(ctx: Any, q: Tensor, k: Tensor, lam: Tensor, tables: EdgeTables, desc: Tensor, heads: int,
-                scale: float) -> Tensor:
+    def forward(ctx: Any, q: Tensor, k: Tensor, lam: Tensor, tables: EdgeTables, maps: Maps, scale: float) -> Tensor:
         train = any(ctx.needs_input_grad)
-        if train:
-            tables.group_sources()  # here: the backward may be captured, or run on a thread and stream of its own
+        if train:  # found here: the backward runs on a thread and perhaps a stream of its own
+            tables.group_sources()
+            tables.source_rows(maps.slots(tables))
         with torch.profiler.record_function("gm::attention/differential_softmax"):
-            alpha, lse = _native.differential_forward(q, k, lam, tables, desc, heads, scale, train)
+            alpha, lse = _native.differential_forward(q, k, lam, tables, maps, scale, train)
         if train:
             ctx.save_for_backward(q, k, lam, lse)
-            ctx.rest = (tables, desc, heads, scale)
+            ctx.rest = (tables, maps, scale)
         return alpha
 
     @staticmethod
@@ -177,7 +222,7 @@ class DifferentialSoftmax(torch.autograd.Function):
         q, k, lam, lse = ctx.saved_tensors
         with torch.profiler.record_function("gm::attention/differential_softmax_backward"):
             dq, dk, dlam = _native.differential_backward(grad_alpha.contiguous(), q, k, lam, lse, *ctx.rest)
-        return dq, dk, dlam, None, None, None, None
+        return dq, dk, dlam, None, None, None
 
 
 def differential_softmax(q: Tensor, k: Tensor, lam: Tensor, tables: EdgeTables, map_type: SO2FieldType, heads: int,
@@ -185,26 +230,31 @@ def differential_softmax(q: Tensor, k: Tensor, lam: Tensor, tables: EdgeTables, 
     """The heads' attention weights ``(n_edges, heads)`` of ``q (n_targets, D)`` and
     ``k (n_sources, D)``, rows of ``2 heads`` maps of ``map_type``, under ``lam
     (heads,)``; ``scale`` is ``1 / sqrt(dim map_type)`` by default."""
-    plan = maps_plan(map_type, heads)
+    maps = maps_of(map_type, heads)
+    width = maps.plan.width
     table = torch.float32 if q.dtype == torch.bfloat16 else q.dtype
     if table != tables.dtype or k.dtype != q.dtype:
         raise ValueError(f"q and k must share a dtype, {tables.dtype} (or bfloat16 with float32 tables), "
                          f"got {q.dtype} and {k.dtype}.")
-    if tuple(q.shape) != (tables.n_targets, plan.width) or tuple(k.shape) != (tables.n_sources, plan.width):
-        raise ValueError(f"q and k must be ({tables.n_targets}, {plan.width}) and ({tables.n_sources}, {plan.width}), "
+    if tuple(q.shape) != (tables.n_targets, width) or tuple(k.shape) != (tables.n_sources, width):
+        raise ValueError(f"q and k must be ({tables.n_targets}, {width}) and ({tables.n_sources}, {width}), "
                          f"got {tuple(q.shape)} and {tuple(k.shape)}.")
     if tuple(lam.shape) != (heads,):
         raise ValueError(f"lam must be ({heads},), got {tuple(lam.shape)}.")
     if any(t.device != tables.device for t in (q, k, lam)):
         raise ValueError("q, k and lam must live on the tables' device.")
-    top = max((n for n, *_ in plan.rows), default=0)
-    if top >= tables.orders:
-        raise ValueError(f"the tables hold orders below {tables.orders}, the maps need {top}.")
-    scale = 1.0 / math.sqrt(map_type.dimension) if scale is None else float(scale)
+    if maps.top >= tables.orders:
+        raise ValueError(f"the tables hold orders below {tables.orders}, the maps need {maps.top}.")
+    scale = maps.scale if scale is None else float(scale)
     if q.device.type != "cuda":
-        return _eager(q, k, lam, tables, plan, scale)
-    return DifferentialSoftmax.apply(q.contiguous(), k.contiguous(), lam.to(table).contiguous(), tables,
-                                     _host_rows(map_type, heads), heads, scale)
+        return _eager(q, k, lam, tables, maps.plan, scale)
+    return DifferentialSoftmax.apply(_whole(q), _whole(k), lam.to(table).contiguous(), tables, maps, scale)
+
+
+def _whole(rows: Tensor) -> Tensor:
+    """Contiguous rows at a multiple of 16 bytes, as the lane kernels load them."""
+    rows = rows.contiguous()
+    return rows if rows.data_ptr() % 16 == 0 else rows.clone()
 
 
 def _eager(q: Tensor, k: Tensor, lam: Tensor, tables: EdgeTables, plan: fused_attention.Plan, scale: float) -> Tensor:

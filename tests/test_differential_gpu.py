@@ -509,7 +509,7 @@ def test_the_oracle_is_the_single_softmax_at_lambda_zero():
     graph = Graph(t.row_ptr, t.source, t.transport[:, :3], t.bias, t.inside, t.n_nodes, torch.float64)
     q, k, _, g = inputs(graph, copies, heads, torch.float64)
     want = oracle(graph, q, k, torch.zeros(heads, dtype=torch.float64), g, copies, heads, 1e-16)["alpha"][0]
-    plan = differential.maps_plan(SO2FieldType(copies), heads)
+    plan = differential.maps_of(SO2FieldType(copies), heads).plan
     single = eager.softmax_op(q, k, graph.transport, graph.bias, graph.inside, plan.rows, graph.row_ptr, graph.source,
                               2 * heads, 10 ** -0.5)
     torch.testing.assert_close(want, single[:, 0::2], rtol=1e-12, atol=1e-14)
@@ -565,8 +565,9 @@ def test_the_library_refuses_bad_arguments():
     def forward(rows=((0, 2, 0, 0, 1), (1, 1, 8, 0, 2)), n=0, D=16, orders=2, H=2, F=None):
         flat = [x for row in rows for x in row]
         desc = (ctypes.c_int64 * len(flat))(*flat)
-        return lib.gm_differential_forward_f32(None, None, None, None, ctypes.cast(desc, ctypes.c_void_p), None, n, 0,
-                                               0, D, orders, len(rows) if F is None else F, H, 1.0, None, None, None)
+        return lib.gm_differential_forward_f32(None, None, None, None, ctypes.cast(desc, ctypes.c_void_p), None, None,
+                                               None, n, 0, 0, D, orders, len(rows) if F is None else F, H, 1.0, None,
+                                               None, None)
 
     assert forward() == 0
     for kw, message in ((dict(n=-1), b"non-negative"), (dict(n=1), b"device pointers"),
