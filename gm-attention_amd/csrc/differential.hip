@@ -19,9 +19,10 @@
 // targets.  No atomics: sums are in a fixed order.
 //
 // Per edge both passes read one record of 32-bit words (64-bit for double): the
-// other node, the bias (-inf outside the window) and the transport's (cos, sin) of
-// orders 1 .., packed once for an edge set; the source side's, in the order of the
-// edges sorted by source, name the edge too, whose g they read.
+// other node, the bias (in units of log 2, as the scores here; -inf outside the
+// window) and the transport's (cos, sin) of orders 1 .., packed once for an edge
+// set; the source side's, in the order of the edges sorted by source, name the edge
+// too, whose g they read.
 #include "differential.hpp"
 
 namespace gm {
@@ -42,8 +43,8 @@ __device__ __forceinline__ int64_t node_of(const T* word) {
 }
 
 // ------------------------------------------------------------- generic path
-// Any layout within the bounds: lanes (edge slot, map) over a target's edges, two
-// walks (the online sums, the weights); gradients of rows by a lane a column.
+// Any layout within the bounds: lanes (edge slot, map) over a target's edges, three
+// walks (the maxima, the sums, the weights); gradients of rows by a lane a column.
 
 template <typename T, typename R>
 __device__ T generic_map_score(const DfArgs<T, R>& a, const R* qi, const R* kj, const T* phases, int p) {
@@ -77,6 +78,19 @@ __device__ __forceinline__ T generic_logit(const DfArgs<T, R>& a, const R* qi, i
   return a.scale * generic_map_score(a, qi, a.k + node_of(rec) * a.L.D, rec + 2, p) + bias;
 }
 
+// Maximum over lanes h, h + G, ...: as group_sum.
+template <typename T>
+__device__ __forceinline__ T group_max(T v, int lane, int G, int S) {
+  const int s = lane / G, h = lane % G;
+  if (s >= S) v = neg_inf<T>();
+  for (int step = 1; step < S; step <<= 1) {
+    const int from = lane + step * G;
+    const T o = __shfl(v, from < kWave ? from : lane, kWave);
+    if ((s % (2 * step)) == 0 && s + step < S) v = o > v ? o : v;
+  }
+  return __shfl(v, h, kWave);
+}
+
 template <typename T, typename R>
 __global__ __launch_bounds__(256) void differential_forward_generic(DfArgs<T, R> a) {
   const int lane = threadIdx.x & 63;
@@ -87,17 +101,26 @@ __global__ __launch_bounds__(256) void differential_forward_generic(DfArgs<T, R>
   const R* qi = a.q + i * a.L.D;
   T m = neg_inf<T>(), l = T(0);
   if (s < S)
-    for (int64_t e = e0 + s; e < e1; e += S) online_add(m, l, generic_logit(a, qi, e, p));
-  group_online(m, l, lane, P, S);
-  const T inv = m == neg_inf<T>() ? T(0) : T(1) / l;
-  if (a.lse && lane < P) a.lse[i * P + p] = m + df_log(l);
+    for (int64_t e = e0 + s; e < e1; e += S) {
+      const T lw = generic_logit(a, qi, e, p);
+      m = lw > m ? lw : m;
+    }
+  m = group_max(m, lane, P, S);
+  if (s < S)
+    for (int64_t e = e0 + s; e < e1; e += S) {
+      const T lw = generic_logit(a, qi, e, p);
+      if (lw != neg_inf<T>()) l += df_exp2(lw - m);
+    }
+  l = group_sum(l, lane, P, S);
+  const T inv = l == T(0) ? T(0) : T(1) / l;
+  if (a.lse && lane < P) a.lse[i * P + p] = l == T(0) ? neg_inf<T>() : m + df_log2(l);
   const T lambda = a.lambda[p >> 1];
   for (int64_t e = e0; e < e1; e += S) {  // whole waves: the pair's second map comes by a shuffle
     const bool live = s < S && e + s < e1;
     T w = T(0);
     if (live) {
       const T lw = generic_logit(a, qi, e + s, p);
-      if (lw != neg_inf<T>()) w = gm_exp(lw - m) * inv;
+      if (lw != neg_inf<T>()) w = df_exp2(lw - m) * inv;
     }
     const T other = __shfl(w, lane | 1, kWave);
     if (live && (p & 1) == 0) a.alpha[(e + s) * a.L.H + (p >> 1)] = w - lambda * other;
@@ -118,7 +141,7 @@ __global__ __launch_bounds__(256) void differential_backward_scores_generic(DfAr
   if (s < S)
     for (int64_t e = e0 + s; e < e1; e += S) {
       const T lw = generic_logit(a, qi, e, p);
-      const T w = lw == neg_inf<T>() ? T(0) : gm_exp(lw - lse);
+      const T w = lw == neg_inf<T>() ? T(0) : df_exp2(lw - lse);
       if (lw != neg_inf<T>()) total += w * a.g[e * a.L.H + (p >> 1)];
       a.ds[e * P + p] = w;
     }
@@ -127,7 +150,7 @@ __global__ __launch_bounds__(256) void differential_backward_scores_generic(DfAr
     a.pairs[(i * P + p) * 2] = lse;
     a.pairs[(i * P + p) * 2 + 1] = total;
   }
-  const T factor = a.scale * ((p & 1) ? -a.lambda[p >> 1] : T(1));
+  const T factor = a.gradient_scale * ((p & 1) ? -a.lambda[p >> 1] : T(1));
   if (s < S)
     for (int64_t e = e0 + s; e < e1; e += S) {
       const T w = a.ds[e * P + p];
@@ -287,7 +310,9 @@ int df_prepare(DfArgs<T, R>& a, const R* q, const R* k, const T* lambda, const T
   a.row_ptr = row_ptr;
   a.n_targets = n_targets;
   a.n_sources = n_sources;
-  a.scale = (T)scale;
+  a.n_edges = n_edges;
+  a.scale = (T)(scale * kLog2e);
+  a.gradient_scale = (T)scale;
   return GM_OK;
 }
 

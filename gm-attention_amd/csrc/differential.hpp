@@ -30,23 +30,29 @@ struct DfArgs {
   const R* q;
   const R* k;
   const T* lambda;         // (H)
-  const T* records;        // (n_edges, 2 orders): other node, bias, (cos, sin) of orders 1 ..
+  const T* records;        // (n_edges, 2 orders): other node, bias / log 2, (cos, sin) of orders 1 ..
   const T* records_s;      // (n_edges, 2 + 2 orders): target, edge, bias, 0, (cos, sin) of orders 1 ..
   const int64_t* row_ptr;  // over targets
   const int64_t* src_ptr;  // over sources
   const T* g;              // (n_edges, H)
   T* alpha;                // (n_edges, H)
-  T* lse;                  // (n_targets, 2 H): log sum exp (-inf where no edge is inside)
+  T* lse;                  // (n_targets, 2 H): log2 sum 2^s (-inf where no edge is inside)
   T* pairs;                // (n_targets, 2 H, 2): that beside T, the backward's workspace
   T* ds;                   // (n_edges, 2 H): the generic backward's workspace
   R* dq;
   R* dk;
-  int64_t n_targets, n_sources;
-  T scale;
+  int64_t n_targets, n_sources, n_edges;
+  T scale;           // of the scores, in units of log 2
+  T gradient_scale;  // of the scores
 };
 
-__device__ __forceinline__ float df_log(float x) { return logf(x); }
-__device__ __forceinline__ double df_log(double x) { return log(x); }
+// Scores, their biases and their log sums are in units of log 2: a weight is 2^(s - lse).
+constexpr double kLog2e = 1.4426950408889634074;
+
+__device__ __forceinline__ float df_log2(float x) { return log2f(x); }
+__device__ __forceinline__ double df_log2(double x) { return log2(x); }
+__device__ __forceinline__ float df_exp2(float x) { return exp2f(x); }
+__device__ __forceinline__ double df_exp2(double x) { return exp2(x); }
 __device__ __forceinline__ float df_widen(float x) { return x; }
 __device__ __forceinline__ double df_widen(double x) { return x; }
 __device__ __forceinline__ float df_widen(uint16_t x) { return __uint_as_float((uint32_t)x << 16); }

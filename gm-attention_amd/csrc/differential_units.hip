@@ -23,16 +23,26 @@ namespace {
 constexpr int kDfSteps = 32;     // steps of a wave whose scores LDS holds: 32 S edges
 constexpr int kDfInFlight = 4;   // the forward's steps whose rows are requested together
 constexpr int kDfInFlightB = 2;  // the backward's
+constexpr int kDfMinLanes = 4;   // a batch of 64 edges is whole groups of those steps
 
 struct DfUnits {
   int units, per_map;    // lanes of an edge that hold something; units a map
-  int lanes, shift;      // units rounded up to a power of two; log2
+  int lanes, shift;      // units rounded up to a power of two, four at least; log2
   int slots;             // 64 / lanes
-  int base0, base1, base2;
+  int base[3];           // the frequencies' flat offsets
+  uint32_t row_bytes;
   const int32_t* order;
   int64_t first, count;  // rows order[first .. first + count)
   int per_row;           // waves a row: 1 (four rows a workgroup) or the workgroup's
 };
+
+__device__ __forceinline__ int uniform(int v) { return __builtin_amdgcn_readfirstlane(v); }
+__device__ __forceinline__ int64_t uniform(int64_t v) {
+  const uint32_t lo = (uint32_t)uniform((int)(uint32_t)v), hi = (uint32_t)uniform((int)(v >> 32));
+  return (int64_t)(((uint64_t)hi << 32) | lo);
+}
+// A weight: one v_exp_f32 (a step off; zero below the smallest normal number).
+__device__ __forceinline__ float exp2_of(float x) { return __builtin_amdgcn_exp2f(x); }
 
 // W numbers of a row at p.
 template <int W>
@@ -101,17 +111,31 @@ struct Unit {
   static constexpr int NO = A2 > 0 ? 2 : 1;  // orders above 0
   static constexpr int RW = 2 + 2 * NO;      // a record's words; the sources' two more
 
-  template <typename R>
-  static __device__ __forceinline__ void load(const R* row, const DfUnits& w, int unit, float (&v)[N]) {
-    load_w<W0>(row + w.base0 + unit * W0, v);
-    load_w<W1>(row + w.base1 + unit * W1, v + W0);
-    if constexpr (W2 > 0) load_w<W2>(row + w.base2 + unit * W2, v + W0 + W1);
+  // A unit of node `node`'s row.  kNear: the table is below 4 GB and 2^24 rows, so a lane's place in it is a 24-bit
+  // product and a 32-bit offset from a scalar address (the 64-bit form was a third of a step's instructions).
+  template <bool kNear, typename R>
+  static __device__ __forceinline__ void load(const R* rows, const DfUnits& w, int unit, int node, float (&v)[N]) {
+    if constexpr (kNear) {
+      const uint32_t row = __umul24((uint32_t)node, w.row_bytes);
+      auto at = [&](int f, int width) {
+        return reinterpret_cast<const R*>(reinterpret_cast<const char*>(rows + w.base[f]) +
+                                          (row + (uint32_t)(unit * width) * (uint32_t)sizeof(R)));
+      };
+      load_w<W0>(at(0, W0), v);
+      load_w<W1>(at(1, W1), v + W0);
+      if constexpr (W2 > 0) load_w<W2>(at(2, W2), v + W0 + W1);
+    } else {
+      const R* row = reinterpret_cast<const R*>(reinterpret_cast<const char*>(rows) + (int64_t)node * w.row_bytes);
+      load_w<W0>(row + w.base[0] + unit * W0, v);
+      load_w<W1>(row + w.base[1] + unit * W1, v + W0);
+      if constexpr (W2 > 0) load_w<W2>(row + w.base[2] + unit * W2, v + W0 + W1);
+    }
   }
   template <typename R>
   static __device__ __forceinline__ void store(R* row, const DfUnits& w, int unit, const float (&v)[N]) {
-    store_w<W0>(row + w.base0 + unit * W0, v);
-    store_w<W1>(row + w.base1 + unit * W1, v + W0);
-    if constexpr (W2 > 0) store_w<W2>(row + w.base2 + unit * W2, v + W0 + W1);
+    store_w<W0>(row + w.base[0] + unit * W0, v);
+    store_w<W1>(row + w.base[1] + unit * W1, v + W0);
+    if constexpr (W2 > 0) store_w<W2>(row + w.base[2] + unit * W2, v + W0 + W1);
   }
   // Re< q, tau k >: per order cos sum (q0 k0 + q1 k1) + sin sum (q1 k0 - q0 k1)
   static __device__ __forceinline__ float dot(const float (&q)[N], const float (&k)[N], const float (&cs)[NO],
@@ -153,7 +177,7 @@ template <int WORDS>
 struct Records {
   static constexpr int kLoads = WORDS / 2;
   float2 next[kLoads];
-  // request the records of edges [base, min(base + 64, end)); what lies past them is an edge outside the window of node 0
+  // request the records of edges [base, min(base + 64, end)); past them: edges of node 0 outside the window
   __device__ __forceinline__ void request(const float* records, int64_t base, int64_t end, int lane) {
     const int64_t left = end - base;
     const int pieces = (int)(left < kWave ? left : kWave) * kLoads;
@@ -177,78 +201,90 @@ __device__ __forceinline__ void wave_lds() {
   __builtin_amdgcn_wave_barrier();
 }
 
-__device__ __forceinline__ float sum_units(float v, int per_map) {
-  for (int o = 1; o < per_map; o <<= 1) v += __shfl_xor(v, o, kWave);
-  return v;
+// A map's units added, for the steps at hand.
+template <int UN>
+__device__ __forceinline__ void sum_units(float (&v)[UN], int per_map) {
+  if (per_map > 1) {
+    for (int o = 1; o < per_map; o <<= 1) {
+#pragma unroll
+      for (int n = 0; n < UN; ++n) v[n] += __shfl_xor(v[n], o, kWave);
+    }
+  }
 }
 
-// Which row a wave works on, and which of its edges.
+// Which row a wave works on, and which of its edges; all of it scalar.
 struct Share {
-  int64_t row, e0, e1;  // the row; this wave's edges
-  int part;
+  int64_t e0, e1;  // this wave's edges
+  int row, wave, part, steps;
   bool live;
 };
 __device__ __forceinline__ Share share_of(const DfUnits& w, const int64_t* ptr) {
-  const int wave = threadIdx.x >> 6, waves = blockDim.x >> 6;
-  const int64_t at = xcd_spread_block(blockIdx.x, gridDim.x) * (waves / w.per_row) + wave / w.per_row;
   Share s;
-  s.part = wave % w.per_row;
+  s.wave = uniform((int)(threadIdx.x >> 6));
+  const int rows = w.per_row == 1 ? kWavesPerBlock : 1;  // of a workgroup
+  const int64_t at = xcd_spread_block(blockIdx.x, gridDim.x) * rows + (w.per_row == 1 ? s.wave : 0);
+  s.part = w.per_row == 1 ? 0 : s.wave;
   s.live = at < w.count;
-  s.row = s.live ? w.order[w.first + at] : 0;
-  const int64_t e0 = s.live ? ptr[s.row] : 0, e1 = s.live ? ptr[s.row + 1] : 0;
-  const int64_t steps = (e1 - e0 + w.slots - 1) / w.slots;
-  const int64_t per = (steps + w.per_row - 1) / w.per_row * w.slots;
+  s.row = s.live ? uniform((int)w.order[w.first + at]) : 0;
+  const int64_t e0 = s.live ? uniform(ptr[s.row]) : 0, e1 = s.live ? uniform(ptr[s.row + 1]) : 0;
+  const int64_t steps = (e1 - e0 + w.slots - 1) >> (6 - w.shift);
+  const int64_t per = (w.per_row == 1 ? steps : (steps + w.per_row - 1) / w.per_row) << (6 - w.shift);
   s.e0 = e0 + s.part * per < e1 ? e0 + s.part * per : e1;
   s.e1 = s.e0 + per < e1 ? s.e0 + per : e1;
+  s.steps = (int)((s.e1 - s.e0 + w.slots - 1) >> (6 - w.shift));
   return s;
 }
 
 // ---------------------------------------------------------------- forward
 
-template <typename R, int A0, int A1, int A2>
+template <typename R, int A0, int A1, int A2, bool kNear>
 __global__ __launch_bounds__(1024) void differential_forward_units(DfArgs<float, R> a, DfUnits w) {
   using U = Unit<A0, A1, A2>;
   constexpr int kWords = kWave * U::RW, UN = kDfInFlight;
   extern __shared__ __align__(16) float df_lds[];
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, waves = blockDim.x >> 6;
   const Share sh = share_of(w, a.row_ptr);
   if (!sh.live) return;  // one wave a row, or the whole workgroup
-  float* rec = df_lds + wave * (kWords + kDfSteps * kWave);
+  const int lane = threadIdx.x & 63, waves = blockDim.x >> 6;
+  float* rec = df_lds + sh.wave * (kWords + kDfSteps * kWave);
   float* sc = rec + kWords + lane;
   float* shared = df_lds + waves * (kWords + kDfSteps * kWave);  // (waves, 64): the waves' maxima, then sums
   const int u = lane & (w.lanes - 1), s = lane >> w.shift, unit = u < w.units ? u : w.units - 1;
   const int p = unit / w.per_map;
+  const float* mine = rec + s * U::RW;  // this lane's edge of step 0
   float q[U::N];
-  U::load(a.q + sh.row * a.L.D, w, unit, q);
-  const float lambda = a.lambda[p >> 1];
+  U::template load<false>(a.q, w, unit, sh.row, q);
+  const float lambda = a.lambda[p >> 1], scale = a.scale;
   const bool second = p & 1, writes = u < w.units && unit % w.per_map == 0;
-  const int steps = (int)((sh.e1 - sh.e0 + w.slots - 1) / w.slots);
-  const int held = steps < kDfSteps ? steps : kDfSteps;
+  const int held = sh.steps < kDfSteps ? sh.steps : kDfSteps;
   float m = neg_inf<float>(), l = 0.f, inv = 0.f;
 
+  // over a lane's slots and the row's waves.  A score that is not a number is not a maximum; its exponential makes the
+  // sum, and with it the row, not a number.
   auto over_waves = [&](float v, bool maximum) {
     for (int o = w.lanes; o < kWave; o <<= 1) {
       const float x = __shfl_xor(v, o, kWave);
-      v = maximum ? (x > v || x != x ? x : v) : v + x;
+      v = maximum ? fmaxf(x, v) : v + x;
     }
     if (w.per_row > 1) {
       __syncthreads();
-      shared[wave * kWave + lane] = v;
+      shared[sh.wave * kWave + lane] = v;
       __syncthreads();
       v = shared[lane];
       for (int o = 1; o < waves; ++o) {
         const float x = shared[o * kWave + lane];
-        v = maximum ? (x > v || x != x ? x : v) : v + x;
+        v = maximum ? fmaxf(x, v) : v + x;
       }
     }
     return v;
   };
-  // two steps' weights: the pair of maps' lanes exchange one each and write one edge each
-  auto write = [&](int t, float w0, float w1) {
+  // steps t and t + 1 of the edges from `e`: the lanes of a pair of maps exchange a weight and write an edge each
+  const int ahead = writes ? (second ? w.slots : 0) + s : INT32_MAX;
+  const uint32_t place = (uint32_t)(ahead * a.L.H + (p >> 1));
+  auto write = [&](int64_t e, int t, float w0, float w1) {
     const float other = __shfl_xor(second ? w0 : w1, w.per_map, kWave);
-    const int64_t e = sh.e0 + (int64_t)(t + (second ? 1 : 0)) * w.slots + s;
     const float v = second ? other - lambda * w1 : w0 - lambda * other;
-    if (writes && e < sh.e1) a.alpha[e * a.L.H + (p >> 1)] = v;
+    float* to = a.alpha + (e + t * w.slots) * a.L.H;
+    if (ahead < (int)(sh.e1 - e) - t * w.slots) to[place] = v;
   };
 
   // phase 0: every score, its maximum; the first kDfSteps steps' stay in LDS.  The steps past them are scored again
@@ -256,9 +292,9 @@ __global__ __launch_bounds__(1024) void differential_forward_units(DfArgs<float,
   for (int phase = 0; phase < 3; ++phase) {
     if (phase == 1) {
       m = over_waves(m, true);
-      const float top = m == neg_inf<float>() ? 0.f : m;  // no edge inside: exp(-inf) = 0 everywhere
+      m = m == neg_inf<float>() ? 0.f : m;  // no edge inside: exp(-inf) = 0 everywhere
       for (int t = 0; t < held; ++t) {
-        const float x = gm_exp(sc[t * kWave] - top);
+        const float x = exp2_of(sc[t * kWave] - m);
         sc[t * kWave] = x;
         l += x;
       }
@@ -267,62 +303,60 @@ __global__ __launch_bounds__(1024) void differential_forward_units(DfArgs<float,
       l = over_waves(l, false);
       inv = l == 0.f ? 0.f : 1.f / l;
       if (a.lse && sh.part == 0 && s == 0 && writes)
-        a.lse[sh.row * a.L.P + p] = l == 0.f ? neg_inf<float>() : m + df_log(l);
-      for (int t = 0; t < held; t += 2) {
-        const float w0 = sc[t * kWave] * inv, w1 = t + 1 < held ? sc[(t + 1) * kWave] * inv : 0.f;
-        write(t, w0, w1);
-      }
+        a.lse[(int64_t)sh.row * a.L.P + p] = l == 0.f ? neg_inf<float>() : m + log2f(l);
+      for (int t = 0; t < held; t += 2)
+        write(sh.e0, t, sc[t * kWave] * inv, t + 1 < held ? sc[(t + 1) * kWave] * inv : 0.f);
     }
-    const int first = phase == 0 ? 0 : kDfSteps / w.lanes * w.lanes;  // a batch's first step
     const int skip = phase == 0 ? 0 : kDfSteps;
-    if (skip >= steps) continue;
+    if (skip >= sh.steps) continue;
+    const int first = skip & ~(w.lanes - 1);  // a batch's first step
     Records<U::RW> records;
     records.request(a.records, sh.e0 + (int64_t)first * w.slots, sh.e1, lane);
-    for (int b = first; b < steps; b += w.lanes) {
+    for (int b = first; b < sh.steps; b += w.lanes) {
+      const int64_t e = sh.e0 + (int64_t)b * w.slots;  // the batch's first edge
       wave_lds();
       records.put(rec, lane);
       wave_lds();
-      if (b + w.lanes < steps) records.request(a.records, sh.e0 + (int64_t)(b + w.lanes) * w.slots, sh.e1, lane);
-      const int ends = steps - b < w.lanes ? steps - b : w.lanes;
+      if (b + w.lanes < sh.steps) records.request(a.records, e + kWave, sh.e1, lane);
+      const int ends = sh.steps - b < w.lanes ? sh.steps - b : w.lanes;
       for (int t = skip > b ? skip - b : 0; t < ends; t += UN) {
-        float k[UN][U::N], bias[UN], cs[UN][U::NO], sn[UN][U::NO], v[UN];
+        float2 head[UN];
+        float k[UN][U::N], cs[UN][U::NO], sn[UN][U::NO], v[UN];
 #pragma unroll
         for (int n = 0; n < UN; ++n) {
-          // a step past the batch takes its last record once more
-          const int at = t + n < w.lanes ? t + n : w.lanes - 1;
-          const float* r = rec + (at * w.slots + s) * U::RW;
-          const float2 head = *reinterpret_cast<const float2*>(r);
-          bias[n] = t + n < w.lanes ? head.y : neg_inf<float>();
+          const float* r = mine + (t + n) * w.slots * U::RW;
+          head[n] = *reinterpret_cast<const float2*>(r);
 #pragma unroll
           for (int o = 0; o < U::NO; ++o) {
             const float2 x = *reinterpret_cast<const float2*>(r + 2 + 2 * o);
             cs[n][o] = x.x;
             sn[n][o] = x.y;
           }
-          U::load(a.k + (int64_t)__float_as_int(head.x) * a.L.D, w, unit, k[n]);
         }
 #pragma unroll
-        for (int n = 0; n < UN; ++n) {
-          const float d = sum_units(U::dot(q, k[n], cs[n], sn[n]), w.per_map);
-          v[n] = bias[n] == neg_inf<float>() ? neg_inf<float>() : fmaf(a.scale, d, bias[n]);
-        }
+        for (int n = 0; n < UN; ++n) U::template load<kNear>(a.k, w, unit, __float_as_int(head[n].x), k[n]);
+#pragma unroll
+        for (int n = 0; n < UN; ++n) v[n] = U::dot(q, k[n], cs[n], sn[n]);
+        sum_units<UN>(v, w.per_map);
+#pragma unroll
+        for (int n = 0; n < UN; ++n)  // outside the window: excluded, whatever its row holds
+          v[n] = head[n].y == neg_inf<float>() ? neg_inf<float>() : fmaf(scale, v[n], head[n].y);
         if (phase == 0) {
 #pragma unroll
-          for (int n = 0; n < UN; ++n) {
-            if (b + t + n < kDfSteps && t + n < w.lanes) sc[(b + t + n) * kWave] = v[n];
-            m = v[n] > m || v[n] != v[n] ? v[n] : m;
+          for (int n = 0; n < UN; ++n) m = fmaxf(m, v[n]);
+          if (b + t < kDfSteps) {
+#pragma unroll
+            for (int n = 0; n < UN; ++n) sc[(b + t + n) * kWave] = v[n];
           }
         } else {
-          const float top = m == neg_inf<float>() ? 0.f : m;
 #pragma unroll
-          for (int n = 0; n < UN; ++n) {
-            v[n] = gm_exp(v[n] - top);
-            if (phase == 1) l += v[n];
-          }
-          if (phase == 2) {
+          for (int n = 0; n < UN; ++n) v[n] = exp2_of(v[n] - m);
+          if (phase == 1) {
 #pragma unroll
-            for (int n = 0; n < UN; n += 2)
-              if (t + n < w.lanes) write(b + t + n, v[n] * inv, v[n + 1] * inv);
+            for (int n = 0; n < UN; ++n) l += v[n];
+          } else {
+#pragma unroll
+            for (int n = 0; n < UN; n += 2) write(e, t + n, v[n] * inv, v[n + 1] * inv);
           }
         }
       }
@@ -334,11 +368,12 @@ __global__ __launch_bounds__(1024) void differential_forward_units(DfArgs<float,
 
 // Sums over the wave's slots, then over a row's waves; the first wave's lanes of slot 0 hold them.
 template <int M>
-__device__ __forceinline__ void row_sums(const DfUnits& w, float (&v)[M], float* shared) {
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, waves = blockDim.x >> 6;
+__device__ __forceinline__ void row_sums(const DfUnits& w, int wave, float (&v)[M], float* shared) {
+  const int lane = threadIdx.x & 63, waves = blockDim.x >> 6;
+  for (int o = w.lanes; o < kWave; o <<= 1) {
 #pragma unroll
-  for (int i = 0; i < M; ++i)
-    for (int o = w.lanes; o < kWave; o <<= 1) v[i] += __shfl_xor(v[i], o, kWave);
+    for (int i = 0; i < M; ++i) v[i] += __shfl_xor(v[i], o, kWave);
+  }
   if (w.per_row == 1) return;
   __syncthreads();  // the records have been read
   if (lane < w.lanes) {
@@ -353,56 +388,64 @@ __device__ __forceinline__ void row_sums(const DfUnits& w, float (&v)[M], float*
   }
 }
 
-// Per target, in one walk: T = sum a g, sum a g tau k and sum a tau k, of which dq = scale c (the second - T the third).
-template <typename R, int A0, int A1, int A2>
+// Per target, in one walk: T = sum a g, A = sum a g tau k and B = sum a tau k, of which dq = scale c (A - T B).
+template <typename R, int A0, int A1, int A2, bool kNear>
 __global__ __launch_bounds__(1024) void differential_backward_target_units(DfArgs<float, R> a, DfUnits w) {
   using U = Unit<A0, A1, A2>;
   constexpr int kWords = kWave * U::RW, UN = kDfInFlightB, M = 2 * U::N + 1;
   extern __shared__ __align__(16) float df_lds[];
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   const Share sh = share_of(w, a.row_ptr);
   if (!sh.live) return;
-  float* rec = df_lds + wave * kWords;
+  const int lane = threadIdx.x & 63;
+  float* rec = df_lds + sh.wave * kWords;
   const int u = lane & (w.lanes - 1), s = lane >> w.shift, unit = u < w.units ? u : w.units - 1;
   const int p = unit / w.per_map;
+  const float* mine = rec + s * U::RW;
+  const float scale = a.scale;
   float q[U::N];
-  U::load(a.q + sh.row * a.L.D, w, unit, q);
-  const float lse = a.lse[sh.row * a.L.P + p];
-  const int steps = (int)((sh.e1 - sh.e0 + w.slots - 1) / w.slots);
+  U::template load<false>(a.q, w, unit, sh.row, q);
+  const float lse = a.lse[(int64_t)sh.row * a.L.P + p];
   float sums[M];
 #pragma unroll
   for (int i = 0; i < M; ++i) sums[i] = 0.f;
   Records<U::RW> records;
-  if (steps > 0) records.request(a.records, sh.e0, sh.e1, lane);
-  for (int b = 0; b < steps; b += w.lanes) {
+  if (sh.steps > 0) records.request(a.records, sh.e0, sh.e1, lane);
+  for (int b = 0; b < sh.steps; b += w.lanes) {
+    const int64_t e = sh.e0 + (int64_t)b * w.slots;  // the batch's first edge
     wave_lds();
     records.put(rec, lane);
     wave_lds();
-    if (b + w.lanes < steps) records.request(a.records, sh.e0 + (int64_t)(b + w.lanes) * w.slots, sh.e1, lane);
-    const int ends = steps - b < w.lanes ? steps - b : w.lanes;
+    if (b + w.lanes < sh.steps) records.request(a.records, e + kWave, sh.e1, lane);
+    const int ends = sh.steps - b < w.lanes ? sh.steps - b : w.lanes;
+    const int last = (int)(sh.e1 - e < kWave ? sh.e1 - e : kWave) - 1;  // the batch's last edge
+    const float* weights = a.g + e * a.L.H;
     for (int t = 0; t < ends; t += UN) {
-      float k[UN][U::N], bias[UN], cs[UN][U::NO], sn[UN][U::NO], g[UN];
+      float2 head[UN];
+      float k[UN][U::N], cs[UN][U::NO], sn[UN][U::NO], g[UN], v[UN];
 #pragma unroll
       for (int n = 0; n < UN; ++n) {
-        const int at = t + n < w.lanes ? t + n : w.lanes - 1;
-        const float* r = rec + (at * w.slots + s) * U::RW;
-        const float2 head = *reinterpret_cast<const float2*>(r);
-        bias[n] = t + n < w.lanes ? head.y : neg_inf<float>();
+        const float* r = mine + (t + n) * w.slots * U::RW;
+        head[n] = *reinterpret_cast<const float2*>(r);
 #pragma unroll
         for (int o = 0; o < U::NO; ++o) {
           const float2 x = *reinterpret_cast<const float2*>(r + 2 + 2 * o);
           cs[n][o] = x.x;
           sn[n][o] = x.y;
         }
-        U::load(a.k + (int64_t)__float_as_int(head.x) * a.L.D, w, unit, k[n]);
-        const int64_t e = sh.e0 + (int64_t)(b + at) * w.slots + s;
-        g[n] = a.g[(e < sh.e1 ? e : sh.e0) * a.L.H + (p >> 1)];
       }
 #pragma unroll
       for (int n = 0; n < UN; ++n) {
-        const float d = sum_units(U::dot(q, k[n], cs[n], sn[n]), w.per_map);
-        if (bias[n] != neg_inf<float>()) {
-          const float al = gm_exp(fmaf(a.scale, d, bias[n]) - lse), ag = al * g[n];
+        const int at = min((t + n) * w.slots + s, last);
+        g[n] = weights[(uint32_t)(at * a.L.H + (p >> 1))];
+        U::template load<kNear>(a.k, w, unit, __float_as_int(head[n].x), k[n]);
+      }
+#pragma unroll
+      for (int n = 0; n < UN; ++n) v[n] = U::dot(q, k[n], cs[n], sn[n]);
+      sum_units<UN>(v, w.per_map);
+#pragma unroll
+      for (int n = 0; n < UN; ++n) {
+        if (head[n].y != neg_inf<float>()) {
+          const float al = exp2_of(fmaf(scale, v[n], head[n].y - lse)), ag = al * g[n];
           U::turn(k[n], cs[n], sn[n], false);
           sums[2 * U::N] += ag;
 #pragma unroll
@@ -414,72 +457,89 @@ __global__ __launch_bounds__(1024) void differential_backward_target_units(DfArg
       }
     }
   }
-  row_sums<M>(w, sums, df_lds);
+  row_sums<M>(w, sh.wave, sums, df_lds);
   if (sh.part == 0 && s == 0 && u < w.units) {
     const float total = sums[2 * U::N];
-    const float factor = a.scale * ((p & 1) ? -a.lambda[p >> 1] : 1.f);
+    const float factor = a.gradient_scale * ((p & 1) ? -a.lambda[p >> 1] : 1.f);
     float dq[U::N];
 #pragma unroll
     for (int i = 0; i < U::N; ++i) dq[i] = factor * (sums[i] - total * sums[U::N + i]);
-    U::store(a.dq + sh.row * a.L.D, w, unit, dq);
+    U::store(a.dq + (int64_t)sh.row * a.L.D, w, unit, dq);
     if (unit % w.per_map == 0)
-      *reinterpret_cast<float2*>(a.pairs + (sh.row * a.L.P + p) * 2) = make_float2(lse, total);
+      *reinterpret_cast<float2*>(a.pairs + ((int64_t)sh.row * a.L.P + p) * 2) = make_float2(lse, total);
   }
 }
 
 // Per source, over the edges sorted by source: dk = scale c sum a (g - T) conj(tau) q.
-template <typename R, int A0, int A1, int A2>
+template <typename R, int A0, int A1, int A2, bool kNear>
 __global__ __launch_bounds__(1024) void differential_backward_source_units(DfArgs<float, R> a, DfUnits w) {
   using U = Unit<A0, A1, A2>;
-  constexpr int kWords = kWave * (U::RW + 2), UN = kDfInFlightB;
+  constexpr int kRecord = U::RW + 2, kWords = kWave * kRecord, UN = kDfInFlightB;
   extern __shared__ __align__(16) float df_lds[];
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   const Share sh = share_of(w, a.src_ptr);
   if (!sh.live) return;
-  float* rec = df_lds + wave * kWords;
+  const int lane = threadIdx.x & 63;
+  float* rec = df_lds + sh.wave * kWords;
   const int u = lane & (w.lanes - 1), s = lane >> w.shift, unit = u < w.units ? u : w.units - 1;
   const int p = unit / w.per_map;
+  const float* mine = rec + s * kRecord;
+  const float scale = a.scale;
   float k[U::N];
-  U::load(a.k + sh.row * a.L.D, w, unit, k);
-  const int steps = (int)((sh.e1 - sh.e0 + w.slots - 1) / w.slots);
+  U::template load<false>(a.k, w, unit, sh.row, k);
   float sums[U::N];
 #pragma unroll
   for (int i = 0; i < U::N; ++i) sums[i] = 0.f;
-  Records<U::RW + 2> records;
-  if (steps > 0) records.request(a.records_s, sh.e0, sh.e1, lane);
-  for (int b = 0; b < steps; b += w.lanes) {
+  Records<kRecord> records;
+  if (sh.steps > 0) records.request(a.records_s, sh.e0, sh.e1, lane);
+  for (int b = 0; b < sh.steps; b += w.lanes) {
+    const int64_t e = sh.e0 + (int64_t)b * w.slots;
     wave_lds();
     records.put(rec, lane);
     wave_lds();
-    if (b + w.lanes < steps) records.request(a.records_s, sh.e0 + (int64_t)(b + w.lanes) * w.slots, sh.e1, lane);
-    const int ends = steps - b < w.lanes ? steps - b : w.lanes;
+    if (b + w.lanes < sh.steps) records.request(a.records_s, e + kWave, sh.e1, lane);
+    const int ends = sh.steps - b < w.lanes ? sh.steps - b : w.lanes;
+    const int left = (int)(sh.e1 - e < kWave ? sh.e1 - e : kWave);
     for (int t = 0; t < ends; t += UN) {
-      float q[UN][U::N], bias[UN], cs[UN][U::NO], sn[UN][U::NO], g[UN];
-      float2 pair[UN];
+      float2 head[UN], pair[UN];
+      float q[UN][U::N], bias[UN], cs[UN][U::NO], sn[UN][U::NO], g[UN], v[UN];
 #pragma unroll
       for (int n = 0; n < UN; ++n) {
-        const int at = t + n < w.lanes ? t + n : w.lanes - 1;
-        const float* r = rec + (at * w.slots + s) * (U::RW + 2);
-        const float2 head = *reinterpret_cast<const float2*>(r);
-        // past the row's end: node 0, edge -inf's bits -- the row's first edge instead
-        const bool in = sh.e0 + (int64_t)(b + t + n) * w.slots + s < sh.e1 && t + n < w.lanes;
-        bias[n] = in ? r[2] : neg_inf<float>();
+        const float* r = mine + (t + n) * w.slots * kRecord;
+        const bool in = (t + n) * w.slots + s < left;  // past the row: node 0's row, edge 0's weight, excluded
+        head[n] = *reinterpret_cast<const float2*>(r);
+        bias[n] = r[2];
 #pragma unroll
         for (int o = 0; o < U::NO; ++o) {
           const float2 x = *reinterpret_cast<const float2*>(r + 4 + 2 * o);
           cs[n][o] = x.x;
           sn[n][o] = x.y;
         }
-        const int64_t i = __float_as_int(head.x), e = in ? __float_as_int(head.y) : 0;
-        U::load(a.q + i * a.L.D, w, unit, q[n]);
-        pair[n] = *reinterpret_cast<const float2*>(a.pairs + (i * a.L.P + p) * 2);
-        g[n] = a.g[e * a.L.H + (p >> 1)];
+        head[n].y = in ? head[n].y : 0.f;
+        bias[n] = in ? bias[n] : neg_inf<float>();
       }
 #pragma unroll
       for (int n = 0; n < UN; ++n) {
-        const float d = sum_units(U::dot(q[n], k, cs[n], sn[n]), w.per_map);
+        const int i = __float_as_int(head[n].x);
+        U::template load<kNear>(a.q, w, unit, i, q[n]);
+        if constexpr (kNear) {
+          pair[n] = *reinterpret_cast<const float2*>(reinterpret_cast<const char*>(a.pairs) +
+                                                     (__umul24((uint32_t)i, (uint32_t)(8 * a.L.P)) + 8u * (uint32_t)p));
+          g[n] = *reinterpret_cast<const float*>(
+              reinterpret_cast<const char*>(a.g) +
+              (__float_as_uint(head[n].y) * (uint32_t)(4 * a.L.H) + 4u * (uint32_t)(p >> 1)));
+        } else {
+          pair[n] = *reinterpret_cast<const float2*>(a.pairs + ((int64_t)i * a.L.P + p) * 2);
+          g[n] = a.g[(int64_t)__float_as_int(head[n].y) * a.L.H + (p >> 1)];
+        }
+      }
+#pragma unroll
+      for (int n = 0; n < UN; ++n) v[n] = U::dot(q[n], k, cs[n], sn[n]);
+      sum_units<UN>(v, w.per_map);
+#pragma unroll
+      for (int n = 0; n < UN; ++n) {
         if (bias[n] != neg_inf<float>()) {
-          const float ds = gm_exp(fmaf(a.scale, d, bias[n]) - pair[n].x) * (g[n] - pair[n].y);
+          const float al = exp2_of(fmaf(scale, v[n], bias[n] - pair[n].x));
+          const float ds = al * (g[n] - pair[n].y);
           U::turn(q[n], cs[n], sn[n], true);
 #pragma unroll
           for (int i = 0; i < U::N; ++i) sums[i] = fmaf(ds, q[n][i], sums[i]);
@@ -487,12 +547,12 @@ __global__ __launch_bounds__(1024) void differential_backward_source_units(DfArg
       }
     }
   }
-  row_sums<U::N>(w, sums, df_lds);
+  row_sums<U::N>(w, sh.wave, sums, df_lds);
   if (sh.part == 0 && s == 0 && u < w.units) {
-    const float factor = a.scale * ((p & 1) ? -a.lambda[p >> 1] : 1.f);
+    const float factor = a.gradient_scale * ((p & 1) ? -a.lambda[p >> 1] : 1.f);
 #pragma unroll
     for (int i = 0; i < U::N; ++i) sums[i] *= factor;
-    U::store(a.dk + sh.row * a.L.D, w, unit, sums);
+    U::store(a.dk + (int64_t)sh.row * a.L.D, w, unit, sums);
   }
 }
 
@@ -521,7 +581,7 @@ int find_shape(const DfLayout& L, int& per_map) {
 }
 
 int lanes_for(int units) {
-  int lanes = 1;
+  int lanes = kDfMinLanes;
   while (lanes < units) lanes *= 2;
   return lanes;
 }
@@ -540,13 +600,15 @@ size_t lds_bytes(DfPass pass, int waves, int lanes) {
   return words * sizeof(float);
 }
 
-template <typename R, int A0, int A1, int A2>
+template <typename R, int A0, int A1, int A2, bool kNear>
 int launch_shape(DfPass pass, const DfArgs<float, R>& a, DfUnits w, const DfRows& rows, hipStream_t stream) {
   using U = Unit<A0, A1, A2>;
+  using Kernel = void (*)(DfArgs<float, R>, DfUnits);
+  constexpr Kernel kKernels[3] = {&differential_forward_units<R, A0, A1, A2, kNear>,
+                                  &differential_backward_target_units<R, A0, A1, A2, kNear>,
+                                  &differential_backward_source_units<R, A0, A1, A2, kNear>};
+  const Kernel kernel = kKernels[(int)pass];
   constexpr int kWaves[3] = {16, 4, 1};
-  const void* kernels[3] = {reinterpret_cast<const void*>(&differential_forward_units<R, A0, A1, A2>),
-                            reinterpret_cast<const void*>(&differential_backward_target_units<R, A0, A1, A2>),
-                            reinterpret_cast<const void*>(&differential_backward_source_units<R, A0, A1, A2>)};
   w.first = 0;
   for (int c = 0; c < 3; ++c) {
     w.count = rows.count[c];
@@ -555,29 +617,29 @@ int launch_shape(DfPass pass, const DfArgs<float, R>& a, DfUnits w, const DfRows
     if (w.count > 0) {
       const int64_t blocks = c == 2 ? blocks_for(w.count) : w.count;
       const size_t lds = lds_bytes<U>(pass, waves, w.lanes);
-      if (lds > 64 * 1024 &&
-          hipFuncSetAttribute(kernels[(int)pass], hipFuncAttributeMaxDynamicSharedMemorySize, 160 * 1024) != hipSuccess)
+      if (lds > 64 * 1024 && hipFuncSetAttribute(reinterpret_cast<const void*>(kernel),
+                                                 hipFuncAttributeMaxDynamicSharedMemorySize, 160 * 1024) != hipSuccess)
         return check_launch("differential (LDS)");
-      switch (pass) {
-        case DfPass::Forward:
-          hipLaunchKernelGGL((differential_forward_units<R, A0, A1, A2>), dim3((unsigned)blocks), dim3(waves * kWave),
-                             lds, stream, a, w);
-          break;
-        case DfPass::BackwardTarget:
-          hipLaunchKernelGGL((differential_backward_target_units<R, A0, A1, A2>), dim3((unsigned)blocks),
-                             dim3(waves * kWave), lds, stream, a, w);
-          break;
-        case DfPass::BackwardSource:
-          hipLaunchKernelGGL((differential_backward_source_units<R, A0, A1, A2>), dim3((unsigned)blocks),
-                             dim3(waves * kWave), lds, stream, a, w);
-          break;
-      }
+      hipLaunchKernelGGL(kernel, dim3((unsigned)blocks), dim3(waves * kWave), lds, stream, a, w);
       const int rc = check_launch("differential");
       if (rc != GM_OK) return rc;
     }
     w.first += w.count;
   }
   return GM_OK;
+}
+
+template <bool kNear, typename R>
+int launch_near(DfPass pass, int shape, const DfArgs<float, R>& a, const DfUnits& w, const DfRows& rows,
+                hipStream_t stream) {
+  switch (shape) {
+    case 0: return launch_shape<R, 4, 2, 1, kNear>(pass, a, w, rows, stream);
+    case 1: return launch_shape<R, 2, 2, 2, kNear>(pass, a, w, rows, stream);
+    case 2: return launch_shape<R, 2, 2, 0, kNear>(pass, a, w, rows, stream);
+    case 3: return launch_shape<R, 2, 1, 1, kNear>(pass, a, w, rows, stream);
+    case 4: return launch_shape<R, 1, 1, 1, kNear>(pass, a, w, rows, stream);
+    default: return launch_shape<R, 1, 1, 0, kNear>(pass, a, w, rows, stream);
+  }
 }
 
 template <typename R>
@@ -589,18 +651,14 @@ int launch_units(DfPass pass, const DfArgs<float, R>& a, const DfRows& rows, hip
   w.lanes = lanes_for(w.units);
   while ((1 << w.shift) < w.lanes) ++w.shift;
   w.slots = kWave / w.lanes;
-  w.base0 = a.L.off[0];
-  w.base1 = a.L.off[1];
-  w.base2 = a.L.F == 3 ? a.L.off[2] : 0;
+  for (int f = 0; f < a.L.F; ++f) w.base[f] = a.L.off[f];
+  w.row_bytes = (uint32_t)(a.L.D * sizeof(R));
   w.order = rows.order;
-  switch (shape) {
-    case 0: return launch_shape<R, 4, 2, 1>(pass, a, w, rows, stream);
-    case 1: return launch_shape<R, 2, 2, 2>(pass, a, w, rows, stream);
-    case 2: return launch_shape<R, 2, 2, 0>(pass, a, w, rows, stream);
-    case 3: return launch_shape<R, 2, 1, 1>(pass, a, w, rows, stream);
-    case 4: return launch_shape<R, 1, 1, 1>(pass, a, w, rows, stream);
-    default: return launch_shape<R, 1, 1, 0>(pass, a, w, rows, stream);
-  }
+  const int64_t nodes = std::max(a.n_targets, a.n_sources), limit = int64_t(1) << 32;
+  const bool near = nodes < (int64_t(1) << 24) && nodes * w.row_bytes < limit && nodes * a.L.P * 8 < limit &&
+                    a.n_edges * a.L.H * 4 < limit;
+  return near ? launch_near<true>(pass, shape, a, w, rows, stream)
+              : launch_near<false>(pass, shape, a, w, rows, stream);
 }
 
 }  // namespace

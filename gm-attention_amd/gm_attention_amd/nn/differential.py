@@ -89,7 +89,9 @@ class EdgeTables:
         records = torch.empty(n_edges, 2 * self.orders, dtype=self.dtype, device=self.device)
         words = records.view(_WORD[self.dtype])
         words[:, 0] = source
-        records[:, 1] = masked
+        # in units of log 2; the type's lowest value stays a finite one
+        lowest = torch.finfo(self.dtype).min
+        records[:, 1] = torch.where(masked == -math.inf, masked, (masked * _LOG2E).clamp_min(lowest))
         records[:, 2:] = phases
         self.records = records
         self._kept = [_native.Made(self.row_ptr, records)]
@@ -159,6 +161,7 @@ class EdgeTables:
             made.found()
 
 
+_LOG2E = 1.0 / math.log(2.0)
 _WORD = {torch.float32: torch.int32, torch.float64: torch.int64}
 
 

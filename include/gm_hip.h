@@ -276,12 +276,13 @@ int gm_edge_tables_f64(const double* targets, const double* target_frames, const
  * an edge outside hold is not read into anything.
  * records (n_edges, 2 orders) in the order of the CSR row_ptr over targets, in
  * words of the tables' type: the source node (as an integer of that size), the
- * bias (-inf outside the window), then (cos, sin) of orders 1 .. orders - 1.
+ * bias over log 2 (-inf outside the window), then (cos, sin) of orders
+ * 1 .. orders - 1.
  * records_s (n_edges, 2 + 2 orders) in the order of the edges sorted by source,
  * src_ptr its CSR: target, edge (integers), bias, 0, (cos, sin).  Nodes must lie
  * inside their tables (the kernels follow them).
- * lse (n_targets, 2 H), or NULL where no backward follows: the log sum of
- * exponentials.  Backward from g = d alpha: dq, dk in the rows' type,
+ * lse (n_targets, 2 H), or NULL where no backward follows: the base-2 logarithm
+ * of the sum of exponentials.  Backward from g = d alpha: dq, dk in the rows' type,
  * dlambda (H); pairs (n_targets, 2 H, 2), ds (n_edges, 2 H) and partial
  * (gm_differential_partials(H) doubles) are workspaces.  Sums in a fixed order.
  * order, or NULL: every target once, those of more than 128 S edges first, then
