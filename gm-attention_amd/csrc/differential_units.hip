@@ -32,8 +32,8 @@ struct DfUnits {
   int base[3];           // the frequencies' flat offsets
   uint32_t row_bytes;
   const int32_t* order;
-  int64_t first, count;  // rows order[first .. first + count)
-  int per_row;           // waves a row: 1 (four rows a workgroup) or the workgroup's
+  // the rows of this launch, order[first ..): `shared` of all the workgroup's waves each, then `single` of one wave
+  int64_t first, shared, single;
 };
 
 __device__ __forceinline__ int uniform(int v) { return __builtin_amdgcn_readfirstlane(v); }
@@ -215,20 +215,23 @@ __device__ __forceinline__ void sum_units(float (&v)[UN], int per_map) {
 // Which row a wave works on, and which of its edges; all of it scalar.
 struct Share {
   int64_t e0, e1;  // this wave's edges
-  int row, wave, part, steps;
+  int row, wave, part, parts, steps;  // parts: the row's waves
   bool live;
 };
 __device__ __forceinline__ Share share_of(const DfUnits& w, const int64_t* ptr) {
   Share s;
   s.wave = uniform((int)(threadIdx.x >> 6));
-  const int rows = w.per_row == 1 ? kWavesPerBlock : 1;  // of a workgroup
-  const int64_t at = xcd_spread_block(blockIdx.x, gridDim.x) * rows + (w.per_row == 1 ? s.wave : 0);
-  s.part = w.per_row == 1 ? 0 : s.wave;
-  s.live = at < w.count;
+  const int waves = blockDim.x >> 6;
+  const bool one = blockIdx.x >= w.shared;
+  const int64_t at = one ? w.shared + xcd_spread_block(blockIdx.x - w.shared, gridDim.x - w.shared) * waves + s.wave
+                         : xcd_spread_block(blockIdx.x, w.shared);
+  s.part = one ? 0 : s.wave;
+  s.parts = one ? 1 : waves;
+  s.live = at < w.shared + w.single;
   s.row = s.live ? uniform((int)w.order[w.first + at]) : 0;
   const int64_t e0 = s.live ? uniform(ptr[s.row]) : 0, e1 = s.live ? uniform(ptr[s.row + 1]) : 0;
   const int64_t steps = (e1 - e0 + w.slots - 1) >> (6 - w.shift);
-  const int64_t per = (w.per_row == 1 ? steps : (steps + w.per_row - 1) / w.per_row) << (6 - w.shift);
+  const int64_t per = (one ? steps : (steps + waves - 1) / waves) << (6 - w.shift);
   s.e0 = e0 + s.part * per < e1 ? e0 + s.part * per : e1;
   s.e1 = s.e0 + per < e1 ? s.e0 + per : e1;
   s.steps = (int)((s.e1 - s.e0 + w.slots - 1) >> (6 - w.shift));
@@ -265,7 +268,7 @@ __global__ __launch_bounds__(1024) void differential_forward_units(DfArgs<float,
       const float x = __shfl_xor(v, o, kWave);
       v = maximum ? fmaxf(x, v) : v + x;
     }
-    if (w.per_row > 1) {
+    if (sh.parts > 1) {
       __syncthreads();
       shared[sh.wave * kWave + lane] = v;
       __syncthreads();
@@ -368,13 +371,13 @@ __global__ __launch_bounds__(1024) void differential_forward_units(DfArgs<float,
 
 // Sums over the wave's slots, then over a row's waves; the first wave's lanes of slot 0 hold them.
 template <int M>
-__device__ __forceinline__ void row_sums(const DfUnits& w, int wave, float (&v)[M], float* shared) {
-  const int lane = threadIdx.x & 63, waves = blockDim.x >> 6;
+__device__ __forceinline__ void row_sums(const DfUnits& w, const Share& sh, float (&v)[M], float* shared) {
+  const int lane = threadIdx.x & 63, wave = sh.wave;
   for (int o = w.lanes; o < kWave; o <<= 1) {
 #pragma unroll
     for (int i = 0; i < M; ++i) v[i] += __shfl_xor(v[i], o, kWave);
   }
-  if (w.per_row == 1) return;
+  if (sh.parts == 1) return;
   __syncthreads();  // the records have been read
   if (lane < w.lanes) {
 #pragma unroll
@@ -382,7 +385,7 @@ __device__ __forceinline__ void row_sums(const DfUnits& w, int wave, float (&v)[
   }
   __syncthreads();
   if (wave == 0 && lane < w.lanes) {
-    for (int o = 1; o < waves; ++o)
+    for (int o = 1; o < sh.parts; ++o)
 #pragma unroll
       for (int i = 0; i < M; ++i) v[i] += shared[(o * M + i) * w.lanes + lane];
   }
@@ -457,7 +460,7 @@ __global__ __launch_bounds__(1024) void differential_backward_target_units(DfArg
       }
     }
   }
-  row_sums<M>(w, sh.wave, sums, df_lds);
+  row_sums<M>(w, sh, sums, df_lds);
   if (sh.part == 0 && s == 0 && u < w.units) {
     const float total = sums[2 * U::N];
     const float factor = a.gradient_scale * ((p & 1) ? -a.lambda[p >> 1] : 1.f);
@@ -547,7 +550,7 @@ __global__ __launch_bounds__(1024) void differential_backward_source_units(DfArg
       }
     }
   }
-  row_sums<U::N>(w, sh.wave, sums, df_lds);
+  row_sums<U::N>(w, sh, sums, df_lds);
   if (sh.part == 0 && s == 0 && u < w.units) {
     const float factor = a.gradient_scale * ((p & 1) ? -a.lambda[p >> 1] : 1.f);
 #pragma unroll
@@ -608,14 +611,14 @@ int launch_shape(DfPass pass, const DfArgs<float, R>& a, DfUnits w, const DfRows
                                   &differential_backward_target_units<R, A0, A1, A2, kNear>,
                                   &differential_backward_source_units<R, A0, A1, A2, kNear>};
   const Kernel kernel = kKernels[(int)pass];
-  constexpr int kWaves[3] = {16, 4, 1};
+  // the rows of sixteen waves; those of four and of one, in one launch of workgroups of four
   w.first = 0;
-  for (int c = 0; c < 3; ++c) {
-    w.count = rows.count[c];
-    w.per_row = kWaves[c];
-    const int waves = c == 2 ? kWavesPerBlock : kWaves[c];
-    if (w.count > 0) {
-      const int64_t blocks = c == 2 ? blocks_for(w.count) : w.count;
+  for (int c = 0; c < 2; ++c) {
+    w.shared = rows.count[c];
+    w.single = c == 0 ? 0 : rows.count[2];
+    const int waves = c == 0 ? 16 : kWavesPerBlock;
+    if (w.shared + w.single > 0) {
+      const int64_t blocks = w.shared + blocks_for(w.single);
       const size_t lds = lds_bytes<U>(pass, waves, w.lanes);
       if (lds > 64 * 1024 && hipFuncSetAttribute(reinterpret_cast<const void*>(kernel),
                                                  hipFuncAttributeMaxDynamicSharedMemorySize, 160 * 1024) != hipSuccess)
@@ -624,7 +627,7 @@ int launch_shape(DfPass pass, const DfArgs<float, R>& a, DfUnits w, const DfRows
       const int rc = check_launch("differential");
       if (rc != GM_OK) return rc;
     }
-    w.first += w.count;
+    w.first += w.shared;
   }
   return GM_OK;
 }

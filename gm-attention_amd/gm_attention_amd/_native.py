@@ -18,10 +18,12 @@ silent fallback.
 
 from __future__ import annotations
 
+import contextlib
 import ctypes
 import functools
 import threading
 import weakref
+from collections.abc import Sequence
 from pathlib import Path
 from typing import Any
 
@@ -160,6 +162,23 @@ def _call(name: str, *args: Any) -> None:
     if status != 0:
         message = library().gm_last_error().decode()
         raise RuntimeError(f"{name}: {message}")
+
+
+def _call_on(device: torch.device, name: str, *args: Any) -> None:
+    """:func:`_call` with ``device`` the current one."""
+    if torch.cuda.current_device() == device.index:
+        _call(name, *args)
+    else:
+        with torch.cuda.device(device):
+            _call(name, *args)
+
+
+_NO_SPAN = contextlib.nullcontext()
+
+
+def span(name: str) -> Any:
+    """A profiler's label, where one looks (five microseconds otherwise)."""
+    return torch.profiler.record_function(name) if torch.autograd._profiler_enabled() else _NO_SPAN
 
 
 def _ptr(t: Tensor | None) -> int | None:
@@ -1398,9 +1417,30 @@ class PointwiseLayout:
         self.offsets = (ctypes.c_int64 * max(1, self.nf))(*[slices[n].start for n, _ in nonzero])
         self.mults = (ctypes.c_int64 * max(1, self.nf))(*[m for _, m in nonzero])
         self.G = sum(m for _, m in nonzero)
+        self._args = (self.D, self.a0, self.nf, ctypes.cast(self.offsets, _P), ctypes.cast(self.mults, _P))
+        self._slots: dict[tuple[int, ...], tuple] = {}
 
     def args(self) -> tuple:
-        return (self.D, self.a0, self.nf, ctypes.cast(self.offsets, _P), ctypes.cast(self.mults, _P))
+        return self._args
+
+    def parameter_slots(self, counts: tuple[int, ...]) -> tuple[Any, list[int], list[int]]:
+        """For the residual sum's parameters, ``counts`` of them a group (the branch's
+        gains and offset, the scales, the next norm's gains and offset): the type of
+        the host array of their pointers, and each one's place and length."""
+        held = self._slots.get(counts)
+        if held is None:
+            slots = self.nf + 1
+            by_frequency = list(range(0 if self.a0 else 1, slots))
+            starts, places, lengths = (0, 3 * slots, slots, 2 * slots, 3 * slots + 1), [], []
+            mults = [self.a0] + list(self.mults[: self.nf])
+            for i, (start, count) in enumerate(zip(starts, counts, strict=True)):
+                mine = ([0] if i in (1, 4) else by_frequency) if count else []
+                if len(mine) != count:
+                    raise RuntimeError("a group of the residual sum's parameters holds a vector of every frequency")
+                places += [start + f for f in mine]
+                lengths += [mults[f] for f in mine]
+            held = self._slots[counts] = (ctypes.c_void_p * (3 * slots + 2), places, lengths)
+        return held
 
 
 def _pointers(ts: list[Tensor]) -> Any:
@@ -1559,103 +1599,68 @@ def gate_backward(gy: Tensor, h: Tensor, pre: Tensor, layout: PointwiseLayout,
     return dh, dpre
 
 
-class ResidualParameters:
-    """The residual sum's parameter vectors by frequency, ``gains``, ``scales`` and
-    ``next_gains`` (None where left out), and the two offsets: checked, with the
-    host array of their pointers that the entry points take."""
-
-    def __init__(self, layout: PointwiseLayout, x: Tensor, gains: list[Tensor] | None, offset: Tensor | None,
-                 scales: list[Tensor] | None, next_gains: list[Tensor] | None, next_offset: Tensor | None):
-        self.next = next_gains is not None
-        pd, device = param_dtype(x.dtype), x.device
-        mults = ([layout.a0] if layout.a0 else []) + list(layout.mults[: layout.nf])
-        pointers: list[int | None] = []
-        for name, group in (("gains", gains), ("scales", scales), ("next_gains", next_gains)):
-            if group is None:
-                pointers += [None] * (layout.nf + 1)
-                continue
-            _check(len(group) == len(mults), f"{name} must hold a vector of every frequency")
-            for t, m in zip(group, mults):
-                _check(t.dtype == pd and t.device == device and t.ndim == 1 and t.shape[0] == m and t.is_contiguous(),
-                       f"{name} must be contiguous {pd} vectors of {mults} on the rows' device")
-            pointers += ([] if layout.a0 else [None]) + [t.data_ptr() for t in group]
-        for name, t in (("offset", offset), ("next_offset", next_offset)):
-            _check(t is None or (t.dtype == pd and t.device == device and tuple(t.shape) == (layout.a0,)
-                                 and t.is_contiguous()), f"{name} must be a contiguous ({layout.a0},) {pd} vector")
-            pointers.append(_ptr(t))
-        self.array = (ctypes.c_void_p * len(pointers))(*pointers)
-
-    def arg(self) -> Any:
-        return ctypes.cast(self.array, _P)
+def _residual_parameters(layout: PointwiseLayout, counts: tuple[int, ...], params: Sequence[Tensor]) -> Any:
+    """The host array of the parameters' pointers (kept alive by the caller's reference)."""
+    array, places, _ = layout.parameter_slots(counts)
+    out = array()
+    for place, p in zip(places, params):
+        out[place] = p.data_ptr()
+    return out
 
 
-def _residual_check(x: Tensor, u: Tensor, z: Tensor | None, layout: PointwiseLayout) -> str:
-    """The residual sum's suffix, its rows checked."""
-    sfx = _pw_check(x, layout)
-    _require_device(x, u, *(() if z is None else (z,)))
-    wide = x.dtype == torch.bfloat16 and u.dtype == torch.float32
-    _check(u.dtype == x.dtype or wide, f"u must be {x.dtype} (or float32 for bfloat16 rows), got {u.dtype}")
-    _check(u.shape == x.shape, "u must be shaped as x")
-    copies = layout.a0 + layout.G
-    _check(z is None or (z.dtype == x.dtype and tuple(z.shape) == (x.shape[0], copies)),
-           f"z must be (n_nodes, {copies}) in x's dtype")
-    return sfx + ("_f32" if wide else "")
-
-
-def residual_norm_forward(x: Tensor, u: Tensor, z: Tensor | None, params: ResidualParameters,
+def residual_norm_forward(x: Tensor, u: Tensor, z: Tensor | None, counts: tuple[int, ...], params: Sequence[Tensor],
                           layout: PointwiseLayout, factor: float, eps: float, next_eps: float,
                           train: bool) -> tuple[Tensor, Tensor | None, Tensor | None]:
     """``(y, normed, stats)``: the residual sum and the norm behind it (None without next gains);
-    ``stats (n_nodes, 4)``, what the backward reads of both norms, under ``train``."""
-    sfx = _residual_check(x, u, z, layout)
+    ``stats (n_nodes, 4)``, what the backward reads of both norms, under ``train``.  ``params``:
+    a vector a frequency, ``counts`` of them in every group (:meth:`PointwiseLayout.parameter_slots`)."""
+    sfx, device = _pw_check(x, layout), x.device
+    pd = torch.float64 if x.dtype == torch.float64 else torch.float32
+    if u.dtype != x.dtype:
+        if x.dtype != torch.bfloat16 or u.dtype != torch.float32:
+            raise RuntimeError(f"u must be {x.dtype} (or float32 for bfloat16 rows), got {u.dtype}")
+        sfx = "bf16_f32"
+    if u.shape != x.shape or not u.is_contiguous() or u.device != device:
+        raise RuntimeError("u must be contiguous, shaped as x and on its device")
+    if z is not None and (z.dtype != x.dtype or z.shape != (x.shape[0], layout.a0 + layout.G)
+                          or not z.is_contiguous() or z.device != device):
+        raise RuntimeError(f"z must be contiguous (n_nodes, {layout.a0 + layout.G}) in x's dtype and on its device")
+    for p, m in zip(params, layout.parameter_slots(counts)[2], strict=True):
+        if p.dtype != pd or p.device != device or p.ndim != 1 or p.shape[0] != m or not p.is_contiguous():
+            raise RuntimeError(f"the parameters must be contiguous {pd} vectors of their frequencies' copies on {device}")
     y = torch.empty_like(x)
-    normed = torch.empty_like(x) if params.next else None
-    stats = torch.empty(x.shape[0], 4, dtype=param_dtype(x.dtype), device=x.device) if train else None
-    with torch.cuda.device(x.device):
-        _call(f"gm_residual_norm_forward_{sfx}", _ptr(x), _ptr(u), _ptr(z), params.arg(), x.shape[0], *layout.args(),
-              float(factor), float(eps), float(next_eps), _ptr(y), _ptr(normed), _ptr(stats), _stream(x.device))
+    normed = torch.empty_like(x) if counts[3] else None
+    stats = torch.empty(x.shape[0], 4, dtype=pd, device=device) if train else None
+    _call_on(device, "gm_residual_norm_forward_" + sfx, _ptr(x), _ptr(u), _ptr(z),
+             _residual_parameters(layout, counts, params), x.shape[0], *layout.args(), factor, eps, next_eps, _ptr(y),
+             _ptr(normed), _ptr(stats), _stream(device))
     return y, normed, stats
 
 
 def residual_norm_backward(dy: Tensor | None, dn: Tensor | None, x: Tensor, u: Tensor, z: Tensor | None,
-                           params: ResidualParameters, stats: Tensor, layout: PointwiseLayout,
+                           counts: tuple[int, ...], params: Sequence[Tensor], stats: Tensor, layout: PointwiseLayout,
                            factor: float) -> tuple[Tensor, Tensor, Tensor | None, Tensor]:
-    """``(dx, du, dz, dparams)`` with ``dparams = (dgain (copies), doffset (a0), dscale (copies),
-    dnext_gain (copies), dnext_offset (a0))`` summed over the nodes in a fixed order."""
-    n, copies = x.shape[0], layout.a0 + layout.G
-    sfx = _residual_check(x, u, z, layout)
-    pd = param_dtype(x.dtype)
+    """``(dx, du, dz, dparams)`` of what a forward took and gave (contiguous ``dy``, ``dn``, either None), with
+    ``dparams = (dgain (copies), doffset (a0), dscale (copies), dnext_gain (copies), dnext_offset (a0))`` summed
+    over the nodes in a fixed order."""
+    n, copies, device = x.shape[0], layout.a0 + layout.G, x.device
+    sfx = "bf16_f32" if u.dtype != x.dtype else _PW_SUFFIX[x.dtype]
     for name, t in (("dy", dy), ("dn", dn)):
-        _check(t is None or (t.dtype == x.dtype and t.shape == x.shape and t.is_contiguous()
-                             and t.device == x.device), f"{name} must match x (contiguous)")
-    _check(stats.dtype == pd and tuple(stats.shape) == (n, 4) and stats.is_contiguous(), f"stats must be ({n}, 4) {pd}")
+        if t is not None and (t.dtype != x.dtype or t.shape != x.shape or not t.is_contiguous() or t.device != device):
+            raise RuntimeError(f"{name} must match x (contiguous)")
     dx, du = torch.empty_like(x), torch.empty_like(u)
     dz = None if z is None else torch.empty_like(z)
-    partial = torch.empty(int(library().gm_residual_norm_partial_rows(n)), layout.D + layout.a0, dtype=pd,
-                          device=x.device)
-    dparams = torch.empty(3 * copies + 2 * layout.a0, dtype=pd, device=x.device)
-    with torch.cuda.device(x.device):
-        _call(f"gm_residual_norm_backward_{sfx}", _ptr(dy), _ptr(dn), _ptr(x), _ptr(u), _ptr(z), params.arg(),
-              _ptr(stats), n, *layout.args(), float(factor), _ptr(dx), _ptr(du), _ptr(dz), _ptr(partial),
-              _ptr(dparams), _stream(x.device))
+    rows, width = int(library().gm_residual_norm_partial_rows(n)), layout.D + layout.a0
+    # one allocation: the parameters' gradients, then the kernel's rows of sums
+    sums = torch.empty(3 * copies + 2 * layout.a0 + rows * width, dtype=stats.dtype, device=device)
+    dparams, partial = sums[: 3 * copies + 2 * layout.a0], sums[3 * copies + 2 * layout.a0:]
+    _call_on(device, "gm_residual_norm_backward_" + sfx, _ptr(dy), _ptr(dn), _ptr(x), _ptr(u), _ptr(z),
+             _residual_parameters(layout, counts, params), _ptr(stats), n, *layout.args(), factor, _ptr(dx), _ptr(du),
+             _ptr(dz), _ptr(partial), _ptr(dparams), _stream(device))
     return dx, du, dz, dparams
 
 
 # ---------------------------------------------------------------- differential softmax
-
-
-def _differential_check(q: Tensor, k: Tensor, lam: Tensor, tables: Any, maps: Any) -> str:
-    """The differential softmax's suffix, its rows checked against the tables."""
-    _require_device(q, k, lam, tables.records, tables.row_ptr)
-    _check(q.dtype in _PW_SUFFIX and k.dtype == q.dtype, "q and k must share float32, float64 or bfloat16")
-    table = param_dtype(q.dtype)
-    _check(tables.dtype == table and lam.dtype == table,
-           "the tables and lam must be q's dtype (float32 for bfloat16 rows)")
-    _check(q.dim() == 2 and k.dim() == 2 and q.shape[0] == tables.n_targets and k.shape[0] == tables.n_sources
-           and q.shape[1] == k.shape[1] == maps.plan.width, "q must be (n_targets, D) and k (n_sources, D)")
-    _check(tuple(lam.shape) == (maps.heads,), "lam must be (H,)")
-    _check(maps.top < tables.orders, "the maps need higher orders than the tables hold")
-    return _PW_SUFFIX[q.dtype]
 
 
 def differential_slots(desc: Tensor, D: int, orders: int, H: int) -> int:
@@ -1668,40 +1673,38 @@ def differential_slots(desc: Tensor, D: int, orders: int, H: int) -> int:
 def differential_forward(q: Tensor, k: Tensor, lam: Tensor, tables: Any, maps: Any, scale: float,
                          train: bool) -> tuple[Tensor, Tensor | None]:
     """``(alpha (n_edges, H), lse)``: the differential softmax's weights and, under ``train``,
-    the log sums of exponentials ``(n_targets, 2 H)`` its backward reads."""
-    sfx = _differential_check(q, k, lam, tables, maps)
-    H, desc = maps.heads, maps.desc
+    the log sums of exponentials ``(n_targets, 2 H)`` its backward reads.  The rows are whole
+    (contiguous, at multiples of 16 bytes) and match the tables: nn.differential's checks."""
+    H, desc, device = maps.heads, maps.desc, q.device
     order, counts = tables.target_rows(maps.slots(tables))
     tables.found()
-    alpha = torch.empty(tables.n_edges, H, dtype=tables.dtype, device=q.device)
-    lse = torch.empty(tables.n_targets, 2 * H, dtype=tables.dtype, device=q.device) if train else None
-    with torch.cuda.device(q.device):
-        _call(f"gm_differential_forward_{sfx}", _ptr(q), _ptr(k), _ptr(lam), _ptr(tables.records), desc.data_ptr(),
-              _ptr(tables.row_ptr), _ptr(order), counts, tables.n_targets, tables.n_sources, tables.n_edges,
-              q.shape[1], tables.orders, desc.shape[0], H, float(scale), _ptr(alpha), _ptr(lse), _stream(q.device))
+    alpha = torch.empty(tables.n_edges, H, dtype=tables.dtype, device=device)
+    lse = torch.empty(tables.n_targets, 2 * H, dtype=tables.dtype, device=device) if train else None
+    _call_on(device, "gm_differential_forward_" + _PW_SUFFIX[q.dtype], _ptr(q), _ptr(k), _ptr(lam),
+             _ptr(tables.records), desc.data_ptr(), _ptr(tables.row_ptr), _ptr(order), counts, tables.n_targets,
+             tables.n_sources, tables.n_edges, q.shape[1], tables.orders, desc.shape[0], H, scale, _ptr(alpha),
+             _ptr(lse), _stream(device))
     return alpha, lse
 
 
 def differential_backward(g: Tensor, q: Tensor, k: Tensor, lam: Tensor, lse: Tensor, tables: Any, maps: Any,
                           scale: float) -> tuple[Tensor, Tensor, Tensor]:
-    """``(dq, dk, dlam)``: the rows' gradients in their dtype, the factors' in the tables'; no atomics."""
-    sfx = _differential_check(q, k, lam, tables, maps)
-    H, desc, slots = maps.heads, maps.desc, maps.slots(tables)
-    _check(g.dtype == tables.dtype and tuple(g.shape) == (tables.n_edges, H) and g.is_contiguous()
-           and g.device == q.device, "g must be contiguous (n_edges, H) in the tables' dtype")
-    _check(lse.dtype == tables.dtype and tuple(lse.shape) == (tables.n_targets, 2 * H) and lse.is_contiguous(),
-           "lse must be the forward's")
+    """``(dq, dk, dlam)`` of what a forward took and gave and the weights' gradient (contiguous): the rows'
+    gradients in their dtype, the factors' in the tables'; no atomics."""
+    H, desc, slots, device = maps.heads, maps.desc, maps.slots(tables), q.device
+    if g.dtype != tables.dtype or g.shape != (tables.n_edges, H) or not g.is_contiguous() or g.device != device:
+        raise RuntimeError("g must be contiguous (n_edges, H) in the tables' dtype")
     src_ptr, records_s = tables.group_sources()
     (order, counts), (order_s, counts_s) = tables.target_rows(slots), tables.source_rows(slots)
     tables.found()
-    pairs = torch.empty(tables.n_targets, 2 * H, 2, dtype=tables.dtype, device=q.device)
+    pairs = torch.empty(tables.n_targets, 2 * H, 2, dtype=tables.dtype, device=device)
     # the simple kernels' workspace
-    ds = None if slots else torch.empty(tables.n_edges, 2 * H, dtype=tables.dtype, device=q.device)
-    partial = torch.empty(int(library().gm_differential_partials(H)), dtype=torch.float64, device=q.device)
+    ds = None if slots else torch.empty(tables.n_edges, 2 * H, dtype=tables.dtype, device=device)
+    partial = torch.empty(int(library().gm_differential_partials(H)), dtype=torch.float64, device=device)
     dq, dk, dlam = torch.empty_like(q), torch.empty_like(k), torch.empty_like(lam)
-    with torch.cuda.device(q.device):
-        _call(f"gm_differential_backward_{sfx}", _ptr(g), _ptr(q), _ptr(k), _ptr(lam), _ptr(tables.records),
-              _ptr(records_s), desc.data_ptr(), _ptr(tables.row_ptr), _ptr(src_ptr), _ptr(order), counts,
-              _ptr(order_s), counts_s, tables.n_targets, tables.n_sources, tables.n_edges, q.shape[1], tables.orders, desc.shape[0], H, float(scale),
-              _ptr(lse), _ptr(pairs), _ptr(ds), _ptr(partial), _ptr(dq), _ptr(dk), _ptr(dlam), _stream(q.device))
+    _call_on(device, "gm_differential_backward_" + _PW_SUFFIX[q.dtype], _ptr(g), _ptr(q), _ptr(k), _ptr(lam),
+             _ptr(tables.records), _ptr(records_s), desc.data_ptr(), _ptr(tables.row_ptr), _ptr(src_ptr), _ptr(order),
+             counts, _ptr(order_s), counts_s, tables.n_targets, tables.n_sources, tables.n_edges, q.shape[1],
+             tables.orders, desc.shape[0], H, scale, _ptr(lse), _ptr(pairs), _ptr(ds), _ptr(partial), _ptr(dq),
+             _ptr(dk), _ptr(dlam), _stream(device))
     return dq, dk, dlam

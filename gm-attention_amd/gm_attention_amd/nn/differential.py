@@ -157,8 +157,10 @@ class EdgeTables:
 
     def found(self) -> None:
         """The current stream reads what is kept from here on."""
+        here = _native.stream_handle(self.device)
         for made in self._kept:
-            made.found()
+            if made.handle != here:
+                made.found()
 
 
 _LOG2E = 1.0 / math.log(2.0)
@@ -212,7 +214,7 @@ class DifferentialSoftmax(torch.autograd.Function):
         if train:  # found here: the backward runs on a thread and perhaps a stream of its own
             tables.group_sources()
             tables.source_rows(maps.slots(tables))
-        with torch.profiler.record_function("gm::attention/differential_softmax"):
+        with _native.span("gm::attention/differential_softmax"):
             alpha, lse = _native.differential_forward(q, k, lam, tables, maps, scale, train)
         if train:
             ctx.save_for_backward(q, k, lam, lse)
@@ -223,7 +225,7 @@ class DifferentialSoftmax(torch.autograd.Function):
     @torch.autograd.function.once_differentiable
     def backward(ctx: Any, grad_alpha: Tensor) -> tuple:
         q, k, lam, lse = ctx.saved_tensors
-        with torch.profiler.record_function("gm::attention/differential_softmax_backward"):
+        with _native.span("gm::attention/differential_softmax_backward"):
             dq, dk, dlam = _native.differential_backward(grad_alpha.contiguous(), q, k, lam, lse, *ctx.rest)
         return dq, dk, dlam, None, None, None
 

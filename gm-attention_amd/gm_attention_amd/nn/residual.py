@@ -37,27 +37,23 @@ GateKind = Literal["sigmoid", "double_sigmoid"]
 _GATES = {"sigmoid": 1.0, "double_sigmoid": 2.0}
 
 
-#: Groups of parameters by their place in the op's arguments: the branch's gains
-#: and offset, the scales, the next norm's gains and offset.
-_OFFSETS = (1, 4)
-
-
 class ResidualNormOp(torch.autograd.Function):
     """``(x', h)`` (``x'`` alone without a next norm) from the rows, the branch, the
     gates' pre-activations and the parameters, a vector a frequency; ``counts``
-    how many of ``params`` each group has, zero for a group left out."""
+    how many of ``params`` each group has (the branch's gains and offset, the
+    scales, the next norm's gains and offset), zero for a group left out."""
 
     @staticmethod
     def forward(ctx, x: Tensor, u: Tensor, z: Tensor | None, layout, factor: float, eps: float, next_eps: float,
                 counts: tuple[int, ...], *params: Tensor):
         ctx.set_materialize_grads(False)
         train = any(ctx.needs_input_grad)
-        with torch.profiler.record_function("gm::pointwise/residual_norm"):
-            y, normed, stats = _native.residual_norm_forward(x, u, z, _grouped(layout, x, counts, params), layout,
-                                                             factor, eps, next_eps, train)
+        with _native.span("gm::pointwise/residual_norm"):
+            y, normed, stats = _native.residual_norm_forward(x, u, z, counts, params, layout, factor, eps, next_eps,
+                                                             train)
         if train:
             ctx.save_for_backward(x, u, z, stats, *params)
-            ctx.layout, ctx.factor, ctx.counts = layout, factor, counts
+            ctx.rest = (layout, factor, counts)
         return y if normed is None else (y, normed)
 
     @staticmethod
@@ -66,25 +62,24 @@ class ResidualNormOp(torch.autograd.Function):
         x, u, z, stats, *params = ctx.saved_tensors
         if dy is None and dn is None:
             return (None,) * len(ctx.needs_input_grad)
-        layout, counts = ctx.layout, ctx.counts
-        with torch.profiler.record_function("gm::pointwise/residual_norm_backward"):
+        layout, factor, counts = ctx.rest
+        with _native.span("gm::pointwise/residual_norm_backward"):
             dx, du, dz, dparams = _native.residual_norm_backward(
-                None if dy is None else dy.contiguous(), None if dn is None else dn.contiguous(), x, u, z,
-                _grouped(layout, x, counts, params), stats, layout, ctx.factor)
+                None if dy is None else dy.contiguous(), None if dn is None else dn.contiguous(), x, u, z, counts,
+                params, stats, layout, factor)
+        # dparams: the groups' gradients in order, a left-out group's too
         copies, sizes, held = layout.a0 + layout.G, [], []
-        mults = ([layout.a0] if layout.a0 else []) + list(layout.mults[: layout.nf])
-        for i, count in enumerate(counts):
-            split = [layout.a0] if i in _OFFSETS else (mults if count else [copies])
-            sizes += split
-            held += [count > 0] * len(split)
+        lengths = iter(layout.parameter_slots(counts)[2])
+        for group, count in enumerate(counts):
+            sizes += [next(lengths) for _ in range(count)] if count else [layout.a0 if group in (1, 4) else copies]
+            held += [True] * count or [False]
         return (dx, du, dz, None, None, None, None, None,
                 *(g for g, h in zip(dparams.split(sizes), held, strict=True) if h))
 
 
-def _grouped(layout, x: Tensor, counts: tuple[int, ...], params) -> _native.ResidualParameters:
-    it = iter(params)
-    groups = [[next(it) for _ in range(count)] if count else None for count in counts]
-    return _native.ResidualParameters(layout, x, *(g[0] if i in _OFFSETS and g else g for i, g in enumerate(groups)))
+def _by_frequency(held: nn.ParameterDict | None) -> list[Tensor]:
+    """A dictionary's vectors in the order of the field's frequencies, in which they were entered."""
+    return [] if held is None else list(held._parameters.values())
 
 
 class SO2ResidualNorm(nn.Module):
@@ -104,7 +99,7 @@ class SO2ResidualNorm(nn.Module):
             raise ValueError(f"gate must be None or one of {tuple(_GATES)}, got {gate!r}.")
         self.field_type = field_type
         self.gate = gate
-        self.copies = sum(m for _, m in field_type.items())
+        self.width, self.copies = field_type.dimension, sum(m for _, m in field_type.items())
         kw = dict(dtype=dtype, device=device)
         self.post = SO2LayerNorm(field_type, eps=eps, bias=bias, **kw) if post_norm else None
         self.norm = SO2LayerNorm(field_type, eps=eps, bias=bias, **kw) if norm else None
@@ -139,26 +134,20 @@ class SO2ResidualNorm(nn.Module):
             self.__dict__["_pw_layout"] = layout
         return layout
 
-    def _groups(self) -> list[list[Tensor] | None]:
-        """The branch's gains and offset, the scales, the next norm's gains and
-        offset: each by frequency (an offset is one tensor), None where left out."""
-        frequencies = self.field_type.frequencies
-
-        def gains(norm: SO2LayerNorm | None) -> list[Tensor] | None:
-            return None if norm is None else [norm.gamma[str(f)] for f in frequencies]
-
-        def offset(norm: SO2LayerNorm | None) -> list[Tensor] | None:
-            return None if norm is None or not norm.has_bias else [norm.beta]
-
-        scales = None if self.scale is None else [self.scale[str(f)] for f in frequencies]
-        return [gains(self.post), offset(self.post), scales, gains(self.norm), offset(self.norm)]
+    def _params(self) -> tuple[tuple[int, ...], list[Tensor]]:
+        """``(counts, params)`` as the op takes them: every group's vectors by frequency."""
+        groups = [_by_frequency(None if self.post is None else self.post.gamma),
+                  [self.post.beta] if self.post is not None and self.post.has_bias else [],
+                  _by_frequency(self.scale), _by_frequency(None if self.norm is None else self.norm.gamma),
+                  [self.norm.beta] if self.norm is not None and self.norm.has_bias else []]
+        return tuple(map(len, groups)), [p for group in groups for p in group]
 
     def uses_hip(self, flat: Tensor) -> bool:
-        return flat.device.type == "cuda" and flat.dtype in (torch.float32, torch.float64, torch.bfloat16) \
-            and self.field_type.dimension <= MAX_WIDTH
+        return flat.is_cuda and flat.dtype in (torch.float32, torch.float64, torch.bfloat16) \
+            and self.width <= MAX_WIDTH
 
     def _check(self, rows: Tensor, branch: Tensor, pre: Tensor | None) -> None:
-        width = self.field_type.dimension
+        width = self.width
         if rows.ndim != 2 or rows.shape[1] != width:
             raise ValueError(f"rows must be (N, {width}), got {tuple(rows.shape)}.")
         if branch.shape != rows.shape:
@@ -176,13 +165,13 @@ class SO2ResidualNorm(nn.Module):
             return self._eager(rows, branch, pre)
         if branch.dtype != rows.dtype and not (rows.dtype == torch.bfloat16 and branch.dtype == torch.float32):
             branch = branch.to(rows.dtype)
-        pd, groups = _native.param_dtype(rows.dtype), self._groups()
+        pd, (counts, params) = _native.param_dtype(rows.dtype), self._params()
+        params = [p if p.dtype == pd and p.is_contiguous() else p.to(pd).contiguous() for p in params]
         out = ResidualNormOp.apply(rows.contiguous(), branch.contiguous(),
                                    None if pre is None else pre.to(rows.dtype).contiguous(), self._layout(),
                                    _GATES.get(self.gate, 1.0), self.post.eps if self.post is not None else 1.0,
                                    self.norm.eps if self.norm is not None else 1.0,
-                                   tuple(0 if group is None else len(group) for group in groups),
-                                   *(p.to(pd).contiguous() for group in groups if group is not None for p in group))
+                                   counts, *params)
         return out if self.norm is not None else (out, None)
 
     def forward(self, x: SO2FeatureField, branch: SO2FeatureField,
