@@ -42,6 +42,10 @@ constexpr int kRnMaxFreq = 8;           // nonzero frequencies
 constexpr int kRnSlots = kRnMaxFreq + 1;  // frequency 0, then the nonzero ones
 constexpr int kRnThreads = 256;
 constexpr int kRnWaves = kRnThreads / kWave;
+// The backward's workgroups: eight waves where their registers let a CU hold eight (half as many rows of sums to add
+// as with four: that kernel 17 -> 10 us), four above that.
+template <typename X, bool kCopies, int NS>
+constexpr int kRnBackThreads = NS <= (kCopies ? 4 : (sizeof(X) == 8 ? 2 : 3)) && sizeof(X) * NS <= 16 ? 512 : 256;
 constexpr int kRnMaxWidth = 1024;
 
 struct rbf16 {
@@ -210,7 +214,7 @@ struct RnUnit {
     if constexpr (kCopies) {
       g[0] = g[1] = widen(row[unit]);
     } else {
-      // selects, not a branch's stores: those went through scratch for bfloat16 (510 us against 345 for the backward of
+      // selects, not a branch's stores: those went through scratch for bfloat16 (510 us against 345 then for the backward of
       // 262,144 rows of 160 with a float branch, 189 against 108 for the forward)
       const bool scalar = unit < a.scalar_units;
       A lo[V / 2], hi[V / 2];
@@ -253,7 +257,7 @@ struct RnTables {
   A* lds;
   __device__ __forceinline__ void fill(const Args& a, A* shared) {
     lds = shared;
-    for (int k = threadIdx.x; k < a.D; k += kRnThreads) {
+    for (int k = threadIdx.x; k < a.D; k += blockDim.x) {
       const RnPlace at = place_of(a, k);
       const A s = a.scaled ? a.scale[at.slot][at.copy] : A(1);
       lds[kGain * a.D + k] = a.normalise ? s * a.gain[at.slot][at.copy] : s;
@@ -283,7 +287,19 @@ __device__ __forceinline__ A row_sum(A v, int lanes) {
   return v;
 }
 
-// Mean of the scalars and 1 / d of the numbers a row's lanes hold.
+// A lane's j-th unit of a row: past the last one it is that one once more, loaded and not stored, its numbers zeroed
+// where they would count (no branches: predicated loads waited for one another).
+struct RnLane {
+  int unit;
+  bool on, scalar;
+};
+template <typename Args>
+__device__ __forceinline__ RnLane lane_unit(const Args& a, int lane, int j) {
+  const int unit = lane + j * a.lanes;
+  return {unit < a.units ? unit : a.units - 1, unit < a.units, unit < a.scalar_units};
+}
+
+// Mean of the scalars and 1 / d of the numbers a row's lanes hold (zero past the last unit).
 template <typename X, typename U, bool kCopies, int NS>
 __device__ __forceinline__ void row_stats(const RnArgs<X, U>& a, const RnTables<X, U, kCopies>& tables, int lane,
                                           const typename RnAcc<X>::type (&v)[NS][RnUnit<X, U, kCopies>::V],
@@ -291,36 +307,50 @@ __device__ __forceinline__ void row_stats(const RnArgs<X, U>& a, const RnTables<
                                           typename RnAcc<X>::type& inv_d) {
   using A = typename RnAcc<X>::type;
   constexpr int V = RnUnit<X, U, kCopies>::V;
-  A s = A(0);
+  mean = A(0);
+  if (a.a0 > 0) {
+    A s = A(0);
 #pragma unroll
-  for (int j = 0; j < NS; ++j) {
-    if (lane + j * a.lanes < a.scalar_units) {
+    for (int j = 0; j < NS; ++j) {
+      const bool scalar = lane_unit(a, lane, j).scalar;
 #pragma unroll
-      for (int i = 0; i < V; ++i) s += v[j][i];  // a scalar copy's second number is zero
+      for (int i = 0; i < V; ++i) s += scalar ? v[j][i] : A(0);  // a scalar copy's second number is zero
     }
+    mean = row_sum(s, a.lanes) / A(a.a0);
   }
-  mean = a.a0 > 0 ? row_sum(s, a.lanes) / A(a.a0) : A(0);
   A q = A(0);
 #pragma unroll
   for (int j = 0; j < NS; ++j) {
-    const int unit = lane + j * a.lanes;
-    if (unit < a.units) {
-      A w[V];
-      tables.get(a, kShare, unit, w);
-      const A m = unit < a.scalar_units ? mean : A(0);
+    const RnLane at = lane_unit(a, lane, j);
+    A w[V];
+    tables.get(a, kShare, at.unit, w);
+    const A m = at.scalar ? mean : A(0);
 #pragma unroll
-      for (int i = 0; i < V; ++i) {
-        const A c = v[j][i] - m;
-        q += w[i] * c * c;
-      }
+    for (int i = 0; i < V; ++i) {
+      const A c = v[j][i] - m;
+      q += w[i] * c * c;
     }
   }
   inv_d = A(1) / sqrt(row_sum(q, a.lanes) + eps);
 }
 
-template <typename A>
-__device__ __forceinline__ A rn_sigmoid(A z) {
-  return A(1) / (A(1) + gm_exp(-z));
+// 1 / (1 + exp(-z)); in float from v_exp_f32 and v_rcp_f32, each a step off (the exponent's rounding |z| / 2 steps
+// more of what exp(-z) contributes): a tenth of a call's and a division's instructions.
+__device__ __forceinline__ float rn_sigmoid(float z) {
+  return __builtin_amdgcn_rcpf(1.f + __builtin_amdgcn_exp2f(-1.44269504088896340736f * z));
+}
+__device__ __forceinline__ double rn_sigmoid(double z) { return 1.0 / (1.0 + exp(-z)); }
+// The gates of a unit's numbers from their pre-activations; `pairs`: no lane's unit of this step is scalars, and a
+// pair's two numbers share one.
+template <int V, typename A>
+__device__ __forceinline__ void rn_gates(A (&g)[V], bool pairs) {
+  if (pairs) {
+#pragma unroll
+    for (int i = 0; i < V; i += 2) g[i] = g[i + 1] = rn_sigmoid(g[i]);
+  } else {
+#pragma unroll
+    for (int i = 0; i < V; ++i) g[i] = rn_sigmoid(g[i]);
+  }
 }
 
 template <typename X, typename U, bool kCopies, int NS>
@@ -342,49 +372,61 @@ __global__ __launch_bounds__(kRnThreads) void residual_norm_forward_kernel(RnArg
     A x[NS][V], u[NS][V], g[NS][V];
 #pragma unroll
     for (int j = 0; j < NS; ++j) {
-      const int unit = lane + j * a.lanes;
+      const RnLane at_j = lane_unit(a, lane, j);
+      Unit::load(a, a.u + r * a.D, at_j.unit, u[j]);
+      Unit::load(a, a.x + r * a.D, at_j.unit, x[j]);
+    }
+    if (a.z) {
 #pragma unroll
-      for (int i = 0; i < V; ++i) x[j][i] = u[j][i] = g[j][i] = A(0);
-      if (unit < a.units) {
-        Unit::load(a, a.u + r * a.D, unit, u[j]);
-        Unit::load(a, a.x + r * a.D, unit, x[j]);
-        if (a.z) Unit::load_gates(a, a.z + r * a.copies, unit, g[j]);
-      }
+      for (int j = 0; j < NS; ++j) Unit::load_gates(a, a.z + r * a.copies, lane_unit(a, lane, j).unit, g[j]);
+    }
+#pragma unroll
+    for (int j = 0; j < NS; ++j) {
+      const bool on = lane_unit(a, lane, j).on;
+#pragma unroll
+      for (int i = 0; i < V; ++i) u[j][i] = on ? u[j][i] : A(0);
     }
     A mean = A(0), inv = A(1);
     if (a.normalise) row_stats<X, U, kCopies, NS>(a, tables, lane, u, a.eps, mean, inv);
 #pragma unroll
     for (int j = 0; j < NS; ++j) {
-      const int unit = lane + j * a.lanes;
-      if (unit < a.units) {
-        A gain[V], offset[V];
-        tables.get(a, kGain, unit, gain);
-        tables.get(a, kOffset, unit, offset);
-        const A m = unit < a.scalar_units ? mean : A(0);
+      const RnLane at_j = lane_unit(a, lane, j);
+      A gain[V], offset[V];
+      tables.get(a, kGain, at_j.unit, gain);
+      tables.get(a, kOffset, at_j.unit, offset);
+      const A m = at_j.scalar ? mean : A(0);
 #pragma unroll
-        for (int i = 0; i < V; ++i) {
-          const A b = gain[i] * ((u[j][i] - m) * inv) + offset[i];
-          x[j][i] += a.z ? a.factor * rn_sigmoid(g[j][i]) * b : b;
-        }
-        if (kCopies && unit < a.a0) x[j][1] = A(0);
-        if (live) Unit::store(a, a.y + r * a.D, unit, x[j]);
+      for (int i = 0; i < V; ++i) u[j][i] = gain[i] * ((u[j][i] - m) * inv) + offset[i];
+    }
+    if (a.z) {
+#pragma unroll
+      for (int j = 0; j < NS; ++j) {
+        rn_gates<V>(g[j], j * a.lanes >= a.scalar_units);
+#pragma unroll
+        for (int i = 0; i < V; ++i) u[j][i] *= a.factor * g[j][i];
       }
+    }
+#pragma unroll
+    for (int j = 0; j < NS; ++j) {
+      const RnLane at_j = lane_unit(a, lane, j);
+#pragma unroll
+      for (int i = 0; i < V; ++i) x[j][i] = at_j.on ? x[j][i] + u[j][i] : A(0);
+      if (kCopies && at_j.scalar) x[j][1] = A(0);
+      if (live && at_j.on) Unit::store(a, a.y + r * a.D, at_j.unit, x[j]);
     }
     A mean2 = A(0), inv2 = A(1);
     if (a.next) {
       row_stats<X, U, kCopies, NS>(a, tables, lane, x, a.next_eps, mean2, inv2);
 #pragma unroll
       for (int j = 0; j < NS; ++j) {
-        const int unit = lane + j * a.lanes;
-        if (unit < a.units) {
-          A gain[V], offset[V], out[V];
-          tables.get(a, kNextGain, unit, gain);
-          tables.get(a, kNextOffset, unit, offset);
-          const A m = unit < a.scalar_units ? mean2 : A(0);
+        const RnLane at_j = lane_unit(a, lane, j);
+        A gain[V], offset[V], out[V];
+        tables.get(a, kNextGain, at_j.unit, gain);
+        tables.get(a, kNextOffset, at_j.unit, offset);
+        const A m = at_j.scalar ? mean2 : A(0);
 #pragma unroll
-          for (int i = 0; i < V; ++i) out[i] = gain[i] * ((x[j][i] - m) * inv2) + offset[i];
-          if (live) Unit::store(a, a.normed + r * a.D, unit, out);
-        }
+        for (int i = 0; i < V; ++i) out[i] = gain[i] * ((x[j][i] - m) * inv2) + offset[i];
+        if (live && at_j.on) Unit::store(a, a.normed + r * a.D, at_j.unit, out);
       }
     }
     if (a.stats && live && lane == 0) {
@@ -398,18 +440,18 @@ __global__ __launch_bounds__(kRnThreads) void residual_norm_forward_kernel(RnArg
 }
 
 template <typename X, typename U, bool kCopies, int NS>
-__global__ __launch_bounds__(kRnThreads) void residual_norm_backward_kernel(RnArgs<X, U> a) {
+__global__ __launch_bounds__((kRnBackThreads<X, kCopies, NS>)) void residual_norm_backward_kernel(RnArgs<X, U> a) {
   using A = typename RnAcc<X>::type;
   using Unit = RnUnit<X, U, kCopies>;
-  constexpr int V = Unit::V;
+  constexpr int V = Unit::V, kThreads = kRnBackThreads<X, kCopies, NS>, kWaves = kThreads / kWave;
   extern __shared__ __align__(16) unsigned char rn_lds[];
   RnTables<X, U, kCopies> tables;
   tables.fill(a, reinterpret_cast<A*>(rn_lds));
   const int in_wave = threadIdx.x % kWave, lane = in_wave & (a.lanes - 1);
   const int per_wave = kWave >> a.shift;
-  const int64_t step = (int64_t)gridDim.x * kRnWaves * per_wave;
+  const int64_t step = (int64_t)gridDim.x * kWaves * per_wave;
   const A by_scalars = a.a0 > 0 ? A(1) / A(a.a0) : A(0);
-  // the sums over this lane's rows: G act uhat, G act, dn xhat, dn
+  // the sums over this lane's rows: G act uhat, G act, dn xhat, dn (the second and fourth are read of scalars only)
   A sums[4][NS][V];
 #pragma unroll
   for (int t = 0; t < 4; ++t)
@@ -417,7 +459,7 @@ __global__ __launch_bounds__(kRnThreads) void residual_norm_backward_kernel(RnAr
     for (int j = 0; j < NS; ++j)
 #pragma unroll
       for (int i = 0; i < V; ++i) sums[t][j][i] = A(0);
-  int64_t row = ((int64_t)blockIdx.x * kRnWaves + threadIdx.x / kWave) * per_wave + (in_wave >> a.shift);
+  int64_t row = ((int64_t)blockIdx.x * kWaves + threadIdx.x / kWave) * per_wave + (in_wave >> a.shift);
   for (int64_t at = row - (in_wave >> a.shift); at < a.n_rows; at += step, row += step) {
     const bool live = row < a.n_rows;
     const int64_t r = live ? row : a.n_rows - 1;
@@ -426,108 +468,120 @@ __global__ __launch_bounds__(kRnThreads) void residual_norm_backward_kernel(RnAr
     A uh[NS][V], G[NS][V], act[NS][V], xh[NS][V], dn[NS][V];
 #pragma unroll
     for (int j = 0; j < NS; ++j) {
-      const int unit = lane + j * a.lanes;
+      Unit::load(a, a.u + r * a.D, lane_unit(a, lane, j).unit, uh[j]);
 #pragma unroll
-      for (int i = 0; i < V; ++i) uh[j][i] = G[j][i] = xh[j][i] = dn[j][i] = act[j][i] = A(0);
-      if (unit < a.units) {
-        Unit::load(a, a.u + r * a.D, unit, uh[j]);
-        if (a.z) Unit::load_gates(a, a.z + r * a.copies, unit, act[j]);
-        if (a.dy) Unit::load(a, a.dy + r * a.D, unit, G[j]);
-        if (a.dn) {
-          Unit::load(a, a.x + r * a.D, unit, xh[j]);
-          Unit::load(a, a.dn + r * a.D, unit, dn[j]);
-        }
-      }
-    }
-    // uhat, and xhat from the sum formed again; p and m, the next norm's two sums
-    A p = A(0), m = A(0);
-#pragma unroll
-    for (int j = 0; j < NS; ++j) {
-      const int unit = lane + j * a.lanes;
-      if (unit < a.units) {
-        const bool scalar = unit < a.scalar_units;
-#pragma unroll
-        for (int i = 0; i < V; ++i) {
-          uh[j][i] = (uh[j][i] - (scalar ? mean : A(0))) * inv;
-          act[j][i] = a.z ? rn_sigmoid(act[j][i]) : A(1);
-        }
-        if (a.dn) {
-          A gain[V], offset[V], next[V];
-          tables.get(a, kGain, unit, gain);
-          tables.get(a, kOffset, unit, offset);
-          tables.get(a, kNextGain, unit, next);
-#pragma unroll
-          for (int i = 0; i < V; ++i) {
-            const A b = gain[i] * uh[j][i] + offset[i];
-            const A y = xh[j][i] + (a.z ? a.factor * act[j][i] * b : b);
-            xh[j][i] = (y - (scalar ? mean2 : A(0))) * inv2;
-            const A gh = next[i] * dn[j][i];
-            p += gh * xh[j][i];
-            if (scalar) m += gh;
-          }
-        }
+      for (int i = 0; i < V; ++i) {
+        G[j][i] = A(0);
+        act[j][i] = A(1);
       }
     }
     if (a.dn) {
+#pragma unroll
+      for (int j = 0; j < NS; ++j) {
+        const int unit = lane_unit(a, lane, j).unit;
+        Unit::load(a, a.x + r * a.D, unit, xh[j]);
+        Unit::load(a, a.dn + r * a.D, unit, dn[j]);
+      }
+    }
+    if (a.dy) {
+#pragma unroll
+      for (int j = 0; j < NS; ++j) Unit::load(a, a.dy + r * a.D, lane_unit(a, lane, j).unit, G[j]);
+    }
+    if (a.z) {
+#pragma unroll
+      for (int j = 0; j < NS; ++j) Unit::load_gates(a, a.z + r * a.copies, lane_unit(a, lane, j).unit, act[j]);
+#pragma unroll
+      for (int j = 0; j < NS; ++j) rn_gates<V>(act[j], j * a.lanes >= a.scalar_units);
+    }
+    const A factor = a.z ? a.factor : A(1);
+#pragma unroll
+    for (int j = 0; j < NS; ++j) {
+      const RnLane at_j = lane_unit(a, lane, j);
+      const bool counts = at_j.on && live;
+#pragma unroll
+      for (int i = 0; i < V; ++i) {
+        uh[j][i] = at_j.on ? (uh[j][i] - (at_j.scalar ? mean : A(0))) * inv : A(0);
+        G[j][i] = counts ? G[j][i] : A(0);
+      }
+    }
+    // xhat from the sum formed again; p and m, the next norm's two sums; its part of G
+    if (a.dn) {
+      A p = A(0), m = A(0);
+#pragma unroll
+      for (int j = 0; j < NS; ++j) {
+        const RnLane at_j = lane_unit(a, lane, j);
+        const bool counts = at_j.on && live;
+        A gain[V], offset[V], next[V];
+        tables.get(a, kGain, at_j.unit, gain);
+        tables.get(a, kOffset, at_j.unit, offset);
+        tables.get(a, kNextGain, at_j.unit, next);
+#pragma unroll
+        for (int i = 0; i < V; ++i) {
+          const A y = xh[j][i] + factor * act[j][i] * (gain[i] * uh[j][i] + offset[i]);
+          xh[j][i] = (y - (at_j.scalar ? mean2 : A(0))) * inv2;
+          dn[j][i] = counts ? dn[j][i] : A(0);
+          sums[2][j][i] += dn[j][i] * xh[j][i];
+          sums[3][j][i] += dn[j][i];
+          dn[j][i] *= next[i];
+          p += dn[j][i] * xh[j][i];
+          m += at_j.scalar ? dn[j][i] : A(0);
+        }
+      }
       p = row_sum(p, a.lanes);
       m = row_sum(m, a.lanes) * by_scalars;
+#pragma unroll
+      for (int j = 0; j < NS; ++j) {
+        const RnLane at_j = lane_unit(a, lane, j);
+        A w[V];
+        tables.get(a, kShare, at_j.unit, w);
+#pragma unroll
+        for (int i = 0; i < V; ++i) {
+          const A d = inv2 * (dn[j][i] - (at_j.scalar ? m : A(0)) - p * xh[j][i] * w[i]);
+          G[j][i] += at_j.on ? d : A(0);
+        }
+        if (kCopies && at_j.scalar) G[j][1] = A(0);
+      }
     }
     A p1 = A(0), m1 = A(0);
 #pragma unroll
     for (int j = 0; j < NS; ++j) {
-      const int unit = lane + j * a.lanes;
-      if (unit < a.units) {
-        const bool scalar = unit < a.scalar_units;
-        A gain[V], offset[V], d[V];
-        if (a.dn) {
-          A next[V], w[V];
-          tables.get(a, kNextGain, unit, next);
-          tables.get(a, kShare, unit, w);
+      const RnLane at_j = lane_unit(a, lane, j);
+      A gain[V], offset[V], d[V];
+      if (live && at_j.on) Unit::store(a, a.dx + r * a.D, at_j.unit, G[j]);
+      tables.get(a, kGain, at_j.unit, gain);
+      tables.get(a, kOffset, at_j.unit, offset);
 #pragma unroll
-          for (int i = 0; i < V; ++i)
-            G[j][i] += inv2 * (next[i] * dn[j][i] - (scalar ? m : A(0)) - p * xh[j][i] * w[i]);
-        }
-        if (kCopies && scalar) G[j][1] = A(0);
-        if (live) Unit::store(a, a.dx + r * a.D, unit, G[j]);
-        tables.get(a, kGain, unit, gain);
-        tables.get(a, kOffset, unit, offset);
-#pragma unroll
-        for (int i = 0; i < V; ++i) {
-          const A s = act[j][i], f = a.z ? a.factor * s : A(1);
-          d[i] = G[j][i] * (gain[i] * uh[j][i] + offset[i]) * f * (A(1) - s);  // of the gate's argument
-          G[j][i] *= f;
-          if (live) {
-            sums[0][j][i] += G[j][i] * uh[j][i];
-            if (scalar) sums[1][j][i] += G[j][i];
-            if (a.dn) {
-              sums[2][j][i] += dn[j][i] * xh[j][i];
-              if (scalar) sums[3][j][i] += dn[j][i];
-            }
-          }
-          G[j][i] *= gain[i];
-          p1 += G[j][i] * uh[j][i];
-          if (scalar) m1 += G[j][i];
-        }
-        if (a.z && live) Unit::store_gates(a, a.dz + r * a.copies, unit, d);
+      for (int i = 0; i < V; ++i) {
+        const A s = act[j][i];
+        G[j][i] *= factor * s;
+        d[i] = G[j][i] * (gain[i] * uh[j][i] + offset[i]) * (A(1) - s);  // of the gate's argument
+        sums[0][j][i] += G[j][i] * uh[j][i];
+        sums[1][j][i] += G[j][i];
+        G[j][i] *= gain[i];
+        p1 += G[j][i] * uh[j][i];
+        m1 += at_j.scalar ? G[j][i] : A(0);
+      }
+      if (a.z) {
+        if (live && at_j.on) Unit::store_gates(a, a.dz + r * a.copies, at_j.unit, d);
       }
     }
     if (a.normalise) {
       p1 = row_sum(p1, a.lanes);
       m1 = row_sum(m1, a.lanes) * by_scalars;
+#pragma unroll
+      for (int j = 0; j < NS; ++j) {
+        const RnLane at_j = lane_unit(a, lane, j);
+        A w[V];
+        tables.get(a, kShare, at_j.unit, w);
+#pragma unroll
+        for (int i = 0; i < V; ++i)
+          G[j][i] = inv * (G[j][i] - (at_j.scalar ? m1 : A(0)) - p1 * uh[j][i] * w[i]);
+      }
     }
 #pragma unroll
     for (int j = 0; j < NS; ++j) {
-      const int unit = lane + j * a.lanes;
-      if (unit < a.units) {
-        if (a.normalise) {
-          A w[V];
-          tables.get(a, kShare, unit, w);
-#pragma unroll
-          for (int i = 0; i < V; ++i)
-            G[j][i] = inv * (G[j][i] - (unit < a.scalar_units ? m1 : A(0)) - p1 * uh[j][i] * w[i]);
-        }
-        if (live) Unit::store(a, a.du + r * a.D, unit, G[j]);
-      }
+      const RnLane at_j = lane_unit(a, lane, j);
+      if (live && at_j.on) Unit::store(a, a.du + r * a.D, at_j.unit, G[j]);
     }
   }
   // over the wave's rows, then over the workgroup's waves in order
@@ -542,7 +596,7 @@ __global__ __launch_bounds__(kRnThreads) void residual_norm_backward_kernel(RnAr
       for (int i = 0; i < V; ++i)
         for (int o = a.lanes; o < kWave; o <<= 1) sums[t][j][i] += __shfl_xor(sums[t][j][i], o, kWave);
     __syncthreads();  // the coefficients, and the last table's sums, have been read
-    for (int w = 0; w < kRnWaves; ++w) {
+    for (int w = 0; w < kWaves; ++w) {
       if (wave == w && in_wave < a.lanes) {
 #pragma unroll
         for (int j = 0; j < NS; ++j) {
@@ -558,19 +612,19 @@ __global__ __launch_bounds__(kRnThreads) void residual_norm_backward_kernel(RnAr
       }
       __syncthreads();
     }
-    for (int k = threadIdx.x; k < width; k += kRnThreads)
+    for (int k = threadIdx.x; k < width; k += kThreads)
       a.partial[((int64_t)blockIdx.x * 4 + t) * width + k] = shared[k];
   }
 }
 
 // The parameters' gradients from the workgroups' sums: kRnCols copies a workgroup, kParts threads a copy, each over
-// every kParts-th row in order, then in order over the threads.
+// every kParts-th row in order, then over the threads in a fixed order.
 constexpr int kRnCols = 4;
 template <typename X, typename U, bool kCopies>
 __global__ __launch_bounds__(kRnThreads) void residual_norm_reduce_kernel(RnArgs<X, U> a, int64_t blocks) {
   using A = typename RnAcc<X>::type;
   constexpr int V = RnUnit<X, U, kCopies>::V, kParts = kRnThreads / kRnCols;
-  __shared__ A part[4][kParts][kRnCols];
+  __shared__ A part[4][kRnWaves][kRnCols];
   const int col = threadIdx.x % kRnCols, from = threadIdx.x / kRnCols;
   const int c = blockIdx.x * kRnCols + col, width = a.units * V;
   const bool live = c < a.copies, scalar = c < a.a0;
@@ -587,14 +641,17 @@ __global__ __launch_bounds__(kRnThreads) void residual_norm_reduce_kernel(RnArgs
       }
   }
 #pragma unroll
-  for (int t = 0; t < 4; ++t) part[t][from][col] = s[t];
+  for (int t = 0; t < 4; ++t) {
+    for (int o = kRnCols; o < kWave; o <<= 1) s[t] += __shfl_xor(s[t], o, kWave);
+    if (threadIdx.x % kWave < kRnCols) part[t][threadIdx.x / kWave][col] = s[t];
+  }
   __syncthreads();
   if (from != 0 || !live) return;
 #pragma unroll
   for (int t = 0; t < 4; ++t) {
     s[t] = A(0);
-#pragma unroll 8
-    for (int w = 0; w < kParts; ++w) s[t] += part[t][w][col];
+#pragma unroll
+    for (int w = 0; w < kRnWaves; ++w) s[t] += part[t][w][col];
   }
   const RnPlace p = place_of(a, scalar ? c : 2 * c - a.a0);
   const A scale = a.scaled ? a.scale[p.slot][p.copy] : A(1), gain = a.normalise ? a.gain[p.slot][p.copy] : A(1);
@@ -618,21 +675,22 @@ constexpr int kMaxUnits = kCopies ? 16 : (sizeof(X) == 8 ? 8 : 5);
 template <typename X, typename U, bool kCopies, int NS>
 int launch_rn(bool backward, const RnArgs<X, U>& a, hipStream_t stream, int64_t& blocks) {
   using A = typename RnAcc<X>::type;
-  const int64_t rows_per_block = (int64_t)kRnWaves * (kWave >> a.shift);
+  constexpr int kBack = kRnBackThreads<X, kCopies, NS>;
+  const int threads = backward ? kBack : kRnThreads;
+  const int64_t rows_per_block = (int64_t)(threads / kWave) * (kWave >> a.shift);
   const int width = a.units * RnUnit<X, U, kCopies>::V;
   const size_t lds = sizeof(A) * std::max<size_t>((size_t)kTables * a.D, backward ? width : 0);
   const void* kernel = backward ? reinterpret_cast<const void*>(&residual_norm_backward_kernel<X, U, kCopies, NS>)
                                 : reinterpret_cast<const void*>(&residual_norm_forward_kernel<X, U, kCopies, NS>);
   const int64_t want = (a.n_rows + rows_per_block - 1) / rows_per_block;
-  const int64_t slots = resident_blocks(kernel, kRnThreads, lds);
-  // the backward writes a row of sums a workgroup: as many as the caller's array was sized for
+  // the backward writes a row of sums a workgroup: as many as the caller's array was sized for, and no more than the
+  // CUs hold at once
+  const int64_t slots = resident_blocks(kernel, threads, lds);
+  blocks = std::min<int64_t>(want, backward ? std::min<int64_t>(blocks, kBack == 512 ? 256 : 512)
+                                            : (slots > 0 ? slots : 1024));
   if (backward)
-    blocks = std::min<int64_t>(want, blocks);
-  else
-    blocks = std::min<int64_t>(want, slots > 0 ? slots : 1024);
-  if (backward)
-    hipLaunchKernelGGL((residual_norm_backward_kernel<X, U, kCopies, NS>), dim3((unsigned)blocks), dim3(kRnThreads),
-                       lds, stream, a);
+    hipLaunchKernelGGL((residual_norm_backward_kernel<X, U, kCopies, NS>), dim3((unsigned)blocks), dim3(kBack), lds,
+                       stream, a);
   else
     hipLaunchKernelGGL((residual_norm_forward_kernel<X, U, kCopies, NS>), dim3((unsigned)blocks), dim3(kRnThreads),
                        lds, stream, a);
@@ -741,7 +799,7 @@ int take_parameters(RnArgs<X, U>& a, const void* const* params) {
   return GM_OK;
 }
 
-constexpr int64_t kRnMaxBlocks = 512;  // two workgroups a CU: what the backward's registers leave room for
+constexpr int64_t kRnMaxBlocks = 512;  // two of four waves a CU: what the backward's registers leave room for
 
 int64_t rn_blocks(int64_t n_rows) {
   // at least 32 rows a workgroup, so that few rows do not leave many rows of sums to add
