@@ -13,7 +13,9 @@ signatures and call structure:
   ``_attend_batched`` (:858-909): the heads' stacked query and key maps
   (:653-669), the scores and softmax of every head in one fused op, the value
   kernels in the factored order with one shared source grouping
-  (``_aggregated_factored``, :801-822).
+  (``_aggregated_factored``, :801-822).  With ``differential`` (no reference
+  counterpart) a head's weights are the difference of two softmax maps over the
+  halves of its query and key copies (``nn.differential``).
 
 Every score, softmax and value aggregation runs in the HIP ops
 (``fused_attention.Softmax``, ``fused_factored.FactoredAggregate``; under
@@ -37,7 +39,7 @@ import torch.utils.checkpoint
 from torch import Tensor, nn
 
 from gm_attention_amd.discretization.discretization import SphericalDiscretization
-from gm_attention_amd.nn import assembly, fused_attention, fused_factored, kernels, radial
+from gm_attention_amd.nn import assembly, differential, fused_attention, fused_factored, kernels, radial
 from gm_attention_amd.nn.kernels import SO2SteerableKernel
 from gm_attention_amd.nn.linear import (
     FlatLinear, SO2Linear, apply_linear, block_matrix, flat_bias, linear_parameters, matrix_and_bias, weights_matrix,
@@ -160,8 +162,8 @@ class SO2Attention(nn.Module):
 class SO2MHSA(nn.Module):
     def __init__(self, field_type_in: SO2FieldType, num_heads: int, *, cutoff: float, window: str = "hard",
                  n_radial_basis: int = 8, radial_hidden_features: Sequence[int] = (16,), radial_basis: str = "gaussian",
-                 bias: bool = True, batched: bool = False, value_kind: str = "steerable", dtype=None,
-                 device=None) -> None:
+                 bias: bool = True, batched: bool = False, value_kind: str = "steerable", differential: bool = False,
+                 lambda_init: float = 0.8, dtype=None, device=None) -> None:
         super().__init__()
         if num_heads < 1:
             raise ValueError(f"num_heads must be at least 1, got {num_heads}.")
@@ -169,7 +171,16 @@ class SO2MHSA(nn.Module):
         if offending:
             raise ValueError(f"num_heads ({num_heads}) must divide the multiplicity of every present frequency; "
                              f"offending frequencies (as frequency: multiplicity): {offending}.")
+        if differential:
+            if not batched:
+                raise ValueError("differential attention scores every head at once: it needs batched=True.")
+            odd = {f: m for f, m in field_type_in.items() if m % (2 * num_heads) != 0}
+            if odd:
+                raise ValueError(f"twice num_heads ({2 * num_heads}) must divide the multiplicity of every present "
+                                 f"frequency of a differential layer; offending frequencies (as frequency: "
+                                 f"multiplicity): {odd}.")
         self.batched = bool(batched)
+        self.differential = bool(differential)
         self.value_kind = value_kind
         self.field_type_in = field_type_in
         self.num_heads = num_heads
@@ -181,6 +192,21 @@ class SO2MHSA(nn.Module):
                          radial_basis=radial_basis, bias=bias, value_kind=value_kind, dtype=dtype, device=device)
             for _ in range(num_heads)])
         self.output_projection = SO2Linear(field_type_in, field_type_in, bias=bias, dtype=dtype, device=device)
+        if differential:
+            self.field_type_map = SO2FieldType({f: m // (2 * num_heads) for f, m in field_type_in.items()})
+            self.lambda_init = float(lambda_init)
+            shape = (2, num_heads, self.field_type_map.dimension)
+            self.lambda_query = nn.Parameter(torch.empty(shape, dtype=dtype, device=device))
+            self.lambda_key = nn.Parameter(torch.empty(shape, dtype=dtype, device=device))
+            for p in (self.lambda_query, self.lambda_key):
+                nn.init.normal_(p, std=0.1)
+
+    def lambdas(self) -> Tensor:
+        """A differential layer's factors ``(n_heads,)`` of the second maps:
+        ``exp <q_1, k_1> - exp <q_2, k_2> + lambda_init`` of learned vectors a head
+        (the differential transformer's parametrisation, arXiv 2410.05258)."""
+        first, second = (self.lambda_query * self.lambda_key).sum(-1).exp().unbind(0)
+        return first - second + self.lambda_init
 
     def forward(self, x: SO2FeatureField, edges) -> SO2FeatureField:
         edges = _resolve_edges(edges, self.cutoff)
@@ -195,6 +221,12 @@ class SO2MHSA(nn.Module):
 
     def forward_chunked(self, x: SO2FeatureField, edges, *, chunk_size: int) -> SO2FeatureField:
         edges = _resolve_edges(edges, self.cutoff)
+        if self.differential:  # every head at once, over the same ranges
+            _validate_node_field(x, self.field_type_in, edges)
+            partials = [_checkpointed(self, functools.partial(_attend_batched, self, x, chunk))
+                        for chunk in edges.chunks(chunk_size)]
+            return self.output_projection(SO2FeatureField(
+                self.field_type_in, sum_partials(partials) if partials else _attend_batched(self, x, edges)))
         outs = [cast(SO2Attention, h).forward_chunked(x, edges, chunk_size=chunk_size) for h in self.heads]
         return self.output_projection(_concatenate_heads(outs, self.field_type_in))
 
@@ -321,8 +353,15 @@ def batched_flat_serves(mhsa: SO2MHSA, x: SO2FeatureField, edges) -> bool:
         return False
     edges = _resolve_edges(edges, mhsa.cutoff)
     values = [cast(SO2SteerableKernel, head.value) for head in mhsa.heads]
-    return (fused_attention.softmax_enabled(mhsa, x, edges) and kernels.factored_enabled()
+    return (_scores_enabled(mhsa, x, edges) and kernels.factored_enabled()
             and fused_factored.enabled(values[0], x, edges))
+
+
+def _scores_enabled(mhsa: SO2MHSA, x: SO2FeatureField, edges) -> bool:
+    """Whether the layer's scores and softmax take their fused op."""
+    if mhsa.differential:
+        return differential.enabled(mhsa, x, edges)
+    return fused_attention.softmax_enabled(mhsa, x, edges)
 
 
 def _attend_batched_flat(mhsa: SO2MHSA, x: SO2FeatureField, edges) -> Tensor | None:
@@ -333,7 +372,7 @@ def _attend_batched_flat(mhsa: SO2MHSA, x: SO2FeatureField, edges) -> Tensor | N
     in the heads' column order -- no per-frequency splits or concatenations."""
     heads = [cast(SO2Attention, h) for h in mhsa.heads]
     values = [cast(SO2SteerableKernel, head.value) for head in heads]
-    if (not fused_attention.softmax_enabled(mhsa, x, edges) or not kernels.factored_enabled()
+    if (not _scores_enabled(mhsa, x, edges) or not kernels.factored_enabled()
             or not fused_factored.enabled(values[0], x, edges)):
         return None
     rows = x._rows()
@@ -350,7 +389,8 @@ def _attend_batched_flat(mhsa: SO2MHSA, x: SO2FeatureField, edges) -> Tensor | N
         else:
             queries = _stacked_flat([h.query for h in heads], mhsa.field_type_in, rows)
             keys = _stacked_flat([h.key for h in heads], mhsa.field_type_in, rows)
-        alpha = fused_attention.softmax(mhsa, queries, keys, edges)  # (n_edges, n_heads)
+        weights = differential.attention_weights if mhsa.differential else fused_attention.softmax
+        alpha = weights(mhsa, queries, keys, edges)  # (n_edges, n_heads)
         groups = fused_factored.groups_for(edges, edges.source_index)
         if fused_trunk:
             h, trunk = None, functools.partial(radial.trunk_hidden_heads, values,
@@ -373,7 +413,9 @@ def _attend_batched(mhsa: SO2MHSA, x: SO2FeatureField, edges) -> dict[int, Tenso
     with torch.profiler.record_function("gm::attention/attend"):
         queries = _stacked_projection([h.query for h in heads], x)
         keys = _stacked_projection([h.key for h in heads], x)
-        if fused_attention.softmax_enabled(mhsa, x, edges):
+        if mhsa.differential:
+            alpha = differential.attention_weights(mhsa, queries._rows(), keys._rows(), edges)
+        elif fused_attention.softmax_enabled(mhsa, x, edges):
             alpha = fused_attention.softmax(mhsa, queries._rows(), keys._rows(), edges)  # (n_edges, n_heads)
         else:  # the reference's eager weights (attention.py:880-886)
             alpha = fused_attention.softmax_eager(fused_attention.plan(mhsa), queries._rows(), keys._rows(), edges,

@@ -21,6 +21,16 @@ float32, the feed-forward GEMMs run in bfloat16 with float accumulation, and
 the mixer, whose kernels are float32, takes its input rounded up to float32 and
 hands back float32 that the residual addition rounds to bfloat16.
 
+``norm_placement="sandwich"`` (no reference counterpart) normalises each
+sub-layer's output too, scaled and gated per copy on request,
+
+    x' = x + s_1 * act(z_1) * LN(Drop(Mixer(h))),   h = LN(x),  h' = LN(x'),
+    x'' = x' + s_2 * act(z_2) * LN(Drop(W_2 sigma(W_1 h'))),
+
+each sum with the norms around it one HIP pass (``nn.residual``); ``z`` is affine
+in the scalars of the sub-layer's input.  ``attention_differential`` makes the
+batched attention's weights differences of two softmax maps (``nn.differential``).
+
 ``IcoEncode`` / ``EquiEncode`` (reference :359-505, :799-869) restrict a
 field from a fine grid onto a coarse one over bipartite edges
 (``discretization.hierarchy``): the steerable-kernel integral of
@@ -45,10 +55,12 @@ from gm_attention_amd.nn import ffn
 from gm_attention_amd.nn.linear import SO2Linear, flat_forward
 from gm_attention_amd.nn.nonlinearities import SO2ScalarGatedNonlinearity
 from gm_attention_amd.nn.normalization import SO2Dropout, SO2LayerNorm
+from gm_attention_amd.nn.residual import SO2ResidualNorm
 from gm_attention_amd.representations.field_type import SO2FeatureField, SO2FieldType
 
 MixerKind = Literal["attention", "convolution"]
 NonlinearityKind = Literal["scalar_gate", "scalar_gate_double_sigmoid"]
+NormPlacement = Literal["pre", "sandwich"]
 
 _FFN_MULTIPLIER_DEFAULT = 2
 
@@ -75,7 +87,10 @@ class SO2TransformerBlock(nn.Module):
                  n_radial_basis: int = 8, radial_hidden_features=(16,), radial_basis: str = "gaussian",
                  dropout: float = 0.0, eps: float = 1e-5, bias: bool = True,
                  nonlinearity: NonlinearityKind = "scalar_gate_double_sigmoid", mixer: MixerKind = "attention",
-                 attention_batched: bool = False, value_kind: str = "steerable", dtype=None, device=None) -> None:
+                 attention_batched: bool = False, value_kind: str = "steerable",
+                 attention_differential: bool = False, norm_placement: NormPlacement = "pre",
+                 residual_gate: str | None = None, residual_scale: float | None = None, dtype=None,
+                 device=None) -> None:
         super().__init__()
         if not isinstance(field_type, SO2FieldType):
             raise TypeError(f"field_type must be an SO2FieldType, got {type(field_type).__name__}.")
@@ -89,7 +104,16 @@ class SO2TransformerBlock(nn.Module):
             raise ValueError(f"nonlinearity must be one of {tuple(_NONLINEARITIES)}, got {nonlinearity!r}.")
         if mixer not in ("attention", "convolution"):
             raise ValueError(f"mixer must be 'attention' or 'convolution', got {mixer!r}.")
+        if norm_placement not in ("pre", "sandwich"):
+            raise ValueError(f"norm_placement must be 'pre' or 'sandwich', got {norm_placement!r}.")
+        if norm_placement == "pre" and (residual_gate is not None or residual_scale is not None):
+            raise ValueError("residual_gate and residual_scale belong to norm_placement='sandwich'.")
+        if residual_gate is not None and 0 not in field_type:
+            raise ValueError(f"residual_gate needs frequency-0 channels to condition its gates on, got {field_type!r}.")
+        if attention_differential and mixer != "attention":
+            raise ValueError("attention_differential needs mixer='attention'.")
         self.nonlinearity = nonlinearity
+        self.norm_placement = norm_placement
         self.field_type = field_type
         self.hidden_field_type = hidden_field_type if hidden_field_type is not None else field_type.scaled(ffn_multiplier)
         self.mixer = mixer
@@ -100,14 +124,19 @@ class SO2TransformerBlock(nn.Module):
             self.attention = SO2MHSA(field_type, num_heads, cutoff=cutoff, window=window,
                                       n_radial_basis=n_radial_basis, radial_hidden_features=radial_hidden_features,
                                       radial_basis=radial_basis, bias=bias, batched=attention_batched,
-                                      value_kind=value_kind, **kw)
+                                      value_kind=value_kind, differential=attention_differential, **kw)
         else:
             self.attention = SO2Convolution(field_type, field_type, cutoff=cutoff, window=window,
                                             self_interaction="none", n_radial_basis=n_radial_basis,
                                             radial_hidden_features=radial_hidden_features,
                                             radial_basis=radial_basis, bias=bias, **kw)
         self.attention_dropout = SO2Dropout(field_type, p=dropout)
-        self.norm2 = SO2LayerNorm(field_type, eps=eps, bias=bias, **kw)
+        if norm_placement == "pre":
+            self.norm2 = SO2LayerNorm(field_type, eps=eps, bias=bias, **kw)
+        else:
+            residual = dict(eps=eps, bias=bias, gate=residual_gate, scale=residual_scale, **kw)
+            self.residual1 = SO2ResidualNorm(field_type, **residual)
+            self.residual2 = SO2ResidualNorm(field_type, norm=False, **residual)
         self.linear1 = SO2Linear(field_type, self.hidden_field_type, bias=bias, **kw)
         self.activation = build_nonlinearity(nonlinearity, self.hidden_field_type, **kw)
         self.linear2 = SO2Linear(self.hidden_field_type, field_type, bias=bias, **kw)
@@ -146,7 +175,10 @@ class SO2TransformerBlock(nn.Module):
 
     def forward_flat(self, rows: Tensor, edges, chunk_size: int | None = None) -> Tensor:
         """The block on flat rows ``(N, D)``; returns ``(N, D)`` in the rows' dtype."""
-        attended = self._mix(self.norm1.forward_flat(rows), edges, chunk_size)
+        normed = self.norm1.forward_flat(rows)
+        attended = self._mix(normed, edges, chunk_size)
+        if self.norm_placement == "sandwich":
+            return self._sandwich(rows, normed, attended)
         rows = rows + self.attention_dropout.forward_flat(attended).to(rows.dtype)
         if ffn.serves(self, rows):  # bfloat16 rows: the whole feed-forward as one fused pass per direction
             return ffn.forward(self, rows)
@@ -155,9 +187,23 @@ class SO2TransformerBlock(nn.Module):
         hidden = flat_forward(self.linear2, hidden)
         return rows + self.mlp_dropout.forward_flat(hidden)
 
+    def _sandwich(self, rows: Tensor, normed: Tensor, attended: Tensor) -> Tensor:
+        """The sums and the feed-forward of a block that normalises before and after its sub-layers."""
+        a0 = self.field_type.multiplicity(0) if 0 in self.field_type else 0
+
+        def gates(residual: SO2ResidualNorm, given: Tensor) -> Tensor | None:
+            return None if residual.gate is None else residual.pre_activations(given[:, :a0])
+
+        rows, normed2 = self.residual1.forward_flat(rows, self.attention_dropout.forward_flat(attended),
+                                                    gates(self.residual1, normed))
+        hidden = flat_forward(self.linear2, self.activation.forward_flat(flat_forward(self.linear1, normed2)))
+        return self.residual2.forward_flat(rows, self.mlp_dropout.forward_flat(hidden),
+                                           gates(self.residual2, normed2))[0]
+
     def extra_repr(self) -> str:
+        placement = "" if self.norm_placement == "pre" else f", norm_placement={self.norm_placement!r}"
         return (f"field_type={self.field_type!r}, hidden_field_type={self.hidden_field_type!r}, "
-                f"nonlinearity={self.nonlinearity!r}")
+                f"nonlinearity={self.nonlinearity!r}{placement}")
 
 
 class IcoEncode(nn.Module):

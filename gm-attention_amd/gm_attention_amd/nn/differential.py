@@ -256,6 +256,46 @@ def differential_softmax(q: Tensor, k: Tensor, lam: Tensor, tables: EdgeTables, 
     return DifferentialSoftmax.apply(_whole(q), _whole(k), lam.to(table).contiguous(), tables, maps, scale)
 
 
+def enabled(mhsa: Any, x: Any, edges: Any) -> bool:
+    """Whether a differential layer's scores take the fused op on the GPU."""
+    if fused_attention.MODE == "0" or x.device.type != "cuda" or edges.n_edges == 0:
+        return False
+    if x.dtype not in (torch.float32, torch.float64, torch.bfloat16) or mhsa.num_heads > MAX_H:
+        return False
+    maps = mhsa.field_type_map
+    return (len(maps) <= MAX_F and mhsa.field_type_in.dimension <= MAX_D
+            and maps.max_frequency <= edges.max_frequency)
+
+
+def edge_tables(edges: Any, cutoff: float, window: str, dtype: torch.dtype, top: int) -> EdgeTables:
+    """The tables of ``edges`` under a cutoff and window, with the transport's orders
+    up to ``top``: built once and kept with the edge set's geometry."""
+    g = fused_attention.geometry(edges, cutoff, window, dtype)
+    held = g.derived.get(("differential", top))
+    if held is None:
+        with _native.LOCK:
+            held = g.derived.get(("differential", top))
+            if held is None:
+                held = g.derived["differential", top] = EdgeTables(g.row_ptr, g.source, g.transport[:, : top + 1],
+                                                                   g.bias, g.inside)
+    return held
+
+
+def attention_weights(mhsa: Any, q: Tensor, k: Tensor, edges: Any) -> Tensor:
+    """A differential layer's weights ``(n_edges, n_heads)`` from its flat query and
+    key rows: the fused op where it serves, else the single softmax's eager
+    arithmetic over the ``2 n_heads`` maps and their difference."""
+    lam, maps = mhsa.lambdas(), mhsa.field_type_map
+    window = mhsa.heads[0].window
+    if enabled(mhsa, q, edges):
+        table = torch.float32 if q.dtype == torch.bfloat16 else q.dtype
+        tables = edge_tables(edges, mhsa.cutoff, window, table, maps.max_frequency)
+        return differential_softmax(q, k, lam, tables, maps, mhsa.num_heads)
+    held = maps_of(maps, mhsa.num_heads)
+    weights = fused_attention.softmax_eager(held.plan, q, k, edges, mhsa.cutoff, window, held.scale)
+    return weights[:, 0::2] - lam.to(weights.dtype) * weights[:, 1::2]
+
+
 def _whole(rows: Tensor) -> Tensor:
     """Contiguous rows at a multiple of 16 bytes, as the lane kernels load them."""
     rows = rows.contiguous()
