@@ -331,15 +331,16 @@ int df_rows(const DfArgs<T, R>& a, const int32_t* order, const int64_t* counts, 
   }
   GM_REQUIRE(sum == n, "the classes must hold every row once");
   GM_REQUIRE(aligned(a.q, 16) && aligned(a.k, 16) && aligned(a.dq, 16) && aligned(a.dk, 16) && aligned(a.records, 8) &&
-                 aligned(a.records_s, 8) && aligned(a.pairs, 8),
-             "the lane kernels take rows at multiples of 16 bytes");
+                 aligned(a.records_s, 8) && aligned(a.pairs, 16),
+             "the lane kernels take rows and pairs at multiples of 16 bytes");
   return GM_OK;
 }
 
 template <typename T, typename R>
 int differential_forward(const R* q, const R* k, const T* lambda, const T* records, const int64_t* desc,
-                         const int64_t* row_ptr, const int32_t* order, const int64_t* counts, int64_t n_targets, int64_t n_sources, int64_t n_edges, int64_t D,
-                         int64_t orders, int64_t F, int64_t H, double scale, T* alpha, T* lse, void* stream) {
+                         const int64_t* row_ptr, const int32_t* order, const int64_t* counts, int64_t n_targets,
+                         int64_t n_sources, int64_t n_edges, int64_t D, int64_t orders, int64_t F, int64_t H,
+                         double scale, T* alpha, T* lse, void* stream) {
   DfArgs<T, R> a{};
   const int rc = df_prepare(a, q, k, lambda, records, desc, row_ptr, n_targets, n_sources, n_edges, D, orders, F, H,
                             scale);
@@ -364,7 +365,8 @@ int differential_backward(const T* g, const R* q, const R* k, const T* lambda, c
                           const int64_t* desc, const int64_t* row_ptr, const int64_t* src_ptr, const int32_t* order,
                           const int64_t* counts, const int32_t* order_s, const int64_t* counts_s, int64_t n_targets,
                           int64_t n_sources, int64_t n_edges, int64_t D, int64_t orders, int64_t F, int64_t H,
-                          double scale, const T* lse, T* pairs, T* ds, double* partial, R* dq, R* dk, T* dlambda, void* stream) {
+                          double scale, const T* lse, T* pairs, T* ds, double* partial, R* dq, R* dk, T* dlambda,
+                          void* stream) {
   DfArgs<T, R> a{};
   const int rc = df_prepare(a, q, k, lambda, records, desc, row_ptr, n_targets, n_sources, n_edges, D, orders, F, H,
                             scale);

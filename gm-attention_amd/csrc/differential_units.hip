@@ -22,7 +22,12 @@ namespace {
 
 constexpr int kDfSteps = 32;     // steps of a wave whose scores LDS holds: 32 S edges
 constexpr int kDfInFlight = 4;   // the forward's steps whose rows are requested together
-constexpr int kDfInFlightB = 2;  // the backward's
+constexpr int kDfInFlightB = 2;  // the backward's, of which a lane reads one's gradient
+constexpr int kDfThreadsB = kWavesPerBlock * kWave;
+// the backward's waves a SIMD: five of float rows (the target pass of 256x512, B = 4, in 2.78 ms for 2.93 of four);
+// with bfloat16 rows, whose halves take registers of their own, five spill (250 us for 164 at 64x128)
+template <typename R>
+constexpr int kDfWavesB = sizeof(R) == 4 ? 5 : 4;
 constexpr int kDfMinLanes = 4;   // a batch of 64 edges is whole groups of those steps
 
 struct DfUnits {
@@ -169,6 +174,13 @@ struct Unit {
         k[at + i + 1] = cs[o] * k1 + s * k0;
       }
     }
+  }
+  // < q, k >, of a row that is turned already
+  static __device__ __forceinline__ float dot(const float (&q)[N], const float (&k)[N]) {
+    float acc = 0.f;
+#pragma unroll
+    for (int i = 0; i < N; ++i) acc = fmaf(q[i], k[i], acc);
+    return acc;
   }
 };
 
@@ -393,7 +405,8 @@ __device__ __forceinline__ void row_sums(const DfUnits& w, const Share& sh, floa
 
 // Per target, in one walk: T = sum a g, A = sum a g tau k and B = sum a tau k, of which dq = scale c (A - T B).
 template <typename R, int A0, int A1, int A2, bool kNear>
-__global__ __launch_bounds__(1024) void differential_backward_target_units(DfArgs<float, R> a, DfUnits w) {
+__global__ __launch_bounds__(kDfThreadsB, kDfWavesB<R>)
+void differential_backward_target_units(DfArgs<float, R> a, DfUnits w) {
   using U = Unit<A0, A1, A2>;
   constexpr int kWords = kWave * U::RW, UN = kDfInFlightB, M = 2 * U::N + 1;
   extern __shared__ __align__(16) float df_lds[];
@@ -408,6 +421,8 @@ __global__ __launch_bounds__(1024) void differential_backward_target_units(DfArg
   float q[U::N];
   U::template load<false>(a.q, w, unit, sh.row, q);
   const float lse = a.lse[(int64_t)sh.row * a.L.P + p];
+  const bool second = p & 1;
+  const int ahead = (second ? w.slots : 0) + s;
   float sums[M];
 #pragma unroll
   for (int i = 0; i < M; ++i) sums[i] = 0.f;
@@ -424,7 +439,7 @@ __global__ __launch_bounds__(1024) void differential_backward_target_units(DfArg
     const float* weights = a.g + e * a.L.H;
     for (int t = 0; t < ends; t += UN) {
       float2 head[UN];
-      float k[UN][U::N], cs[UN][U::NO], sn[UN][U::NO], g[UN], v[UN];
+      float k[UN][U::N], cs[UN][U::NO], sn[UN][U::NO], v[UN];
 #pragma unroll
       for (int n = 0; n < UN; ++n) {
         const float* r = mine + (t + n) * w.slots * U::RW;
@@ -437,19 +452,21 @@ __global__ __launch_bounds__(1024) void differential_backward_target_units(DfArg
         }
       }
 #pragma unroll
-      for (int n = 0; n < UN; ++n) {
-        const int at = min((t + n) * w.slots + s, last);
-        g[n] = weights[(uint32_t)(at * a.L.H + (p >> 1))];
-        U::template load<kNear>(a.k, w, unit, __float_as_int(head[n].x), k[n]);
-      }
+      for (int n = 0; n < UN; ++n) U::template load<kNear>(a.k, w, unit, __float_as_int(head[n].x), k[n]);
+      // the lanes of a pair of maps read a step's gradient each
+      const float held = weights[(uint32_t)(min(t * w.slots + ahead, last) * a.L.H + (p >> 1))];
 #pragma unroll
-      for (int n = 0; n < UN; ++n) v[n] = U::dot(q, k[n], cs[n], sn[n]);
+      for (int n = 0; n < UN; ++n) {
+        U::turn(k[n], cs[n], sn[n], false);
+        v[n] = U::dot(q, k[n]);
+      }
       sum_units<UN>(v, w.per_map);
+      const float other = __shfl_xor(held, w.per_map, kWave);
+      const float g[UN] = {second ? other : held, second ? held : other};
 #pragma unroll
       for (int n = 0; n < UN; ++n) {
         if (head[n].y != neg_inf<float>()) {
           const float al = exp2_of(fmaf(scale, v[n], head[n].y - lse)), ag = al * g[n];
-          U::turn(k[n], cs[n], sn[n], false);
           sums[2 * U::N] += ag;
 #pragma unroll
           for (int i = 0; i < U::N; ++i) {
@@ -475,7 +492,8 @@ __global__ __launch_bounds__(1024) void differential_backward_target_units(DfArg
 
 // Per source, over the edges sorted by source: dk = scale c sum a (g - T) conj(tau) q.
 template <typename R, int A0, int A1, int A2, bool kNear>
-__global__ __launch_bounds__(1024) void differential_backward_source_units(DfArgs<float, R> a, DfUnits w) {
+__global__ __launch_bounds__(kDfThreadsB, kDfWavesB<R>)
+void differential_backward_source_units(DfArgs<float, R> a, DfUnits w) {
   using U = Unit<A0, A1, A2>;
   constexpr int kRecord = U::RW + 2, kWords = kWave * kRecord, UN = kDfInFlightB;
   extern __shared__ __align__(16) float df_lds[];
@@ -536,14 +554,16 @@ __global__ __launch_bounds__(1024) void differential_backward_source_units(DfArg
         }
       }
 #pragma unroll
-      for (int n = 0; n < UN; ++n) v[n] = U::dot(q[n], k, cs[n], sn[n]);
+      for (int n = 0; n < UN; ++n) {
+        U::turn(q[n], cs[n], sn[n], true);
+        v[n] = U::dot(q[n], k);
+      }
       sum_units<UN>(v, w.per_map);
 #pragma unroll
       for (int n = 0; n < UN; ++n) {
         if (bias[n] != neg_inf<float>()) {
           const float al = exp2_of(fmaf(scale, v[n], bias[n] - pair[n].x));
           const float ds = al * (g[n] - pair[n].y);
-          U::turn(q[n], cs[n], sn[n], true);
 #pragma unroll
           for (int i = 0; i < U::N; ++i) sums[i] = fmaf(ds, q[n][i], sums[i]);
         }
@@ -611,10 +631,14 @@ int launch_shape(DfPass pass, const DfArgs<float, R>& a, DfUnits w, const DfRows
                                   &differential_backward_target_units<R, A0, A1, A2, kNear>,
                                   &differential_backward_source_units<R, A0, A1, A2, kNear>};
   const Kernel kernel = kKernels[(int)pass];
-  // the rows of sixteen waves; those of four and of one, in one launch of workgroups of four
+  // the rows of sixteen waves; those of four and of one, in one launch of workgroups of four.  The backward holds no
+  // scores, and gives the rows of sixteen four too: four workgroups a CU of as many rows, whose neighbours overlap,
+  // find each other's in the L1, where one row's sixteen waves read 87 % of it from the L2 (1.21 and 1.52 ms against
+  // 1.84 and 1.90 for the rows above 512 edges of 256x512, B = 4).
+  const bool forward = pass == DfPass::Forward;
   w.first = 0;
-  for (int c = 0; c < 2; ++c) {
-    w.shared = rows.count[c];
+  for (int c = forward ? 0 : 1; c < 2; ++c) {
+    w.shared = forward ? rows.count[c] : rows.count[0] + rows.count[1];
     w.single = c == 0 ? 0 : rows.count[2];
     const int waves = c == 0 ? 16 : kWavesPerBlock;
     if (w.shared + w.single > 0) {
