@@ -1409,6 +1409,7 @@ class PointwiseLayout:
     """A field type's flat layout as the pointwise entry points take it (host arrays)."""
 
     def __init__(self, field_type: Any):
+        self._field_type = field_type
         self.D = field_type.dimension
         self.a0 = field_type.multiplicity(0) if 0 in field_type else 0
         nonzero = [(n, field_type.multiplicity(n)) for n in field_type.frequencies if n != 0]
@@ -1419,6 +1420,9 @@ class PointwiseLayout:
         self.G = sum(m for _, m in nonzero)
         self._args = (self.D, self.a0, self.nf, ctypes.cast(self.offsets, _P), ctypes.cast(self.mults, _P))
         self._slots: dict[tuple[int, ...], tuple] = {}
+
+    def __reduce__(self) -> tuple:  # a copy of a module that holds one makes its own arrays
+        return type(self), (self._field_type,)
 
     def args(self) -> tuple:
         return self._args
@@ -1651,9 +1655,8 @@ def residual_norm_backward(dy: Tensor | None, dn: Tensor | None, x: Tensor, u: T
     dx, du = torch.empty_like(x), torch.empty_like(u)
     dz = None if z is None else torch.empty_like(z)
     rows, width = int(library().gm_residual_norm_partial_rows(n)), layout.D + layout.a0
-    # one allocation: the parameters' gradients, then the kernel's rows of sums
-    sums = torch.empty(3 * copies + 2 * layout.a0 + rows * width, dtype=stats.dtype, device=device)
-    dparams, partial = sums[: 3 * copies + 2 * layout.a0], sums[3 * copies + 2 * layout.a0:]
+    dparams = torch.empty(3 * copies + 2 * layout.a0, dtype=stats.dtype, device=device)
+    partial = torch.empty(rows * width, dtype=stats.dtype, device=device)  # the kernel's rows of sums
     _call_on(device, "gm_residual_norm_backward_" + sfx, _ptr(dy), _ptr(dn), _ptr(x), _ptr(u), _ptr(z),
              _residual_parameters(layout, counts, params), _ptr(stats), n, *layout.args(), factor, _ptr(dx), _ptr(du),
              _ptr(dz), _ptr(partial), _ptr(dparams), _stream(device))

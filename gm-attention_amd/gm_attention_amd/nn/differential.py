@@ -209,8 +209,8 @@ class DifferentialSoftmax(torch.autograd.Function):
     in the rows' dtype and ``dlam`` back."""
 
     @staticmethod
-    def forward(ctx: Any, q: Tensor, k: Tensor, lam: Tensor, tables: EdgeTables, maps: Maps, scale: float) -> Tensor:
-        train = any(ctx.needs_input_grad)
+    def forward(ctx: Any, q: Tensor, k: Tensor, lam: Tensor, tables: EdgeTables, maps: Maps, scale: float,
+                train: bool) -> Tensor:
         if train:  # found here: the backward runs on a thread and perhaps a stream of its own
             tables.group_sources()
             tables.source_rows(maps.slots(tables))
@@ -227,7 +227,7 @@ class DifferentialSoftmax(torch.autograd.Function):
         q, k, lam, lse = ctx.saved_tensors
         with _native.span("gm::attention/differential_softmax_backward"):
             dq, dk, dlam = _native.differential_backward(grad_alpha.contiguous(), q, k, lam, lse, *ctx.rest)
-        return dq, dk, dlam, None, None, None
+        return dq, dk, dlam, None, None, None, None
 
 
 def differential_softmax(q: Tensor, k: Tensor, lam: Tensor, tables: EdgeTables, map_type: SO2FieldType, heads: int,
@@ -253,7 +253,9 @@ def differential_softmax(q: Tensor, k: Tensor, lam: Tensor, tables: EdgeTables, 
     scale = maps.scale if scale is None else float(scale)
     if q.device.type != "cuda":
         return _eager(q, k, lam, tables, maps.plan, scale)
-    return DifferentialSoftmax.apply(_whole(q), _whole(k), lam.to(table).contiguous(), tables, maps, scale)
+    # whether a backward can follow: inside the op a parameter looks the same under no_grad
+    train = torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or lam.requires_grad)
+    return DifferentialSoftmax.apply(_whole(q), _whole(k), lam.to(table).contiguous(), tables, maps, scale, train)
 
 
 def enabled(mhsa: Any, x: Any, edges: Any) -> bool:

@@ -41,13 +41,13 @@ class ResidualNormOp(torch.autograd.Function):
     """``(x', h)`` (``x'`` alone without a next norm) from the rows, the branch, the
     gates' pre-activations and the parameters, a vector a frequency; ``counts``
     how many of ``params`` each group has (the branch's gains and offset, the
-    scales, the next norm's gains and offset), zero for a group left out."""
+    scales, the next norm's gains and offset), zero for a group left out;
+    ``train`` whether a backward can follow."""
 
     @staticmethod
     def forward(ctx, x: Tensor, u: Tensor, z: Tensor | None, layout, factor: float, eps: float, next_eps: float,
-                counts: tuple[int, ...], *params: Tensor):
+                counts: tuple[int, ...], train: bool, *params: Tensor):
         ctx.set_materialize_grads(False)
-        train = any(ctx.needs_input_grad)
         with _native.span("gm::pointwise/residual_norm"):
             y, normed, stats = _native.residual_norm_forward(x, u, z, counts, params, layout, factor, eps, next_eps,
                                                              train)
@@ -73,7 +73,7 @@ class ResidualNormOp(torch.autograd.Function):
         for group, count in enumerate(counts):
             sizes += [next(lengths) for _ in range(count)] if count else [layout.a0 if group in (1, 4) else copies]
             held += [True] * count or [False]
-        return (dx, du, dz, None, None, None, None, None,
+        return (dx, du, dz, None, None, None, None, None, None,
                 *(g for g, h in zip(dparams.split(sizes), held, strict=True) if h))
 
 
@@ -167,11 +167,13 @@ class SO2ResidualNorm(nn.Module):
             branch = branch.to(rows.dtype)
         pd, (counts, params) = _native.param_dtype(rows.dtype), self._params()
         params = [p if p.dtype == pd and p.is_contiguous() else p.to(pd).contiguous() for p in params]
+        # inside the op a parameter looks the same under no_grad
+        train = torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (rows, branch, pre, *params))
         out = ResidualNormOp.apply(rows.contiguous(), branch.contiguous(),
                                    None if pre is None else pre.to(rows.dtype).contiguous(), self._layout(),
                                    _GATES.get(self.gate, 1.0), self.post.eps if self.post is not None else 1.0,
                                    self.norm.eps if self.norm is not None else 1.0,
-                                   counts, *params)
+                                   counts, train, *params)
         return out if self.norm is not None else (out, None)
 
     def forward(self, x: SO2FeatureField, branch: SO2FeatureField,

@@ -12,6 +12,7 @@ absolute values of what it multiplies, and by a half step an edge for the sum
 itself.  A result held in bfloat16 is off by another eps / 2 = 2^-8 of its value.
 """
 
+import concurrent.futures
 import itertools
 import math
 
@@ -431,6 +432,60 @@ def test_tables_are_built_before_a_capture(cuda):
     captured.replay()
     torch.cuda.synchronize()
     assert torch.equal(held, q)
+
+
+@pytest.mark.gpu
+def test_inference_needs_no_source_side(cuda):
+    """Under no_grad a layer's parameters still require gradients: the op neither sorts
+    the edges by source nor needs that done before a capture."""
+    copies, heads = {0: 2, 1: 2, 2: 2}, 8
+    graph = sphere(8, 16)
+    q, k, lam, g = (v.float().to(cuda) for v in inputs(graph, copies, heads, torch.float32))
+    tables, maps = graph.tables(torch.float32, cuda), SO2FieldType(copies)
+    lam = torch.nn.Parameter(lam)
+    with torch.no_grad():
+        want = differential_softmax(q, k, lam, tables, maps, heads)
+        torch.cuda.synchronize()
+        captured = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(captured):
+            got = differential_softmax(q, k, lam, tables, maps, heads)
+        for _ in range(3):
+            got.zero_()
+            captured.replay()
+            torch.cuda.synchronize()
+            assert torch.equal(got, want)
+            assert torch.equal(differential_softmax(q, k, lam, tables, maps, heads), want)
+    assert tables._sources is None
+    alpha = differential_softmax(q, k, lam, tables, maps, heads)
+    assert torch.equal(alpha, want) and tables._sources is not None
+
+
+@pytest.mark.gpu
+def test_two_threads_at_once(cuda):
+    """Two threads' first steps over the same new tables, each on its own stream."""
+    copies, heads = {0: 2, 1: 2, 2: 2}, 8
+    graph = sphere(12, 24, batch=2)
+    q, k, lam, g = (v.float().to(cuda) for v in inputs(graph, copies, heads, torch.float32))
+
+    def step(tables):
+        leaves = [v.detach().requires_grad_(True) for v in (q, k, lam)]
+        alpha = differential_softmax(*leaves, tables, SO2FieldType(copies), heads)
+        return [alpha.detach(), *torch.autograd.grad(alpha, leaves, g)]
+
+    want = step(graph.tables(torch.float32, cuda))
+    tables = graph.tables(torch.float32, cuda)
+    torch.cuda.synchronize()
+
+    def work(_):
+        stream = torch.cuda.Stream()
+        with torch.cuda.stream(stream):
+            out = [step(tables) for _ in range(5)]
+        stream.synchronize()
+        return out
+
+    with concurrent.futures.ThreadPoolExecutor(2) as pool:
+        runs = list(pool.map(work, range(2)))
+    assert all(torch.equal(a, b) for run in runs for got in run for a, b in zip(got, want))
 
 
 @pytest.mark.gpu

@@ -11,12 +11,17 @@ twenty products, quotients and exponentials.  A result held in bfloat16 is off b
 another eps / 2 = 2^-8 of its value.
 """
 
+import copy
 import itertools
+import pickle
 
 import pytest
 import torch
 
 import problems
+from gm_attention_amd.nn import residual
+from gm_attention_amd.nn.nonlinearities import SO2ScalarGatedNonlinearity
+from gm_attention_amd.nn.normalization import SO2LayerNorm
 from gm_attention_amd.nn.residual import SO2ResidualNorm
 from gm_attention_amd.representations.field_type import SO2FieldType
 
@@ -339,6 +344,30 @@ def test_on_another_stream(cuda):
 
 
 @pytest.mark.gpu
+def test_nothing_is_kept_for_a_backward_that_cannot_follow(cuda, monkeypatch):
+    m = SO2ResidualNorm(SO2FieldType({0: 16, 1: 16}), scale=1.0, device=cuda)
+    x, u = (problems.normal((50, 48), i).float().to(cuda) for i in range(2))
+    given, real = [], residual._native.residual_norm_forward
+    monkeypatch.setattr(residual._native, "residual_norm_forward", lambda *a: given.append(a[-1]) or real(*a))
+    with torch.no_grad():
+        without = m.forward_flat(x, u)
+    with_graph = m.forward_flat(x, u)
+    m.requires_grad_(False)
+    m.forward_flat(x, u)
+    assert given == [False, True, False]
+    assert all(torch.equal(a, b) for a, b in zip(without, with_graph))
+
+
+@pytest.mark.gpu
+def test_gradients_hold_no_workspace(cuda):
+    m = SO2ResidualNorm(SO2FieldType({0: 16, 1: 16}), scale=1.0, device=cuda)
+    x, u = (problems.normal((5000, 48), i).float().to(cuda) for i in range(2))
+    y, h = m.forward_flat(x, u)
+    (y.sum() + h.sum()).backward()
+    assert all(p.grad.untyped_storage().nbytes() <= 4 * (3 * 32 + 2 * 16) for p in m.parameters())
+
+
+@pytest.mark.gpu
 def test_infinite_and_nan_rows_stay_in_their_rows(cuda):
     m = SO2ResidualNorm(SO2FieldType({0: 16, 1: 16, 2: 16}), scale=1.0, device=cuda)
     x, u = (problems.normal((200, 80), i).float().to(cuda) for i in range(2))
@@ -419,3 +448,25 @@ def test_the_library_refuses_bad_arguments():
     assert forward(n=0) == 0
     params[1] = 64  # the gains of one frequency alone (an address nothing reads)
     assert forward(n=0) == 1 and b"every frequency" in lib.gm_last_error()
+
+
+@pytest.mark.parametrize("make", [SO2LayerNorm, SO2ScalarGatedNonlinearity, SO2ResidualNorm])
+def test_modules_are_copied_with_their_layouts(make):
+    """Modules keep their layout for the entry points; copies have their own."""
+    m = make(SO2FieldType({0: 4, 1: 3, 2: 2}))
+    args = m._layout().args()
+    for other in (copy.deepcopy(m), pickle.loads(pickle.dumps(m))):
+        layout = other._layout()
+        assert layout is not m._layout() and layout.args()[:3] == args[:3]
+        assert list(layout.offsets) == [4, 10] and list(layout.mults) == [3, 2]
+        assert layout.args()[3].value != args[3].value
+
+
+def test_a_used_module_is_copied():
+    m = SO2ResidualNorm(SO2FieldType({0: 4, 1: 3}), scale=0.5)
+    counts, params = m._params()
+    m._layout().parameter_slots(counts)
+    other = copy.deepcopy(m)
+    x, u = (problems.normal((7, 10), i).float() for i in range(2))
+    assert all(torch.equal(a, b) for a, b in zip(m.forward_flat(x, u), other.forward_flat(x, u)))
+    assert other._layout().parameter_slots(counts)[1:] == m._layout().parameter_slots(counts)[1:]
