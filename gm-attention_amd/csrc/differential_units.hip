@@ -4,10 +4,19 @@
 // so that the lanes of an edge read its row as whole cache lines.  A wave's 64 lanes
 // are (edge slot, unit), units rounded up to a power of two.
 //
-// What bounds them is the L1's line accesses: an edge's row is D words whatever is
-// done with it.  (The single softmax's lanes hold a head's 16-byte pieces, which at
-// frequencies above 0 lie 32 bytes apart, so each load touches twice the lines it
-// uses: nine line accesses an edge at 160 numbers a row against the five here.)
+// What bounds them is the path from the L1 to the registers: an edge's row is D words
+// whatever is done with it.  On 256x512, B = 4 (79 million edges of 640 bytes) the
+// forward's 3.1 ms are 31 bytes a cycle of a CU, its load unit busy for 97 % of them
+// and its vector ALUs for half; with every source among 16 rows, all in the L1, they
+// are 7 % fewer, so it is not the L2.  (Contiguous loads of 16 bytes a lane from the L1
+// reach 50 bytes a cycle.)  Fewer, wider loads did not help: a lane for both of a
+// head's maps, five loads of 16 bytes for two units in place of six, took 3.1, 4.0 and
+// 3.9 ms in the three passes against 3.1, 2.75 and 3.3, for the registers it needs; the
+// two maps' lanes reading the pieces of up to 8 bytes together, each for one of two
+// steps, 3.06, 3.0 and 3.2, and 9 % more with bfloat16 rows.  (The single softmax's lanes hold a
+// head's 16-byte pieces, which at frequencies above 0 lie 32 bytes apart, so each load
+// touches twice the lines it uses: nine line accesses an edge at 160 numbers a row
+// against the five here.)
 //
 // Each edge's record is copied once per 64 edges into the wave's LDS (the next 64
 // requested before the present ones are used) and read from there by the lanes of

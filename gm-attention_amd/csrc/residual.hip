@@ -214,8 +214,8 @@ struct RnUnit {
     if constexpr (kCopies) {
       g[0] = g[1] = widen(row[unit]);
     } else {
-      // selects, not a branch's stores: those went through scratch for bfloat16 (510 us against 345 then for the backward of
-      // 262,144 rows of 160 with a float branch, 189 against 108 for the forward)
+      // selects, not a branch's stores: those went through scratch for bfloat16 (510 us against 345 then for the
+      // backward of 262,144 rows of 160 with a float branch, 189 against 108 for the forward)
       const bool scalar = unit < a.scalar_units;
       A lo[V / 2], hi[V / 2];
       const X* p = row + (scalar ? unit * V : (unit * V + a.a0) / 2);
