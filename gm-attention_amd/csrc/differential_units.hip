@@ -4,25 +4,25 @@
 // so that the lanes of an edge read its row as whole cache lines.  A wave's 64 lanes
 // are (edge slot, unit), units rounded up to a power of two.
 //
-// What bounds them is the path from the L1 to the registers: an edge's row is D words
-// whatever is done with it.  On 256x512, B = 4 (79 million edges of 640 bytes) the
-// forward's 3.1 ms are 31 bytes a cycle of a CU, its load unit busy for 97 % of them
-// and its vector ALUs for half; with every source among 16 rows, all in the L1, they
-// are 7 % fewer, so it is not the L2.  (Contiguous loads of 16 bytes a lane from the L1
-// reach 50 bytes a cycle.)  Fewer, wider loads did not help: a lane for both of a
-// head's maps, five loads of 16 bytes for two units in place of six, took 3.1, 4.0 and
-// 3.9 ms in the three passes against 3.1, 2.75 and 3.3, for the registers it needs; the
-// two maps' lanes reading the pieces of up to 8 bytes together, each for one of two
-// steps, 3.06, 3.0 and 3.2, and 9 % more with bfloat16 rows.  (The single softmax's lanes hold a
-// head's 16-byte pieces, which at frequencies above 0 lie 32 bytes apart, so each load
-// touches twice the lines it uses: nine line accesses an edge at 160 numbers a row
-// against the five here.)
+// Measured on 256x512, B = 4 (79 million edges of 640 bytes): the forward 3.05 ms, the
+// passes of the backward 2.75 (targets) and 3.3 (sources); 31 bytes a cycle of a CU
+// arrive from the L1, where contiguous loads reach 50.  No one unit bounds them.  The
+// forward's load path is busy for 97 % of the time and its vector ALUs for 51 %, yet
+// timing copies of it without the dot products take 1 % less, without the rows' loads 27 %
+// less, without the records' reads from LDS nothing less, and with every source among
+// 16 rows, all in the L1, 7 % less: what remains is the waves' latency, four of them a
+// SIMD by their registers and the LDS of their scores (the backward, without scores,
+// has five).  Fewer, wider loads did not help: a lane for both of a head's maps, five
+// loads of 16 bytes for two units in place of six, took 3.1, 4.0 and 3.9 ms for the
+// registers it needs; the two maps' lanes reading the pieces of up to 8 bytes together,
+// each for one of two steps, 3.06, 3.0 and 3.2, and 9 % more with bfloat16 rows.
 //
 // Each edge's record is copied once per 64 edges into the wave's LDS (the next 64
 // requested before the present ones are used) and read from there by the lanes of
 // its edge.  A row of more edges than a wave's LDS holds scores of goes to four or
 // sixteen waves, which combine their maxima and sums (their gradients) through LDS.
 #include <algorithm>
+#include <type_traits>
 
 #include "differential.hpp"
 
@@ -57,6 +57,14 @@ __device__ __forceinline__ int64_t uniform(int64_t v) {
 }
 // A weight: one v_exp_f32 (a step off; zero below the smallest normal number).
 __device__ __forceinline__ float exp2_of(float x) { return __builtin_amdgcn_exp2f(x); }
+
+// The value of the lane of the head's other map, `per_map` lanes away: a DPP operand where that is the next lane (the
+// backward of bfloat16 rows at 64x128 145 + 147 us against 158 + 149 with an LDS permute).
+__device__ __forceinline__ float other_map(float v, int per_map) {
+  if (per_map == 1)  // the quads' lanes 1, 0, 3, 2
+    return __int_as_float(__builtin_amdgcn_mov_dpp(__float_as_int(v), 0xB1, 0xF, 0xF, true));
+  return __shfl_xor(v, per_map, kWave);
+}
 
 // W numbers of a row at p.
 template <int W>
@@ -264,7 +272,7 @@ __device__ __forceinline__ Share share_of(const DfUnits& w, const int64_t* ptr) 
 template <typename R, int A0, int A1, int A2, bool kNear>
 __global__ __launch_bounds__(1024) void differential_forward_units(DfArgs<float, R> a, DfUnits w) {
   using U = Unit<A0, A1, A2>;
-  constexpr int kWords = kWave * U::RW, UN = kDfInFlight;
+  constexpr int kWords = kWave * U::RW;
   extern __shared__ __align__(16) float df_lds[];
   const Share sh = share_of(w, a.row_ptr);
   if (!sh.live) return;  // one wave a row, or the whole workgroup
@@ -305,7 +313,7 @@ __global__ __launch_bounds__(1024) void differential_forward_units(DfArgs<float,
   const int ahead = writes ? (second ? w.slots : 0) + s : INT32_MAX;
   const uint32_t place = (uint32_t)(ahead * a.L.H + (p >> 1));
   auto write = [&](int64_t e, int t, float w0, float w1) {
-    const float other = __shfl_xor(second ? w0 : w1, w.per_map, kWave);
+    const float other = other_map(second ? w0 : w1, w.per_map);
     const float v = second ? other - lambda * w1 : w0 - lambda * other;
     float* to = a.alpha + (e + t * w.slots) * a.L.H;
     if (ahead < (int)(sh.e1 - e) - t * w.slots) to[place] = v;
@@ -317,10 +325,11 @@ __global__ __launch_bounds__(1024) void differential_forward_units(DfArgs<float,
     if (phase == 1) {
       m = over_waves(m, true);
       m = m == neg_inf<float>() ? 0.f : m;  // no edge inside: exp(-inf) = 0 everywhere
-      for (int t = 0; t < held; ++t) {
-        const float x = exp2_of(sc[t * kWave] - m);
-        sc[t * kWave] = x;
-        l += x;
+      for (int t = 0; t < held; t += 2) {  // a step past `held` is outside: its weight is zero
+        const float x0 = exp2_of(sc[t * kWave] - m), x1 = exp2_of(sc[(t + 1) * kWave] - m);
+        sc[t * kWave] = x0;
+        sc[(t + 1) * kWave] = x1;
+        l += x0 + x1;
       }
     }
     if (phase == 2) {
@@ -328,8 +337,7 @@ __global__ __launch_bounds__(1024) void differential_forward_units(DfArgs<float,
       inv = l == 0.f ? 0.f : 1.f / l;
       if (a.lse && sh.part == 0 && s == 0 && writes)
         a.lse[(int64_t)sh.row * a.L.P + p] = l == 0.f ? neg_inf<float>() : m + log2f(l);
-      for (int t = 0; t < held; t += 2)
-        write(sh.e0, t, sc[t * kWave] * inv, t + 1 < held ? sc[(t + 1) * kWave] * inv : 0.f);
+      for (int t = 0; t < held; t += 2) write(sh.e0, t, sc[t * kWave] * inv, sc[(t + 1) * kWave] * inv);
     }
     const int skip = phase == 0 ? 0 : kDfSteps;
     if (skip >= sh.steps) continue;
@@ -343,7 +351,10 @@ __global__ __launch_bounds__(1024) void differential_forward_units(DfArgs<float,
       wave_lds();
       if (b + w.lanes < sh.steps) records.request(a.records, e + kWave, sh.e1, lane);
       const int ends = sh.steps - b < w.lanes ? sh.steps - b : w.lanes;
-      for (int t = skip > b ? skip - b : 0; t < ends; t += UN) {
+      // `group` steps from t together: four in the rows of up to four waves (1.58 ms against 1.67 with two at 256x512,
+      // B = 4), two in those of sixteen (1.47 against 1.53) and for the last
+      auto take = [&](int t, auto group) {
+        constexpr int UN = decltype(group)::value;
         float2 head[UN];
         float k[UN][U::N], cs[UN][U::NO], sn[UN][U::NO], v[UN];
 #pragma unroll
@@ -383,7 +394,11 @@ __global__ __launch_bounds__(1024) void differential_forward_units(DfArgs<float,
             for (int n = 0; n < UN; n += 2) write(e, t + n, v[n] * inv, v[n + 1] * inv);
           }
         }
-      }
+      };
+      int t = skip > b ? skip - b : 0;
+      for (; ends - t > 2 && sh.parts <= kWavesPerBlock; t += kDfInFlight)
+        take(t, std::integral_constant<int, kDfInFlight>());
+      for (; t < ends; t += 2) take(t, std::integral_constant<int, 2>());
     }
   }
 }
@@ -470,7 +485,7 @@ void differential_backward_target_units(DfArgs<float, R> a, DfUnits w) {
         v[n] = U::dot(q, k[n]);
       }
       sum_units<UN>(v, w.per_map);
-      const float other = __shfl_xor(held, w.per_map, kWave);
+      const float other = other_map(held, w.per_map);
       const float g[UN] = {second ? other : held, second ? held : other};
 #pragma unroll
       for (int n = 0; n < UN; ++n) {
