@@ -5,7 +5,7 @@
 // are (edge slot, unit), units rounded up to a power of two.
 //
 // Measured on 256x512, B = 4 (79 million edges of 640 bytes): the forward 3.05 ms, the
-// passes of the backward 2.75 (targets) and 3.3 (sources); 31 bytes a cycle of a CU
+// passes of the backward 2.8 (targets) and 3.3 (sources); 31 bytes a cycle of a CU
 // arrive from the L1, where contiguous loads reach 50.  No one unit bounds them.  The
 // forward's load path is busy for 97 % of the time and its vector ALUs for 51 %, yet
 // timing copies of it without the dot products take 1 % less, without the rows' loads 27 %
@@ -58,8 +58,8 @@ __device__ __forceinline__ int64_t uniform(int64_t v) {
 // A weight: one v_exp_f32 (a step off; zero below the smallest normal number).
 __device__ __forceinline__ float exp2_of(float x) { return __builtin_amdgcn_exp2f(x); }
 
-// The value of the lane of the head's other map, `per_map` lanes away: a DPP operand where that is the next lane (the
-// backward of bfloat16 rows at 64x128 145 + 147 us against 158 + 149 with an LDS permute).
+// The value of the lane of the head's other map, `per_map` lanes away: a DPP operand where that is the next lane, an
+// LDS permute otherwise.
 __device__ __forceinline__ float other_map(float v, int per_map) {
   if (per_map == 1)  // the quads' lanes 1, 0, 3, 2
     return __int_as_float(__builtin_amdgcn_mov_dpp(__float_as_int(v), 0xB1, 0xF, 0xF, true));
@@ -159,6 +159,9 @@ struct Unit {
     store_w<W1>(row + w.base[1] + unit * W1, v + W0);
     if constexpr (W2 > 0) store_w<W2>(row + w.base[2] + unit * W2, v + W0 + W1);
   }
+  // The three passes form a score by the same roundings, so that a row's ds sum to zero as nearly as its weights to one:
+  // a key bias's gradient, zero but for rounding, is a third smaller than with the gathered row turned before the dot in
+  // the backward's passes (which saves a fifth of their instructions and 1 % of their time).
   // Re< q, tau k >: per order cos sum (q0 k0 + q1 k1) + sin sum (q1 k0 - q0 k1)
   static __device__ __forceinline__ float dot(const float (&q)[N], const float (&k)[N], const float (&cs)[NO],
                                               const float (&sn)[NO]) {
@@ -191,13 +194,6 @@ struct Unit {
         k[at + i + 1] = cs[o] * k1 + s * k0;
       }
     }
-  }
-  // < q, k >, of a row that is turned already
-  static __device__ __forceinline__ float dot(const float (&q)[N], const float (&k)[N]) {
-    float acc = 0.f;
-#pragma unroll
-    for (int i = 0; i < N; ++i) acc = fmaf(q[i], k[i], acc);
-    return acc;
   }
 };
 
@@ -480,10 +476,7 @@ void differential_backward_target_units(DfArgs<float, R> a, DfUnits w) {
       // the lanes of a pair of maps read a step's gradient each
       const float held = weights[(uint32_t)(min(t * w.slots + ahead, last) * a.L.H + (p >> 1))];
 #pragma unroll
-      for (int n = 0; n < UN; ++n) {
-        U::turn(k[n], cs[n], sn[n], false);
-        v[n] = U::dot(q, k[n]);
-      }
+      for (int n = 0; n < UN; ++n) v[n] = U::dot(q, k[n], cs[n], sn[n]);
       sum_units<UN>(v, w.per_map);
       const float other = other_map(held, w.per_map);
       const float g[UN] = {second ? other : held, second ? held : other};
@@ -491,6 +484,7 @@ void differential_backward_target_units(DfArgs<float, R> a, DfUnits w) {
       for (int n = 0; n < UN; ++n) {
         if (head[n].y != neg_inf<float>()) {
           const float al = exp2_of(fmaf(scale, v[n], head[n].y - lse)), ag = al * g[n];
+          U::turn(k[n], cs[n], sn[n], false);
           sums[2 * U::N] += ag;
 #pragma unroll
           for (int i = 0; i < U::N; ++i) {
@@ -578,16 +572,14 @@ void differential_backward_source_units(DfArgs<float, R> a, DfUnits w) {
         }
       }
 #pragma unroll
-      for (int n = 0; n < UN; ++n) {
-        U::turn(q[n], cs[n], sn[n], true);
-        v[n] = U::dot(q[n], k);
-      }
+      for (int n = 0; n < UN; ++n) v[n] = U::dot(q[n], k, cs[n], sn[n]);
       sum_units<UN>(v, w.per_map);
 #pragma unroll
       for (int n = 0; n < UN; ++n) {
         if (bias[n] != neg_inf<float>()) {
           const float al = exp2_of(fmaf(scale, v[n], bias[n] - pair[n].x));
           const float ds = al * (g[n] - pair[n].y);
+          U::turn(q[n], cs[n], sn[n], true);
 #pragma unroll
           for (int i = 0; i < U::N; ++i) sums[i] = fmaf(ds, q[n][i], sums[i]);
         }

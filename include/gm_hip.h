@@ -288,8 +288,8 @@ int gm_edge_tables_f64(const double* targets, const double* target_frames, const
  * order, or NULL: every target once, those of more than 128 S edges first, then
  * those of more than 32 S, then the rest, counts (HOST) how many of each, for the
  * S of gm_differential_slots; order_s and counts_s the same of the sources.  With
- * them (float and bfloat16 rows, at multiples of 16 bytes) the lane kernels run
- * and ds is not used; without, kernels for any layout.
+ * them (float and bfloat16 rows; rows and pairs at multiples of 16 bytes, records
+ * of 8) the lane kernels run and ds is not used; without, kernels for any layout.
  * Suffix _bf16: bfloat16 rows, float tables and arithmetic.  No reference
  * counterpart (the single map's: gm_softmax_*). */
 int64_t gm_differential_partials(int64_t heads);
