@@ -33,8 +33,8 @@ constexpr int kDfSteps = 32;     // steps of a wave whose scores LDS holds: 32 S
 constexpr int kDfInFlight = 4;   // the forward's steps whose rows are requested together
 constexpr int kDfInFlightB = 2;  // the backward's, of which a lane reads one's gradient
 constexpr int kDfThreadsB = kWavesPerBlock * kWave;
-// the backward's waves a SIMD: five of float rows (the target pass of 256x512, B = 4, in 2.78 ms for 2.93 of four);
-// with bfloat16 rows, whose halves take registers of their own, five spill (250 us for 164 at 64x128)
+// the backward's waves a SIMD: five of float rows (the target pass of 256x512, B = 4, in 2.78 ms for 2.93 of four); with
+// bfloat16 rows, whose halves take registers of their own, four (171 us against 210 of five at 64x128)
 template <typename R>
 constexpr int kDfWavesB = sizeof(R) == 4 ? 5 : 4;
 constexpr int kDfMinLanes = 4;   // a batch of 64 edges is whole groups of those steps
