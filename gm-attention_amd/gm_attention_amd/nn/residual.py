@@ -77,9 +77,12 @@ class ResidualNormOp(torch.autograd.Function):
                 *(g for g, h in zip(dparams.split(sizes), held, strict=True) if h))
 
 
-def _by_frequency(held: nn.ParameterDict | None) -> list[Tensor]:
-    """A dictionary's vectors in the order of the field's frequencies, in which they were entered."""
-    return [] if held is None else list(held._parameters.values())
+def _by_key(held: nn.ParameterDict, keys: list[str]) -> list[Tensor]:
+    """A dictionary's vectors under ``keys`` (its own order is its keys' as texts, 10 before 2)."""
+    own = held._parameters
+    if all(k in own for k in keys):
+        return [own[k] for k in keys]
+    return [held[k] for k in keys]  # a replica's are plain attributes, a pruned or parametrised one's is computed
 
 
 class SO2ResidualNorm(nn.Module):
@@ -135,11 +138,14 @@ class SO2ResidualNorm(nn.Module):
         return layout
 
     def _params(self) -> tuple[tuple[int, ...], list[Tensor]]:
-        """``(counts, params)`` as the op takes them: every group's vectors by frequency."""
-        groups = [_by_frequency(None if self.post is None else self.post.gamma),
-                  [self.post.beta] if self.post is not None and self.post.has_bias else [],
-                  _by_frequency(self.scale), _by_frequency(None if self.norm is None else self.norm.gamma),
-                  [self.norm.beta] if self.norm is not None and self.norm.has_bias else []]
+        """``(counts, params)`` as the op takes them: every group's vectors by frequency, a
+        group left out where the module was made without it."""
+        post, norm, keys = self.post, self.norm, [str(f) for f in self.field_type.frequencies]
+        groups = [[] if post is None else _by_key(post.gamma, keys),
+                  [post.beta] if post is not None and post.has_bias else [],
+                  [] if self.scale is None else _by_key(self.scale, keys),
+                  [] if norm is None else _by_key(norm.gamma, keys),
+                  [norm.beta] if norm is not None and norm.has_bias else []]
         return tuple(map(len, groups)), [p for group in groups for p in group]
 
     def uses_hip(self, flat: Tensor) -> bool:

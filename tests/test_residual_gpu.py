@@ -470,3 +470,91 @@ def test_a_used_module_is_copied():
     x, u = (problems.normal((7, 10), i).float() for i in range(2))
     assert all(torch.equal(a, b) for a, b in zip(m.forward_flat(x, u), other.forward_flat(x, u)))
     assert other._layout().parameter_slots(counts)[1:] == m._layout().parameter_slots(counts)[1:]
+
+
+# ------------------------------------------------------- where the parameters are read
+
+
+def replica_of(module):
+    """A module's replica as a data-parallel step makes one: its parameters are plain attributes."""
+    replica = module._replicate_for_data_parallel()
+    for key, child in module._modules.items():
+        setattr(replica, key, None if child is None else replica_of(child))
+    for key, p in module._parameters.items():
+        if p is None:
+            replica._parameters[key] = None
+        else:
+            setattr(replica, key, p * 1.0)
+    return replica
+
+
+def by_name(module):
+    """The vectors of every group in the order of the field's frequencies."""
+    keys = [str(f) for f in module.field_type.frequencies]
+    named = dict(module.named_parameters())
+    return [named[n] for group in (["post.gamma." + k for k in keys], ["post.beta"], ["scale." + k for k in keys],
+                                   ["norm.gamma." + k for k in keys], ["norm.beta"]) for n in group if n in named]
+
+
+FORMS = [dict(scale=0.5), dict(scale=0.5, norm=False), dict(post_norm=False, scale=1.0), dict(norm=False),
+         dict(scale=0.5, bias=False)]
+
+
+@pytest.mark.parametrize("form", FORMS)
+@pytest.mark.parametrize("copies", [{0: 4, 1: 3, 2: 2}, {1: 3, 2: 3}, {0: 3, 2: 3, 10: 3}, {2: 2, 9: 4, 11: 5}])
+def test_parameters_are_read_by_frequency_in_modules_and_replicas(copies, form):
+    module = SO2ResidualNorm(SO2FieldType(copies), **form)
+    with torch.no_grad():
+        for i, p in enumerate(module.parameters()):
+            p.add_(torch.arange(p.numel()) + 10.0 * i)
+    want = by_name(module)
+    counts, params = module._params()
+    assert len(params) == len(want) and all(a is b for a, b in zip(params, want))
+    replicated, copied = replica_of(module)._params()
+    assert replicated == counts
+    assert len(copied) == len(want) and all(torch.equal(a, b) for a, b in zip(copied, want))
+
+
+def test_pruned_and_parametrised_vectors_are_read_as_they_act():
+    from torch.nn.utils import parametrize, prune
+
+    class Doubled(torch.nn.Module):
+        def forward(self, p):
+            return 2 * p
+
+    module = SO2ResidualNorm(SO2FieldType({0: 4, 1: 4}), scale=0.5)
+    prune.custom_from_mask(module.post.gamma, "1", torch.tensor([1.0, 0.0, 1.0, 0.0]))
+    parametrize.register_parametrization(module.norm.gamma, "0", Doubled())
+    counts, params = module._params()
+    assert counts == (2, 1, 2, 2, 1)
+    assert params[1].tolist() == [1.0, 0.0, 1.0, 0.0]  # the branch's gains of frequency 1
+    assert params[5].tolist() == [2.0] * 4  # the next norm's of frequency 0
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("copies", [{0: 4, 2: 3, 10: 3}, {0: 5, 2: 2, 10: 4}, {2: 4, 11: 8}])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_frequencies_of_two_digits(copies, dtype, cuda):
+    check(copies, 40, True, "sigmoid", True, True, dtype, dtype, cuda)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("form", FORMS)
+def test_a_replica_gives_the_modules_results(form, cuda):
+    from torch.nn.parallel import replicate
+
+    module = SO2ResidualNorm(SO2FieldType({0: 8, 1: 8, 2: 4}), gate="sigmoid", device=cuda, **form)
+    with torch.no_grad():
+        for i, p in enumerate(module.parameters()):
+            p.add_(0.1 * problems.normal(p.shape, i).float().to(cuda))
+    x, u, z = (problems.normal((50, w), 30 + w).float().to(cuda) for w in (32, 32, 20))
+    u = u.flip(0)
+    (replica,) = replicate(module, [cuda])
+    params = list(module.parameters())
+
+    def step(m):
+        outs = [o for o in m.forward_flat(x, u, z) if o is not None]
+        return outs + list(torch.autograd.grad(sum((o * x).sum() for o in outs), params, allow_unused=True))
+
+    for a, b in zip(step(replica), step(module), strict=True):
+        assert (a is None and b is None) or torch.equal(a, b)
