@@ -187,7 +187,8 @@ class Maps:
         self.heads, self.scale = heads, 1.0 / math.sqrt(map_type.dimension)
         self.plan = fused_attention.plan_of(map_type, full, 2 * heads)
         self.top = max(n for n, *_ in self.plan.rows)
-        self.desc = torch.tensor([list(row) for row in self.plan.rows], dtype=torch.int64)
+        # read on the host, whatever the default device of the call that makes the (kept) maps
+        self.desc = torch.tensor([list(row) for row in self.plan.rows], dtype=torch.int64, device="cpu")
         self._slots: dict[int, int] = {}
 
     def slots(self, tables: EdgeTables) -> int:

@@ -633,3 +633,13 @@ def test_the_library_refuses_bad_arguments():
                         (dict(rows=((0, 2, 4, 0, 1), (1, 1, 8, 0, 2))), b"follow each other")):
         assert forward(**kw) == 1
         assert message in lib.gm_last_error(), kw
+
+
+def test_maps_made_under_a_default_device_serve_every_call():
+    """The layout the library reads on the host is in host memory, whatever device was the default."""
+    map_type, graph = SO2FieldType({0: 4, 1: 4, 2: 4}), scattered([3, 1, 4], 5, torch.float32)
+    tables = graph.tables(torch.float32, "cpu")
+    with torch.device("meta"):
+        held = differential.maps_of(map_type, 3)
+    assert differential.maps_of(map_type, 3) is held
+    assert held.desc.device.type == "cpu" and held.slots(tables) == 4
