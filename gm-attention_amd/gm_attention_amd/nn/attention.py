@@ -160,6 +160,8 @@ class SO2Attention(nn.Module):
 
 
 class SO2MHSA(nn.Module):
+    differential = False  # a layer pickled before there was the option reads as one without it
+
     def __init__(self, field_type_in: SO2FieldType, num_heads: int, *, cutoff: float, window: str = "hard",
                  n_radial_basis: int = 8, radial_hidden_features: Sequence[int] = (16,), radial_basis: str = "gaussian",
                  bias: bool = True, batched: bool = False, value_kind: str = "steerable", differential: bool = False,

@@ -82,6 +82,8 @@ def _add_fields(a: SO2FeatureField, b: SO2FeatureField) -> SO2FeatureField:
 
 
 class SO2TransformerBlock(nn.Module):
+    norm_placement: NormPlacement = "pre"  # a block pickled before there was the option reads as it was
+
     def __init__(self, field_type: SO2FieldType, num_heads: int, *, ffn_multiplier: int = 2,
                  hidden_field_type: SO2FieldType | None = None, cutoff: float, window: str = "hard",
                  n_radial_basis: int = 8, radial_hidden_features=(16,), radial_basis: str = "gaussian",

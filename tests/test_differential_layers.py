@@ -314,3 +314,25 @@ def test_refusals():
         SO2TransformerBlock(ft, 2, cutoff=1.0, norm_placement="sandwich", residual_gate="silu")
     with pytest.raises(ValueError, match="needs mixer='attention'"):
         SO2TransformerBlock(ft, 2, cutoff=1.0, mixer="convolution", attention_differential=True)
+
+
+def test_modules_pickled_before_there_were_the_options_run_as_they_did():
+    import pickle
+
+    edges, cutoff = edges_of()
+    torch.manual_seed(0)
+    for make, option in ((lambda: SO2MHSA(SO2FieldType({0: 4, 1: 4}), 2, cutoff=cutoff, batched=True, dtype=D64),
+                          "differential"),
+                         (lambda: SO2TransformerBlock(SO2FieldType({0: 4, 1: 4}), 2, cutoff=cutoff,
+                                                      attention_batched=True, dtype=D64), "norm_placement")):
+        module = make()
+        older = pickle.loads(pickle.dumps(module))
+        for m in older.modules():
+            m.__dict__.pop(option, None)
+            m.__dict__.pop("differential", None)
+        x = problems.normal((edges.row_ptr.shape[0] - 1, 12), 1)
+        probe = problems.normal(x.shape, 2)
+        for chunk in (None, 50):
+            want, got = run(module, x, edges, probe, chunk), run(older, x, edges, probe, chunk)
+            assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
+        assert repr(older) == repr(module)
