@@ -1409,24 +1409,20 @@ class PointwiseLayout:
     """A field type's flat layout as the pointwise entry points take it (host arrays)."""
 
     def __init__(self, field_type: Any):
+        self._field_type = field_type
+        self.D = field_type.dimension
+        self.a0 = field_type.multiplicity(0) if 0 in field_type else 0
         nonzero = [(n, field_type.multiplicity(n)) for n in field_type.frequencies if n != 0]
         slices = field_type.slices()
-        self._hold(field_type.dimension, field_type.multiplicity(0) if 0 in field_type else 0,
-                   [slices[n].start for n, _ in nonzero], [m for _, m in nonzero])
-
-    def _hold(self, D: int, a0: int, offsets: list[int], mults: list[int]) -> None:
-        self.D, self.a0, self.nf, self.G = D, a0, len(mults), sum(mults)
-        self.offsets = (ctypes.c_int64 * max(1, self.nf))(*offsets)
-        self.mults = (ctypes.c_int64 * max(1, self.nf))(*mults)
+        self.nf = len(nonzero)
+        self.offsets = (ctypes.c_int64 * max(1, self.nf))(*[slices[n].start for n, _ in nonzero])
+        self.mults = (ctypes.c_int64 * max(1, self.nf))(*[m for _, m in nonzero])
+        self.G = sum(m for _, m in nonzero)
         self._args = (self.D, self.a0, self.nf, ctypes.cast(self.offsets, _P), ctypes.cast(self.mults, _P))
         self._slots: dict[tuple[int, ...], tuple] = {}
 
-    def __getstate__(self) -> dict:  # a copy of a module that holds one makes its own arrays
-        return dict(D=self.D, a0=self.a0, nf=self.nf, offsets=list(self.offsets), mults=list(self.mults))
-
-    def __setstate__(self, state: dict) -> None:  # the host arrays themselves in modules pickled before
-        nf = state["nf"]
-        self._hold(state["D"], state["a0"], list(state["offsets"])[:nf], list(state["mults"])[:nf])
+    def __reduce__(self) -> tuple:  # a copy of a module that holds one makes its own arrays
+        return type(self), (self._field_type,)
 
     def args(self) -> tuple:
         return self._args

@@ -472,34 +472,6 @@ def test_a_used_module_is_copied():
     assert other._layout().parameter_slots(counts)[1:] == m._layout().parameter_slots(counts)[1:]
 
 
-@pytest.mark.parametrize("copies", [{0: 4, 1: 3, 2: 2}, {0: 5}, {1: 2}])
-def test_layouts_pickled_with_their_host_arrays_are_read(copies):
-    """A norm or gate pickled after a call held its layout with the host arrays and nothing else."""
-    import copyreg
-    import io
-
-    m = SO2LayerNorm(SO2FieldType(copies))
-    layout = m._layout()
-
-    class Older(pickle.Pickler):
-        def reducer_override(self, obj):
-            if obj is not layout:
-                return NotImplemented
-            held = {n: getattr(obj, n) for n in ("D", "a0", "nf", "offsets", "mults", "G")}
-            return copyreg.__newobj__, (type(obj),), held
-
-    written = io.BytesIO()
-    Older(written).dump(m)
-    other = pickle.loads(written.getvalue())
-    for read in (other, copy.deepcopy(other), pickle.loads(pickle.dumps(other))):
-        got = read._layout()
-        assert got is not layout and got.args()[:3] == layout.args()[:3] and got.G == layout.G
-        assert list(got.offsets) == list(layout.offsets) and list(got.mults) == list(layout.mults)
-        assert got.args()[3].value != layout.args()[3].value
-        counts = (len(copies), int(0 in copies), 0, 0, 0)
-        assert got.parameter_slots(counts)[1:] == layout.parameter_slots(counts)[1:]
-
-
 # ------------------------------------------------------- where the parameters are read
 
 
