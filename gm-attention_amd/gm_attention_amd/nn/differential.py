@@ -294,8 +294,8 @@ def attention_weights(mhsa: Any, q: Tensor, k: Tensor, edges: Any) -> Tensor:
         table = torch.float32 if q.dtype == torch.bfloat16 else q.dtype
         tables = edge_tables(edges, mhsa.cutoff, window, table, maps.max_frequency)
         return differential_softmax(q, k, lam, tables, maps, mhsa.num_heads)
-    held = maps_of(maps, mhsa.num_heads)
-    weights = fused_attention.softmax_eager(held.plan, q, k, edges, mhsa.cutoff, window, held.scale)
+    plan = fused_attention.plan_of(maps, mhsa.field_type_in, 2 * mhsa.num_heads)  # of any size, unlike the op's
+    weights = fused_attention.softmax_eager(plan, q, k, edges, mhsa.cutoff, window, 1.0 / math.sqrt(maps.dimension))
     return weights[:, 0::2] - lam.to(weights.dtype) * weights[:, 1::2]
 
 

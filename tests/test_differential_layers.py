@@ -336,3 +336,25 @@ def test_modules_pickled_before_there_were_the_options_run_as_they_did():
             want, got = run(module, x, edges, probe, chunk), run(older, x, edges, probe, chunk)
             assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
         assert repr(older) == repr(module)
+
+
+@pytest.mark.parametrize("field,heads", [({0: 34, 1: 34}, 17), ({f: 2 for f in range(9)}, 1), ({0: 1028}, 1)])
+def test_layers_beyond_the_ops_bounds_run_in_torch(field, heads):
+    """More heads, frequencies or numbers a row than the fused op takes."""
+    from gm_attention_amd.nn import differential
+
+    cutoff = math.pi / 3
+    edges = SphericalDiscretization.from_grid(build_equiangular_grid(10, 20), cutoff, max_frequency=8).edge_geometry
+    module = SO2MHSA(SO2FieldType(field), heads, cutoff=cutoff, window="quartic", batched=True, differential=True,
+                     dtype=D64)
+    q, k = (problems.normal((edges.row_ptr.shape[0] - 1, module.field_type_in.dimension), i) for i in range(2))
+    got = differential.attention_weights(module, q, k, edges)
+    t = problems.tables(10, 20, window="quartic")
+    transport = torch.view_as_real(edges.transport_phases)
+    rows, at = [], 0
+    for f, m in field.items():
+        rows.append((f, m // (2 * heads), at, 0, 1 if f == 0 else 2))
+        at += m * (1 if f == 0 else 2)
+    maps = eager.softmax_op(q, k, transport, t.bias, t.inside, rows, t.row_ptr, t.source, 2 * heads,
+                            (at / (2 * heads)) ** -0.5)
+    torch.testing.assert_close(got, maps[:, 0::2] - module.lambdas() * maps[:, 1::2], rtol=1e-10, atol=1e-12)
