@@ -83,10 +83,14 @@ class EdgeTables:
         self._sources, self._classes = None, {}
         masked = bias.detach().masked_fill(inside == 0, -math.inf)
         phases = transport.detach()[:, 1:].reshape(n_edges, 2 * (self.orders - 1))
+        self._hold(source.detach(), phases, masked)
+
+    def _hold(self, source: Tensor, phases: Tensor, masked: Tensor) -> None:
+        """The checked tables in the form their device reads."""
         if self.device.type != "cuda":
-            self._source, self._phases, self._bias = source.detach(), phases, masked
+            self._source, self._phases, self._bias = source, phases, masked
             return
-        records = torch.empty(n_edges, 2 * self.orders, dtype=self.dtype, device=self.device)
+        records = torch.empty(self.n_edges, 2 * self.orders, dtype=self.dtype, device=self.device)
         words = records.view(_WORD[self.dtype])
         words[:, 0] = source
         # in units of log 2; the type's lowest value stays a finite one
@@ -95,6 +99,23 @@ class EdgeTables:
         records[:, 2:] = phases
         self.records = records
         self._kept = [_native.Made(self.row_ptr, records)]
+
+    def __getstate__(self) -> dict:
+        """A copy (of the edge set that keeps them too) takes the tables alone: what is
+        found from them is found again, and a stream's events are not copied."""
+        if self.device.type == "cuda":
+            self.found()
+        return {n: v for n, v in self.__dict__.items() if n not in ("_kept", "_sources", "_classes")}
+
+    def __setstate__(self, state: dict) -> None:
+        self.__dict__.update(state, _sources=None, _classes={}, device=state["row_ptr"].device)
+        if self.device.type == "cuda" and "records" in state:
+            self._kept = [_native.Made(self.row_ptr, self.records)]
+        elif self.device.type == "cuda":  # read back on another device than the one they were written from
+            self._hold(*(self.__dict__.pop(n) for n in ("_source", "_phases", "_bias")))
+        elif "records" in state:
+            records = self.__dict__.pop("records")
+            self._hold(records.view(_WORD[self.dtype])[:, 0].long(), records[:, 2:], records[:, 1] / _LOG2E)
 
     def group_sources(self) -> tuple[Tensor, Tensor]:
         """``(src_ptr, records_s)``: the edges sorted by source, each with its target,

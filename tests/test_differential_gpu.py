@@ -13,8 +13,10 @@ itself.  A result held in bfloat16 is off by another eps / 2 = 2^-8 of its value
 """
 
 import concurrent.futures
+import copy
 import itertools
 import math
+import pickle
 
 import pytest
 import torch
@@ -643,3 +645,46 @@ def test_maps_made_under_a_default_device_serve_every_call():
         held = differential.maps_of(map_type, 3)
     assert differential.maps_of(map_type, 3) is held
     assert held.desc.device.type == "cpu" and held.slots(tables) == 4
+
+
+# ------------------------------------------------------------- copies of the tables
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("rows", [torch.float32, torch.float64])
+def test_copied_tables_give_the_same_results(rows, cuda, tmp_path):
+    copies, heads = {0: 2, 1: 2, 2: 2}, 4
+    graph = scattered([3, 0, 70, 9, 1, 200], 40, rows)
+    tables = graph.tables(rows, cuda)
+    values = inputs(graph, copies, heads, rows)
+    want = run(graph, tables, *values, copies, heads, rows, cuda)
+    torch.save(tables, tmp_path / "tables")
+    for other in (copy.deepcopy(tables), pickle.loads(pickle.dumps(tables)),
+                  torch.load(tmp_path / "tables", weights_only=False)):
+        got = run(graph, other, *values, copies, heads, rows, cuda)
+        assert all(torch.equal(got[n], want[n]) for n in want)
+    read = torch.load(tmp_path / "tables", weights_only=False, map_location="cpu")
+    assert read.device.type == "cpu"
+    got = run(graph, read, *values, copies, heads, rows, "cpu")
+    want = oracle(graph, *values, copies, heads, torch.finfo(rows).eps)
+    for name in want:  # the biases were kept in units of log 2: two roundings, of the many the bound counts for them
+        compare(got[name], want[name], name)
+
+
+def test_copied_tables_on_the_cpu_give_the_same_results():
+    copies, heads, rows = {0: 2, 1: 2}, 2, torch.float64
+    graph = scattered([3, 0, 70, 9, 1], 40, rows)
+    tables = graph.tables(rows, "cpu")
+    values = inputs(graph, copies, heads, rows)
+    want = run(graph, tables, *values, copies, heads, rows, "cpu")
+    for other in (copy.deepcopy(tables), pickle.loads(pickle.dumps(tables))):
+        got = run(graph, other, *values, copies, heads, rows, "cpu")
+        assert all(torch.equal(got[n], want[n]) for n in want)
+
+
+def test_what_a_stream_made_stays_out_of_a_copy():
+    """Beside the tables their owner keeps the events of the streams that made them, which are not copied."""
+    tables = scattered([3, 0, 7], 4, torch.float64).tables(torch.float64, "cpu")
+    tables._kept = [torch.cuda.Event.__new__(torch.cuda.Event)]
+    tables._classes[("targets", 4)] = (None, tables._kept[0])
+    assert copy.deepcopy(tables)._classes == {} and not hasattr(pickle.loads(pickle.dumps(tables)), "_kept")

@@ -235,6 +235,44 @@ def test_switched_off_the_layer_runs_in_torch(cuda, monkeypatch):
         close(plain[2][n], fused[2][n], D64, f"d{n}")
 
 
+@pytest.mark.gpu
+@pytest.mark.parametrize("gate,scale", [("sigmoid", 0.5), (None, None)])
+def test_a_replica_of_a_block_gives_its_results(gate, scale, cuda):
+    """A data-parallel step's replica, whose parameters are plain attributes."""
+    from torch.nn.parallel import replicate
+
+    module = block({0: 8, 1: 8, 2: 8}, 2, True, gate, scale, dtype=torch.float32, device=cuda)
+    edges = edges_of()[0].to(cuda, torch.float32)
+    x = problems.normal((edges.row_ptr.shape[0] - 1, 40), 1).float().to(cuda)
+    (replica,) = replicate(module, [cuda])
+    params = list(module.parameters())
+
+    def step(m):
+        out = m.forward_flat(x, edges)
+        return [out, *torch.autograd.grad((out * x).sum(), params, allow_unused=True)]
+
+    want = step(module)
+    for a, b, name in zip(step(replica), want, ["out", *(n for n, _ in module.named_parameters())], strict=True):
+        # a replica's matrices are built, not assembled: the same numbers in another order
+        close(a, torch.zeros_like(a) if b is None else b, torch.float32, name, reduction=True)
+
+
+@pytest.mark.gpu
+def test_edge_sets_are_copied_and_saved_after_a_step(cuda):
+    """An edge set that a differential layer has run on is copied and pickled as any other."""
+    import copy
+    import pickle
+
+    module = layer({0: 8, 1: 8, 2: 8}, 2, torch.float32, cuda)
+    edges = edges_of(2)[0].to(cuda, torch.float32)
+    n = edges.row_ptr.shape[0] - 1
+    x, probe = problems.normal((n, 40), 1).float().to(cuda), problems.normal((n, 40), 7)
+    want = run(module, x, edges, probe)
+    for other in (copy.deepcopy(edges), pickle.loads(pickle.dumps(edges))):
+        got = run(module, x, other, probe)
+        assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
+
+
 # ---------------------------------------------------------------- without a GPU
 
 
