@@ -52,7 +52,7 @@ from gm_attention_amd.nn.convolution import SO2Convolution
 from gm_attention_amd.nn.fused_attention import evaluate_aggregation_window
 from gm_attention_amd.nn.kernels import SO2SteerableKernel
 from gm_attention_amd.nn import ffn
-from gm_attention_amd.nn.linear import SO2Linear, flat_forward
+from gm_attention_amd.nn.linear import SO2Linear, flat_forward, parameter_dtype
 from gm_attention_amd.nn.nonlinearities import SO2ScalarGatedNonlinearity
 from gm_attention_amd.nn.normalization import SO2Dropout, SO2LayerNorm
 from gm_attention_amd.nn.residual import SO2ResidualNorm
@@ -159,7 +159,7 @@ class SO2TransformerBlock(nn.Module):
             field = SO2FeatureField.from_flat(self.field_type, h)
             if batched_flat_serves(self.attention, field, edges):
                 return self.attention(field, edges)._rows()
-        pdtype = next(self.attention.parameters()).dtype
+        pdtype = parameter_dtype(self.attention)
         field = SO2FeatureField.from_flat(self.field_type, h.to(pdtype))
         if chunk_size is None:
             out = self.attention(field, edges)

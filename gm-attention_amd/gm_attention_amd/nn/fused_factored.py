@@ -34,6 +34,7 @@ from torch import Tensor
 
 from gm_attention_amd import _native
 from gm_attention_amd.nn import assembly
+from gm_attention_amd.nn.linear import parameter_dtype
 from gm_attention_amd.representations.field_type import SO2FeatureField, SO2FieldType
 
 MAX_K, MAX_OUT, MAX_BM, MAX_C, DESC = 20, 128, 32, 320, 8
@@ -357,7 +358,7 @@ def tiles(kernel: Any) -> tuple[Tile, ...] | None:
         out_type = kernel.field_type_out
         slices = out_type.slices()
         # float32 tiles stay within the MFMA kernels' packed width
-        width = MAX_C_MFMA if next(kernel.parameters()).dtype == torch.float32 else MAX_C
+        width = MAX_C_MFMA if parameter_dtype(kernel) == torch.float32 else MAX_C
 
         def fits(rows, zc_cols, zr_cols, out_cols) -> bool:
             # the op takes one real block, covering the tile's real mixes

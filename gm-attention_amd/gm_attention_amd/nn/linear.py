@@ -124,6 +124,16 @@ def flat_bias(bias: Tensor | None, fout: SO2FieldType) -> Tensor | None:
     return torch.cat([bias, bias.new_zeros(fout.dimension - fout.multiplicity(0))])
 
 
+def parameter_dtype(module: nn.Module) -> torch.dtype:
+    """The dtype of a module's first parameter; a data-parallel replica's are plain
+    attributes, which it lists apart."""
+    for m in module.modules():
+        for p in (*m._parameters.values(), *m.__dict__.get("_former_parameters", {}).values()):
+            if p is not None:
+                return p.dtype
+    raise ValueError(f"{type(module).__name__} has no parameters.")
+
+
 def linear_parameters(lin: "SO2Linear") -> list[Tensor]:
     """The layer's weights by frequency, then its bias where it has one."""
     weights = [lin.weight[str(f)] for f in lin.common_frequencies]
