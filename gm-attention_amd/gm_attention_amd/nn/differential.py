@@ -28,8 +28,10 @@ from __future__ import annotations
 import ctypes
 import functools
 import math
+from collections import OrderedDict
 from typing import Any
 
+import numpy as np
 import torch
 from torch import Tensor
 
@@ -305,6 +307,76 @@ def edge_tables(edges: Any, cutoff: float, window: str, dtype: torch.dtype, top:
     return held
 
 
+class _Ranges:
+    """The tables of an edge set's chunks, ``{(e0, e1): (tables, first target, first source)}``:
+    the ranges found last, up to ``limit`` edges of them.  A range that a captured graph
+    reads stays."""
+
+    def __init__(self, limit: int) -> None:
+        self.limit, self.edges = limit, 0
+        self.held: OrderedDict[tuple[int, int], tuple[EdgeTables, int, int]] = OrderedDict()
+        self.captured: dict[tuple[int, int], tuple[EdgeTables, int, int]] = {}
+
+    def find(self, span: tuple[int, int]) -> tuple[EdgeTables, int, int] | None:
+        with _native.LOCK:
+            found = self.captured.get(span)
+            if found is None and (found := self.held.get(span)) is not None:
+                if found[0].device.type == "cuda" and torch.cuda.is_current_stream_capturing():
+                    self.captured[span] = self.held.pop(span)
+                    self.edges -= found[0].n_edges
+                else:
+                    self.held.move_to_end(span)
+            return found
+
+    def keep(self, span: tuple[int, int], made: tuple[EdgeTables, int, int]) -> tuple[EdgeTables, int, int]:
+        with _native.LOCK:
+            found = self.find(span)
+            if found is not None:  # another thread was first
+                return found
+            self.held[span] = made
+            self.edges += made[0].n_edges
+            while self.edges > self.limit:
+                self.edges -= self.held.popitem(last=False)[1][0].n_edges
+            return made
+
+
+def chunk_tables(chunk: Any, cutoff: float, window: str, dtype: torch.dtype,
+                 top: int) -> tuple[EdgeTables, int, int]:
+    """The tables of a chunk (``EdgeGeometry.chunks``) over its own targets and the range of
+    nodes its sources lie in, and the first of each.  Chunks are made anew for every pass:
+    the tables are kept with the edge set they are ranges of, as many as two passes over all
+    of its edges take, where a range's lists of nodes take no more than its edges (a chunk
+    with sources all over a large set keeps its own)."""
+    parent, e0, e1 = fused_attention.chunk_of(chunk)
+    outer = fused_attention.geometry(parent, cutoff, window, dtype)
+    ranges = outer.derived.get(("differential ranges", top))
+    if ranges is None:
+        with _native.LOCK:
+            ranges = outer.derived.setdefault(("differential ranges", top), _Ranges(2 * int(parent.n_edges)))
+    # an edge set registered as a chunk under numbers of its own is not the range of its span
+    same = (chunk.edge_index.data_ptr() == parent.edge_index[:, e0:].data_ptr()
+            and chunk.row_ptr.shape == parent.row_ptr.shape)
+    found = ranges.find((e0, e1)) if same else None
+    if found is not None:
+        return found
+    g = fused_attention.geometry(chunk, cutoff, window, dtype)
+    found = g.derived.get(("differential range", top))
+    if found is not None:
+        return found
+    _outside_capture(g.row_ptr, "EdgeTables")
+    ptr, begin = (outer.host_row_ptr(), e0) if same else (g.host_row_ptr(), 0)
+    first = int(np.searchsorted(ptr, begin, side="right")) - 1
+    last = int(np.searchsorted(ptr, begin + e1 - e0, side="left"))
+    source, behind = int(g.source.min()), int(g.source.max()) + 1
+    made = EdgeTables(g.row_ptr[first:last + 1], g.source - source, g.transport[:, : top + 1], g.bias, g.inside,
+                      n_sources=behind - source), first, source
+    # 12 bytes a node of either list, 24 and 32 an edge at two orders
+    if same and made[0].n_targets + made[0].n_sources <= 4 * (e1 - e0):
+        return ranges.keep((e0, e1), made)
+    with _native.LOCK:
+        return g.derived.setdefault(("differential range", top), made)
+
+
 def attention_weights(mhsa: Any, q: Tensor, k: Tensor, edges: Any) -> Tensor:
     """A differential layer's weights ``(n_edges, n_heads)`` from its flat query and
     key rows: the fused op where it serves, else the single softmax's eager
@@ -313,7 +385,11 @@ def attention_weights(mhsa: Any, q: Tensor, k: Tensor, edges: Any) -> Tensor:
     window = mhsa.heads[0].window
     if enabled(mhsa, q, edges):
         table = torch.float32 if q.dtype == torch.bfloat16 else q.dtype
-        tables = edge_tables(edges, mhsa.cutoff, window, table, maps.max_frequency)
+        if fused_attention.chunk_of(edges) is not None:
+            tables, first, source = chunk_tables(edges, mhsa.cutoff, window, table, maps.max_frequency)
+            q, k = q[first:first + tables.n_targets], k[source:source + tables.n_sources]
+        else:
+            tables = edge_tables(edges, mhsa.cutoff, window, table, maps.max_frequency)
         return differential_softmax(q, k, lam, tables, maps, mhsa.num_heads)
     plan = fused_attention.plan_of(maps, mhsa.field_type_in, 2 * mhsa.num_heads)  # of any size, unlike the op's
     weights = fused_attention.softmax_eager(plan, q, k, edges, mhsa.cutoff, window, 1.0 / math.sqrt(maps.dimension))

@@ -276,6 +276,51 @@ def test_edge_sets_are_copied_and_saved_after_a_step(cuda):
         assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
 
 
+@pytest.mark.gpu
+@pytest.mark.parametrize("train", [True, False])
+def test_a_chunked_step_builds_its_tables_once_and_is_captured(train, cuda, monkeypatch):
+    from gm_attention_amd.nn import differential
+
+    module = layer({0: 16, 1: 16, 2: 16}, 4, torch.float32, cuda).train(train)
+    edges = edges_of(2)[0].to(cuda, torch.float32)
+    n = edges.row_ptr.shape[0] - 1
+    x, up = (problems.normal((n, 80), i).float().to(cuda) for i in (1, 7))
+    built, init = [], differential.EdgeTables.__init__
+    monkeypatch.setattr(differential.EdgeTables, "__init__",
+                        lambda self, *a, **kw: (built.append(1), init(self, *a, **kw))[1])
+
+    def step():
+        leaf = x.detach().requires_grad_(train)
+        with torch.set_grad_enabled(train):
+            out = module.forward_chunked(SO2FeatureField.from_flat(module.field_type_in, leaf), edges,
+                                         chunk_size=75).to_flat()
+        return [out.detach(), *(torch.autograd.grad(out, leaf, up) if train else ())]
+
+    want = [t.clone() for t in step()]
+    chunks = sum(1 for _ in edges.chunks(75))
+    assert len(built) == chunks == 6
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        step()
+    torch.cuda.current_stream().wait_stream(side)
+    captured = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(captured):
+        got = step()
+    assert len(built) == chunks
+    for size in (40, 50, 60, 90):  # other chunkings, beyond what is kept of them
+        with torch.no_grad():
+            module.forward_chunked(SO2FeatureField.from_flat(module.field_type_in, x), edges, chunk_size=size)
+    for replay in range(3):
+        for t in got:
+            t.zero_()
+        captured.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(got, want, strict=True)), replay
+        assert all(torch.equal(a, b) for a, b in zip(step(), want, strict=True)), replay
+        torch.cuda.synchronize()
+
+
 # ---------------------------------------------------------------- without a GPU
 
 
@@ -432,3 +477,49 @@ def test_replicas_of_blocks_give_their_results(placement, mixer):
         for a, b in ((replica.residual1, module.residual1), (replica.residual2, module.residual2)):
             (counts, mine), (want, theirs) = a._params(), b._params()
             assert counts == want and all(torch.equal(p, q) for p, q in zip(mine, theirs, strict=True))
+
+
+def test_chunks_tables_are_kept_with_the_edge_set():
+    """Every pass over the chunks finds the tables of the first, over the chunk's own targets and the range of
+    its sources, and its weights are the whole edge set's."""
+    from gm_attention_amd.nn import differential
+
+    edges, cutoff = edges_of(2)
+    n, maps, heads = edges.row_ptr.shape[0] - 1, SO2FieldType({0: 2, 1: 1}), 2
+    q, k = (problems.normal((n, 16), i) for i in range(2))
+    lam = torch.tensor([0.3, 0.6], dtype=D64)
+    whole = differential.edge_tables(edges, cutoff, "quartic", D64, 1)
+    want = differential.differential_softmax(q, k, lam, whole, maps, heads)
+    first_pass, got = [], []
+    for chunk in edges.chunks(37):
+        tables, first, source = differential.chunk_tables(chunk, cutoff, "quartic", D64, 1)
+        first_pass.append(tables)
+        assert tables.n_targets <= 37 and tables.n_sources < n  # but for a sample's border, a band of rows
+        got.append(differential.differential_softmax(q[first:first + tables.n_targets],
+                                                     k[source:source + tables.n_sources], lam, tables, maps, heads))
+    torch.testing.assert_close(torch.cat(got), want, rtol=1e-13, atol=1e-15)
+    for chunk, held in zip(edges.chunks(37), first_pass, strict=True):
+        assert differential.chunk_tables(chunk, cutoff, "quartic", D64, 1)[0] is held
+    # other chunkings: what is kept stays within two passes over the edges
+    for size in (11, 50, 60, 90):
+        for chunk in edges.chunks(size):
+            differential.chunk_tables(chunk, cutoff, "quartic", D64, 1)
+    from gm_attention_amd.nn import fused_attention
+
+    ranges = fused_attention.geometry(edges, cutoff, "quartic", D64).derived["differential ranges", 1]
+    assert sum(t.n_edges for t, *_ in ranges.held.values()) == ranges.edges <= 2 * edges.n_edges
+
+
+def test_a_chunk_under_numbers_of_its_own_has_tables_of_its_own():
+    """An edge set registered as a chunk keeps its own: another may have its span with other numbers."""
+    from gm_attention_amd.nn import differential, fused_attention
+
+    edges, cutoff = edges_of()
+    (chunk, *_), n = list(edges.chunks(50)), edges.row_ptr.shape[0] - 1
+    own = chunk.select(torch.arange(chunk.n_edges), n_nodes=n)  # copies, not views
+    fused_attention.register_chunk(own, edges, 0, chunk.n_edges)
+    mine = differential.chunk_tables(own, cutoff, "quartic", D64, 1)
+    theirs = differential.chunk_tables(chunk, cutoff, "quartic", D64, 1)
+    assert mine[0] is not theirs[0] and mine[1:] == theirs[1:]
+    assert torch.equal(mine[0].row_ptr, theirs[0].row_ptr) and torch.equal(mine[0]._source, theirs[0]._source)
+    assert differential.chunk_tables(own, cutoff, "quartic", D64, 1)[0] is mine[0]
