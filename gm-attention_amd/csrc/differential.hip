@@ -11,11 +11,11 @@
 //   dq_i = sum_e ds tau k_j,  dk_j = sum_e ds conj(tau) q_i
 //   dlambda_h = - sum_i T_2h+1(i).
 //
-// Neither the maps nor ds are written: the forward keeps log sum exp s_p of every
-// target, the backward forms a_p again from it.  The pass over the targets needs
+// Neither the maps nor ds are written: the forward keeps the maximum of s_p and its
+// weights' sum for every target, the backward forms a_p again from them.  The pass over the targets needs
 // no second walk for T either: sum ds tau k = scale c (sum a g tau k - T sum a tau k),
 // two sums beside T in one walk (each off by the roundings T itself has, times
-// sum a tau k).  The pass over the sources reads T and the log sums of its edges'
+// sum a tau k).  The pass over the sources reads T and both numbers of its edges'
 // targets.  No atomics: sums are in a fixed order.
 //
 // Per edge both passes read one record of 32-bit words (64-bit for double): the
@@ -113,7 +113,10 @@ __global__ __launch_bounds__(256) void differential_forward_generic(DfArgs<T, R>
     }
   l = group_sum(l, lane, P, S);
   const T inv = l == T(0) ? T(0) : T(1) / l;
-  if (a.lse && lane < P) a.lse[i * P + p] = l == T(0) ? neg_inf<T>() : m + df_log2(l);
+  if (a.stats && lane < P) {
+    a.stats[(i * P + p) * 2] = m == neg_inf<T>() ? T(0) : m;
+    a.stats[(i * P + p) * 2 + 1] = inv;
+  }
   const T lambda = a.lambda[p >> 1];
   for (int64_t e = e0; e < e1; e += S) {  // whole waves: the pair's second map comes by a shuffle
     const bool live = s < S && e + s < e1;
@@ -136,19 +139,20 @@ __global__ __launch_bounds__(256) void differential_backward_scores_generic(DfAr
   const int P = a.L.P, S = kWave / P, p = lane % P, s = lane / P;
   const int64_t e0 = a.row_ptr[i], e1 = a.row_ptr[i + 1];
   const R* qi = a.q + i * a.L.D;
-  const T lse = a.lse[i * P + p];
+  const T m = a.stats[(i * P + p) * 2], inv = a.stats[(i * P + p) * 2 + 1];
   T total = T(0);
   if (s < S)
     for (int64_t e = e0 + s; e < e1; e += S) {
       const T lw = generic_logit(a, qi, e, p);
-      const T w = lw == neg_inf<T>() ? T(0) : df_exp2(lw - lse);
+      const T w = lw == neg_inf<T>() ? T(0) : df_exp2(lw - m) * inv;
       if (lw != neg_inf<T>()) total += w * a.g[e * a.L.H + (p >> 1)];
       a.ds[e * P + p] = w;
     }
   total = group_sum(total, lane, P, S);
   if (lane < P) {
-    a.pairs[(i * P + p) * 2] = lse;
-    a.pairs[(i * P + p) * 2 + 1] = total;
+    a.rows[(i * P + p) * 3] = m;
+    a.rows[(i * P + p) * 3 + 1] = inv;
+    a.rows[(i * P + p) * 3 + 2] = total;
   }
   const T factor = a.gradient_scale * ((p & 1) ? -a.lambda[p >> 1] : T(1));
   if (s < S)
@@ -236,14 +240,14 @@ __global__ __launch_bounds__(256) void differential_backward_source_generic(DfAr
 constexpr int kLambdaBlocks = 256;
 
 template <typename T>
-__global__ __launch_bounds__(256) void differential_lambda_partial(const T* pairs, int64_t n_targets, int H,
+__global__ __launch_bounds__(256) void differential_lambda_partial(const T* rows, int64_t n_targets, int H,
                                                                    double* partial) {
   __shared__ double sums[256];
   const int per = 256 / H, h = threadIdx.x % H, at = threadIdx.x / H;  // 256 / H targets a step
   double s = 0.0;
   if (at < per)
     for (int64_t i = (int64_t)blockIdx.x * per + at; i < n_targets; i += (int64_t)gridDim.x * per)
-      s -= (double)pairs[((i * H + h) * 2 + 1) * 2 + 1];
+      s -= (double)rows[((i * H + h) * 2 + 1) * 3 + 2];
   sums[threadIdx.x] = s;
   __syncthreads();
   if (threadIdx.x < H) {
@@ -331,8 +335,8 @@ int df_rows(const DfArgs<T, R>& a, const int32_t* order, const int64_t* counts, 
   }
   GM_REQUIRE(sum == n, "the classes must hold every row once");
   GM_REQUIRE(aligned(a.q, 16) && aligned(a.k, 16) && aligned(a.dq, 16) && aligned(a.dk, 16) && aligned(a.records, 8) &&
-                 aligned(a.records_s, 8) && aligned(a.pairs, 16),
-             "the lane kernels take rows and pairs at multiples of 16 bytes");
+                 aligned(a.records_s, 8) && aligned(a.stats, 8),
+             "the lane kernels take rows at multiples of 16 bytes, records and statistics of 8");
   return GM_OK;
 }
 
@@ -340,7 +344,7 @@ template <typename T, typename R>
 int differential_forward(const R* q, const R* k, const T* lambda, const T* records, const int64_t* desc,
                          const int64_t* row_ptr, const int32_t* order, const int64_t* counts, int64_t n_targets,
                          int64_t n_sources, int64_t n_edges, int64_t D, int64_t orders, int64_t F, int64_t H,
-                         double scale, T* alpha, T* lse, void* stream) {
+                         double scale, T* alpha, T* stats, void* stream) {
   DfArgs<T, R> a{};
   const int rc = df_prepare(a, q, k, lambda, records, desc, row_ptr, n_targets, n_sources, n_edges, D, orders, F, H,
                             scale);
@@ -348,7 +352,7 @@ int differential_forward(const R* q, const R* k, const T* lambda, const T* recor
   if (n_targets == 0) return GM_OK;
   if (n_edges > 0) GM_REQUIRE(alpha, "alpha must be a device pointer");
   a.alpha = alpha;
-  a.lse = lse;
+  a.stats = stats;
   DfRows rows;
   const int status = df_rows(a, order, counts, n_targets, rows);
   if (status != GM_OK) return status;
@@ -365,14 +369,14 @@ int differential_backward(const T* g, const R* q, const R* k, const T* lambda, c
                           const int64_t* desc, const int64_t* row_ptr, const int64_t* src_ptr, const int32_t* order,
                           const int64_t* counts, const int32_t* order_s, const int64_t* counts_s, int64_t n_targets,
                           int64_t n_sources, int64_t n_edges, int64_t D, int64_t orders, int64_t F, int64_t H,
-                          double scale, const T* lse, T* pairs, T* ds, double* partial, R* dq, R* dk, T* dlambda,
+                          double scale, const T* stats, T* rows, T* ds, double* partial, R* dq, R* dk, T* dlambda,
                           void* stream) {
   DfArgs<T, R> a{};
   const int rc = df_prepare(a, q, k, lambda, records, desc, row_ptr, n_targets, n_sources, n_edges, D, orders, F, H,
                             scale);
   if (rc != GM_OK) return rc;
   GM_REQUIRE(partial && dlambda, "partial and dlambda must be device pointers");
-  if (n_targets > 0) GM_REQUIRE(lse && pairs && dq, "lse, pairs and dq must be device pointers");
+  if (n_targets > 0) GM_REQUIRE(stats && rows && dq, "stats, rows and dq must be device pointers");
   if (n_sources > 0) GM_REQUIRE(src_ptr && dk, "src_ptr and dk must be device pointers");
   if (n_edges > 0) GM_REQUIRE(g && records_s, "g and the sources' records must be device pointers");
   GM_REQUIRE(!order == !order_s || n_targets == 0 || n_sources == 0, "both sides' rows are in classes, or neither's");
@@ -381,8 +385,8 @@ int differential_backward(const T* g, const R* q, const R* k, const T* lambda, c
   a.g = g;
   a.records_s = records_s;
   a.src_ptr = src_ptr;
-  a.lse = const_cast<T*>(lse);  // read only here
-  a.pairs = pairs;
+  a.stats = const_cast<T*>(stats);  // read only here
+  a.rows = rows;
   a.ds = ds;
   a.dq = dq;
   a.dk = dk;
@@ -406,7 +410,7 @@ int differential_backward(const T* g, const R* q, const R* k, const T* lambda, c
   if (n_sources > 0 && !lanes)
     hipLaunchKernelGGL((differential_backward_source_generic<T, R>), dim3((unsigned)blocks_for(n_sources)), dim3(256),
                        0, s, a);
-  hipLaunchKernelGGL(differential_lambda_partial<T>, dim3(kLambdaBlocks), dim3(256), 0, s, (const T*)pairs, n_targets,
+  hipLaunchKernelGGL(differential_lambda_partial<T>, dim3(kLambdaBlocks), dim3(256), 0, s, (const T*)rows, n_targets,
                      (int)H, partial);
   hipLaunchKernelGGL(differential_lambda_sum<T>, dim3((unsigned)H), dim3(64), 0, s, (const double*)partial,
                      kLambdaBlocks, (int)H, dlambda);
@@ -433,19 +437,19 @@ extern "C" int gm_differential_slots(const int64_t* desc, int64_t F, int64_t H, 
   extern "C" int gm_differential_forward_##SFX(                                                                       \
       const R* q, const R* k, const T* lambda, const T* records, const int64_t* desc, const int64_t* row_ptr,         \
       const int32_t* order, const int64_t* counts, int64_t n_targets, int64_t n_sources, int64_t n_edges, int64_t D,  \
-      int64_t orders, int64_t F, int64_t H, double scale, T* alpha, T* lse, void* stream) {                           \
+      int64_t orders, int64_t F, int64_t H, double scale, T* alpha, T* stats, void* stream) {                           \
     return gm::differential_forward<T, R>(q, k, lambda, records, desc, row_ptr, order, counts, n_targets, n_sources,  \
-                                          n_edges, D, orders, F, H, scale, alpha, lse, stream);                       \
+                                          n_edges, D, orders, F, H, scale, alpha, stats, stream);                       \
   }                                                                                                                   \
   extern "C" int gm_differential_backward_##SFX(                                                                      \
       const T* g, const R* q, const R* k, const T* lambda, const T* records, const T* records_s, const int64_t* desc, \
       const int64_t* row_ptr, const int64_t* src_ptr, const int32_t* order, const int64_t* counts,                    \
       const int32_t* order_s, const int64_t* counts_s, int64_t n_targets, int64_t n_sources, int64_t n_edges,         \
-      int64_t D, int64_t orders, int64_t F, int64_t H, double scale, const T* lse, T* pairs, T* ds, double* partial,  \
+      int64_t D, int64_t orders, int64_t F, int64_t H, double scale, const T* stats, T* rows, T* ds, double* partial,  \
       R* dq, R* dk, T* dlambda, void* stream) {                                                                       \
     return gm::differential_backward<T, R>(g, q, k, lambda, records, records_s, desc, row_ptr, src_ptr, order,        \
                                            counts, order_s, counts_s, n_targets, n_sources, n_edges, D, orders, F, H, \
-                                           scale, lse, pairs, ds, partial, dq, dk, dlambda, stream);                  \
+                                           scale, stats, rows, ds, partial, dq, dk, dlambda, stream);                  \
   }
 
 GM_DIFFERENTIAL_ENTRY(f32, float, float)

@@ -36,8 +36,8 @@ struct DfArgs {
   const int64_t* src_ptr;  // over sources
   const T* g;              // (n_edges, H)
   T* alpha;                // (n_edges, H)
-  T* lse;                  // (n_targets, 2 H): log2 sum 2^s (-inf where no edge is inside)
-  T* pairs;                // (n_targets, 2 H, 2): that beside T, the backward's workspace
+  T* stats;                // (n_targets, 2 H, 2): m, the largest s, and 1 / sum 2^(s - m) (zeros where no edge is inside)
+  T* rows;                 // (n_targets, 2 H, 3): both beside T, the backward's workspace
   T* ds;                   // (n_edges, 2 H): the generic backward's workspace
   R* dq;
   R* dk;
@@ -46,11 +46,11 @@ struct DfArgs {
   T gradient_scale;  // of the scores
 };
 
-// Scores, their biases and their log sums are in units of log 2: a weight is 2^(s - lse).
+// Scores, their biases and their maxima are in units of log 2: a weight is 2^(s - m) / sum 2^(s - m), in the backward
+// as in the forward.  (m + log2 of the sum as one number is as wrong as that number's spacing: beside a bias of -1e9 by
+// more than the sum itself, and the backward's weights were not the forward's.)
 constexpr double kLog2e = 1.4426950408889634074;
 
-__device__ __forceinline__ float df_log2(float x) { return log2f(x); }
-__device__ __forceinline__ double df_log2(double x) { return log2(x); }
 __device__ __forceinline__ float df_exp2(float x) { return exp2f(x); }
 __device__ __forceinline__ double df_exp2(double x) { return exp2(x); }
 __device__ __forceinline__ float df_widen(float x) { return x; }

@@ -331,8 +331,8 @@ __global__ __launch_bounds__(1024) void differential_forward_units(DfArgs<float,
     if (phase == 2) {
       l = over_waves(l, false);
       inv = l == 0.f ? 0.f : 1.f / l;
-      if (a.lse && sh.part == 0 && s == 0 && writes)
-        a.lse[(int64_t)sh.row * a.L.P + p] = l == 0.f ? neg_inf<float>() : m + log2f(l);
+      if (a.stats && sh.part == 0 && s == 0 && writes)
+        *reinterpret_cast<float2*>(a.stats + ((int64_t)sh.row * a.L.P + p) * 2) = make_float2(m, inv);
       for (int t = 0; t < held; t += 2) write(sh.e0, t, sc[t * kWave] * inv, sc[(t + 1) * kWave] * inv);
     }
     const int skip = phase == 0 ? 0 : kDfSteps;
@@ -440,7 +440,7 @@ void differential_backward_target_units(DfArgs<float, R> a, DfUnits w) {
   const float scale = a.scale;
   float q[U::N];
   U::template load<false>(a.q, w, unit, sh.row, q);
-  const float lse = a.lse[(int64_t)sh.row * a.L.P + p];
+  const float2 stats = *reinterpret_cast<const float2*>(a.stats + ((int64_t)sh.row * a.L.P + p) * 2);
   const bool second = p & 1;
   const int ahead = (second ? w.slots : 0) + s;
   float sums[M];
@@ -483,7 +483,7 @@ void differential_backward_target_units(DfArgs<float, R> a, DfUnits w) {
 #pragma unroll
       for (int n = 0; n < UN; ++n) {
         if (head[n].y != neg_inf<float>()) {
-          const float al = exp2_of(fmaf(scale, v[n], head[n].y - lse)), ag = al * g[n];
+          const float al = exp2_of(fmaf(scale, v[n], head[n].y) - stats.x), ag = al * g[n];
           U::turn(k[n], cs[n], sn[n], false);
           sums[2 * U::N] += ag;
 #pragma unroll
@@ -497,14 +497,14 @@ void differential_backward_target_units(DfArgs<float, R> a, DfUnits w) {
   }
   row_sums<M>(w, sh, sums, df_lds);
   if (sh.part == 0 && s == 0 && u < w.units) {
-    const float total = sums[2 * U::N];
-    const float factor = a.gradient_scale * ((p & 1) ? -a.lambda[p >> 1] : 1.f);
+    const float total = sums[2 * U::N] * stats.y;
+    const float factor = a.gradient_scale * ((p & 1) ? -a.lambda[p >> 1] : 1.f) * stats.y;
     float dq[U::N];
 #pragma unroll
     for (int i = 0; i < U::N; ++i) dq[i] = factor * (sums[i] - total * sums[U::N + i]);
     U::store(a.dq + (int64_t)sh.row * a.L.D, w, unit, dq);
     if (unit % w.per_map == 0)
-      *reinterpret_cast<float2*>(a.pairs + ((int64_t)sh.row * a.L.P + p) * 2) = make_float2(lse, total);
+      *reinterpret_cast<float3*>(a.rows + ((int64_t)sh.row * a.L.P + p) * 3) = make_float3(stats.x, stats.y, total);
   }
 }
 
@@ -539,7 +539,8 @@ void differential_backward_source_units(DfArgs<float, R> a, DfUnits w) {
     const int ends = sh.steps - b < w.lanes ? sh.steps - b : w.lanes;
     const int left = (int)(sh.e1 - e < kWave ? sh.e1 - e : kWave);
     for (int t = 0; t < ends; t += UN) {
-      float2 head[UN], pair[UN];
+      float2 head[UN];
+      float3 row[UN];
       float q[UN][U::N], bias[UN], cs[UN][U::NO], sn[UN][U::NO], g[UN], v[UN];
 #pragma unroll
       for (int n = 0; n < UN; ++n) {
@@ -561,13 +562,14 @@ void differential_backward_source_units(DfArgs<float, R> a, DfUnits w) {
         const int i = __float_as_int(head[n].x);
         U::template load<kNear>(a.q, w, unit, i, q[n]);
         if constexpr (kNear) {
-          pair[n] = *reinterpret_cast<const float2*>(reinterpret_cast<const char*>(a.pairs) +
-                                                     (__umul24((uint32_t)i, (uint32_t)(8 * a.L.P)) + 8u * (uint32_t)p));
+          row[n] = *reinterpret_cast<const float3*>(
+              reinterpret_cast<const char*>(a.rows) +
+              (__umul24((uint32_t)i, (uint32_t)(12 * a.L.P)) + 12u * (uint32_t)p));
           g[n] = *reinterpret_cast<const float*>(
               reinterpret_cast<const char*>(a.g) +
               (__float_as_uint(head[n].y) * (uint32_t)(4 * a.L.H) + 4u * (uint32_t)(p >> 1)));
         } else {
-          pair[n] = *reinterpret_cast<const float2*>(a.pairs + ((int64_t)i * a.L.P + p) * 2);
+          row[n] = *reinterpret_cast<const float3*>(a.rows + ((int64_t)i * a.L.P + p) * 3);
           g[n] = a.g[(int64_t)__float_as_int(head[n].y) * a.L.H + (p >> 1)];
         }
       }
@@ -577,8 +579,7 @@ void differential_backward_source_units(DfArgs<float, R> a, DfUnits w) {
 #pragma unroll
       for (int n = 0; n < UN; ++n) {
         if (bias[n] != neg_inf<float>()) {
-          const float al = exp2_of(fmaf(scale, v[n], bias[n] - pair[n].x));
-          const float ds = al * (g[n] - pair[n].y);
+          const float ds = exp2_of(fmaf(scale, v[n], bias[n]) - row[n].x) * (row[n].y * (g[n] - row[n].z));
           U::turn(q[n], cs[n], sn[n], true);
 #pragma unroll
           for (int i = 0; i < U::N; ++i) sums[i] = fmaf(ds, q[n][i], sums[i]);
@@ -698,7 +699,7 @@ int launch_units(DfPass pass, const DfArgs<float, R>& a, const DfRows& rows, hip
   w.row_bytes = (uint32_t)(a.L.D * sizeof(R));
   w.order = rows.order;
   const int64_t nodes = std::max(a.n_targets, a.n_sources), limit = int64_t(1) << 32;
-  const bool near = nodes < (int64_t(1) << 24) && nodes * w.row_bytes < limit && nodes * a.L.P * 8 < limit &&
+  const bool near = nodes < (int64_t(1) << 24) && nodes * w.row_bytes < limit && nodes * a.L.P * 12 < limit &&
                     a.n_edges * a.L.H * 4 < limit;
   return near ? launch_near<true>(pass, shape, a, w, rows, stream)
               : launch_near<false>(pass, shape, a, w, rows, stream);

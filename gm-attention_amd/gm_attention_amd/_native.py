@@ -1675,22 +1675,22 @@ def differential_slots(desc: Tensor, D: int, orders: int, H: int) -> int:
 
 def differential_forward(q: Tensor, k: Tensor, lam: Tensor, tables: Any, maps: Any, scale: float,
                          train: bool) -> tuple[Tensor, Tensor | None]:
-    """``(alpha (n_edges, H), lse)``: the differential softmax's weights and, under ``train``,
-    the log sums of exponentials ``(n_targets, 2 H)`` its backward reads.  The rows are whole
+    """``(alpha (n_edges, H), stats)``: the differential softmax's weights and, under ``train``, what its
+    backward reads of a target's maps ``(n_targets, 2 H, 2)``, the largest score and one over the weights' sum.  The rows are whole
     (contiguous, at multiples of 16 bytes) and match the tables: nn.differential's checks."""
     H, desc, device = maps.heads, maps.desc, q.device
     order, counts = tables.target_rows(maps.slots(tables))
     tables.found()
     alpha = torch.empty(tables.n_edges, H, dtype=tables.dtype, device=device)
-    lse = torch.empty(tables.n_targets, 2 * H, dtype=tables.dtype, device=device) if train else None
+    stats = torch.empty(tables.n_targets, 2 * H, 2, dtype=tables.dtype, device=device) if train else None
     _call_on(device, "gm_differential_forward_" + _PW_SUFFIX[q.dtype], _ptr(q), _ptr(k), _ptr(lam),
              _ptr(tables.records), desc.data_ptr(), _ptr(tables.row_ptr), _ptr(order), counts, tables.n_targets,
              tables.n_sources, tables.n_edges, q.shape[1], tables.orders, desc.shape[0], H, scale, _ptr(alpha),
-             _ptr(lse), _stream(device))
-    return alpha, lse
+             _ptr(stats), _stream(device))
+    return alpha, stats
 
 
-def differential_backward(g: Tensor, q: Tensor, k: Tensor, lam: Tensor, lse: Tensor, tables: Any, maps: Any,
+def differential_backward(g: Tensor, q: Tensor, k: Tensor, lam: Tensor, stats: Tensor, tables: Any, maps: Any,
                           scale: float) -> tuple[Tensor, Tensor, Tensor]:
     """``(dq, dk, dlam)`` of what a forward took and gave and the weights' gradient (contiguous): the rows'
     gradients in their dtype, the factors' in the tables'; no atomics."""
@@ -1700,7 +1700,7 @@ def differential_backward(g: Tensor, q: Tensor, k: Tensor, lam: Tensor, lse: Ten
     src_ptr, records_s = tables.group_sources()
     (order, counts), (order_s, counts_s) = tables.target_rows(slots), tables.source_rows(slots)
     tables.found()
-    pairs = torch.empty(tables.n_targets, 2 * H, 2, dtype=tables.dtype, device=device)
+    rows = torch.empty(tables.n_targets, 2 * H, 3, dtype=tables.dtype, device=device)
     # the simple kernels' workspace
     ds = None if slots else torch.empty(tables.n_edges, 2 * H, dtype=tables.dtype, device=device)
     partial = torch.empty(int(library().gm_differential_partials(H)), dtype=torch.float64, device=device)
@@ -1708,6 +1708,6 @@ def differential_backward(g: Tensor, q: Tensor, k: Tensor, lam: Tensor, lse: Ten
     _call_on(device, "gm_differential_backward_" + _PW_SUFFIX[q.dtype], _ptr(g), _ptr(q), _ptr(k), _ptr(lam),
              _ptr(tables.records), _ptr(records_s), desc.data_ptr(), _ptr(tables.row_ptr), _ptr(src_ptr), _ptr(order),
              counts, _ptr(order_s), counts_s, tables.n_targets, tables.n_sources, tables.n_edges, q.shape[1],
-             tables.orders, desc.shape[0], H, scale, _ptr(lse), _ptr(pairs), _ptr(ds), _ptr(partial), _ptr(dq),
+             tables.orders, desc.shape[0], H, scale, _ptr(stats), _ptr(rows), _ptr(ds), _ptr(partial), _ptr(dq),
              _ptr(dk), _ptr(dlam), _stream(device))
     return dq, dk, dlam

@@ -18,8 +18,8 @@ with no edge inside has only zero weights (and zero gradients).
 
 The op reads an edge set through :class:`EdgeTables`, which its owner builds once
 and keeps.  On the GPU (``gm_differential_*``) neither the maps nor their
-gradients are written: the forward keeps one number a target and map for the
-backward.  bfloat16 rows take float32 tables, arithmetic and weights, and get
+gradients are written: the forward keeps two numbers a target and map for
+the backward.  bfloat16 rows take float32 tables, arithmetic and weights, and get
 bfloat16 gradients, rounded once.  CPU tensors take the formulas in torch.
 """
 
@@ -239,18 +239,18 @@ class DifferentialSoftmax(torch.autograd.Function):
             tables.group_sources()
             tables.source_rows(maps.slots(tables))
         with _native.span("gm::attention/differential_softmax"):
-            alpha, lse = _native.differential_forward(q, k, lam, tables, maps, scale, train)
+            alpha, stats = _native.differential_forward(q, k, lam, tables, maps, scale, train)
         if train:
-            ctx.save_for_backward(q, k, lam, lse)
+            ctx.save_for_backward(q, k, lam, stats)
             ctx.rest = (tables, maps, scale)
         return alpha
 
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx: Any, grad_alpha: Tensor) -> tuple:
-        q, k, lam, lse = ctx.saved_tensors
+        q, k, lam, stats = ctx.saved_tensors
         with _native.span("gm::attention/differential_softmax_backward"):
-            dq, dk, dlam = _native.differential_backward(grad_alpha.contiguous(), q, k, lam, lse, *ctx.rest)
+            dq, dk, dlam = _native.differential_backward(grad_alpha.contiguous(), q, k, lam, stats, *ctx.rest)
         return dq, dk, dlam, None, None, None, None
 
 

@@ -281,15 +281,16 @@ int gm_edge_tables_f64(const double* targets, const double* target_frames, const
  * records_s (n_edges, 2 + 2 orders) in the order of the edges sorted by source,
  * src_ptr its CSR: target, edge (integers), bias, 0, (cos, sin).  Nodes must lie
  * inside their tables (the kernels follow them).
- * lse (n_targets, 2 H), or NULL where no backward follows: the base-2 logarithm
- * of the sum of exponentials.  Backward from g = d alpha: dq, dk in the rows' type,
- * dlambda (H); pairs (n_targets, 2 H, 2), ds (n_edges, 2 H) and partial
+ * stats (n_targets, 2 H, 2), or NULL where no backward follows: a target's largest
+ * score m (over log 2) and 1 / sum 2^(s - m), zeros where no edge is inside.
+ * Backward from g = d alpha: dq, dk in the rows' type, dlambda (H); rows
+ * (n_targets, 2 H, 3), ds (n_edges, 2 H) and partial
  * (gm_differential_partials(H) doubles) are workspaces.  Sums in a fixed order.
  * order, or NULL: every target once, those of more than 128 S edges first, then
  * those of more than 32 S, then the rest, counts (HOST) how many of each, for the
  * S of gm_differential_slots; order_s and counts_s the same of the sources.  With
- * them (float and bfloat16 rows; rows and pairs at multiples of 16 bytes, records
- * of 8) the lane kernels run and ds is not used; without, kernels for any layout.
+ * them (float and bfloat16 rows; q, k, dq and dk at multiples of 16 bytes, records
+ * and stats of 8) the lane kernels run and ds is not used; without, kernels for any layout.
  * Suffix _bf16: bfloat16 rows, float tables and arithmetic.  No reference
  * counterpart (the single map's: gm_softmax_*). */
 int64_t gm_differential_partials(int64_t heads);
@@ -298,35 +299,35 @@ int gm_differential_slots(const int64_t* desc, int64_t F, int64_t H, int64_t D, 
 int gm_differential_forward_f32(const float* q, const float* k, const float* lambda, const float* records, const
                                 int64_t* desc, const int64_t* row_ptr, const int32_t* order, const int64_t* counts,
                                 int64_t n_targets, int64_t n_sources, int64_t n_edges, int64_t D, int64_t orders,
-                                int64_t F, int64_t H, double scale, float* alpha, float* lse, void* stream);
+                                int64_t F, int64_t H, double scale, float* alpha, float* stats, void* stream);
 int gm_differential_forward_f64(const double* q, const double* k, const double* lambda, const double* records, const
                                 int64_t* desc, const int64_t* row_ptr, const int32_t* order, const int64_t* counts,
                                 int64_t n_targets, int64_t n_sources, int64_t n_edges, int64_t D, int64_t orders,
-                                int64_t F, int64_t H, double scale, double* alpha, double* lse, void* stream);
+                                int64_t F, int64_t H, double scale, double* alpha, double* stats, void* stream);
 int gm_differential_forward_bf16(const uint16_t* q, const uint16_t* k, const float* lambda, const float* records,
                                  const int64_t* desc, const int64_t* row_ptr, const int32_t* order, const int64_t*
                                  counts, int64_t n_targets, int64_t n_sources, int64_t n_edges, int64_t D, int64_t
-                                 orders, int64_t F, int64_t H, double scale, float* alpha, float* lse, void* stream);
+                                 orders, int64_t F, int64_t H, double scale, float* alpha, float* stats, void* stream);
 int gm_differential_backward_f32(const float* g, const float* q, const float* k, const float* lambda, const float*
                                  records, const float* records_s, const int64_t* desc, const int64_t* row_ptr, const
                                  int64_t* src_ptr, const int32_t* order, const int64_t* counts, const int32_t*
                                  order_s, const int64_t* counts_s, int64_t n_targets, int64_t n_sources, int64_t
                                  n_edges, int64_t D, int64_t orders, int64_t F, int64_t H, double scale, const float*
-                                 lse, float* pairs, float* ds, double* partial, float* dq, float* dk, float* dlambda,
+                                 stats, float* rows, float* ds, double* partial, float* dq, float* dk, float* dlambda,
                                  void* stream);
 int gm_differential_backward_f64(const double* g, const double* q, const double* k, const double* lambda, const
                                  double* records, const double* records_s, const int64_t* desc, const int64_t*
                                  row_ptr, const int64_t* src_ptr, const int32_t* order, const int64_t* counts, const
                                  int32_t* order_s, const int64_t* counts_s, int64_t n_targets, int64_t n_sources,
                                  int64_t n_edges, int64_t D, int64_t orders, int64_t F, int64_t H, double scale, const
-                                 double* lse, double* pairs, double* ds, double* partial, double* dq, double* dk,
+                                 double* stats, double* rows, double* ds, double* partial, double* dq, double* dk,
                                  double* dlambda, void* stream);
 int gm_differential_backward_bf16(const float* g, const uint16_t* q, const uint16_t* k, const float* lambda, const
                                   float* records, const float* records_s, const int64_t* desc, const int64_t* row_ptr,
                                   const int64_t* src_ptr, const int32_t* order, const int64_t* counts, const int32_t*
                                   order_s, const int64_t* counts_s, int64_t n_targets, int64_t n_sources, int64_t
                                   n_edges, int64_t D, int64_t orders, int64_t F, int64_t H, double scale, const float*
-                                  lse, float* pairs, float* ds, double* partial, uint16_t* dq, uint16_t* dk, float*
+                                  stats, float* rows, float* ds, double* partial, uint16_t* dq, uint16_t* dk, float*
                                   dlambda, void* stream);
 
 /* ---------------- transformer block pointwise operators ----------------

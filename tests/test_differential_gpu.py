@@ -280,6 +280,74 @@ def test_biases_of_the_lowest_value_inside_the_window(cuda):
     assert all(bool(torch.isfinite(x).all()) for x in got.values())
 
 
+def bounds(graph, q, k, lam, g, copies, eps):
+    """What a row's gradient may be off by where its weights sum to one: (64 + degree) half steps of the weights and
+    as many of T, of a sum of a (|g| + T) |tau k| <= 2 max|g| sqrt(2) max|k|; a source's of its edges' sum."""
+    scale = sum(c * (1 if f == 0 else 2) for f, c in copies.items()) ** -0.5
+    degree = float((graph.row_ptr[1:] - graph.row_ptr[:-1]).max())
+    sources = float(torch.bincount(graph.source).max())
+    each = eps * scale * max(1.0, float(lam.abs().max())) * 2 * float(g.abs().max()) * 2 ** 0.5
+    return (64 + degree) * each * float(k.abs().max()), (64 + degree + sources) * each * float(q.abs().max()) * sources
+
+
+def assert_within(got, want, name, tol):
+    if got.dtype == torch.bfloat16:
+        tol = tol + torch.finfo(torch.bfloat16).eps / 2 * (want.abs() + tol)
+    off = (got.detach().double().cpu() - want).abs()
+    assert bool((off <= tol).all()), f"{name}: off by {float(off.max())}"
+
+
+BIASED = [({0: 2, 1: 2, 2: 2}, 8, torch.float32), ({0: 2, 1: 2, 2: 2}, 8, torch.bfloat16),
+          ({0: 4, 1: 4, 2: 4}, 4, torch.float32), ({0: 3, 1: 2}, 3, torch.float32), ({0: 3, 1: 2}, 3, torch.bfloat16),
+          ({0: 2, 1: 2, 2: 2}, 2, torch.float64)]
+DEGREES = [4, 1, 0, 7, 40, 140, 600]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("copies,heads,rows", BIASED)
+def test_gradients_of_rows_whose_biases_are_all_the_lowest_value(copies, heads, rows, cuda):
+    """Such a row's scores are all its bias, in any type: its weights are 1 / degree, forward and backward."""
+    table = tables_dtype(rows)
+    graph = scattered(DEGREES, 30, table, outside=0.0)
+    graph.inside[:] = 1
+    graph.bias[:] = torch.finfo(table).min
+    q, k, lam, g = inputs(graph, copies, heads, rows)
+    got = run(graph, graph.tables(table, cuda), q, k, lam, g, copies, heads, rows, cuda)
+    want = run(graph, graph.tables(torch.float64, "cpu"), q, k, lam, g, copies, heads, torch.float64, "cpu")
+    uniform = (1.0 / (graph.row_ptr[1:] - graph.row_ptr[:-1]).double())[graph.target]
+    torch.testing.assert_close(want["alpha"], uniform.unsqueeze(-1) * (1 - lam), rtol=1e-12, atol=1e-14)
+    eps = torch.finfo(table).eps
+    tol_q, tol_k = bounds(graph, q, k, lam, g, copies, eps)
+    assert_within(got["alpha"], want["alpha"], "alpha", 2 * (64 + max(DEGREES)) * eps * want["alpha"].abs() + eps)
+    assert_within(got["dq"], want["dq"], "dq", tol_q)
+    assert_within(got["dk"], want["dk"], "dk", tol_k)
+    assert_within(got["dlam"], want["dlam"], "dlam", len(DEGREES) * (64 + max(DEGREES)) * eps * float(g.abs().max()))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("exponent", [12, 20, 29])
+@pytest.mark.parametrize("copies,heads,rows", BIASED)
+def test_weights_of_the_backward_are_the_forwards_beside_large_biases(copies, heads, rows, exponent, cuda):
+    """A gradient that is the same for every edge meets weights that sum to one: nothing is left of it in the
+    rows, whatever the scores' own rounding beside biases of up to -2^29 (-2^60 in float64)."""
+    table = tables_dtype(rows)
+    graph = scattered(DEGREES, 30, table, outside=0.0)
+    graph.inside[:] = 1
+    graph.bias -= 2.0 ** (exponent if table == torch.float32 else 2 * exponent + 2)
+    graph.bias = graph.bias.to(table).double()
+    q, k, lam, g = inputs(graph, copies, heads, rows)
+    g = g[:1].expand_as(g)
+    got = run(graph, graph.tables(table, cuda), q, k, lam, g, copies, heads, rows, cuda)
+    eps = torch.finfo(table).eps
+    tol_q, tol_k = bounds(graph, q, k, lam, g, copies, eps)
+    assert_within(got["dq"], torch.zeros_like(q), "dq", tol_q)
+    assert_within(got["dk"], torch.zeros_like(k), "dk", tol_k)
+    filled = sum(d > 0 for d in DEGREES)
+    assert_within(got["dlam"], -filled * g[0], "dlam", filled * (64 + max(DEGREES)) * eps * float(g.abs().max()))
+    sums = torch.zeros(len(DEGREES), heads, dtype=torch.float64).index_add_(0, graph.target, got["alpha"].detach().double().cpu())
+    assert_within(sums, (torch.tensor(DEGREES) > 0).double().unsqueeze(-1) * (1 - lam), "sums", 2 * (64 + max(DEGREES)) * eps)
+
+
 @pytest.mark.gpu
 def test_sources_at_the_far_end_of_a_large_table(cuda):
     """Key rows whose offsets pass 2^31 numbers."""
