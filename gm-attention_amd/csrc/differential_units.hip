@@ -306,8 +306,8 @@ __global__ __launch_bounds__(1024) void differential_forward_units(DfArgs<float,
     return v;
   };
   // steps t and t + 1 of the edges from `e`: the lanes of a pair of maps exchange a weight and write an edge each
-  const int ahead = writes ? (second ? w.slots : 0) + s : INT32_MAX;
-  const uint32_t place = (uint32_t)(ahead * a.L.H + (p >> 1));
+  const int step = (second ? w.slots : 0) + s, ahead = writes ? step : INT32_MAX;
+  const uint32_t place = (uint32_t)(step * a.L.H + (p >> 1));
   auto write = [&](int64_t e, int t, float w0, float w1) {
     const float other = other_map(second ? w0 : w1, w.per_map);
     const float v = second ? other - lambda * w1 : w0 - lambda * other;
