@@ -669,63 +669,62 @@ __global__ __launch_bounds__(kRnThreads) void residual_norm_reduce_kernel(RnArgs
 
 // ------------------------------------------------------------------ launch
 
-// Units a lane holds at most: the rows' numbers and the backward's sums are registers (20 numbers of float and
-// bfloat16 rows, 16 of double ones; a wide row's copies, 32).
-template <typename X, bool kCopies>
-constexpr int kMaxUnits = kCopies ? 16 : (sizeof(X) == 8 ? 8 : 5);
+// Units a lane holds at most, the rows' numbers being registers: 20 numbers of float and bfloat16 rows in the forward,
+// 16 in the backward, whose lanes are more (dispatch_rn) and whose sums take as many registers again as its rows; 16 of
+// double rows, and of a wide row's copies 32.
+template <typename X, bool kCopies, bool kBackward>
+constexpr int kMaxUnits = kCopies ? 16 : (sizeof(X) == 8 ? 8 : (kBackward ? 4 : 5));
 
-template <typename X, typename U, bool kCopies, int NS>
-int launch_rn(bool backward, const RnArgs<X, U>& a, hipStream_t stream, int64_t& blocks) {
+template <typename X, typename U, bool kCopies, int NS, bool kBackward>
+int launch_rn(const RnArgs<X, U>& a, hipStream_t stream, int64_t& blocks) {
   using A = typename RnAcc<X>::type;
-  constexpr int kBack = kRnBackThreads<X, kCopies, NS>;
-  const int threads = backward ? kBack : kRnThreads;
-  const int64_t rows_per_block = (int64_t)(threads / kWave) * (kWave >> a.shift);
+  constexpr int kBlock = kBackward ? kRnBackThreads<X, kCopies, NS> : kRnThreads;
+  const int64_t rows_per_block = (int64_t)(kBlock / kWave) * (kWave >> a.shift);
   const int width = a.units * RnUnit<X, U, kCopies>::V;
-  const size_t lds = sizeof(A) * std::max<size_t>((size_t)kTables * a.D, backward ? width : 0);
-  const void* kernel = backward ? reinterpret_cast<const void*>(&residual_norm_backward_kernel<X, U, kCopies, NS>)
-                                : reinterpret_cast<const void*>(&residual_norm_forward_kernel<X, U, kCopies, NS>);
+  const size_t lds = sizeof(A) * std::max<size_t>((size_t)kTables * a.D, kBackward ? width : 0);
   const int64_t want = (a.n_rows + rows_per_block - 1) / rows_per_block;
-  // the backward writes a row of sums a workgroup: as many as the caller's array was sized for, and no more than the
-  // CUs hold at once
-  const int64_t slots = resident_blocks(kernel, threads, lds);
-  blocks = std::min<int64_t>(want, backward ? std::min<int64_t>(blocks, kBack == 512 ? 256 : 512)
-                                            : (slots > 0 ? slots : 1024));
-  if (backward)
-    hipLaunchKernelGGL((residual_norm_backward_kernel<X, U, kCopies, NS>), dim3((unsigned)blocks), dim3(kBack), lds,
+  if constexpr (kBackward) {
+    // a row of sums a workgroup: as many as the caller's array was sized for, eight waves a CU
+    blocks = std::min<int64_t>(want, std::min<int64_t>(blocks, kBlock == 512 ? 256 : 512));
+    hipLaunchKernelGGL((residual_norm_backward_kernel<X, U, kCopies, NS>), dim3((unsigned)blocks), dim3(kBlock), lds,
                        stream, a);
-  else
-    hipLaunchKernelGGL((residual_norm_forward_kernel<X, U, kCopies, NS>), dim3((unsigned)blocks), dim3(kRnThreads),
-                       lds, stream, a);
-  return check_launch(backward ? "residual_norm_backward" : "residual_norm_forward");
+  } else {
+    const int64_t slots = resident_blocks(
+        reinterpret_cast<const void*>(&residual_norm_forward_kernel<X, U, kCopies, NS>), kBlock, lds);
+    blocks = std::min<int64_t>(want, slots > 0 ? slots : 1024);
+    hipLaunchKernelGGL((residual_norm_forward_kernel<X, U, kCopies, NS>), dim3((unsigned)blocks), dim3(kBlock), lds,
+                       stream, a);
+  }
+  return check_launch(kBackward ? "residual_norm_backward" : "residual_norm_forward");
 }
 
-template <typename X, typename U, bool kCopies>
-int dispatch_rn(bool backward, RnArgs<X, U>& a, hipStream_t stream, int64_t& blocks) {
+template <bool kCopies, bool kBackward, typename X, typename U>
+int dispatch_rn(RnArgs<X, U>& a, hipStream_t stream, int64_t& blocks) {
   a.units = kCopies ? a.copies : a.D / RnUnit<X, U, kCopies>::V;
   a.scalar_units = kCopies ? a.a0 : a.a0 / RnUnit<X, U, kCopies>::V;
   a.lanes = 1;
   a.shift = 0;
-  // as few lanes a row as hold it within kMaxUnits a lane, or four copies (whose loads are a number each); the
-  // backward within three units, since its sums take as many registers again as its rows (float rows of five units a
-  // lane: 266 registers and one wave a SIMD, of three 180 and two); the widest rows take the whole wave
-  const int most = kCopies ? 4 : std::min(backward ? 3 : 5, kMaxUnits<X, kCopies>);
-  while (a.lanes < kWave && (a.units + a.lanes - 1) / a.lanes > most) {
+  constexpr int kMost = kMaxUnits<X, kCopies, kBackward>;
+  // as few lanes a row as hold it within kMost a lane, or four copies (whose loads are a number each); the backward
+  // within three units, since its sums take as many registers again as its rows (float rows of five units a lane: 266
+  // registers and one wave a SIMD, of three 180 and two); the widest rows take the whole wave
+  constexpr int kLane = kCopies ? 4 : (kBackward ? 3 : (kMost < 5 ? kMost : 5));
+  while (a.lanes < kWave && (a.units + a.lanes - 1) / a.lanes > kLane) {
     a.lanes *= 2;
     ++a.shift;
   }
   const int ns = (a.units + a.lanes - 1) / a.lanes;
-#define GM_RN_CASE(n)                                           \
-  if constexpr (n <= kMaxUnits<X, kCopies>) {                   \
-    if (ns <= n) return launch_rn<X, U, kCopies, n>(backward, a, stream, blocks); \
+#define GM_RN_CASE(n)                                                                        \
+  if constexpr (n <= kMost) {                                                                \
+    if (ns <= n) return launch_rn<X, U, kCopies, n, kBackward>(a, stream, blocks);           \
   }
   GM_RN_CASE(1)
   GM_RN_CASE(2)
   GM_RN_CASE(3)
+  GM_RN_CASE(4)
   if constexpr (!kCopies && sizeof(X) != 8) {
-    GM_RN_CASE(4)
     GM_RN_CASE(5)
   } else {
-    GM_RN_CASE(4)
     GM_RN_CASE(8)
     GM_RN_CASE(16)
   }
@@ -826,8 +825,8 @@ int residual_forward(const X* x, const U* u, const X* z, const void* const* para
   a.normed = normed;
   a.stats = stats;
   int64_t blocks = 0;
-  return whole_units(a) ? dispatch_rn<X, U, false>(false, a, (hipStream_t)stream, blocks)
-                        : dispatch_rn<X, U, true>(false, a, (hipStream_t)stream, blocks);
+  return whole_units(a) ? dispatch_rn<false, false>(a, (hipStream_t)stream, blocks)
+                        : dispatch_rn<true, false>(a, (hipStream_t)stream, blocks);
 }
 
 template <typename X, typename U>
@@ -861,7 +860,7 @@ int residual_backward(const X* dy, const X* dn, const X* x, const U* u, const X*
   const hipStream_t s = (hipStream_t)stream;
   if (n_rows > 0) {
     const int status =
-        units ? dispatch_rn<X, U, false>(true, a, s, blocks) : dispatch_rn<X, U, true>(true, a, s, blocks);
+        units ? dispatch_rn<false, true>(a, s, blocks) : dispatch_rn<true, true>(a, s, blocks);
     if (status != GM_OK) return status;
   }
   const dim3 grid((unsigned)((a.copies + kRnCols - 1) / kRnCols));
