@@ -21,7 +21,7 @@ int check_launch(const char* what);               // hipGetLastError after a lau
 // ---- launch geometry (runtime.hip) ----
 // Workgroups of `kernel` (`threads` threads, `lds` bytes of dynamic LDS)
 // resident on the current device at once, CUs x workgroups per CU; 0 when the
-// runtime cannot say (no device).  Cached per device and kernel.
+// runtime cannot say (no device).  Cached per device and arguments.
 int64_t resident_blocks(const void* kernel, int threads, size_t lds = 0);
 // The workgroups of a grid whose workgroups share the work evenly: about
 // `want`, in whole rounds of `slots` resident ones (r slots, r = want / slots

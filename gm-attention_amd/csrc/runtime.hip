@@ -4,7 +4,7 @@
 #include <map>
 #include <mutex>
 #include <string>
-#include <utility>
+#include <tuple>
 
 #include "common.hpp"
 #include "layout.hpp"
@@ -30,14 +30,14 @@ int check_launch(const char* what) {
 
 int64_t resident_blocks(const void* kernel, int threads, size_t lds) {
   static std::mutex mu;
-  static std::map<std::pair<int, const void*>, int64_t> cache;
+  static std::map<std::tuple<int, const void*, int, size_t>, int64_t> cache;
   int dev = -1;
   if (hipGetDevice(&dev) != hipSuccess) {
     (void)hipGetLastError();  // not left for the next launch check
     return 0;
   }
   std::lock_guard<std::mutex> lock(mu);
-  const auto key = std::make_pair(dev, kernel);
+  const auto key = std::make_tuple(dev, kernel, threads, lds);
   const auto it = cache.find(key);
   if (it != cache.end()) return it->second;
   int cus = 0, per = 0;

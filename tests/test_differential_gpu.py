@@ -283,6 +283,7 @@ def test_biases_of_the_lowest_value_inside_the_window(cuda):
 def bounds(graph, q, k, lam, g, copies, eps):
     """What a row's gradient may be off by where its weights sum to one: (64 + degree) half steps of the weights and
     as many of T, of a sum of a (|g| + T) |tau k| <= 2 max|g| sqrt(2) max|k|; a source's of its edges' sum."""
+    q, k, lam, g = (t.detach() for t in (q, k, lam, g))
     scale = sum(c * (1 if f == 0 else 2) for f, c in copies.items()) ** -0.5
     degree = float((graph.row_ptr[1:] - graph.row_ptr[:-1]).max())
     sources = float(torch.bincount(graph.source).max())
