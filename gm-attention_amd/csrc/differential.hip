@@ -14,9 +14,12 @@
 // Neither the maps nor ds are written: the forward keeps the maximum of s_p and its
 // weights' sum for every target, the backward forms a_p again from them.  The pass over the targets needs
 // no second walk for T either: sum ds tau k = scale c (sum a g tau k - T sum a tau k),
-// two sums beside T in one walk (each off by the roundings T itself has, times
-// sum a tau k).  The pass over the sources reads T and both numbers of its edges'
-// targets.  No atomics: sums are in a fixed order.
+// two sums beside T in one walk.  What a row's g share cancels in that difference and
+// leaves the roundings of both sums, where a second walk over a (g - T) would leave
+// T's: twice as far off for g = 10 + N(0, 1) over 120 edges (3.3e-6 against 1.7e-6 of
+// the result in float32), nothing without a common part (2.4e-7 against 2.1e-7).  The
+// pass over the sources reads T and both numbers of its edges' targets.  No atomics:
+// sums are in a fixed order.
 //
 // Per edge both passes read one record of 32-bit words (64-bit for double): the
 // other node, the bias (in units of log 2, as the scores here; -inf outside the

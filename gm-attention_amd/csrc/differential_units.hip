@@ -159,7 +159,7 @@ struct Unit {
     store_w<W1>(row + w.base[1] + unit * W1, v + W0);
     if constexpr (W2 > 0) store_w<W2>(row + w.base[2] + unit * W2, v + W0 + W1);
   }
-  // The three passes form a score by the same roundings, so that a row's ds sum to zero as nearly as its weights to one:
+  // The three passes form a weight by the same roundings, so that a row's ds sum to zero as nearly as its weights to one:
   // a key bias's gradient, zero but for rounding, is a third smaller than with the gathered row turned before the dot in
   // the backward's passes (which saves a fifth of their instructions and 1 % of their time).
   // Re< q, tau k >: per order cos sum (q0 k0 + q1 k1) + sin sum (q1 k0 - q0 k1)

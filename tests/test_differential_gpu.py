@@ -350,6 +350,23 @@ def test_weights_of_the_backward_are_the_forwards_beside_large_biases(copies, he
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("common", [0.0, 10.0, 1000.0])
+@pytest.mark.parametrize("copies,heads,rows", BIASED)
+def test_gradients_with_a_common_part(copies, heads, rows, common, cuda):
+    """What a smooth field's values give: the weights' gradients of a row nearly alike, and its keys too.  The
+    part they share cancels, and leaves the roundings it had (the oracle's bounds count |g| whole)."""
+    table = tables_dtype(rows)
+    graph = scattered(DEGREES, 30, table)
+    q, k, lam, g = inputs(graph, copies, heads, rows)
+    k = (k + common / 100).to(rows).double()
+    g = (g + common).to(table).double()
+    got = run(graph, graph.tables(table, cuda), q, k, lam, g, copies, heads, rows, cuda)
+    want = oracle(graph, q, k, lam, g, copies, heads, torch.finfo(table).eps)
+    for name in want:
+        compare(got[name], want[name], name)
+
+
+@pytest.mark.gpu
 def test_sources_at_the_far_end_of_a_large_table(cuda):
     """Key rows whose offsets pass 2^31 numbers."""
     copies, heads, n = {0: 2, 1: 2, 2: 2}, 8, 13_600_000  # 160 numbers a row: 2.2e9
