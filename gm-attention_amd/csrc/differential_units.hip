@@ -4,15 +4,18 @@
 // so that the lanes of an edge read its row as whole cache lines.  A wave's 64 lanes
 // are (edge slot, unit), units rounded up to a power of two.
 //
-// Measured on 256x512, B = 4 (79 million edges of 640 bytes): the forward 3.05 ms, the
-// passes of the backward 2.8 (targets) and 3.3 (sources); 31 bytes a cycle of a CU
-// arrive from the L1, where contiguous loads reach 50.  No one unit bounds them.  The
-// forward's load path is busy for 97 % of the time and its vector ALUs for 51 %, yet
-// timing copies of it without the dot products take 1 % less, without the rows' loads 27 %
-// less, without the records' reads from LDS nothing less, and with every source among
-// 16 rows, all in the L1, 7 % less: what remains is the waves' latency, four of them a
-// SIMD by their registers and the LDS of their scores (the backward, without scores,
-// has five).  Fewer, wider loads did not help: a lane for both of a head's maps, five
+// Measured on 256x512, B = 4 (63 million edges, 40 GB of rows a pass): the forward 3.11
+// ms, the passes of the backward 2.86 (targets) and 3.51 (sources).  The targets' is bound
+// by its vector ALUs, busy for 91 % of the time; the sources' (62 %) and the forward (50 %
+// of the time of the rows of one and four waves, 44 % of those of sixteen) by no one unit.
+// The forward's rows arrive from the L1 at 23 to 24 bytes a cycle of a CU, half of the 50
+// that contiguous loads reach, with the load path busy for 98 and 79 %; timing copies of it
+// without the dot products take 1 % less, without the rows' loads 27 % less, without the
+// records' reads from LDS nothing less, and with every source among 16 rows, all in the
+// L1, 7 % less: what remains is the waves' latency, four of them a SIMD by their registers
+// and the LDS of their scores (the backward, without scores, has five).  Source rows that
+// neighbouring targets share are loaded for each of them: that is what would take fewer
+// loads.  Fewer, wider loads did not help: a lane for both of a head's maps, five
 // loads of 16 bytes for two units in place of six, took 3.1, 4.0 and 3.9 ms for the
 // registers it needs; the two maps' lanes reading the pieces of up to 8 bytes together,
 // each for one of two steps, 3.06, 3.0 and 3.2, and 9 % more with bfloat16 rows.

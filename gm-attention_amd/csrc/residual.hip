@@ -22,7 +22,8 @@
 //
 // One pass over the data each way, so the bytes bound it: 524,288 rows of 160 in
 // float with gates take 301 us forward (5.1 TB/s) and 511 backward (4.75), 262,144
-// bfloat16 rows with a float branch 95 and 213.  A row's units (16
+// bfloat16 rows with a float branch 95 and 213 (the latter at 3.6 TB/s: its registers
+// leave two waves a SIMD).  A row's units (16
 // bytes of float or double, 8 of bfloat16, or one copy where a multiplicity, a
 // pointer or the gates' rows are not whole units) are shared by 2^k lanes with at most
 // kMaxUnits<...> units a lane, all in registers; the norms' sums are shuffles

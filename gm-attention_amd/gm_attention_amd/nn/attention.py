@@ -205,8 +205,11 @@ class SO2MHSA(nn.Module):
 
     def lambdas(self) -> Tensor:
         """A differential layer's factors ``(n_heads,)`` of the second maps:
-        ``exp <q_1, k_1> - exp <q_2, k_2> + lambda_init`` of learned vectors a head
-        (the differential transformer's parametrisation, arXiv 2410.05258)."""
+        ``exp <q_1, k_1> - exp <q_2, k_2> + lambda_init`` of learned vectors.  The
+        form is the differential transformer's (arXiv 2410.05258), the layer is not:
+        there the heads share one pair of vectors, and each head's output is
+        normalised and multiplied by ``1 - lambda_init``; here every head has its
+        own, and nothing makes up for weights that sum to ``1 - lambda``."""
         first, second = (self.lambda_query * self.lambda_key).sum(-1).exp().unbind(0)
         return first - second + self.lambda_init
 

@@ -16,8 +16,9 @@ branch's norm, the gate, the scale and the next norm may be left out.
 On the GPU the sum and both norms are one HIP pass each way over flat rows
 (``gm_residual_norm_*``; parameter gradients reduced in a fixed order) for
 float32, float64 and bfloat16 rows; bfloat16 rows keep float32 parameters and
-arithmetic, take a branch in bfloat16 or float32, and are rounded once: ``h`` is
-normalised from the sum before its rounding.  CPU tensors take the same
+arithmetic, take a branch in bfloat16 or float32 (the gates' pre-activations in
+the rows' type), and are rounded once: ``h`` is normalised from the sum before
+its rounding.  CPU tensors take the same
 formulas in torch.
 """
 
