@@ -1676,8 +1676,9 @@ def differential_slots(desc: Tensor, D: int, orders: int, H: int) -> int:
 def differential_forward(q: Tensor, k: Tensor, lam: Tensor, tables: Any, maps: Any, scale: float,
                          train: bool) -> tuple[Tensor, Tensor | None]:
     """``(alpha (n_edges, H), stats)``: the differential softmax's weights and, under ``train``, what its
-    backward reads of a target's maps ``(n_targets, 2 H, 2)``, the largest score and one over the weights' sum.  The rows are whole
-    (contiguous, at multiples of 16 bytes) and match the tables: nn.differential's checks."""
+    backward reads of a target's maps ``(n_targets, 2 H, 2)``, the largest score and one over the weights'
+    sum.  The rows are whole (contiguous, at multiples of 16 bytes) and match the tables: nn.differential's
+    checks."""
     H, desc, device = maps.heads, maps.desc, q.device
     order, counts = tables.target_rows(maps.slots(tables))
     tables.found()
