@@ -56,13 +56,13 @@ __device__ T generic_map_score(const DfArgs<T, R>& a, const R* qi, const R* kj, 
     const int n = a.L.n[f], an = a.L.a[f];
     if (n == 0) {
       const int at = a.L.off[f] + p * an;
-      for (int u = 0; u < an; ++u) acc += df_widen(qi[at + u]) * df_widen(kj[at + u]);
+      for (int u = 0; u < an; ++u) acc += row_widen(qi[at + u]) * row_widen(kj[at + u]);
     } else {
       const int at = a.L.off[f] + 2 * p * an;
       T re = T(0), im = T(0);
       for (int u = 0; u < an; ++u) {
-        const T q0 = df_widen(qi[at + 2 * u]), q1 = df_widen(qi[at + 2 * u + 1]);
-        const T k0 = df_widen(kj[at + 2 * u]), k1 = df_widen(kj[at + 2 * u + 1]);
+        const T q0 = row_widen(qi[at + 2 * u]), q1 = row_widen(qi[at + 2 * u + 1]);
+        const T k0 = row_widen(kj[at + 2 * u]), k1 = row_widen(kj[at + 2 * u + 1]);
         re += q0 * k0 + q1 * k1;
         im += q1 * k0 - q0 * k1;
       }
@@ -112,7 +112,7 @@ __global__ __launch_bounds__(256) void differential_forward_generic(DfArgs<T, R>
   if (s < S)
     for (int64_t e = e0 + s; e < e1; e += S) {
       const T lw = generic_logit(a, qi, e, p);
-      if (lw != neg_inf<T>()) l += df_exp2(lw - m);
+      if (lw != neg_inf<T>()) l += row_exp2(lw - m);
     }
   l = group_sum(l, lane, P, S);
   const T inv = l == T(0) ? T(0) : T(1) / l;
@@ -126,7 +126,7 @@ __global__ __launch_bounds__(256) void differential_forward_generic(DfArgs<T, R>
     T w = T(0);
     if (live) {
       const T lw = generic_logit(a, qi, e + s, p);
-      if (lw != neg_inf<T>()) w = df_exp2(lw - m) * inv;
+      if (lw != neg_inf<T>()) w = row_exp2(lw - m) * inv;
     }
     const T other = __shfl(w, lane | 1, kWave);
     if (live && (p & 1) == 0) a.alpha[(e + s) * a.L.H + (p >> 1)] = w - lambda * other;
@@ -147,7 +147,7 @@ __global__ __launch_bounds__(256) void differential_backward_scores_generic(DfAr
   if (s < S)
     for (int64_t e = e0 + s; e < e1; e += S) {
       const T lw = generic_logit(a, qi, e, p);
-      const T w = lw == neg_inf<T>() ? T(0) : df_exp2(lw - m) * inv;
+      const T w = lw == neg_inf<T>() ? T(0) : row_exp2(lw - m) * inv;
       if (lw != neg_inf<T>()) total += w * a.g[e * a.L.H + (p >> 1)];
       a.ds[e * P + p] = w;
     }
@@ -196,15 +196,15 @@ __global__ __launch_bounds__(256) void differential_backward_target_generic(DfAr
         const T ds = a.ds[e * a.L.P + col.p];
         const R* kj = a.k + node_of(rec) * a.L.D;
         if (col.n == 0) {
-          acc += ds * df_widen(kj[c]);
+          acc += ds * row_widen(kj[c]);
         } else {
           const T cr = rec[2 * col.n], ci = rec[2 * col.n + 1];
-          const T k0 = df_widen(kj[col.pair]), k1 = df_widen(kj[col.pair + 1]);
+          const T k0 = row_widen(kj[col.pair]), k1 = row_widen(kj[col.pair + 1]);
           acc += ds * (col.part == 0 ? cr * k0 - ci * k1 : cr * k1 + ci * k0);
         }
       }
     }
-    df_narrow(acc, a.dq[i * a.L.D + c]);
+    row_narrow(acc, a.dq[i * a.L.D + c]);
   }
 }
 
@@ -224,15 +224,15 @@ __global__ __launch_bounds__(256) void differential_backward_source_generic(DfAr
         const T ds = a.ds[node_of(rec + 1) * a.L.P + col.p];
         const R* qi = a.q + node_of(rec) * a.L.D;
         if (col.n == 0) {
-          acc += ds * df_widen(qi[c]);
+          acc += ds * row_widen(qi[c]);
         } else {
           const T cr = rec[2 * col.n + 2], ci = rec[2 * col.n + 3];
-          const T q0 = df_widen(qi[col.pair]), q1 = df_widen(qi[col.pair + 1]);
+          const T q0 = row_widen(qi[col.pair]), q1 = row_widen(qi[col.pair + 1]);
           acc += ds * (col.part == 0 ? cr * q0 + ci * q1 : cr * q1 - ci * q0);
         }
       }
     }
-    df_narrow(acc, a.dk[j * a.L.D + c]);
+    row_narrow(acc, a.dk[j * a.L.D + c]);
   }
 }
 

@@ -5,6 +5,7 @@
 #include <cstdint>
 
 #include "common.hpp"
+#include "edge_units.hpp"
 
 namespace gm {
 
@@ -50,17 +51,6 @@ struct DfArgs {
 // as in the forward.  (m + log2 of the sum as one number is as wrong as that number's spacing: beside a bias of -1e9 by
 // more than the sum itself, and the backward's weights were not the forward's.)
 constexpr double kLog2e = 1.4426950408889634074;
-
-__device__ __forceinline__ float df_exp2(float x) { return exp2f(x); }
-__device__ __forceinline__ double df_exp2(double x) { return exp2(x); }
-__device__ __forceinline__ float df_widen(float x) { return x; }
-__device__ __forceinline__ double df_widen(double x) { return x; }
-__device__ __forceinline__ float df_widen(uint16_t x) { return __uint_as_float((uint32_t)x << 16); }
-__device__ __forceinline__ void df_narrow(float v, float& o) { o = v; }
-__device__ __forceinline__ void df_narrow(double v, double& o) { o = v; }
-__device__ __forceinline__ void df_narrow(float v, uint16_t& o) {  // to nearest even
-  o = __builtin_bit_cast(uint16_t, static_cast<__bf16>(v));
-}
 
 // The lane kernels (differential_units.hip): a map's copies as `per_map` units of (A0, A1, A2) copies, one lane a unit.
 enum class DfPass { Forward, BackwardTarget, BackwardSource };

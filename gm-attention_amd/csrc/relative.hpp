@@ -1,0 +1,81 @@
+// What the kernels of the softmax with a learned relative bias share: the heads' layout, the arguments.
+#pragma once
+#include <hip/hip_runtime.h>
+
+#include <cstdint>
+
+#include "common.hpp"
+#include "edge_units.hpp"
+
+namespace gm {
+
+constexpr int kRelMaxFreq = GM_ATTN_MAX_F;
+constexpr int kRelMaxBuckets = 256;  // a float record's word holds a bucket above its source's 24 bits
+
+// The H heads in the rows: frequency f's order n, copies a a head, flat offset.
+struct RelLayout {
+  int F, H, D, orders;
+  int n[kRelMaxFreq], a[kRelMaxFreq], off[kRelMaxFreq];
+};
+
+// The rows (targets, or sources) as the lane kernels take them: `order` lists them in three classes, those of 16 waves
+// each, of four, of one; (count of each).
+struct RelRows {
+  const int32_t* order;
+  int64_t count[3];
+};
+
+// T: the arithmetic's type; rows of T, or of bfloat16 (uint16_t) with T = float.
+template <typename T, typename R>
+struct RelArgs {
+  RelLayout L;
+  int buckets;
+  const R* q;
+  const R* k;
+  const T* table;          // (buckets, H)
+  const T* records;        // (n_edges, 2 orders): source and bucket, bias / log 2, (cos, sin) of orders 1 ..
+  const T* records_s;      // (n_edges, 2 orders): target, edge, (cos, sin) of orders 1 ..; sorted by source
+  const int64_t* row_ptr;  // over targets
+  const int64_t* src_ptr;  // over sources
+  const T* g;              // (n_edges, H)
+  T* alpha;                // (n_edges, H); read by the backward
+  T* ds;                   // (n_edges, H): the backward's workspace
+  T* partial;              // (gm_relative_partial_rows, buckets, H): sums of ds
+  R* dq;
+  R* dk;
+  int64_t n_targets, n_sources, n_edges;
+  T scale;           // of the scores, in units of log 2
+  T gradient_scale;  // of the scores
+};
+
+// Scores, their biases and their maxima are in units of log 2.
+constexpr double kRelLog2e = 1.4426950408889634074;
+
+// A record's first word: the source below, the bucket above.
+__device__ __forceinline__ int rel_source(const float* word) { return *reinterpret_cast<const int*>(word) & 0xFFFFFF; }
+__device__ __forceinline__ int rel_bucket(const float* word) { return *reinterpret_cast<const uint32_t*>(word) >> 24; }
+__device__ __forceinline__ int rel_source(const double* word) {
+  return (int)(*reinterpret_cast<const int64_t*>(word) & 0xFFFFFFFF);
+}
+__device__ __forceinline__ int rel_bucket(const double* word) {
+  return (int)(*reinterpret_cast<const int64_t*>(word) >> 32);
+}
+// A node or an edge in a word of its own.
+__device__ __forceinline__ int rel_index(const float* word) { return *reinterpret_cast<const int*>(word); }
+__device__ __forceinline__ int rel_index(const double* word) {
+  return (int)*reinterpret_cast<const int64_t*>(word);
+}
+
+constexpr int kRelTableRows = 1024;  // rows of sums of ds by bucket that the backward adds
+
+// The lane kernels (relative_units.hip).
+enum class RelPass { Forward, BackwardTarget, BackwardSource };
+
+// The edge slots of a wave (64 over the units rounded up to a power of two), or 0 where the lane kernels do not serve
+// the layout.
+int rel_slots(const RelLayout& L);
+
+int rel_launch_units(RelPass pass, const RelArgs<float, float>& a, const RelRows& rows, hipStream_t stream);
+int rel_launch_units(RelPass pass, const RelArgs<float, uint16_t>& a, const RelRows& rows, hipStream_t stream);
+
+}  // namespace gm

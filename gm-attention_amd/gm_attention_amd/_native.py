@@ -119,6 +119,12 @@ SIGNATURES_F32 = {
        for sfx in ("f32", "f64", "bf16")},
     **{f"gm_differential_backward_{sfx}": (ctypes.c_int, [_P] * 13 + [_I] * 7 + [_D] + [_P] * 8)
        for sfx in ("f32", "f64", "bf16")},
+    "gm_relative_partial_rows": (ctypes.c_int64, []),
+    "gm_relative_slots": (ctypes.c_int, [_P] + [_I] * 4 + [_P]),
+    **{f"gm_relative_forward_{sfx}": (ctypes.c_int, [_P] * 8 + [_I] * 8 + [_D] + [_P] * 2)
+       for sfx in ("f32", "f64", "bf16")},
+    **{f"gm_relative_backward_{sfx}": (ctypes.c_int, [_P] * 13 + [_I] * 8 + [_D] + [_P] * 6)
+       for sfx in ("f32", "f64", "bf16")},
     "gm_residual_norm_partial_rows": (ctypes.c_int64, [_I]),
     **{f"gm_residual_norm_forward_{sfx}": (ctypes.c_int, [_P] * 4 + [_I] * 4 + [_P, _P, _D, _D, _D] + [_P] * 4)
        for sfx in ("f32", "f64", "bf16", "bf16_f32")},
@@ -1712,3 +1718,50 @@ def differential_backward(g: Tensor, q: Tensor, k: Tensor, lam: Tensor, stats: T
              tables.orders, desc.shape[0], H, scale, _ptr(stats), _ptr(rows), _ptr(ds), _ptr(partial), _ptr(dq),
              _ptr(dk), _ptr(dlam), _stream(device))
     return dq, dk, dlam
+
+
+# ---------------------------------------------------------------- softmax with a learned relative bias
+
+
+def relative_slots(desc: Tensor, D: int, orders: int, H: int) -> int:
+    """The edge slots of a wave of the lane kernels, 0 where they do not serve the layout."""
+    slots = ctypes.c_int64(0)
+    _call("gm_relative_slots", desc.data_ptr(), desc.shape[0], H, D, orders, ctypes.addressof(slots))
+    return int(slots.value)
+
+
+def relative_forward(q: Tensor, k: Tensor, table: Tensor, tables: Any, heads: Any, scale: float) -> Tensor:
+    """``alpha (n_edges, H)``: the weights under the learned bias ``table (n_buckets, H)``.  The rows are whole
+    (contiguous, at multiples of 16 bytes) and match the tables: nn.relative's checks."""
+    H, desc, device = heads.heads, heads.desc, q.device
+    order, counts = tables.target_rows(heads.slots(tables))
+    tables.found()
+    alpha = torch.empty(tables.n_edges, H, dtype=tables.dtype, device=device)
+    _call_on(device, "gm_relative_forward_" + _PW_SUFFIX[q.dtype], _ptr(q), _ptr(k), _ptr(table),
+             _ptr(tables.records), desc.data_ptr(), _ptr(tables.row_ptr), _ptr(order), counts, tables.n_targets,
+             tables.n_sources, tables.n_edges, q.shape[1], tables.orders, desc.shape[0], H, tables.n_buckets, scale,
+             _ptr(alpha), _stream(device))
+    return alpha
+
+
+def relative_backward(g: Tensor, alpha: Tensor, q: Tensor, k: Tensor, tables: Any, heads: Any,
+                      scale: float) -> tuple[Tensor, Tensor, Tensor]:
+    """``(dq, dk, dtable)`` of what a forward took and gave and the weights' gradient (contiguous): the rows'
+    gradients in their dtype, the learned table's in the tables'; sums in a fixed order."""
+    H, desc, slots, device = heads.heads, heads.desc, heads.slots(tables), q.device
+    if g.dtype != tables.dtype or g.shape != (tables.n_edges, H) or not g.is_contiguous() or g.device != device:
+        raise RuntimeError("g must be contiguous (n_edges, H) in the tables' dtype")
+    src_ptr, records_s = tables.group_sources()
+    (order, counts), (order_s, counts_s) = tables.target_rows(slots), tables.source_rows(slots)
+    tables.found()
+    ds = torch.empty_like(g)
+    partial = torch.empty(int(library().gm_relative_partial_rows()) * tables.n_buckets * H, dtype=g.dtype,
+                          device=device)
+    dq, dk = torch.empty_like(q), torch.empty_like(k)
+    dtable = torch.empty(tables.n_buckets, H, dtype=g.dtype, device=device)
+    _call_on(device, "gm_relative_backward_" + _PW_SUFFIX[q.dtype], _ptr(g), _ptr(alpha), _ptr(q), _ptr(k),
+             _ptr(tables.records), _ptr(records_s), desc.data_ptr(), _ptr(tables.row_ptr), _ptr(src_ptr), _ptr(order),
+             counts, _ptr(order_s), counts_s, tables.n_targets, tables.n_sources, tables.n_edges, q.shape[1],
+             tables.orders, desc.shape[0], H, tables.n_buckets, scale, _ptr(ds), _ptr(partial), _ptr(dq), _ptr(dk),
+             _ptr(dtable), _stream(device))
+    return dq, dk, dtable

@@ -29,7 +29,8 @@ import ctypes
 import functools
 import math
 from collections import OrderedDict
-from typing import Any
+from collections.abc import Callable
+from typing import Any, NamedTuple
 
 import numpy as np
 import torch
@@ -94,7 +95,7 @@ class EdgeTables:
             return
         records = torch.empty(self.n_edges, 2 * self.orders, dtype=self.dtype, device=self.device)
         words = records.view(_WORD[self.dtype])
-        words[:, 0] = source
+        words[:, 0] = self._packed(source)
         # in units of log 2; the type's lowest value stays a finite one
         lowest = torch.finfo(self.dtype).min
         records[:, 1] = torch.where(masked == -math.inf, masked, (masked * _LOG2E).clamp_min(lowest))
@@ -117,7 +118,15 @@ class EdgeTables:
             self._hold(*(self.__dict__.pop(n) for n in ("_source", "_phases", "_bias")))
         elif "records" in state:
             records = self.__dict__.pop("records")
-            self._hold(records.view(_WORD[self.dtype])[:, 0].long(), records[:, 2:], records[:, 1] / _LOG2E)
+            self._hold(self._unpacked(records), records[:, 2:], records[:, 1] / _LOG2E)
+
+    def _packed(self, source: Tensor) -> Tensor:
+        """The records' first words."""
+        return source
+
+    def _unpacked(self, records: Tensor) -> Tensor:
+        """The sources in the records."""
+        return records.view(_WORD[self.dtype])[:, 0].long()
 
     def group_sources(self) -> tuple[Tensor, Tensor]:
         """``(src_ptr, records_s)``: the edges sorted by source, each with its target,
@@ -131,21 +140,24 @@ class EdgeTables:
     def _group(self) -> tuple[Tensor, Tensor]:
         _outside_capture(self.row_ptr, "EdgeTables.group_sources")
         self.found()
-        sorted_source, order = torch.sort(self.records.view(_WORD[self.dtype])[:, 0].to(torch.int32), stable=True)
+        sorted_source, order = torch.sort(self._unpacked(self.records).to(torch.int32), stable=True)
         bounds = torch.arange(self.n_sources + 1, dtype=torch.int32, device=self.device)
         src_ptr = torch.searchsorted(sorted_source, bounds)
         target = torch.repeat_interleave(torch.arange(self.n_targets, device=self.device),
                                          self.row_ptr[1:] - self.row_ptr[:-1], output_size=self.n_edges)
-        records_s = torch.empty(self.n_edges, 2 + 2 * self.orders, dtype=self.dtype, device=self.device)
-        words = records_s.view(_WORD[self.dtype])
-        words[:, 0] = target.index_select(0, order)
-        words[:, 1] = order
-        words[:, 3] = 0
-        mine = self.records.index_select(0, order)
-        records_s[:, 2] = mine[:, 1]
-        records_s[:, 4:] = mine[:, 2:]
+        records_s = self._source_records(target.index_select(0, order), order, self.records.index_select(0, order))
         self._kept.append(_native.Made(src_ptr, records_s))
         return src_ptr, records_s
+
+    def _source_records(self, target: Tensor, edge: Tensor, records: Tensor) -> Tensor:
+        records_s = torch.empty(self.n_edges, 2 + 2 * self.orders, dtype=self.dtype, device=self.device)
+        words = records_s.view(_WORD[self.dtype])
+        words[:, 0] = target
+        words[:, 1] = edge
+        words[:, 3] = 0
+        records_s[:, 2] = records[:, 1]
+        records_s[:, 4:] = records[:, 2:]
+        return records_s
 
     def target_rows(self, slots: int) -> tuple[Tensor | None, Any]:
         """The targets in the classes of degree that the lane kernels with ``slots``
@@ -293,17 +305,32 @@ def enabled(mhsa: Any, x: Any, edges: Any) -> bool:
             and maps.max_frequency <= edges.max_frequency)
 
 
-def edge_tables(edges: Any, cutoff: float, window: str, dtype: torch.dtype, top: int) -> EdgeTables:
+class _Kind(NamedTuple):
+    """Which tables of an edge set: their name among what is kept of its geometry, and how
+    they are made of a geometry and the CSR ``(row_ptr, source)`` over ``n_sources`` rows."""
+
+    name: tuple
+    make: Callable[..., EdgeTables]
+
+
+def _kind(top: int) -> _Kind:
+    return _Kind((top,), lambda g, row_ptr, source, n_sources: EdgeTables(
+        row_ptr, source, g.transport[:, : top + 1], g.bias, g.inside, n_sources=n_sources))
+
+
+def edge_tables(edges: Any, cutoff: float, window: str, dtype: torch.dtype, top: int,
+                kind: _Kind | None = None) -> EdgeTables:
     """The tables of ``edges`` under a cutoff and window, with the transport's orders
     up to ``top``: built once and kept with the edge set's geometry."""
+    kind = _kind(top) if kind is None else kind
     g = fused_attention.geometry(edges, cutoff, window, dtype)
-    held = g.derived.get(("differential", top))
+    key = ("differential", *kind.name)
+    held = g.derived.get(key)
     if held is None:
         with _native.LOCK:
-            held = g.derived.get(("differential", top))
+            held = g.derived.get(key)
             if held is None:
-                held = g.derived["differential", top] = EdgeTables(g.row_ptr, g.source, g.transport[:, : top + 1],
-                                                                   g.bias, g.inside)
+                held = g.derived[key] = kind.make(g, g.row_ptr, g.source, None)
     return held
 
 
@@ -340,19 +367,20 @@ class _Ranges:
             return made
 
 
-def chunk_tables(chunk: Any, cutoff: float, window: str, dtype: torch.dtype,
-                 top: int) -> tuple[EdgeTables, int, int]:
+def chunk_tables(chunk: Any, cutoff: float, window: str, dtype: torch.dtype, top: int,
+                 kind: _Kind | None = None) -> tuple[EdgeTables, int, int]:
     """The tables of a chunk (``EdgeGeometry.chunks``) over its own targets and the range of
     nodes its sources lie in, and the first of each.  Chunks are made anew for every pass:
     the tables are kept with the edge set they are ranges of, as many as two passes over all
     of its edges take, where a range's lists of nodes take no more than its edges (a chunk
     with sources all over a large set keeps its own)."""
+    kind = _kind(top) if kind is None else kind
     parent, e0, e1 = fused_attention.chunk_of(chunk)
     outer = fused_attention.geometry(parent, cutoff, window, dtype)
-    ranges = outer.derived.get(("differential ranges", top))
+    ranges = outer.derived.get(("differential ranges", *kind.name))
     if ranges is None:
         with _native.LOCK:
-            ranges = outer.derived.setdefault(("differential ranges", top), _Ranges(2 * int(parent.n_edges)))
+            ranges = outer.derived.setdefault(("differential ranges", *kind.name), _Ranges(2 * int(parent.n_edges)))
     # an edge set registered as a chunk under numbers of its own is not the range of its span
     same = (chunk.edge_index.data_ptr() == parent.edge_index[:, e0:].data_ptr()
             and chunk.row_ptr.shape == parent.row_ptr.shape)
@@ -360,7 +388,7 @@ def chunk_tables(chunk: Any, cutoff: float, window: str, dtype: torch.dtype,
     if found is not None:
         return found
     g = fused_attention.geometry(chunk, cutoff, window, dtype)
-    found = g.derived.get(("differential range", top))
+    found = g.derived.get(("differential range", *kind.name))
     if found is not None:
         return found
     _outside_capture(g.row_ptr, "EdgeTables")
@@ -368,13 +396,12 @@ def chunk_tables(chunk: Any, cutoff: float, window: str, dtype: torch.dtype,
     first = int(np.searchsorted(ptr, begin, side="right")) - 1
     last = int(np.searchsorted(ptr, begin + e1 - e0, side="left"))
     source, behind = int(g.source.min()), int(g.source.max()) + 1
-    made = EdgeTables(g.row_ptr[first:last + 1], g.source - source, g.transport[:, : top + 1], g.bias, g.inside,
-                      n_sources=behind - source), first, source
+    made = kind.make(g, g.row_ptr[first:last + 1], g.source - source, behind - source), first, source
     # 12 bytes a node of either list, 24 and 32 an edge at two orders
     if same and made[0].n_targets + made[0].n_sources <= 4 * (e1 - e0):
         return ranges.keep((e0, e1), made)
     with _native.LOCK:
-        return g.derived.setdefault(("differential range", top), made)
+        return g.derived.setdefault(("differential range", *kind.name), made)
 
 
 def attention_weights(mhsa: Any, q: Tensor, k: Tensor, edges: Any) -> Tensor:

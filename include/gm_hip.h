@@ -330,6 +330,65 @@ int gm_differential_backward_bf16(const float* g, const uint16_t* q, const uint1
                                   stats, float* rows, float* ds, double* partial, uint16_t* dq, uint16_t* dk, float*
                                   dlambda, void* stream);
 
+/* ---------------- softmax with a learned relative bias ----------------
+ *
+ * Per edge e = (i <- j) of bucket b(e) and head h
+ *   s_h = scale sum_n Re< q_i,n,h , tau_n(e) k_j,n,h > + bias(e) + table[b(e), h]
+ *   alpha (n_edges, H) = softmax of s_h over i's edges inside the window, zero outside
+ * and from g = d alpha: dq, dk in the rows' type, dtable (buckets, H), the sums of
+ * ds = alpha (g - sum alpha g) over each bucket's edges.  q (n_targets, D) and k
+ * (n_sources, D) hold H heads in desc's layout (frequencies rising, rows of copies
+ * following each other, D filled).  An edge of weight zero adds nothing to any
+ * gradient, whatever its rows and g hold.
+ *   records (n_edges, 2 orders): one word (32 bits; 64 for double) of the source
+ *     with the bucket above its 24 (32) bits, the bias / log 2 (-inf outside the
+ *     window), then (cos, sin) of the orders 1 .. ; float: n_sources <= 2^24
+ *   records_s (n_edges, 2 orders): the edges sorted by source (src_ptr): a word of
+ *     the target, a word of the edge, (cos, sin) of the orders 1 ..
+ *   1 <= buckets <= 256; indices are followed unchecked.
+ * ds (n_edges, H) and partial (gm_relative_partial_rows() rows of buckets H) are
+ * workspaces.  Sums in a fixed order.
+ * order, or NULL: every target once, those of more than 128 S edges first, then
+ * those of more than 32 S, then the rest, counts (HOST) how many of each, for the
+ * S of gm_relative_slots; order_s and counts_s the same of the sources.  With
+ * them (float and bfloat16 rows; q, k, dq and dk at multiples of 16 bytes, records
+ * of 8) the lane kernels run; without, kernels for any layout.
+ * Suffix _bf16: bfloat16 rows, float tables and arithmetic.  No reference
+ * counterpart (the softmax without the learned bias: gm_softmax_*). */
+int64_t gm_relative_partial_rows(void);
+/* *slots (HOST): the edges a wave of the lane kernels takes at once, S, or 0 where they do not serve the layout. */
+int gm_relative_slots(const int64_t* desc, int64_t F, int64_t H, int64_t D, int64_t orders, int64_t* slots);
+int gm_relative_forward_f32(const float* q, const float* k, const float* table, const float* records, const int64_t*
+                            desc, const int64_t* row_ptr, const int32_t* order, const int64_t* counts, int64_t
+                            n_targets, int64_t n_sources, int64_t n_edges, int64_t D, int64_t orders, int64_t F, int64_t
+                            H, int64_t buckets, double scale, float* alpha, void* stream);
+int gm_relative_backward_f32(const float* g, const float* alpha, const float* q, const float* k, const float* records,
+                             const float* records_s, const int64_t* desc, const int64_t* row_ptr, const int64_t*
+                             src_ptr, const int32_t* order, const int64_t* counts, const int32_t* order_s, const
+                             int64_t* counts_s, int64_t n_targets, int64_t n_sources, int64_t n_edges, int64_t D,
+                             int64_t orders, int64_t F, int64_t H, int64_t buckets, double scale, float* ds, float*
+                             partial, float* dq, float* dk, float* dtable, void* stream);
+int gm_relative_forward_f64(const double* q, const double* k, const double* table, const double* records, const int64_t*
+                            desc, const int64_t* row_ptr, const int32_t* order, const int64_t* counts, int64_t
+                            n_targets, int64_t n_sources, int64_t n_edges, int64_t D, int64_t orders, int64_t F, int64_t
+                            H, int64_t buckets, double scale, double* alpha, void* stream);
+int gm_relative_backward_f64(const double* g, const double* alpha, const double* q, const double* k, const double*
+                             records, const double* records_s, const int64_t* desc, const int64_t* row_ptr, const
+                             int64_t* src_ptr, const int32_t* order, const int64_t* counts, const int32_t* order_s,
+                             const int64_t* counts_s, int64_t n_targets, int64_t n_sources, int64_t n_edges, int64_t D,
+                             int64_t orders, int64_t F, int64_t H, int64_t buckets, double scale, double* ds, double*
+                             partial, double* dq, double* dk, double* dtable, void* stream);
+int gm_relative_forward_bf16(const uint16_t* q, const uint16_t* k, const float* table, const float* records, const
+                             int64_t* desc, const int64_t* row_ptr, const int32_t* order, const int64_t* counts, int64_t
+                             n_targets, int64_t n_sources, int64_t n_edges, int64_t D, int64_t orders, int64_t F,
+                             int64_t H, int64_t buckets, double scale, float* alpha, void* stream);
+int gm_relative_backward_bf16(const float* g, const float* alpha, const uint16_t* q, const uint16_t* k, const float*
+                              records, const float* records_s, const int64_t* desc, const int64_t* row_ptr, const
+                              int64_t* src_ptr, const int32_t* order, const int64_t* counts, const int32_t* order_s,
+                              const int64_t* counts_s, int64_t n_targets, int64_t n_sources, int64_t n_edges, int64_t D,
+                              int64_t orders, int64_t F, int64_t H, int64_t buckets, double scale, float* ds, float*
+                              partial, uint16_t* dq, uint16_t* dk, float* dtable, void* stream);
+
 /* ---------------- transformer block pointwise operators ----------------
  *
  * Flat node rows of width D: frequency 0 in [0, a0), then the nf nonzero
