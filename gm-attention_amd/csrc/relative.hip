@@ -18,6 +18,7 @@
 // the transport's (cos, sin) of orders 1 .., packed once for an edge set; the source
 // side's name the target and the edge.
 #include "relative.hpp"
+#include "partial_sum.hpp"
 
 #include <type_traits>
 
@@ -191,49 +192,14 @@ __global__ __launch_bounds__(64) void relative_table_simple(RelArgs<T, R> a) {
   for (int i = lane; i < a.buckets * H; i += kWave) a.partial[(int64_t)blockIdx.x * a.buckets * H + i] = bins[i];
 }
 
-template <typename T>
-__global__ __launch_bounds__(256) void relative_table_sum(const T* partial, int64_t rows, int columns, T* out) {
-  __shared__ double sums[16][17];
-  const int c = threadIdx.x & 15, part = threadIdx.x >> 4, column = blockIdx.x * 16 + c;
-  double s = 0.0;
-  if (column < columns)
-    for (int64_t r = part; r < rows; r += 16) s += (double)partial[r * columns + column];
-  sums[part][c] = s;
-  __syncthreads();
-  if (part == 0 && column < columns) {
-    double t = 0.0;
-    for (int i = 0; i < 16; ++i) t += sums[i][c];
-    out[column] = (T)t;
-  }
-}
-
 // ------------------------------------------------------------------- launch
 
 int rel_parse(const int64_t* desc, int64_t F, int64_t H, int64_t D, int64_t orders, RelLayout& L) {
-  GM_REQUIRE(desc != nullptr, "desc must be a host pointer to (F, 5) int64");
-  GM_REQUIRE(F >= 1 && F <= kRelMaxFreq, "desc must have 1 to 8 frequency rows");
-  GM_REQUIRE(H >= 1 && H <= GM_ATTN_MAX_H, "at most 16 heads");
-  GM_REQUIRE(D >= 1 && D <= GM_ATTN_MAX_D, "D must be in [1, 1024]");
   GM_REQUIRE(orders >= 1 && orders <= 256, "the phase tables need at least one order, 256 at most");
-  L.F = (int)F;
-  L.H = (int)H;
-  L.D = (int)D;
+  const int rc = parse_heads(desc, F, H, GM_ATTN_MAX_H, D, L);
+  if (rc != GM_OK) return rc;
   L.orders = (int)orders;
-  int64_t next = 0;
-  for (int f = 0; f < F; ++f) {
-    const int64_t* row = desc + f * GM_ATTN_DESC;
-    GM_REQUIRE(row[0] >= 0 && row[0] < orders, "a descriptor frequency exceeds the phase tables");
-    GM_REQUIRE(f == 0 || row[0] > desc[(f - 1) * GM_ATTN_DESC], "the descriptor's frequencies must rise");
-    GM_REQUIRE(row[4] == (row[0] == 0 ? 1 : 2), "descriptor dim must be 1 at frequency 0 and 2 above");
-    GM_REQUIRE(row[1] >= 1 && row[1] <= GM_ATTN_MAX_D && row[2] == next,
-               "the descriptor's rows must hold copies and follow each other");
-    next += H * row[1] * row[4];
-    GM_REQUIRE(next <= D, "a descriptor row runs past the flat width D");
-    L.n[f] = (int)row[0];
-    L.a[f] = (int)row[1];
-    L.off[f] = (int)row[2];
-  }
-  GM_REQUIRE(next == D, "the heads must fill the flat width");
+  GM_REQUIRE(L.n[L.F - 1] < L.orders, "a descriptor frequency exceeds the phase tables");
   return GM_OK;
 }
 
@@ -342,8 +308,7 @@ int relative_backward(const T* g, const T* alpha, const R* q, const R* k, const 
       status = rel_launch_units(RelPass::BackwardTarget, a, targets, s);
       if (status == GM_OK) status = rel_launch_units(RelPass::BackwardSource, a, sources, s);
       if (status != GM_OK) return status;
-      hipLaunchKernelGGL(relative_table_sum<T>, dim3((unsigned)((columns + 15) / 16)), dim3(256), 0, s,
-                         (const T*)partial, (int64_t)kRelTableRows, columns, dtable);
+      launch_partial_sum<T>(partial, kRelTableRows, columns, dtable, s);
       return check_launch("relative_backward");
     }
   }
@@ -355,8 +320,7 @@ int relative_backward(const T* g, const T* alpha, const R* q, const R* k, const 
   if (n_sources > 0)
     hipLaunchKernelGGL((relative_rows_simple<T, R, false>), dim3((unsigned)blocks_for(n_sources)), dim3(256), 0, s, a);
   hipLaunchKernelGGL((relative_table_simple<T, R>), dim3(kRelTableRows), dim3(kWave), sizeof(T) * columns, s, a);
-  hipLaunchKernelGGL(relative_table_sum<T>, dim3((unsigned)((columns + 15) / 16)), dim3(256), 0, s, (const T*)partial,
-                     (int64_t)kRelTableRows, columns, dtable);
+  launch_partial_sum<T>(partial, kRelTableRows, columns, dtable, s);
   return check_launch("relative_backward");
 }
 

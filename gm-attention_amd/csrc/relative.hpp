@@ -6,16 +6,14 @@
 
 #include "common.hpp"
 #include "edge_units.hpp"
+#include "heads.hpp"
 
 namespace gm {
 
-constexpr int kRelMaxFreq = GM_ATTN_MAX_F;
 constexpr int kRelMaxBuckets = 256;  // a float record's word holds a bucket above its source's 24 bits
 
-// The H heads in the rows: frequency f's order n, copies a a head, flat offset.
-struct RelLayout {
-  int F, H, D, orders;
-  int n[kRelMaxFreq], a[kRelMaxFreq], off[kRelMaxFreq];
+struct RelLayout : HeadsLayout {
+  int orders;
 };
 
 // The rows (targets, or sources) as the lane kernels take them: `order` lists them in three classes, those of 16 waves

@@ -125,6 +125,13 @@ SIGNATURES_F32 = {
        for sfx in ("f32", "f64", "bf16")},
     **{f"gm_relative_backward_{sfx}": (ctypes.c_int, [_P] * 13 + [_I] * 8 + [_D] + [_P] * 6)
        for sfx in ("f32", "f64", "bf16")},
+    "gm_head_norm_partial_rows": (ctypes.c_int64, [_I]),
+    **{f"gm_head_norm_forward_{sfx}": (ctypes.c_int, [_P] * 3 + [_I, _P] + [_I] * 4 + [_P] * 2 + [_I] * 2 + [_D] +
+                                       [_P] * 2)
+       for sfx in ("f32", "f64", "bf16")},
+    **{f"gm_head_norm_backward_{sfx}": (ctypes.c_int, [_P] * 4 + [_I, _P] + [_I] * 4 + [_P] * 2 + [_I] * 2 + [_D] +
+                                        [_P] * 4)
+       for sfx in ("f32", "f64", "bf16")},
     "gm_residual_norm_partial_rows": (ctypes.c_int64, [_I]),
     **{f"gm_residual_norm_forward_{sfx}": (ctypes.c_int, [_P] * 4 + [_I] * 4 + [_P, _P, _D, _D, _D] + [_P] * 4)
        for sfx in ("f32", "f64", "bf16", "bf16_f32")},
@@ -1765,3 +1772,73 @@ def relative_backward(g: Tensor, alpha: Tensor, q: Tensor, k: Tensor, tables: An
              tables.orders, desc.shape[0], H, tables.n_buckets, scale, _ptr(ds), _ptr(partial), _ptr(dq), _ptr(dk),
              _ptr(dtable), _stream(device))
     return dq, dk, dtable
+
+
+# ---------------------------------------------------------------- norm and rotation of rows of heads
+
+
+_PAIR, _STRIDES = ctypes.c_void_p * 2, ctypes.c_int64 * 2
+
+
+def _addresses(ts: Sequence[Tensor | None]) -> Any:
+    return _PAIR(*[None if t is None else t.data_ptr() for t in ts])
+
+
+def _head_norm_check(rows: Sequence[Tensor], gains: Sequence[Tensor | None], layout: Any, positions: Tensor | None,
+                     frequencies: Tensor | None) -> None:
+    first, pd = rows[0], param_dtype(rows[0].dtype)
+    for x in rows:
+        if (x.dtype != first.dtype or x.device != first.device or x.shape != (first.shape[0], layout.width)
+                or (x.shape[1] > 1 and x.stride(1) != 1) or (x.shape[0] > 1 and x.stride(0) < layout.width)):
+            raise RuntimeError(f"rows must be (N, {layout.width}) with each row's numbers side by side, alike")
+    for g in gains:
+        if g is not None and (g.dtype != pd or g.device != first.device or g.shape != (layout.copies,)
+                              or not g.is_contiguous()):
+            raise RuntimeError(f"gains must be contiguous {pd} ({layout.copies},) on the rows' device")
+    for t in (positions, frequencies):
+        if t is not None and (t.dtype != torch.float64 or t.device != first.device or not t.is_contiguous()):
+            raise RuntimeError("positions and frequencies must be contiguous float64 on the rows' device")
+
+
+def head_norm_forward(rows: Sequence[Tensor], gains: Sequence[Tensor | None], layout: Any, eps: float | None,
+                      positions: Tensor | None, frequencies: Tensor | None) -> list[Tensor]:
+    """One or two sets of rows of heads normalised (not with ``eps`` None), multiplied by their gains and turned
+    by their positions' angles: contiguous, in the rows' dtype."""
+    _head_norm_check(rows, gains, layout, positions, frequencies)
+    first, desc = rows[0], layout.desc
+    n, device = first.shape[0], first.device
+    out = [torch.empty(n, layout.width, dtype=first.dtype, device=device) for _ in rows]
+    _call_on(device, "gm_head_norm_forward_" + _PW_SUFFIX[first.dtype], _addresses(rows),
+             _STRIDES(*[x.stride(0) for x in rows]), _addresses(gains), len(rows), desc.data_ptr(), n, layout.width,
+             desc.shape[0], layout.heads, None if positions is None else _ptr(positions),
+             None if frequencies is None else _ptr(frequencies), 0 if frequencies is None else frequencies.shape[0],
+             int(eps is not None), 1.0 if eps is None else eps, _addresses(out), _stream(device))
+    return out
+
+
+def head_norm_backward(grads: Sequence[Tensor], rows: Sequence[Tensor], gains: Sequence[Tensor | None], layout: Any,
+                       eps: float | None, positions: Tensor | None, frequencies: Tensor | None,
+                       with_gains: bool) -> tuple[list[Tensor], list[Tensor | None]]:
+    """``(dx, dgain)`` of every set a forward took, from the outputs' gradients (contiguous); the gains' (under
+    ``with_gains``) summed over nodes and heads in a fixed order."""
+    _head_norm_check(rows, gains, layout, positions, frequencies)
+    first, desc = rows[0], layout.desc
+    n, device, sets, pd = first.shape[0], first.device, len(rows), param_dtype(first.dtype)
+    for g in grads:
+        if g.dtype != first.dtype or g.shape != first.shape or not g.is_contiguous() or g.device != device:
+            raise RuntimeError("the gradients must match the rows (contiguous)")
+    dx = [torch.empty_like(g) for g in grads]
+    dgain = torch.empty(sets, layout.copies, dtype=pd, device=device) if with_gains else None
+    if n == 0:
+        return dx, [None] * sets if dgain is None else list(dgain.zero_().unbind(0))
+    partial = None
+    if dgain is not None:
+        blocks = int(library().gm_head_norm_partial_rows(n))
+        partial = torch.empty(blocks * sets * layout.copies, dtype=pd, device=device)
+    _call_on(device, "gm_head_norm_backward_" + _PW_SUFFIX[first.dtype], _addresses(grads), _addresses(rows),
+             _STRIDES(*[x.stride(0) for x in rows]), _addresses(gains), sets, desc.data_ptr(), n, layout.width,
+             desc.shape[0], layout.heads, None if positions is None else _ptr(positions),
+             None if frequencies is None else _ptr(frequencies), 0 if frequencies is None else frequencies.shape[0],
+             int(eps is not None), 1.0 if eps is None else eps, _addresses(dx), _ptr(partial), _ptr(dgain),
+             _stream(device))
+    return dx, [None] * sets if dgain is None else list(dgain.unbind(0))

@@ -389,6 +389,47 @@ int gm_relative_backward_bf16(const float* g, const float* alpha, const uint16_t
                               int64_t orders, int64_t F, int64_t H, int64_t buckets, double scale, float* ds, float*
                               partial, uint16_t* dq, uint16_t* dk, float* dtable, void* stream);
 
+/* ---------------- norm and rotation of rows of heads ----------------
+ *
+ * One or two sets (queries and keys) of rows (n_rows, D) of H heads in desc's layout
+ * (frequencies rising, rows of copies following each other, D filled; H <= 64), over
+ * the same nodes.  For every head's P numbers x of a row
+ *   xhat = x / sqrt(mean x^2 + eps)          (xhat = x unless normalise)
+ *   y    = exp(i theta) (gain xhat),  theta = sum_a positions[row, a] frequencies[a, slot]
+ * with a gain a copy (copies of a head; NULL: ones) and a slot a pair of frequency-0
+ * copies (a last odd one stays), then every copy of the frequencies above; axes <= 8, 0
+ * without a rotation.  Backward from dy: dx, and dgain (sets, copies) through partial
+ * (gm_head_norm_partial_rows(n_rows) rows of sets copies), both NULL or neither; sums in a
+ * fixed order.
+ * x, gains, y, dy, dx: HOST arrays of `sets` device pointers; strides (HOST): the sets'
+ * numbers from a row of x to the next, D or more; y, dy and dx rows lie D apart.
+ * Suffix _bf16: bfloat16 rows, float gains and arithmetic.  No reference counterpart. */
+int64_t gm_head_norm_partial_rows(int64_t n_rows);
+int gm_head_norm_forward_f32(const float* const* x, const int64_t* strides, const float* const* gains, int64_t sets,
+                             const int64_t* desc, int64_t n_rows, int64_t D, int64_t F, int64_t H, const double*
+                             positions, const double* frequencies, int64_t axes, int64_t normalise, double eps, float*
+                             const* y, void* stream);
+int gm_head_norm_backward_f32(const float* const* dy, const float* const* x, const int64_t* strides, const float* const*
+                              gains, int64_t sets, const int64_t* desc, int64_t n_rows, int64_t D, int64_t F, int64_t H,
+                              const double* positions, const double* frequencies, int64_t axes, int64_t normalise,
+                              double eps, float* const* dx, float* partial, float* dgain, void* stream);
+int gm_head_norm_forward_f64(const double* const* x, const int64_t* strides, const double* const* gains, int64_t sets,
+                             const int64_t* desc, int64_t n_rows, int64_t D, int64_t F, int64_t H, const double*
+                             positions, const double* frequencies, int64_t axes, int64_t normalise, double eps, double*
+                             const* y, void* stream);
+int gm_head_norm_backward_f64(const double* const* dy, const double* const* x, const int64_t* strides, const double*
+                              const* gains, int64_t sets, const int64_t* desc, int64_t n_rows, int64_t D, int64_t F,
+                              int64_t H, const double* positions, const double* frequencies, int64_t axes, int64_t
+                              normalise, double eps, double* const* dx, double* partial, double* dgain, void* stream);
+int gm_head_norm_forward_bf16(const uint16_t* const* x, const int64_t* strides, const float* const* gains, int64_t sets,
+                              const int64_t* desc, int64_t n_rows, int64_t D, int64_t F, int64_t H, const double*
+                              positions, const double* frequencies, int64_t axes, int64_t normalise, double eps,
+                              uint16_t* const* y, void* stream);
+int gm_head_norm_backward_bf16(const uint16_t* const* dy, const uint16_t* const* x, const int64_t* strides, const float*
+                               const* gains, int64_t sets, const int64_t* desc, int64_t n_rows, int64_t D, int64_t F,
+                               int64_t H, const double* positions, const double* frequencies, int64_t axes, int64_t
+                               normalise, double eps, uint16_t* const* dx, float* partial, float* dgain, void* stream);
+
 /* ---------------- transformer block pointwise operators ----------------
  *
  * Flat node rows of width D: frequency 0 in [0, a0), then the nf nonzero

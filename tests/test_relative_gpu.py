@@ -544,6 +544,14 @@ def test_on_another_stream(cuda):
 
 @pytest.mark.gpu
 def test_no_targets_and_no_edges(cuda):
+    nothing(cuda)
+
+
+def test_no_targets_and_no_edges_on_the_cpu():
+    nothing("cpu")
+
+
+def nothing(cuda):
     for copies in ({0: 4, 1: 4}, {0: 3, 1: 1}):
         head = SO2FieldType(copies)
         for n, m in ((0, 0), (0, 5), (4, 0), (4, 5)):
