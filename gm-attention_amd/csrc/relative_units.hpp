@@ -1,0 +1,634 @@
+// The lane kernels of the softmax with a learned relative bias: a head's copies are
+// `per_map` units of (A0, A1, A2) copies of frequencies 0, 1, 2, one lane a unit
+// (edge_units.hpp).
+#pragma once
+#include <algorithm>
+#include <type_traits>
+
+#include "edge_units.hpp"
+#include "relative.hpp"
+
+namespace gm {
+namespace rel {
+
+constexpr int kRelSteps = 32;     // steps of a wave whose scores LDS holds, at most: 32 S edges
+constexpr int kRelInFlight = 4;   // steps whose rows are requested together
+constexpr int kRelThreadsB = kWavesPerBlock * kWave;
+
+// A lane's shape; NO, the orders of the tables above 0.
+template <int A0, int A1, int A2, int ORD>
+struct RelUnit {
+  static constexpr int W0 = A0, W1 = 2 * A1, W2 = 2 * A2, N = W0 + W1 + W2;
+  static constexpr int NO = ORD;
+  static constexpr int NA = NO > 0 ? NO : 1;  // arrays of none
+  static constexpr int RW = 2 + 2 * NO;
+
+  template <bool kNear, typename R>
+  static __device__ __forceinline__ void load(const R* rows, const EdgeUnits& w, int unit, int node, float (&v)[N]) {
+    if constexpr (kNear) {
+      const uint32_t row = __umul24((uint32_t)node, w.row_bytes);
+      auto at = [&](int f, int width) {
+        return reinterpret_cast<const R*>(reinterpret_cast<const char*>(rows + w.base[f]) +
+                                          (row + (uint32_t)(unit * width) * (uint32_t)sizeof(R)));
+      };
+      if constexpr (W0 > 0) load_w<W0>(at(0, W0), v);
+      if constexpr (W1 > 0) load_w<W1>(at(1, W1), v + W0);
+      if constexpr (W2 > 0) load_w<W2>(at(2, W2), v + W0 + W1);
+    } else {
+      const R* row = reinterpret_cast<const R*>(reinterpret_cast<const char*>(rows) + (int64_t)node * w.row_bytes);
+      if constexpr (W0 > 0) load_w<W0>(row + w.base[0] + unit * W0, v);
+      if constexpr (W1 > 0) load_w<W1>(row + w.base[1] + unit * W1, v + W0);
+      if constexpr (W2 > 0) load_w<W2>(row + w.base[2] + unit * W2, v + W0 + W1);
+    }
+  }
+  template <typename R>
+  static __device__ __forceinline__ void store(R* row, const EdgeUnits& w, int unit, const float (&v)[N]) {
+    if constexpr (W0 > 0) store_w<W0>(row + w.base[0] + unit * W0, v);
+    if constexpr (W1 > 0) store_w<W1>(row + w.base[1] + unit * W1, v + W0);
+    if constexpr (W2 > 0) store_w<W2>(row + w.base[2] + unit * W2, v + W0 + W1);
+  }
+  // the frequency of order o + 1's numbers: where they start, how many
+  static constexpr int start(int o) { return o == 0 ? W0 : W0 + W1; }
+  static constexpr int width(int o) { return o == 0 ? W1 : W2; }
+
+  // Re< q, tau k >: per order cos sum (q0 k0 + q1 k1) + sin sum (q1 k0 - q0 k1)
+  static __device__ __forceinline__ float dot(const float (&q)[N], const float (&k)[N], const float (&cs)[NA],
+                                              const float (&sn)[NA]) {
+    float acc = 0.f;
+#pragma unroll
+    for (int i = 0; i < W0; ++i) acc = fmaf(q[i], k[i], acc);
+#pragma unroll
+    for (int o = 0; o < NO; ++o) {
+      float re = 0.f, im = 0.f;
+#pragma unroll
+      for (int i = 0; i < width(o); i += 2) {
+        const int at = start(o) + i;
+        re = fmaf(q[at], k[at], fmaf(q[at + 1], k[at + 1], re));
+        im = fmaf(q[at + 1], k[at], fmaf(-q[at], k[at + 1], im));
+      }
+      if (width(o) > 0) acc = fmaf(cs[o], re, fmaf(sn[o], im, acc));
+    }
+    return acc;
+  }
+  // sums += d tau k, or with `back` d conj(tau) k
+  static __device__ __forceinline__ void add(float (&sums)[N], float d, const float (&k)[N], const float (&cs)[NA],
+                                             const float (&sn)[NA], bool back) {
+#pragma unroll
+    for (int i = 0; i < W0; ++i) sums[i] = fmaf(d, k[i], sums[i]);
+#pragma unroll
+    for (int o = 0; o < NO; ++o) {
+      const float c = d * cs[o], s = back ? -d * sn[o] : d * sn[o];
+#pragma unroll
+      for (int i = 0; i < width(o); i += 2) {
+        const int at = start(o) + i;
+        sums[at] = fmaf(c, k[at], fmaf(-s, k[at + 1], sums[at]));
+        sums[at + 1] = fmaf(c, k[at + 1], fmaf(s, k[at], sums[at + 1]));
+      }
+    }
+  }
+};
+
+// The value of the neighbouring lane, which holds the other step of a pair for the same head: a DPP operand.
+__device__ __forceinline__ float next_lane(float v) {
+  return __int_as_float(__builtin_amdgcn_mov_dpp(__float_as_int(v), 0xB1, 0xF, 0xF, true));
+}
+
+// The block's rows: block b of `blocks` holds the rows order[first + ...), as share_of.
+__device__ __forceinline__ Share rel_share(const EdgeUnits& w, const int64_t* ptr, int64_t block, int64_t blocks) {
+  Share s;
+  s.wave = uniform((int)(threadIdx.x >> 6));
+  const int waves = blockDim.x >> 6;
+  const bool one = block >= w.shared;
+  const int64_t at = one ? w.shared + xcd_spread_block(block - w.shared, blocks - w.shared) * waves + s.wave
+                         : xcd_spread_block(block, w.shared);
+  s.part = one ? 0 : s.wave;
+  s.parts = one ? 1 : waves;
+  s.live = at < w.shared + w.single;
+  s.row = s.live ? uniform((int)w.order[w.first + at]) : 0;
+  const int64_t e0 = s.live ? uniform(ptr[s.row]) : 0, e1 = s.live ? uniform(ptr[s.row + 1]) : 0;
+  const int64_t steps = (e1 - e0 + w.slots - 1) >> (6 - w.shift);
+  const int64_t per = (one ? steps : (steps + waves - 1) / waves) << (6 - w.shift);
+  s.e0 = e0 + s.part * per < e1 ? e0 + s.part * per : e1;
+  s.e1 = s.e0 + per < e1 ? s.e0 + per : e1;
+  s.steps = (int)((s.e1 - s.e0 + w.slots - 1) >> (6 - w.shift));
+  return s;
+}
+
+// ---------------------------------------------------------------- forward
+
+// kPair: a head has two units or more, whose lanes hold the same scores: two of them keep every second step's each.
+template <typename R, typename U, bool kNear, bool kPair>
+__global__ __launch_bounds__(1024) void relative_forward_units(RelArgs<float, R> a, EdgeUnits w, int64_t blocks,
+                                                               int steps) {
+  constexpr int kWords = kWave * U::RW;
+  const int kept = kPair ? steps / 2 : steps;  // a wave's rows of scores in LDS
+  extern __shared__ __align__(16) float rel_lds[];
+  const int waves = blockDim.x >> 6, lane = threadIdx.x & 63, wave = uniform((int)(threadIdx.x >> 6));
+  float* rec = rel_lds + wave * (kWords + kept * kWave);
+  float* sc = rec + kWords + lane;
+  float* shared = rel_lds + waves * (kWords + kept * kWave);  // (waves, 64): the waves' maxima, then sums
+  float* learned = shared + (waves > 1 ? waves * kWave : 0);   // (buckets, H), in units of log 2
+  for (int i = threadIdx.x; i < a.buckets * a.L.H; i += blockDim.x) learned[i] = a.table[i] * (float)kRelLog2e;
+  __syncthreads();
+  const int u = lane & (w.lanes - 1), s = lane >> w.shift, unit = u < w.units ? u : w.units - 1;
+  const int h = unit / w.per_map, own = unit % w.per_map;
+  const bool odd = kPair && (own & 1), writes = u < w.units && own < (kPair ? 2 : 1);
+  const float* mine = rec + s * U::RW;  // this lane's edge of step 0
+  const float scale = a.scale;
+  const float* bias_of = learned + h;
+
+  const Share sh = rel_share(w, a.row_ptr, blockIdx.x, blocks);
+  if (!sh.live) return;  // one wave a row, or the whole workgroup
+  float q[U::N];
+  U::template load<false>(a.q, w, unit, sh.row, q);
+  const int held = sh.steps < steps ? sh.steps : steps;
+  float m = neg_inf<float>(), l = 0.f, inv = 0.f;
+
+  // over a lane's slots (and, of a sum, the two lanes with a step each) and the row's waves.  A score that is not a
+  // number is not a maximum; its exponential makes the sum, and with it the row, not a number.
+  auto over_waves = [&](float v, bool maximum) {
+    for (int o = w.lanes; o < kWave; o <<= 1) {
+      const float x = __shfl_xor(v, o, kWave);
+      v = maximum ? fmaxf(x, v) : v + x;
+    }
+    if constexpr (kPair) {
+      const float x = next_lane(v);
+      v = maximum ? fmaxf(x, v) : v + x;
+    }
+    if (sh.parts > 1) {
+      __syncthreads();
+      shared[sh.wave * kWave + lane] = v;
+      __syncthreads();
+      v = shared[lane];
+      for (int o = 1; o < waves; ++o) {
+        const float x = shared[o * kWave + lane];
+        v = maximum ? fmaxf(x, v) : v + x;
+      }
+    }
+    return v;
+  };
+  const uint32_t place = (uint32_t)(s * a.L.H + h);
+  // the weight of step t of the edges from `e`
+  auto write = [&](int64_t e, int t, float v) {
+    float* to = a.alpha + (e + t * w.slots) * a.L.H;
+    if (writes && s < (int)(sh.e1 - e) - t * w.slots) to[place] = v;
+  };
+
+  // phase 0: every score, its maximum; the first `steps` steps' stay in LDS.  The steps past them are scored again
+  // for the sum (1) and the weights (2): rows beyond 16 waves' LDS only.
+  for (int phase = 0; phase < 3; ++phase) {
+    if (phase == 1) {
+      m = over_waves(m, true);
+      m = m == neg_inf<float>() ? 0.f : m;  // no edge inside: exp(-inf) = 0 everywhere
+      if constexpr (kPair) {
+        for (int t = 0; t < held; t += 2) {  // a step past `held` is outside: its weight is zero
+          const float x = exp2_of(sc[t / 2 * kWave] - m);
+          sc[t / 2 * kWave] = x;
+          l += x;
+        }
+      } else {
+        for (int t = 0; t < held; ++t) {
+          const float x = exp2_of(sc[t * kWave] - m);
+          sc[t * kWave] = x;
+          l += x;
+        }
+      }
+    }
+    if (phase == 2) {
+      l = over_waves(l, false);
+      inv = l == 0.f ? 0.f : 1.f / l;
+      if constexpr (kPair) {
+        for (int t = 0; t < held; t += 2) write(sh.e0, t + odd, sc[t / 2 * kWave] * inv);
+      } else {
+        for (int t = 0; t < held; ++t) write(sh.e0, t, sc[t * kWave] * inv);
+      }
+    }
+    const int skip = phase == 0 ? 0 : steps;
+    if (skip >= sh.steps) continue;
+    const int first = skip & ~(w.lanes - 1);  // a batch's first step
+    Records<U::RW> records;
+    records.request(a.records, sh.e0 + (int64_t)first * w.slots, sh.e1, lane);
+    for (int b = first; b < sh.steps; b += w.lanes) {
+      const int64_t e = sh.e0 + (int64_t)b * w.slots;  // the batch's first edge
+      wave_lds();
+      records.put(rec, lane);
+      wave_lds();
+      if (b + w.lanes < sh.steps) records.request(a.records, e + kWave, sh.e1, lane);
+      const int ends = sh.steps - b < w.lanes ? sh.steps - b : w.lanes;
+      auto take = [&](int t, auto group) {
+        constexpr int UN = decltype(group)::value;
+        float2 head[UN];
+        float k[UN][U::N], cs[UN][U::NA], sn[UN][U::NA], v[UN];
+#pragma unroll
+        for (int n = 0; n < UN; ++n) {
+          const float* r = mine + (t + n) * w.slots * U::RW;
+          head[n] = *reinterpret_cast<const float2*>(r);
+#pragma unroll
+          for (int o = 0; o < U::NO; ++o) {
+            const float2 x = *reinterpret_cast<const float2*>(r + 2 + 2 * o);
+            cs[n][o] = x.x;
+            sn[n][o] = x.y;
+          }
+        }
+#pragma unroll
+        for (int n = 0; n < UN; ++n)
+          U::template load<kNear>(a.k, w, unit, __float_as_int(head[n].x) & 0xFFFFFF, k[n]);
+        float bias[UN];
+#pragma unroll
+        for (int n = 0; n < UN; ++n) bias[n] = bias_of[(__float_as_uint(head[n].x) >> 24) * a.L.H];
+#pragma unroll
+        for (int n = 0; n < UN; ++n) v[n] = U::dot(q, k[n], cs[n], sn[n]);
+        sum_units<UN>(v, w.per_map);
+#pragma unroll
+        for (int n = 0; n < UN; ++n)  // outside the window: excluded, whatever its row holds
+          v[n] = head[n].y == neg_inf<float>() ? neg_inf<float>() : fmaf(scale, v[n], head[n].y + bias[n]);
+        if constexpr (kPair) {
+#pragma unroll
+          for (int n = 0; n < UN; n += 2) {
+            const float even = v[n], next = v[n + 1], x = odd ? next : even;
+            if (phase == 0) {
+              m = fmaxf(m, x);
+              if (b + t < steps) sc[(b + t + n) / 2 * kWave] = x;
+            } else if (phase == 1) {
+              l += exp2_of(x - m);
+            } else {
+              write(e, t + n + odd, exp2_of(x - m) * inv);
+            }
+          }
+        } else {
+#pragma unroll
+          for (int n = 0; n < UN; ++n) {
+            if (phase == 0) {
+              m = fmaxf(m, v[n]);
+              if (b + t < steps) sc[(b + t + n) * kWave] = v[n];
+            } else if (phase == 1) {
+              l += exp2_of(v[n] - m);
+            } else {
+              write(e, t + n, exp2_of(v[n] - m) * inv);
+            }
+          }
+        }
+      };
+      int t = skip > b ? skip - b : 0;
+      for (; ends - t > 2 && sh.parts <= kWavesPerBlock; t += kRelInFlight)
+        take(t, std::integral_constant<int, kRelInFlight>());
+      for (; t < ends; t += 2) take(t, std::integral_constant<int, 2>());
+    }
+  }
+}
+
+// ---------------------------------------------------------------- backward
+
+// Per target: T = sum alpha g over its edges, then ds = alpha (g - T), written, added to the wave's bins (buckets,
+// columns) in LDS and to dq = scale sum ds tau k.  A workgroup takes rows until none is left and writes its bins.
+template <typename R, typename U, bool kNear, bool kPair>
+__global__ __launch_bounds__(kRelThreadsB) void relative_backward_target_units(RelArgs<float, R> a, EdgeUnits w,
+                                                                               int64_t blocks, int spread) {
+  constexpr int kWords = kWave * U::RW, UN = 2;
+  extern __shared__ __align__(16) float rel_lds[];
+  const int lane = threadIdx.x & 63, wave = uniform((int)(threadIdx.x >> 6)), H = a.L.H;
+  float* rec = rel_lds + wave * kWords;
+  float* shared = rel_lds + kWavesPerBlock * kWords;  // the waves' sums: (waves, max(N lanes, 64))
+  const int sums_words = kWavesPerBlock * std::max(U::N * w.lanes, kWave);
+  // a bin for every lane that holds a step, or one for those of all slots
+  const int per_slot = H * (kPair ? 2 : 1), columns = per_slot * (spread ? w.slots : 1);
+  float* bins = shared + sums_words + wave * a.buckets * columns;
+  const int u = lane & (w.lanes - 1), s = lane >> w.shift, unit = u < w.units ? u : w.units - 1;
+  const int h = unit / w.per_map, own = unit % w.per_map;
+  const bool odd = kPair && (own & 1), mine_too = u < w.units && own < (kPair ? 2 : 1);
+  const float* mine = rec + s * U::RW;
+  float* bin = bins + (spread ? s * per_slot : 0) + h * (kPair ? 2 : 1) + odd;
+  for (int i = lane; i < a.buckets * columns; i += kWave) bins[i] = 0.f;
+  wave_lds();
+
+  for (int64_t block = blockIdx.x; block < blocks; block += gridDim.x) {
+    const Share sh = rel_share(w, a.row_ptr, block, blocks);
+    if (!sh.live) continue;  // one wave a row, or the whole workgroup
+    const float* alpha = a.alpha + sh.e0 * H + h;
+    const float* grad = a.g + sh.e0 * H + h;
+    const int count = (int)(sh.e1 - sh.e0);
+    float total = 0.f;
+    for (int t = 0; t < sh.steps; t += kPair ? 2 : 1) {
+      const int e = (t + odd) * w.slots + s;
+      if (mine_too && e < count) {
+        const float al = alpha[(int64_t)e * H];
+        if (al != 0.f) total = fmaf(al, grad[(int64_t)e * H], total);
+      }
+    }
+    for (int o = w.lanes; o < kWave; o <<= 1) total += __shfl_xor(total, o, kWave);
+    if constexpr (kPair) {  // the lanes that hold steps, to all of a head's
+      total += next_lane(total);
+      total = __shfl(total, lane & ~(w.per_map - 1), kWave);
+    }
+    if constexpr (!kPair) total = __shfl(total, lane & ~(w.per_map - 1), kWave);
+    if (sh.parts > 1) {
+      __syncthreads();
+      shared[sh.wave * kWave + lane] = total;
+      __syncthreads();
+      total = shared[lane];
+      for (int o = 1; o < sh.parts; ++o) total += shared[o * kWave + lane];
+    }
+    float sums[U::N];
+#pragma unroll
+    for (int i = 0; i < U::N; ++i) sums[i] = 0.f;
+    Records<U::RW> records;
+    if (sh.steps > 0) records.request(a.records, sh.e0, sh.e1, lane);
+    for (int b = 0; b < sh.steps; b += w.lanes) {
+      const int64_t e = sh.e0 + (int64_t)b * w.slots;  // the batch's first edge
+      wave_lds();
+      records.put(rec, lane);
+      wave_lds();
+      if (b + w.lanes < sh.steps) records.request(a.records, e + kWave, sh.e1, lane);
+      const int ends = sh.steps - b < w.lanes ? sh.steps - b : w.lanes;
+      const int left = (int)(sh.e1 - e < kWave ? sh.e1 - e : kWave);
+      const float* al_of = a.alpha + e * H + h;
+      const float* g_of = a.g + e * H + h;
+      float* ds_of = a.ds + e * H + h;
+      for (int t = 0; t < ends; t += UN) {
+        float k[UN][U::N], cs[UN][U::NA], sn[UN][U::NA], d[UN];
+        uint32_t word[UN];
+#pragma unroll
+        for (int n = 0; n < UN; ++n) {
+          const float* r = mine + (t + n) * w.slots * U::RW;
+          word[n] = *reinterpret_cast<const uint32_t*>(r);
+#pragma unroll
+          for (int o = 0; o < U::NO; ++o) {
+            const float2 x = *reinterpret_cast<const float2*>(r + 2 + 2 * o);
+            cs[n][o] = x.x;
+            sn[n][o] = x.y;
+          }
+        }
+#pragma unroll
+        for (int n = 0; n < UN; ++n) U::template load<kNear>(a.k, w, unit, (int)(word[n] & 0xFFFFFF), k[n]);
+        auto weigh = [&](int n) {  // ds of step t + n, written and added to its bin by the lane that holds it
+          const int at = (t + n) * w.slots + s;
+          float ds = 0.f;
+          if (at < left) {
+            const float al = al_of[(uint32_t)(at * H)];
+            if (al != 0.f) ds = al * (g_of[(uint32_t)(at * H)] - total);
+          }
+          return ds;
+        };
+        auto keep = [&](int n, float ds, uint32_t bucket) {
+          const int at = (t + n) * w.slots + s;
+          const bool live = mine_too && at < left;
+          if (live) ds_of[(uint32_t)(at * H)] = ds;
+          float* to = bin + bucket * columns;
+          if (spread) {
+            if (live) atomicAdd(to, ds);  // this lane's own: in the order of its steps
+          } else {
+            for (int o = 0; o < w.slots; ++o) {  // slot by slot: a wave's LDS operations are done in order
+              if (live && s == o) atomicAdd(to, ds);
+              __builtin_amdgcn_wave_barrier();
+            }
+          }
+        };
+        if constexpr (kPair) {
+          const float ds = odd ? weigh(1) : weigh(0);
+          keep(odd, ds, (odd ? word[1] : word[0]) >> 24);
+          const float other = next_lane(ds);
+          d[0] = odd ? other : ds;
+          d[1] = odd ? ds : other;
+        } else {
+#pragma unroll
+          for (int n = 0; n < UN; ++n) {
+            d[n] = weigh(n);
+            keep(n, d[n], word[n] >> 24);
+          }
+        }
+#pragma unroll
+        for (int n = 0; n < UN; ++n)
+          if (d[n] != 0.f) U::add(sums, d[n], k[n], cs[n], sn[n], false);
+      }
+    }
+    row_sums<U::N>(w, sh, sums, shared);
+    if (sh.part == 0 && s == 0 && u < w.units) {
+#pragma unroll
+      for (int i = 0; i < U::N; ++i) sums[i] *= a.gradient_scale;
+      U::store(a.dq + (int64_t)sh.row * a.L.D, w, unit, sums);
+    }
+  }
+  // the workgroup's bins: a head's lanes of every slot and wave, in order
+  __syncthreads();
+  float* first = shared + sums_words;
+  for (int i = threadIdx.x; i < a.buckets * H; i += blockDim.x) {
+    const int bucket = i / H, head = i % H;
+    float v = 0.f;
+    for (int wv = 0; wv < kWavesPerBlock; ++wv)
+      for (int sl = 0; sl < (spread ? w.slots : 1); ++sl)
+        for (int o = 0; o < (kPair ? 2 : 1); ++o)
+          v += first[((size_t)wv * a.buckets + bucket) * columns + sl * per_slot + head * (kPair ? 2 : 1) + o];
+    a.partial[((int64_t)blockIdx.x * a.buckets + bucket) * H + head] = v;
+  }
+}
+
+// Per source, over the edges sorted by source: dk = scale sum ds conj(tau) q.
+template <typename R, typename U, bool kNear, bool kPair>
+__global__ __launch_bounds__(kRelThreadsB) void relative_backward_source_units(RelArgs<float, R> a, EdgeUnits w,
+                                                                               int64_t blocks) {
+  constexpr int kWords = kWave * U::RW, UN = kRelInFlight;
+  extern __shared__ __align__(16) float rel_lds[];
+  const Share sh = rel_share(w, a.src_ptr, blockIdx.x, blocks);
+  if (!sh.live) return;
+  const int lane = threadIdx.x & 63, H = a.L.H;
+  float* rec = rel_lds + sh.wave * kWords;
+  const int u = lane & (w.lanes - 1), s = lane >> w.shift, unit = u < w.units ? u : w.units - 1;
+  const int h = unit / w.per_map;
+  const float* mine = rec + s * U::RW;
+  float sums[U::N];
+#pragma unroll
+  for (int i = 0; i < U::N; ++i) sums[i] = 0.f;
+  Records<U::RW> records;
+  if (sh.steps > 0) records.request(a.records_s, sh.e0, sh.e1, lane);
+  for (int b = 0; b < sh.steps; b += w.lanes) {
+    const int64_t e = sh.e0 + (int64_t)b * w.slots;
+    wave_lds();
+    records.put(rec, lane);
+    wave_lds();
+    if (b + w.lanes < sh.steps) records.request(a.records_s, e + kWave, sh.e1, lane);
+    const int ends = sh.steps - b < w.lanes ? sh.steps - b : w.lanes;
+    const int left = (int)(sh.e1 - e < kWave ? sh.e1 - e : kWave);
+    for (int t = 0; t < ends; t += UN) {
+      float2 head[UN];
+      float q[UN][U::N], cs[UN][U::NA], sn[UN][U::NA], d[UN];
+#pragma unroll
+      for (int n = 0; n < UN; ++n) {
+        const float* r = mine + (t + n) * w.slots * U::RW;
+        head[n] = *reinterpret_cast<const float2*>(r);
+        // past the row (and the batch's last step): node 0's row, edge 0's ds, not counted
+        const bool in = (t + n) * w.slots + s < left;
+        head[n].x = in ? head[n].x : 0.f;
+        head[n].y = in ? head[n].y : 0.f;
+#pragma unroll
+        for (int o = 0; o < U::NO; ++o) {
+          const float2 x = *reinterpret_cast<const float2*>(r + 2 + 2 * o);
+          cs[n][o] = x.x;
+          sn[n][o] = x.y;
+        }
+      }
+#pragma unroll
+      for (int n = 0; n < UN; ++n) {
+        d[n] = a.ds[(int64_t)__float_as_int(head[n].y) * H + h];
+        U::template load<kNear>(a.q, w, unit, __float_as_int(head[n].x), q[n]);
+      }
+#pragma unroll
+      for (int n = 0; n < UN; ++n)
+        if ((t + n) * w.slots + s < left && d[n] != 0.f) U::add(sums, d[n], q[n], cs[n], sn[n], true);
+    }
+  }
+  row_sums<U::N>(w, sh, sums, rel_lds);
+  if (sh.part == 0 && s == 0 && u < w.units) {
+#pragma unroll
+    for (int i = 0; i < U::N; ++i) sums[i] *= a.gradient_scale;
+    U::store(a.dk + (int64_t)sh.row * a.L.D, w, unit, sums);
+  }
+}
+
+// ------------------------------------------------------------------ launch
+
+// The unit a head's copies (a0, a1, a2) are `per_map` of, a power of two of them; the widest that serves.
+struct RelShape {
+  int a0, a1, a2;
+};
+constexpr RelShape kRelShapes[] = {{4, 2, 2}, {4, 2, 1}, {2, 2, 2}, {2, 1, 1}, {1, 1, 1},
+                                   {2, 2, 0}, {1, 1, 0}, {4, 0, 0}, {1, 0, 0}, {0, 2, 2}, {0, 1, 1}};
+constexpr int kRelShapeCount = sizeof(kRelShapes) / sizeof(kRelShapes[0]);
+
+// A head's copies at frequencies 0, 1, 2; false where there are others, or the tables hold more orders than that.
+inline bool rel_copies(const RelLayout& L, int (&c)[3], int (&base)[3]) {
+  for (int f = 0; f < 3; ++f) c[f] = base[f] = 0;
+  for (int f = 0; f < L.F; ++f) {
+    if (L.n[f] > 2) return false;
+    c[L.n[f]] = L.a[f];
+    base[L.n[f]] = L.off[f];
+  }
+  return L.orders == (c[2] > 0 ? 3 : (c[1] > 0 ? 2 : 1));
+}
+
+// The shape's index and the units a head, or -1.
+inline int rel_shape(const RelLayout& L, int& per_map, int (&base)[3]) {
+  int c[3];
+  if (!rel_copies(L, c, base)) return -1;
+  for (int i = 0; i < kRelShapeCount; ++i) {
+    const RelShape& u = kRelShapes[i];
+    for (per_map = 1; per_map * L.H <= kWave; per_map *= 2)
+      if (c[0] == per_map * u.a0 && c[1] == per_map * u.a1 && c[2] == per_map * u.a2) return i;
+  }
+  return -1;
+}
+
+constexpr size_t kRelLds = 160 * 1024;
+
+// LDS of a pass: the records a wave (and the forward's scores, and the learned table), the waves' sums, the bins.
+template <typename U>
+size_t rel_forward_lds(int waves, bool pair, int steps, int table) {
+  return sizeof(float) * ((size_t)waves * (kWave * U::RW + (pair ? steps / 2 : steps) * kWave + (waves > 1 ? kWave : 0)) +
+                          table);
+}
+template <typename U>
+size_t rel_target_lds(int lanes, int bins) {
+  return sizeof(float) * kWavesPerBlock * ((size_t)kWave * U::RW + std::max(U::N * lanes, kWave) + bins);
+}
+template <typename U>
+size_t rel_source_lds(int lanes) {
+  return sizeof(float) * kWavesPerBlock * (size_t)std::max(kWave * U::RW, U::N * lanes);
+}
+
+inline int rel_lds_limit(const void* kernel, size_t lds) {
+  if (lds > 64 * 1024 &&
+      hipFuncSetAttribute(kernel, hipFuncAttributeMaxDynamicSharedMemorySize, (int)kRelLds) != hipSuccess)
+    return check_launch("relative (LDS)");
+  return GM_OK;
+}
+
+template <typename R, typename U, bool kNear, bool kPair>
+int rel_launch(RelPass pass, const RelArgs<float, R>& a, EdgeUnits w, const RelRows& rows, hipStream_t stream) {
+  w.first = 0;
+  if (pass == RelPass::Forward) {
+    // the rows of sixteen waves; those of four and of one, in one launch of workgroups of four
+    const auto kernel = &relative_forward_units<R, U, kNear, kPair>;
+    for (int c = 0; c < 2; ++c) {
+      w.shared = rows.count[c];
+      w.single = c == 0 ? 0 : rows.count[2];
+      const int waves = c == 0 ? 16 : kWavesPerBlock;
+      if (w.shared + w.single > 0) {
+        const int64_t blocks = w.shared + blocks_for(w.single);
+        // sixteen waves' scores beside a large table: fewer steps of them (longer rows are scored again)
+        int steps = kRelSteps;
+        const int table = a.buckets * a.L.H;
+        while (rel_forward_lds<U>(waves, kPair, steps, table) > kRelLds) steps -= kRelInFlight;
+        const size_t lds = rel_forward_lds<U>(waves, kPair, steps, table);
+        int rc = rel_lds_limit(reinterpret_cast<const void*>(kernel), lds);
+        if (rc != GM_OK) return rc;
+        hipLaunchKernelGGL(kernel, dim3((unsigned)blocks), dim3(waves * kWave), lds, stream, a, w, blocks, steps);
+        rc = check_launch("relative");
+        if (rc != GM_OK) return rc;
+      }
+      w.first += w.shared;
+    }
+    return GM_OK;
+  }
+  w.shared = rows.count[0] + rows.count[1];
+  w.single = rows.count[2];
+  const int64_t blocks = w.shared + blocks_for(w.single);
+  if (pass == RelPass::BackwardTarget) {
+    const auto kernel = &relative_backward_target_units<R, U, kNear, kPair>;
+    const int bins = a.buckets * a.L.H * (kPair ? 2 : 1), spread = bins * w.slots <= 2048 ? 1 : 0;
+    const size_t lds = rel_target_lds<U>(w.lanes, bins * (spread ? w.slots : 1));
+    const int rc = rel_lds_limit(reinterpret_cast<const void*>(kernel), lds);
+    if (rc != GM_OK) return rc;
+    // every workgroup writes a row of bins, those without a row of their own too
+    hipLaunchKernelGGL(kernel, dim3(kRelTableRows), dim3(kRelThreadsB), lds, stream, a, w, blocks, spread);
+    return check_launch("relative");
+  }
+  if (blocks > 0) {
+    const auto kernel = &relative_backward_source_units<R, U, kNear, kPair>;
+    const size_t lds = rel_source_lds<U>(w.lanes);
+    const int rc = rel_lds_limit(reinterpret_cast<const void*>(kernel), lds);
+    if (rc != GM_OK) return rc;
+    hipLaunchKernelGGL(kernel, dim3((unsigned)blocks), dim3(kRelThreadsB), lds, stream, a, w, blocks);
+  }
+  return check_launch("relative");
+}
+
+template <typename R, int A0, int A1, int A2>
+int rel_launch_shape(RelPass pass, const RelArgs<float, R>& a, const EdgeUnits& w, const RelRows& rows, bool near,
+                     hipStream_t stream) {
+  using U = RelUnit<A0, A1, A2, (A2 > 0 ? 2 : (A1 > 0 ? 1 : 0))>;
+  if (near)
+    return w.per_map > 1 ? rel_launch<R, U, true, true>(pass, a, w, rows, stream)
+                         : rel_launch<R, U, true, false>(pass, a, w, rows, stream);
+  return w.per_map > 1 ? rel_launch<R, U, false, true>(pass, a, w, rows, stream)
+                       : rel_launch<R, U, false, false>(pass, a, w, rows, stream);
+}
+
+template <typename R>
+int rel_launch_any(RelPass pass, const RelArgs<float, R>& a, const RelRows& rows, hipStream_t stream) {
+  EdgeUnits w{};
+  const int shape = rel_shape(a.L, w.per_map, w.base);
+  if (shape < 0) return fail(GM_ERR_UNSUPPORTED, "relative: the lane kernels do not serve this layout");
+  w.units = a.L.H * w.per_map;
+  w.lanes = lanes_for(w.units);
+  while ((1 << w.shift) < w.lanes) ++w.shift;
+  w.slots = kWave / w.lanes;
+  w.row_bytes = (uint32_t)(a.L.D * sizeof(R));
+  w.order = rows.order;
+  const int64_t nodes = std::max(a.n_targets, a.n_sources), limit = int64_t(1) << 32;
+  const bool near = nodes <= (int64_t(1) << 24) && nodes * w.row_bytes < limit;
+  switch (shape) {
+    case 0: return rel_launch_shape<R, 4, 2, 2>(pass, a, w, rows, near, stream);
+    case 1: return rel_launch_shape<R, 4, 2, 1>(pass, a, w, rows, near, stream);
+    case 2: return rel_launch_shape<R, 2, 2, 2>(pass, a, w, rows, near, stream);
+    case 3: return rel_launch_shape<R, 2, 1, 1>(pass, a, w, rows, near, stream);
+    case 4: return rel_launch_shape<R, 1, 1, 1>(pass, a, w, rows, near, stream);
+    case 5: return rel_launch_shape<R, 2, 2, 0>(pass, a, w, rows, near, stream);
+    case 6: return rel_launch_shape<R, 1, 1, 0>(pass, a, w, rows, near, stream);
+    case 7: return rel_launch_shape<R, 4, 0, 0>(pass, a, w, rows, near, stream);
+    case 8: return rel_launch_shape<R, 1, 0, 0>(pass, a, w, rows, near, stream);
+    case 9: return rel_launch_shape<R, 0, 2, 2>(pass, a, w, rows, near, stream);
+    default: return rel_launch_shape<R, 0, 1, 1>(pass, a, w, rows, near, stream);
+  }
+}
+
+}  // namespace rel
+}  // namespace gm
