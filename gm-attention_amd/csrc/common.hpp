@@ -79,6 +79,17 @@ __host__ __device__ __forceinline__ int64_t xcd_spread_block(int64_t b, int64_t 
   return (r * 8 + x) * chunk + i % chunk;
 }
 
+// The same, for blocks that walk their grid in a loop: 32-bit divisions.
+__device__ __forceinline__ uint32_t xcd_spread_block32(uint32_t b, uint32_t nb) {
+  const uint32_t chunk = nb >= 256 ? 32 : (nb >= 64 ? nb >> 5 : 1);
+  const uint32_t rounds = nb / (8 * chunk), full = rounds * 8 * chunk, head = (nb - full) & ~7u;
+  if (b < head) return full + b;
+  if (b >= head + full) return b;
+  const uint32_t x = b & 7, i = (b - head) >> 3, k = i / chunk;
+  const uint32_t r = (k & 1) ? rounds - 1 - (k >> 1) : k >> 1;
+  return (r * 8 + x) * chunk + i % chunk;
+}
+
 // xcd_block while its contiguous ranges hold about equal work (every range's
 // CSR entries within a quarter of an eighth of the total), else
 // xcd_spread_block.  `ptr` holds the CSR offsets of the n_items items the

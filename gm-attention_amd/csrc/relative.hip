@@ -7,9 +7,9 @@
 //   ds = alpha (g - T),   dtable[b, h] = sum of ds over the edges of bucket b
 //   dq_i = scale sum_e ds tau k_j,   dk_j = scale sum_e ds conj(tau) q_i
 //
-// The backward reads the forward's weights: a score is formed once.  The pass over
-// the targets walks alpha and g, which lie edge by edge, for T, then writes ds and
-// adds dq and the buckets' sums; the pass over the sources reads ds.  An edge of
+// The backward reads the forward's weights: a score is formed once.  A pass over
+// alpha and g, which lie edge by edge, writes ds and adds the buckets' sums; one over
+// the targets and one over the sources read ds.  An edge of
 // weight zero counts for nothing, whatever its rows and its g hold: so do the edges
 // outside the window.  No atomics between waves: sums are in a fixed order.
 //
@@ -20,6 +20,7 @@
 #include "relative.hpp"
 #include "partial_sum.hpp"
 
+#include <algorithm>
 #include <type_traits>
 
 namespace gm {
@@ -102,28 +103,6 @@ __global__ __launch_bounds__(256) void relative_forward_simple(RelArgs<T, R> a) 
     }
 }
 
-// T of a target and ds of its edges.
-template <typename T, typename R>
-__global__ __launch_bounds__(256) void relative_scores_simple(RelArgs<T, R> a) {
-  const int lane = threadIdx.x & 63;
-  const int64_t i = xcd_block(blockIdx.x, gridDim.x) * kWavesPerBlock + (threadIdx.x >> 6);
-  if (i >= a.n_targets) return;
-  const int H = a.L.H, S = kWave / H, h = lane % H, s = lane / H;
-  const int64_t e0 = a.row_ptr[i], e1 = a.row_ptr[i + 1];
-  T total = T(0);
-  if (s < S)
-    for (int64_t e = e0 + s; e < e1; e += S) {
-      const T w = a.alpha[e * H + h];
-      if (w != T(0)) total += w * a.g[e * H + h];
-    }
-  total = group_sum(total, lane, H, S);
-  if (s < S)
-    for (int64_t e = e0 + s; e < e1; e += S) {
-      const T w = a.alpha[e * H + h];
-      a.ds[e * H + h] = w != T(0) ? w * (a.g[e * H + h] - total) : T(0);
-    }
-}
-
 struct RelColumn {
   int n, h, part, pair;  // pair: the column of the pair's real part
 };
@@ -166,30 +145,154 @@ __global__ __launch_bounds__(256) void relative_rows_simple(RelArgs<T, R> a) {
   }
 }
 
-// ------------------------------------------------------------------- dtable
-// A wave a workgroup over a range of the edges, its bins (buckets, H) in LDS.  The edge
-// slots of a step add one after the other: two may hold edges of one bucket, and a
-// wave's LDS operations are done in order.  Then the rows of bins are added in double.
+// --------------------------------------------------------------------- ds
+// T of a target and ds of its edges, which are added to the wave's bins (buckets, columns) in LDS.  Lanes (edge slot,
+// head) read alpha and g, which lie edge by edge, as whole lines; a wave holds kRelHeld steps of both, so that a row
+// of up to that many (times the waves it is shared by) is read once.  The workgroups are persistent, find their next
+// row while the present one's numbers are on their way, and each writes a row of bins.  Bound by bytes and by how many
+// are on their way: 63 million edges of eight heads take 1.47 ms, 5.3 GB from and to memory (3.6 TB/s).
+// Holding 16 steps takes as long, 8 takes 5 % more: long rows are read twice.
+//
+// A bin is a slot's own, added to in the order of its steps, while the bins take up to kRelBins bytes a wave; of more
+// buckets several slots share one and add one after the other (a wave's LDS operations are done in order): two of them
+// may hold edges of one bucket.  A read, an add and a write, not LDS's atomic add: that takes a cycle a lane (2.9 ms
+// against 1.9, before the loads of a row were all requested together).
 
-template <typename T, typename R>
-__global__ __launch_bounds__(64) void relative_table_simple(RelArgs<T, R> a) {
+constexpr int kRelHeld = 12;
+constexpr int kRelBins = 8 * 1024;
+
+template <typename T>
+struct RelScores {
+  int H, S, buckets, shares;  // shares: the slots that add to one bin
+  const int64_t* row_ptr;
+  const int32_t* order;       // the rows by length, or null: as they come
+  uint32_t shared, rows;      // the first `shared` are a workgroup's each, the others a wave's
+  const uint8_t* bucket;      // (n_edges)
+  const T* alpha;
+  const T* g;
+  T* ds;
+  T* partial;
+};
+
+// `count` numbers from p as a buffer: what is read past them is zero, what is written there is dropped.
+template <typename T>
+__device__ __forceinline__ __amdgpu_buffer_rsrc_t rel_span(const T* p, int count) {
+  return __builtin_amdgcn_make_buffer_rsrc(const_cast<T*>(p), (short)0, count * (int)sizeof(T), 0x00020000);
+}
+typedef uint32_t rel_u2 __attribute__((ext_vector_type(2)));
+template <typename T>
+__device__ __forceinline__ T rel_read(__amdgpu_buffer_rsrc_t r, int off) {
+  if constexpr (sizeof(T) == 8)
+    return __builtin_bit_cast(T, __builtin_amdgcn_raw_buffer_load_b64(r, off, 0, 0));
+  else
+    return __builtin_bit_cast(T, __builtin_amdgcn_raw_buffer_load_b32(r, off, 0, 0));
+}
+template <typename T>
+__device__ __forceinline__ void rel_write(T v, __amdgpu_buffer_rsrc_t r, int off) {
+  if constexpr (sizeof(T) == 8)
+    __builtin_amdgcn_raw_buffer_store_b64(__builtin_bit_cast(rel_u2, v), r, off, 0, 0);
+  else
+    __builtin_amdgcn_raw_buffer_store_b32(__builtin_bit_cast(uint32_t, v), r, off, 0, 0);
+}
+
+template <typename T>
+__global__ __launch_bounds__(256) void relative_scores(RelScores<T> a, uint32_t blocks) {
   extern __shared__ __align__(16) char rel_lds[];
-  T* bins = reinterpret_cast<T*>(rel_lds);
-  const int lane = threadIdx.x, H = a.L.H, S = kWave / H, h = lane % H, s = lane / H;
-  for (int i = lane; i < a.buckets * H; i += kWave) bins[i] = T(0);
-  __syncthreads();
-  const int64_t per = ((a.n_edges + gridDim.x - 1) / gridDim.x + S - 1) / S * S;
-  const int64_t e0 = (int64_t)blockIdx.x * per, e1 = e0 + per < a.n_edges ? e0 + per : a.n_edges;
-  for (int64_t e = e0; e < e1; e += S) {
-    const bool live = s < S && e + s < e1;
-    const T v = live ? a.ds[(e + s) * H + h] : T(0);
-    const int at = live ? rel_bucket(a.records + (e + s) * 2 * a.L.orders) * H + h : 0;
-    for (int t = 0; t < S; ++t) {
-      if (s == t && live) bins[at] += v;
-      __syncthreads();  // one wave: its LDS reads after its writes
+  const int lane = threadIdx.x & 63, wave = uniform((int)(threadIdx.x >> 6)), H = a.H, S = a.S;
+  const int s = lane / H, h = lane % H;
+  const bool on = s < S;
+  T* shared = reinterpret_cast<T*>(rel_lds);  // (waves, H): a row's waves' parts of T
+  T* all = shared + kWavesPerBlock * H;
+  const int columns = (S + a.shares - 1) / a.shares * H, size = a.buckets * columns;
+  T* bins = all + wave * size;
+  T* bin = bins + (on ? s / a.shares * H + h : 0);
+  const int turn = s % a.shares;
+  const int step = S * H * (int)sizeof(T);                         // a step's bytes
+  const int mine = on ? lane * (int)sizeof(T) : (int)0xC0000000u;  // past every span
+  for (int i = lane; i < size; i += kWave) bins[i] = T(0);
+  __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+  __builtin_amdgcn_wave_barrier();
+  // the edges of this wave in a block's row (whole: of the workgroup's); none where the wave has no row
+  struct Range {
+    int64_t e0, e1;
+  };
+  auto range = [&](uint32_t block) {
+    if (block >= blocks) return Range{0, 0};
+    const bool whole = block < a.shared;
+    const uint32_t at = whole ? xcd_spread_block32(block, a.shared)
+                              : a.shared + xcd_spread_block32(block - a.shared, blocks - a.shared) * kWavesPerBlock + wave;
+    if (at >= a.rows) return Range{0, 0};
+    const uint32_t row = a.order ? uniform((int)a.order[at]) : at;
+    const int64_t r0 = uniform(a.row_ptr[row]), r1 = uniform(a.row_ptr[row + 1]);
+    if (!whole) return Range{r0, r1};
+    const uint32_t steps = ((uint32_t)(r1 - r0) + S - 1) / S, per = (steps + kWavesPerBlock - 1) / kWavesPerBlock * S;
+    const int64_t first = r0 + (int64_t)wave * per, e0 = first < r1 ? first : r1;
+    return Range{e0, e0 + per < r1 ? e0 + per : r1};
+  };
+  Range next = range(blockIdx.x);
+  for (uint32_t block = blockIdx.x; block < blocks; block += gridDim.x) {
+    const bool whole = block < a.shared;
+    const int64_t e0 = next.e0, e1 = next.e1;
+    next = range(block + gridDim.x);  // found while this row's numbers are on their way
+    T al[kRelHeld], g[kRelHeld];
+    int b[kRelHeld];
+    // the steps from edge e; what lies past the row's share (and lanes without a head) reads as zero
+    auto read = [&](int64_t e) {
+      const int left = (int)(e1 - e < kRelHeld * S ? e1 - e : kRelHeld * S);
+      const auto al_of = rel_span(a.alpha + e * H, left * H), g_of = rel_span(a.g + e * H, left * H);
+      const auto b_of = rel_span(a.bucket + e, left);
+#pragma unroll
+      for (int n = 0; n < kRelHeld; ++n) {
+        al[n] = rel_read<T>(al_of, mine + n * step);
+        g[n] = rel_read<T>(g_of, mine + n * step);
+        b[n] = __builtin_amdgcn_raw_buffer_load_b8(b_of, s + n * S, 0, 0);
+      }
+    };
+    const bool once = e1 - e0 <= kRelHeld * S;
+    T total = T(0);
+    for (int64_t e = e0; e < e1; e += kRelHeld * S) {
+      read(e);
+#pragma unroll
+      for (int n = 0; n < kRelHeld; ++n) total += al[n] != T(0) ? al[n] * g[n] : T(0);
+    }
+    total = group_sum(total, lane, H, S);
+    if (whole) {
+      __syncthreads();
+      if (lane < H) shared[wave * H + lane] = total;
+      __syncthreads();
+      total = shared[h];
+      for (int o = 1; o < kWavesPerBlock; ++o) total += shared[o * H + h];
+    }
+    for (int64_t e = e0; e < e1; e += kRelHeld * S) {
+      if (!once) read(e);
+      const int left = (int)(e1 - e < kRelHeld * S ? e1 - e : kRelHeld * S);
+      const auto ds_of = rel_span(a.ds + e * H, left * H);
+#pragma unroll
+      for (int n = 0; n < kRelHeld; ++n) {
+        if (n * S < left) {
+          const T d = al[n] != T(0) ? al[n] * (g[n] - total) : T(0);
+          rel_write(d, ds_of, mine + n * step);
+          T* to = bin + b[n] * columns;
+          if (a.shares == 1) {
+            if (on) *to += d;  // this lane's alone
+          } else {
+            for (int o = 0; o < a.shares; ++o) {
+              if (on && turn == o) *to += d;
+              wave_lds();
+            }
+          }
+        }
+      }
     }
   }
-  for (int i = lane; i < a.buckets * H; i += kWave) a.partial[(int64_t)blockIdx.x * a.buckets * H + i] = bins[i];
+  __syncthreads();
+  for (int i = threadIdx.x; i < a.buckets * H; i += blockDim.x) {
+    const int bucket = i / H, head = i % H;
+    T v = T(0);
+    for (int w = 0; w < kWavesPerBlock; ++w)
+      for (int c = head; c < columns; c += H) v += all[w * size + bucket * columns + c];
+    a.partial[(int64_t)blockIdx.x * a.buckets * H + i] = v;
+  }
 }
 
 // ------------------------------------------------------------------- launch
@@ -274,10 +377,44 @@ int relative_forward(const R* q, const R* k, const T* table, const T* records, c
   return check_launch("relative_forward");
 }
 
+// ds of every edge, and the sums of its buckets.
+template <typename T, typename R>
+int relative_scores_launch(const RelArgs<T, R>& a, const RelRows& rows, const uint8_t* bucket, T* dtable,
+                           hipStream_t stream) {
+  RelScores<T> k{};
+  k.H = a.L.H;
+  k.S = kWave / a.L.H;
+  k.buckets = a.buckets;
+  for (k.shares = 1; k.shares < k.S; k.shares *= 2)
+    if ((size_t)a.buckets * ((k.S + k.shares - 1) / k.shares) * a.L.H * sizeof(T) <= kRelBins) break;
+  k.shares = std::min(k.shares, k.S);
+  k.row_ptr = a.row_ptr;
+  k.order = rows.order;
+  k.shared = rows.order ? (uint32_t)(rows.count[0] + rows.count[1]) : 0;
+  k.rows = (uint32_t)a.n_targets;
+  k.bucket = bucket;
+  k.alpha = a.alpha;
+  k.g = a.g;
+  k.ds = a.ds;
+  k.partial = a.partial;
+  const int columns = (k.S + k.shares - 1) / k.shares * a.L.H;
+  const size_t lds = sizeof(T) * kWavesPerBlock * ((size_t)a.L.H + (size_t)a.buckets * columns);
+  const auto kernel = &relative_scores<T>;
+  if (lds > 64 * 1024 && hipFuncSetAttribute(reinterpret_cast<const void*>(kernel),
+                                             hipFuncAttributeMaxDynamicSharedMemorySize, 160 * 1024) != hipSuccess)
+    return check_launch("relative (LDS)");
+  const int64_t blocks = k.shared + blocks_for(a.n_targets - k.shared);
+  const int64_t resident = resident_blocks(reinterpret_cast<const void*>(kernel), 256, lds);
+  const int64_t grid = std::max<int64_t>(1, std::min({blocks, (int64_t)kRelTableRows, resident > 0 ? resident : blocks}));
+  hipLaunchKernelGGL(kernel, dim3((unsigned)grid), dim3(256), lds, stream, k, (uint32_t)blocks);
+  launch_partial_sum<T>(a.partial, grid, a.buckets * a.L.H, dtable, stream);
+  return check_launch("relative_scores");
+}
+
 template <typename T, typename R>
 int relative_backward(const T* g, const T* alpha, const R* q, const R* k, const T* records, const T* records_s,
-                      const int64_t* desc, const int64_t* row_ptr, const int64_t* src_ptr, const int32_t* order,
-                      const int64_t* counts, const int32_t* order_s, const int64_t* counts_s, int64_t n_targets,
+                      const uint8_t* bucket, const int64_t* desc, const int64_t* row_ptr, const int64_t* src_ptr,
+                      const int32_t* order, const int64_t* counts, const int32_t* order_s, const int64_t* counts_s, int64_t n_targets,
                       int64_t n_sources, int64_t n_edges, int64_t D, int64_t orders, int64_t F, int64_t H,
                       int64_t buckets, double scale, T* ds, T* partial, R* dq, R* dk, T* dtable, void* stream) {
   RelArgs<T, R> a{};
@@ -287,7 +424,8 @@ int relative_backward(const T* g, const T* alpha, const R* q, const R* k, const 
   GM_REQUIRE(partial && dtable, "partial and dtable must be device pointers");
   if (n_targets > 0) GM_REQUIRE(dq, "dq must be a device pointer");
   if (n_sources > 0) GM_REQUIRE(src_ptr && dk, "src_ptr and dk must be device pointers");
-  if (n_edges > 0) GM_REQUIRE(g && alpha && ds && records_s, "g, alpha, ds and the sources' records must be device pointers");
+  if (n_edges > 0) GM_REQUIRE(g && alpha && ds && records_s && bucket,
+                              "g, alpha, ds, the sources' records and the buckets must be device pointers");
   a.g = g;
   a.alpha = const_cast<T*>(alpha);  // read only here
   a.records_s = records_s;
@@ -297,30 +435,23 @@ int relative_backward(const T* g, const T* alpha, const R* q, const R* k, const 
   a.dq = dq;
   a.dk = dk;
   const hipStream_t s = (hipStream_t)stream;
-  const int columns = a.buckets * a.L.H;
   GM_REQUIRE(!order == !order_s || n_targets == 0 || n_sources == 0, "both sides' rows are in classes, or neither's");
   RelRows targets, sources;
   int status = rel_rows(a, order, counts, n_targets, targets);
   if (status == GM_OK) status = rel_rows(a, order_s, counts_s, n_sources, sources);
   if (status != GM_OK) return status;
+  status = relative_scores_launch(a, targets, bucket, dtable, s);
+  if (status != GM_OK) return status;
   if constexpr (std::is_same<T, float>::value) {
     if (order || order_s) {
       status = rel_launch_units(RelPass::BackwardTarget, a, targets, s);
-      if (status == GM_OK) status = rel_launch_units(RelPass::BackwardSource, a, sources, s);
-      if (status != GM_OK) return status;
-      launch_partial_sum<T>(partial, kRelTableRows, columns, dtable, s);
-      return check_launch("relative_backward");
+      return status == GM_OK ? rel_launch_units(RelPass::BackwardSource, a, sources, s) : status;
     }
   }
-  if (n_targets > 0) {
-    const dim3 grid((unsigned)blocks_for(n_targets));
-    hipLaunchKernelGGL((relative_scores_simple<T, R>), grid, dim3(256), 0, s, a);
-    hipLaunchKernelGGL((relative_rows_simple<T, R, true>), grid, dim3(256), 0, s, a);
-  }
+  if (n_targets > 0)
+    hipLaunchKernelGGL((relative_rows_simple<T, R, true>), dim3((unsigned)blocks_for(n_targets)), dim3(256), 0, s, a);
   if (n_sources > 0)
     hipLaunchKernelGGL((relative_rows_simple<T, R, false>), dim3((unsigned)blocks_for(n_sources)), dim3(256), 0, s, a);
-  hipLaunchKernelGGL((relative_table_simple<T, R>), dim3(kRelTableRows), dim3(kWave), sizeof(T) * columns, s, a);
-  launch_partial_sum<T>(partial, kRelTableRows, columns, dtable, s);
   return check_launch("relative_backward");
 }
 
@@ -349,12 +480,12 @@ extern "C" int gm_relative_slots(const int64_t* desc, int64_t F, int64_t H, int6
                                       n_edges, D, orders, F, H, buckets, scale, alpha, stream);                       \
   }                                                                                                                   \
   extern "C" int gm_relative_backward_##SFX(                                                                          \
-      const T* g, const T* alpha, const R* q, const R* k, const T* records, const T* records_s, const int64_t* desc,  \
-      const int64_t* row_ptr, const int64_t* src_ptr, const int32_t* order, const int64_t* counts,                    \
-      const int32_t* order_s, const int64_t* counts_s, int64_t n_targets, int64_t n_sources, int64_t n_edges,         \
+      const T* g, const T* alpha, const R* q, const R* k, const T* records, const T* records_s,                       \
+      const uint8_t* bucket, const int64_t* desc, const int64_t* row_ptr, const int64_t* src_ptr,                     \
+      const int32_t* order, const int64_t* counts, const int32_t* order_s, const int64_t* counts_s, int64_t n_targets, int64_t n_sources, int64_t n_edges,         \
       int64_t D, int64_t orders, int64_t F, int64_t H, int64_t buckets, double scale, T* ds, T* partial, R* dq,       \
       R* dk, T* dtable, void* stream) {                                                                               \
-    return gm::relative_backward<T, R>(g, alpha, q, k, records, records_s, desc, row_ptr, src_ptr, order, counts,     \
+    return gm::relative_backward<T, R>(g, alpha, q, k, records, records_s, bucket, desc, row_ptr, src_ptr, order, counts,     \
                                        order_s, counts_s, n_targets, n_sources, n_edges, D, orders, F, H, buckets,    \
                                        scale, ds, partial, dq, dk, dtable, stream);                                   \
   }

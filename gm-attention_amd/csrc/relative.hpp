@@ -64,7 +64,7 @@ __device__ __forceinline__ int rel_index(const double* word) {
   return (int)*reinterpret_cast<const int64_t*>(word);
 }
 
-constexpr int kRelTableRows = 1024;  // rows of sums of ds by bucket that the backward adds
+constexpr int kRelTableRows = 2048;  // rows of sums of ds by bucket that the backward adds
 
 // The lane kernels (relative_units.hip).
 enum class RelPass { Forward, BackwardTarget, BackwardSource };

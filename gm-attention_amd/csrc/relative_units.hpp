@@ -279,208 +279,80 @@ __global__ __launch_bounds__(1024) void relative_forward_units(RelArgs<float, R>
 
 // ---------------------------------------------------------------- backward
 
-// Per target: T = sum alpha g over its edges, then ds = alpha (g - T), written, added to the wave's bins (buckets,
-// columns) in LDS and to dq = scale sum ds tau k.  A workgroup takes rows until none is left and writes its bins.
-template <typename R, typename U, bool kNear, bool kPair>
-__global__ __launch_bounds__(kRelThreadsB) void relative_backward_target_units(RelArgs<float, R> a, EdgeUnits w,
-                                                                               int64_t blocks, int spread) {
-  constexpr int kWords = kWave * U::RW, UN = 2;
+// Per target or per source (kTargets or not): dq = scale sum ds tau k over a target's edges, dk = scale sum ds conj(tau) q
+// over a source's, its edges sorted by source.
+template <typename R, typename U, bool kNear, bool kTargets>
+__global__ __launch_bounds__(kRelThreadsB) void relative_rows_units(RelArgs<float, R> a, EdgeUnits w, int64_t blocks) {
+  constexpr int kWords = kWave * U::RW, kTogether = U::N > 12 ? 2 : 4;  // steps whose rows are requested together
   extern __shared__ __align__(16) float rel_lds[];
-  const int lane = threadIdx.x & 63, wave = uniform((int)(threadIdx.x >> 6)), H = a.L.H;
-  float* rec = rel_lds + wave * kWords;
-  float* shared = rel_lds + kWavesPerBlock * kWords;  // the waves' sums: (waves, max(N lanes, 64))
-  const int sums_words = kWavesPerBlock * std::max(U::N * w.lanes, kWave);
-  // a bin for every lane that holds a step, or one for those of all slots
-  const int per_slot = H * (kPair ? 2 : 1), columns = per_slot * (spread ? w.slots : 1);
-  float* bins = shared + sums_words + wave * a.buckets * columns;
-  const int u = lane & (w.lanes - 1), s = lane >> w.shift, unit = u < w.units ? u : w.units - 1;
-  const int h = unit / w.per_map, own = unit % w.per_map;
-  const bool odd = kPair && (own & 1), mine_too = u < w.units && own < (kPair ? 2 : 1);
-  const float* mine = rec + s * U::RW;
-  float* bin = bins + (spread ? s * per_slot : 0) + h * (kPair ? 2 : 1) + odd;
-  for (int i = lane; i < a.buckets * columns; i += kWave) bins[i] = 0.f;
-  wave_lds();
-
-  for (int64_t block = blockIdx.x; block < blocks; block += gridDim.x) {
-    const Share sh = rel_share(w, a.row_ptr, block, blocks);
-    if (!sh.live) continue;  // one wave a row, or the whole workgroup
-    const float* alpha = a.alpha + sh.e0 * H + h;
-    const float* grad = a.g + sh.e0 * H + h;
-    const int count = (int)(sh.e1 - sh.e0);
-    float total = 0.f;
-    for (int t = 0; t < sh.steps; t += kPair ? 2 : 1) {
-      const int e = (t + odd) * w.slots + s;
-      if (mine_too && e < count) {
-        const float al = alpha[(int64_t)e * H];
-        if (al != 0.f) total = fmaf(al, grad[(int64_t)e * H], total);
-      }
-    }
-    for (int o = w.lanes; o < kWave; o <<= 1) total += __shfl_xor(total, o, kWave);
-    if constexpr (kPair) {  // the lanes that hold steps, to all of a head's
-      total += next_lane(total);
-      total = __shfl(total, lane & ~(w.per_map - 1), kWave);
-    }
-    if constexpr (!kPair) total = __shfl(total, lane & ~(w.per_map - 1), kWave);
-    if (sh.parts > 1) {
-      __syncthreads();
-      shared[sh.wave * kWave + lane] = total;
-      __syncthreads();
-      total = shared[lane];
-      for (int o = 1; o < sh.parts; ++o) total += shared[o * kWave + lane];
-    }
-    float sums[U::N];
-#pragma unroll
-    for (int i = 0; i < U::N; ++i) sums[i] = 0.f;
-    Records<U::RW> records;
-    if (sh.steps > 0) records.request(a.records, sh.e0, sh.e1, lane);
-    for (int b = 0; b < sh.steps; b += w.lanes) {
-      const int64_t e = sh.e0 + (int64_t)b * w.slots;  // the batch's first edge
-      wave_lds();
-      records.put(rec, lane);
-      wave_lds();
-      if (b + w.lanes < sh.steps) records.request(a.records, e + kWave, sh.e1, lane);
-      const int ends = sh.steps - b < w.lanes ? sh.steps - b : w.lanes;
-      const int left = (int)(sh.e1 - e < kWave ? sh.e1 - e : kWave);
-      const float* al_of = a.alpha + e * H + h;
-      const float* g_of = a.g + e * H + h;
-      float* ds_of = a.ds + e * H + h;
-      for (int t = 0; t < ends; t += UN) {
-        float k[UN][U::N], cs[UN][U::NA], sn[UN][U::NA], d[UN];
-        uint32_t word[UN];
-#pragma unroll
-        for (int n = 0; n < UN; ++n) {
-          const float* r = mine + (t + n) * w.slots * U::RW;
-          word[n] = *reinterpret_cast<const uint32_t*>(r);
-#pragma unroll
-          for (int o = 0; o < U::NO; ++o) {
-            const float2 x = *reinterpret_cast<const float2*>(r + 2 + 2 * o);
-            cs[n][o] = x.x;
-            sn[n][o] = x.y;
-          }
-        }
-#pragma unroll
-        for (int n = 0; n < UN; ++n) U::template load<kNear>(a.k, w, unit, (int)(word[n] & 0xFFFFFF), k[n]);
-        auto weigh = [&](int n) {  // ds of step t + n, written and added to its bin by the lane that holds it
-          const int at = (t + n) * w.slots + s;
-          float ds = 0.f;
-          if (at < left) {
-            const float al = al_of[(uint32_t)(at * H)];
-            if (al != 0.f) ds = al * (g_of[(uint32_t)(at * H)] - total);
-          }
-          return ds;
-        };
-        auto keep = [&](int n, float ds, uint32_t bucket) {
-          const int at = (t + n) * w.slots + s;
-          const bool live = mine_too && at < left;
-          if (live) ds_of[(uint32_t)(at * H)] = ds;
-          float* to = bin + bucket * columns;
-          if (spread) {
-            if (live) atomicAdd(to, ds);  // this lane's own: in the order of its steps
-          } else {
-            for (int o = 0; o < w.slots; ++o) {  // slot by slot: a wave's LDS operations are done in order
-              if (live && s == o) atomicAdd(to, ds);
-              __builtin_amdgcn_wave_barrier();
-            }
-          }
-        };
-        if constexpr (kPair) {
-          const float ds = odd ? weigh(1) : weigh(0);
-          keep(odd, ds, (odd ? word[1] : word[0]) >> 24);
-          const float other = next_lane(ds);
-          d[0] = odd ? other : ds;
-          d[1] = odd ? ds : other;
-        } else {
-#pragma unroll
-          for (int n = 0; n < UN; ++n) {
-            d[n] = weigh(n);
-            keep(n, d[n], word[n] >> 24);
-          }
-        }
-#pragma unroll
-        for (int n = 0; n < UN; ++n)
-          if (d[n] != 0.f) U::add(sums, d[n], k[n], cs[n], sn[n], false);
-      }
-    }
-    row_sums<U::N>(w, sh, sums, shared);
-    if (sh.part == 0 && s == 0 && u < w.units) {
-#pragma unroll
-      for (int i = 0; i < U::N; ++i) sums[i] *= a.gradient_scale;
-      U::store(a.dq + (int64_t)sh.row * a.L.D, w, unit, sums);
-    }
-  }
-  // the workgroup's bins: a head's lanes of every slot and wave, in order
-  __syncthreads();
-  float* first = shared + sums_words;
-  for (int i = threadIdx.x; i < a.buckets * H; i += blockDim.x) {
-    const int bucket = i / H, head = i % H;
-    float v = 0.f;
-    for (int wv = 0; wv < kWavesPerBlock; ++wv)
-      for (int sl = 0; sl < (spread ? w.slots : 1); ++sl)
-        for (int o = 0; o < (kPair ? 2 : 1); ++o)
-          v += first[((size_t)wv * a.buckets + bucket) * columns + sl * per_slot + head * (kPair ? 2 : 1) + o];
-    a.partial[((int64_t)blockIdx.x * a.buckets + bucket) * H + head] = v;
-  }
-}
-
-// Per source, over the edges sorted by source: dk = scale sum ds conj(tau) q.
-template <typename R, typename U, bool kNear, bool kPair>
-__global__ __launch_bounds__(kRelThreadsB) void relative_backward_source_units(RelArgs<float, R> a, EdgeUnits w,
-                                                                               int64_t blocks) {
-  constexpr int kWords = kWave * U::RW, UN = kRelInFlight;
-  extern __shared__ __align__(16) float rel_lds[];
-  const Share sh = rel_share(w, a.src_ptr, blockIdx.x, blocks);
+  const Share sh = rel_share(w, kTargets ? a.row_ptr : a.src_ptr, blockIdx.x, blocks);
   if (!sh.live) return;
   const int lane = threadIdx.x & 63, H = a.L.H;
   float* rec = rel_lds + sh.wave * kWords;
   const int u = lane & (w.lanes - 1), s = lane >> w.shift, unit = u < w.units ? u : w.units - 1;
   const int h = unit / w.per_map;
   const float* mine = rec + s * U::RW;
+  const float* records_of = kTargets ? a.records : a.records_s;
   float sums[U::N];
 #pragma unroll
   for (int i = 0; i < U::N; ++i) sums[i] = 0.f;
   Records<U::RW> records;
-  if (sh.steps > 0) records.request(a.records_s, sh.e0, sh.e1, lane);
+  if (sh.steps > 0) records.request(records_of, sh.e0, sh.e1, lane);
   for (int b = 0; b < sh.steps; b += w.lanes) {
     const int64_t e = sh.e0 + (int64_t)b * w.slots;
     wave_lds();
     records.put(rec, lane);
     wave_lds();
-    if (b + w.lanes < sh.steps) records.request(a.records_s, e + kWave, sh.e1, lane);
+    if (b + w.lanes < sh.steps) records.request(records_of, e + kWave, sh.e1, lane);
     const int ends = sh.steps - b < w.lanes ? sh.steps - b : w.lanes;
     const int left = (int)(sh.e1 - e < kWave ? sh.e1 - e : kWave);
-    for (int t = 0; t < ends; t += UN) {
+    const float* ds_of = a.ds + e * H;
+    auto take = [&](int t, auto group) {
+      constexpr int UN = decltype(group)::value;
       float2 head[UN];
-      float q[UN][U::N], cs[UN][U::NA], sn[UN][U::NA], d[UN];
+      float x[UN][U::N], cs[UN][U::NA], sn[UN][U::NA], d[UN];
+      bool in[UN];
 #pragma unroll
       for (int n = 0; n < UN; ++n) {
         const float* r = mine + (t + n) * w.slots * U::RW;
         head[n] = *reinterpret_cast<const float2*>(r);
-        // past the row (and the batch's last step): node 0's row, edge 0's ds, not counted
-        const bool in = (t + n) * w.slots + s < left;
-        head[n].x = in ? head[n].x : 0.f;
-        head[n].y = in ? head[n].y : 0.f;
+        // past the row (and the batch's last step): node 0's row, the first edge's ds, not counted
+        in[n] = (t + n) * w.slots + s < left;
+        if constexpr (!kTargets) {
+          head[n].x = in[n] ? head[n].x : 0.f;
+          head[n].y = in[n] ? head[n].y : 0.f;
+        }
 #pragma unroll
         for (int o = 0; o < U::NO; ++o) {
-          const float2 x = *reinterpret_cast<const float2*>(r + 2 + 2 * o);
-          cs[n][o] = x.x;
-          sn[n][o] = x.y;
+          const float2 p = *reinterpret_cast<const float2*>(r + 2 + 2 * o);
+          cs[n][o] = p.x;
+          sn[n][o] = p.y;
         }
       }
 #pragma unroll
       for (int n = 0; n < UN; ++n) {
-        d[n] = a.ds[(int64_t)__float_as_int(head[n].y) * H + h];
-        U::template load<kNear>(a.q, w, unit, __float_as_int(head[n].x), q[n]);
+        if constexpr (kTargets) {
+          d[n] = ds_of[(uint32_t)((in[n] ? (t + n) * w.slots + s : 0) * H + h)];
+          U::template load<kNear>(a.k, w, unit, __float_as_int(head[n].x) & 0xFFFFFF, x[n]);
+        } else {
+          d[n] = a.ds[(int64_t)__float_as_int(head[n].y) * H + h];
+          U::template load<kNear>(a.q, w, unit, __float_as_int(head[n].x), x[n]);
+        }
       }
 #pragma unroll
       for (int n = 0; n < UN; ++n)
-        if ((t + n) * w.slots + s < left && d[n] != 0.f) U::add(sums, d[n], q[n], cs[n], sn[n], true);
-    }
+        if (in[n] && d[n] != 0.f) U::add(sums, d[n], x[n], cs[n], sn[n], !kTargets);
+    };
+    int t = 0;
+    for (; t + kTogether <= ends; t += kTogether) take(t, std::integral_constant<int, kTogether>());
+    for (; t + 2 <= ends; t += 2) take(t, std::integral_constant<int, 2>());
+    if (t < ends) take(t, std::integral_constant<int, 1>());
   }
   row_sums<U::N>(w, sh, sums, rel_lds);
   if (sh.part == 0 && s == 0 && u < w.units) {
 #pragma unroll
     for (int i = 0; i < U::N; ++i) sums[i] *= a.gradient_scale;
-    U::store(a.dk + (int64_t)sh.row * a.L.D, w, unit, sums);
+    U::store((kTargets ? a.dq : a.dk) + (int64_t)sh.row * a.L.D, w, unit, sums);
   }
 }
 
@@ -526,11 +398,7 @@ size_t rel_forward_lds(int waves, bool pair, int steps, int table) {
                           table);
 }
 template <typename U>
-size_t rel_target_lds(int lanes, int bins) {
-  return sizeof(float) * kWavesPerBlock * ((size_t)kWave * U::RW + std::max(U::N * lanes, kWave) + bins);
-}
-template <typename U>
-size_t rel_source_lds(int lanes) {
+size_t rel_rows_lds(int lanes) {
   return sizeof(float) * kWavesPerBlock * (size_t)std::max(kWave * U::RW, U::N * lanes);
 }
 
@@ -571,23 +439,13 @@ int rel_launch(RelPass pass, const RelArgs<float, R>& a, EdgeUnits w, const RelR
   w.shared = rows.count[0] + rows.count[1];
   w.single = rows.count[2];
   const int64_t blocks = w.shared + blocks_for(w.single);
-  if (pass == RelPass::BackwardTarget) {
-    const auto kernel = &relative_backward_target_units<R, U, kNear, kPair>;
-    const int bins = a.buckets * a.L.H * (kPair ? 2 : 1), spread = bins * w.slots <= 2048 ? 1 : 0;
-    const size_t lds = rel_target_lds<U>(w.lanes, bins * (spread ? w.slots : 1));
-    const int rc = rel_lds_limit(reinterpret_cast<const void*>(kernel), lds);
-    if (rc != GM_OK) return rc;
-    // every workgroup writes a row of bins, those without a row of their own too
-    hipLaunchKernelGGL(kernel, dim3(kRelTableRows), dim3(kRelThreadsB), lds, stream, a, w, blocks, spread);
-    return check_launch("relative");
-  }
-  if (blocks > 0) {
-    const auto kernel = &relative_backward_source_units<R, U, kNear, kPair>;
-    const size_t lds = rel_source_lds<U>(w.lanes);
-    const int rc = rel_lds_limit(reinterpret_cast<const void*>(kernel), lds);
-    if (rc != GM_OK) return rc;
-    hipLaunchKernelGGL(kernel, dim3((unsigned)blocks), dim3(kRelThreadsB), lds, stream, a, w, blocks);
-  }
+  if (blocks == 0) return GM_OK;
+  const auto kernel = pass == RelPass::BackwardTarget ? &relative_rows_units<R, U, kNear, true>
+                                                      : &relative_rows_units<R, U, kNear, false>;
+  const size_t lds = rel_rows_lds<U>(w.lanes);
+  const int rc = rel_lds_limit(reinterpret_cast<const void*>(kernel), lds);
+  if (rc != GM_OK) return rc;
+  hipLaunchKernelGGL(kernel, dim3((unsigned)blocks), dim3(kRelThreadsB), lds, stream, a, w, blocks);
   return check_launch("relative");
 }
 

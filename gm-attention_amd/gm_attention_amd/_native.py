@@ -123,7 +123,7 @@ SIGNATURES_F32 = {
     "gm_relative_slots": (ctypes.c_int, [_P] + [_I] * 4 + [_P]),
     **{f"gm_relative_forward_{sfx}": (ctypes.c_int, [_P] * 8 + [_I] * 8 + [_D] + [_P] * 2)
        for sfx in ("f32", "f64", "bf16")},
-    **{f"gm_relative_backward_{sfx}": (ctypes.c_int, [_P] * 13 + [_I] * 8 + [_D] + [_P] * 6)
+    **{f"gm_relative_backward_{sfx}": (ctypes.c_int, [_P] * 14 + [_I] * 8 + [_D] + [_P] * 6)
        for sfx in ("f32", "f64", "bf16")},
     "gm_head_norm_partial_rows": (ctypes.c_int64, [_I]),
     **{f"gm_head_norm_forward_{sfx}": (ctypes.c_int, [_P] * 3 + [_I, _P] + [_I] * 4 + [_P] * 2 + [_I] * 2 + [_D] +
@@ -1767,9 +1767,9 @@ def relative_backward(g: Tensor, alpha: Tensor, q: Tensor, k: Tensor, tables: An
     dq, dk = torch.empty_like(q), torch.empty_like(k)
     dtable = torch.empty(tables.n_buckets, H, dtype=g.dtype, device=device)
     _call_on(device, "gm_relative_backward_" + _PW_SUFFIX[q.dtype], _ptr(g), _ptr(alpha), _ptr(q), _ptr(k),
-             _ptr(tables.records), _ptr(records_s), desc.data_ptr(), _ptr(tables.row_ptr), _ptr(src_ptr), _ptr(order),
-             counts, _ptr(order_s), counts_s, tables.n_targets, tables.n_sources, tables.n_edges, q.shape[1],
-             tables.orders, desc.shape[0], H, tables.n_buckets, scale, _ptr(ds), _ptr(partial), _ptr(dq), _ptr(dk),
+             _ptr(tables.records), _ptr(records_s), _ptr(tables.buckets), desc.data_ptr(), _ptr(tables.row_ptr),
+             _ptr(src_ptr), _ptr(order), counts, _ptr(order_s), counts_s, tables.n_targets, tables.n_sources,
+             tables.n_edges, q.shape[1], tables.orders, desc.shape[0], H, tables.n_buckets, scale, _ptr(ds), _ptr(partial), _ptr(dq), _ptr(dk),
              _ptr(dtable), _stream(device))
     return dq, dk, dtable
 

@@ -68,25 +68,24 @@ class RelativeEdgeTables(EdgeTables):
         if transport.dtype == torch.float32 and nodes > MAX_SOURCES:
             raise ValueError(f"float32 tables hold at most {MAX_SOURCES} sources, got {nodes}.")
         self.n_buckets = int(n_buckets)
-        self._buckets = buckets.detach().long()
+        self.buckets = buckets.detach().to(torch.uint8, copy=True)
         super().__init__(row_ptr, source, transport, bias, inside, n_sources=n_sources)
 
     def _hold(self, source: Tensor, phases: Tensor, masked: Tensor) -> None:
         super()._hold(source, phases, masked)
         if self.device.type == "cuda":
-            del self._buckets  # in the records
+            self._kept.append(_native.Made(self.buckets))
 
     def __setstate__(self, state: dict) -> None:
-        if "records" in state and state["row_ptr"].device.type != "cuda":
-            word = state["records"].view(differential._WORD[state["dtype"]])[:, 0].long()
-            buckets = (word >> 24) & 0xFF if state["dtype"] == torch.float32 else word >> 32
-            state = dict(state, _buckets=buckets)
         super().__setstate__(state)
+        if self.device.type == "cuda" and "records" in state:
+            self._kept.append(_native.Made(self.buckets))
 
     def _packed(self, source: Tensor) -> Tensor:
+        buckets = self.buckets.long()
         if self.dtype == torch.float64:
-            return source + (self._buckets << 32)
-        word = source + (self._buckets << 24)
+            return source + (buckets << 32)
+        word = source + (buckets << 24)
         return torch.where(word >= 2**31, word - 2**32, word)  # the same 32 bits
 
     def _unpacked(self, records: Tensor) -> Tensor:
@@ -238,7 +237,7 @@ def attention_weights(mhsa: Any, q: Tensor, k: Tensor, edges: Any) -> Tensor:
 
 def _eager(q: Tensor, k: Tensor, table: Tensor, tables: RelativeEdgeTables, plan: fused_attention.Plan,
            scale: float) -> Tensor:
-    return _weights(q, k, table, tables._buckets, tables.row_ptr, tables._source, tables._phases, tables._bias, plan,
+    return _weights(q, k, table, tables.buckets.long(), tables.row_ptr, tables._source, tables._phases, tables._bias, plan,
                     scale)
 
 

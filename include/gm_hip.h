@@ -345,6 +345,7 @@ int gm_differential_backward_bf16(const float* g, const uint16_t* q, const uint1
  *     window), then (cos, sin) of the orders 1 .. ; float: n_sources <= 2^24
  *   records_s (n_edges, 2 orders): the edges sorted by source (src_ptr): a word of
  *     the target, a word of the edge, (cos, sin) of the orders 1 ..
+ *   bucket (n_edges): the buckets again, a byte each
  *   1 <= buckets <= 256; indices are followed unchecked.
  * ds (n_edges, H) and partial (gm_relative_partial_rows() rows of buckets H) are
  * workspaces.  Sums in a fixed order.
@@ -363,31 +364,32 @@ int gm_relative_forward_f32(const float* q, const float* k, const float* table, 
                             n_targets, int64_t n_sources, int64_t n_edges, int64_t D, int64_t orders, int64_t F, int64_t
                             H, int64_t buckets, double scale, float* alpha, void* stream);
 int gm_relative_backward_f32(const float* g, const float* alpha, const float* q, const float* k, const float* records,
-                             const float* records_s, const int64_t* desc, const int64_t* row_ptr, const int64_t*
-                             src_ptr, const int32_t* order, const int64_t* counts, const int32_t* order_s, const
-                             int64_t* counts_s, int64_t n_targets, int64_t n_sources, int64_t n_edges, int64_t D,
-                             int64_t orders, int64_t F, int64_t H, int64_t buckets, double scale, float* ds, float*
-                             partial, float* dq, float* dk, float* dtable, void* stream);
+                             const float* records_s, const uint8_t* bucket, const int64_t* desc, const int64_t* row_ptr,
+                             const int64_t* src_ptr, const int32_t* order, const int64_t* counts, const int32_t*
+                             order_s, const int64_t* counts_s, int64_t n_targets, int64_t n_sources, int64_t n_edges,
+                             int64_t D, int64_t orders, int64_t F, int64_t H, int64_t buckets, double scale, float* ds,
+                             float* partial, float* dq, float* dk, float* dtable, void* stream);
 int gm_relative_forward_f64(const double* q, const double* k, const double* table, const double* records, const int64_t*
                             desc, const int64_t* row_ptr, const int32_t* order, const int64_t* counts, int64_t
                             n_targets, int64_t n_sources, int64_t n_edges, int64_t D, int64_t orders, int64_t F, int64_t
                             H, int64_t buckets, double scale, double* alpha, void* stream);
 int gm_relative_backward_f64(const double* g, const double* alpha, const double* q, const double* k, const double*
-                             records, const double* records_s, const int64_t* desc, const int64_t* row_ptr, const
-                             int64_t* src_ptr, const int32_t* order, const int64_t* counts, const int32_t* order_s,
-                             const int64_t* counts_s, int64_t n_targets, int64_t n_sources, int64_t n_edges, int64_t D,
-                             int64_t orders, int64_t F, int64_t H, int64_t buckets, double scale, double* ds, double*
-                             partial, double* dq, double* dk, double* dtable, void* stream);
+                             records, const double* records_s, const uint8_t* bucket, const int64_t* desc, const
+                             int64_t* row_ptr, const int64_t* src_ptr, const int32_t* order, const int64_t* counts,
+                             const int32_t* order_s, const int64_t* counts_s, int64_t n_targets, int64_t n_sources,
+                             int64_t n_edges, int64_t D, int64_t orders, int64_t F, int64_t H, int64_t buckets, double
+                             scale, double* ds, double* partial, double* dq, double* dk, double* dtable, void* stream);
 int gm_relative_forward_bf16(const uint16_t* q, const uint16_t* k, const float* table, const float* records, const
                              int64_t* desc, const int64_t* row_ptr, const int32_t* order, const int64_t* counts, int64_t
                              n_targets, int64_t n_sources, int64_t n_edges, int64_t D, int64_t orders, int64_t F,
                              int64_t H, int64_t buckets, double scale, float* alpha, void* stream);
 int gm_relative_backward_bf16(const float* g, const float* alpha, const uint16_t* q, const uint16_t* k, const float*
-                              records, const float* records_s, const int64_t* desc, const int64_t* row_ptr, const
-                              int64_t* src_ptr, const int32_t* order, const int64_t* counts, const int32_t* order_s,
-                              const int64_t* counts_s, int64_t n_targets, int64_t n_sources, int64_t n_edges, int64_t D,
-                              int64_t orders, int64_t F, int64_t H, int64_t buckets, double scale, float* ds, float*
-                              partial, uint16_t* dq, uint16_t* dk, float* dtable, void* stream);
+                              records, const float* records_s, const uint8_t* bucket, const int64_t* desc, const
+                              int64_t* row_ptr, const int64_t* src_ptr, const int32_t* order, const int64_t* counts,
+                              const int32_t* order_s, const int64_t* counts_s, int64_t n_targets, int64_t n_sources,
+                              int64_t n_edges, int64_t D, int64_t orders, int64_t F, int64_t H, int64_t buckets, double
+                              scale, float* ds, float* partial, uint16_t* dq, uint16_t* dk, float* dtable, void*
+                              stream);
 
 /* ---------------- norm and rotation of rows of heads ----------------
  *
