@@ -15,7 +15,11 @@ signatures and call structure:
   kernels in the factored order with one shared source grouping
   (``_aggregated_factored``, :801-822).  With ``differential`` (no reference
   counterpart) a head's weights are the difference of two softmax maps over the
-  halves of its query and key copies (``nn.differential``).
+  halves of its query and key copies (``nn.differential``); ``relative_bias``
+  adds a learned number a head and ring of distance to the scores
+  (``nn.relative``); ``query_key_norm`` and ``rotary`` normalise each head's
+  queries and keys and turn them by angles of their nodes' positions
+  (``nn.head_norm``).
 
 Every score, softmax and value aggregation runs in the HIP ops
 (``fused_attention.Softmax``, ``fused_factored.FactoredAggregate``; under
@@ -39,7 +43,8 @@ import torch.utils.checkpoint
 from torch import Tensor, nn
 
 from gm_attention_amd.discretization.discretization import SphericalDiscretization
-from gm_attention_amd.nn import assembly, differential, fused_attention, fused_factored, kernels, radial
+from gm_attention_amd.nn import assembly, differential, fused_attention, fused_factored, kernels, radial, relative
+from gm_attention_amd.nn.head_norm import SO2QueryKeyNorm
 from gm_attention_amd.nn.kernels import SO2SteerableKernel
 from gm_attention_amd.nn.linear import (
     FlatLinear, SO2Linear, apply_linear, block_matrix, flat_bias, linear_parameters, matrix_and_bias, weights_matrix,
@@ -160,12 +165,23 @@ class SO2Attention(nn.Module):
 
 
 class SO2MHSA(nn.Module):
-    differential = False  # a layer pickled before there was the option reads as one without it
+    """``relative_bias``: the number of rings of distance up to the cutoff that each head
+    learns a bias of (``relative_bias (rings, num_heads)``, zero at first).
+    ``query_key_norm``: each head's queries and keys (each map's, in a differential layer)
+    normalised, with a learned gain a copy.  ``rotary``: frequencies ``(axes, slots)`` that
+    turn them by their nodes' ``positions (N, axes)``, which ``forward`` then takes."""
+
+    # a layer pickled before there was an option reads as one without it
+    differential = False
+    rings = 0
+    scored = False  # whether queries and keys are normalised or turned
+    rotated = False
 
     def __init__(self, field_type_in: SO2FieldType, num_heads: int, *, cutoff: float, window: str = "hard",
                  n_radial_basis: int = 8, radial_hidden_features: Sequence[int] = (16,), radial_basis: str = "gaussian",
                  bias: bool = True, batched: bool = False, value_kind: str = "steerable", differential: bool = False,
-                 lambda_init: float = 0.8, dtype=None, device=None) -> None:
+                 lambda_init: float = 0.8, relative_bias: int | None = None, query_key_norm: bool = False,
+                 rotary: Tensor | Sequence[Sequence[float]] | None = None, dtype=None, device=None) -> None:
         super().__init__()
         if num_heads < 1:
             raise ValueError(f"num_heads must be at least 1, got {num_heads}.")
@@ -181,6 +197,14 @@ class SO2MHSA(nn.Module):
                 raise ValueError(f"twice num_heads ({2 * num_heads}) must divide the multiplicity of every present "
                                  f"frequency of a differential layer; offending frequencies (as frequency: "
                                  f"multiplicity): {odd}.")
+        if not batched and (relative_bias is not None or query_key_norm or rotary is not None):
+            raise ValueError("relative_bias, query_key_norm and rotary act on every head's scores at once: they need "
+                             "batched=True.")
+        if relative_bias is not None:
+            if differential:
+                raise ValueError("a differential layer takes no relative_bias.")
+            if not 1 <= relative_bias <= relative.MAX_BUCKETS:
+                raise ValueError(f"relative_bias must lie in 1..{relative.MAX_BUCKETS}, got {relative_bias}.")
         self.batched = bool(batched)
         self.differential = bool(differential)
         self.value_kind = value_kind
@@ -202,6 +226,14 @@ class SO2MHSA(nn.Module):
             self.lambda_key = nn.Parameter(torch.empty(shape, dtype=dtype, device=device))
             for p in (self.lambda_query, self.lambda_key):
                 nn.init.normal_(p, std=0.1)
+        if relative_bias is not None:
+            self.rings = int(relative_bias)
+            self.relative_bias = nn.Parameter(torch.zeros(self.rings, num_heads, dtype=dtype, device=device))
+        if query_key_norm or rotary is not None:
+            self.scored, self.rotated = True, rotary is not None
+            head, count = (self.field_type_map, 2 * num_heads) if differential else (self.field_type_attn, num_heads)
+            self.query_key = SO2QueryKeyNorm(head, count, norm=query_key_norm, gain=query_key_norm, frequencies=rotary,
+                                             dtype=dtype, device=device)
 
     def lambdas(self) -> Tensor:
         """A differential layer's factors ``(n_heads,)`` of the second maps:
@@ -213,25 +245,34 @@ class SO2MHSA(nn.Module):
         first, second = (self.lambda_query * self.lambda_key).sum(-1).exp().unbind(0)
         return first - second + self.lambda_init
 
-    def forward(self, x: SO2FeatureField, edges) -> SO2FeatureField:
+    def _check_positions(self, positions: Tensor | None) -> None:
+        if (positions is not None) != self.rotated:
+            raise ValueError("positions must be given exactly where the layer was made with rotary frequencies.")
+
+    def forward(self, x: SO2FeatureField, edges, positions: Tensor | None = None) -> SO2FeatureField:
         edges = _resolve_edges(edges, self.cutoff)
+        self._check_positions(positions)
         if self.batched:
             _validate_node_field(x, self.field_type_in, edges)
-            rows = _attend_batched_flat(self, x, edges)
+            rows = _attend_batched_flat(self, x, edges, positions)
             if rows is not None:
                 return SO2FeatureField.from_flat(self.field_type_in, rows)
-            return self.output_projection(SO2FeatureField(self.field_type_in, _attend_batched(self, x, edges)))
+            return self.output_projection(SO2FeatureField(self.field_type_in,
+                                                          _attend_batched(self, x, edges, positions)))
         fused = _concatenate_heads([head(x, edges) for head in self.heads], self.field_type_in)
         return self.output_projection(fused)
 
-    def forward_chunked(self, x: SO2FeatureField, edges, *, chunk_size: int) -> SO2FeatureField:
+    def forward_chunked(self, x: SO2FeatureField, edges, *, chunk_size: int,
+                        positions: Tensor | None = None) -> SO2FeatureField:
         edges = _resolve_edges(edges, self.cutoff)
-        if self.differential:  # every head at once, over the same ranges
+        self._check_positions(positions)
+        if self.differential or self.rings or self.scored:  # every head at once, over the same ranges
             _validate_node_field(x, self.field_type_in, edges)
-            partials = [_checkpointed(self, functools.partial(_attend_batched, self, x, chunk))
+            partials = [_checkpointed(self, functools.partial(_attend_batched, self, x, chunk, positions))
                         for chunk in edges.chunks(chunk_size)]
             return self.output_projection(SO2FeatureField(
-                self.field_type_in, sum_partials(partials) if partials else _attend_batched(self, x, edges)))
+                self.field_type_in, sum_partials(partials) if partials
+                else _attend_batched(self, x, edges, positions)))
         outs = [cast(SO2Attention, h).forward_chunked(x, edges, chunk_size=chunk_size) for h in self.heads]
         return self.output_projection(_concatenate_heads(outs, self.field_type_in))
 
@@ -366,10 +407,15 @@ def _scores_enabled(mhsa: SO2MHSA, x: SO2FeatureField, edges) -> bool:
     """Whether the layer's scores and softmax take their fused op."""
     if mhsa.differential:
         return differential.enabled(mhsa, x, edges)
-    return fused_attention.softmax_enabled(mhsa, x, edges)
+    return relative.enabled(mhsa, x, edges) if mhsa.rings else fused_attention.softmax_enabled(mhsa, x, edges)
 
 
-def _attend_batched_flat(mhsa: SO2MHSA, x: SO2FeatureField, edges) -> Tensor | None:
+def _scored(mhsa: SO2MHSA, queries: Tensor, keys: Tensor, positions: Tensor | None) -> tuple[Tensor, Tensor]:
+    """The query and key rows as the scores read them."""
+    return mhsa.query_key.forward_flat(queries, keys, positions) if mhsa.scored else (queries, keys)
+
+
+def _attend_batched_flat(mhsa: SO2MHSA, x: SO2FeatureField, edges, positions: Tensor | None = None) -> Tensor | None:
     """The batched layer on flat rows when the fused softmax and the fused
     factored heads serve it (else None): the stacked query and key
     projections as one GEMM each, and the output projection reading the heads'
@@ -394,7 +440,9 @@ def _attend_batched_flat(mhsa: SO2MHSA, x: SO2FeatureField, edges) -> Tensor | N
         else:
             queries = _stacked_flat([h.query for h in heads], mhsa.field_type_in, rows)
             keys = _stacked_flat([h.key for h in heads], mhsa.field_type_in, rows)
-        weights = differential.attention_weights if mhsa.differential else fused_attention.softmax
+        queries, keys = _scored(mhsa, queries, keys, positions)
+        weights = (differential.attention_weights if mhsa.differential else
+                   relative.attention_weights if mhsa.rings else fused_attention.softmax)
         alpha = weights(mhsa, queries, keys, edges)  # (n_edges, n_heads)
         groups = fused_factored.groups_for(edges, edges.source_index)
         if fused_trunk:
@@ -413,17 +461,20 @@ def _attend_batched_flat(mhsa: SO2MHSA, x: SO2FeatureField, edges) -> Tensor | N
     return FlatLinear.apply(out.reshape(out.shape[0], -1), m, bias)
 
 
-def _attend_batched(mhsa: SO2MHSA, x: SO2FeatureField, edges) -> dict[int, Tensor]:
+def _attend_batched(mhsa: SO2MHSA, x: SO2FeatureField, edges, positions: Tensor | None = None) -> dict[int, Tensor]:
     heads = [cast(SO2Attention, h) for h in mhsa.heads]
     with torch.profiler.record_function("gm::attention/attend"):
-        queries = _stacked_projection([h.query for h in heads], x)
-        keys = _stacked_projection([h.key for h in heads], x)
+        queries = _stacked_projection([h.query for h in heads], x)._rows()
+        keys = _stacked_projection([h.key for h in heads], x)._rows()
+        queries, keys = _scored(mhsa, queries, keys, positions)
         if mhsa.differential:
-            alpha = differential.attention_weights(mhsa, queries._rows(), keys._rows(), edges)
+            alpha = differential.attention_weights(mhsa, queries, keys, edges)
+        elif mhsa.rings:
+            alpha = relative.attention_weights(mhsa, queries, keys, edges)
         elif fused_attention.softmax_enabled(mhsa, x, edges):
-            alpha = fused_attention.softmax(mhsa, queries._rows(), keys._rows(), edges)  # (n_edges, n_heads)
+            alpha = fused_attention.softmax(mhsa, queries, keys, edges)  # (n_edges, n_heads)
         else:  # the reference's eager weights (attention.py:880-886)
-            alpha = fused_attention.softmax_eager(fused_attention.plan(mhsa), queries._rows(), keys._rows(), edges,
+            alpha = fused_attention.softmax_eager(fused_attention.plan(mhsa), queries, keys, edges,
                                                   mhsa.cutoff, heads[0].window, heads[0]._score_scale)
         return _aggregated_factored(mhsa, x, edges, alpha)
 

@@ -29,7 +29,10 @@ sub-layer's output too, scaled and gated per copy on request,
 
 each sum with the norms around it one HIP pass (``nn.residual``); ``z`` is affine
 in the scalars of the sub-layer's input.  ``attention_differential`` makes the
-batched attention's weights differences of two softmax maps (``nn.differential``).
+batched attention's weights differences of two softmax maps (``nn.differential``);
+``attention_relative_bias``, ``attention_query_key_norm`` and ``attention_rotary`` are
+``SO2MHSA``'s ``relative_bias``, ``query_key_norm`` and ``rotary`` (the last takes the
+nodes' ``positions`` with the rows).
 
 ``IcoEncode`` / ``EquiEncode`` (reference :359-505, :799-869) restrict a
 field from a fine grid onto a coarse one over bipartite edges
@@ -90,7 +93,8 @@ class SO2TransformerBlock(nn.Module):
                  dropout: float = 0.0, eps: float = 1e-5, bias: bool = True,
                  nonlinearity: NonlinearityKind = "scalar_gate_double_sigmoid", mixer: MixerKind = "attention",
                  attention_batched: bool = False, value_kind: str = "steerable",
-                 attention_differential: bool = False, norm_placement: NormPlacement = "pre",
+                 attention_differential: bool = False, attention_relative_bias: int | None = None,
+                 attention_query_key_norm: bool = False, attention_rotary=None, norm_placement: NormPlacement = "pre",
                  residual_gate: str | None = None, residual_scale: float | None = None, dtype=None,
                  device=None) -> None:
         super().__init__()
@@ -114,6 +118,10 @@ class SO2TransformerBlock(nn.Module):
             raise ValueError(f"residual_gate needs frequency-0 channels to condition its gates on, got {field_type!r}.")
         if attention_differential and mixer != "attention":
             raise ValueError("attention_differential needs mixer='attention'.")
+        if mixer != "attention" and (attention_relative_bias is not None or attention_query_key_norm
+                                     or attention_rotary is not None):
+            raise ValueError("attention_relative_bias, attention_query_key_norm and attention_rotary need "
+                             "mixer='attention'.")
         self.nonlinearity = nonlinearity
         self.norm_placement = norm_placement
         self.field_type = field_type
@@ -126,7 +134,9 @@ class SO2TransformerBlock(nn.Module):
             self.attention = SO2MHSA(field_type, num_heads, cutoff=cutoff, window=window,
                                       n_radial_basis=n_radial_basis, radial_hidden_features=radial_hidden_features,
                                       radial_basis=radial_basis, bias=bias, batched=attention_batched,
-                                      value_kind=value_kind, differential=attention_differential, **kw)
+                                      value_kind=value_kind, differential=attention_differential,
+                                      relative_bias=attention_relative_bias, query_key_norm=attention_query_key_norm,
+                                      rotary=attention_rotary, **kw)
         else:
             self.attention = SO2Convolution(field_type, field_type, cutoff=cutoff, window=window,
                                             self_interaction="none", n_radial_basis=n_radial_basis,
@@ -144,41 +154,50 @@ class SO2TransformerBlock(nn.Module):
         self.linear2 = SO2Linear(self.hidden_field_type, field_type, bias=bias, **kw)
         self.mlp_dropout = SO2Dropout(field_type, p=dropout)
 
-    def forward(self, x: SO2FeatureField, edges) -> SO2FeatureField:
-        return self._run(x, edges, chunk_size=None)
+    def forward(self, x: SO2FeatureField, edges, positions: Tensor | None = None) -> SO2FeatureField:
+        return self._run(x, edges, chunk_size=None, positions=positions)
 
-    def forward_chunked(self, x: SO2FeatureField, edges, *, chunk_size: int) -> SO2FeatureField:
-        return self._run(x, edges, chunk_size=chunk_size)
+    def forward_chunked(self, x: SO2FeatureField, edges, *, chunk_size: int,
+                        positions: Tensor | None = None) -> SO2FeatureField:
+        return self._run(x, edges, chunk_size=chunk_size, positions=positions)
 
-    def _mix(self, h: Tensor, edges, chunk_size: int | None) -> Tensor:
+    def _mix(self, h: Tensor, edges, chunk_size: int | None, positions: Tensor | None = None) -> Tensor:
         """The mixer on flat rows: bfloat16 rows straight into the batched
         attention's fused path where it serves them (its scores and node mixes
         read them, its arithmetic is float32), else the rows in the mixer's
         parameter dtype; the result in float32 or that dtype."""
+        given = {}
+        if positions is not None:
+            if self.mixer != "attention":
+                raise ValueError("positions belong to mixer='attention' with attention_rotary.")
+            given["positions"] = positions
         if h.dtype == torch.bfloat16 and chunk_size is None and self.mixer == "attention":
             field = SO2FeatureField.from_flat(self.field_type, h)
             if batched_flat_serves(self.attention, field, edges):
-                return self.attention(field, edges)._rows()
+                return self.attention(field, edges, **given)._rows()
         pdtype = parameter_dtype(self.attention)
         field = SO2FeatureField.from_flat(self.field_type, h.to(pdtype))
         if chunk_size is None:
-            out = self.attention(field, edges)
+            out = self.attention(field, edges, **given)
         else:
-            out = self.attention.forward_chunked(field, edges, chunk_size=chunk_size)
+            out = self.attention.forward_chunked(field, edges, chunk_size=chunk_size, **given)
         return out._rows()
 
-    def _run(self, x: SO2FeatureField, edges, *, chunk_size: int | None) -> SO2FeatureField:
+    def _run(self, x: SO2FeatureField, edges, *, chunk_size: int | None,
+             positions: Tensor | None = None) -> SO2FeatureField:
         if x.field_type != self.field_type:
             raise ValueError(f"Expected a field of type {self.field_type!r}, got {x.field_type!r}.")
         flat = x._rows()
         batch = flat.shape[:-1]
         rows = flat.reshape(-1, flat.shape[-1])
-        return SO2FeatureField.from_flat(self.field_type, self.forward_flat(rows, edges, chunk_size).reshape(*batch, -1))
+        return SO2FeatureField.from_flat(
+            self.field_type, self.forward_flat(rows, edges, chunk_size, positions).reshape(*batch, -1))
 
-    def forward_flat(self, rows: Tensor, edges, chunk_size: int | None = None) -> Tensor:
+    def forward_flat(self, rows: Tensor, edges, chunk_size: int | None = None,
+                     positions: Tensor | None = None) -> Tensor:
         """The block on flat rows ``(N, D)``; returns ``(N, D)`` in the rows' dtype."""
         normed = self.norm1.forward_flat(rows)
-        attended = self._mix(normed, edges, chunk_size)
+        attended = self._mix(normed, edges, chunk_size, positions)
         if self.norm_placement == "sandwich":
             return self._sandwich(rows, normed, attended)
         rows = rows + self.attention_dropout.forward_flat(attended).to(rows.dtype)

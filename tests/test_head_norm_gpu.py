@@ -487,7 +487,8 @@ def test_refusals():
         call(head={0: 8})
     with pytest.raises(ValueError, match="nothing to do"):
         query_key_norm(q, q, head, 2, eps=None)
-    for kw, message in ((dict(eps=0.0), "eps must be positive"), (dict(frequencies=torch.ones(1, 3)), "frequencies must"),
+    for kw, message in ((dict(eps=0.0), "eps must be positive"),
+                        (dict(frequencies=torch.ones(1, 3)), "frequencies must"),
                         (dict(norm=False, gain=False), "nothing to do")):
         with pytest.raises(ValueError, match=message):
             SO2QueryKeyNorm(head, 2, **kw)
