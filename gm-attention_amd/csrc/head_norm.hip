@@ -8,13 +8,17 @@
 //   dgain = sum over nodes and heads of d xhat
 //   dx    = (t - xhat mean(t xhat)) / sqrt(mean x^2 + eps)
 //
-// A pass reads its rows once and writes once; angles are made in the pass, in double
-// up to the whole turns (a far position's angle has no bits left in float), once for
-// all heads and both sets.  A thread holds the same unit of a row (V numbers: whole
-// pairs, or scalars) for all the rows of its workgroup, so that neighbouring lanes
-// read neighbouring numbers, and gains, and sums for their gradients, stay in
-// registers.  A head's squares meet in LDS, in double: no row overflows.  The
-// workgroups are persistent; their sums are added in a fixed order, no atomics.
+// A pass reads its rows once and writes once, and the bytes bound it: 524,288 rows of 160 of queries and keys each take
+// 257 us forward and 411 backward in float (5.2 and 4.9 TB/s), 126 and 225 in bfloat16 (5.3 and 4.5: its registers
+// leave two waves a SIMD).  Angles are made in the pass, in double up to the whole turns (a far position's angle has no
+// bits left in float), once for all heads and both sets; sums of a head are in double from what a lane (a unit) adds in
+// float, so that no row overflows.
+//
+// The lane kernels hold a unit of a head a lane and need no other wave's numbers.  Layouts without such units (odd
+// copies, frequencies above 2, rows at odd addresses) and double take the general kernels, where a thread holds the same
+// piece of a row for all the rows of its workgroup and a head's squares meet in LDS between barriers (305 and 497 us
+// for the float rows above, 245 and 507 for the bfloat16 ones).  All are persistent; gains, and sums for their
+// gradients, stay in registers over a workgroup's rows, whose sums are added in a fixed order, no atomics.
 #include <algorithm>
 #include <type_traits>
 
@@ -48,7 +52,7 @@ struct HnArgs {
   T* partial;                     // (workgroups, sets, copies) or null
   const double* positions;        // (n_rows, axes)
   const double* frequencies;      // (axes, slots)
-  double eps;
+  double eps, share;              // share: 1 / numbers
 };
 
 // Unit u of a row: `width` numbers from column `col` (V but for a last odd scalar), the copy of each among its head's,
@@ -111,17 +115,23 @@ __device__ __forceinline__ void hn_store(R* p, int width, const T (&v)[V]) {
 __device__ __forceinline__ void hn_sincos(double turns, float& s, float& c) { sincospif(2.f * (float)turns, &s, &c); }
 __device__ __forceinline__ void hn_sincos(double turns, double& s, double& c) { sincospi(2.0 * turns, &s, &c); }
 
+// (cos, sin) of a row's angle in a slot.
+template <typename T, typename R>
+__device__ __forceinline__ void hn_angle(const HnArgs<T, R>& a, int64_t row, int slot, T& c, T& s) {
+  double theta = 0.0;
+  for (int axis = 0; axis < a.axes; ++axis)
+    theta = fma(a.positions[row * a.axes + axis], a.frequencies[axis * a.slots + slot], theta);
+  const double turns = theta * 0.15915494309189535;
+  hn_sincos(turns - rint(turns), s, c);
+}
+
 // (cos, sin) of the angles of `rows` rows from `first`, into LDS.
 template <typename T, typename R>
 __device__ __forceinline__ void hn_angles(const HnArgs<T, R>& a, int64_t first, int rows, T* cs) {
   for (int i = threadIdx.x; i < rows * a.slots; i += blockDim.x) {
     const int k = i / a.slots, slot = i - k * a.slots;
     const int64_t row = first + k < a.n_rows ? first + k : a.n_rows - 1;
-    double theta = 0.0;
-    for (int axis = 0; axis < a.axes; ++axis)
-      theta = fma(a.positions[row * a.axes + axis], a.frequencies[axis * a.slots + slot], theta);
-    const double turns = theta * 0.15915494309189535;
-    hn_sincos(turns - rint(turns), cs[2 * i + 1], cs[2 * i]);
+    hn_angle(a, row, slot, cs[2 * i], cs[2 * i + 1]);
   }
 }
 
@@ -135,6 +145,42 @@ __device__ __forceinline__ void hn_turn(T (&v)[V], const T* cs, bool back) {
     v[j] = c * v0 - s * v1;
     v[j + 1] = c * v1 + s * v0;
   }
+}
+
+// 1 / sqrt, for float to better than its half step: the approximation in double and a Newton step (of zero and
+// infinity the approximation).
+template <typename T>
+__device__ __forceinline__ double hn_rsqrt(double v) {
+  if constexpr (sizeof(T) == 8) return 1.0 / sqrt(v);
+  const double y = __builtin_amdgcn_rsq(v);
+  const double refined = y * fma(-0.5 * v * y, y, 1.5);
+  return v > 0.0 && v < (double)INFINITY ? refined : y;
+}
+// Sum of a_j b_j in float (two sums, of even and odd j); where that is out of float's range, or near zero, once more of
+// numbers scaled by 2^-70 or 2^70.
+template <int V>
+__device__ __forceinline__ double hn_dot(const float (&a)[V], const float (&b)[V]) {
+  auto sum = [&](float scale) {
+    float s = 0.f, t = 0.f;
+#pragma unroll
+    for (int j = 0; j + 1 < V; j += 2) {
+      s = fmaf(a[j] * scale, b[j] * scale, s);
+      t = fmaf(a[j + 1] * scale, b[j + 1] * scale, t);
+    }
+    if constexpr (V % 2) s = fmaf(a[V - 1] * scale, b[V - 1] * scale, s);
+    return s + t;
+  };
+  const float s = sum(1.f);
+  if (fabsf(s) > 1e-30f && fabsf(s) < INFINITY) return (double)s;
+  const bool small = fabsf(s) <= 1e-30f;
+  return (double)sum(small ? 0x1p70f : 0x1p-70f) * (small ? 0x1p-140 : 0x1p140);
+}
+template <int V>
+__device__ __forceinline__ double hn_dot(const double (&a)[V], const double (&b)[V]) {
+  double s = 0.0;
+#pragma unroll
+  for (int j = 0; j < V; ++j) s = fma(a[j], b[j], s);
+  return s;
 }
 
 // Sum over a head's units of sums[..] (one row's units), shared by `parts` lanes; all of them get it.
@@ -203,17 +249,14 @@ __global__ __launch_bounds__(kHnThreads) void head_norm_forward(HnArgs<T, R> a) 
         for (int st = 0; st < NS; ++st)
 #pragma unroll
           for (int k = 0; k < TR; ++k) {
-            double s = 0.0;
-#pragma unroll
-            for (int j = 0; j < V; ++j) s = fma((double)v[st][k][j], (double)v[st][k][j], s);
-            sums[(st * rows + k * a.groups + group) * a.units + u] = s;
+            sums[(st * rows + k * a.groups + group) * a.units + u] = hn_dot<V>(v[st][k], v[st][k]);
           }
       }
       __syncthreads();
       const int tasks = NS * rows * a.L.H, part = threadIdx.x % a.parts;
       for (int t = threadIdx.x / a.parts; t < tasks; t += blockDim.x / a.parts) {
         const double s = hn_head_sum<V>(a, sums + t / a.L.H * a.units, t % a.L.H, part);
-        if (part == 0) heads[t] = (T)(1.0 / sqrt(s / a.numbers + a.eps));
+        if (part == 0) heads[t] = (T)hn_rsqrt<T>(fma(s, a.share, a.eps));
       }
     }
     __syncthreads();
@@ -290,15 +333,12 @@ __global__ __launch_bounds__(kHnThreads) void head_norm_backward(HnArgs<T, R> a)
         for (int st = 0; st < NS; ++st)
 #pragma unroll
           for (int k = 0; k < TR; ++k) {
-            double s = 0.0, m = 0.0;
+            T t[V];
 #pragma unroll
-            for (int j = 0; j < V; ++j) {
-              s = fma((double)v[st][k][j], (double)v[st][k][j], s);
-              m = fma((double)(gain[st][j] * d[st][k][j]), (double)v[st][k][j], m);
-            }
+            for (int j = 0; j < V; ++j) t[j] = gain[st][j] * d[st][k][j];
             const int at = (st * rows + k * a.groups + group) * a.units + u;
-            sums[at] = s;
-            sums[products + at] = m;
+            sums[at] = hn_dot<V>(v[st][k], v[st][k]);
+            sums[products + at] = hn_dot<V>(t, v[st][k]);
           }
       }
       __syncthreads();
@@ -308,9 +348,9 @@ __global__ __launch_bounds__(kHnThreads) void head_norm_backward(HnArgs<T, R> a)
         const double s = hn_head_sum<V>(a, row, t % a.L.H, part);
         const double m = hn_head_sum<V>(a, row + products, t % a.L.H, part);
         if (part == 0) {
-          const double inv = 1.0 / sqrt(s / a.numbers + a.eps);
+          const double inv = hn_rsqrt<T>(fma(s, a.share, a.eps));
           heads[t] = (T)inv;
-          heads[means + t] = (T)(m * inv / a.numbers);
+          heads[means + t] = (T)(m * inv * a.share);
         }
       }
       __syncthreads();
@@ -363,6 +403,200 @@ __global__ __launch_bounds__(kHnThreads) void head_norm_backward(HnArgs<T, R> a)
           const T* at = held + (g * a.units + base + h * per + i) * V + j;
           s += n == 0 ? at[0] : at[0] + at[1];
         }
+      a.partial[((int64_t)blockIdx.x * NS + st) * a.copies + c] = s;
+    }
+  }
+}
+
+// ------------------------------------------------------------- lane kernels
+// A head's copies as `per` units of (A0, A1, A2) copies of frequencies 0, 1, 2, a lane a unit: a head's sums are in
+// its own lanes, so a wave's rows need nothing of the other waves.  A row's angles are made by its lanes, each some of
+// them, and handed over through the wave's LDS.
+
+struct HnShape {
+  int a0, a1, a2;
+};
+struct HnLanes {
+  int per, lanes, rows;  // units a head; lanes a row, rows a wave
+  int base[3];           // the frequencies' flat offsets
+  int c0, c1, c2;        // a head's copies at frequencies 0, 1, 2
+};
+
+template <int A0, int A1, int A2>
+struct HnRow {
+  static constexpr int W0 = A0, W1 = 2 * A1, W2 = 2 * A2, N = W0 + W1 + W2, C = A0 + A1 + A2;
+  static constexpr int kPairs = A0 / 2, S = kPairs + A1 + A2;  // pairs of scalars; the unit's slots
+  template <typename R>
+  static __device__ __forceinline__ void load(const R* row, const HnLanes& w, int u, float (&v)[N]) {
+    if constexpr (W0 > 0) load_piece<W0>(row + w.base[0] + u * W0, v);
+    if constexpr (W1 > 0) load_piece<W1>(row + w.base[1] + u * W1, v + W0);
+    if constexpr (W2 > 0) load_piece<W2>(row + w.base[2] + u * W2, v + W0 + W1);
+  }
+  template <typename R>
+  static __device__ __forceinline__ void store(R* row, const HnLanes& w, int u, const float (&v)[N]) {
+    if constexpr (W0 > 0) store_piece<W0>(row + w.base[0] + u * W0, v);
+    if constexpr (W1 > 0) store_piece<W1>(row + w.base[1] + u * W1, v + W0);
+    if constexpr (W2 > 0) store_piece<W2>(row + w.base[2] + u * W2, v + W0 + W1);
+  }
+  template <int W, typename R>
+  static __device__ __forceinline__ void load_piece(const R* p, float* v) {
+    if constexpr (W == 8 && sizeof(R) == 2) {
+      const uint4 x = *reinterpret_cast<const uint4*>(p);
+      const uint32_t word[4] = {x.x, x.y, x.z, x.w};
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        v[2 * i] = __uint_as_float(word[i] << 16);
+        v[2 * i + 1] = __uint_as_float(word[i] & 0xFFFF0000u);
+      }
+    } else {
+      load_w<W>(p, v);
+    }
+  }
+  template <int W, typename R>
+  static __device__ __forceinline__ void store_piece(R* p, const float* v) {
+    if constexpr (W == 8 && sizeof(R) == 2)
+      *reinterpret_cast<uint4*>(p) = make_uint4(row_pack(v[0], v[1]), row_pack(v[2], v[3]), row_pack(v[4], v[5]),
+                                                row_pack(v[6], v[7]));
+    else
+      store_w<W>(p, v);
+  }
+  // the copy of a head that the unit's number i belongs to
+  static __device__ __forceinline__ int copy(const HnLanes& w, int own, int i) {
+    if (i < W0) return own * A0 + i;
+    if (i < W0 + W1) return w.c0 + own * A1 + (i - W0) / 2;
+    return w.c0 + w.c1 + own * A2 + (i - W0 - W1) / 2;
+  }
+  // the head's slot of the unit's pair j
+  static __device__ __forceinline__ int slot(const HnLanes& w, int own, int j) {
+    if (j < kPairs) return own * kPairs + j;
+    if (j < kPairs + A1) return w.c0 / 2 + own * A1 + j - kPairs;
+    return w.c0 / 2 + w.c1 + own * A2 + j - kPairs - A1;
+  }
+  static constexpr int pair(int j) { return j < kPairs ? 2 * j : W0 + 2 * (j - kPairs); }
+  static __device__ __forceinline__ void turn(float (&v)[N], const float2 (&cs)[S > 0 ? S : 1], bool back) {
+#pragma unroll
+    for (int j = 0; j < S; ++j) {
+      const float c = cs[j].x, s = back ? -cs[j].y : cs[j].y, v0 = v[pair(j)], v1 = v[pair(j) + 1];
+      v[pair(j)] = c * v0 - s * v1;
+      v[pair(j) + 1] = c * v1 + s * v0;
+    }
+  }
+};
+
+__device__ __forceinline__ double hn_lane_sum(double v, int per) {
+  for (int o = 1; o < per; o <<= 1) v += __shfl_xor(v, o, kWave);
+  return v;
+}
+
+// The angles of a lane's pairs; `cs` the wave's LDS (rows, slots).
+template <typename U, typename R>
+__device__ __forceinline__ void hn_lane_angles(const HnArgs<float, R>& a, const HnLanes& w, int64_t row, int r, int u,
+                                               int own, float2* cs, float2 (&out)[U::S > 0 ? U::S : 1]) {
+  wave_lds();  // the rows before have been read
+  if (r < w.rows)
+    for (int slot = u; slot < a.slots; slot += w.lanes)
+      hn_angle(a, row, slot, cs[r * a.slots + slot].x, cs[r * a.slots + slot].y);
+  wave_lds();
+#pragma unroll
+  for (int j = 0; j < U::S; ++j) out[j] = cs[(r < w.rows ? r : 0) * a.slots + U::slot(w, own, j)];
+}
+
+template <typename R, typename U, int NS>
+__global__ __launch_bounds__(256) void head_norm_forward_lanes(HnArgs<float, R> a, HnLanes w) {
+  extern __shared__ __align__(16) char hn_mem[];
+  const int lane = threadIdx.x & 63, wave = uniform((int)(threadIdx.x >> 6));
+  float2* cs = reinterpret_cast<float2*>(hn_mem) + wave * w.rows * a.slots;
+  const int r = lane / w.lanes, u = lane % w.lanes, own = u % w.per;
+  float gain[NS][U::N];
+#pragma unroll
+  for (int st = 0; st < NS; ++st)
+#pragma unroll
+    for (int i = 0; i < U::N; ++i) gain[st][i] = a.gain[st] ? a.gain[st][U::copy(w, own, i)] : 1.f;
+  const int64_t step = (int64_t)gridDim.x * kWavesPerBlock * w.rows;
+  for (int64_t first = ((int64_t)blockIdx.x * kWavesPerBlock + wave) * w.rows; first < a.n_rows; first += step) {
+    const bool live = r < w.rows && first + r < a.n_rows;
+    const int64_t row = live ? first + r : first;
+    float v[NS][U::N];
+#pragma unroll
+    for (int st = 0; st < NS; ++st) U::load(a.x[st] + row * a.stride[st], w, u, v[st]);
+    float2 turn[U::S > 0 ? U::S : 1];
+    if (a.axes) hn_lane_angles<U>(a, w, row, r, u, own, cs, turn);
+#pragma unroll
+    for (int st = 0; st < NS; ++st) {
+      const float inv = a.normalise ? (float)hn_rsqrt<float>(fma(hn_lane_sum(hn_dot(v[st], v[st]), w.per), a.share, a.eps)) : 1.f;
+#pragma unroll
+      for (int i = 0; i < U::N; ++i) v[st][i] = gain[st][i] * (v[st][i] * inv);
+      if (a.axes) U::turn(v[st], turn, false);
+      if (live) U::store(a.y[st] + row * a.L.D, w, u, v[st]);
+    }
+  }
+}
+
+template <typename R, typename U, int NS>
+__global__ __launch_bounds__(256) void head_norm_backward_lanes(HnArgs<float, R> a, HnLanes w) {
+  extern __shared__ __align__(16) char hn_mem[];
+  const int lane = threadIdx.x & 63, wave = uniform((int)(threadIdx.x >> 6));
+  float2* cs = reinterpret_cast<float2*>(hn_mem) + wave * w.rows * a.slots;
+  const int r = lane / w.lanes, u = lane % w.lanes, own = u % w.per;
+  float gain[NS][U::N], acc[NS][U::C];
+#pragma unroll
+  for (int st = 0; st < NS; ++st) {
+#pragma unroll
+    for (int i = 0; i < U::N; ++i) gain[st][i] = a.gain[st] ? a.gain[st][U::copy(w, own, i)] : 1.f;
+#pragma unroll
+    for (int c = 0; c < U::C; ++c) acc[st][c] = 0.f;
+  }
+  const int64_t step = (int64_t)gridDim.x * kWavesPerBlock * w.rows;
+  for (int64_t first = ((int64_t)blockIdx.x * kWavesPerBlock + wave) * w.rows; first < a.n_rows; first += step) {
+    const bool live = r < w.rows && first + r < a.n_rows;
+    const int64_t row = live ? first + r : first;
+    float v[NS][U::N], d[NS][U::N];
+#pragma unroll
+    for (int st = 0; st < NS; ++st) {
+      U::load(a.x[st] + row * a.stride[st], w, u, v[st]);
+      U::load(a.dy[st] + row * a.L.D, w, u, d[st]);
+    }
+    float2 turn[U::S > 0 ? U::S : 1];
+    if (a.axes) hn_lane_angles<U>(a, w, row, r, u, own, cs, turn);
+#pragma unroll
+    for (int st = 0; st < NS; ++st) {
+      if (a.axes) U::turn(d[st], turn, true);
+      float t[U::N], inv = 1.f, mean = 0.f;
+#pragma unroll
+      for (int i = 0; i < U::N; ++i) t[i] = gain[st][i] * d[st][i];
+      if (a.normalise) {
+        const double wide = hn_rsqrt<float>(fma(hn_lane_sum(hn_dot(v[st], v[st]), w.per), a.share, a.eps));
+        inv = (float)wide;
+        mean = (float)(hn_lane_sum(hn_dot(t, v[st]), w.per) * wide * a.share);
+      }
+#pragma unroll
+      for (int i = 0; i < U::N; ++i) {
+        const float hat = v[st][i] * inv;
+        const int c = i < U::W0 ? i : U::W0 + (i - U::W0) / 2;
+        acc[st][c] = fmaf(live ? d[st][i] : 0.f, hat, acc[st][c]);
+        t[i] = inv * (t[i] - hat * mean);
+      }
+      if (live) U::store(a.dx[st] + row * a.L.D, w, u, t);
+    }
+  }
+  if (!a.partial) return;
+  // the workgroup's sums, in the order of its waves, rows and heads
+  float* held = reinterpret_cast<float*>(hn_mem);  // (C, 256)
+#pragma unroll
+  for (int st = 0; st < NS; ++st) {
+    __syncthreads();
+#pragma unroll
+    for (int c = 0; c < U::C; ++c) held[c * 256 + threadIdx.x] = acc[st][c];
+    __syncthreads();
+    for (int c = threadIdx.x; c < a.copies; c += blockDim.x) {
+      const int freq = c < w.c0 ? 0 : (c < w.c0 + w.c1 ? 1 : 2);
+      const int wide = freq == 0 ? U::W0 : (freq == 1 ? U::W1 / 2 : U::W2 / 2);
+      const int local = c - (freq == 0 ? 0 : (freq == 1 ? w.c0 : w.c0 + w.c1)), unit = local / wide;
+      const int at = local % wide + (freq == 0 ? 0 : (freq == 1 ? U::W0 : U::W0 + U::W1 / 2));
+      float s = 0.f;
+      for (int wv = 0; wv < kWavesPerBlock; ++wv)
+        for (int row = 0; row < w.rows; ++row)
+          for (int h = unit; h < w.lanes; h += w.per) s += held[at * 256 + wv * kWave + row * w.lanes + h];
       a.partial[((int64_t)blockIdx.x * NS + st) * a.copies + c] = s;
     }
   }
@@ -427,9 +661,105 @@ int hn_launch(HnArgs<T, R> a, T* dgain, hipStream_t stream) {
   return check_launch("head_norm");
 }
 
+// A workgroup of four waves of whole rows each; resident ones.
+template <typename R, int A0, int A1, int A2, int NS, bool kBackward>
+int hn_launch_lanes(const HnArgs<float, R>& a, const HnLanes& w, float* dgain, hipStream_t stream) {
+  using U = HnRow<A0, A1, A2>;
+  using Kernel = void (*)(HnArgs<float, R>, HnLanes);
+  constexpr Kernel kernel = kBackward ? &head_norm_backward_lanes<R, U, NS> : &head_norm_forward_lanes<R, U, NS>;
+  size_t lds = a.axes ? (size_t)kWavesPerBlock * w.rows * a.slots * sizeof(float2) : 0;
+  if (kBackward && a.partial) lds = std::max(lds, (size_t)U::C * 256 * sizeof(float));
+  const int64_t per = kWavesPerBlock * w.rows, tiles = (a.n_rows + per - 1) / per;
+  const int64_t resident = resident_blocks(reinterpret_cast<const void*>(kernel), 256, lds);
+  const int64_t most = std::min<int64_t>(kHnPartialRows, resident > 0 ? resident : kHnPartialRows);
+  const int64_t blocks = std::min(tiles, most);
+  hipLaunchKernelGGL(kernel, dim3((unsigned)blocks), dim3(256), lds, stream, a, w);
+  if (kBackward && a.partial) launch_partial_sum<float>(a.partial, blocks, NS * a.copies, dgain, stream);
+  return check_launch("head_norm");
+}
+
+// The units of the lane kernels: pieces of 16 bytes at the frequencies above 0 where the copies allow, at frequency 0
+// whole pairs of scalars (a last odd one only where a head is one unit).
+constexpr HnShape kHnFloat[] = {{2, 2, 2}, {4, 2, 2}, {4, 2, 0}, {2, 2, 0}, {4, 2, 1}, {4, 0, 0}, {0, 2, 2}, {2, 1, 1}};
+constexpr HnShape kHnHalf[] = {{4, 4, 4}, {8, 4, 4}, {4, 4, 0}, {8, 4, 2}, {8, 0, 0}, {0, 4, 4}, {2, 2, 2}, {2, 1, 1}};
+
+// The shape's index, or -1: the layout has other frequencies, no such units, or rows beside their alignment.
+template <typename R>
+int hn_shape(const HnArgs<float, R>& a, int sets, bool backward, HnLanes& w) {
+  int c[3] = {0, 0, 0};
+  for (int f = 0; f < 3; ++f) w.base[f] = 0;
+  for (int f = 0; f < a.L.F; ++f) {
+    if (a.L.n[f] > 2) return -1;
+    c[a.L.n[f]] = a.L.a[f];
+    w.base[a.L.n[f]] = a.L.off[f];
+  }
+  w.c0 = c[0];
+  w.c1 = c[1];
+  w.c2 = c[2];
+  constexpr int kCount = 8;
+  const HnShape(&shapes)[kCount] = sizeof(R) == 4 ? kHnFloat : kHnHalf;
+  for (int i = 0; i < kCount; ++i) {
+    const HnShape& s = shapes[i];
+    for (w.per = 1; w.per * a.L.H <= kWave; w.per *= 2) {
+      if (c[0] != w.per * s.a0 || c[1] != w.per * s.a1 || c[2] != w.per * s.a2) continue;
+      const int width[3] = {s.a0, 2 * s.a1, 2 * s.a2};
+      size_t unit = 1;
+      for (int f = 0; f < 3; ++f) {
+        if (width[f] == 0) continue;
+        // pieces of up to 16 bytes
+        const int piece = std::min<int>(width[f], 16 / (int)sizeof(R));
+        if (w.base[f] % piece != 0 || a.L.D % piece != 0) return -1;
+        for (int st = 0; st < sets; ++st)
+          if (a.stride[st] % piece != 0) return -1;
+        unit = std::max(unit, piece * sizeof(R));
+      }
+      for (int st = 0; st < sets; ++st) {
+        if (!aligned(a.x[st], unit)) return -1;
+        if (backward ? !(aligned(a.dy[st], unit) && aligned(a.dx[st], unit)) : !aligned(a.y[st], unit)) return -1;
+      }
+      w.lanes = a.L.H * w.per;
+      w.rows = kWave / w.lanes;
+      return i;
+    }
+  }
+  return -1;
+}
+
+template <bool kBackward, int NS, typename R>
+int hn_lanes(int shape, const HnArgs<float, R>& a, const HnLanes& w, float* dgain, hipStream_t stream) {
+  if constexpr (sizeof(R) == 4) {
+    switch (shape) {
+      case 0: return hn_launch_lanes<R, 2, 2, 2, NS, kBackward>(a, w, dgain, stream);
+      case 1: return hn_launch_lanes<R, 4, 2, 2, NS, kBackward>(a, w, dgain, stream);
+      case 2: return hn_launch_lanes<R, 4, 2, 0, NS, kBackward>(a, w, dgain, stream);
+      case 3: return hn_launch_lanes<R, 2, 2, 0, NS, kBackward>(a, w, dgain, stream);
+      case 4: return hn_launch_lanes<R, 4, 2, 1, NS, kBackward>(a, w, dgain, stream);
+      case 5: return hn_launch_lanes<R, 4, 0, 0, NS, kBackward>(a, w, dgain, stream);
+      case 6: return hn_launch_lanes<R, 0, 2, 2, NS, kBackward>(a, w, dgain, stream);
+      default: return hn_launch_lanes<R, 2, 1, 1, NS, kBackward>(a, w, dgain, stream);
+    }
+  } else {
+    switch (shape) {
+      case 0: return hn_launch_lanes<R, 4, 4, 4, NS, kBackward>(a, w, dgain, stream);
+      case 1: return hn_launch_lanes<R, 8, 4, 4, NS, kBackward>(a, w, dgain, stream);
+      case 2: return hn_launch_lanes<R, 4, 4, 0, NS, kBackward>(a, w, dgain, stream);
+      case 3: return hn_launch_lanes<R, 8, 4, 2, NS, kBackward>(a, w, dgain, stream);
+      case 4: return hn_launch_lanes<R, 8, 0, 0, NS, kBackward>(a, w, dgain, stream);
+      case 5: return hn_launch_lanes<R, 0, 4, 4, NS, kBackward>(a, w, dgain, stream);
+      case 6: return hn_launch_lanes<R, 2, 2, 2, NS, kBackward>(a, w, dgain, stream);
+      default: return hn_launch_lanes<R, 2, 1, 1, NS, kBackward>(a, w, dgain, stream);
+    }
+  }
+}
+
 template <bool kBackward, typename T, typename R>
 int hn_dispatch(const HnArgs<T, R>& a, int sets, T* dgain, hipStream_t stream) {
   if constexpr (!std::is_same<T, double>::value) {
+    HnLanes w{};
+    const int shape = hn_shape(a, sets, kBackward, w);
+    if (shape >= 0)
+      return sets == 1 ? hn_lanes<kBackward, 1>(shape, a, w, dgain, stream)
+                       : hn_lanes<kBackward, 2>(shape, a, w, dgain, stream);
     if (hn_wide(a, sets, kBackward))
       return sets == 1 ? hn_launch<T, R, 4, 1, kBackward>(a, dgain, stream)
                        : hn_launch<T, R, 4, 2, kBackward>(a, dgain, stream);
@@ -454,6 +784,7 @@ int hn_prepare(HnArgs<T, R>& a, const R* const* x, const int64_t* strides, const
     a.slots += a.L.n[f] == 0 ? a.L.a[f] / 2 : a.L.a[f];
     a.numbers += a.L.a[f] * (a.L.n[f] == 0 ? 1 : 2);
   }
+  a.share = 1.0 / a.numbers;
   a.axes = a.slots > 0 ? (int)axes : 0;
   a.normalise = normalise != 0;
   a.n_rows = n_rows;

@@ -1,15 +1,17 @@
 """The norm and rotation of rows of heads (nn/head_norm.py) against its formulas and
 their derivatives written out in float64.
 
-Tolerances follow the roundings, in half steps (eps / 2).  xhat: the sum is formed
-in double, so 1 / sqrt is off by one and x / sqrt by two more; the gain's product by
-one; the angle's fraction of a turn by 2^-26 of a turn in float (1.6 half steps of a
-radian), its sine and cosine by two steps (4), the turned pair by three: 16 half steps of
-what the pair's terms sum to.  An angle in double is off by 2^-52 (axes + 3) of the sum
-of its terms' absolute values.  Backward: d as the pair above, t = gain d by one more,
-mean(t xhat) by 20 of mean |t xhat|, dx by 24 of its terms' absolute sum; a gain's
-gradient by 20 of each term and one an addition, of which there are one a node and head.
-A result held in bfloat16 is off by another eps / 2 = 2^-8 of its value.
+Tolerances follow the roundings, in half steps (eps / 2).  A lane adds up to 24 squares in
+two sums (12 additions and the last: 13), the head in double: 1 / sqrt is off by 6.5 and
+its own rounding, 7; xhat by 8, gain xhat by 9; the angle's fraction of a turn by 2^-26 of
+a turn in float (1.6 half steps of a radian), its sine and cosine by two steps (4), the
+turned pair by three: 18 half steps of what the pair's terms sum to.  An angle in double is
+off by 2^-52 (axes + 3) of the sum of its terms' absolute values.  Backward: d as a pair
+alone, 8.6, t = gain d by one more, mean(t xhat) by 9.6 + 13 (its sum) + 7 + 1 = 31 of mean
+|t xhat|, dx by 8 + 31 + 2 (product, difference) + 8 (1 / sqrt and its product) = 49, 50 of
+its terms' absolute sum; a gain's gradient by 8.6 + 8 + 1, 20 of each term, and one an
+addition, of which there are one a node and head.  A result held in bfloat16 is off by
+another eps / 2 = 2^-8 of its value.
 """
 
 import copy
@@ -79,20 +81,20 @@ def oracle(x, gain, dy, copies, heads, eps_norm, positions, frequencies, eps):
                 za, da = sum(v.abs() for v in z), sum(v.abs() for v in d)
             for i, c in enumerate(cols):
                 y[:, c] = z[i]
-                ty[:, c] = (16 * half + off) * za
+                ty[:, c] = (18 * half + off) * za
                 t = g[us[i]] * d[i]
                 dgain[us[i]] += (d[i] * hat[i]).sum()
                 tg[us[i]] += ((20 * half + off) * da * hat[i].abs()).sum() + \
                     half * 2 * n * heads * (da * hat[i].abs()).sum()
                 mean += t * hat[i]
-                size += (1 + off / (20 * half)) * g[us[i]].abs() * da * hat[i].abs()
-                back.append((c, t, hat[i], g[us[i]].abs() * da * (1 + off / (24 * half))))
+                size += (1 + off / (31 * half)) * g[us[i]].abs() * da * hat[i].abs()
+                back.append((c, t, hat[i], g[us[i]].abs() * da * (1 + off / (50 * half))))
         for c, t, hat, ta in back:
             if eps_norm is None:
-                dx[:, c], tx[:, c] = t, 24 * half * ta
+                dx[:, c], tx[:, c] = t, 50 * half * ta
             else:
                 dx[:, c] = inv * (t - hat * mean / numbers)
-                tx[:, c] = 24 * half * inv * (ta + hat.abs() * size / numbers)
+                tx[:, c] = 50 * half * inv * (ta + hat.abs() * size / numbers)
     return {"y": (y, ty), "dx": (dx, tx), "dgain": (dgain, tg)}
 
 
