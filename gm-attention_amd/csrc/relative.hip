@@ -295,6 +295,30 @@ __global__ __launch_bounds__(256) void relative_scores(RelScores<T> a, uint32_t 
   }
 }
 
+// ------------------------------------------------------------------- repack
+// Rows of heads from one layout into another of the same heads with more or fewer copies: what is missing is zero, what
+// is over is left out.  A workgroup finds its columns once and takes rows until none is left.
+
+template <typename R>
+__global__ __launch_bounds__(256) void relative_repack(HeadsLayout from, HeadsLayout to, const R* src, int64_t n_rows,
+                                                       R* dst) {
+  __shared__ int place[GM_ATTN_MAX_D];
+  for (int c = threadIdx.x; c < to.D; c += blockDim.x) {
+    int f = 0;
+    for (int i = 1; i < to.F; ++i)
+      if (c >= to.off[i]) f = i;
+    const int dim = to.n[f] == 0 ? 1 : 2, local = c - to.off[f], h = local / (to.a[f] * dim);
+    const int at = local - h * to.a[f] * dim;
+    place[c] = -1;
+    for (int i = 0; i < from.F; ++i)
+      if (from.n[i] == to.n[f] && at < from.a[i] * dim) place[c] = from.off[i] + h * from.a[i] * dim + at;
+  }
+  __syncthreads();
+  for (int64_t row = blockIdx.x; row < n_rows; row += gridDim.x)
+    for (int c = threadIdx.x; c < to.D; c += blockDim.x)
+      dst[row * to.D + c] = place[c] < 0 ? R(0) : src[row * from.D + place[c]];
+}
+
 // ------------------------------------------------------------------- launch
 
 int rel_parse(const int64_t* desc, int64_t F, int64_t H, int64_t D, int64_t orders, RelLayout& L) {
@@ -455,8 +479,46 @@ int relative_backward(const T* g, const T* alpha, const R* q, const R* k, const 
   return check_launch("relative_backward");
 }
 
+template <typename R>
+int relative_repack_rows(const R* src, const int64_t* desc, int64_t F, int64_t D, const int64_t* to_desc, int64_t to_F,
+                         int64_t to_D, int64_t H, int64_t n_rows, R* dst, void* stream) {
+  HeadsLayout from, to;
+  int rc = parse_heads(desc, F, H, GM_ATTN_MAX_H, D, from);
+  if (rc == GM_OK) rc = parse_heads(to_desc, to_F, H, GM_ATTN_MAX_H, to_D, to);
+  if (rc != GM_OK) return rc;
+  GM_REQUIRE(n_rows >= 0, "sizes must be non-negative");
+  if (n_rows == 0) return GM_OK;
+  GM_REQUIRE(src && dst, "src and dst must be device pointers");
+  hipLaunchKernelGGL(relative_repack<R>, dim3((unsigned)std::min<int64_t>(n_rows, 4096)), dim3(256), 0,
+                     (hipStream_t)stream, from, to, src, n_rows, dst);
+  return check_launch("relative_repack");
+}
+
 }  // namespace
 }  // namespace gm
+
+extern "C" int gm_relative_padded(const int64_t* desc, int64_t F, int64_t H, int64_t D, int64_t orders,
+                                  int64_t* copies) {
+  GM_REQUIRE(copies, "copies must be a host array of three");
+  gm::RelLayout L{};
+  const int rc = gm::rel_parse(desc, F, H, D, orders, L);
+  if (rc != GM_OK) return rc;
+  int found[3] = {0, 0, 0};
+  (void)gm::rel_padded(L, found);
+  for (int n = 0; n < 3; ++n) copies[n] = found[n];
+  return GM_OK;
+}
+
+extern "C" int gm_relative_repack_f32(const float* src, const int64_t* desc, int64_t F, int64_t D,
+                                      const int64_t* to_desc, int64_t to_F, int64_t to_D, int64_t H, int64_t n_rows,
+                                      float* dst, void* stream) {
+  return gm::relative_repack_rows(src, desc, F, D, to_desc, to_F, to_D, H, n_rows, dst, stream);
+}
+extern "C" int gm_relative_repack_bf16(const uint16_t* src, const int64_t* desc, int64_t F, int64_t D,
+                                       const int64_t* to_desc, int64_t to_F, int64_t to_D, int64_t H, int64_t n_rows,
+                                       uint16_t* dst, void* stream) {
+  return gm::relative_repack_rows(src, desc, F, D, to_desc, to_F, to_D, H, n_rows, dst, stream);
+}
 
 extern "C" int64_t gm_relative_partial_rows(void) { return gm::kRelTableRows; }
 

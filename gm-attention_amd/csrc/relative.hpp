@@ -73,6 +73,9 @@ enum class RelPass { Forward, BackwardTarget, BackwardSource };
 // the layout.
 int rel_slots(const RelLayout& L);
 
+// A head's copies (of orders 0, 1, 2) filled up to a layout that the lane kernels serve, or false.
+bool rel_padded(const RelLayout& L, int (&copies)[3]);
+
 int rel_launch_units(RelPass pass, const RelArgs<float, float>& a, const RelRows& rows, hipStream_t stream);
 int rel_launch_units(RelPass pass, const RelArgs<float, uint16_t>& a, const RelRows& rows, hipStream_t stream);
 

@@ -121,6 +121,9 @@ SIGNATURES_F32 = {
        for sfx in ("f32", "f64", "bf16")},
     "gm_relative_partial_rows": (ctypes.c_int64, []),
     "gm_relative_slots": (ctypes.c_int, [_P] + [_I] * 4 + [_P]),
+    "gm_relative_padded": (ctypes.c_int, [_P] + [_I] * 4 + [_P]),
+    **{f"gm_relative_repack_{sfx}": (ctypes.c_int, [_P] * 2 + [_I] * 2 + [_P] + [_I] * 4 + [_P] * 2)
+       for sfx in ("f32", "bf16")},
     **{f"gm_relative_forward_{sfx}": (ctypes.c_int, [_P] * 8 + [_I] * 8 + [_D] + [_P] * 2)
        for sfx in ("f32", "f64", "bf16")},
     **{f"gm_relative_backward_{sfx}": (ctypes.c_int, [_P] * 14 + [_I] * 8 + [_D] + [_P] * 6)
@@ -1737,11 +1740,32 @@ def relative_slots(desc: Tensor, D: int, orders: int, H: int) -> int:
     return int(slots.value)
 
 
+def relative_padded(desc: Tensor, D: int, orders: int, H: int) -> dict[int, int]:
+    """A head's copies filled up to a layout that the lane kernels serve, ``{}`` where there is none."""
+    copies = (ctypes.c_int64 * 3)()
+    _call("gm_relative_padded", desc.data_ptr(), desc.shape[0], H, D, orders, ctypes.addressof(copies))
+    return {n: c for n, c in enumerate(copies) if c}
+
+
+def relative_repack(rows: Tensor, heads: Any, to: Any) -> Tensor:
+    """Rows of ``heads`` in the layout of ``to``: copies it has not are left out, others are zero."""
+    if rows.shape[1] != heads.plan.width or not rows.is_contiguous() or heads.heads != to.heads:
+        raise RuntimeError("rows must be contiguous, of the heads' width")
+    out = torch.empty(rows.shape[0], to.plan.width, dtype=rows.dtype, device=rows.device)
+    _call_on(rows.device, "gm_relative_repack_" + _PW_SUFFIX[rows.dtype], _ptr(rows), heads.desc.data_ptr(),
+             heads.desc.shape[0], heads.plan.width, to.desc.data_ptr(), to.desc.shape[0], to.plan.width, heads.heads,
+             rows.shape[0], _ptr(out), _stream(rows.device))
+    return out
+
+
 def relative_forward(q: Tensor, k: Tensor, table: Tensor, tables: Any, heads: Any, scale: float) -> Tensor:
     """``alpha (n_edges, H)``: the weights under the learned bias ``table (n_buckets, H)``.  The rows are whole
     (contiguous, at multiples of 16 bytes) and match the tables: nn.relative's checks."""
-    H, desc, device = heads.heads, heads.desc, q.device
-    order, counts = tables.target_rows(heads.slots(tables))
+    served = heads.served(tables)
+    if served is not heads:
+        q, k = relative_repack(q, heads, served), relative_repack(k, heads, served)
+    H, desc, device = served.heads, served.desc, q.device
+    order, counts = tables.target_rows(served.slots(tables))
     tables.found()
     alpha = torch.empty(tables.n_edges, H, dtype=tables.dtype, device=device)
     _call_on(device, "gm_relative_forward_" + _PW_SUFFIX[q.dtype], _ptr(q), _ptr(k), _ptr(table),
@@ -1755,9 +1779,12 @@ def relative_backward(g: Tensor, alpha: Tensor, q: Tensor, k: Tensor, tables: An
                       scale: float) -> tuple[Tensor, Tensor, Tensor]:
     """``(dq, dk, dtable)`` of what a forward took and gave and the weights' gradient (contiguous): the rows'
     gradients in their dtype, the learned table's in the tables'; sums in a fixed order."""
-    H, desc, slots, device = heads.heads, heads.desc, heads.slots(tables), q.device
+    served = heads.served(tables)
+    H, desc, slots, device = served.heads, served.desc, served.slots(tables), q.device
     if g.dtype != tables.dtype or g.shape != (tables.n_edges, H) or not g.is_contiguous() or g.device != device:
         raise RuntimeError("g must be contiguous (n_edges, H) in the tables' dtype")
+    if served is not heads:
+        q, k = relative_repack(q, heads, served), relative_repack(k, heads, served)
     src_ptr, records_s = tables.group_sources()
     (order, counts), (order_s, counts_s) = tables.target_rows(slots), tables.source_rows(slots)
     tables.found()
@@ -1769,8 +1796,10 @@ def relative_backward(g: Tensor, alpha: Tensor, q: Tensor, k: Tensor, tables: An
     _call_on(device, "gm_relative_backward_" + _PW_SUFFIX[q.dtype], _ptr(g), _ptr(alpha), _ptr(q), _ptr(k),
              _ptr(tables.records), _ptr(records_s), _ptr(tables.buckets), desc.data_ptr(), _ptr(tables.row_ptr),
              _ptr(src_ptr), _ptr(order), counts, _ptr(order_s), counts_s, tables.n_targets, tables.n_sources,
-             tables.n_edges, q.shape[1], tables.orders, desc.shape[0], H, tables.n_buckets, scale, _ptr(ds), _ptr(partial), _ptr(dq), _ptr(dk),
-             _ptr(dtable), _stream(device))
+             tables.n_edges, q.shape[1], tables.orders, desc.shape[0], H, tables.n_buckets, scale, _ptr(ds),
+             _ptr(partial), _ptr(dq), _ptr(dk), _ptr(dtable), _stream(device))
+    if served is not heads:
+        dq, dk = relative_repack(dq, served, heads), relative_repack(dk, served, heads)
     return dq, dk, dtable
 
 

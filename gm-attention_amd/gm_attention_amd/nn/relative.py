@@ -117,6 +117,19 @@ class Heads:
         # read on the host, whatever the default device of the call that makes the (kept) heads
         self.desc = torch.tensor([list(row) for row in self.plan.rows], dtype=torch.int64, device="cpu")
         self._slots: dict[int, int] = {}
+        self._served: dict[tuple[int, torch.dtype], Heads] = {}
+
+    def served(self, tables: EdgeTables) -> Heads:
+        """The heads as the kernels take them: these, or with copies of zeros where that gives the lane kernels
+        whole units (rows are repacked: little beside an edge set's many edges a row)."""
+        held = self._served.get((tables.orders, tables.dtype))
+        if held is None:
+            held = self
+            if tables.dtype != torch.float64 and not self.slots(tables):
+                copies = _native.relative_padded(self.desc, self.plan.width, tables.orders, self.heads)
+                held = heads_of(SO2FieldType(copies), self.heads) if copies else self
+            self._served[tables.orders, tables.dtype] = held
+        return held
 
     def slots(self, tables: EdgeTables) -> int:
         """Edge slots of a wave of the lane kernels (0: the simple kernels serve)."""
@@ -141,7 +154,7 @@ class RelativeSoftmax(torch.autograd.Function):
                 train: bool) -> Tensor:
         if train:  # found here: the backward runs on a thread and perhaps a stream of its own
             tables.group_sources()
-            tables.source_rows(heads.slots(tables))
+            tables.source_rows(heads.served(tables).slots(tables))
         with _native.span("gm::attention/relative_softmax"):
             alpha = _native.relative_forward(q, k, table, tables, heads, scale)
         if train:

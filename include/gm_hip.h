@@ -359,6 +359,14 @@ int gm_differential_backward_bf16(const float* g, const uint16_t* q, const uint1
 int64_t gm_relative_partial_rows(void);
 /* *slots (HOST): the edges a wave of the lane kernels takes at once, S, or 0 where they do not serve the layout. */
 int gm_relative_slots(const int64_t* desc, int64_t F, int64_t H, int64_t D, int64_t orders, int64_t* slots);
+/* copies (HOST, three): a head's copies of orders 0, 1, 2 filled up with zeros to a layout that the lane kernels serve
+ * with tables of as many orders, zeros where there is none; gm_relative_repack_* moves rows (n_rows, D) of the same H
+ * heads from one layout into another (missing copies zero, those over left out). */
+int gm_relative_padded(const int64_t* desc, int64_t F, int64_t H, int64_t D, int64_t orders, int64_t* copies);
+int gm_relative_repack_f32(const float* src, const int64_t* desc, int64_t F, int64_t D, const int64_t* to_desc,
+                           int64_t to_F, int64_t to_D, int64_t H, int64_t n_rows, float* dst, void* stream);
+int gm_relative_repack_bf16(const uint16_t* src, const int64_t* desc, int64_t F, int64_t D, const int64_t* to_desc,
+                            int64_t to_F, int64_t to_D, int64_t H, int64_t n_rows, uint16_t* dst, void* stream);
 int gm_relative_forward_f32(const float* q, const float* k, const float* table, const float* records, const int64_t*
                             desc, const int64_t* row_ptr, const int32_t* order, const int64_t* counts, int64_t
                             n_targets, int64_t n_sources, int64_t n_edges, int64_t D, int64_t orders, int64_t F, int64_t

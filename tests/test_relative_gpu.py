@@ -662,6 +662,43 @@ def test_refusals():
         relative_softmax(q, q, table, EdgeTables(row_ptr, source, phases, bias, inside), head, 2)
 
 
+@pytest.mark.parametrize("copies,heads,orders,padded", [
+    ({0: 4, 1: 4, 2: 4}, 8, 3, None), ({0: 3, 1: 2, 2: 1}, 6, 3, {0: 4, 1: 2, 2: 1}), ({0: 12}, 8, 1, {0: 16}),
+    ({0: 5, 1: 3, 2: 3}, 7, 3, {0: 8, 1: 4, 2: 4}), ({0: 4, 1: 4}, 4, 3, {0: 8, 1: 4, 2: 2}),
+    ({2: 4}, 4, 3, {1: 4, 2: 4}), ({0: 2, 3: 2}, 4, 4, None), ({0: 4, 1: 4}, 4, 4, None), ({0: 1024}, 1, 1, None)])
+def test_layouts_filled_up_to_whole_units(copies, heads, orders, padded):
+    """The layout that the lane kernels take in a layout's place, or the simple kernels with the layout itself."""
+    phases = torch.zeros(1, orders, 2)
+    tables = RelativeEdgeTables(torch.tensor([0, 1]), torch.tensor([0]), phases, torch.zeros(1),
+                                torch.ones(1, dtype=torch.uint8), torch.zeros(1, dtype=torch.uint8), 1)
+    given = relative.heads_of(SO2FieldType(copies), heads)
+    served = given.served(tables)
+    if padded is None:
+        assert served is given
+    else:
+        assert served is relative.heads_of(SO2FieldType(padded), heads) and served.slots(tables) > 0
+        assert given.slots(tables) == 0
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("rows", [torch.float32, torch.bfloat16])
+def test_rows_are_repacked_as_they_are(rows, cuda):
+    from gm_attention_amd import _native
+
+    heads = 5
+    small, large = (relative.heads_of(SO2FieldType(c), heads) for c in ({0: 3, 2: 1}, {0: 4, 1: 2, 2: 2}))
+    x = problems.normal((7001, small.plan.width), 1).to(rows).to(cuda)
+    big = _native.relative_repack(x, small, large)
+    want = torch.zeros(7001, 60, dtype=rows, device=cuda)
+    for h in range(heads):
+        want[:, 4 * h:4 * h + 3] = x[:, 3 * h:3 * h + 3]
+        want[:, 40 + 4 * h:42 + 4 * h] = x[:, 15 + 2 * h:17 + 2 * h]
+    assert torch.equal(big, want)
+    assert torch.equal(_native.relative_repack(big, large, small), x)
+    with pytest.raises(RuntimeError, match="rows must be contiguous"):
+        _native.relative_repack(x, large, small)
+
+
 def test_the_library_refuses_bad_arguments():
     """Through the C interface, before anything is launched (no GPU touched)."""
     import ctypes
