@@ -335,7 +335,11 @@ __global__ __launch_bounds__(kRelThreadsB) void relative_rows_units(RelArgs<floa
           d[n] = ds_of[(uint32_t)((in[n] ? (t + n) * w.slots + s : 0) * H + h)];
           U::template load<kNear>(a.k, w, unit, __float_as_int(head[n].x) & 0xFFFFFF, x[n]);
         } else {
-          d[n] = a.ds[(int64_t)__float_as_int(head[n].y) * H + h];
+          if constexpr (kNear)  // as the rows': a 32-bit offset from a scalar address
+            d[n] = *reinterpret_cast<const float*>(reinterpret_cast<const char*>(a.ds) +
+                                                   (__float_as_uint(head[n].y) * (uint32_t)(4 * H) + 4u * (uint32_t)h));
+          else
+            d[n] = a.ds[(int64_t)__float_as_int(head[n].y) * H + h];
           U::template load<kNear>(a.q, w, unit, __float_as_int(head[n].x), x[n]);
         }
       }
@@ -472,7 +476,7 @@ int rel_launch_any(RelPass pass, const RelArgs<float, R>& a, const RelRows& rows
   w.row_bytes = (uint32_t)(a.L.D * sizeof(R));
   w.order = rows.order;
   const int64_t nodes = std::max(a.n_targets, a.n_sources), limit = int64_t(1) << 32;
-  const bool near = nodes <= (int64_t(1) << 24) && nodes * w.row_bytes < limit;
+  const bool near = nodes <= (int64_t(1) << 24) && nodes * w.row_bytes < limit && a.n_edges * a.L.H * 4 < limit;
   switch (shape) {
     case 0: return rel_launch_shape<R, 4, 2, 2>(pass, a, w, rows, near, stream);
     case 1: return rel_launch_shape<R, 4, 2, 1>(pass, a, w, rows, near, stream);

@@ -1754,7 +1754,7 @@ def relative_repack(rows: Tensor, heads: Any, to: Any) -> Tensor:
     out = torch.empty(rows.shape[0], to.plan.width, dtype=rows.dtype, device=rows.device)
     _call_on(rows.device, "gm_relative_repack_" + _PW_SUFFIX[rows.dtype], _ptr(rows), heads.desc.data_ptr(),
              heads.desc.shape[0], heads.plan.width, to.desc.data_ptr(), to.desc.shape[0], to.plan.width, heads.heads,
-             rows.shape[0], _ptr(out), _stream(rows.device))
+             rows.shape[0], _ptr(out), stream_handle(rows.device))
     return out
 
 
@@ -1771,7 +1771,7 @@ def relative_forward(q: Tensor, k: Tensor, table: Tensor, tables: Any, heads: An
     _call_on(device, "gm_relative_forward_" + _PW_SUFFIX[q.dtype], _ptr(q), _ptr(k), _ptr(table),
              _ptr(tables.records), desc.data_ptr(), _ptr(tables.row_ptr), _ptr(order), counts, tables.n_targets,
              tables.n_sources, tables.n_edges, q.shape[1], tables.orders, desc.shape[0], H, tables.n_buckets, scale,
-             _ptr(alpha), _stream(device))
+             _ptr(alpha), stream_handle(device))
     return alpha
 
 
@@ -1797,7 +1797,7 @@ def relative_backward(g: Tensor, alpha: Tensor, q: Tensor, k: Tensor, tables: An
              _ptr(tables.records), _ptr(records_s), _ptr(tables.buckets), desc.data_ptr(), _ptr(tables.row_ptr),
              _ptr(src_ptr), _ptr(order), counts, _ptr(order_s), counts_s, tables.n_targets, tables.n_sources,
              tables.n_edges, q.shape[1], tables.orders, desc.shape[0], H, tables.n_buckets, scale, _ptr(ds),
-             _ptr(partial), _ptr(dq), _ptr(dk), _ptr(dtable), _stream(device))
+             _ptr(partial), _ptr(dq), _ptr(dk), _ptr(dtable), stream_handle(device))
     if served is not heads:
         dq, dk = relative_repack(dq, served, heads), relative_repack(dk, served, heads)
     return dq, dk, dtable
@@ -1841,7 +1841,7 @@ def head_norm_forward(rows: Sequence[Tensor], gains: Sequence[Tensor | None], la
              _STRIDES(*[x.stride(0) for x in rows]), _addresses(gains), len(rows), desc.data_ptr(), n, layout.width,
              desc.shape[0], layout.heads, None if positions is None else _ptr(positions),
              None if frequencies is None else _ptr(frequencies), 0 if frequencies is None else frequencies.shape[0],
-             int(eps is not None), 1.0 if eps is None else eps, _addresses(out), _stream(device))
+             int(eps is not None), 1.0 if eps is None else eps, _addresses(out), stream_handle(device))
     return out
 
 
@@ -1869,5 +1869,5 @@ def head_norm_backward(grads: Sequence[Tensor], rows: Sequence[Tensor], gains: S
              desc.shape[0], layout.heads, None if positions is None else _ptr(positions),
              None if frequencies is None else _ptr(frequencies), 0 if frequencies is None else frequencies.shape[0],
              int(eps is not None), 1.0 if eps is None else eps, _addresses(dx), _ptr(partial), _ptr(dgain),
-             _stream(device))
+             stream_handle(device))
     return dx, [None] * sets if dgain is None else list(dgain.unbind(0))
