@@ -357,12 +357,10 @@ int rel_prepare(RelArgs<T, R>& a, const T* records, const int64_t* desc, const i
   return GM_OK;
 }
 
-// The rows' classes (order null: the simple kernels), which the lane kernels must serve.
-template <typename T, typename R>
-int rel_rows(const RelArgs<T, R>& a, const int32_t* order, const int64_t* counts, int64_t n, RelRows& rows) {
+// The rows' classes; order null: none.
+int rel_rows(const int32_t* order, const int64_t* counts, int64_t n, RelRows& rows) {
   rows = RelRows{order, {0, 0, 0}};
   if (!order) return GM_OK;
-  GM_REQUIRE((std::is_same<T, float>::value) && rel_slots(a.L) > 0, "the lane kernels do not serve this layout");
   GM_REQUIRE(counts, "the classes' counts (a host array of three) are required");
   int64_t sum = 0;
   for (int c = 0; c < 3; ++c) {
@@ -371,17 +369,24 @@ int rel_rows(const RelArgs<T, R>& a, const int32_t* order, const int64_t* counts
     sum += counts[c];
   }
   GM_REQUIRE(sum == n, "the classes must hold every row once");
-  GM_REQUIRE(aligned(a.q, 16) && aligned(a.k, 16) && aligned(a.dq, 16) && aligned(a.dk, 16) && aligned(a.records, 8) &&
-                 aligned(a.records_s, 8),
-             "the lane kernels take rows at multiples of 16 bytes, records of 8");
+  return GM_OK;
+}
+
+// Whether the lane kernels can run: they serve the layout, and the addresses are whole.
+template <typename T, typename R>
+int rel_lanes_check(const RelArgs<T, R>& a) {
+  GM_REQUIRE((std::is_same<T, float>::value) && rel_slots(a.L) > 0, "the lane kernels do not serve this layout");
+  GM_REQUIRE(aligned(a.q, 16) && aligned(a.k, 16) && aligned(a.dq, 16) && aligned(a.dk, 16) && aligned(a.pairs, 8) &&
+                 aligned(a.pairs_s, 8),
+             "the lane kernels take rows at multiples of 16 bytes, entries of 8");
   return GM_OK;
 }
 
 template <typename T, typename R>
 int relative_forward(const R* q, const R* k, const T* table, const T* records, const int64_t* desc,
-                     const int64_t* row_ptr, const int32_t* order, const int64_t* counts, int64_t n_targets,
-                     int64_t n_sources, int64_t n_edges, int64_t D, int64_t orders, int64_t F, int64_t H,
-                     int64_t buckets, double scale, T* alpha, void* stream) {
+                     const int64_t* row_ptr, const float* pairs, const int64_t* pair_ptr, const int32_t* order,
+                     const int64_t* counts, int64_t n_targets, int64_t n_sources, int64_t n_edges, int64_t D,
+                     int64_t orders, int64_t F, int64_t H, int64_t buckets, double scale, T* alpha, void* stream) {
   RelArgs<T, R> a{};
   const int rc = rel_prepare(a, records, desc, row_ptr, n_targets, n_sources, n_edges, D, orders, F, H, buckets, scale,
                              q, k);
@@ -390,12 +395,18 @@ int relative_forward(const R* q, const R* k, const T* table, const T* records, c
   GM_REQUIRE(alpha && table, "alpha and table must be device pointers");
   a.alpha = alpha;
   a.table = table;
-  RelRows rows;
-  const int status = rel_rows(a, order, counts, n_targets, rows);
-  if (status != GM_OK) return status;
   if constexpr (std::is_same<T, float>::value) {
-    if (order) return rel_launch_units(RelPass::Forward, a, rows, (hipStream_t)stream);
+    if (pairs) {
+      a.pairs = pairs;
+      a.pair_ptr = pair_ptr;
+      GM_REQUIRE(pair_ptr && order, "the pairs' offsets and classes must be device pointers");
+      RelRows rows;
+      int status = rel_lanes_check(a);
+      if (status == GM_OK) status = rel_rows(order, counts, (n_targets + 1) / 2, rows);
+      return status == GM_OK ? rel_launch_units(RelPass::Forward, a, rows, (hipStream_t)stream) : status;
+    }
   }
+  GM_REQUIRE(!pairs, "the lane kernels take float tables");
   hipLaunchKernelGGL((relative_forward_simple<T, R>), dim3((unsigned)blocks_for(n_targets)), dim3(256), 0,
                      (hipStream_t)stream, a);
   return check_launch("relative_forward");
@@ -438,18 +449,24 @@ int relative_scores_launch(const RelArgs<T, R>& a, const RelRows& rows, const ui
 template <typename T, typename R>
 int relative_backward(const T* g, const T* alpha, const R* q, const R* k, const T* records, const T* records_s,
                       const uint8_t* bucket, const int64_t* desc, const int64_t* row_ptr, const int64_t* src_ptr,
-                      const int32_t* order, const int64_t* counts, const int32_t* order_s, const int64_t* counts_s, int64_t n_targets,
-                      int64_t n_sources, int64_t n_edges, int64_t D, int64_t orders, int64_t F, int64_t H,
-                      int64_t buckets, double scale, T* ds, T* partial, R* dq, R* dk, T* dtable, void* stream) {
+                      const int32_t* order, const int64_t* counts, const float* pairs, const int64_t* pair_ptr,
+                      const int32_t* pair_order, const int64_t* pair_counts, const float* pairs_s,
+                      const int64_t* pair_ptr_s, const int32_t* pair_order_s, const int64_t* pair_counts_s,
+                      int64_t n_targets, int64_t n_sources, int64_t n_edges, int64_t D, int64_t orders, int64_t F,
+                      int64_t H, int64_t buckets, double scale, T* ds, T* partial, R* dq, R* dk, T* dtable,
+                      void* stream) {
   RelArgs<T, R> a{};
   const int rc = rel_prepare(a, records, desc, row_ptr, n_targets, n_sources, n_edges, D, orders, F, H, buckets, scale,
                              q, k);
   if (rc != GM_OK) return rc;
   GM_REQUIRE(partial && dtable, "partial and dtable must be device pointers");
   if (n_targets > 0) GM_REQUIRE(dq, "dq must be a device pointer");
-  if (n_sources > 0) GM_REQUIRE(src_ptr && dk, "src_ptr and dk must be device pointers");
-  if (n_edges > 0) GM_REQUIRE(g && alpha && ds && records_s && bucket,
-                              "g, alpha, ds, the sources' records and the buckets must be device pointers");
+  if (n_sources > 0) GM_REQUIRE(dk, "dk must be a device pointer");
+  const bool lanes = pairs && pairs_s;
+  GM_REQUIRE(!pairs == !pairs_s, "both sides' pairs, or neither's");
+  if (n_edges > 0) GM_REQUIRE(g && alpha && ds && bucket, "g, alpha, ds and the buckets must be device pointers");
+  if (n_edges > 0 && !lanes) GM_REQUIRE(records_s, "the sources' records must be a device pointer");
+  if (n_sources > 0 && !lanes) GM_REQUIRE(src_ptr, "src_ptr must be a device pointer");
   a.g = g;
   a.alpha = const_cast<T*>(alpha);  // read only here
   a.records_s = records_s;
@@ -459,19 +476,30 @@ int relative_backward(const T* g, const T* alpha, const R* q, const R* k, const 
   a.dq = dq;
   a.dk = dk;
   const hipStream_t s = (hipStream_t)stream;
-  GM_REQUIRE(!order == !order_s || n_targets == 0 || n_sources == 0, "both sides' rows are in classes, or neither's");
-  RelRows targets, sources;
-  int status = rel_rows(a, order, counts, n_targets, targets);
-  if (status == GM_OK) status = rel_rows(a, order_s, counts_s, n_sources, sources);
-  if (status != GM_OK) return status;
-  status = relative_scores_launch(a, targets, bucket, dtable, s);
+  RelRows targets;
+  int status = rel_rows(order, counts, n_targets, targets);
   if (status != GM_OK) return status;
   if constexpr (std::is_same<T, float>::value) {
-    if (order || order_s) {
-      status = rel_launch_units(RelPass::BackwardTarget, a, targets, s);
-      return status == GM_OK ? rel_launch_units(RelPass::BackwardSource, a, sources, s) : status;
+    if (lanes) {
+      if (n_targets > 0) GM_REQUIRE(pair_ptr && pair_order, "the pairs' offsets and classes must be device pointers");
+      if (n_sources > 0)
+        GM_REQUIRE(pair_ptr_s && pair_order_s, "the pairs' offsets and classes must be device pointers");
+      a.pairs = pairs;
+      a.pair_ptr = pair_ptr;
+      a.pairs_s = pairs_s;
+      a.pair_ptr_s = pair_ptr_s;
+      RelRows rows, rows_s;
+      status = rel_lanes_check(a);
+      if (status == GM_OK) status = rel_rows(pair_order, pair_counts, (n_targets + 1) / 2, rows);
+      if (status == GM_OK) status = rel_rows(pair_order_s, pair_counts_s, (n_sources + 1) / 2, rows_s);
+      if (status == GM_OK) status = relative_scores_launch(a, targets, bucket, dtable, s);
+      if (status == GM_OK) status = rel_launch_units(RelPass::BackwardTarget, a, rows, s);
+      return status == GM_OK ? rel_launch_units(RelPass::BackwardSource, a, rows_s, s) : status;
     }
   }
+  GM_REQUIRE(!lanes, "the lane kernels take float tables");
+  status = relative_scores_launch(a, targets, bucket, dtable, s);
+  if (status != GM_OK) return status;
   if (n_targets > 0)
     hipLaunchKernelGGL((relative_rows_simple<T, R, true>), dim3((unsigned)blocks_for(n_targets)), dim3(256), 0, s, a);
   if (n_sources > 0)
@@ -536,20 +564,24 @@ extern "C" int gm_relative_slots(const int64_t* desc, int64_t F, int64_t H, int6
 #define GM_RELATIVE_ENTRY(SFX, T, R)                                                                                  \
   extern "C" int gm_relative_forward_##SFX(                                                                           \
       const R* q, const R* k, const T* table, const T* records, const int64_t* desc, const int64_t* row_ptr,          \
-      const int32_t* order, const int64_t* counts, int64_t n_targets, int64_t n_sources, int64_t n_edges, int64_t D,  \
-      int64_t orders, int64_t F, int64_t H, int64_t buckets, double scale, T* alpha, void* stream) {                  \
-    return gm::relative_forward<T, R>(q, k, table, records, desc, row_ptr, order, counts, n_targets, n_sources,       \
-                                      n_edges, D, orders, F, H, buckets, scale, alpha, stream);                       \
+      const float* pairs, const int64_t* pair_ptr, const int32_t* order, const int64_t* counts, int64_t n_targets,    \
+      int64_t n_sources, int64_t n_edges, int64_t D, int64_t orders, int64_t F, int64_t H, int64_t buckets,           \
+      double scale, T* alpha, void* stream) {                                                                         \
+    return gm::relative_forward<T, R>(q, k, table, records, desc, row_ptr, pairs, pair_ptr, order, counts, n_targets, \
+                                      n_sources, n_edges, D, orders, F, H, buckets, scale, alpha, stream);            \
   }                                                                                                                   \
   extern "C" int gm_relative_backward_##SFX(                                                                          \
       const T* g, const T* alpha, const R* q, const R* k, const T* records, const T* records_s,                       \
       const uint8_t* bucket, const int64_t* desc, const int64_t* row_ptr, const int64_t* src_ptr,                     \
-      const int32_t* order, const int64_t* counts, const int32_t* order_s, const int64_t* counts_s, int64_t n_targets, int64_t n_sources, int64_t n_edges,         \
-      int64_t D, int64_t orders, int64_t F, int64_t H, int64_t buckets, double scale, T* ds, T* partial, R* dq,       \
-      R* dk, T* dtable, void* stream) {                                                                               \
-    return gm::relative_backward<T, R>(g, alpha, q, k, records, records_s, bucket, desc, row_ptr, src_ptr, order, counts,     \
-                                       order_s, counts_s, n_targets, n_sources, n_edges, D, orders, F, H, buckets,    \
-                                       scale, ds, partial, dq, dk, dtable, stream);                                   \
+      const int32_t* order, const int64_t* counts, const float* pairs, const int64_t* pair_ptr,                       \
+      const int32_t* pair_order, const int64_t* pair_counts, const float* pairs_s, const int64_t* pair_ptr_s,         \
+      const int32_t* pair_order_s, const int64_t* pair_counts_s, int64_t n_targets, int64_t n_sources,                \
+      int64_t n_edges, int64_t D, int64_t orders, int64_t F, int64_t H, int64_t buckets, double scale, T* ds,         \
+      T* partial, R* dq, R* dk, T* dtable, void* stream) {                                                            \
+    return gm::relative_backward<T, R>(g, alpha, q, k, records, records_s, bucket, desc, row_ptr, src_ptr, order,     \
+                                       counts, pairs, pair_ptr, pair_order, pair_counts, pairs_s, pair_ptr_s,         \
+                                       pair_order_s, pair_counts_s, n_targets, n_sources, n_edges, D, orders, F, H,   \
+                                       buckets, scale, ds, partial, dq, dk, dtable, stream);                          \
   }
 
 GM_RELATIVE_ENTRY(f32, float, float)

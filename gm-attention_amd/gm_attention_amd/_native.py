@@ -124,9 +124,9 @@ SIGNATURES_F32 = {
     "gm_relative_padded": (ctypes.c_int, [_P] + [_I] * 4 + [_P]),
     **{f"gm_relative_repack_{sfx}": (ctypes.c_int, [_P] * 2 + [_I] * 2 + [_P] + [_I] * 4 + [_P] * 2)
        for sfx in ("f32", "bf16")},
-    **{f"gm_relative_forward_{sfx}": (ctypes.c_int, [_P] * 8 + [_I] * 8 + [_D] + [_P] * 2)
+    **{f"gm_relative_forward_{sfx}": (ctypes.c_int, [_P] * 10 + [_I] * 8 + [_D] + [_P] * 2)
        for sfx in ("f32", "f64", "bf16")},
-    **{f"gm_relative_backward_{sfx}": (ctypes.c_int, [_P] * 14 + [_I] * 8 + [_D] + [_P] * 6)
+    **{f"gm_relative_backward_{sfx}": (ctypes.c_int, [_P] * 20 + [_I] * 8 + [_D] + [_P] * 6)
        for sfx in ("f32", "f64", "bf16")},
     "gm_head_norm_partial_rows": (ctypes.c_int64, [_I]),
     **{f"gm_head_norm_forward_{sfx}": (ctypes.c_int, [_P] * 3 + [_I, _P] + [_I] * 4 + [_P] * 2 + [_I] * 2 + [_D] +
@@ -1765,11 +1765,11 @@ def relative_forward(q: Tensor, k: Tensor, table: Tensor, tables: Any, heads: An
     if served is not heads:
         q, k = relative_repack(q, heads, served), relative_repack(k, heads, served)
     H, desc, device = served.heads, served.desc, q.device
-    order, counts = tables.target_rows(served.slots(tables))
+    pairs = tables.pairs("targets", served.slots(tables))
     tables.found()
     alpha = torch.empty(tables.n_edges, H, dtype=tables.dtype, device=device)
     _call_on(device, "gm_relative_forward_" + _PW_SUFFIX[q.dtype], _ptr(q), _ptr(k), _ptr(table),
-             _ptr(tables.records), desc.data_ptr(), _ptr(tables.row_ptr), _ptr(order), counts, tables.n_targets,
+             _ptr(tables.records), desc.data_ptr(), _ptr(tables.row_ptr), *pairs, tables.n_targets,
              tables.n_sources, tables.n_edges, q.shape[1], tables.orders, desc.shape[0], H, tables.n_buckets, scale,
              _ptr(alpha), stream_handle(device))
     return alpha
@@ -1785,8 +1785,9 @@ def relative_backward(g: Tensor, alpha: Tensor, q: Tensor, k: Tensor, tables: An
         raise RuntimeError("g must be contiguous (n_edges, H) in the tables' dtype")
     if served is not heads:
         q, k = relative_repack(q, heads, served), relative_repack(k, heads, served)
-    src_ptr, records_s = tables.group_sources()
-    (order, counts), (order_s, counts_s) = tables.target_rows(slots), tables.source_rows(slots)
+    src_ptr, records_s = tables.sources(slots)
+    order, counts = tables.target_rows(heads.score_slots)
+    pairs, pairs_s = tables.pairs("targets", slots), tables.pairs("sources", slots)
     tables.found()
     ds = torch.empty_like(g)
     partial = torch.empty(int(library().gm_relative_partial_rows()) * tables.n_buckets * H, dtype=g.dtype,
@@ -1795,7 +1796,7 @@ def relative_backward(g: Tensor, alpha: Tensor, q: Tensor, k: Tensor, tables: An
     dtable = torch.empty(tables.n_buckets, H, dtype=g.dtype, device=device)
     _call_on(device, "gm_relative_backward_" + _PW_SUFFIX[q.dtype], _ptr(g), _ptr(alpha), _ptr(q), _ptr(k),
              _ptr(tables.records), _ptr(records_s), _ptr(tables.buckets), desc.data_ptr(), _ptr(tables.row_ptr),
-             _ptr(src_ptr), _ptr(order), counts, _ptr(order_s), counts_s, tables.n_targets, tables.n_sources,
+             _ptr(src_ptr), _ptr(order), counts, *pairs, *pairs_s, tables.n_targets, tables.n_sources,
              tables.n_edges, q.shape[1], tables.orders, desc.shape[0], H, tables.n_buckets, scale, _ptr(ds),
              _ptr(partial), _ptr(dq), _ptr(dk), _ptr(dtable), stream_handle(device))
     if served is not heads:

@@ -51,7 +51,14 @@ def distance_buckets(distances: Tensor, cutoff: float, n_buckets: int) -> Tensor
 
 class RelativeEdgeTables(EdgeTables):
     """:class:`differential.EdgeTables` with every edge's bucket ``(n_edges,)``, whole
-    numbers in ``0 .. n_buckets - 1`` (checked here, once)."""
+    numbers in ``0 .. n_buckets - 1`` (checked here, once).
+
+    The lane kernels read pairs of neighbouring targets (and, in the backward, of
+    sources), each with the list of the nodes that either has an edge to: neighbours on
+    a grid share most of theirs, whose rows are then loaded once for both.  The lists
+    are found with a first call (:meth:`group_sources`: the sources'), outside a capture,
+    and kept: 56 bytes an entry at two orders and 48, of four entries for seven edges or
+    fewer on a grid."""
 
     def __init__(self, row_ptr: Tensor, source: Tensor, transport: Tensor, bias: Tensor, inside: Tensor,
                  buckets: Tensor, n_buckets: int, *, n_sources: int | None = None) -> None:
@@ -69,6 +76,7 @@ class RelativeEdgeTables(EdgeTables):
             raise ValueError(f"float32 tables hold at most {MAX_SOURCES} sources, got {nodes}.")
         self.n_buckets = int(n_buckets)
         self.buckets = buckets.detach().to(torch.uint8, copy=True)
+        self._pairs: dict[str, tuple[Tensor, Tensor]] = {}
         super().__init__(row_ptr, source, transport, bias, inside, n_sources=n_sources)
 
     def _hold(self, source: Tensor, phases: Tensor, masked: Tensor) -> None:
@@ -76,10 +84,88 @@ class RelativeEdgeTables(EdgeTables):
         if self.device.type == "cuda":
             self._kept.append(_native.Made(self.buckets))
 
+    def __getstate__(self) -> dict:
+        return {n: v for n, v in super().__getstate__().items() if n != "_pairs"}
+
     def __setstate__(self, state: dict) -> None:
+        self._pairs = {}
         super().__setstate__(state)
         if self.device.type == "cuda" and "records" in state:
             self._kept.append(_native.Made(self.buckets))
+
+    def group_sources(self) -> tuple[Tensor, Tensor]:
+        """What a backward reads of the sources' side: the pairs of sources, or for float64
+        tables the edges sorted by source; found once."""
+        return super().group_sources() if self.dtype == torch.float64 else self._paired("sources")
+
+    def sources(self, slots: int) -> tuple[Tensor | None, Tensor | None]:
+        """``(src_ptr, records_s)`` for the simple kernels (``slots`` 0)."""
+        return (None, None) if slots else super().group_sources()
+
+    def pairs(self, side: str, slots: int) -> tuple:
+        """The pairs of ``"targets"`` or ``"sources"`` as the entry points take them, for lane
+        kernels with ``slots`` edge slots a wave (0: none, the simple kernels)."""
+        if slots == 0:
+            return None, None, None, None
+        entries, ptr = self._paired(side)
+        # the classes are of 32 and 128 times their slots: of 16 and 64 steps
+        order, counts = self._rows((f"{side}' pairs", max(1, slots // 2)), lambda: ptr)
+        # an edge set without edges has entries of no pair, and an address all the same
+        return entries.data_ptr(), _native._ptr(ptr), _native._ptr(order), counts
+
+    def _paired(self, side: str) -> tuple[Tensor, Tensor]:
+        held = self._pairs.get(side)
+        if held is None:
+            with _native.LOCK:
+                held = self._pairs.get(side)
+                if held is None:
+                    held = self._pairs[side] = self._pair(side == "targets")
+        return held
+
+    def _pair(self, targets: bool) -> tuple[Tensor, Tensor]:
+        """``(entries, ptr)``: every pair's entries, in order of their nodes."""
+        differential._outside_capture(self.row_ptr, "RelativeEdgeTables' pairs (a first call with these tables)")
+        self.found()
+        target = torch.repeat_interleave(torch.arange(self.n_targets, device=self.device),
+                                         self.row_ptr[1:] - self.row_ptr[:-1], output_size=self.n_edges)
+        source = self._unpacked(self.records)
+        row, node, rows, nodes = ((target, source, self.n_targets, self.n_sources) if targets else
+                                  (source, target, self.n_sources, self.n_targets))
+        # by pair, node and row; edges of one row to one node stand apart
+        key, edge = torch.sort(((row >> 1) * nodes + node) * 2 + (row & 1), stable=True)
+        again = torch.zeros_like(key)
+        if self.n_edges > 1 and bool((key[1:] == key[:-1]).any()):
+            place = torch.arange(self.n_edges, device=self.device)
+            first = torch.ones_like(key, dtype=torch.bool)
+            first[1:] = key[1:] != key[:-1]
+            again = place - torch.cummax(torch.where(first, place, 0), 0).values
+            by = torch.sort(again, stable=True).indices
+            by = by[torch.sort(key[by] >> 1, stable=True).indices]
+            key, edge, again = key[by], edge[by], again[by]
+        second, key = key & 1, key >> 1
+        new = torch.ones_like(key, dtype=torch.bool)
+        new[1:] = (key[1:] != key[:-1]) | (again[1:] != again[:-1])
+        entry = torch.cumsum(new, 0) - 1
+        key = key[new]
+        n = key.shape[0]
+        ptr = torch.searchsorted(key // max(nodes, 1), torch.arange((rows + 1) // 2 + 1, device=self.device))
+        edges = torch.full((n, 2), -1, dtype=torch.int64, device=self.device)
+        edges.view(-1)[2 * entry + second] = edge
+        there, at = edges >= 0, edges.clamp_min(0)
+        head = 6 if targets else 4
+        entries = torch.zeros(max(n, 1), head + 4 * (self.orders - 1), dtype=torch.float32, device=self.device)
+        words, made = entries.view(torch.int32), entries[:n]
+        words[:n, 0] = key % max(nodes, 1)
+        words[:n, 2:4] = edges
+        mine = self.records[at]  # (n, 2, 2 orders)
+        if targets:
+            buckets = self.buckets[at].int() * there
+            words[:n, 1] = buckets[:, 0] + (buckets[:, 1] << 8)
+            made[:, 4:6] = mine[:, :, 1].masked_fill(~there, -math.inf)
+        phases = mine[:, :, 2:].reshape(n, 2, self.orders - 1, 2).masked_fill(~there[:, :, None, None], 0.0)
+        made[:, head:] = phases.transpose(1, 2).flatten(1)
+        self._kept.append(_native.Made(entries, ptr))
+        return entries, ptr
 
     def _packed(self, source: Tensor) -> Tensor:
         buckets = self.buckets.long()
@@ -114,6 +200,8 @@ class Heads:
         self.heads, self.scale = heads, 1.0 / math.sqrt(head_type.dimension)
         self.plan = fused_attention.plan_of(head_type, full, heads)
         self.top = head_type.max_frequency
+        # rows of more than 32 of these go to a workgroup where ds is formed: a wave holds 12 steps of 64 / heads edges
+        self.score_slots = max(1, 12 * (64 // heads) // 32)
         # read on the host, whatever the default device of the call that makes the (kept) heads
         self.desc = torch.tensor([list(row) for row in self.plan.rows], dtype=torch.int64, device="cpu")
         self._slots: dict[int, int] = {}
@@ -153,8 +241,10 @@ class RelativeSoftmax(torch.autograd.Function):
     def forward(ctx: Any, q: Tensor, k: Tensor, table: Tensor, tables: RelativeEdgeTables, heads: Heads, scale: float,
                 train: bool) -> Tensor:
         if train:  # found here: the backward runs on a thread and perhaps a stream of its own
-            tables.group_sources()
-            tables.source_rows(heads.served(tables).slots(tables))
+            slots = heads.served(tables).slots(tables)
+            tables.sources(slots)
+            tables.pairs("sources", slots)
+            tables.target_rows(heads.score_slots)
         with _native.span("gm::attention/relative_softmax"):
             alpha = _native.relative_forward(q, k, table, tables, heads, scale)
         if train:
