@@ -376,17 +376,17 @@ int rel_rows(const int32_t* order, const int64_t* counts, int64_t n, RelRows& ro
 template <typename T, typename R>
 int rel_lanes_check(const RelArgs<T, R>& a) {
   GM_REQUIRE((std::is_same<T, float>::value) && rel_slots(a.L) > 0, "the lane kernels do not serve this layout");
-  GM_REQUIRE(aligned(a.q, 16) && aligned(a.k, 16) && aligned(a.dq, 16) && aligned(a.dk, 16) && aligned(a.pairs, 8) &&
-                 aligned(a.pairs_s, 8),
-             "the lane kernels take rows at multiples of 16 bytes, entries of 8");
+  GM_REQUIRE(aligned(a.q, 16) && aligned(a.k, 16) && aligned(a.dq, 16) && aligned(a.dk, 16) &&
+                 aligned(a.records, 8) && aligned(a.pairs, 8) && aligned(a.pairs_s, 8),
+             "the lane kernels take rows at multiples of 16 bytes, records and entries of 8");
   return GM_OK;
 }
 
 template <typename T, typename R>
 int relative_forward(const R* q, const R* k, const T* table, const T* records, const int64_t* desc,
-                     const int64_t* row_ptr, const float* pairs, const int64_t* pair_ptr, const int32_t* order,
-                     const int64_t* counts, int64_t n_targets, int64_t n_sources, int64_t n_edges, int64_t D,
-                     int64_t orders, int64_t F, int64_t H, int64_t buckets, double scale, T* alpha, void* stream) {
+                     const int64_t* row_ptr, const int32_t* order, const int64_t* counts, int64_t n_targets,
+                     int64_t n_sources, int64_t n_edges, int64_t D, int64_t orders, int64_t F, int64_t H,
+                     int64_t buckets, double scale, T* alpha, void* stream) {
   RelArgs<T, R> a{};
   const int rc = rel_prepare(a, records, desc, row_ptr, n_targets, n_sources, n_edges, D, orders, F, H, buckets, scale,
                              q, k);
@@ -396,17 +396,14 @@ int relative_forward(const R* q, const R* k, const T* table, const T* records, c
   a.alpha = alpha;
   a.table = table;
   if constexpr (std::is_same<T, float>::value) {
-    if (pairs) {
-      a.pairs = pairs;
-      a.pair_ptr = pair_ptr;
-      GM_REQUIRE(pair_ptr && order, "the pairs' offsets and classes must be device pointers");
+    if (order) {
       RelRows rows;
       int status = rel_lanes_check(a);
-      if (status == GM_OK) status = rel_rows(order, counts, (n_targets + 1) / 2, rows);
+      if (status == GM_OK) status = rel_rows(order, counts, n_targets, rows);
       return status == GM_OK ? rel_launch_units(RelPass::Forward, a, rows, (hipStream_t)stream) : status;
     }
   }
-  GM_REQUIRE(!pairs, "the lane kernels take float tables");
+  GM_REQUIRE(!order, "the lane kernels take float tables");
   hipLaunchKernelGGL((relative_forward_simple<T, R>), dim3((unsigned)blocks_for(n_targets)), dim3(256), 0,
                      (hipStream_t)stream, a);
   return check_launch("relative_forward");
@@ -564,11 +561,10 @@ extern "C" int gm_relative_slots(const int64_t* desc, int64_t F, int64_t H, int6
 #define GM_RELATIVE_ENTRY(SFX, T, R)                                                                                  \
   extern "C" int gm_relative_forward_##SFX(                                                                           \
       const R* q, const R* k, const T* table, const T* records, const int64_t* desc, const int64_t* row_ptr,          \
-      const float* pairs, const int64_t* pair_ptr, const int32_t* order, const int64_t* counts, int64_t n_targets,    \
-      int64_t n_sources, int64_t n_edges, int64_t D, int64_t orders, int64_t F, int64_t H, int64_t buckets,           \
-      double scale, T* alpha, void* stream) {                                                                         \
-    return gm::relative_forward<T, R>(q, k, table, records, desc, row_ptr, pairs, pair_ptr, order, counts, n_targets, \
-                                      n_sources, n_edges, D, orders, F, H, buckets, scale, alpha, stream);            \
+      const int32_t* order, const int64_t* counts, int64_t n_targets, int64_t n_sources, int64_t n_edges, int64_t D,  \
+      int64_t orders, int64_t F, int64_t H, int64_t buckets, double scale, T* alpha, void* stream) {                  \
+    return gm::relative_forward<T, R>(q, k, table, records, desc, row_ptr, order, counts, n_targets, n_sources,       \
+                                      n_edges, D, orders, F, H, buckets, scale, alpha, stream);                       \
   }                                                                                                                   \
   extern "C" int gm_relative_backward_##SFX(                                                                          \
       const T* g, const T* alpha, const R* q, const R* k, const T* records, const T* records_s,                       \

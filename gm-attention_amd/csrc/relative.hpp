@@ -16,12 +16,11 @@ struct RelLayout : HeadsLayout {
   int orders;
 };
 
-// The lane kernels take two neighbouring rows (targets, or sources) at a time, a pair, over the entries of both: an
-// entry is a node that either row has an edge to (from), with the edge of each, so that a node's row is loaded once for
-// two edges.  Words of an entry: the node; (the targets' side) the buckets of both edges, a byte each; the edges (-1: the
-// row has none); (the targets' side) their biases / log 2 (-inf outside the window); (cos, sin) of both edges for the
-// orders 1 ..
-constexpr int kRelPairHead = 6, kRelPairHeadS = 4;
+// The backward's lane kernels take two neighbouring rows (targets, or sources) at a time, a pair, over the entries of
+// both: an entry is a node that either row has an edge with, and the edge of each, so that a node's row is loaded once
+// for two edges.  Words of an entry: the node; one left free; the edges (-1: the row has none); (cos, sin) of both edges
+// for the orders 1 ..
+constexpr int kRelPairHead = 4;
 
 // Rows (pairs, or targets) by length: `order` lists them in three classes, those of 16 waves each, of four, of one;
 // (count of each).
@@ -42,9 +41,9 @@ struct RelArgs {
   const T* records_s;      // (n_edges, 2 orders): target, edge, (cos, sin) of orders 1 ..; sorted by source
   const int64_t* row_ptr;  // over targets
   const int64_t* src_ptr;  // over sources
-  const float* pairs;        // the lane kernels': entries of pairs of targets, and their CSR over the pairs
+  const float* pairs;      // the backward's lane kernels': entries of pairs of targets, and their CSR over the pairs
   const int64_t* pair_ptr;
-  const float* pairs_s;      // of pairs of sources
+  const float* pairs_s;    // of pairs of sources
   const int64_t* pair_ptr_s;
   const T* g;              // (n_edges, H)
   T* alpha;                // (n_edges, H); read by the backward

@@ -11,7 +11,7 @@
 namespace gm {
 namespace rel {
 
-constexpr int kRelSteps = 16;     // steps of a wave whose scores LDS holds: 16 S entries
+constexpr int kRelSteps = 32;     // steps of a wave whose scores LDS holds, at most: 32 S edges
 constexpr int kRelInFlight = 4;   // steps whose rows are requested together
 constexpr int kRelThreadsB = kWavesPerBlock * kWave;
 
@@ -20,6 +20,8 @@ template <int A0, int A1, int A2, int ORD>
 struct RelUnit {
   static constexpr int W0 = A0, W1 = 2 * A1, W2 = 2 * A2, N = W0 + W1 + W2;
   static constexpr int NO = ORD;
+  static constexpr int RW = 2 + 2 * NO;                     // words of an edge's record
+  static constexpr int PW = kRelPairHead + 4 * NO;          // of a pair's entry
   static constexpr int NA = NO > 0 ? NO : 1;  // arrays of none
 
   template <bool kNear, typename R>
@@ -101,7 +103,7 @@ __device__ __forceinline__ float next_lane(float v) {
   return __int_as_float(__builtin_amdgcn_mov_dpp(__float_as_int(v), 0xB1, 0xF, 0xF, true));
 }
 
-// The pair that a wave works on, and which of its entries; all of it scalar.
+// The row (a target, or a pair) that a wave works on, and which of its edges or entries; all of it scalar.
 __device__ __forceinline__ Share rel_share(const EdgeUnits& w, const int64_t* ptr, int64_t block, int64_t blocks) {
   Share s;
   s.wave = uniform((int)(threadIdx.x >> 6));
@@ -124,157 +126,155 @@ __device__ __forceinline__ Share rel_share(const EdgeUnits& w, const int64_t* pt
 
 // ---------------------------------------------------------------- forward
 
-// kSplit: a head has two units or more, whose lanes form its scores of both targets together: even lanes keep the first
-// target's, odd ones the second's; else a lane keeps both.
+// kSplit: a head has two units or more, whose lanes hold the same scores: two of them keep every second step's each.
 template <typename R, typename U, bool kNear, bool kSplit>
 __global__ __launch_bounds__(1024) void relative_forward_units(RelArgs<float, R> a, EdgeUnits w, int64_t blocks,
                                                                int steps) {
-  constexpr int RW = kRelPairHead + 4 * U::NO, kWords = kWave * RW, kT = kSplit ? 1 : 2;
+  constexpr int kWords = kWave * U::RW;
+  const int kept = kSplit ? steps / 2 : steps;  // a wave's rows of scores in LDS
   extern __shared__ __align__(16) float rel_lds[];
-  const int waves = blockDim.x >> 6, lane = threadIdx.x & 63, wave = uniform((int)(threadIdx.x >> 6)), H = a.L.H;
-  float* rec = rel_lds + wave * (kWords + steps * kT * kWave);
+  const int waves = blockDim.x >> 6, lane = threadIdx.x & 63, wave = uniform((int)(threadIdx.x >> 6));
+  float* rec = rel_lds + wave * (kWords + kept * kWave);
   float* sc = rec + kWords + lane;
-  float* shared = rel_lds + waves * (kWords + steps * kT * kWave);   // (waves, kT, 64): the waves' maxima, then sums
-  float* learned = shared + (waves > 1 ? waves * kT * kWave : 0);    // (buckets, H), in units of log 2
-  for (int i = threadIdx.x; i < a.buckets * H; i += blockDim.x) learned[i] = a.table[i] * (float)kRelLog2e;
+  float* shared = rel_lds + waves * (kWords + kept * kWave);  // (waves, 64): the waves' maxima, then sums
+  float* learned = shared + (waves > 1 ? waves * kWave : 0);   // (buckets, H), in units of log 2
+  for (int i = threadIdx.x; i < a.buckets * a.L.H; i += blockDim.x) learned[i] = a.table[i] * (float)kRelLog2e;
   __syncthreads();
-  const Share sh = rel_share(w, a.pair_ptr, blockIdx.x, blocks);
-  if (!sh.live) return;  // one wave a pair, or the whole workgroup
   const int u = lane & (w.lanes - 1), s = lane >> w.shift, unit = u < w.units ? u : w.units - 1;
-  const int h = unit / w.per_map, own = unit % w.per_map, odd = kSplit ? own & 1 : 0;
-  const bool writes = u < w.units && own < (kSplit ? 2 : 1);
-  const float* mine = rec + s * RW;  // this lane's entry of step 0
+  const int h = unit / w.per_map, own = unit % w.per_map;
+  const bool odd = kSplit && (own & 1), writes = u < w.units && own < (kSplit ? 2 : 1);
+  const float* mine = rec + s * U::RW;  // this lane's edge of step 0
   const float scale = a.scale;
   const float* bias_of = learned + h;
-  const int64_t t0 = 2 * (int64_t)sh.row, t1 = t0 + 1 < a.n_targets ? t0 + 1 : t0;
-  float q[2][U::N];
-  U::template load<false>(a.q, w, unit, (int)t0, q[0]);
-  U::template load<false>(a.q, w, unit, (int)t1, q[1]);
-  const int held = sh.steps < steps ? sh.steps : steps;
-  float m[kT], l[kT], inv[kT];
-#pragma unroll
-  for (int j = 0; j < kT; ++j) {
-    m[j] = neg_inf<float>();
-    l[j] = inv[j] = 0.f;
-  }
 
-  // over a lane's slots and the pair's waves.  A score that is not a number is not a maximum; its exponential makes the
-  // sum, and with it the row, not a number.
-  auto over_waves = [&](float (&v)[kT], bool maximum) {
+  const Share sh = rel_share(w, a.row_ptr, blockIdx.x, blocks);
+  if (!sh.live) return;  // one wave a row, or the whole workgroup
+  float q[U::N];
+  U::template load<false>(a.q, w, unit, sh.row, q);
+  const int held = sh.steps < steps ? sh.steps : steps;
+  float m = neg_inf<float>(), l = 0.f, inv = 0.f;
+
+  // over a lane's slots (and, of a sum, the two lanes with a step each) and the row's waves.  A score that is not a
+  // number is not a maximum; its exponential makes the sum, and with it the row, not a number.
+  auto over_waves = [&](float v, bool maximum) {
     for (int o = w.lanes; o < kWave; o <<= 1) {
-#pragma unroll
-      for (int j = 0; j < kT; ++j) {
-        const float x = __shfl_xor(v[j], o, kWave);
-        v[j] = maximum ? fmaxf(x, v[j]) : v[j] + x;
-      }
+      const float x = __shfl_xor(v, o, kWave);
+      v = maximum ? fmaxf(x, v) : v + x;
+    }
+    if constexpr (kSplit) {
+      const float x = next_lane(v);
+      v = maximum ? fmaxf(x, v) : v + x;
     }
     if (sh.parts > 1) {
       __syncthreads();
-#pragma unroll
-      for (int j = 0; j < kT; ++j) shared[(sh.wave * kT + j) * kWave + lane] = v[j];
+      shared[sh.wave * kWave + lane] = v;
       __syncthreads();
-#pragma unroll
-      for (int j = 0; j < kT; ++j) {
-        v[j] = shared[j * kWave + lane];
-        for (int o = 1; o < waves; ++o) {
-          const float x = shared[(o * kT + j) * kWave + lane];
-          v[j] = maximum ? fmaxf(x, v[j]) : v[j] + x;
-        }
+      v = shared[lane];
+      for (int o = 1; o < waves; ++o) {
+        const float x = shared[o * kWave + lane];
+        v = maximum ? fmaxf(x, v) : v + x;
       }
     }
+    return v;
   };
-  auto write = [&](int edge, float v) {
-    if (writes && edge >= 0) a.alpha[(int64_t)edge * H + h] = v;
+  const uint32_t place = (uint32_t)(s * a.L.H + h);
+  // the weight of step t of the edges from `e`
+  auto write = [&](int64_t e, int t, float v) {
+    float* to = a.alpha + (e + t * w.slots) * a.L.H;
+    if (writes && s < (int)(sh.e1 - e) - t * w.slots) to[place] = v;
   };
 
-  // phase 0: every score, its maximum; the first `steps` steps' stay in LDS.  The steps past them are scored again for
-  // the sum (1) and the weights (2): pairs beyond 16 waves' LDS only.
+  // phase 0: every score, its maximum; the first `steps` steps' stay in LDS.  The steps past them are scored again
+  // for the sum (1) and the weights (2): rows beyond 16 waves' LDS only.
   for (int phase = 0; phase < 3; ++phase) {
     if (phase == 1) {
-      over_waves(m, true);
-#pragma unroll
-      for (int j = 0; j < kT; ++j) m[j] = m[j] == neg_inf<float>() ? 0.f : m[j];  // no edge inside: exp(-inf) = 0
-      for (int t = 0; t < held; ++t) {
-#pragma unroll
-        for (int j = 0; j < kT; ++j) {
-          const float x = exp2_of(sc[(t * kT + j) * kWave] - m[j]);
-          sc[(t * kT + j) * kWave] = x;
-          l[j] += x;
+      m = over_waves(m, true);
+      m = m == neg_inf<float>() ? 0.f : m;  // no edge inside: exp(-inf) = 0 everywhere
+      if constexpr (kSplit) {
+        for (int t = 0; t < held; t += 2) {  // a step past `held` is outside: its weight is zero
+          const float x = exp2_of(sc[t / 2 * kWave] - m);
+          sc[t / 2 * kWave] = x;
+          l += x;
+        }
+      } else {
+        for (int t = 0; t < held; ++t) {
+          const float x = exp2_of(sc[t * kWave] - m);
+          sc[t * kWave] = x;
+          l += x;
         }
       }
     }
     if (phase == 2) {
-      over_waves(l, false);
-#pragma unroll
-      for (int j = 0; j < kT; ++j) inv[j] = l[j] == 0.f ? 0.f : 1.f / l[j];
-      const int64_t rest = sh.e1 - sh.e0;
-      const float* from = a.pairs + sh.e0 * RW + 2 + odd;
-      for (int t = 0; t < held; ++t) {
-        const int at = t * w.slots + s;
-        const bool in = at < rest;
-#pragma unroll
-        for (int j = 0; j < kT; ++j) {
-          const int edge = in ? *reinterpret_cast<const int*>(from + (int64_t)at * RW + j) : -1;
-          write(edge, sc[(t * kT + j) * kWave] * inv[j]);
-        }
+      l = over_waves(l, false);
+      inv = l == 0.f ? 0.f : 1.f / l;
+      if constexpr (kSplit) {
+        for (int t = 0; t < held; t += 2) write(sh.e0, t + odd, sc[t / 2 * kWave] * inv);
+      } else {
+        for (int t = 0; t < held; ++t) write(sh.e0, t, sc[t * kWave] * inv);
       }
     }
     const int skip = phase == 0 ? 0 : steps;
     if (skip >= sh.steps) continue;
     const int first = skip & ~(w.lanes - 1);  // a batch's first step
-    Records<RW> records;
-    records.request(a.pairs, sh.e0 + (int64_t)first * w.slots, sh.e1, lane);
+    Records<U::RW> records;
+    records.request(a.records, sh.e0 + (int64_t)first * w.slots, sh.e1, lane);
     for (int b = first; b < sh.steps; b += w.lanes) {
-      const int64_t e = sh.e0 + (int64_t)b * w.slots;  // the batch's first entry
+      const int64_t e = sh.e0 + (int64_t)b * w.slots;  // the batch's first edge
       wave_lds();
       records.put(rec, lane);
       wave_lds();
-      if (b + w.lanes < sh.steps) records.request(a.pairs, e + kWave, sh.e1, lane);
+      if (b + w.lanes < sh.steps) records.request(a.records, e + kWave, sh.e1, lane);
       const int ends = sh.steps - b < w.lanes ? sh.steps - b : w.lanes;
-      const int left = (int)(sh.e1 - e < kWave ? sh.e1 - e : kWave);
       auto take = [&](int t, auto group) {
         constexpr int UN = decltype(group)::value;
-        float k[UN][U::N];
-        uint32_t bucket[UN];
+        float2 head[UN];
+        float k[UN][U::N], cs[UN][U::NA], sn[UN][U::NA], v[UN];
 #pragma unroll
         for (int n = 0; n < UN; ++n) {
-          const float2 head = *reinterpret_cast<const float2*>(mine + (t + n) * w.slots * RW);
-          const bool in = (t + n) * w.slots + s < left;  // past the end: node 0's row, excluded
-          bucket[n] = __float_as_uint(head.y);
-          U::template load<kNear>(a.k, w, unit, in ? __float_as_int(head.x) : 0, k[n]);
+          const float* r = mine + (t + n) * w.slots * U::RW;
+          head[n] = *reinterpret_cast<const float2*>(r);
+#pragma unroll
+          for (int o = 0; o < U::NO; ++o) {
+            const float2 x = *reinterpret_cast<const float2*>(r + 2 + 2 * o);
+            cs[n][o] = x.x;
+            sn[n][o] = x.y;
+          }
         }
 #pragma unroll
-        for (int n = 0; n < UN; ++n) {
-          const float* r = mine + (t + n) * w.slots * RW;
-          const bool in = (t + n) * w.slots + s < left;
-          float v[2];
+        for (int n = 0; n < UN; ++n)
+          U::template load<kNear>(a.k, w, unit, __float_as_int(head[n].x) & 0xFFFFFF, k[n]);
+        float bias[UN];
 #pragma unroll
-          for (int j = 0; j < 2; ++j) {
-            float cs[U::NA], sn[U::NA];
-            U::phases(r + kRelPairHead, j, cs, sn);
-            v[j] = U::dot(q[j], k[n], cs, sn);
-          }
-          float score[kT];
-          if constexpr (kSplit) {
-            const float keep = odd ? v[1] : v[0], give = odd ? v[0] : v[1];
-            score[0] = keep + next_lane(give);
-            for (int o = 2; o < w.per_map; o <<= 1) score[0] += __shfl_xor(score[0], o, kWave);
-          } else {
-            score[0] = v[0];
-            score[kT - 1] = v[1];
-          }
+        for (int n = 0; n < UN; ++n) bias[n] = bias_of[(__float_as_uint(head[n].x) >> 24) * a.L.H];
 #pragma unroll
-          for (int j = 0; j < kT; ++j) {
-            const float bias = r[4 + odd + j], table = bias_of[((bucket[n] >> (8 * (odd + j))) & 0xFF) * H];
-            // outside the window (or another target's edge): excluded, whatever its row holds
-            score[j] = !in || bias == neg_inf<float>() ? neg_inf<float>() : fmaf(scale, score[j], bias + table);
+        for (int n = 0; n < UN; ++n) v[n] = U::dot(q, k[n], cs[n], sn[n]);
+        sum_units<UN>(v, w.per_map);
+#pragma unroll
+        for (int n = 0; n < UN; ++n)  // outside the window: excluded, whatever its row holds
+          v[n] = head[n].y == neg_inf<float>() ? neg_inf<float>() : fmaf(scale, v[n], head[n].y + bias[n]);
+        if constexpr (kSplit) {
+#pragma unroll
+          for (int n = 0; n < UN; n += 2) {
+            const float even = v[n], next = v[n + 1], x = odd ? next : even;
             if (phase == 0) {
-              m[j] = fmaxf(m[j], score[j]);
-              if (b + t < steps) sc[((b + t + n) * kT + j) * kWave] = score[j];
+              m = fmaxf(m, x);
+              if (b + t < steps) sc[(b + t + n) / 2 * kWave] = x;
             } else if (phase == 1) {
-              l[j] += exp2_of(score[j] - m[j]);
+              l += exp2_of(x - m);
             } else {
-              write(in ? __float_as_int(r[2 + odd + j]) : -1, exp2_of(score[j] - m[j]) * inv[j]);
+              write(e, t + n + odd, exp2_of(x - m) * inv);
+            }
+          }
+        } else {
+#pragma unroll
+          for (int n = 0; n < UN; ++n) {
+            if (phase == 0) {
+              m = fmaxf(m, v[n]);
+              if (b + t < steps) sc[(b + t + n) * kWave] = v[n];
+            } else if (phase == 1) {
+              l += exp2_of(v[n] - m);
+            } else {
+              write(e, t + n, exp2_of(v[n] - m) * inv);
             }
           }
         }
@@ -293,7 +293,7 @@ __global__ __launch_bounds__(1024) void relative_forward_units(RelArgs<float, R>
 // conj(tau) q over a source's.
 template <typename R, typename U, bool kNear, bool kTargets, bool kSplit>
 __global__ __launch_bounds__(kRelThreadsB) void relative_rows_units(RelArgs<float, R> a, EdgeUnits w, int64_t blocks) {
-  constexpr int kHead = kTargets ? kRelPairHead : kRelPairHeadS, RW = kHead + 4 * U::NO, kWords = kWave * RW;
+  constexpr int RW = U::PW, kWords = kWave * RW;
   constexpr int kTogether = U::N > 12 ? 2 : 4, kT = kSplit ? 1 : 2;  // steps whose rows are requested together
   extern __shared__ __align__(16) float rel_lds[];
   const Share sh = rel_share(w, kTargets ? a.pair_ptr : a.pair_ptr_s, blockIdx.x, blocks);
@@ -354,7 +354,7 @@ __global__ __launch_bounds__(kRelThreadsB) void relative_rows_units(RelArgs<floa
         for (int j = 0; j < 2; ++j) {
           if (both[j] != 0.f) {
             float cs[U::NA], sn[U::NA];
-            U::phases(r + kHead, j, cs, sn);
+            U::phases(r + kRelPairHead, j, cs, sn);
             U::add(sums + j * U::N, both[j], x[n], cs, sn, !kTargets);
           }
         }
@@ -415,17 +415,15 @@ inline int rel_shape(const RelLayout& L, int& per_map, int (&base)[3]) {
 
 constexpr size_t kRelLds = 160 * 1024;
 
-// LDS of a pass: the entries a wave (and the forward's scores, and the learned table), or the waves' sums.
+// LDS of a pass: the records a wave (and the forward's scores, and the learned table), the waves' sums, the bins.
 template <typename U>
 size_t rel_forward_lds(int waves, bool split, int steps, int table) {
-  const size_t targets = split ? 1 : 2;
-  return sizeof(float) * ((size_t)waves * (kWave * (kRelPairHead + 4 * U::NO) + targets * steps * kWave +
-                                           (waves > 1 ? targets * kWave : 0)) + table);
+  return sizeof(float) * ((size_t)waves * (kWave * U::RW + (split ? steps / 2 : steps) * kWave + (waves > 1 ? kWave : 0)) +
+                          table);
 }
 template <typename U>
-size_t rel_rows_lds(bool targets, int lanes) {
-  return sizeof(float) * kWavesPerBlock *
-         (size_t)std::max(kWave * ((targets ? kRelPairHead : kRelPairHeadS) + 4 * U::NO), 2 * U::N * lanes);
+size_t rel_rows_lds(int lanes) {
+  return sizeof(float) * kWavesPerBlock * (size_t)std::max(kWave * U::PW, 2 * U::N * lanes);
 }
 
 inline int rel_lds_limit(const void* kernel, size_t lds) {
@@ -447,9 +445,8 @@ int rel_launch(RelPass pass, const RelArgs<float, R>& a, EdgeUnits w, const RelR
       const int waves = c == 0 ? 16 : kWavesPerBlock;
       if (w.shared + w.single > 0) {
         const int64_t blocks = w.shared + blocks_for(w.single);
-        // as many steps as the rows of these classes have; sixteen waves' beside a large table fewer (longer rows are
-        // scored again)
-        int steps = c == 0 || w.slots == 1 ? 2 * kRelSteps : kRelSteps;
+        // sixteen waves' scores beside a large table: fewer steps of them (longer rows are scored again)
+        int steps = kRelSteps;
         const int table = a.buckets * a.L.H;
         while (rel_forward_lds<U>(waves, kSplit, steps, table) > kRelLds) steps -= kRelInFlight;
         const size_t lds = rel_forward_lds<U>(waves, kSplit, steps, table);
@@ -469,7 +466,7 @@ int rel_launch(RelPass pass, const RelArgs<float, R>& a, EdgeUnits w, const RelR
   if (blocks == 0) return GM_OK;
   const auto kernel = pass == RelPass::BackwardTarget ? &relative_rows_units<R, U, kNear, true, kSplit>
                                                       : &relative_rows_units<R, U, kNear, false, kSplit>;
-  const size_t lds = rel_rows_lds<U>(pass == RelPass::BackwardTarget, w.lanes);
+  const size_t lds = rel_rows_lds<U>(w.lanes);
   const int rc = rel_lds_limit(reinterpret_cast<const void*>(kernel), lds);
   if (rc != GM_OK) return rc;
   hipLaunchKernelGGL(kernel, dim3((unsigned)blocks), dim3(kRelThreadsB), lds, stream, a, w, blocks);

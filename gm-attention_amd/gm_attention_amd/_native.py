@@ -124,7 +124,7 @@ SIGNATURES_F32 = {
     "gm_relative_padded": (ctypes.c_int, [_P] + [_I] * 4 + [_P]),
     **{f"gm_relative_repack_{sfx}": (ctypes.c_int, [_P] * 2 + [_I] * 2 + [_P] + [_I] * 4 + [_P] * 2)
        for sfx in ("f32", "bf16")},
-    **{f"gm_relative_forward_{sfx}": (ctypes.c_int, [_P] * 10 + [_I] * 8 + [_D] + [_P] * 2)
+    **{f"gm_relative_forward_{sfx}": (ctypes.c_int, [_P] * 8 + [_I] * 8 + [_D] + [_P] * 2)
        for sfx in ("f32", "f64", "bf16")},
     **{f"gm_relative_backward_{sfx}": (ctypes.c_int, [_P] * 20 + [_I] * 8 + [_D] + [_P] * 6)
        for sfx in ("f32", "f64", "bf16")},
@@ -1765,11 +1765,11 @@ def relative_forward(q: Tensor, k: Tensor, table: Tensor, tables: Any, heads: An
     if served is not heads:
         q, k = relative_repack(q, heads, served), relative_repack(k, heads, served)
     H, desc, device = served.heads, served.desc, q.device
-    pairs = tables.pairs("targets", served.slots(tables))
+    order, counts = tables.target_rows(served.slots(tables))
     tables.found()
     alpha = torch.empty(tables.n_edges, H, dtype=tables.dtype, device=device)
     _call_on(device, "gm_relative_forward_" + _PW_SUFFIX[q.dtype], _ptr(q), _ptr(k), _ptr(table),
-             _ptr(tables.records), desc.data_ptr(), _ptr(tables.row_ptr), *pairs, tables.n_targets,
+             _ptr(tables.records), desc.data_ptr(), _ptr(tables.row_ptr), _ptr(order), counts, tables.n_targets,
              tables.n_sources, tables.n_edges, q.shape[1], tables.orders, desc.shape[0], H, tables.n_buckets, scale,
              _ptr(alpha), stream_handle(device))
     return alpha

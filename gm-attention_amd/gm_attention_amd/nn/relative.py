@@ -53,12 +53,12 @@ class RelativeEdgeTables(EdgeTables):
     """:class:`differential.EdgeTables` with every edge's bucket ``(n_edges,)``, whole
     numbers in ``0 .. n_buckets - 1`` (checked here, once).
 
-    The lane kernels read pairs of neighbouring targets (and, in the backward, of
-    sources), each with the list of the nodes that either has an edge to: neighbours on
-    a grid share most of theirs, whose rows are then loaded once for both.  The lists
-    are found with a first call (:meth:`group_sources`: the sources'), outside a capture,
-    and kept: 56 bytes an entry at two orders and 48, of four entries for seven edges or
-    fewer on a grid."""
+    The backward's lane kernels read pairs of neighbouring targets, and of sources, each
+    with the list of the nodes that either has an edge with: neighbours on a grid share
+    most of theirs, whose rows are then loaded once for both.  The lists are found with
+    the first call that a backward can follow (or by :meth:`group_sources`), outside a
+    capture, and kept: of each side 48 bytes an entry at three orders, four entries for
+    seven edges or fewer on a grid."""
 
     def __init__(self, row_ptr: Tensor, source: Tensor, transport: Tensor, bias: Tensor, inside: Tensor,
                  buckets: Tensor, n_buckets: int, *, n_sources: int | None = None) -> None:
@@ -94,9 +94,12 @@ class RelativeEdgeTables(EdgeTables):
             self._kept.append(_native.Made(self.buckets))
 
     def group_sources(self) -> tuple[Tensor, Tensor]:
-        """What a backward reads of the sources' side: the pairs of sources, or for float64
-        tables the edges sorted by source; found once."""
-        return super().group_sources() if self.dtype == torch.float64 else self._paired("sources")
+        """Finds what a backward reads beside the edges, once: the pairs of targets and of sources
+        (returned: the sources'), or for float64 tables the edges sorted by source."""
+        if self.dtype == torch.float64:
+            return super().group_sources()
+        self._paired("targets")
+        return self._paired("sources")
 
     def sources(self, slots: int) -> tuple[Tensor | None, Tensor | None]:
         """``(src_ptr, records_s)`` for the simple kernels (``slots`` 0)."""
@@ -152,18 +155,12 @@ class RelativeEdgeTables(EdgeTables):
         edges = torch.full((n, 2), -1, dtype=torch.int64, device=self.device)
         edges.view(-1)[2 * entry + second] = edge
         there, at = edges >= 0, edges.clamp_min(0)
-        head = 6 if targets else 4
-        entries = torch.zeros(max(n, 1), head + 4 * (self.orders - 1), dtype=torch.float32, device=self.device)
-        words, made = entries.view(torch.int32), entries[:n]
+        entries = torch.zeros(max(n, 1), 4 * self.orders, dtype=torch.float32, device=self.device)
+        words = entries.view(torch.int32)
         words[:n, 0] = key % max(nodes, 1)
         words[:n, 2:4] = edges
-        mine = self.records[at]  # (n, 2, 2 orders)
-        if targets:
-            buckets = self.buckets[at].int() * there
-            words[:n, 1] = buckets[:, 0] + (buckets[:, 1] << 8)
-            made[:, 4:6] = mine[:, :, 1].masked_fill(~there, -math.inf)
-        phases = mine[:, :, 2:].reshape(n, 2, self.orders - 1, 2).masked_fill(~there[:, :, None, None], 0.0)
-        made[:, head:] = phases.transpose(1, 2).flatten(1)
+        phases = self.records[at][:, :, 2:].reshape(n, 2, self.orders - 1, 2).masked_fill(~there[:, :, None, None], 0.0)
+        entries[:n, 4:] = phases.transpose(1, 2).flatten(1)
         self._kept.append(_native.Made(entries, ptr))
         return entries, ptr
 
@@ -243,6 +240,7 @@ class RelativeSoftmax(torch.autograd.Function):
         if train:  # found here: the backward runs on a thread and perhaps a stream of its own
             slots = heads.served(tables).slots(tables)
             tables.sources(slots)
+            tables.pairs("targets", slots)
             tables.pairs("sources", slots)
             tables.target_rows(heads.score_slots)
         with _native.span("gm::attention/relative_softmax"):

@@ -349,19 +349,21 @@ int gm_differential_backward_bf16(const float* g, const uint16_t* q, const uint1
  *   1 <= buckets <= 256; indices are followed unchecked.
  * ds (n_edges, H) and partial (gm_relative_partial_rows() rows of buckets H) are
  * workspaces.  Sums in a fixed order.
- * order of the backward, or NULL: every target once, long rows (a workgroup's each)
- * first, in three classes, counts (HOST) how many of each (the first two are long).
- * pairs, or NULL: the lane kernels run (float and bfloat16 rows; q, k, dq and dk at
- * multiples of 16 bytes, entries of 8); without, kernels for any layout.  The targets
- * 2 i and 2 i + 1 are a pair, and its entries pairs[pair_ptr[i] ..) are the sources
- * that either has an edge to, float words (the first four, or both of the middle, as
- * integers): the source, the buckets of both edges (a byte each from below), the edges
- * (-1: that target has none), their biases / log 2 (-inf: outside, or none), then for
- * every order 1 .. (cos, sin) of both edges.  Each edge is in one entry.  order (in the
- * backward pair_order): every pair once, those of more than 64 S entries first, then
- * those of more than 16 S, then the rest, counts how many of each, for the S of
- * gm_relative_slots (128 and 32 where S is 1).  pairs_s, pair_ptr_s, .. the same of the sources and the targets
- * with an edge to either, without buckets (a word left free) and without biases.
+ * order of the forward, or NULL: every target once, those of more than 128 S edges
+ * first, then those of more than 32 S, then the rest, counts (HOST) how many of each,
+ * for the S of gm_relative_slots.  With it (float and bfloat16 rows; q and k at
+ * multiples of 16 bytes, records of 8) the lane kernels run; without, kernels for any
+ * layout.  order of the backward, or NULL: every target once, long rows (a workgroup's
+ * each) first, in three classes, counts how many of each (the first two are long).
+ * pairs, or NULL: the backward's lane kernels run (float and bfloat16 rows; q, k, dq
+ * and dk at multiples of 16 bytes, entries of 8).  The targets 2 i and 2 i + 1 are a
+ * pair, and its entries pairs[pair_ptr[i] ..) are the sources that either has an edge
+ * to, 4 orders words: the source, one left free, the edge of each target (-1: none),
+ * integers all, then for every order 1 .. (cos, sin) of both edges.  Each edge is in one
+ * entry.  pair_order: every pair once, those of more than 64 S entries first, then those
+ * of more than 16 S, then the rest, pair_counts (HOST) how many of each (128 and 32
+ * where S is 1).  pairs_s, pair_ptr_s, .. the same of the sources and the targets with
+ * an edge to either.
  * Suffix _bf16: bfloat16 rows, float tables and arithmetic.  No reference
  * counterpart (the softmax without the learned bias: gm_softmax_*). */
 int64_t gm_relative_partial_rows(void);
@@ -376,10 +378,9 @@ int gm_relative_repack_f32(const float* src, const int64_t* desc, int64_t F, int
 int gm_relative_repack_bf16(const uint16_t* src, const int64_t* desc, int64_t F, int64_t D, const int64_t* to_desc,
                             int64_t to_F, int64_t to_D, int64_t H, int64_t n_rows, uint16_t* dst, void* stream);
 int gm_relative_forward_f32(const float* q, const float* k, const float* table, const float* records, const int64_t*
-                            desc, const int64_t* row_ptr, const float* pairs, const int64_t* pair_ptr, const int32_t*
-                            order, const int64_t* counts, int64_t n_targets, int64_t n_sources, int64_t n_edges, int64_t
-                            D, int64_t orders, int64_t F, int64_t H, int64_t buckets, double scale, float* alpha, void*
-                            stream);
+                            desc, const int64_t* row_ptr, const int32_t* order, const int64_t* counts, int64_t
+                            n_targets, int64_t n_sources, int64_t n_edges, int64_t D, int64_t orders, int64_t F, int64_t
+                            H, int64_t buckets, double scale, float* alpha, void* stream);
 int gm_relative_backward_f32(const float* g, const float* alpha, const float* q, const float* k, const float* records,
                              const float* records_s, const uint8_t* bucket, const int64_t* desc, const int64_t* row_ptr,
                              const int64_t* src_ptr, const int32_t* order, const int64_t* counts, const float* pairs,
@@ -389,10 +390,9 @@ int gm_relative_backward_f32(const float* g, const float* alpha, const float* q,
                              orders, int64_t F, int64_t H, int64_t buckets, double scale, float* ds, float* partial,
                              float* dq, float* dk, float* dtable, void* stream);
 int gm_relative_forward_f64(const double* q, const double* k, const double* table, const double* records, const int64_t*
-                            desc, const int64_t* row_ptr, const float* pairs, const int64_t* pair_ptr, const int32_t*
-                            order, const int64_t* counts, int64_t n_targets, int64_t n_sources, int64_t n_edges, int64_t
-                            D, int64_t orders, int64_t F, int64_t H, int64_t buckets, double scale, double* alpha, void*
-                            stream);
+                            desc, const int64_t* row_ptr, const int32_t* order, const int64_t* counts, int64_t
+                            n_targets, int64_t n_sources, int64_t n_edges, int64_t D, int64_t orders, int64_t F, int64_t
+                            H, int64_t buckets, double scale, double* alpha, void* stream);
 int gm_relative_backward_f64(const double* g, const double* alpha, const double* q, const double* k, const double*
                              records, const double* records_s, const uint8_t* bucket, const int64_t* desc, const
                              int64_t* row_ptr, const int64_t* src_ptr, const int32_t* order, const int64_t* counts,
@@ -402,10 +402,9 @@ int gm_relative_backward_f64(const double* g, const double* alpha, const double*
                              int64_t D, int64_t orders, int64_t F, int64_t H, int64_t buckets, double scale, double* ds,
                              double* partial, double* dq, double* dk, double* dtable, void* stream);
 int gm_relative_forward_bf16(const uint16_t* q, const uint16_t* k, const float* table, const float* records, const
-                             int64_t* desc, const int64_t* row_ptr, const float* pairs, const int64_t* pair_ptr, const
-                             int32_t* order, const int64_t* counts, int64_t n_targets, int64_t n_sources, int64_t
-                             n_edges, int64_t D, int64_t orders, int64_t F, int64_t H, int64_t buckets, double scale,
-                             float* alpha, void* stream);
+                             int64_t* desc, const int64_t* row_ptr, const int32_t* order, const int64_t* counts, int64_t
+                             n_targets, int64_t n_sources, int64_t n_edges, int64_t D, int64_t orders, int64_t F,
+                             int64_t H, int64_t buckets, double scale, float* alpha, void* stream);
 int gm_relative_backward_bf16(const float* g, const float* alpha, const uint16_t* q, const uint16_t* k, const float*
                               records, const float* records_s, const uint8_t* bucket, const int64_t* desc, const
                               int64_t* row_ptr, const int64_t* src_ptr, const int32_t* order, const int64_t* counts,
