@@ -15,9 +15,9 @@
 // float, so that no row overflows.
 //
 // The lane kernels hold a unit of a head a lane and need no other wave's numbers.  Layouts without such units (odd
-// copies, frequencies above 2, rows at odd addresses) and double take the general kernels, where a thread holds the same
-// piece of a row for all the rows of its workgroup and a head's squares meet in LDS between barriers (305 and 497 us
-// for the float rows above, 245 and 507 for the bfloat16 ones).  All are persistent; gains, and sums for their
+// copies, frequencies above 2, rows at odd addresses) and double take the general kernels, where a thread holds the
+// same piece of a row for all the rows of its workgroup and a head's squares meet in LDS between barriers (305 and
+// 497 us for the float rows above, 245 and 507 for the bfloat16 ones).  All are persistent; gains, and sums for their
 // gradients, stay in registers over a workgroup's rows, whose sums are added in a fixed order, no atomics.
 #include <algorithm>
 #include <type_traits>
@@ -523,7 +523,8 @@ __global__ __launch_bounds__(256) void head_norm_forward_lanes(HnArgs<float, R> 
     if (a.axes) hn_lane_angles<U>(a, w, row, r, u, own, cs, turn);
 #pragma unroll
     for (int st = 0; st < NS; ++st) {
-      const float inv = a.normalise ? (float)hn_rsqrt<float>(fma(hn_lane_sum(hn_dot(v[st], v[st]), w.per), a.share, a.eps)) : 1.f;
+      const double square = hn_lane_sum(hn_dot(v[st], v[st]), w.per);
+      const float inv = a.normalise ? (float)hn_rsqrt<float>(fma(square, a.share, a.eps)) : 1.f;
 #pragma unroll
       for (int i = 0; i < U::N; ++i) v[st][i] = gain[st][i] * (v[st][i] * inv);
       if (a.axes) U::turn(v[st], turn, false);
@@ -795,7 +796,8 @@ int hn_prepare(HnArgs<T, R>& a, const R* const* x, const int64_t* strides, const
     a.x[st] = x[st];
     a.stride[st] = strides[st];
     a.gain[st] = gains[st];
-    if (n_rows > 0) GM_REQUIRE(x[st] && (n_rows == 1 || strides[st] >= D), "rows must be device pointers, D apart or more");
+    if (n_rows > 0)
+      GM_REQUIRE(x[st] && (n_rows == 1 || strides[st] >= D), "rows must be device pointers, D apart or more");
   }
   if (n_rows > 0 && a.axes) GM_REQUIRE(positions && frequencies, "positions and frequencies must be device pointers");
   return GM_OK;

@@ -10,8 +10,8 @@ namespace gm {
 
 constexpr int kPartialColumns = 8, kPartialParts = 32;
 
-// out[c] = sum over rows of partial (rows, columns): a workgroup eight columns, 32 parts of the rows, whose loads do not
-// wait for each other.
+// out[c] = sum over rows of partial (rows, columns): a workgroup eight columns, 32 parts of the rows, whose loads do
+// not wait for each other.
 template <typename T>
 __global__ __launch_bounds__(256) void partial_sum_kernel(const T* partial, int64_t rows, int columns, T* out) {
   __shared__ double sums[kPartialParts][kPartialColumns + 1];
@@ -33,8 +33,8 @@ __global__ __launch_bounds__(256) void partial_sum_kernel(const T* partial, int6
 
 template <typename T>
 void launch_partial_sum(const T* partial, int64_t rows, int columns, T* out, hipStream_t stream) {
-  hipLaunchKernelGGL(partial_sum_kernel<T>, dim3((unsigned)((columns + kPartialColumns - 1) / kPartialColumns)), dim3(256), 0, stream, partial, rows,
-                     columns, out);
+  const int groups = (columns + kPartialColumns - 1) / kPartialColumns;
+  hipLaunchKernelGGL(partial_sum_kernel<T>, dim3((unsigned)groups), dim3(256), 0, stream, partial, rows, columns, out);
 }
 
 }  // namespace gm

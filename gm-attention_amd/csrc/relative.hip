@@ -219,8 +219,8 @@ __global__ __launch_bounds__(256) void relative_scores(RelScores<T> a, uint32_t 
   auto range = [&](uint32_t block) {
     if (block >= blocks) return Range{0, 0};
     const bool whole = block < a.shared;
-    const uint32_t at = whole ? xcd_spread_block32(block, a.shared)
-                              : a.shared + xcd_spread_block32(block - a.shared, blocks - a.shared) * kWavesPerBlock + wave;
+    uint32_t at = xcd_spread_block32(whole ? block : block - a.shared, whole ? a.shared : blocks - a.shared);
+    if (!whole) at = a.shared + at * kWavesPerBlock + wave;
     if (at >= a.rows) return Range{0, 0};
     const uint32_t row = a.order ? uniform((int)a.order[at]) : at;
     const int64_t r0 = uniform(a.row_ptr[row]), r1 = uniform(a.row_ptr[row + 1]);
@@ -437,7 +437,8 @@ int relative_scores_launch(const RelArgs<T, R>& a, const RelRows& rows, const ui
     return check_launch("relative (LDS)");
   const int64_t blocks = k.shared + blocks_for(a.n_targets - k.shared);
   const int64_t resident = resident_blocks(reinterpret_cast<const void*>(kernel), 256, lds);
-  const int64_t grid = std::max<int64_t>(1, std::min({blocks, (int64_t)kRelTableRows, resident > 0 ? resident : blocks}));
+  const int64_t most = std::min<int64_t>(kRelTableRows, resident > 0 ? resident : blocks);
+  const int64_t grid = std::max<int64_t>(1, std::min(blocks, most));
   hipLaunchKernelGGL(kernel, dim3((unsigned)grid), dim3(256), lds, stream, k, (uint32_t)blocks);
   launch_partial_sum<T>(a.partial, grid, a.buckets * a.L.H, dtable, stream);
   return check_launch("relative_scores");

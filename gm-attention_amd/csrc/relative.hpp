@@ -18,8 +18,8 @@ struct RelLayout : HeadsLayout {
 
 // The backward's lane kernels take two neighbouring rows (targets, or sources) at a time, a pair, over the entries of
 // both: an entry is a node that either row has an edge with, and the edge of each, so that a node's row is loaded once
-// for two edges.  Words of an entry: the node; one left free; the edges (-1: the row has none); (cos, sin) of both edges
-// for the orders 1 ..
+// for two edges.  Words of an entry: the node; one left free; the edges (-1: the row has none); (cos, sin) of both
+// edges for the orders 1 ..
 constexpr int kRelPairHead = 4;
 
 // Rows (pairs, or targets) by length: `order` lists them in three classes, those of 16 waves each, of four, of one;

@@ -418,8 +418,8 @@ constexpr size_t kRelLds = 160 * 1024;
 // LDS of a pass: the records a wave (and the forward's scores, and the learned table), the waves' sums, the bins.
 template <typename U>
 size_t rel_forward_lds(int waves, bool split, int steps, int table) {
-  return sizeof(float) * ((size_t)waves * (kWave * U::RW + (split ? steps / 2 : steps) * kWave + (waves > 1 ? kWave : 0)) +
-                          table);
+  const int kept = split ? steps / 2 : steps;
+  return sizeof(float) * ((size_t)waves * kWave * (U::RW + kept + (waves > 1 ? 1 : 0)) + table);
 }
 template <typename U>
 size_t rel_rows_lds(int lanes) {

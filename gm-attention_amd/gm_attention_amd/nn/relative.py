@@ -338,8 +338,8 @@ def attention_weights(mhsa: Any, q: Tensor, k: Tensor, edges: Any) -> Tensor:
 
 def _eager(q: Tensor, k: Tensor, table: Tensor, tables: RelativeEdgeTables, plan: fused_attention.Plan,
            scale: float) -> Tensor:
-    return _weights(q, k, table, tables.buckets.long(), tables.row_ptr, tables._source, tables._phases, tables._bias, plan,
-                    scale)
+    return _weights(q, k, table, tables.buckets.long(), tables.row_ptr, tables._source, tables._phases, tables._bias,
+                    plan, scale)
 
 
 def _weights(q: Tensor, k: Tensor, table: Tensor, buckets: Tensor, row_ptr: Tensor, source: Tensor, phases: Tensor,

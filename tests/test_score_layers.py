@@ -193,8 +193,8 @@ def test_both_operators_in_a_row(rows, cuda):
     heads, head = 4, SO2FieldType({0: 4, 1: 4, 2: 4})
     t = problems.tables(10, 20, batch=2, window="quartic")
     n, E = t.n_nodes, t.source.shape[0]
-    given = dict(q=problems.normal((n, 80), 1), k=problems.normal((n, 80), 2), q_gain=1 + 0.2 * problems.normal((12,), 3),
-                 k_gain=1 + 0.2 * problems.normal((12,), 4), table=problems.normal((12, heads), 5))
+    given = dict(q=problems.normal((n, 80), 1), k=problems.normal((n, 80), 2),
+                 q_gain=1 + 0.2 * problems.normal((12,), 3), k_gain=1 + 0.2 * problems.normal((12,), 4), table=problems.normal((12, heads), 5))
     at, f = positions_of(n), rotary_frequencies(head, (6.0, 4.0), (0.5, 1.0), (False, True))
     up = problems.normal((E, heads), 6)
     given, up = {name: v.to(rows).double() for name, v in given.items()}, up.to(rows).double()
@@ -203,7 +203,8 @@ def test_both_operators_in_a_row(rows, cuda):
 
     def step(dtype, device):
         edges = RelativeEdgeTables(t.row_ptr.to(device), t.source.to(device),
-                                   *(x.to(dtype).to(device) for x in tables), t.inside.to(device), buckets.to(device), 12)
+                                   *(x.to(dtype).to(device) for x in tables), t.inside.to(device), buckets.to(device),
+                                   12)
         leaves = {name: v.to(dtype).to(device).requires_grad_(True) for name, v in given.items()}
         q, k = query_key_norm(leaves["q"], leaves["k"], head, heads, leaves["q_gain"], leaves["k_gain"],
                               positions=at.to(device), frequencies=f.to(device))
