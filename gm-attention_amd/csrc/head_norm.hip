@@ -156,24 +156,23 @@ __device__ __forceinline__ double hn_rsqrt(double v) {
   const double refined = y * fma(-0.5 * v * y, y, 1.5);
   return v > 0.0 && v < (double)INFINITY ? refined : y;
 }
-// Sum of a_j b_j in float (two sums, of even and odd j); where that is out of float's range, or near zero, once more of
-// numbers scaled by 2^-70 or 2^70.
+// Sum of a_j b_j in float (two sums, of even and odd j); where that is out of float's range, or near zero (small terms,
+// or large ones that cancel), once more in double.
 template <int V>
 __device__ __forceinline__ double hn_dot(const float (&a)[V], const float (&b)[V]) {
-  auto sum = [&](float scale) {
-    float s = 0.f, t = 0.f;
+  float s = 0.f, t = 0.f;
 #pragma unroll
-    for (int j = 0; j + 1 < V; j += 2) {
-      s = fmaf(a[j] * scale, b[j] * scale, s);
-      t = fmaf(a[j + 1] * scale, b[j + 1] * scale, t);
-    }
-    if constexpr (V % 2) s = fmaf(a[V - 1] * scale, b[V - 1] * scale, s);
-    return s + t;
-  };
-  const float s = sum(1.f);
+  for (int j = 0; j + 1 < V; j += 2) {
+    s = fmaf(a[j], b[j], s);
+    t = fmaf(a[j + 1], b[j + 1], t);
+  }
+  if constexpr (V % 2) s = fmaf(a[V - 1], b[V - 1], s);
+  s += t;
   if (fabsf(s) > 1e-30f && fabsf(s) < INFINITY) return (double)s;
-  const bool small = fabsf(s) <= 1e-30f;
-  return (double)sum(small ? 0x1p70f : 0x1p-70f) * (small ? 0x1p-140 : 0x1p140);
+  double wide = 0.0;
+#pragma unroll
+  for (int j = 0; j < V; ++j) wide = fma((double)a[j], (double)b[j], wide);
+  return wide;
 }
 template <int V>
 __device__ __forceinline__ double hn_dot(const double (&a)[V], const double (&b)[V]) {

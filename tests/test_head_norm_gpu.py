@@ -271,6 +271,19 @@ def test_the_smallest_and_largest_numbers(rows, cuda):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("rows", ROWS)
+@pytest.mark.parametrize("copies,heads", [({0: 4, 1: 4, 2: 4}, 4), ({0: 1, 1: 1}, 2), ({0: 11, 1: 5, 2: 3}, 3)])
+def test_products_that_cancel(copies, heads, rows, cuda):
+    """Whole numbers: sums of a piece's products are often zero though its terms are not."""
+    made = inputs(copies, heads, 500, 0, rows, gains=False)
+    for t in (made["q"], made["k"], *made["up"]):
+        t.copy_(t.round().clamp(-2, 2))
+    got = run(made, copies, heads, 1e-6, cuda)
+    for name, want in wanted(made, copies, heads, 1e-6, torch.finfo(tables_dtype(rows)).eps).items():
+        compare(got[name], want, name)
+
+
+@pytest.mark.gpu
 def test_infinite_and_nan_heads_stay_in_their_heads(cuda):
     copies, heads = {0: 4, 1: 4, 2: 4}, 4
     made = inputs(copies, heads, 20, 2, torch.float32)
