@@ -12,7 +12,9 @@ namespace gm {
 namespace rel {
 
 constexpr int kRelSteps = 32;     // steps of a wave whose scores LDS holds, at most: 32 S edges
-constexpr int kRelInFlight = 4;   // steps whose rows are requested together
+// Steps whose rows are requested together: two, and the registers that this leaves go to more waves, five or six a SIMD
+// (with four steps and four waves the scores of 33 M edges take 1.55 ms and the rows of 63 M 2.15, so 1.42 and 1.86).
+constexpr int kRelInFlight = 2;
 constexpr int kRelThreadsB = kWavesPerBlock * kWave;
 
 // A lane's shape; NO, the orders of the tables above 0.
@@ -128,7 +130,7 @@ __device__ __forceinline__ Share rel_share(const EdgeUnits& w, const int64_t* pt
 
 // kSplit: a head has two units or more, whose lanes hold the same scores: two of them keep every second step's each.
 template <typename R, typename U, bool kNear, bool kSplit>
-__global__ __launch_bounds__(1024) void relative_forward_units(RelArgs<float, R> a, EdgeUnits w, int64_t blocks,
+__global__ __launch_bounds__(1024, 5) void relative_forward_units(RelArgs<float, R> a, EdgeUnits w, int64_t blocks,
                                                                int steps) {
   constexpr int kWords = kWave * U::RW;
   const int kept = kSplit ? steps / 2 : steps;  // a wave's rows of scores in LDS
@@ -225,8 +227,8 @@ __global__ __launch_bounds__(1024) void relative_forward_units(RelArgs<float, R>
       wave_lds();
       if (b + w.lanes < sh.steps) records.request(a.records, e + kWave, sh.e1, lane);
       const int ends = sh.steps - b < w.lanes ? sh.steps - b : w.lanes;
-      auto take = [&](int t, auto group) {
-        constexpr int UN = decltype(group)::value;
+      auto take = [&](int t) {
+        constexpr int UN = kRelInFlight;
         float2 head[UN];
         float k[UN][U::N], cs[UN][U::NA], sn[UN][U::NA], v[UN];
 #pragma unroll
@@ -280,9 +282,7 @@ __global__ __launch_bounds__(1024) void relative_forward_units(RelArgs<float, R>
         }
       };
       int t = skip > b ? skip - b : 0;
-      for (; ends - t > 2 && sh.parts <= kWavesPerBlock; t += kRelInFlight)
-        take(t, std::integral_constant<int, kRelInFlight>());
-      for (; t < ends; t += 2) take(t, std::integral_constant<int, 2>());
+      for (; t < ends; t += kRelInFlight) take(t);
     }
   }
 }
@@ -292,9 +292,10 @@ __global__ __launch_bounds__(1024) void relative_forward_units(RelArgs<float, R>
 // Per pair of targets or of sources (kTargets or not): dq = scale sum ds tau k over a target's edges, dk = scale sum ds
 // conj(tau) q over a source's.
 template <typename R, typename U, bool kNear, bool kTargets, bool kSplit>
-__global__ __launch_bounds__(kRelThreadsB) void relative_rows_units(RelArgs<float, R> a, EdgeUnits w, int64_t blocks) {
+__global__ __launch_bounds__(kRelThreadsB, (U::N > 10 ? 5 : 6)) void relative_rows_units(RelArgs<float, R> a,
+                                                                                         EdgeUnits w, int64_t blocks) {
   constexpr int RW = U::PW, kWords = kWave * RW;
-  constexpr int kTogether = U::N > 12 ? 2 : 4, kT = kSplit ? 1 : 2;  // steps whose rows are requested together
+  constexpr int kT = kSplit ? 1 : 2;
   extern __shared__ __align__(16) float rel_lds[];
   const Share sh = rel_share(w, kTargets ? a.pair_ptr : a.pair_ptr_s, blockIdx.x, blocks);
   if (!sh.live) return;
@@ -361,8 +362,7 @@ __global__ __launch_bounds__(kRelThreadsB) void relative_rows_units(RelArgs<floa
       }
     };
     int t = 0;
-    for (; t + kTogether <= ends; t += kTogether) take(t, std::integral_constant<int, kTogether>());
-    for (; t + 2 <= ends; t += 2) take(t, std::integral_constant<int, 2>());
+    for (; t + kRelInFlight <= ends; t += kRelInFlight) take(t, std::integral_constant<int, kRelInFlight>());
     if (t < ends) take(t, std::integral_constant<int, 1>());
   }
   row_sums<2 * U::N>(w, sh, sums, rel_lds);
