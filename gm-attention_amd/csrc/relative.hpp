@@ -22,8 +22,8 @@ struct RelLayout : HeadsLayout {
 // edges for the orders 1 ..
 constexpr int kRelPairHead = 4;
 
-// Rows (pairs, or targets) by length: `order` lists them in three classes, those of 16 waves each, of four, of one;
-// (count of each).
+// Rows (pairs, or targets) by length: `order` lists them in three classes, a workgroup a row in the first two, a wave a
+// row in the last; (count of each).
 struct RelRows {
   const int32_t* order;
   int64_t count[3];

@@ -1,6 +1,17 @@
 // The lane kernels of the softmax with a learned relative bias: a head's copies are
 // `per_map` units of (A0, A1, A2) copies of frequencies 0, 1, 2, one lane a unit
-// (edge_units.hpp).
+// (edge_units.hpp), so that a step of a wave takes S = 64 / lanes edges.
+//
+// Forward, a wave a target (a long row four): a step gathers S rows of k and sums a
+// score over its units' lanes; scores wait in LDS (a long row's in alpha) for their
+// maximum and sum.  63.0 M edges of 160 numbers take 2.87 ms: 14 TB/s of rows out of L1,
+// whose accesses keep it 60 % busy while vector instructions fill 55 % of the time;
+// neither gives way alone.
+//
+// Backward, dq and dk: a wave a pair of neighbouring rows over the nodes of both, whose
+// rows are loaded once for two edges (four loads for seven edges on a grid).  1.86 and
+// 1.88 ms for the edges above; a row at a time 2.50 and 2.64.  The forward gains nothing
+// from pairs (2.99 ms): it has half the sums to keep, and its scores twice the places.
 #pragma once
 #include <algorithm>
 #include <type_traits>
@@ -11,11 +22,11 @@
 namespace gm {
 namespace rel {
 
-constexpr int kRelSteps = 32;     // steps of a wave whose scores LDS holds, at most: 32 S edges
+constexpr int kRelKept = 16;  // rows of scores that LDS holds a wave: 16 steps, or 32 where two lanes share a head's
 // Steps whose rows are requested together: two, and the registers that this leaves go to more waves, five or six a SIMD
 // (with four steps and four waves the scores of 33 M edges take 1.55 ms and the rows of 63 M 2.15, so 1.42 and 1.86).
 constexpr int kRelInFlight = 2;
-constexpr int kRelThreadsB = kWavesPerBlock * kWave;
+constexpr int kRelThreads = kWavesPerBlock * kWave;
 
 // A lane's shape; NO, the orders of the tables above 0.
 template <int A0, int A1, int A2, int ORD>
@@ -130,21 +141,21 @@ __device__ __forceinline__ Share rel_share(const EdgeUnits& w, const int64_t* pt
 
 // kSplit: a head has two units or more, whose lanes hold the same scores: two of them keep every second step's each.
 template <typename R, typename U, bool kNear, bool kSplit>
-__global__ __launch_bounds__(1024, 5) void relative_forward_units(RelArgs<float, R> a, EdgeUnits w, int64_t blocks,
-                                                               int steps) {
-  constexpr int kWords = kWave * U::RW;
-  const int kept = kSplit ? steps / 2 : steps;  // a wave's rows of scores in LDS
+__global__ __launch_bounds__(kRelThreads, 5) void relative_forward_units(RelArgs<float, R> a, EdgeUnits w,
+                                                                         int64_t blocks) {
+  constexpr int kWords = kWave * U::RW, kEvery = kSplit ? 2 : 1;  // steps of a row of scores, of which a lane keeps one
   extern __shared__ __align__(16) float rel_lds[];
-  const int waves = blockDim.x >> 6, lane = threadIdx.x & 63, wave = uniform((int)(threadIdx.x >> 6));
-  float* rec = rel_lds + wave * (kWords + kept * kWave);
+  const int lane = threadIdx.x & 63, wave = uniform((int)(threadIdx.x >> 6)), H = a.L.H;
+  float* rec = rel_lds + wave * (kWords + kRelKept * kWave);
   float* sc = rec + kWords + lane;
-  float* shared = rel_lds + waves * (kWords + kept * kWave);  // (waves, 64): the waves' maxima, then sums
-  float* learned = shared + (waves > 1 ? waves * kWave : 0);   // (buckets, H), in units of log 2
-  for (int i = threadIdx.x; i < a.buckets * a.L.H; i += blockDim.x) learned[i] = a.table[i] * (float)kRelLog2e;
+  float* shared = rel_lds + kWavesPerBlock * (kWords + kRelKept * kWave);  // (waves, 64): the waves' maxima, then sums
+  float* learned = shared + kWavesPerBlock * kWave;                        // (buckets, H), in units of log 2
+  for (int i = threadIdx.x; i < a.buckets * H; i += blockDim.x) learned[i] = a.table[i] * (float)kRelLog2e;
   __syncthreads();
   const int u = lane & (w.lanes - 1), s = lane >> w.shift, unit = u < w.units ? u : w.units - 1;
   const int h = unit / w.per_map, own = unit % w.per_map;
-  const bool odd = kSplit && (own & 1), writes = u < w.units && own < (kSplit ? 2 : 1);
+  const int odd = kSplit ? own & 1 : 0;
+  const bool writes = u < w.units && own < kEvery;
   const float* mine = rec + s * U::RW;  // this lane's edge of step 0
   const float scale = a.scale;
   const float* bias_of = learned + h;
@@ -153,11 +164,10 @@ __global__ __launch_bounds__(1024, 5) void relative_forward_units(RelArgs<float,
   if (!sh.live) return;  // one wave a row, or the whole workgroup
   float q[U::N];
   U::template load<false>(a.q, w, unit, sh.row, q);
-  const int held = sh.steps < steps ? sh.steps : steps;
-  float m = neg_inf<float>(), l = 0.f, inv = 0.f;
+  float m = neg_inf<float>(), l = 0.f;
 
-  // over a lane's slots (and, of a sum, the two lanes with a step each) and the row's waves.  A score that is not a
-  // number is not a maximum; its exponential makes the sum, and with it the row, not a number.
+  // over a lane's slots (and the two lanes with a step each) and the row's waves.  A score that is not a number is not
+  // a maximum; its exponential makes the sum, and with it the row, not a number.
   auto over_waves = [&](float v, bool maximum) {
     for (int o = w.lanes; o < kWave; o <<= 1) {
       const float x = __shfl_xor(v, o, kWave);
@@ -172,119 +182,84 @@ __global__ __launch_bounds__(1024, 5) void relative_forward_units(RelArgs<float,
       shared[sh.wave * kWave + lane] = v;
       __syncthreads();
       v = shared[lane];
-      for (int o = 1; o < waves; ++o) {
+      for (int o = 1; o < kWavesPerBlock; ++o) {
         const float x = shared[o * kWave + lane];
         v = maximum ? fmaxf(x, v) : v + x;
       }
     }
     return v;
   };
-  const uint32_t place = (uint32_t)(s * a.L.H + h);
-  // the weight of step t of the edges from `e`
-  auto write = [&](int64_t e, int t, float v) {
-    float* to = a.alpha + (e + t * w.slots) * a.L.H;
-    if (writes && s < (int)(sh.e1 - e) - t * w.slots) to[place] = v;
-  };
 
-  // phase 0: every score, its maximum; the first `steps` steps' stay in LDS.  The steps past them are scored again
-  // for the sum (1) and the weights (2): rows beyond 16 waves' LDS only.
-  for (int phase = 0; phase < 3; ++phase) {
-    if (phase == 1) {
-      m = over_waves(m, true);
-      m = m == neg_inf<float>() ? 0.f : m;  // no edge inside: exp(-inf) = 0 everywhere
-      if constexpr (kSplit) {
-        for (int t = 0; t < held; t += 2) {  // a step past `held` is outside: its weight is zero
-          const float x = exp2_of(sc[t / 2 * kWave] - m);
-          sc[t / 2 * kWave] = x;
-          l += x;
-        }
-      } else {
-        for (int t = 0; t < held; ++t) {
-          const float x = exp2_of(sc[t * kWave] - m);
-          sc[t * kWave] = x;
-          l += x;
+  // The scores: the first kRelKept rows stay in LDS, those past them wait in alpha, each for the lane that wrote it.
+  const int rows = (sh.steps + kEvery - 1) / kEvery, held = rows < kRelKept ? rows : kRelKept;
+  const uint32_t place = (uint32_t)((odd * w.slots + s) * H + h);
+  auto at = [&](int r) { return a.alpha + (sh.e0 + (int64_t)r * (kEvery * w.slots)) * H + place; };
+  auto has = [&](int r) { return writes && sh.e0 + (int64_t)r * (kEvery * w.slots) + odd * w.slots + s < sh.e1; };
+
+  Records<U::RW> records;
+  if (sh.steps > 0) records.request(a.records, sh.e0, sh.e1, lane);
+  for (int b = 0; b < sh.steps; b += w.lanes) {
+    const int64_t e = sh.e0 + (int64_t)b * w.slots;  // the batch's first edge
+    wave_lds();
+    records.put(rec, lane);
+    wave_lds();
+    if (b + w.lanes < sh.steps) records.request(a.records, e + kWave, sh.e1, lane);
+    const int ends = sh.steps - b < w.lanes ? sh.steps - b : w.lanes;
+    for (int t = 0; t < ends; t += kRelInFlight) {  // a step past the row's last is outside the window
+      constexpr int UN = kRelInFlight;
+      float2 head[UN];
+      float k[UN][U::N], cs[UN][U::NA], sn[UN][U::NA], v[UN];
+#pragma unroll
+      for (int n = 0; n < UN; ++n) {
+        const float* r = mine + (t + n) * w.slots * U::RW;
+        head[n] = *reinterpret_cast<const float2*>(r);
+#pragma unroll
+        for (int o = 0; o < U::NO; ++o) {
+          const float2 x = *reinterpret_cast<const float2*>(r + 2 + 2 * o);
+          cs[n][o] = x.x;
+          sn[n][o] = x.y;
         }
       }
-    }
-    if (phase == 2) {
-      l = over_waves(l, false);
-      inv = l == 0.f ? 0.f : 1.f / l;
-      if constexpr (kSplit) {
-        for (int t = 0; t < held; t += 2) write(sh.e0, t + odd, sc[t / 2 * kWave] * inv);
-      } else {
-        for (int t = 0; t < held; ++t) write(sh.e0, t, sc[t * kWave] * inv);
+#pragma unroll
+      for (int n = 0; n < UN; ++n)
+        U::template load<kNear>(a.k, w, unit, __float_as_int(head[n].x) & 0xFFFFFF, k[n]);
+      float bias[UN];
+#pragma unroll
+      for (int n = 0; n < UN; ++n) bias[n] = bias_of[(__float_as_uint(head[n].x) >> 24) * H];
+#pragma unroll
+      for (int n = 0; n < UN; ++n) v[n] = U::dot(q, k[n], cs[n], sn[n]);
+      sum_units<UN>(v, w.per_map);
+#pragma unroll
+      for (int n = 0; n < UN; ++n)  // outside the window: excluded, whatever its row holds
+        v[n] = head[n].y == neg_inf<float>() ? neg_inf<float>() : fmaf(scale, v[n], head[n].y + bias[n]);
+#pragma unroll
+      for (int n = 0; n < UN; n += kEvery) {
+        const float even = v[n], next = v[n + kEvery - 1], x = odd ? next : even;
+        const int r = (b + t + n) / kEvery;
+        m = fmaxf(m, x);
+        if (r < kRelKept)
+          sc[r * kWave] = x;
+        else if (has(r))
+          *at(r) = x;
       }
-    }
-    const int skip = phase == 0 ? 0 : steps;
-    if (skip >= sh.steps) continue;
-    const int first = skip & ~(w.lanes - 1);  // a batch's first step
-    Records<U::RW> records;
-    records.request(a.records, sh.e0 + (int64_t)first * w.slots, sh.e1, lane);
-    for (int b = first; b < sh.steps; b += w.lanes) {
-      const int64_t e = sh.e0 + (int64_t)b * w.slots;  // the batch's first edge
-      wave_lds();
-      records.put(rec, lane);
-      wave_lds();
-      if (b + w.lanes < sh.steps) records.request(a.records, e + kWave, sh.e1, lane);
-      const int ends = sh.steps - b < w.lanes ? sh.steps - b : w.lanes;
-      auto take = [&](int t) {
-        constexpr int UN = kRelInFlight;
-        float2 head[UN];
-        float k[UN][U::N], cs[UN][U::NA], sn[UN][U::NA], v[UN];
-#pragma unroll
-        for (int n = 0; n < UN; ++n) {
-          const float* r = mine + (t + n) * w.slots * U::RW;
-          head[n] = *reinterpret_cast<const float2*>(r);
-#pragma unroll
-          for (int o = 0; o < U::NO; ++o) {
-            const float2 x = *reinterpret_cast<const float2*>(r + 2 + 2 * o);
-            cs[n][o] = x.x;
-            sn[n][o] = x.y;
-          }
-        }
-#pragma unroll
-        for (int n = 0; n < UN; ++n)
-          U::template load<kNear>(a.k, w, unit, __float_as_int(head[n].x) & 0xFFFFFF, k[n]);
-        float bias[UN];
-#pragma unroll
-        for (int n = 0; n < UN; ++n) bias[n] = bias_of[(__float_as_uint(head[n].x) >> 24) * a.L.H];
-#pragma unroll
-        for (int n = 0; n < UN; ++n) v[n] = U::dot(q, k[n], cs[n], sn[n]);
-        sum_units<UN>(v, w.per_map);
-#pragma unroll
-        for (int n = 0; n < UN; ++n)  // outside the window: excluded, whatever its row holds
-          v[n] = head[n].y == neg_inf<float>() ? neg_inf<float>() : fmaf(scale, v[n], head[n].y + bias[n]);
-        if constexpr (kSplit) {
-#pragma unroll
-          for (int n = 0; n < UN; n += 2) {
-            const float even = v[n], next = v[n + 1], x = odd ? next : even;
-            if (phase == 0) {
-              m = fmaxf(m, x);
-              if (b + t < steps) sc[(b + t + n) / 2 * kWave] = x;
-            } else if (phase == 1) {
-              l += exp2_of(x - m);
-            } else {
-              write(e, t + n + odd, exp2_of(x - m) * inv);
-            }
-          }
-        } else {
-#pragma unroll
-          for (int n = 0; n < UN; ++n) {
-            if (phase == 0) {
-              m = fmaxf(m, v[n]);
-              if (b + t < steps) sc[(b + t + n) * kWave] = v[n];
-            } else if (phase == 1) {
-              l += exp2_of(v[n] - m);
-            } else {
-              write(e, t + n, exp2_of(v[n] - m) * inv);
-            }
-          }
-        }
-      };
-      int t = skip > b ? skip - b : 0;
-      for (; t < ends; t += kRelInFlight) take(t);
     }
   }
+  m = over_waves(m, true);
+  m = m == neg_inf<float>() ? 0.f : m;  // no edge inside: exp(-inf) = 0 everywhere
+  for (int r = 0; r < held; ++r) {
+    const float x = exp2_of(sc[r * kWave] - m);
+    sc[r * kWave] = x;
+    l += x;
+  }
+#pragma unroll 4
+  for (int r = kRelKept; r < rows; ++r) l += has(r) ? exp2_of(*at(r) - m) : 0.f;
+  l = over_waves(l, false);
+  const float inv = l == 0.f ? 0.f : 1.f / l;
+  for (int r = 0; r < held; ++r)
+    if (has(r)) *at(r) = sc[r * kWave] * inv;
+#pragma unroll 4
+  for (int r = kRelKept; r < rows; ++r)
+    if (has(r)) *at(r) = exp2_of(*at(r) - m) * inv;
 }
 
 // ---------------------------------------------------------------- backward
@@ -292,7 +267,7 @@ __global__ __launch_bounds__(1024, 5) void relative_forward_units(RelArgs<float,
 // Per pair of targets or of sources (kTargets or not): dq = scale sum ds tau k over a target's edges, dk = scale sum ds
 // conj(tau) q over a source's.
 template <typename R, typename U, bool kNear, bool kTargets, bool kSplit>
-__global__ __launch_bounds__(kRelThreadsB, (U::N > 10 ? 5 : 6)) void relative_rows_units(RelArgs<float, R> a,
+__global__ __launch_bounds__(kRelThreads, (U::N > 10 ? 5 : 6)) void relative_rows_units(RelArgs<float, R> a,
                                                                                          EdgeUnits w, int64_t blocks) {
   constexpr int RW = U::PW, kWords = kWave * RW;
   constexpr int kT = kSplit ? 1 : 2;
@@ -417,9 +392,8 @@ constexpr size_t kRelLds = 160 * 1024;
 
 // LDS of a pass: the records a wave (and the forward's scores, and the learned table), the waves' sums, the bins.
 template <typename U>
-size_t rel_forward_lds(int waves, bool split, int steps, int table) {
-  const int kept = split ? steps / 2 : steps;
-  return sizeof(float) * ((size_t)waves * kWave * (U::RW + kept + (waves > 1 ? 1 : 0)) + table);
+size_t rel_forward_lds(int table) {
+  return sizeof(float) * ((size_t)kWavesPerBlock * kWave * (U::RW + kRelKept + 1) + table);
 }
 template <typename U>
 size_t rel_rows_lds(int lanes) {
@@ -436,40 +410,17 @@ inline int rel_lds_limit(const void* kernel, size_t lds) {
 template <typename R, typename U, bool kNear, bool kSplit>
 int rel_launch(RelPass pass, const RelArgs<float, R>& a, EdgeUnits w, const RelRows& rows, hipStream_t stream) {
   w.first = 0;
-  if (pass == RelPass::Forward) {
-    // the rows of sixteen waves; those of four and of one, in one launch of workgroups of four
-    const auto kernel = &relative_forward_units<R, U, kNear, kSplit>;
-    for (int c = 0; c < 2; ++c) {
-      w.shared = rows.count[c];
-      w.single = c == 0 ? 0 : rows.count[2];
-      const int waves = c == 0 ? 16 : kWavesPerBlock;
-      if (w.shared + w.single > 0) {
-        const int64_t blocks = w.shared + blocks_for(w.single);
-        // sixteen waves' scores beside a large table: fewer steps of them (longer rows are scored again)
-        int steps = kRelSteps;
-        const int table = a.buckets * a.L.H;
-        while (rel_forward_lds<U>(waves, kSplit, steps, table) > kRelLds) steps -= kRelInFlight;
-        const size_t lds = rel_forward_lds<U>(waves, kSplit, steps, table);
-        int rc = rel_lds_limit(reinterpret_cast<const void*>(kernel), lds);
-        if (rc != GM_OK) return rc;
-        hipLaunchKernelGGL(kernel, dim3((unsigned)blocks), dim3(waves * kWave), lds, stream, a, w, blocks, steps);
-        rc = check_launch("relative");
-        if (rc != GM_OK) return rc;
-      }
-      w.first += w.shared;
-    }
-    return GM_OK;
-  }
   w.shared = rows.count[0] + rows.count[1];
   w.single = rows.count[2];
   const int64_t blocks = w.shared + blocks_for(w.single);
   if (blocks == 0) return GM_OK;
-  const auto kernel = pass == RelPass::BackwardTarget ? &relative_rows_units<R, U, kNear, true, kSplit>
-                                                      : &relative_rows_units<R, U, kNear, false, kSplit>;
-  const size_t lds = rel_rows_lds<U>(w.lanes);
+  const auto kernel = pass == RelPass::Forward          ? &relative_forward_units<R, U, kNear, kSplit>
+                      : pass == RelPass::BackwardTarget ? &relative_rows_units<R, U, kNear, true, kSplit>
+                                                        : &relative_rows_units<R, U, kNear, false, kSplit>;
+  const size_t lds = pass == RelPass::Forward ? rel_forward_lds<U>(a.buckets * a.L.H) : rel_rows_lds<U>(w.lanes);
   const int rc = rel_lds_limit(reinterpret_cast<const void*>(kernel), lds);
   if (rc != GM_OK) return rc;
-  hipLaunchKernelGGL(kernel, dim3((unsigned)blocks), dim3(kRelThreadsB), lds, stream, a, w, blocks);
+  hipLaunchKernelGGL(kernel, dim3((unsigned)blocks), dim3(kRelThreads), lds, stream, a, w, blocks);
   return check_launch("relative");
 }
 

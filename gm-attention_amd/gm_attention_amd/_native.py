@@ -1765,7 +1765,7 @@ def relative_forward(q: Tensor, k: Tensor, table: Tensor, tables: Any, heads: An
     if served is not heads:
         q, k = relative_repack(q, heads, served), relative_repack(k, heads, served)
     H, desc, device = served.heads, served.desc, q.device
-    order, counts = tables.target_rows(served.slots(tables))
+    order, counts = tables.lane_rows(served.slots(tables))
     tables.found()
     alpha = torch.empty(tables.n_edges, H, dtype=tables.dtype, device=device)
     _call_on(device, "gm_relative_forward_" + _PW_SUFFIX[q.dtype], _ptr(q), _ptr(k), _ptr(table),

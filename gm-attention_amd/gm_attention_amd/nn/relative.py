@@ -37,6 +37,9 @@ from gm_attention_amd.representations.field_type import SO2FieldType
 
 MAX_H, MAX_F, MAX_D = fused_attention.MAX_H, fused_attention.MAX_F, fused_attention.MAX_D
 MAX_BUCKETS = 256
+# up to here the scores' rows of more than 8 steps, not 32, take four waves: 2,048 targets 14.2 -> 9.1 us, 12,285
+# 46 -> 34; beyond it not (32,768: 131 -> 174)
+FEW_TARGETS = 16384
 MAX_SOURCES = 2**24  # of float32 tables: a record's word holds the source and the bucket
 
 
@@ -111,10 +114,15 @@ class RelativeEdgeTables(EdgeTables):
         if slots == 0:
             return None, None, None, None
         entries, ptr = self._paired(side)
-        # the classes are of 32 and 128 times their slots: of 16 and 64 steps
+        # rows beyond 16 steps of a wave are a workgroup's: 32 times these slots
         order, counts = self._rows((f"{side}' pairs", max(1, slots // 2)), lambda: ptr)
         # an edge set without edges has entries of no pair, and an address all the same
         return entries.data_ptr(), _native._ptr(ptr), _native._ptr(order), counts
+
+    def lane_rows(self, slots: int) -> tuple[Tensor | None, Any]:
+        """The targets in classes for the forward's lane kernels: rows beyond 32 steps of a wave are a
+        workgroup's, of few targets, where the longest row decides, beyond 8."""
+        return self.target_rows(max(1, slots // 4) if slots and self.n_targets <= FEW_TARGETS else slots)
 
     def _paired(self, side: str) -> tuple[Tensor, Tensor]:
         held = self._pairs.get(side)

@@ -349,21 +349,18 @@ int gm_differential_backward_bf16(const float* g, const uint16_t* q, const uint1
  *   1 <= buckets <= 256; indices are followed unchecked.
  * ds (n_edges, H) and partial (gm_relative_partial_rows() rows of buckets H) are
  * workspaces.  Sums in a fixed order.
- * order of the forward, or NULL: every target once, those of more than 128 S edges
- * first, then those of more than 32 S, then the rest, counts (HOST) how many of each,
- * for the S of gm_relative_slots.  With it (float and bfloat16 rows; q and k at
- * multiples of 16 bytes, records of 8) the lane kernels run; without, kernels for any
- * layout.  order of the backward, or NULL: every target once, long rows (a workgroup's
- * each) first, in three classes, counts how many of each (the first two are long).
+ * order, or NULL: every target once, in three classes, counts (HOST) how many of each;
+ * rows of the first two are a workgroup's each, so the long ones, of the last a wave's.
+ * With it the forward's lane kernels run (float and bfloat16 rows; q and k at multiples
+ * of 16 bytes, records of 8; S edges of a row at a time, gm_relative_slots); without,
+ * kernels for any layout.
  * pairs, or NULL: the backward's lane kernels run (float and bfloat16 rows; q, k, dq
  * and dk at multiples of 16 bytes, entries of 8).  The targets 2 i and 2 i + 1 are a
  * pair, and its entries pairs[pair_ptr[i] ..) are the sources that either has an edge
  * to, 4 orders words: the source, one left free, the edge of each target (-1: none),
  * integers all, then for every order 1 .. (cos, sin) of both edges.  Each edge is in one
- * entry.  pair_order: every pair once, those of more than 64 S entries first, then those
- * of more than 16 S, then the rest, pair_counts (HOST) how many of each (128 and 32
- * where S is 1).  pairs_s, pair_ptr_s, .. the same of the sources and the targets with
- * an edge to either.
+ * entry.  pair_order, pair_counts (HOST): the pairs in classes as the targets are.
+ * pairs_s, pair_ptr_s, .. the same of the sources and the targets with an edge to either.
  * Suffix _bf16: bfloat16 rows, float tables and arithmetic.  No reference
  * counterpart (the softmax without the learned bias: gm_softmax_*). */
 int64_t gm_relative_partial_rows(void);
