@@ -207,12 +207,11 @@ __global__ __launch_bounds__(kRelThreads, 5) void relative_forward_units(RelArgs
     const int ends = sh.steps - b < w.lanes ? sh.steps - b : w.lanes;
     for (int t = 0; t < ends; t += kRelInFlight) {  // a step past the row's last is outside the window
       constexpr int UN = kRelInFlight;
-      float2 head[UN];
       float k[UN][U::N], cs[UN][U::NA], sn[UN][U::NA], v[UN];
 #pragma unroll
       for (int n = 0; n < UN; ++n) {
         const float* r = mine + (t + n) * w.slots * U::RW;
-        head[n] = *reinterpret_cast<const float2*>(r);
+        U::template load<kNear>(a.k, w, unit, __float_as_int(r[0]) & 0xFFFFFF, k[n]);
 #pragma unroll
         for (int o = 0; o < U::NO; ++o) {
           const float2 x = *reinterpret_cast<const float2*>(r + 2 + 2 * o);
@@ -221,20 +220,19 @@ __global__ __launch_bounds__(kRelThreads, 5) void relative_forward_units(RelArgs
         }
       }
 #pragma unroll
-      for (int n = 0; n < UN; ++n)
-        U::template load<kNear>(a.k, w, unit, __float_as_int(head[n].x) & 0xFFFFFF, k[n]);
-      float bias[UN];
-#pragma unroll
-      for (int n = 0; n < UN; ++n) bias[n] = bias_of[(__float_as_uint(head[n].x) >> 24) * H];
-#pragma unroll
       for (int n = 0; n < UN; ++n) v[n] = U::dot(q, k[n], cs[n], sn[n]);
-      sum_units<UN>(v, w.per_map);
-#pragma unroll
-      for (int n = 0; n < UN; ++n)  // outside the window: excluded, whatever its row holds
-        v[n] = head[n].y == neg_inf<float>() ? neg_inf<float>() : fmaf(scale, v[n], head[n].y + bias[n]);
 #pragma unroll
       for (int n = 0; n < UN; n += kEvery) {
-        const float even = v[n], next = v[n + kEvery - 1], x = odd ? next : even;
+        const float2 head = *reinterpret_cast<const float2*>(mine + (t + n + odd) * w.slots * U::RW);
+        float x = v[n];
+        if constexpr (kSplit) {  // an even lane keeps the first step's sum, an odd one the second's
+          const float keep = odd ? v[n + 1] : v[n], give = odd ? v[n] : v[n + 1];
+          x = keep + next_lane(give);
+          for (int o = 2; o < w.per_map; o <<= 1) x += __shfl_xor(x, o, kWave);
+        }
+        // outside the window: excluded, whatever its row holds
+        x = head.y == neg_inf<float>() ? neg_inf<float>()
+                                       : fmaf(scale, x, head.y + bias_of[(__float_as_uint(head.x) >> 24) * H]);
         const int r = (b + t + n) / kEvery;
         m = fmaxf(m, x);
         if (r < kRelKept)

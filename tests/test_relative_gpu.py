@@ -228,6 +228,15 @@ def test_many_targets_for_each_workgroup(cuda):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("copies", [{0: 1, 1: 1, 2: 1}, {0: 4, 1: 4, 2: 4}])
+def test_long_rows_among_many_targets(copies, cuda):
+    """Rows that a wave takes alone though its scores fill more than it holds, beside some of a workgroup."""
+    degrees = [1] * 17_000
+    degrees[5], degrees[700], degrees[16_999], degrees[9000] = 300, 470, 511, 2000
+    check(bucketed(scattered(degrees, 3000, torch.float32), 11), copies, 4, torch.float32, cuda)
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("rows", ROWS)
 @pytest.mark.parametrize("copies", [{0: 4, 1: 4, 2: 4}, {0: 3, 1: 1}])
 def test_masked_rows_may_hold_anything(copies, rows, cuda):
