@@ -4,14 +4,15 @@
 //
 // Forward, a wave a target (a long row four): a step gathers S rows of k and sums a
 // score over its units' lanes; scores wait in LDS (a long row's in alpha) for their
-// maximum and sum.  63.0 M edges of 160 numbers take 2.87 ms: 14 TB/s of rows out of L1,
-// whose accesses keep it 60 % busy while vector instructions fill 55 % of the time;
-// neither gives way alone.
+// maximum and sum.  63.0 M edges of 160 numbers take 2.83 ms.  L1 bounds it: rows reach a
+// CU at 25 bytes a cycle (contiguous loads at 50), with all of them among 16 nodes it
+// takes 2.66 ms, without the dots 2.77, without the weights' writes 2.62.
 //
 // Backward, dq and dk: a wave a pair of neighbouring rows over the nodes of both, whose
 // rows are loaded once for two edges (four loads for seven edges on a grid).  1.86 and
-// 1.88 ms for the edges above; a row at a time 2.50 and 2.64.  The forward gains nothing
-// from pairs (2.99 ms): it has half the sums to keep, and its scores twice the places.
+// 1.88 ms for the edges above; a row at a time 2.50 and 2.64.  Scores do not gain from
+// pairs (3.68 ms): twice the registers of q, entries of 56 bytes, and alpha's places edge
+// by edge cost more than the rows' loads they spare.
 #pragma once
 #include <algorithm>
 #include <type_traits>

@@ -98,7 +98,7 @@ class RelativeEdgeTables(EdgeTables):
 
     def group_sources(self) -> tuple[Tensor, Tensor]:
         """Finds what a backward reads beside the edges, once: the pairs of targets and of sources
-        (returned: the sources'), or for float64 tables the edges sorted by source."""
+        (``(ptr, entries)`` of the sources'), or for float64 tables the edges sorted by source."""
         if self.dtype == torch.float64:
             return super().group_sources()
         self._paired("targets")
@@ -113,7 +113,7 @@ class RelativeEdgeTables(EdgeTables):
         kernels with ``slots`` edge slots a wave (0: none, the simple kernels)."""
         if slots == 0:
             return None, None, None, None
-        entries, ptr = self._paired(side)
+        ptr, entries = self._paired(side)
         # rows beyond 16 steps of a wave are a workgroup's: 32 times these slots
         order, counts = self._rows((f"{side}' pairs", max(1, slots // 2)), lambda: ptr)
         # an edge set without edges has entries of no pair, and an address all the same
@@ -134,7 +134,7 @@ class RelativeEdgeTables(EdgeTables):
         return held
 
     def _pair(self, targets: bool) -> tuple[Tensor, Tensor]:
-        """``(entries, ptr)``: every pair's entries, in order of their nodes."""
+        """``(ptr, entries)``: every pair's entries, in order of their nodes."""
         differential._outside_capture(self.row_ptr, "RelativeEdgeTables' pairs (a first call with these tables)")
         self.found()
         target = torch.repeat_interleave(torch.arange(self.n_targets, device=self.device),
@@ -170,7 +170,7 @@ class RelativeEdgeTables(EdgeTables):
         phases = self.records[at][:, :, 2:].reshape(n, 2, self.orders - 1, 2).masked_fill(~there[:, :, None, None], 0.0)
         entries[:n, 4:] = phases.transpose(1, 2).flatten(1)
         self._kept.append(_native.Made(entries, ptr))
-        return entries, ptr
+        return ptr, entries
 
     def _packed(self, source: Tensor) -> Tensor:
         buckets = self.buckets.long()
