@@ -79,9 +79,16 @@ __host__ __device__ __forceinline__ int64_t xcd_spread_block(int64_t b, int64_t 
   return (r * 8 + x) * chunk + i % chunk;
 }
 
-// The same, for blocks that walk their grid in a loop: 32-bit divisions.
+// The same in 32 bits, with shifts where the grid is large: for blocks that walk it in a loop, or are short.
 __device__ __forceinline__ uint32_t xcd_spread_block32(uint32_t b, uint32_t nb) {
-  const uint32_t chunk = nb >= 256 ? 32 : (nb >= 64 ? nb >> 5 : 1);
+  if (nb >= 256) {
+    const uint32_t rounds = nb >> 8, full = rounds << 8, head = (nb - full) & ~7u;
+    if (b < head) return full + b;
+    if (b >= head + full) return b;
+    const uint32_t i = (b - head) >> 3, k = i >> 5, r = (k & 1) ? rounds - 1 - (k >> 1) : k >> 1;
+    return (r << 8) + ((b & 7) << 5) + (i & 31);
+  }
+  const uint32_t chunk = nb >= 64 ? nb >> 5 : 1;
   const uint32_t rounds = nb / (8 * chunk), full = rounds * 8 * chunk, head = (nb - full) & ~7u;
   if (b < head) return full + b;
   if (b >= head + full) return b;

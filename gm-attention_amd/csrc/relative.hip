@@ -354,6 +354,7 @@ int rel_prepare(RelArgs<T, R>& a, const T* records, const int64_t* desc, const i
   a.n_edges = n_edges;
   a.scale = (T)(scale * kRelLog2e);
   a.gradient_scale = (T)scale;
+  a.by_heads = 65536u / (uint32_t)H + 1;
   return GM_OK;
 }
 

@@ -54,6 +54,7 @@ struct RelArgs {
   int64_t n_targets, n_sources, n_edges;
   T scale;           // of the scores, in units of log 2
   T gradient_scale;  // of the scores
+  uint32_t by_heads;  // 2^16 / H and one: lane / H is the upper half of its product
 };
 
 // Scores, their biases and their maxima are in units of log 2.

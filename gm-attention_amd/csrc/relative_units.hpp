@@ -118,13 +118,14 @@ __device__ __forceinline__ float next_lane(float v) {
 }
 
 // The row (a target, or a pair) that a wave works on, and which of its edges or entries; all of it scalar.
-__device__ __forceinline__ Share rel_share(const EdgeUnits& w, const int64_t* ptr, int64_t block, int64_t blocks) {
+__device__ __forceinline__ Share rel_share(const EdgeUnits& w, const int64_t* ptr) {
+  constexpr int waves = kWavesPerBlock;
   Share s;
   s.wave = uniform((int)(threadIdx.x >> 6));
-  const int waves = blockDim.x >> 6;
-  const bool one = block >= w.shared;
-  const int64_t at = one ? w.shared + xcd_spread_block(block - w.shared, blocks - w.shared) * waves + s.wave
-                         : xcd_spread_block(block, w.shared);
+  const uint32_t block = blockIdx.x, shared = (uint32_t)w.shared;
+  const bool one = block >= shared;
+  const uint32_t spread = xcd_spread_block32(one ? block - shared : block, one ? gridDim.x - shared : shared);
+  const int64_t at = one ? shared + (int64_t)spread * waves + s.wave : spread;
   s.part = one ? 0 : s.wave;
   s.parts = one ? 1 : waves;
   s.live = at < w.shared + w.single;
@@ -142,8 +143,7 @@ __device__ __forceinline__ Share rel_share(const EdgeUnits& w, const int64_t* pt
 
 // kSplit: a head has two units or more, whose lanes hold the same scores: two of them keep every second step's each.
 template <typename R, typename U, bool kNear, bool kSplit>
-__global__ __launch_bounds__(kRelThreads, 5) void relative_forward_units(RelArgs<float, R> a, EdgeUnits w,
-                                                                         int64_t blocks) {
+__global__ __launch_bounds__(kRelThreads, 5) void relative_forward_units(RelArgs<float, R> a, EdgeUnits w) {
   constexpr int kWords = kWave * U::RW, kEvery = kSplit ? 2 : 1;  // steps of a row of scores, of which a lane keeps one
   extern __shared__ __align__(16) float rel_lds[];
   const int lane = threadIdx.x & 63, wave = uniform((int)(threadIdx.x >> 6)), H = a.L.H;
@@ -154,14 +154,13 @@ __global__ __launch_bounds__(kRelThreads, 5) void relative_forward_units(RelArgs
   for (int i = threadIdx.x; i < a.buckets * H; i += blockDim.x) learned[i] = a.table[i] * (float)kRelLog2e;
   __syncthreads();
   const int u = lane & (w.lanes - 1), s = lane >> w.shift, unit = u < w.units ? u : w.units - 1;
-  const int h = unit / w.per_map, own = unit % w.per_map;
+  const int per = __builtin_ctz(w.per_map), h = unit >> per, own = unit & (w.per_map - 1);  // powers of two
   const int odd = kSplit ? own & 1 : 0;
-  const bool writes = u < w.units && own < kEvery;
   const float* mine = rec + s * U::RW;  // this lane's edge of step 0
   const float scale = a.scale;
   const float* bias_of = learned + h;
 
-  const Share sh = rel_share(w, a.row_ptr, blockIdx.x, blocks);
+  const Share sh = rel_share(w, a.row_ptr);
   if (!sh.live) return;  // one wave a row, or the whole workgroup
   float q[U::N];
   U::template load<false>(a.q, w, unit, sh.row, q);
@@ -191,11 +190,19 @@ __global__ __launch_bounds__(kRelThreads, 5) void relative_forward_units(RelArgs
     return v;
   };
 
-  // The scores: the first kRelKept rows stay in LDS, those past them wait in alpha, each for the lane that wrote it.
+  // The scores: the first kRelKept rows stay in LDS, those past them wait in alpha.  A row's numbers lie side by side
+  // there, and lane after lane writes and reads them, `from` the lane that formed them (whose own place is lane `to`'s):
+  // a lane's own places alternate between two steps, at several times the way through L1 (2.77 ms against 2.5).
   const int rows = (sh.steps + kEvery - 1) / kEvery, held = rows < kRelKept ? rows : kRelKept;
-  const uint32_t place = (uint32_t)((odd * w.slots + s) * H + h);
-  auto at = [&](int r) { return a.alpha + (sh.e0 + (int64_t)r * (kEvery * w.slots)) * H + place; };
-  auto has = [&](int r) { return writes && sh.e0 + (int64_t)r * (kEvery * w.slots) + odd * w.slots + s < sh.e1; };
+  const int numbers = kEvery * w.slots * H, edge = (int)((uint32_t)lane * a.by_heads >> 16);  // lane / H
+  const int step = edge >> (6 - w.shift), slot = edge & (w.slots - 1);
+  const int from = lane < numbers ? slot * w.lanes + ((lane - edge * H) << per) + step : lane;
+  const int to = own < kEvery && u < w.units ? (odd * w.slots + s) * H + h : lane;
+  // a lane's rows: all but the last for all lanes, the last for those within the row's edges
+  const int last = (int)((sh.e1 - sh.e0) * H - (int64_t)(rows - 1) * numbers);
+  const int mine_rows = lane < numbers ? (lane < last ? rows : rows - 1) : 0;
+  auto has = [&](int r) { return r < mine_rows; };
+  auto out = [&](int r) -> float& { return (a.alpha + (sh.e0 * H + (int64_t)r * numbers))[(uint32_t)lane]; };
 
   Records<U::RW> records;
   if (sh.steps > 0) records.request(a.records, sh.e0, sh.e1, lane);
@@ -206,9 +213,9 @@ __global__ __launch_bounds__(kRelThreads, 5) void relative_forward_units(RelArgs
     wave_lds();
     if (b + w.lanes < sh.steps) records.request(a.records, e + kWave, sh.e1, lane);
     const int ends = sh.steps - b < w.lanes ? sh.steps - b : w.lanes;
-    for (int t = 0; t < ends; t += kRelInFlight) {  // a step past the row's last is outside the window
-      constexpr int UN = kRelInFlight;
-      float k[UN][U::N], cs[UN][U::NA], sn[UN][U::NA], v[UN];
+    auto take = [&](int t, auto group) {
+      constexpr int UN = decltype(group)::value;
+      float k[UN][U::N], cs[UN][U::NA], sn[UN][U::NA], v[kRelInFlight] = {};
 #pragma unroll
       for (int n = 0; n < UN; ++n) {
         const float* r = mine + (t + n) * w.slots * U::RW;
@@ -223,7 +230,7 @@ __global__ __launch_bounds__(kRelThreads, 5) void relative_forward_units(RelArgs
 #pragma unroll
       for (int n = 0; n < UN; ++n) v[n] = U::dot(q, k[n], cs[n], sn[n]);
 #pragma unroll
-      for (int n = 0; n < UN; n += kEvery) {
+      for (int n = 0; n < UN; n += kEvery) {  // a step past the row's last is outside the window
         const float2 head = *reinterpret_cast<const float2*>(mine + (t + n + odd) * w.slots * U::RW);
         float x = v[n];
         if constexpr (kSplit) {  // an even lane keeps the first step's sum, an odd one the second's
@@ -233,15 +240,20 @@ __global__ __launch_bounds__(kRelThreads, 5) void relative_forward_units(RelArgs
         }
         // outside the window: excluded, whatever its row holds
         x = head.y == neg_inf<float>() ? neg_inf<float>()
-                                       : fmaf(scale, x, head.y + bias_of[(__float_as_uint(head.x) >> 24) * H]);
+                                       : fmaf(scale, x, head.y + bias_of[__umul24(__float_as_uint(head.x) >> 24, (uint32_t)H)]);
         const int r = (b + t + n) / kEvery;
         m = fmaxf(m, x);
-        if (r < kRelKept)
+        if (r < kRelKept) {
           sc[r * kWave] = x;
-        else if (has(r))
-          *at(r) = x;
+        } else {
+          const float y = __shfl(x, from, kWave);
+          if (has(r)) out(r) = y;
+        }
       }
-    }
+    };
+    int t = 0;
+    for (; t + kRelInFlight <= ends; t += kRelInFlight) take(t, std::integral_constant<int, kRelInFlight>());
+    if (t < ends) take(t, std::integral_constant<int, 1>());
   }
   m = over_waves(m, true);
   m = m == neg_inf<float>() ? 0.f : m;  // no edge inside: exp(-inf) = 0 everywhere
@@ -250,15 +262,25 @@ __global__ __launch_bounds__(kRelThreads, 5) void relative_forward_units(RelArgs
     sc[r * kWave] = x;
     l += x;
   }
+  if (rows > kRelKept) {
+    const float top = __shfl(m, from, kWave);
+    float sum = 0.f;
 #pragma unroll 4
-  for (int r = kRelKept; r < rows; ++r) l += has(r) ? exp2_of(*at(r) - m) : 0.f;
+    for (int r = kRelKept; r < rows; ++r) sum += has(r) ? exp2_of(out(r) - top) : 0.f;
+    l += __shfl(sum, to, kWave);
+  }
   l = over_waves(l, false);
-  const float inv = l == 0.f ? 0.f : 1.f / l;
+  const float inv = __shfl(l == 0.f ? 0.f : 1.f / l, from, kWave);
+  wave_lds();
+  const float* formed = sc - lane + from;
   for (int r = 0; r < held; ++r)
-    if (has(r)) *at(r) = sc[r * kWave] * inv;
+    if (has(r)) out(r) = formed[r * kWave] * inv;
+  if (rows > kRelKept) {
+    const float top = __shfl(m, from, kWave);
 #pragma unroll 4
-  for (int r = kRelKept; r < rows; ++r)
-    if (has(r)) *at(r) = exp2_of(*at(r) - m) * inv;
+    for (int r = kRelKept; r < rows; ++r)
+      if (has(r)) out(r) = exp2_of(out(r) - top) * inv;
+  }
 }
 
 // ---------------------------------------------------------------- backward
@@ -267,16 +289,16 @@ __global__ __launch_bounds__(kRelThreads, 5) void relative_forward_units(RelArgs
 // conj(tau) q over a source's.
 template <typename R, typename U, bool kNear, bool kTargets, bool kSplit>
 __global__ __launch_bounds__(kRelThreads, (U::N > 10 ? 5 : 6)) void relative_rows_units(RelArgs<float, R> a,
-                                                                                         EdgeUnits w, int64_t blocks) {
+                                                                                         EdgeUnits w) {
   constexpr int RW = U::PW, kWords = kWave * RW;
   constexpr int kT = kSplit ? 1 : 2;
   extern __shared__ __align__(16) float rel_lds[];
-  const Share sh = rel_share(w, kTargets ? a.pair_ptr : a.pair_ptr_s, blockIdx.x, blocks);
+  const Share sh = rel_share(w, kTargets ? a.pair_ptr : a.pair_ptr_s);
   if (!sh.live) return;
   const int lane = threadIdx.x & 63, H = a.L.H;
   float* rec = rel_lds + sh.wave * kWords;
   const int u = lane & (w.lanes - 1), s = lane >> w.shift, unit = u < w.units ? u : w.units - 1;
-  const int h = unit / w.per_map, odd = kSplit ? unit & 1 : 0;
+  const int h = unit >> __builtin_ctz(w.per_map), odd = kSplit ? unit & 1 : 0;  // units a head: a power of two
   const float* mine = rec + s * RW;
   const float* records_of = kTargets ? a.pairs : a.pairs_s;
   float sums[2 * U::N];
@@ -419,7 +441,7 @@ int rel_launch(RelPass pass, const RelArgs<float, R>& a, EdgeUnits w, const RelR
   const size_t lds = pass == RelPass::Forward ? rel_forward_lds<U>(a.buckets * a.L.H) : rel_rows_lds<U>(w.lanes);
   const int rc = rel_lds_limit(reinterpret_cast<const void*>(kernel), lds);
   if (rc != GM_OK) return rc;
-  hipLaunchKernelGGL(kernel, dim3((unsigned)blocks), dim3(kRelThreads), lds, stream, a, w, blocks);
+  hipLaunchKernelGGL(kernel, dim3((unsigned)blocks), dim3(kRelThreads), lds, stream, a, w);
   return check_launch("relative");
 }
 
