@@ -4,9 +4,10 @@
 //
 // Forward, a wave a target (a long row four): a step gathers S rows of k and sums a
 // score over its units' lanes; scores wait in LDS (a long row's in alpha) for their
-// maximum and sum.  63.0 M edges of 160 numbers take 2.83 ms.  L1 bounds it: rows reach a
-// CU at 25 bytes a cycle (contiguous loads at 50), with all of them among 16 nodes it
-// takes 2.66 ms, without the dots 2.77, without the weights' writes 2.62.
+// maximum and sum.  63.0 M edges of 160 numbers take 2.61 ms: rows reach a CU out of L1
+// at 27 bytes a cycle (contiguous loads at 50) while vector instructions fill half of the
+// time, and neither gives way alone (at 2.83 ms: all rows among 16 nodes 6% less, without
+// the dots 2%, without the weights' writes 8%).
 //
 // Backward, dq and dk: a wave a pair of neighbouring rows over the nodes of both, whose
 // rows are loaded once for two edges (four loads for seven edges on a grid).  1.86 and
@@ -192,7 +193,7 @@ __global__ __launch_bounds__(kRelThreads, 5) void relative_forward_units(RelArgs
 
   // The scores: the first kRelKept rows stay in LDS, those past them wait in alpha.  A row's numbers lie side by side
   // there, and lane after lane writes and reads them, `from` the lane that formed them (whose own place is lane `to`'s):
-  // a lane's own places alternate between two steps, at several times the way through L1 (2.77 ms against 2.5).
+  // a lane's own places alternate between two steps (2.77 ms for 2.73, and a fifth more accesses to L1).
   const int rows = (sh.steps + kEvery - 1) / kEvery, held = rows < kRelKept ? rows : kRelKept;
   const int numbers = kEvery * w.slots * H, edge = (int)((uint32_t)lane * a.by_heads >> 16);  // lane / H
   const int step = edge >> (6 - w.shift), slot = edge & (w.slots - 1);
