@@ -262,7 +262,7 @@ class SO2QueryKeyNorm(nn.Module):
     def _on(self, device: torch.device) -> Tensor | None:
         if self.frequencies is None:
             return None
-        key = ("_frequencies", str(device))
+        key = f"_frequencies {device}"
         held = self.__dict__.get(key)
         if held is None:
             held = self.__dict__[key] = torch.tensor(self.frequencies, dtype=torch.float64, device=device)
@@ -270,7 +270,7 @@ class SO2QueryKeyNorm(nn.Module):
         return held
 
     def __getstate__(self) -> dict:
-        return {n: v for n, v in self.__dict__.items() if not isinstance(n, tuple)}
+        return {n: v for n, v in self.__dict__.items() if not n.startswith("_frequencies ")}
 
     def forward_flat(self, q: Tensor, k: Tensor, positions: Tensor | None = None) -> tuple[Tensor, Tensor]:
         """Query and key rows ``(N, D)`` of one node set, with its ``positions (N, axes)``."""

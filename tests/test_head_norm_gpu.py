@@ -458,7 +458,7 @@ def test_module_is_its_function_and_survives_casts_and_copies():
     for other in (module, copy.deepcopy(module), pickle.loads(pickle.dumps(module)),
                   copy.deepcopy(module).to(torch.bfloat16).float()):
         assert all(torch.equal(a, b) for a, b in zip(other.forward_flat(q, k, at), want))
-    assert set(module.state_dict()) == {"query_gain", "key_gain"}
+    assert set(module.state_dict()) == {"query_gain", "key_gain"} and "query_gain" in dir(module)
     assert not list(SO2QueryKeyNorm(head, 2, gain=False).parameters())
 
 
