@@ -18,8 +18,9 @@ struct RelLayout : HeadsLayout {
 
 // The backward's lane kernels take two neighbouring rows (targets, or sources) at a time, a pair, over the entries of
 // both: an entry is a node that either row has an edge with, and the edge of each, so that a node's row is loaded once
-// for two edges.  Words of an entry: the node; one left free; the edges (-1: the row has none); (cos, sin) of both
-// edges for the orders 1 ..
+// for two edges.  Words of an entry: the node; the first row's edge (-1: it has none); one left free; the second's
+// edge; (cos, sin) of both edges for the orders 1 ..  What stands for entries past a pair's last, words of 0 and -inf in
+// turn, so reads as node 0 without edges.
 constexpr int kRelPairHead = 4;
 
 // Rows (pairs, or targets) by length: `order` lists them in three classes, a workgroup a row in the first two, a wave a

@@ -314,17 +314,15 @@ __global__ __launch_bounds__(kRelThreads, (U::N > 10 ? 5 : 6)) void relative_row
     wave_lds();
     if (b + w.lanes < sh.steps) records.request(records_of, e + kWave, sh.e1, lane);
     const int ends = sh.steps - b < w.lanes ? sh.steps - b : w.lanes;
-    const int left = (int)(sh.e1 - e < kWave ? sh.e1 - e : kWave);
     auto take = [&](int t, auto group) {
       constexpr int UN = decltype(group)::value;
       float x[UN][U::N], d[UN][kT];
 #pragma unroll
       for (int n = 0; n < UN; ++n) {
         const float* r = mine + (t + n) * w.slots * RW;
-        const bool in = (t + n) * w.slots + s < left;  // past the end: node 0's row, no edges
 #pragma unroll
         for (int j = 0; j < kT; ++j) {
-          const int edge = in ? __float_as_int(r[2 + odd + j]) : -1;
+          const int edge = __float_as_int(r[1 + 2 * (odd + j)]);  // past the end: negative
           const uint32_t place = edge < 0 ? 0u : (uint32_t)edge;
           float ds;
           if constexpr (kNear)  // as the rows': a 32-bit offset from a scalar address
@@ -334,7 +332,7 @@ __global__ __launch_bounds__(kRelThreads, (U::N > 10 ? 5 : 6)) void relative_row
             ds = a.ds[(int64_t)place * H + h];
           d[n][j] = edge < 0 ? 0.f : ds;
         }
-        U::template load<kNear>(kTargets ? a.k : a.q, w, unit, in ? __float_as_int(r[0]) : 0, x[n]);
+        U::template load<kNear>(kTargets ? a.k : a.q, w, unit, __float_as_int(r[0]), x[n]);
       }
 #pragma unroll
       for (int n = 0; n < UN; ++n) {

@@ -166,7 +166,7 @@ class RelativeEdgeTables(EdgeTables):
         entries = torch.zeros(max(n, 1), 4 * self.orders, dtype=torch.float32, device=self.device)
         words = entries.view(torch.int32)
         words[:n, 0] = key % max(nodes, 1)
-        words[:n, 2:4] = edges
+        words[:n, 1], words[:n, 3] = edges.unbind(1)
         phases = self.records[at][:, :, 2:].reshape(n, 2, self.orders - 1, 2).masked_fill(~there[:, :, None, None], 0.0)
         entries[:n, 4:] = phases.transpose(1, 2).flatten(1)
         self._kept.append(_native.Made(entries, ptr))

@@ -357,8 +357,8 @@ int gm_differential_backward_bf16(const float* g, const uint16_t* q, const uint1
  * pairs, or NULL: the backward's lane kernels run (float and bfloat16 rows; q, k, dq
  * and dk at multiples of 16 bytes, entries of 8).  The targets 2 i and 2 i + 1 are a
  * pair, and its entries pairs[pair_ptr[i] ..) are the sources that either has an edge
- * to, 4 orders words: the source, one left free, the edge of each target (-1: none),
- * integers all, then for every order 1 .. (cos, sin) of both edges.  Each edge is in one
+ * to, 4 orders words: the source, the first target's edge (-1: none), one left free,
+ * the second's edge, integers all, then for every order 1 .. (cos, sin) of both edges.  Each edge is in one
  * entry.  pair_order, pair_counts (HOST): the pairs in classes as the targets are.
  * pairs_s, pair_ptr_s, .. the same of the sources and the targets with an edge to either.
  * Suffix _bf16: bfloat16 rows, float tables and arithmetic.  No reference
