@@ -10,8 +10,8 @@
 // the dots 2%, without the weights' writes 8%).
 //
 // Backward, dq and dk: a wave a pair of neighbouring rows over the nodes of both, whose
-// rows are loaded once for two edges (four loads for seven edges on a grid).  1.86 and
-// 1.88 ms for the edges above; a row at a time 2.50 and 2.64.  Scores do not gain from
+// rows are loaded once for two edges (four loads for seven edges on a grid).  1.77 and
+// 1.84 ms for the edges above; a row at a time 2.50 and 2.64.  Scores do not gain from
 // pairs (3.68 ms): twice the registers of q, entries of 56 bytes, and alpha's places edge
 // by edge cost more than the rows' loads they spare.
 #pragma once
