@@ -9,14 +9,15 @@
 //
 // The backward reads the forward's weights: a score is formed once.  A pass over
 // alpha and g, which lie edge by edge, writes ds and adds the buckets' sums; one over
-// the targets and one over the sources read ds.  An edge of
-// weight zero counts for nothing, whatever its rows and its g hold: so do the edges
-// outside the window.  No atomics between waves: sums are in a fixed order.
+// the targets and one over the sources read ds.  An edge of weight zero counts for
+// nothing, whatever its rows and its g hold: so do the edges outside the window.  No
+// atomics between waves: sums are in a fixed order.
 //
 // Per edge a pass reads one record of 32-bit words (64-bit for double): the source
 // with the bucket above it, the bias in units of log 2 (-inf outside the window) and
 // the transport's (cos, sin) of orders 1 .., packed once for an edge set; the source
-// side's name the target and the edge.
+// side's name the target and the edge.  (The backward's lane kernels read the merged
+// entries of two rows instead: relative.hpp.)
 #include "relative.hpp"
 #include "partial_sum.hpp"
 
