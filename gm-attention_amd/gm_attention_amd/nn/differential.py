@@ -429,28 +429,52 @@ def _whole(rows: Tensor) -> Tensor:
     return rows if rows.data_ptr() % 16 == 0 else rows.clone()
 
 
-def _eager(q: Tensor, k: Tensor, lam: Tensor, tables: EdgeTables, plan: fused_attention.Plan, scale: float) -> Tensor:
-    """The formulas in torch, in the tables' arithmetic."""
-    n, maps = tables.n_targets, plan.heads
-    target = torch.repeat_interleave(torch.arange(n, device=q.device), tables.row_ptr[1:] - tables.row_ptr[:-1])
+def torch_weights(q: Tensor, k: Tensor, row_ptr: Tensor, source: Tensor, phases: Tensor, bias: Tensor,
+                  plan: fused_attention.Plan, scale: float, learned: Tensor | None = None) -> tuple[Tensor, Tensor]:
+    """``(weights, none)``, both ``(n_edges, plan.heads)``: the softmax of every head (or map) in torch, in the
+    arithmetic of ``bias (n_edges,)`` (``-inf`` outside the window), ``learned (n_edges, plan.heads)`` added to the
+    scores; ``none`` marks the weights of zero, whose edges count for nothing in a gradient.
+
+    An edge outside the window, or of a score of -inf, has weight zero in any row: one whose other scores are not
+    numbers too."""
+    n, heads, dtype = row_ptr.shape[0] - 1, plan.heads, bias.dtype
+    target = torch.repeat_interleave(torch.arange(n, device=q.device), row_ptr[1:] - row_ptr[:-1])
     # an edge outside the window reads nothing: its row may hold anything
-    inside = (tables._bias != -math.inf).unsqueeze(-1)
-    qe = q.to(tables.dtype).index_select(0, target).masked_fill(~inside, 0.0)
-    ke = k.to(tables.dtype).index_select(0, tables._source).masked_fill(~inside, 0.0)
+    outside = (bias == -math.inf).unsqueeze(-1)
+    qe = q.to(dtype).index_select(0, target).masked_fill(outside, 0.0)
+    ke = k.to(dtype).index_select(0, source).masked_fill(outside, 0.0)
     score = 0.0
     for f, a, off, _, dim in plan.rows:
-        block = slice(off, off + maps * a * dim)
+        block = slice(off, off + heads * a * dim)
         if f == 0:
-            score = score + (qe[:, block] * ke[:, block]).reshape(-1, maps, a).sum(-1)
+            score = score + (qe[:, block] * ke[:, block]).reshape(-1, heads, a).sum(-1)
         else:
-            qr, qi = qe[:, block].reshape(-1, maps, a, 2).unbind(-1)
-            kr, ki = ke[:, block].reshape(-1, maps, a, 2).unbind(-1)
-            cos, sin = tables._phases[:, 2 * f - 2, None], tables._phases[:, 2 * f - 1, None]
+            qr, qi = qe[:, block].reshape(-1, heads, a, 2).unbind(-1)
+            kr, ki = ke[:, block].reshape(-1, heads, a, 2).unbind(-1)
+            cos, sin = phases[:, 2 * f - 2, None], phases[:, 2 * f - 1, None]
             score = score + cos * (qr * kr + qi * ki).sum(-1) + sin * (qi * kr - qr * ki).sum(-1)
-    score = scale * score + tables._bias.unsqueeze(-1)
-    index = target.unsqueeze(-1).expand(-1, maps)
-    top = score.new_full((n, maps), -math.inf).scatter_reduce(0, index, score.detach(), "amax")
-    weight = torch.exp(score - top.masked_fill(top == -math.inf, 0.0).index_select(0, target))
-    total = score.new_zeros(n, maps).index_add(0, target, weight)
+    score = scale * score + (bias.unsqueeze(-1) if learned is None else bias.unsqueeze(-1) + learned)
+    out = outside | (score == -math.inf)
+    index = target.unsqueeze(-1).expand(-1, heads)
+    top = score.new_full((n, heads), -math.inf).scatter_reduce(0, index, score.detach().masked_fill(out, -math.inf),
+                                                               "amax")
+    weight = torch.exp(score - top.masked_fill(top == -math.inf, 0.0).index_select(0, target)).masked_fill(out, 0.0)
+    total = score.new_zeros(n, heads).index_add(0, target, weight)
     weight = weight / total.masked_fill(total == 0, 1.0).index_select(0, target)
-    return weight[:, 0::2] - lam.to(tables.dtype) * weight[:, 1::2]
+    none = out | (weight == 0)
+
+    # a factor of zero is not enough where the other one is infinite or no number
+    def over_rows(g: Tensor) -> Tensor:
+        return g.masked_fill(torch.cat([none.repeat_interleave(a * dim, 1) for _, a, _, _, dim in plan.rows], 1), 0.0)
+
+    for t, kept in ((score, lambda g: g.masked_fill(none, 0.0)), (qe, over_rows), (ke, over_rows)):
+        if t.requires_grad:
+            t.register_hook(kept)
+    return weight.masked_fill(none, 0.0), none
+
+
+def _eager(q: Tensor, k: Tensor, lam: Tensor, tables: EdgeTables, plan: fused_attention.Plan, scale: float) -> Tensor:
+    """The formulas in torch, in the tables' arithmetic."""
+    weight, none = torch_weights(q, k, tables.row_ptr, tables._source, tables._phases, tables._bias, plan, scale)
+    alpha = weight[:, 0::2] - lam.to(tables.dtype) * weight[:, 1::2]
+    return alpha.masked_fill(none[:, 0::2] & none[:, 1::2], 0.0)

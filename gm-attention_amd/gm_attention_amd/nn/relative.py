@@ -353,25 +353,5 @@ def _eager(q: Tensor, k: Tensor, table: Tensor, tables: RelativeEdgeTables, plan
 def _weights(q: Tensor, k: Tensor, table: Tensor, buckets: Tensor, row_ptr: Tensor, source: Tensor, phases: Tensor,
              bias: Tensor, plan: fused_attention.Plan, scale: float) -> Tensor:
     """The formulas in torch, in the bias's arithmetic (``-inf`` outside the window)."""
-    n, heads, dtype = row_ptr.shape[0] - 1, plan.heads, bias.dtype
-    target = torch.repeat_interleave(torch.arange(n, device=q.device), row_ptr[1:] - row_ptr[:-1])
-    # an edge outside the window reads nothing: its row may hold anything
-    inside = (bias != -math.inf).unsqueeze(-1)
-    qe = q.to(dtype).index_select(0, target).masked_fill(~inside, 0.0)
-    ke = k.to(dtype).index_select(0, source).masked_fill(~inside, 0.0)
-    score = 0.0
-    for f, a, off, _, dim in plan.rows:
-        block = slice(off, off + heads * a * dim)
-        if f == 0:
-            score = score + (qe[:, block] * ke[:, block]).reshape(-1, heads, a).sum(-1)
-        else:
-            qr, qi = qe[:, block].reshape(-1, heads, a, 2).unbind(-1)
-            kr, ki = ke[:, block].reshape(-1, heads, a, 2).unbind(-1)
-            cos, sin = phases[:, 2 * f - 2, None], phases[:, 2 * f - 1, None]
-            score = score + cos * (qr * kr + qi * ki).sum(-1) + sin * (qi * kr - qr * ki).sum(-1)
-    score = scale * score + (bias.unsqueeze(-1) + table.to(dtype).index_select(0, buckets))
-    index = target.unsqueeze(-1).expand(-1, heads)
-    top = score.new_full((n, heads), -math.inf).scatter_reduce(0, index, score.detach(), "amax")
-    weight = torch.exp(score - top.masked_fill(top == -math.inf, 0.0).index_select(0, target))
-    total = score.new_zeros(n, heads).index_add(0, target, weight)
-    return weight / total.masked_fill(total == 0, 1.0).index_select(0, target)
+    learned = table.to(bias.dtype).index_select(0, buckets)
+    return differential.torch_weights(q, k, row_ptr, source, phases, bias, plan, scale, learned)[0]

@@ -757,6 +757,11 @@ def test_copied_tables_give_the_same_results(rows, cuda, tmp_path):
         compare(got[name], want[name], name)
 
 
+@pytest.mark.parametrize("rows", ROWS)
+def test_masked_rows_may_hold_anything_on_the_cpu(rows):
+    test_masked_rows_may_hold_anything(rows, "cpu")
+
+
 def test_copied_tables_on_the_cpu_give_the_same_results():
     copies, heads, rows = {0: 2, 1: 2}, 2, torch.float64
     graph = scattered([3, 0, 70, 9, 1], 40, rows)

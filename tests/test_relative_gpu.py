@@ -607,6 +607,36 @@ def test_cpu_rows_take_the_formulas_in_torch(copies, heads, rows):
     check(bucketed(scattered([0, 1, 5, 9, 40, 3, 70, 0, 8], 13, tables_dtype(rows)), 4), copies, heads, rows, "cpu")
 
 
+@pytest.mark.parametrize("rows", ROWS)
+@pytest.mark.parametrize("copies", [{0: 4, 1: 4, 2: 4}, {0: 3, 1: 1}])
+def test_masked_rows_may_hold_anything_on_the_cpu(copies, rows):
+    test_masked_rows_may_hold_anything(copies, rows, "cpu")
+
+
+def test_learned_biases_of_minus_infinity_on_the_cpu():
+    test_learned_biases_of_minus_infinity_shut_their_buckets({0: 4, 1: 4, 2: 4}, "cpu")
+
+
+def test_edges_of_weight_zero_on_the_cpu():
+    """Inside the window too they add nothing to a gradient, whatever their g, the learned number or the row
+    that made their score -inf hold."""
+    tables = RelativeEdgeTables(torch.tensor([0, 5]), torch.arange(5), torch.ones(5, 1, 2), torch.zeros(5),
+                                torch.tensor([1, 1, 1, 1, 0], dtype=torch.uint8), torch.arange(5), 5, n_sources=5)
+    q = torch.ones(1, 1, requires_grad=True)
+    k = torch.tensor([[0.5], [-0.25], [-math.inf], [-400.0], [math.nan]], requires_grad=True)
+    table = torch.tensor([[0.0], [0.25], [0.0], [0.0], [math.nan]], requires_grad=True)
+    alpha = relative_softmax(q, k, table, tables, SO2FieldType({0: 1}), 1)
+    w = 1 / (1 + math.exp(-0.5))  # of the scores 0.5 and 0
+    torch.testing.assert_close(alpha, torch.tensor([[w], [1 - w], [0.0], [0.0], [0.0]]))
+    dq, dk, dtable = torch.autograd.grad(alpha, (q, k, table),
+                                         torch.tensor([[1.0], [3.0], [math.inf], [math.nan], [math.nan]]))
+    ds = w * (1 - w) * (1 - 3)
+    zeros = [[0.0]] * 3
+    torch.testing.assert_close(dq, torch.tensor([[ds * 0.75]]))
+    torch.testing.assert_close(dk, torch.tensor([[ds], [-ds], *zeros]))
+    torch.testing.assert_close(dtable, torch.tensor([[ds], [-ds], *zeros]))
+
+
 def test_copied_tables_on_the_cpu_give_the_same_results():
     graph = bucketed(scattered([3, 0, 70, 9, 1], 40, torch.float64), 256)
     values = inputs(graph, {0: 2, 1: 2}, 2, torch.float64)
