@@ -29,6 +29,9 @@ constexpr int kRelKept = 16;  // rows of scores that LDS holds a wave: 16 steps,
 // (with four steps and four waves the scores of 33 M edges take 1.55 ms and the rows of 63 M 2.15, so 1.42 and 1.86).
 constexpr int kRelInFlight = 2;
 constexpr int kRelThreads = kWavesPerBlock * kWave;
+// What stands among a row's exponentials for a score of -inf, outside the window for one: no exponential has these
+// bits, and as a number they add nothing.  Its weight is zero in any row, one whose sum is no number too.
+constexpr uint32_t kRelNone = 0x80000000u;
 
 // A lane's shape; NO, the orders of the tables above 0.
 template <int A0, int A1, int A2, int ORD>
@@ -259,8 +262,8 @@ __global__ __launch_bounds__(kRelThreads, 5) void relative_forward_units(RelArgs
   m = over_waves(m, true);
   m = m == neg_inf<float>() ? 0.f : m;  // no edge inside: exp(-inf) = 0 everywhere
   for (int r = 0; r < held; ++r) {
-    const float x = exp2_of(sc[r * kWave] - m);
-    sc[r * kWave] = x;
+    const float score = sc[r * kWave], x = exp2_of(score - m);
+    sc[r * kWave] = score == neg_inf<float>() ? __uint_as_float(kRelNone) : x;
     l += x;
   }
   if (rows > kRelKept) {
@@ -274,13 +277,18 @@ __global__ __launch_bounds__(kRelThreads, 5) void relative_forward_units(RelArgs
   const float inv = __shfl(l == 0.f ? 0.f : 1.f / l, from, kWave);
   wave_lds();
   const float* formed = sc - lane + from;
-  for (int r = 0; r < held; ++r)
-    if (has(r)) out(r) = formed[r * kWave] * inv;
+  for (int r = 0; r < held; ++r) {
+    const float x = formed[r * kWave];
+    if (has(r)) out(r) = __float_as_uint(x) == kRelNone ? 0.f : x * inv;
+  }
   if (rows > kRelKept) {
     const float top = __shfl(m, from, kWave);
 #pragma unroll 4
-    for (int r = kRelKept; r < rows; ++r)
-      if (has(r)) out(r) = exp2_of(out(r) - top) * inv;
+    for (int r = kRelKept; r < rows; ++r) {
+      if (!has(r)) continue;
+      const float score = out(r);
+      out(r) = score == neg_inf<float>() ? 0.f : exp2_of(score - top) * inv;
+    }
   }
 }
 

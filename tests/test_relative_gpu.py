@@ -299,6 +299,59 @@ def test_learned_biases_of_minus_infinity_shut_their_buckets(copies, cuda):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("rows", ROWS)
+@pytest.mark.parametrize("copies,heads", [({0: 4, 1: 4, 2: 4}, 8), ({0: 4, 1: 4, 2: 4}, 16), ({0: 1, 1: 1, 2: 1}, 4),
+                                          ({0: 3, 1: 2, 2: 1}, 5), ({0: 2, 3: 2}, 4)])
+def test_rows_of_no_number_leave_the_edges_that_are_shut(copies, heads, rows, cuda):
+    """A key that is no number makes the weights of the rows that read it no numbers, of its head alone and not those of
+    the edges outside the window or of a learned -inf: these stay zero and add nothing to any gradient."""
+    shut_edges(copies, heads, rows, cuda)
+
+
+@pytest.mark.parametrize("rows", ROWS)
+def test_rows_of_no_number_on_the_cpu(rows):
+    shut_edges({0: 3, 1: 2, 2: 1}, 2, rows, "cpu")
+
+
+def shut_edges(copies, heads, rows, device):
+    dtype = tables_dtype(rows)
+    graph = bucketed(scattered([1, 2, 9, 40, 6, 300, 1, 700, 3, 2100, 5200, 64], 60, dtype, outside=0.4,
+                               order=max(copies)), 4)
+    q, k, table, g = inputs(graph, copies, heads, rows)
+    lost = graph.source == 7
+    shut = (graph.buckets == 0) & ~lost
+    use = graph.inside.bool() & ~shut
+    bad = torch.zeros(graph.n_targets, dtype=torch.bool)
+    bad[graph.target[use & lost]] = True
+    assert 3 <= int(bad.sum()) < graph.n_targets - 3
+    nan = use & bad[graph.target]
+    graph.buckets = torch.where(nan, 1, torch.where(shut, 0, 2 + graph.source % 2))
+    table[0] = -math.inf
+    tables, results = tables_of(graph, dtype, device), []
+    for value in (0.0, math.nan):
+        k[7, copies[0]] = value  # the second head's first number
+        leaves = [x.to(to).to(device, copy=True).requires_grad_(True)
+                  for x, to in ((q, rows), (k, rows), (table, dtype))]
+        alpha = relative_softmax(*leaves, tables, SO2FieldType(copies), heads)
+        grads = torch.autograd.grad(alpha, leaves, g.to(dtype).to(device))
+        results.append([x.detach().cpu() for x in (alpha, *grads)])
+    head, at = torch.zeros(q.shape[1], dtype=torch.bool), 0
+    for f, c in copies.items():
+        w = c * (1 if f == 0 else 2)
+        head[at + w:at + 2 * w] = True
+        at += heads * w
+    sources = torch.zeros(graph.n_sources, dtype=torch.bool)
+    sources[graph.source[nan]] = True
+    second = torch.arange(heads) == 1
+    expected = (nan.unsqueeze(1) & second, bad.unsqueeze(1) & head, sources.unsqueeze(1) & head,
+                (torch.arange(4) == 1).unsqueeze(1) & second)
+    assert bool((results[1][0][~use] == 0).all())
+    for name, clean, got, where in zip(("alpha", "dq", "dk", "dtable"), *results, expected):
+        assert torch.equal(got.isnan(), where), name
+        assert torch.equal(got[~where], clean[~where]), name
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("common", [0.0, 10.0, 1000.0])
 @pytest.mark.parametrize("copies,heads", [({0: 4, 1: 4, 2: 4}, 8), ({0: 3, 1: 1}, 3)])
 def test_gradients_with_a_common_part(copies, heads, common, cuda):
