@@ -176,6 +176,14 @@ __global__ __launch_bounds__(1024) void differential_forward_units(DfArgs<float,
       for (; t < ends; t += 2) take(t, std::integral_constant<int, 2>());
     }
   }
+  // zero times no number: the edges outside the window of such a row have been given that
+  if (__any(inv != inv)) {
+    __threadfence_block();  // behind the writes of other lanes
+    for (int64_t e = sh.e0 + lane; e < sh.e1; e += kWave) {
+      if (a.records[e * U::RW + 1] != neg_inf<float>()) continue;
+      for (int h = 0; h < a.L.H; ++h) a.alpha[e * a.L.H + h] = 0.f;
+    }
+  }
 }
 
 // ---------------------------------------------------------------- backward

@@ -265,6 +265,52 @@ def test_masked_rows_may_hold_anything(rows, cuda):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("rows", ROWS)
+@pytest.mark.parametrize("copies,heads", [({0: 2, 1: 2, 2: 2}, 8), ({0: 4, 1: 4, 2: 4}, 16), ({0: 3, 1: 2, 2: 1}, 3)])
+def test_rows_of_no_number_leave_the_edges_outside(copies, heads, rows, cuda):
+    """A key that is no number makes the weights of the rows that read it no numbers, of its head alone and not those of
+    the edges outside the window: these stay zero and add nothing to any gradient."""
+    edges_outside(copies, heads, rows, cuda)
+
+
+@pytest.mark.parametrize("rows", ROWS)
+def test_rows_of_no_number_on_the_cpu(rows):
+    edges_outside({0: 3, 1: 2, 2: 1}, 2, rows, "cpu")
+
+
+def edges_outside(copies, heads, rows, device):
+    dtype = tables_dtype(rows)
+    graph = scattered([1, 2, 9, 40, 6, 300, 1, 700, 3, 2100, 5200, 64], 60, dtype, outside=0.4)
+    q, k, lam, g = inputs(graph, copies, heads, rows)
+    use = graph.inside.bool()
+    bad = torch.zeros(graph.n_targets, dtype=torch.bool)
+    bad[graph.target[use & (graph.source == 7)]] = True
+    assert 3 <= int(bad.sum()) < graph.n_targets - 3
+    nan = use & bad[graph.target]
+    tables, results = graph.tables(dtype, device), []
+    for value in (0.0, math.nan):
+        k[7, 2 * copies[0]] = value  # the first number of the second head's first map
+        leaves = [x.to(to).to(device, copy=True).requires_grad_(True)
+                  for x, to in ((q, rows), (k, rows), (lam, dtype))]
+        alpha = differential_softmax(*leaves, tables, SO2FieldType(copies), heads)
+        grads = torch.autograd.grad(alpha, leaves[:2], g.to(dtype).to(device))
+        results.append([x.detach().cpu() for x in (alpha, *grads)])
+    columns, at = torch.zeros(q.shape[1], dtype=torch.bool), 0
+    for f, c in copies.items():
+        w = c * (1 if f == 0 else 2)
+        columns[at + 2 * w:at + 3 * w] = True
+        at += 2 * heads * w
+    sources = torch.zeros(graph.n_sources, dtype=torch.bool)
+    sources[graph.source[nan]] = True
+    expected = (nan.unsqueeze(1) & (torch.arange(heads) == 1), bad.unsqueeze(1) & columns,
+                sources.unsqueeze(1) & columns)
+    assert bool((results[1][0][~use] == 0).all())
+    for name, clean, got, where in zip(("alpha", "dq", "dk"), *results, expected):
+        assert torch.equal(got.isnan(), where), name
+        assert torch.equal(got[~where], clean[~where]), name
+
+
+@pytest.mark.gpu
 def test_biases_of_the_lowest_value_inside_the_window(cuda):
     """A row whose every bias is the type's lowest is uniform; beside an ordinary
     one such an edge has weight zero; a row of -inf biases has none inside."""
