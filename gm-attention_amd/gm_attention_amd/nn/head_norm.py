@@ -198,10 +198,11 @@ def _eager(x: Tensor, gain: Tensor | None, layout: HeadRows, eps: float | None, 
     v = x.to(_native.param_dtype(x.dtype))
     n, heads = x.shape[0], layout.heads
     blocks = [v[:, off:off + heads * a * dim].reshape(n, heads, a, dim) for _, a, off, _, dim in layout.plan.rows]
-    if eps is not None:
-        mean = sum(b.square().sum((2, 3)) for b in blocks) / layout.numbers
+    if eps is not None:  # in 64 bits: squares and their sums, forward and back, pass 32 bits' range
+        wide = [b.double() for b in blocks]
+        mean = sum(b.square().sum((2, 3)) for b in wide) / layout.numbers
         inv = torch.rsqrt(mean + eps)[:, :, None, None]
-        blocks = [b * inv for b in blocks]
+        blocks = [(b * inv).to(v.dtype) for b in wide]
     if gain is not None:
         at = gain.split([a for _, a, *_ in layout.plan.rows])
         blocks = [b * g[None, None, :, None] for b, g in zip(blocks, at)]

@@ -448,6 +448,24 @@ def test_cpu_rows_take_the_formulas_in_torch(copies, heads, rows):
     check(copies, heads, 12, 2, rows, "cpu")
 
 
+@pytest.mark.parametrize("rows", [torch.float32, torch.bfloat16])
+def test_the_smallest_and_largest_numbers_on_the_cpu(rows):
+    test_the_smallest_and_largest_numbers(rows, "cpu")
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("rows", [torch.float32, torch.bfloat16])
+def test_the_largest_numbers_beyond_the_kernels_bounds(rows, cuda):
+    """As within them: 65 heads run in torch."""
+    copies, heads = {0: 2, 1: 1}, 65
+    made = inputs(copies, heads, 4, 1, rows)
+    for i, size in enumerate((1e30, 3e37, 1e20)):
+        made["q"][i] = (made["q"][i].double().clamp(-3, 3) * size).to(rows)
+    got = run(made, copies, heads, 1e-6, cuda)
+    for name, want in wanted(made, copies, heads, 1e-6, torch.finfo(torch.float32).eps).items():
+        compare(got[name], want, name)
+
+
 def test_module_is_its_function_and_survives_casts_and_copies():
     head = SO2FieldType({0: 4, 1: 2})
     frequencies = rotary_frequencies(head, (8.0, 5.0), (0.3, 1.0), (False, True))
