@@ -38,7 +38,7 @@ from torch import Tensor, nn
 
 from gm_attention_amd import _native
 from gm_attention_amd.nn import fused_attention
-from gm_attention_amd.representations.field_type import SO2FieldType
+from gm_attention_amd.representations.field_type import SO2FeatureField, SO2FieldType
 
 MAX_HEADS, MAX_F, MAX_D, MAX_AXES = 64, fused_attention.MAX_F, fused_attention.MAX_D, 8
 
@@ -279,6 +279,27 @@ class SO2QueryKeyNorm(nn.Module):
             raise ValueError("positions must be given exactly where there are frequencies.")
         return query_key_norm(q, k, self.head_type, self.heads, self.query_gain, self.key_gain, eps=self.eps,
                               positions=positions, frequencies=self._on(q.device))
+
+    def forward(self, q: SO2FeatureField, k: SO2FeatureField,
+                positions: Tensor | None = None) -> tuple[SO2FeatureField, SO2FeatureField]:
+        """The same of fields of the heads side by side (``head_type.scaled(heads)``), with positions a node."""
+        full = self.head_type.scaled(self.heads)
+        for given in (q, k):
+            if given.field_type != full:
+                raise ValueError(f"Expected a field of type {full!r}, got {given.field_type!r}.")
+        rows, keys = q._rows(), k._rows()
+        batch = rows.shape[:-1]
+        if keys.shape != rows.shape:
+            raise ValueError(f"q and k must be fields on the same nodes, got {tuple(batch)} "
+                             f"and {tuple(keys.shape[:-1])}.")
+        if positions is not None:
+            if positions.shape[:-1] != batch:
+                raise ValueError(f"positions must be ({', '.join(map(str, batch))}, axes), "
+                                 f"got {tuple(positions.shape)}.")
+            positions = positions.reshape(-1, positions.shape[-1])
+        out = self.forward_flat(rows.reshape(-1, rows.shape[-1]), keys.reshape(-1, rows.shape[-1]), positions)
+        turned_q, turned_k = (SO2FeatureField.from_flat(full, t.reshape(*batch, -1)) for t in out)
+        return turned_q, turned_k
 
     def extra_repr(self) -> str:
         axes = 0 if self.frequencies is None else len(self.frequencies)

@@ -24,7 +24,7 @@ import torch
 import problems
 from gm_attention_amd.nn import head_norm
 from gm_attention_amd.nn.head_norm import SO2QueryKeyNorm, query_key_norm, rotary_frequencies
-from gm_attention_amd.representations.field_type import SO2FieldType
+from gm_attention_amd.representations.field_type import SO2FeatureField, SO2FieldType
 from test_differential_gpu import ROWS, compare, tables_dtype
 
 
@@ -478,6 +478,40 @@ def test_module_is_its_function_and_survives_casts_and_copies():
         assert all(torch.equal(a, b) for a, b in zip(other.forward_flat(q, k, at), want))
     assert set(module.state_dict()) == {"query_gain", "key_gain"} and "query_gain" in dir(module)
     assert not list(SO2QueryKeyNorm(head, 2, gain=False).parameters())
+
+
+@pytest.mark.gpu
+def test_the_module_takes_fields_on_the_gpu(cuda):
+    fields_of(cuda)
+
+
+def test_the_module_takes_fields():
+    fields_of("cpu")
+
+
+def fields_of(device):
+    """Called, it gives what its flat form does, in the fields' shape, and its hooks run."""
+    head, heads = SO2FieldType({0: 4, 1: 2}), 3
+    full = head.scaled(heads)
+    frequencies = rotary_frequencies(head, (8.0, 5.0), (0.3, 1.0), (False, True))
+    at = problems.normal((2, 7, 2), 2).double().to(device)
+    q, k = (problems.normal((2, 7, full.dimension), i).float().to(device) for i in range(2))
+    for module, given in ((SO2QueryKeyNorm(head, heads, frequencies=frequencies, device=device), (at,)),
+                          (SO2QueryKeyNorm(head, heads, device=device), ())):
+        called = []
+        module.register_forward_hook(lambda *_: called.append(1))
+        got = module(*(SO2FeatureField.from_flat(full, x) for x in (q, k)), *given)
+        want = module.forward_flat(q.flatten(0, 1), k.flatten(0, 1), *(p.flatten(0, 1) for p in given))
+        assert called == [1]
+        for a, b in zip(got, want):
+            assert a.field_type == full and torch.equal(a.to_flat(), b.reshape(2, 7, -1))
+    field = SO2FeatureField.from_flat(full, q)
+    for call, message in (((SO2FeatureField.from_flat(SO2FieldType({0: 24}), q), field), "Expected a field of type"),
+                          ((field, SO2FeatureField.from_flat(full, k[:1])), "on the same nodes"),
+                          ((field, field, at), "exactly where there are frequencies"),
+                          ((field, field, at[0]), r"positions must be \(2, 7, axes\)")):
+        with pytest.raises(ValueError, match=message):
+            module(*call)
 
 
 def test_frequencies_are_dealt_to_the_axes():
