@@ -228,7 +228,8 @@ class SO2QueryKeyNorm(nn.Module):
     axis, e.g. from :func:`rotary_frequencies`) turn the rows by their nodes' positions.
 
     The frequencies are part of the construction, kept in 64 bits whatever the module is
-    cast to; they are not in its state."""
+    cast to; they are not in its state.  A device's copy is made by the first call there,
+    which a captured step needs to have been made before the capture."""
 
     def __init__(self, head_type: SO2FieldType, heads: int, *, eps: float = 1e-6, norm: bool = True,
                  gain: bool = True, frequencies: Tensor | Sequence[Sequence[float]] | None = None, dtype=None,
@@ -266,6 +267,9 @@ class SO2QueryKeyNorm(nn.Module):
         key = f"_frequencies {device}"
         held = self.__dict__.get(key)
         if held is None:
+            if device.type == "cuda" and torch.cuda.is_current_stream_capturing():
+                raise RuntimeError("the first call of an SO2QueryKeyNorm on a device waits for the device: make it before "
+                                   "the capture.")
             held = self.__dict__[key] = torch.tensor(self.frequencies, dtype=torch.float64, device=device)
             _native.complete(held.device)  # other streams and threads find it unchecked
         return held

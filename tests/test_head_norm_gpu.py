@@ -438,6 +438,29 @@ def test_on_another_stream_and_the_modules_tables(cuda):
     assert all(torch.equal(a, b) for a, b in zip(got, want))
 
 
+@pytest.mark.gpu
+def test_a_modules_first_call_is_before_a_capture(cuda):
+    head = SO2FieldType({0: 4, 1: 4, 2: 4})
+    made = inputs({0: 4, 1: 4, 2: 4}, 4, 50, 2, torch.float32)
+    q, k, at = (made[n].to(cuda) for n in ("q", "k", "positions"))
+    module, other = (SO2QueryKeyNorm(head, 4, frequencies=made["frequencies"], device=cuda).requires_grad_(False)
+                     for _ in range(2))
+    want = [t.clone() for t in module.forward_flat(q, k, at)]
+    torch.cuda.synchronize()
+    captured = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(captured):
+        with pytest.raises(RuntimeError, match="before the capture"):
+            other.forward_flat(q, k, at)
+        got = module.forward_flat(q, k, at)
+    for _ in range(2):
+        for t in got:
+            t.zero_()
+        captured.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(got, want))
+    assert all(torch.equal(a, b) for a, b in zip(other.forward_flat(q, k, at), want))
+
+
 # ---------------------------------------------------------------- without a GPU
 
 
