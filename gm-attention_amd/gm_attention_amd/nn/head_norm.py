@@ -268,10 +268,12 @@ class SO2QueryKeyNorm(nn.Module):
         held = self.__dict__.get(key)
         if held is None:
             if device.type == "cuda" and torch.cuda.is_current_stream_capturing():
-                raise RuntimeError("the first call of an SO2QueryKeyNorm on a device waits for the device: make it before "
-                                   "the capture.")
-            held = self.__dict__[key] = torch.tensor(self.frequencies, dtype=torch.float64, device=device)
+                raise RuntimeError("the first call of an SO2QueryKeyNorm on a device waits for the device: make it "
+                                   "before the capture.")
+            with torch.inference_mode(False):  # a later step may train
+                held = torch.tensor(self.frequencies, dtype=torch.float64, device=device)
             _native.complete(held.device)  # other streams and threads find it unchecked
+            self.__dict__[key] = held
         return held
 
     def __getstate__(self) -> dict:

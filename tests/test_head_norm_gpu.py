@@ -461,7 +461,33 @@ def test_a_modules_first_call_is_before_a_capture(cuda):
     assert all(torch.equal(a, b) for a, b in zip(other.forward_flat(q, k, at), want))
 
 
+@pytest.mark.gpu
+def test_a_module_called_in_inference_mode_trains_on_the_gpu(cuda):
+    inference_first(cuda)
+
+
 # ---------------------------------------------------------------- without a GPU
+
+
+def test_a_module_called_in_inference_mode_trains():
+    inference_first("cpu")
+
+
+def inference_first(device):
+    """What its first call keeps serves a later step's backward."""
+    copies, heads = {0: 4, 1: 4, 2: 4}, 4
+    made = inputs(copies, heads, 9, 2, torch.float32)
+    at, up = made["positions"].to(device), [u.to(device) for u in made["up"]]
+    modules = [SO2QueryKeyNorm(SO2FieldType(copies), heads, frequencies=made["frequencies"], device=device)
+               for _ in range(2)]
+    with torch.inference_mode():
+        modules[0].forward_flat(made["q"].to(device), made["k"].to(device), at)
+    assert not modules[0]._on(at.device).is_inference()
+    grads = []
+    for module in modules:
+        leaves = [made[n].to(device).requires_grad_(True) for n in ("q", "k")] + list(module.parameters())
+        grads.append(torch.autograd.grad(module.forward_flat(*leaves[:2], at), leaves, up))
+    assert all(torch.equal(a, b) for a, b in zip(*grads))
 
 
 @pytest.mark.parametrize("rows", ROWS)
