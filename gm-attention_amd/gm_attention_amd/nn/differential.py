@@ -91,7 +91,9 @@ class EdgeTables:
     def _hold(self, source: Tensor, phases: Tensor, masked: Tensor) -> None:
         """The checked tables in the form their device reads."""
         if self.device.type != "cuda":
-            self._source, self._phases, self._bias = source, phases, masked
+            with torch.inference_mode(False):  # a later step may train: autograd saves no inference tensor
+                self._source, self._phases, self._bias = (t.clone() if t.is_inference() else t
+                                                          for t in (source, phases, masked))
             return
         records = torch.empty(self.n_edges, 2 * self.orders, dtype=self.dtype, device=self.device)
         words = records.view(_WORD[self.dtype])

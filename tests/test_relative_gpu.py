@@ -700,6 +700,19 @@ def test_copied_tables_on_the_cpu_give_the_same_results():
         assert all(torch.equal(got[n], want[n]) for n in want)
 
 
+def test_tables_made_in_inference_mode_train():
+    copies, heads = {0: 2, 1: 2}, 2
+    graph = bucketed(scattered([3, 0, 70, 9, 1], 40, torch.float64), 6)
+    values = inputs(graph, copies, heads, torch.float64)
+    want = run(tables_of(graph, torch.float64, "cpu"), *values, copies, heads, torch.float64, "cpu")
+    with torch.inference_mode():
+        for name in ("row_ptr", "source", "transport", "bias", "inside", "buckets"):
+            setattr(graph, name, getattr(graph, name).clone())
+        tables = tables_of(graph, torch.float64, "cpu")
+    got = run(tables, *values, copies, heads, torch.float64, "cpu")
+    assert all(torch.equal(got[n], want[n]) for n in want)
+
+
 def test_rings_of_distance():
     """Equal distances share a ring whatever their last bit, the borders' too; every distance has one."""
     step = math.pi / 31
