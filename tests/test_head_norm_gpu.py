@@ -184,6 +184,36 @@ def test_numbers_of_rows(copies, heads, n, rows, cuda):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("n", [1, 4097, 12_289, 60_001, 200_001])
+@pytest.mark.parametrize("rows", ROWS)
+@pytest.mark.parametrize("eps", [None, 3.0])
+@pytest.mark.parametrize("copies,heads", [({0: 4, 1: 4, 2: 4}, 8), ({0: 11, 1: 5, 2: 3}, 3), ({0: 12}, 8)])
+def test_gains_gradients_over_every_row(copies, heads, eps, rows, n, cuda):
+    """Sums over more rows than the workgroups hold at once, of numbers whose sums are exact: rows of 1 and -1 (under
+    the norm, mean 1 and eps 3, of halves), gradients of whole numbers up to 2.  All the terms together, 2 n
+    heads of up to 2, stay below 2^24 of their units (6.4 million), so every row counts once, to the last bit, in any
+    order."""
+    head = SO2FieldType(copies)
+    gen = torch.Generator(device=cuda).manual_seed(n)
+    D = heads * head.dimension
+    q, k = (2.0 * torch.randint(0, 2, (n, D), generator=gen, device=cuda) - 1 for _ in range(2))
+    up = [torch.randint(-2, 3, (n, D), generator=gen, device=cuda).double() for _ in range(2)]
+    gains = [torch.ones(sum(copies.values()), dtype=tables_dtype(rows), device=cuda, requires_grad=True)
+             for _ in range(2)]
+    outs = query_key_norm(q.to(rows), k.to(rows), head, heads, *gains, eps=eps)
+    grads = torch.autograd.grad(outs, gains, [u.to(rows) for u in up])
+    for x, u, got in zip((q, k), up, grads):
+        terms, want, at = (x * u).sum(0), [], 0  # whole numbers in double
+        for f, c in copies.items():
+            w = c * (1 if f == 0 else 2)
+            want.append(terms[at:at + heads * w].reshape(heads, c, -1).sum((0, 2)))
+            at += heads * w
+        want = torch.cat(want) * (1.0 if eps is None else 0.5)
+        assert torch.equal(got.double(), want)
+        assert n == 1 or bool((want != 0).any())
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("eps,gains,axes", [(1e-6, True, 0), (1e-6, False, 2), (1e-6, False, 0), (None, True, 2),
                                             (None, False, 1), (None, True, 0), (0.5, True, 8)])
 @pytest.mark.parametrize("copies", [{0: 4, 1: 4, 2: 4}, {0: 3, 1: 5}])

@@ -228,6 +228,37 @@ def test_many_targets_for_each_workgroup(cuda):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("rows", ROWS)
+@pytest.mark.parametrize("copies,heads,n_buckets", [({0: 1, 1: 1, 2: 1}, 4, 11), ({0: 4, 1: 4, 2: 4}, 8, 32),
+                                                    ({0: 3, 1: 1}, 5, 3), ({0: 2, 1: 2, 2: 2}, 16, 256)])
+def test_the_tables_gradient_over_every_edge(copies, heads, n_buckets, rows, cuda):
+    """Sums over more rows than the workgroups hold at once, of numbers whose sums are exact.  Queries of zeros and
+    equal biases make a row of 2^d edges uniform, 2^-d; under whole g up to 2 its ds are whole in 2^-2d, 2^-12 at most
+    here, and sum to at most 4.  A workgroup has at most 160 rows here, one workgroup a CU: its sums stay below 2^12,
+    24 bits above 2^-12; those of the workgroups are in double.  So every edge counts once, to the last bit."""
+    gen = torch.Generator().manual_seed(n_buckets)
+    degrees = (2 ** torch.randint(0, 5, (40_000,), generator=gen)).tolist()
+    degrees[::7] = [0] * len(degrees[::7])
+    degrees[3::997] = [64] * len(degrees[3::997])
+    graph = bucketed(scattered(degrees, 3000, torch.float32, outside=0.0, order=max(copies)), n_buckets)
+    graph.inside[:] = 1
+    graph.bias[:] = 0.0
+    E, D = graph.source.numel(), heads * SO2FieldType(copies).dimension
+    dtype = tables_dtype(rows)
+    g = torch.randint(-2, 3, (E, heads), generator=gen).double()
+    leaves = [torch.zeros(graph.n_targets, D), torch.ones(graph.n_sources, D), torch.zeros(n_buckets, heads)]
+    leaves = [x.to(t).to(cuda).requires_grad_(True) for x, t in zip(leaves, (rows, rows, dtype))]
+    alpha = relative_softmax(*leaves, tables_of(graph, dtype, cuda), SO2FieldType(copies), heads)
+    degree = (graph.row_ptr[1:] - graph.row_ptr[:-1]).double()[graph.target].unsqueeze(1)
+    assert torch.equal(alpha.detach().cpu().double(), (1 / degree).expand(E, heads))
+    (got,) = torch.autograd.grad(alpha, leaves[2:], g.to(dtype).to(cuda))
+    total = torch.zeros(graph.n_targets, heads, dtype=torch.float64).index_add_(0, graph.target, g / degree)
+    ds = (g - total[graph.target]) / degree
+    want = torch.zeros(n_buckets, heads, dtype=torch.float64).index_add_(0, graph.buckets, ds)
+    assert torch.equal(got.cpu(), want.to(dtype)) and float((want != 0).double().mean()) > 0.9
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("copies", [{0: 1, 1: 1, 2: 1}, {0: 4, 1: 4, 2: 4}])
 def test_long_rows_among_many_targets(copies, cuda):
     """Rows that a wave takes alone though its scores fill more than it holds, beside some of a workgroup."""
