@@ -416,9 +416,8 @@ inline int rel_shape(const RelLayout& L, int& per_map, int (&base)[3]) {
   return -1;
 }
 
-constexpr size_t kRelLds = 160 * 1024;
-
-// LDS of a pass: the records a wave (and the forward's scores, and the learned table), the waves' sums, the bins.
+// LDS of a pass: the records a wave (and the forward's scores, the waves' maxima and the learned table), the waves'
+// sums: at most 39 KB forward (256 buckets of 16 heads) and 24 KB backward, of the 64 KB that any launch may ask for.
 template <typename U>
 size_t rel_forward_lds(int table) {
   return sizeof(float) * ((size_t)kWavesPerBlock * kWave * (U::RW + kRelKept + 1) + table);
@@ -426,13 +425,6 @@ size_t rel_forward_lds(int table) {
 template <typename U>
 size_t rel_rows_lds(int lanes) {
   return sizeof(float) * kWavesPerBlock * (size_t)std::max(kWave * U::PW, 2 * U::N * lanes);
-}
-
-inline int rel_lds_limit(const void* kernel, size_t lds) {
-  if (lds > 64 * 1024 &&
-      hipFuncSetAttribute(kernel, hipFuncAttributeMaxDynamicSharedMemorySize, (int)kRelLds) != hipSuccess)
-    return check_launch("relative (LDS)");
-  return GM_OK;
 }
 
 template <typename R, typename U, bool kNear, bool kSplit>
@@ -446,8 +438,6 @@ int rel_launch(RelPass pass, const RelArgs<float, R>& a, EdgeUnits w, const RelR
                       : pass == RelPass::BackwardTarget ? &relative_rows_units<R, U, kNear, true, kSplit>
                                                         : &relative_rows_units<R, U, kNear, false, kSplit>;
   const size_t lds = pass == RelPass::Forward ? rel_forward_lds<U>(a.buckets * a.L.H) : rel_rows_lds<U>(w.lanes);
-  const int rc = rel_lds_limit(reinterpret_cast<const void*>(kernel), lds);
-  if (rc != GM_OK) return rc;
   hipLaunchKernelGGL(kernel, dim3((unsigned)blocks), dim3(kRelThreads), lds, stream, a, w);
   return check_launch("relative");
 }
