@@ -9,7 +9,7 @@
 //   dx    = (t - xhat mean(t xhat)) / sqrt(mean x^2 + eps)
 //
 // A pass reads its rows once and writes once, and the bytes bound it: 524,288 rows of 160 of queries and keys each take
-// 257 us forward and 411 backward in float (5.2 and 4.9 TB/s), 126 and 225 in bfloat16 (5.3 and 4.5: its registers
+// 258 us forward and 420 backward in float (5.2 and 4.8 TB/s), 126 and 230 in bfloat16 (5.3 and 4.4: its registers
 // leave two waves a SIMD).  Angles are made in the pass, in double up to the whole turns (a far position's angle has no
 // bits left in float), once for all heads and both sets; sums of a head are in double from what a lane (a unit) adds in
 // float, so that no row overflows.
@@ -679,7 +679,7 @@ int hn_launch_lanes(const HnArgs<float, R>& a, const HnLanes& w, float* dgain, h
 }
 
 // The units of the lane kernels: pieces of 16 bytes at the frequencies above 0 where the copies allow, at frequency 0
-// whole pairs of scalars (a last odd one only where a head is one unit).
+// whole pairs of scalars.
 constexpr HnShape kHnFloat[] = {{2, 2, 2}, {4, 2, 2}, {4, 2, 0}, {2, 2, 0}, {4, 2, 1}, {4, 0, 0}, {0, 2, 2}, {2, 1, 1}};
 constexpr HnShape kHnHalf[] = {{4, 4, 4}, {8, 4, 4}, {4, 4, 0}, {8, 4, 2}, {8, 0, 0}, {0, 4, 4}, {2, 2, 2}, {2, 1, 1}};
 

@@ -151,7 +151,7 @@ __global__ __launch_bounds__(256) void relative_rows_simple(RelArgs<T, R> a) {
 // head) read alpha and g, which lie edge by edge, as whole lines; a wave holds kRelHeld steps of both, so that a row
 // of up to that many (times the waves it is shared by) is read once.  The workgroups are persistent, find their next
 // row while the present one's numbers are on their way, and each writes a row of bins.  Bound by bytes and by how many
-// are on their way: 63 million edges of eight heads take 1.47 ms, 5.3 GB from and to memory (3.6 TB/s).
+// are on their way: 63 million edges of eight heads take 1.50 ms, 6.1 GB read and written (4.1 TB/s).
 // Holding 16 steps takes as long, 8 takes 5 % more: long rows are read twice.
 //
 // A bin is a slot's own, added to in the order of its steps, while the bins take up to kRelBins bytes a wave; of more

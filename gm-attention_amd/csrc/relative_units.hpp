@@ -4,14 +4,14 @@
 //
 // Forward, a wave a target (a long row four): a step gathers S rows of k and sums a
 // score over its units' lanes; scores wait in LDS (a long row's in alpha) for their
-// maximum and sum.  63.0 M edges of 160 numbers take 2.61 ms: rows reach a CU out of L1
+// maximum and sum.  63.0 M edges of 160 numbers take 2.67 ms: rows reach a CU out of L1
 // at 27 bytes a cycle (contiguous loads at 50) while vector instructions fill half of the
 // time, and neither gives way alone (at 2.83 ms: all rows among 16 nodes 6% less, without
 // the dots 2%, without the weights' writes 8%).
 //
 // Backward, dq and dk: a wave a pair of neighbouring rows over the nodes of both, whose
-// rows are loaded once for two edges (four loads for seven edges on a grid).  1.77 and
-// 1.84 ms for the edges above; a row at a time 2.50 and 2.64.  Scores do not gain from
+// rows are loaded once for two edges (four loads for seven edges on a grid).  1.76 and
+// 1.82 ms for the edges above; a row at a time 2.50 and 2.64.  Scores do not gain from
 // pairs (3.68 ms): twice the registers of q, entries of 56 bytes, and alpha's places edge
 // by edge cost more than the rows' loads they spare.
 #pragma once
@@ -26,7 +26,7 @@ namespace rel {
 
 constexpr int kRelKept = 16;  // rows of scores that LDS holds a wave: 16 steps, or 32 where two lanes share a head's
 // Steps whose rows are requested together: two, and the registers that this leaves go to more waves, five or six a SIMD
-// (with four steps and four waves the scores of 33 M edges take 1.55 ms and the rows of 63 M 2.15, so 1.42 and 1.86).
+// (four steps and four waves took 9 % more for the scores of 33 M edges, 16 % for the rows of 63 M).
 constexpr int kRelInFlight = 2;
 constexpr int kRelThreads = kWavesPerBlock * kWave;
 // What stands among a row's exponentials for a score of -inf, outside the window for one: no exponential has these

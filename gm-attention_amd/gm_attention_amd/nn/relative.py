@@ -9,9 +9,9 @@ its owner sorts edges by), and head h learns one number a bucket,
 so that a layer's weights can depend on where a neighbour sits beside what it
 holds.  The table's gradient is the sum, over a bucket's edges, of the scores'.
 
-Edges outside the window count for nothing, whatever their rows hold, nor do edges
-of weight zero in a gradient; a target with no edge inside has only zero weights
-(and zero gradients).
+Edges outside the window count for nothing, whatever their rows hold and whatever the
+row's other scores are, nor do edges of weight zero in a gradient; a target with no
+edge inside has only zero weights (and zero gradients).
 
 The op reads an edge set through :class:`RelativeEdgeTables`, which its owner builds
 once and keeps.  On the GPU (``gm_relative_*``) neither the scores nor the learned
@@ -37,8 +37,9 @@ from gm_attention_amd.representations.field_type import SO2FieldType
 
 MAX_H, MAX_F, MAX_D = fused_attention.MAX_H, fused_attention.MAX_F, fused_attention.MAX_D
 MAX_BUCKETS = 256
-# up to here the scores' rows of more than 8 steps, not 32, take four waves: 2,048 targets 14.2 -> 9.1 us, 12,285
-# 46 -> 34; beyond it not (32,768: 131 -> 174)
+# up to here the scores' rows of more than 8 steps, not 32, take four waves.  5,120 waves run at once (five a SIMD);
+# while the targets are about three times as many the launch ends with its longest rows, which four waves shorten
+# (2,048 targets 14.2 -> 9.1 us, 12,285 46 -> 34), beyond it the waves' sharing costs more (32,768: 131 -> 174)
 FEW_TARGETS = 16384
 MAX_SOURCES = 2**24  # of float32 tables: a record's word holds the source and the bucket
 
