@@ -465,11 +465,17 @@ def torch_weights(q: Tensor, k: Tensor, row_ptr: Tensor, source: Tensor, phases:
     weight = weight / total.masked_fill(total == 0, 1.0).index_select(0, target)
     none = out | (weight == 0)
 
-    # a factor of zero is not enough where the other one is infinite or no number
-    def over_rows(g: Tensor) -> Tensor:
+    # a factor of zero is not enough where the other one is infinite or no number (no gradient: undefined, or a second
+    # derivative's that does not depend on it)
+    def over_scores(g: Tensor | None) -> Tensor | None:
+        return None if g is None else g.masked_fill(none, 0.0)
+
+    def over_rows(g: Tensor | None) -> Tensor | None:
+        if g is None:
+            return None
         return g.masked_fill(torch.cat([none.repeat_interleave(a * dim, 1) for _, a, _, _, dim in plan.rows], 1), 0.0)
 
-    for t, kept in ((score, lambda g: g.masked_fill(none, 0.0)), (qe, over_rows), (ke, over_rows)):
+    for t, kept in ((score, over_scores), (qe, over_rows), (ke, over_rows)):
         if t.requires_grad:
             t.register_hook(kept)
     return weight.masked_fill(none, 0.0), none

@@ -721,6 +721,29 @@ def test_edges_of_weight_zero_on_the_cpu():
     torch.testing.assert_close(dtable, torch.tensor([[ds], [-ds], *zeros]))
 
 
+def test_derivatives_of_every_kind_on_the_cpu():
+    """Backward, forward and second derivatives, and functions of functions."""
+    copies, heads = {0: 2, 1: 1}, 2
+    graph = bucketed(scattered([1, 3, 4, 6], 5, torch.float64, outside=0.3), 3)
+    *leaves, _ = inputs(graph, copies, heads, torch.float64)
+    tables = tables_of(graph, torch.float64, "cpu")
+
+    def weights(q, k, extra):
+        return relative_softmax(q, k, extra, tables, SO2FieldType(copies), heads)
+
+    given = [x.requires_grad_(True) for x in leaves]
+    assert torch.autograd.gradcheck(weights, given, check_forward_ad=True)
+    assert torch.autograd.gradgradcheck(weights, given)
+    q, k, extra = (x.detach() for x in leaves)
+
+    def loss(q):
+        return weights(q, k, extra).square().sum()
+
+    (want,) = torch.autograd.grad(loss(given[0]), given[:1])
+    torch.testing.assert_close(torch.func.grad(loss)(q), want)
+    torch.testing.assert_close(torch.func.vmap(torch.func.grad(loss))(torch.stack([q, 2 * q]))[0], want)
+
+
 def test_copied_tables_on_the_cpu_give_the_same_results():
     graph = bucketed(scattered([3, 0, 70, 9, 1], 40, torch.float64), 256)
     values = inputs(graph, {0: 2, 1: 2}, 2, torch.float64)
